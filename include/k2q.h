@@ -223,7 +223,9 @@ int k2q_linear_fwd(const uint16_t* x, int64_t ldx, int64_t M, int64_t K, int8_t*
                    const void* qw, const void* sw, const float* bias, int64_t N, uint16_t* y, void* ws,
                    int64_t ws_bytes, void* stream);
 
-/* W4A8 variant: per-group int32 partials scaled by the bf16 group scales and added in f32 over the whole K. */
+/* W4A8 variant: per-group int32 partials scaled by the bf16 group scales and added in f32 over the whole K.
+ * M <= 8 runs a GEMV (no workspace, no tiles): half-group partials scaled and added in f32 in an order that depends
+ * on K alone, so a row's result is the same whatever rows are beside it. */
 int k2q_gemm_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const uint16_t* sw4,
                   const float* bias, const float* u, const float* lora_b, int64_t r, float lora_scale,
                   int64_t M, int64_t N, int64_t K, uint16_t* y, void* stream);
@@ -245,7 +247,8 @@ int k2q_gemm_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const u
  * k2q_gemm_w8a8_grouped with N the segments' total out_features.  Host only: no device call. */
 int k2q_gemm_w8a8_plan(int64_t M, int64_t N, int64_t K, int cus, int grouped, int* split_pieces);
 /* The same for W4: returns the rows per tile (32, 64 or 128) and the K-pieces that every tile is cut into (1 = none).
- * workspace != 0: the W4 GEMM of k2q_linear_fwd with its workspace; 0: k2q_gemm_w4a8, which has none. */
+ * workspace != 0: the W4 GEMM of k2q_linear_fwd with its workspace; 0: k2q_gemm_w4a8, which has none.  M <= 8: what the
+ * tiles would take (k2q_gemm_w4a8_f32 runs them); the forwards run the GEMV. */
 int k2q_gemm_w4a8_plan(int64_t M, int64_t N, int64_t K, int cus, int workspace, int* split_pieces);
 
 /* Debug entries: raw int32 accumulators acc[m,n] = sum_k qx[m,k] qw[n,k] (W8), and for W4 the f32

@@ -2169,7 +2169,7 @@ extern "C" int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, i
 }
 
 int64_t gemm_w4a8_ws_bytes(int64_t M, int64_t N, int64_t K) {
-  if (check_common(M, N, K)) return 0;
+  if (check_common(M, N, K) || M <= K2Q_GEMV_MAX_M) return 0;
   return w4_piece_bytes(M, N, w4_plan(M, N, K, k2q_cu_count(), true));
 }
 
@@ -2197,6 +2197,8 @@ int gemm_w4a8_impl(const int8_t* qx, const float* sx, const uint8_t* qw4, const 
     return K2Q_EINVAL;
   if (bias && !k2q_aligned(bias, 16)) return K2Q_EINVAL;
   if ((rc = check_lora(u, lora_b, r))) return rc;
+  if (M <= K2Q_GEMV_MAX_M)
+    return k2q_launch_gemv_w4a8(qx, sx, qw4, sw4, bias, u, lora_b, (int)r, lora_scale, M, N, K, y, st);
   W4Args p{};
   p.a = qw4; p.s4 = sw4; p.b = qx; p.N = N; p.M = M; p.K = K;
   p.out = y; p.sx = sx; p.bias = bias;

@@ -10,6 +10,14 @@
 // L = sum_j bf16(B[n,j]) bf16(s u[m,j]) in f32 is added to f; the result is rounded to bf16 once.  Without
 // LoRA both paths give identical bits; with LoRA only L's summation order differs (the MFMA's internal
 // order vs sequential here).
+//
+// The W4A8 form (k2q_launch_gemv_w4a8) streams packed int4 rows the same way: N x K / 2 bytes of codes and N x K / 32 of
+// bf16 group scales, once.  A 16-byte load holds 32 weights, half of a 64-wide scale group, so a lane's exact int32 dot
+// with the activation codes is scaled by its own group's scale and added in f32:
+//   y[m][n] = bf16((s_x[m] 2^-7) sum_g s4[g][n] (sum_{k in g} q_x q_w) + bias + LoRA).
+// In a packed chunk of 8 bytes byte j holds code j in its low and code j + 8 in its high nibble: a 32-bit word shifted
+// left by 4 and masked, or masked alone, is four weights of consecutive k times 16, dotted as they are with four
+// consecutive activation codes; the factor 16 leaves in the epilogue (a power of two: exact).
 #include "k2q_common.h"
 
 namespace {
@@ -31,6 +39,20 @@ struct GemvArgs {
   int64_t M, N, K;
   uint16_t* y;           // M x N bf16
 };
+
+// The LoRA term of one output: sum_j bf16(B[n, j]) bf16(scale u[m, j]) in f32, j ascending (r % 4 == 0).
+__device__ __forceinline__ float lora_dot(const float* ub, const float* bb, int r, float scale) {
+  float l = 0.f;
+  for (int j = 0; j < r; j += 4) {
+    const v4f uv = *reinterpret_cast<const v4f*>(ub + j);
+    const v4f bv = *reinterpret_cast<const v4f*>(bb + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      l = __builtin_fmaf(bf16_bits_to_f32(f32_to_bf16_bits(bv[e])),
+                         bf16_bits_to_f32(f32_to_bf16_bits(uv[e] * scale)), l);
+  }
+  return l;
+}
 
 template <int MT>
 __global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8_kernel(GemvArgs p) {
@@ -96,21 +118,94 @@ __global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8_kernel(GemvArgs p) {
   const float sxm = p.sx[m] * 0.0078125f;   // 2^-7: the two unnormalised rotations
   const float bi = p.bias ? p.bias[n] : 0.f;
   float f = __builtin_fmaf((float)a, sxm * p.sw[n], bi);
-  if (p.u) {
-    const float* ub = p.u + (int64_t)m * p.r;
-    const float* bb = p.lora_b + n * p.r;
-    float l = 0.f;
-    for (int j = 0; j < p.r; j += 4) {
-      const v4f uv = *reinterpret_cast<const v4f*>(ub + j);
-      const v4f bv = *reinterpret_cast<const v4f*>(bb + j);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        l = __builtin_fmaf(bf16_bits_to_f32(f32_to_bf16_bits(bv[e])),
-                           bf16_bits_to_f32(f32_to_bf16_bits(uv[e] * p.lora_scale)), l);
-    }
-    f += l;
-  }
+  if (p.u) f += lora_dot(p.u + (int64_t)m * p.r, p.lora_b + n * p.r, p.r, p.lora_scale);
   p.y[(int64_t)m * p.N + n] = (uint16_t)f32_to_bf16_bits(f);
+}
+
+struct Gemv4Args {
+  const int8_t* qx;      // M x K
+  const float* sx;       // M
+  const uint8_t* qw;     // N x K / 2 packed
+  const uint16_t* s4;    // K / 64 x N bf16
+  const float* bias;     // N or null
+  const float* u;        // M x r or null
+  const float* lora_b;   // N x r
+  int r;
+  float lora_scale;
+  int64_t N;
+  int K;
+  uint16_t* y;           // M x N bf16
+};
+
+// 32 weights of one row against 32 activation codes (x[0..7]: four codes a word, k ascending); 16 times the dot.
+__device__ __forceinline__ int dot32_i4(const v4u& w, const v4i& x0, const v4i& x1) {
+  int d = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {      // a 16-wide chunk: words 2 j (k 0-3, 8-11) and 2 j + 1 (k 4-7, 12-15)
+    const v4i& x = j ? x1 : x0;
+    d = __builtin_amdgcn_sdot4((int)((w[2 * j] << 4) & 0xf0f0f0f0u), x[0], d, false);
+    d = __builtin_amdgcn_sdot4((int)((w[2 * j + 1] << 4) & 0xf0f0f0f0u), x[1], d, false);
+    d = __builtin_amdgcn_sdot4((int)(w[2 * j] & 0xf0f0f0f0u), x[2], d, false);
+    d = __builtin_amdgcn_sdot4((int)(w[2 * j + 1] & 0xf0f0f0f0u), x[3], d, false);
+  }
+  return d;
+}
+
+template <int MT>
+__global__ __launch_bounds__(64 * GV_WAVES) void gemv_w4_kernel(Gemv4Args p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n0 = ((int64_t)blockIdx.x * GV_WAVES + (threadIdx.x >> 6)) * GV_ROWS;
+  if (n0 >= p.N) return;   // N % 4 == 0: a wave's four rows are all there; no barriers
+  const int kb = p.K / 2;  // bytes per row
+  const uint8_t* w0 = p.qw + n0 * kb;
+  float acc[GV_ROWS][MT] = {};
+
+  for (int b0 = 16 * lane; b0 < kb; b0 += 1024) {
+    v4u w[GV_ROWS];
+#pragma unroll
+    for (int i = 0; i < GV_ROWS; ++i)
+      w[i] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(w0 + (int64_t)i * kb + b0));
+    const int k = 2 * b0;
+    const v2u sv = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)(k >> 6) * p.N + n0);
+    const float sc[GV_ROWS] = {__uint_as_float(sv[0] << 16), __uint_as_float(sv[0] & 0xffff0000u),
+                               __uint_as_float(sv[1] << 16), __uint_as_float(sv[1] & 0xffff0000u)};
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const v4i x0 = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k);
+      const v4i x1 = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k + 16);
+#pragma unroll
+      for (int i = 0; i < GV_ROWS; ++i) acc[i][m] = __builtin_fmaf((float)dot32_i4(w[i], x0, x1), sc[i], acc[i][m]);
+    }
+  }
+
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < GV_ROWS; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[i][m] += __shfl_xor(acc[i][m], off, 64);
+
+  // Lane i + GV_ROWS m writes y[m][n0 + i].
+  if (lane >= GV_ROWS * MT) return;
+  const int i = lane % GV_ROWS, m = lane / GV_ROWS;
+  const int64_t n = n0 + i;
+  float a = 0.f;
+#pragma unroll
+  for (int ii = 0; ii < GV_ROWS; ++ii)
+#pragma unroll
+    for (int mm = 0; mm < MT; ++mm) a = (ii == i && mm == m) ? acc[ii][mm] : a;
+  float f = __builtin_fmaf(a, p.sx[m] * (0.0078125f * 0.0625f), p.bias ? p.bias[n] : 0.f);
+  if (p.u) f += lora_dot(p.u + (int64_t)m * p.r, p.lora_b + n * p.r, p.r, p.lora_scale);
+  p.y[(int64_t)m * p.N + n] = (uint16_t)f32_to_bf16_bits(f);
+}
+
+template <int MT>
+int launch4_mt(const Gemv4Args& p, hipStream_t st) {
+  const int64_t rows_per_wg = (int64_t)GV_ROWS * GV_WAVES;
+  const int64_t grid = (p.N + rows_per_wg - 1) / rows_per_wg;
+  if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  hipLaunchKernelGGL(gemv_w4_kernel<MT>, dim3((unsigned)grid), dim3(64 * GV_WAVES), 0, st, p);
+  return k2q_launch_status();
 }
 
 template <int MT>
@@ -138,6 +233,25 @@ int k2q_launch_gemv_w8a8(const int8_t* qx, const float* sx, const int8_t* qw, co
     case 6: return launch_mt<6>(p, st);
     case 7: return launch_mt<7>(p, st);
     case 8: return launch_mt<8>(p, st);
+    default: return K2Q_EINVAL;
+  }
+}
+
+// Called by k2q_gemm_w4a8 after its argument checks (N % 4 == 0, K % 128 == 0), for 1 <= M <= K2Q_GEMV_MAX_M.
+int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const uint16_t* sw4, const float* bias,
+                         const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
+                         int64_t K, uint16_t* y, hipStream_t st) {
+  if (K > 0x3fffffff) return K2Q_EUNSUPPORTED;
+  Gemv4Args p{qx, sx, qw4, sw4, bias, u, lora_b, u ? r : 0, lora_scale, N, (int)K, y};
+  switch (M) {
+    case 1: return launch4_mt<1>(p, st);
+    case 2: return launch4_mt<2>(p, st);
+    case 3: return launch4_mt<3>(p, st);
+    case 4: return launch4_mt<4>(p, st);
+    case 5: return launch4_mt<5>(p, st);
+    case 6: return launch4_mt<6>(p, st);
+    case 7: return launch4_mt<7>(p, st);
+    case 8: return launch4_mt<8>(p, st);
     default: return K2Q_EINVAL;
   }
 }

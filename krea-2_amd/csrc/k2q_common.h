@@ -56,9 +56,12 @@ __device__ __forceinline__ void static_for(F&& f) {
   }
 }
 
-// Skinny-M forward (gemv.hip), used by k2q_gemm_w8a8 for 1 <= M <= K2Q_GEMV_MAX_M.
+// Skinny-M forwards (gemv.hip), used by k2q_gemm_w8a8 and k2q_gemm_w4a8 for 1 <= M <= K2Q_GEMV_MAX_M.
 #define K2Q_GEMV_MAX_M 8
 int k2q_launch_gemv_w8a8(const int8_t* qx, const float* sx, const int8_t* qw, const float* sw, const float* bias,
+                         const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
+                         int64_t K, uint16_t* y, hipStream_t st);
+int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const uint16_t* sw4, const float* bias,
                          const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
                          int64_t K, uint16_t* y, hipStream_t st);
 
