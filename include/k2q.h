@@ -42,6 +42,7 @@ extern "C" {
 
 #define K2Q_DTYPE_BF16 0
 #define K2Q_DTYPE_F32 1
+#define K2Q_DTYPE_F16 2      /* k2q_rotary alone */
 
 /* Library version string and device check (K2Q_OK when the current device is gfx950). */
 const char* k2q_version(void);
@@ -92,6 +93,59 @@ int k2q_swiglu_bwd(const uint16_t* dh, const uint16_t* gate, const uint16_t* up,
                    uint16_t* dup, void* stream);
 int k2q_rmsmod_bwd(const uint16_t* dh, const uint16_t* x, int64_t M, int64_t K, const float* norm_scale, float eps,
                    const uint16_t* mod_scale, int64_t ld_mod, int64_t rows_per_batch, uint16_t* dx, void* stream);
+
+/* RMSNorm with the residual's addition, and the codes of its output, in one pass (SingleStreamBlock.forward,
+ * mmdit.py:317-318: `x = x + pregate * self.attn(..)` followed by the modulated norm of x):
+ *   r = bf16(x + t), t = bf16(gate * y) (y without a gate);  n = bf16((r * rsqrt(mean_k r^2 + eps)) * (norm_scale +
+ *   scale_add));  h = bf16(bf16(bf16(1 + p) * n) + b) (n without a modulation);  q, s = k2q_rotquant(h).
+ * x, y: M rows of strides ldx / ldy; r, h, q row stride K.  gate, p = mod_scale and b = mod_shift (both or neither) are
+ * nullable bf16 vectors, row m reading entry m / rows_per_batch of row stride ld_gate / ld_scale / ld_shift (0: one
+ * entry).  scale_add: 1 for a norm whose weight is scale + 1 (mmdit.py:156-161), 0 for a plain weight.  K as for
+ * k2q_rotquant.
+ * k2q_resnorm_bwd is its autograd.  dh, dr (nullable): the gradients of h and of r's other readers; dn = bf16(dh * bf16(1 +
+ * p)), g = dn (norm_scale + scale_add), i = rsqrt(mean_k r^2 + eps):
+ *   dx = bf16(dr + bf16(g i - r (i^3 / K) sum_k g r)),  dy = bf16(gate * dx) (given exactly when gate is; else dy is dx).
+ * The sums over the rows of a batch entry are written where their pointer is given (dscale, dshift, dgate: entries x K
+ * bf16, dnorm: K f32, over all rows); they need y (dgate), M a multiple of rows_per_batch, and ws of
+ * k2q_resnorm_bwd_ws_bytes bytes, 16-byte aligned:
+ *   dscale = sum dh n,  dshift = sum dh,  dgate = sum dx y,  dnorm = sum dh bf16(1 + p) r i,
+ * in f32 in a fixed order.  All M x K operands but y contiguous. */
+int k2q_resnorm_rotquant(const uint16_t* x, int64_t ldx, const uint16_t* y, int64_t ldy, const uint16_t* gate,
+                         int64_t ld_gate, int64_t M, int64_t K, const float* norm_scale, float scale_add, float eps,
+                         const uint16_t* mod_scale, int64_t ld_scale, const uint16_t* mod_shift, int64_t ld_shift,
+                         int64_t rows_per_batch, uint16_t* r, uint16_t* h, int8_t* q, float* s, void* stream);
+int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch);
+int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
+                    const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale, int64_t ld_scale,
+                    const uint16_t* gate, int64_t ld_gate, int64_t rows_per_batch, uint16_t* dx, uint16_t* dy,
+                    const uint16_t* y, int64_t ldy, float* dnorm, uint16_t* dscale, uint16_t* dshift, uint16_t* dgate,
+                    void* ws, int64_t ws_bytes, void* stream);
+
+/* Rotary positions of queries and keys (mmdit.py:13-30, between the projections and the attention): every pair (a, b) of
+ * the first rotary_dim values of a head turns by its token's angle, the rest of the head is copied:
+ *   (a, b) -> factor (a cos t - b sin t, a sin t + b cos t),  t = 2 pi pos[axis[i]] turns[i],  i < rotary_dim / 2.
+ * layout INTERLEAVED: pair i is (2 i, 2 i + 1); HALF: (i, i + rotary_dim / 2).  inverse != 0: t -> -t, the transpose (the
+ * backward pass).  t: one or two tensors (q; q and k) of B x L tokens with their own heads, rows of D values, strides in
+ * elements, x and o apart.  positions: one value per token (axis NULL) or axis, strides pos_b / pos_l / pos_a elements.
+ * turns: rotary_dim / 2 revolutions per position; angles are taken in f64, the rotation in f32, rounded once.
+ * dtype bf16, f32 or f16 for every tensor; any alignment and sizes (16-byte rows and vectors run faster); D <= 4096,
+ * rotary_dim <= 1024, B L heads < 2^31. */
+#define K2Q_ROTARY_INTERLEAVED 0
+#define K2Q_ROTARY_HALF 1
+#define K2Q_POS_I64 0
+#define K2Q_POS_I32 1
+#define K2Q_POS_F32 2
+#define K2Q_POS_F64 3
+typedef struct {
+  const void* x;
+  void* o;
+  int64_t heads;
+  int64_t x_b, x_l, x_h;    /* strides of x: batch, token, head */
+  int64_t o_b, o_l, o_h;
+} k2q_rotary_heads;
+int k2q_rotary(const k2q_rotary_heads* t, int64_t n, int dtype, int64_t B, int64_t L, int64_t D, int64_t rotary_dim,
+               int layout, const void* positions, int pos_type, int64_t pos_b, int64_t pos_l, int64_t pos_a,
+               const double* turns, const int32_t* axis, float factor, int inverse, void* stream);
 
 /* LoRA down-projection u = x.f32 @ A^T (lora.py:47, first product).  When the rows alone do not fill the
  * GPU, K is cut into slices whose partials meet in ws (k2q_lora_down_ws_bytes(M, K, r) bytes; 0 means none

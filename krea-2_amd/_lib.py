@@ -44,6 +44,12 @@ class DxSegment(ctypes.Structure):
     _fields_ = [("dy", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("wt", ctypes.c_void_p), ("N", ctypes.c_int64)]
 
 
+class RotaryHeads(ctypes.Structure):
+    """``k2q_rotary_heads`` of ``include/k2q.h``: one tensor of heads, its result, and their strides in elements."""
+    _fields_ = [("x", ctypes.c_void_p), ("o", ctypes.c_void_p), ("heads", ctypes.c_int64)] + [
+        (name, ctypes.c_int64) for name in ("x_b", "x_l", "x_h", "o_b", "o_l", "o_h")]
+
+
 class LoraMember(ctypes.Structure):
     """``k2q_lora_member`` of ``include/k2q.h``: one linear of a grouped LoRA-gradient call."""
     _fields_ = [("dy", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("N", ctypes.c_int64), ("lora_b", ctypes.c_void_p),
@@ -70,6 +76,13 @@ _SIGNATURES = {
     "k2q_rmsmod_rotquant": ([_p, _i64, _i64, _i64, _p, _f32, _p, _p, _i64, _i64, _p, _p, _p, _p], _int),
     "k2q_swiglu_bwd": ([_p, _p, _p, _i64, _p, _p, _p], _int),
     "k2q_rmsmod_bwd": ([_p, _p, _i64, _i64, _p, _f32, _p, _i64, _i64, _p, _p], _int),
+    "k2q_resnorm_rotquant": ([_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _p,
+                              _p, _p, _p, _p], _int),
+    "k2q_resnorm_bwd_ws_bytes": ([_i64, _i64, _i64], _i64),
+    "k2q_resnorm_bwd": ([_p, _p, _p, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p,
+                         _p, _p, _p, _i64, _p], _int),
+    "k2q_rotary": ([_p, _i64, _int, _i64, _i64, _i64, _i64, _int, _p, _int, _i64, _i64, _i64, _p, _p, _f32, _int, _p],
+                   _int),
     "k2q_lora_down_ws_bytes": ([_i64, _i64, _i64], _i64),
     "k2q_lora_down": ([_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p], _int),
     "k2q_pad_factors": ([_p, _p, _i64, _i64, _i64, _i64, _p, _p, _p], _int),
@@ -416,6 +429,130 @@ def rmsmod_bwd(dh: torch.Tensor, x: torch.Tensor, norm_scale: torch.Tensor, eps:
     _check(load().k2q_rmsmod_bwd(_ptr(dh), _ptr(x), M, K, _ptr(norm_scale), float(eps), _ptr(mod_scale), ldm,
                                  rows_per_batch if B > 1 else M, _ptr(dx), _stream(dev)), "k2q_rmsmod_bwd")
     return dx
+
+
+def _check_entries(t, name: str, K: int, entries: int, dev) -> None:
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != K:
+        raise ValueError(f"{name} must be an (entries, {K}) bf16 tensor")
+    if t.shape[0] not in (1, entries):
+        raise ValueError(f"{name} has {t.shape[0]} entries, expected 1 or {entries}")
+    if t.stride(1) != 1 or t.data_ptr() % 16 or t.device != dev or (t.shape[0] > 1 and t.stride(0) % 8):
+        raise ValueError(f"{name} needs contiguous 16-byte aligned rows on {dev}")
+
+
+def _check_norm_rows(t, name: str, w, rows_per_entry: int) -> None:
+    M, K = t.shape
+    _check_k(K)
+    if M < 1:
+        raise ValueError("no rows")
+    if rows_per_entry < 1 or M % rows_per_entry:
+        raise ValueError(f"{M} rows do not split into entries of {rows_per_entry}")
+    _need(w, "the norm's weight", torch.float32, 1, t.device)
+    if w.shape[0] != K:
+        raise ValueError(f"the norm's weight has {w.shape[0]} entries, {name} has {K} features")
+
+
+def _check_resnorm(x, y, gate, w, ms, mb, rows_per_entry) -> None:
+    _need_rows(x, "x")
+    _need_rows(y, "y", x.device)
+    if x.shape != y.shape:
+        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} differ in shape")
+    _check_norm_rows(x, "x", w, rows_per_entry)
+    for t, name in ((gate, "gate"), (ms, "scale"), (mb, "shift")):
+        _check_entries(t, name, x.shape[1], x.shape[0] // rows_per_entry, x.device)
+    if (ms is None) != (mb is None):
+        raise ValueError("scale and shift come together")
+    _device_check(x.device)
+
+
+def resnorm_rotquant(x, y, gate, w, add: float, eps: float, scale, shift, rows_per_entry: int):
+    """The residual's addition, the RMSNorm of the sum and its codes in one pass (``k2q_resnorm_rotquant``):
+    ``r = bf16(x + bf16(gate * y))``, ``h`` its norm with weight ``w + add``, modulated by ``scale`` / ``shift``.  ``x``,
+    ``y`` (M,K) bf16 rows; ``gate``, ``scale``, ``shift`` (1 or M / rows_per_entry, K) bf16 or None; ``w`` (K,) f32.
+    Returns ``(r, h, q, s)`` with ``(q, s)`` the codes and scales of ``rotquant(h)``."""
+    args = (x, y, gate, w, add, eps, scale, shift, rows_per_entry)
+    r = _fast().resnorm(*args)
+    if r.__class__ is tuple:
+        return r
+    return _refused(r, "k2q_resnorm_rotquant", lambda: _native.resnorm(*args),
+                    lambda: _check_resnorm(x, y, gate, w, scale, shift, rows_per_entry))
+
+
+def _check_resnorm_bwd(dh, dr, r, w, ms, gate, rows_per_entry, y, need_mod) -> None:
+    _need(r, "r", torch.bfloat16, 2)
+    _check_norm_rows(r, "r", w, rows_per_entry)
+    for t, name in ((dh, "dh"), (dr, "dr")):
+        if t is not None or name == "dh":
+            _need(t, name, torch.bfloat16, 2, r.device)
+            if t.shape != r.shape:
+                raise ValueError(f"{name} and r differ in shape")
+    for t, name in ((gate, "gate"), (ms, "scale")):
+        _check_entries(t, name, r.shape[1], r.shape[0] // rows_per_entry, r.device)
+    if y is not None:
+        _need_rows(y, "y", r.device)
+        if y.shape != r.shape or gate is None:
+            raise ValueError("the gate's gradient needs the gate and y of r's shape")
+    if need_mod and ms is None:
+        raise ValueError("no modulation to differentiate")
+    _device_check(r.device)
+
+
+def resnorm_bwd(dh, dr, r, w, add: float, eps: float, scale, gate, rows_per_entry: int, y=None, need_w=False,
+                need_scale=False, need_shift=False):
+    """Autograd of :func:`resnorm_rotquant` (``k2q_resnorm_bwd``): ``(dx, dy, dw, dscale, dshift, dgate)`` from the
+    gradients of ``h`` and (or None) of ``r``.  ``dy`` is None without a gate (it is ``dx``); ``dgate`` comes when ``y``
+    is given, the other sums where asked for, one row per entry."""
+    args = (dh, dr, r, w, add, eps, scale, gate, rows_per_entry, y, need_w, need_scale, need_shift)
+    out = _fast().resnorm_bwd(*args)
+    if out.__class__ is tuple:
+        return out
+    return _refused(out, "k2q_resnorm_bwd", lambda: _native.resnorm_bwd(*args),
+                    lambda: _check_resnorm_bwd(dh, dr, r, w, scale, gate, rows_per_entry, y, need_scale or need_shift))
+
+
+MAX_HEAD, MAX_ROTARY = 4096, 1024       # k2q_rotary's largest head and rotated part
+ROTARY_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+POSITION_DTYPES = (torch.int64, torch.int32, torch.float32, torch.float64)
+
+
+def _check_rotary(q, k, positions, turns, axis, axes: int, heads_first: bool) -> None:
+    dev = q.device
+    token = 2 if heads_first else 1
+    for t, name in ((q, "q"), (k, "k")):
+        if t is None:
+            continue
+        if t.dim() != 4 or t.dtype not in ROTARY_DTYPES or t.dtype != q.dtype or t.device != dev:
+            raise ValueError(f"{name} must be a 4-D tensor of one of {ROTARY_DTYPES}, as q on {dev}, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        if (t.shape[0], t.shape[token], t.shape[3]) != (q.shape[0], q.shape[token], q.shape[3]):
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or head size")
+        if t.stride(3) != 1 or t.numel() == 0:
+            raise ValueError(f"{name} needs contiguous heads and at least one value")
+    if 2 * turns.numel() > q.shape[3]:
+        raise ValueError(f"{2 * turns.numel()} rotated values in heads of {q.shape[3]}")
+    if positions.dtype not in POSITION_DTYPES or positions.device != dev:
+        raise ValueError(f"positions must be one of {POSITION_DTYPES} on {dev}, got {positions.dtype} on "
+                         f"{positions.device}")
+    lead = tuple(positions.shape[:-1] if axis is not None else positions.shape)
+    if axis is not None and positions.shape[-1:] != (axes,):
+        raise ValueError(f"positions {tuple(positions.shape)} need a last dimension of {axes} axes")
+    if len(lead) not in (1, 2) or lead[-1] != q.shape[token] or (len(lead) == 2 and lead[0] not in (1, q.shape[0])):
+        raise ValueError(f"positions {tuple(positions.shape)} do not give {q.shape[0]} x {q.shape[token]} tokens theirs")
+    _device_check(dev)
+
+
+def rotary(q, k, positions, turns, axis, axes: int, half: bool, factor: float, inverse: bool, heads_first: bool):
+    """Rotary positions (``k2q_rotary``): ``(q', k')`` with the strides of ``q`` and ``k`` (k may be None).  ``q``, ``k``
+    (B,L,H,D), or (B,H,L,D) heads first; ``positions`` (L,) or (B,L), with ``axis`` a dimension of ``axes`` more behind;
+    ``turns`` f64 revolutions per position of every pair, ``axis`` int32 their axis (below ``axes``) or None."""
+    args = (q, k, positions, turns, axis, axes, half, factor, inverse, heads_first)
+    r = _fast().rotary(*args)
+    if r.__class__ is tuple:
+        return r
+    return _refused(r, "k2q_rotary", lambda: _native.rotary(*args),
+                    lambda: _check_rotary(q, k, positions, turns, axis, axes, heads_first))
 
 
 def swiglu_bwd(dh: torch.Tensor, g: torch.Tensor, u: torch.Tensor):

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 
 #include "../../include/k2q.h"
 
@@ -33,6 +34,10 @@ struct Api {
   decltype(&k2q_dequant_fp8) dequant_fp8;
   decltype(&k2q_gemm_bf16) gemm_bf16;
   decltype(&k2q_gemm_plan_ws_bytes) gemm_plan_ws_bytes;
+  decltype(&k2q_resnorm_rotquant) resnorm_rotquant;
+  decltype(&k2q_resnorm_bwd) resnorm_bwd;
+  decltype(&k2q_resnorm_bwd_ws_bytes) resnorm_bwd_ws_bytes;
+  decltype(&k2q_rotary) rotary;
 } api{};
 
 PyObject* raw_stream_of = nullptr;   // torch._C._cuda_getCurrentRawStream
@@ -402,6 +407,146 @@ PyObject* py_gemm_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Rows (M, K) bf16, contiguous and 16-byte aligned within a row.
+bool rows_ok(const Tensor* t, int64_t M, int64_t K, c10::Device d) {
+  return t && t->scalar_type() == at::kBFloat16 && t->dim() == 2 && t->size(0) == M && t->size(1) == K && t->device() == d &&
+         t->stride(1) == 1 && t->stride(0) >= K && t->stride(0) % 8 == 0 && aligned(*t);
+}
+
+// Per-entry bf16 vectors (1, K) or (entries, K), or null; ld is their row stride (0: one entry).
+bool entries_ok(const Tensor* t, int64_t entries, int64_t K, c10::Device d, int64_t& ld) {
+  ld = 0;
+  if (!t) return true;
+  if (t->scalar_type() != at::kBFloat16 || t->dim() != 2 || t->size(1) != K || t->device() != d || t->stride(1) != 1 ||
+      !aligned(*t) || (t->size(0) != 1 && t->size(0) != entries))
+    return false;
+  if (t->size(0) > 1) ld = t->stride(0);
+  return ld >= 0 && ld % 8 == 0;
+}
+
+// resnorm(x, y, gate | None, w, add, eps, scale | None, shift | None, rows_per_entry) -> (r, h, q, s)
+PyObject* py_resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(9)
+  return guarded([&]() -> PyObject* {
+    const Tensor *x = tensor_of(a[0], bad), *y = tensor_of(a[1], bad), *gate = tensor_of(a[2], bad),
+                 *w = tensor_of(a[3], bad), *ms = tensor_of(a[6], bad), *mb = tensor_of(a[7], bad);
+    const double add = PyFloat_AsDouble(a[4]), eps = PyFloat_AsDouble(a[5]);
+    const int64_t rpb = PyLong_AsLongLong(a[8]);
+    if (PyErr_Occurred()) return nullptr;
+    if (bad || !x || !y || x->dim() != 2) K2Q_REFUSE;
+    const int64_t M = x->size(0), K = x->size(1);
+    const c10::Device d = x->device();
+    int64_t lg, ls, lb;
+    if (!ready(d) || M < 1 || rpb < 1 || M % rpb || !width_ok(K) || !rows_ok(x, M, K, d) || !rows_ok(y, M, K, d) ||
+        !operand(w, at::kFloat, 1, d) || w->size(0) != K || !entries_ok(gate, M / rpb, K, d, lg) ||
+        !entries_ok(ms, M / rpb, K, d, ls) || !entries_ok(mb, M / rpb, K, d, lb) || !ms != !mb)
+      K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    Tensor r = alloc({M, K}, at::kBFloat16, d), h = alloc({M, K}, at::kBFloat16, d), q = alloc({M, K}, at::kChar, d),
+           s = alloc({M}, at::kFloat, d);
+    const int rc = foreign(api.resnorm_rotquant, as<uint16_t>(ptr(x)), x->stride(0), as<uint16_t>(ptr(y)), y->stride(0),
+                           as<uint16_t>(ptr(gate)), lg, M, K, as<float>(ptr(w)), (float)add, (float)eps,
+                           as<uint16_t>(ptr(ms)), ls, as<uint16_t>(ptr(mb)), lb, rpb, as<uint16_t>(ptr(r)),
+                           as<uint16_t>(ptr(h)), as<int8_t>(ptr(q)), as<float>(ptr(s)), st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({r, h, q, s});
+  });
+}
+
+// resnorm_bwd(dh, dr | None, r, w, add, eps, scale | None, gate | None, rows_per_entry, y | None, need_w, need_scale,
+//             need_shift) -> (dx, dy | None, dw | None, dscale | None, dshift | None, dgate | None)
+PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(13)
+  return guarded([&]() -> PyObject* {
+    const Tensor *dh = tensor_of(a[0], bad), *dr = tensor_of(a[1], bad), *r = tensor_of(a[2], bad),
+                 *w = tensor_of(a[3], bad), *ms = tensor_of(a[6], bad), *gate = tensor_of(a[7], bad),
+                 *y = tensor_of(a[9], bad);
+    const double add = PyFloat_AsDouble(a[4]), eps = PyFloat_AsDouble(a[5]);
+    const int64_t rpb = PyLong_AsLongLong(a[8]);
+    const int need_w = PyObject_IsTrue(a[10]), need_scale = PyObject_IsTrue(a[11]), need_shift = PyObject_IsTrue(a[12]);
+    if (PyErr_Occurred()) return nullptr;
+    if (bad || !dh || !r || r->dim() != 2) K2Q_REFUSE;
+    const int64_t M = r->size(0), K = r->size(1);
+    const c10::Device d = r->device();
+    auto whole = [&](const Tensor* t) { return operand(t, at::kBFloat16, 2, d) && t->size(0) == M && t->size(1) == K; };
+    int64_t lg, ls;
+    if (!ready(d) || M < 1 || rpb < 1 || M % rpb || !width_ok(K) || !whole(dh) || !whole(r) || (dr && !whole(dr)) ||
+        !operand(w, at::kFloat, 1, d) || w->size(0) != K || !entries_ok(gate, M / rpb, K, d, lg) ||
+        !entries_ok(ms, M / rpb, K, d, ls) || (y && (!gate || !rows_ok(y, M, K, d))) ||
+        ((need_scale || need_shift) && !ms))
+      K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    const int64_t E = M / rpb;
+    Tensor dx = alloc({M, K}, at::kBFloat16, d), dy = gate ? alloc({M, K}, at::kBFloat16, d) : Tensor();
+    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = need_scale ? alloc({E, K}, at::kBFloat16, d) : Tensor(),
+           db = need_shift ? alloc({E, K}, at::kBFloat16, d) : Tensor(), dg = y ? alloc({E, K}, at::kBFloat16, d) : Tensor();
+    const int64_t nws = need_w || need_scale || need_shift || y ? api.resnorm_bwd_ws_bytes(M, K, rpb) : 0;
+    Tensor ws = workspace(nws, d);
+    const int rc = foreign(api.resnorm_bwd, as<uint16_t>(ptr(dh)), as<uint16_t>(ptr(dr)), as<uint16_t>(ptr(r)), M, K,
+                           as<float>(ptr(w)), (float)add, (float)eps, as<uint16_t>(ptr(ms)), ls, as<uint16_t>(ptr(gate)),
+                           lg, rpb, as<uint16_t>(ptr(dx)), as<uint16_t>(ptr(dy)), as<uint16_t>(ptr(y)),
+                           y ? y->stride(0) : 0, as<float>(ptr(dw)), as<uint16_t>(ptr(ds)), as<uint16_t>(ptr(db)),
+                           as<uint16_t>(ptr(dg)), ptr(ws), nws, st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({dx, dy, dw, ds, db, dg});
+  });
+}
+
+// rotary(q, k | None, positions, turns, axis | None, axes, half, factor, inverse, heads_first) -> (q', k' | None): q, k (B,
+// L, H, D) or, heads first, (B, H, L, D); positions (L,) or (B, L), with an axis one dimension of `axes` more behind
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(10)
+  return guarded([&]() -> PyObject* {
+    const Tensor *q = tensor_of(a[0], bad), *k = tensor_of(a[1], bad), *p = tensor_of(a[2], bad),
+                 *turns = tensor_of(a[3], bad), *axis = tensor_of(a[4], bad);
+    const int64_t axes = PyLong_AsLongLong(a[5]);
+    const int half = PyObject_IsTrue(a[6]), inverse = PyObject_IsTrue(a[8]), first = PyObject_IsTrue(a[9]);
+    const double factor = PyFloat_AsDouble(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    if (bad || !q || !p || !turns || q->dim() != 4) K2Q_REFUSE;
+    const int ld = first ? 2 : 1, hd = 3 - ld;
+    const int64_t B = q->size(0), L = q->size(ld), D = q->size(3), nf = turns->numel();
+    const c10::Device d = q->device();
+    const auto ty = q->scalar_type();
+    const int dt = ty == at::kBFloat16 ? K2Q_DTYPE_BF16 : ty == at::kHalf ? K2Q_DTYPE_F16 : K2Q_DTYPE_F32;
+    const auto pt = p->scalar_type();
+    const int pos_type = pt == at::kLong ? K2Q_POS_I64 : pt == at::kInt ? K2Q_POS_I32 : pt == at::kFloat ? K2Q_POS_F32 : K2Q_POS_F64;
+    if (!ready(d) || (dt == K2Q_DTYPE_F32 && ty != at::kFloat) || (pos_type == K2Q_POS_F64 && pt != at::kDouble) ||
+        turns->scalar_type() != at::kDouble || !turns->is_contiguous() || turns->device() != d || 2 * nf > D ||
+        p->device() != d ||
+        (axis && (axis->scalar_type() != at::kInt || !axis->is_contiguous() || axis->numel() != nf || axis->device() != d)))
+      K2Q_REFUSE;
+    const int lead = (int)p->dim() - (axis ? 1 : 0);      // positions' batch and token dimensions
+    if (lead < 1 || lead > 2 || p->size(lead - 1) != L || (axis && p->size(lead) != axes) || (lead == 2 && p->size(0) != 1 && p->size(0) != B)) K2Q_REFUSE;
+    k2q_rotary_heads t[2] = {};
+    Tensor out[2];
+    const c10::DeviceGuard guard(d);
+    for (int i = 0; i < (k ? 2 : 1); ++i) {
+      const Tensor& x = i ? *k : *q;
+      if (x.dim() != 4 || x.size(0) != B || x.size(ld) != L || x.size(3) != D || x.scalar_type() != ty || x.device() != d ||
+          x.stride(3) != 1 || x.numel() == 0)
+        K2Q_REFUSE;
+      out[i] = at::empty_like(x);
+      if (out[i].stride(3) != 1) out[i] = at::empty(x.sizes(), x.options());
+      t[i] = {x.data_ptr(), out[i].data_ptr(), x.size(hd), x.stride(0), x.stride(ld), x.stride(hd), out[i].stride(0),
+              out[i].stride(ld), out[i].stride(hd)};
+    }
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    const int rc = foreign(api.rotary, static_cast<const k2q_rotary_heads*>(t), (int64_t)(k ? 2 : 1), dt, B, L, D, 2 * nf,
+                           half ? K2Q_ROTARY_HALF : K2Q_ROTARY_INTERLEAVED, p->data_ptr(), pos_type,
+                           lead == 2 && p->size(0) > 1 ? p->stride(0) : 0, p->stride(lead - 1),
+                           axis ? p->stride(lead) : 0, as<double>(ptr(turns)), as<int32_t>(ptr(axis)), (float)factor,
+                           inverse, st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({out[0], out[1]});
+  });
+}
+
 // bind(dict of entry point addresses, raw stream getter)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(2)
@@ -421,7 +566,9 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !get("k2q_lora_down_ws_bytes", api.lora_down_ws_bytes) || !get("k2q_pad_factors", api.pad_factors) ||
       !get("k2q_dx_prep_eff", api.dx_prep_eff) || !get("k2q_gemm_dx_lin", api.gemm_dx_lin) ||
       !get("k2q_dequant_fp8", api.dequant_fp8) || !get("k2q_gemm_bf16", api.gemm_bf16) ||
-      !get("k2q_gemm_plan_ws_bytes", api.gemm_plan_ws_bytes))
+      !get("k2q_gemm_plan_ws_bytes", api.gemm_plan_ws_bytes) || !get("k2q_resnorm_rotquant", api.resnorm_rotquant) ||
+      !get("k2q_resnorm_bwd", api.resnorm_bwd) || !get("k2q_resnorm_bwd_ws_bytes", api.resnorm_bwd_ws_bytes) ||
+      !get("k2q_rotary", api.rotary))
     return nullptr;
   Py_INCREF(a[1]);
   Py_XSETREF(raw_stream_of, a[1]);
@@ -442,7 +589,8 @@ PyObject* py_device_checked(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2Q_METHOD(alloc_codes),
                          K2Q_METHOD(linear_fwd),  K2Q_METHOD(lora_grads),     K2Q_METHOD(lora_down),
                          K2Q_METHOD(dx_weight),   K2Q_METHOD(gemm_dx),        K2Q_METHOD(dequant_fp8),
-                         K2Q_METHOD(gemm_bf16),   K2Q_METHOD(pad_factors),    {nullptr, nullptr, 0, nullptr}};
+                         K2Q_METHOD(gemm_bf16),   K2Q_METHOD(pad_factors),    K2Q_METHOD(resnorm),
+                         K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

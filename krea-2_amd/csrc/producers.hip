@@ -8,7 +8,11 @@
 //       n = bf16((x * rsqrt(mean(x^2) + eps)) * (w + 1))   [float32, the whole row]
 //       h = bf16(bf16(bf16(1 + p) * n) + b)               [p, b: the bf16 modulation scale / shift of the
 //                                                          row's batch entry]
-// Both write h (bf16, the tensor the next linear receives: its LoRA down-projection and the saved input of
+//   * RMSNorm with the residual's addition (mmdit.py:317-318: `x = x + pregate * attn`, then the norm of x):
+//       t = bf16(gate * y)  (t = y without a gate),  r = bf16(x + t),
+//     and the norm above of r, modulated or not.  r is written too: it is the residual stream.  The roundings are those
+//     of the eager bf16 ops, so r, h and the codes equal those of the separate ops and of the norm on r bit for bit.
+// All write h (bf16, the tensor the next linear receives: its LoRA down-projection and the saved input of
 // the backward read it) and the int8 codes + scales of rotate/quant applied to h, computed from the same
 // registers, so the codes equal those of a separate rotate/quant call on h bit for bit.
 //
@@ -23,19 +27,22 @@ namespace {
 
 using namespace k2q_rot;
 
-enum { PROD_SWIGLU = 0, PROD_RMSMOD = 1 };
+enum { PROD_SWIGLU = 0, PROD_RMSMOD = 1, PROD_RESNORM = 2 };
 
 struct ProdArgs {
   const __bf16* x0;          // SwiGLU: gate output g;  RMSNorm: x
-  const __bf16* x1;          // SwiGLU: up output u
+  const __bf16* x1;          // SwiGLU: up output u;  residual norm: y
   int64_t ld0, ld1;          // row strides of x0 / x1 (elements)
-  const float* nw;           // RMSNorm scale parameter (K,), the norm weight is nw + 1
-  const uint16_t* mscale;    // bf16 modulation scale, entry b = row / rpb at mscale + b * ldm
-  const uint16_t* mshift;    // bf16 modulation shift, same indexing
-  int64_t ldm, rpb;
+  const float* nw;           // RMSNorm scale parameter (K,), the norm weight is nw + nwadd
+  float nwadd;
+  const uint16_t* mscale;    // bf16 modulation scale, entry b = row / rpb at mscale + b * ldm (residual norm: nullable)
+  const uint16_t* mshift;    // bf16 modulation shift, same indexing with ldb
+  const uint16_t* gate;      // residual norm: bf16 gate, same indexing with ldg, or null
+  int64_t ldm, ldb, ldg, rpb;
   float eps;
   int64_t M;
   int K;
+  uint16_t* r;               // residual norm: M x K bf16, the new residual stream
   uint16_t* h;               // M x K bf16 (row stride K)
   int8_t* q;                 // M x K int8 codes of h R
   float* s;                  // M per-row scales
@@ -109,6 +116,35 @@ __global__ __launch_bounds__(256) void prodquant_kernel(ProdArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   } else {
+    const int64_t b = rr / a.rpb;
+    if (PROD == PROD_RESNORM) {
+      const uint16_t* mg = a.gate ? a.gate + b * a.ldg : nullptr;
+#pragma unroll
+      for (int c = 0; c < kNCH; ++c) {
+        const int col = c * CW + off;
+        const bool ok = !kTail || col < K;
+        float y[16];
+        load16<__bf16>(a.x1 + rr * a.ld1 + (ok ? col : 0), true, y);
+        if (mg) {
+          float g[16];
+          load16<__bf16>(reinterpret_cast<const __bf16*>(mg) + (ok ? col : 0), true, g);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            y[i] *= g[i];
+            y[i + 1] *= g[i + 1];
+            bf16r2(y[i], y[i + 1]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float r0 = v[c][i] + y[i], r1 = v[c][i + 1] + y[i + 1];
+          bf16r2(r0, r1);
+          v[c][i] = ok ? r0 : 0.f;
+          v[c][i + 1] = ok ? r1 : 0.f;
+        }
+        if (row_ok && ok) store16_bf16(a.r + row * (int64_t)K + col, v[c]);
+      }
+    }
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < kNCH; ++c)
@@ -124,9 +160,9 @@ __global__ __launch_bounds__(256) void prodquant_kernel(ProdArgs a) {
       for (int w = 0; w < WPR; ++w) ss += sred[0][w0 + w];
     }
     const float rinv = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
-    const int64_t b = rr / a.rpb;
-    const uint16_t* ms = a.mscale + b * a.ldm;
-    const uint16_t* mb = a.mshift + b * a.ldm;
+    const bool mod = PROD == PROD_RMSMOD || a.mscale;
+    const uint16_t* ms = mod ? a.mscale + b * a.ldm : nullptr;
+    const uint16_t* mb = mod ? a.mshift + b * a.ldb : nullptr;
     // Per chunk: the norm weight (f32) and the two modulation vectors (bf16, kept packed) are loaded and
     // consumed before the next chunk's, so at most one chunk of them is live (occupancy).
 #pragma unroll
@@ -137,13 +173,23 @@ __global__ __launch_bounds__(256) void prodquant_kernel(ProdArgs a) {
       // unconditional loads from a clamped (always valid) address; lanes past K are zeroed below
       float w[16];
       load16<float>(a.nw + cc, true, w);
+      if (!mod) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float n0 = (v[c][i] * rinv) * (w[i] + a.nwadd), n1 = (v[c][i + 1] * rinv) * (w[i + 1] + a.nwadd);
+          bf16r2(n0, n1);
+          v[c][i] = !kTail || ok ? n0 : 0.f;
+          v[c][i + 1] = !kTail || ok ? n1 : 0.f;
+        }
+        continue;
+      }
       const uint4 pv0 = reinterpret_cast<const uint4*>(ms + cc)[0], pv1 = reinterpret_cast<const uint4*>(ms + cc)[1];
       const uint4 bv0 = reinterpret_cast<const uint4*>(mb + cc)[0], bv1 = reinterpret_cast<const uint4*>(mb + cc)[1];
       const uint32_t pw[8] = {pv0.x, pv0.y, pv0.z, pv0.w, pv1.x, pv1.y, pv1.z, pv1.w};
       const uint32_t bw[8] = {bv0.x, bv0.y, bv0.z, bv0.w, bv1.x, bv1.y, bv1.z, bv1.w};
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {   // element pairs share each bf16 conversion
-        float n0 = (v[c][i] * rinv) * (w[i] + 1.f), n1 = (v[c][i + 1] * rinv) * (w[i + 1] + 1.f);
+        float n0 = (v[c][i] * rinv) * (w[i] + a.nwadd), n1 = (v[c][i + 1] * rinv) * (w[i + 1] + a.nwadd);
         bf16r2(n0, n1);
         float p0 = 1.f + __uint_as_float(pw[i >> 1] << 16), p1 = 1.f + __uint_as_float(pw[i >> 1] & 0xffff0000u);
         bf16r2(p0, p1);
@@ -261,16 +307,34 @@ __global__ __launch_bounds__(256) void swiglu_bwd_kernel(const uint4* __restrict
   }
 }
 
+struct NormBwdArgs {
+  const uint16_t* dh;        // M x K bf16: gradient of h
+  const uint16_t* x;         // M x K: the norm's input (the residual norm's r)
+  int64_t M;
+  int K;
+  const float* nw;           // norm weight = nw + nwadd
+  float nwadd, eps;
+  const uint16_t* mscale;    // B x K bf16 modulation scale (residual norm: nullable)
+  int64_t ldm, rpb;
+  uint16_t* dx;
+  // the residual norm's
+  const uint16_t* dr;        // gradient of r from its other readers, or null
+  const uint16_t* gate;      // B x K bf16 or null
+  int64_t ldg;
+  uint16_t* dy;              // gradient of y, written where there is a gate (without one it is dx)
+  float* rinv;               // M row statistics for the column sums, or null
+};
+
 // Input gradient of the modulated RMSNorm (the autograd of the forward's eager ops for x alone):
 //   dn = bf16(dh * bf16(1 + p)),  g = dn * (w + 1),  r = rsqrt(mean x^2 + eps),
 //   dx = bf16(g r - x (r^3 / K) sum_k(g x)).
+// With a residual (kRes) x is the new stream, whose other readers' gradient joins it as autograd would add it, and the
+// gate scales it on the way to y:
+//   dR = bf16(dr + dx),  dy = bf16(gate * dR).
 // A team of 64 * WPR lanes owns a row; lane t handles the 8-element chunks at 8 t + 8 T c, c < kNCH, held
 // packed (bf16 pairs) between the two row reductions.
-template <int WPR, int kNCH>
-__global__ __launch_bounds__(256) void rmsmod_bwd_kernel(const uint16_t* __restrict__ dh, const uint16_t* __restrict__ x,
-                                                         int64_t M, int K, const float* __restrict__ nw, float eps,
-                                                         const uint16_t* __restrict__ mscale, int64_t ldm, int64_t rpb,
-                                                         uint16_t* __restrict__ dx) {
+template <bool kRes, int WPR, int kNCH>
+__global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
   constexpr int T = 64 * WPR;
   constexpr int ROWS = 4 / WPR;
   __shared__ float sred[2][4];
@@ -278,9 +342,11 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(const uint16_t* __restr
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR;
   const int t = (wave % WPR) * 64 + lane;
-  const bool row_ok = row < M;
+  const bool row_ok = row < a.M;
   const int64_t rr = row_ok ? row : 0;
-  const uint16_t* ms = mscale + (rr / rpb) * ldm;
+  const int K = a.K;
+  const bool mod = !kRes || a.mscale;
+  const uint16_t* ms = mod ? a.mscale + (rr / a.rpb) * a.ldm : nullptr;
 
   uint4 xv[kNCH], dv[kNCH];
   float ss = 0.f;
@@ -288,14 +354,14 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(const uint16_t* __restr
   for (int c = 0; c < kNCH; ++c) {
     const int col = 8 * t + 8 * T * c;
     const bool ok = col < K;
-    xv[c] = ok ? *reinterpret_cast<const uint4*>(x + rr * K + col) : make_uint4(0, 0, 0, 0);
-    dv[c] = ok ? *reinterpret_cast<const uint4*>(dh + rr * K + col) : make_uint4(0, 0, 0, 0);
+    xv[c] = ok ? *reinterpret_cast<const uint4*>(a.x + rr * K + col) : make_uint4(0, 0, 0, 0);
+    dv[c] = ok ? *reinterpret_cast<const uint4*>(a.dh + rr * K + col) : make_uint4(0, 0, 0, 0);
     const uint32_t w[4] = {xv[c].x, xv[c].y, xv[c].z, xv[c].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float a = __uint_as_float(w[j] << 16), b = __uint_as_float(w[j] & 0xffff0000u);
-      ss += a * a;
-      ss += b * b;
+      const float e0 = __uint_as_float(w[j] << 16), e1 = __uint_as_float(w[j] & 0xffff0000u);
+      ss += e0 * e0;
+      ss += e1 * e1;
     }
   }
   ss = wave_sum(ss);
@@ -307,7 +373,8 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(const uint16_t* __restr
 #pragma unroll
     for (int w = 0; w < WPR; ++w) ss += sred[0][w0 + w];
   }
-  const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + eps));
+  const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
+  if (kRes && a.rinv && t == 0 && row_ok) a.rinv[row] = r;
 
   // g = bf16(dh * p1) * (w + 1), kept in f32 (8 per chunk) for the final pass
   float gv[kNCH][8];
@@ -317,19 +384,19 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(const uint16_t* __restr
     const int col = 8 * t + 8 * T * c;
     const int cc = col < K ? col : 0;
     float w[8];
-    const float4 w0 = *reinterpret_cast<const float4*>(nw + cc), w1 = *reinterpret_cast<const float4*>(nw + cc + 4);
+    const float4 w0 = *reinterpret_cast<const float4*>(a.nw + cc), w1 = *reinterpret_cast<const float4*>(a.nw + cc + 4);
     w[0] = w0.x; w[1] = w0.y; w[2] = w0.z; w[3] = w0.w; w[4] = w1.x; w[5] = w1.y; w[6] = w1.z; w[7] = w1.w;
-    const uint4 pv = *reinterpret_cast<const uint4*>(ms + cc);
+    const uint4 pv = mod ? *reinterpret_cast<const uint4*>(ms + cc) : make_uint4(0, 0, 0, 0);
     const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
     const uint32_t dw[4] = {dv[c].x, dv[c].y, dv[c].z, dv[c].w};
     const uint32_t xw[4] = {xv[c].x, xv[c].y, xv[c].z, xv[c].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 4; ++j) {   // without a modulation p = 0: dh times one, exact
       float p0 = 1.f + __uint_as_float(pw[j] << 16), p1 = 1.f + __uint_as_float(pw[j] & 0xffff0000u);
       bf16r2(p0, p1);
       float n0 = __uint_as_float(dw[j] << 16) * p0, n1 = __uint_as_float(dw[j] & 0xffff0000u) * p1;
       bf16r2(n0, n1);
-      const float g0 = n0 * (w[2 * j] + 1.f), g1 = n1 * (w[2 * j + 1] + 1.f);
+      const float g0 = n0 * (w[2 * j] + a.nwadd), g1 = n1 * (w[2 * j + 1] + a.nwadd);
       gv[c][2 * j] = g0;
       gv[c][2 * j + 1] = g1;
       dot += g0 * __uint_as_float(xw[j] << 16);
@@ -347,37 +414,176 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(const uint16_t* __restr
   }
   if (!row_ok) return;
   const float c3 = __fdiv_rn(r * r * r * dot, (float)K);
+  const uint16_t* mg = kRes && a.gate ? a.gate + (row / a.rpb) * a.ldg : nullptr;
 #pragma unroll
   for (int c = 0; c < kNCH; ++c) {
     const int col = 8 * t + 8 * T * c;
     if (col >= K) continue;
     const uint32_t xw[4] = {xv[c].x, xv[c].y, xv[c].z, xv[c].w};
-    uint32_t o[4];
+    float d[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float d0 = gv[c][2 * j] * r - __uint_as_float(xw[j] << 16) * c3;
-      const float d1 = gv[c][2 * j + 1] * r - __uint_as_float(xw[j] & 0xffff0000u) * c3;
-      o[j] = pack_bf16x2(d0, d1);
+      d[2 * j] = gv[c][2 * j] * r - __uint_as_float(xw[j] << 16) * c3;
+      d[2 * j + 1] = gv[c][2 * j + 1] * r - __uint_as_float(xw[j] & 0xffff0000u) * c3;
     }
-    *reinterpret_cast<uint4*>(dx + row * K + col) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (kRes && a.dr) {
+      const uint4 rv = *reinterpret_cast<const uint4*>(a.dr + row * K + col);
+      const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bf16r2(d[2 * j], d[2 * j + 1]);
+        d[2 * j] = __uint_as_float(rw[j] << 16) + d[2 * j];
+        d[2 * j + 1] = __uint_as_float(rw[j] & 0xffff0000u) + d[2 * j + 1];
+      }
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(d[2 * j], d[2 * j + 1]);
+    *reinterpret_cast<uint4*>(a.dx + row * K + col) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (mg) {
+      const uint4 gg = *reinterpret_cast<const uint4*>(mg + col);
+      const uint32_t gw[4] = {gg.x, gg.y, gg.z, gg.w};
+      uint32_t e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        e[j] = pack_bf16x2(__uint_as_float(gw[j] << 16) * __uint_as_float(o[j] << 16),
+                           __uint_as_float(gw[j] & 0xffff0000u) * __uint_as_float(o[j] & 0xffff0000u));
+      *reinterpret_cast<uint4*>(a.dy + row * K + col) = make_uint4(e[0], e[1], e[2], e[3]);
+    }
   }
 }
 
-template <int WPR>
-void launch_rmsmod_bwd(const uint16_t* dh, const uint16_t* x, int64_t M, int K, const float* nw, float eps,
-                       const uint16_t* ms, int64_t ldm, int64_t rpb, uint16_t* dx, hipStream_t st) {
-  const dim3 grid((unsigned)((M + (4 / WPR) - 1) / (4 / WPR)));
-  const int nch = (K + 512 * WPR - 1) / (512 * WPR);
-#define K2Q_RMB(N)                                                                                            \
-  case N:                                                                                                     \
-    hipLaunchKernelGGL((rmsmod_bwd_kernel<WPR, N>), grid, dim3(256), 0, st, dh, x, M, K, nw, eps, ms, ldm, rpb, dx); \
+template <bool kRes, int WPR>
+void launch_rmsmod_bwd(const NormBwdArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.M + (4 / WPR) - 1) / (4 / WPR)));
+  const int nch = (a.K + 512 * WPR - 1) / (512 * WPR);
+#define K2Q_RMB(N)                                                                             \
+  case N:                                                                                      \
+    hipLaunchKernelGGL((rmsmod_bwd_kernel<kRes, WPR, N>), grid, dim3(256), 0, st, a);          \
     break;
   switch (nch) {
     K2Q_RMB(1) K2Q_RMB(2) K2Q_RMB(3) K2Q_RMB(4) K2Q_RMB(5) K2Q_RMB(6) K2Q_RMB(7)
-    default: hipLaunchKernelGGL((rmsmod_bwd_kernel<WPR, 8>), grid, dim3(256), 0, st, dh, x, M, K, nw, eps, ms, ldm,
-                                rpb, dx); break;
+    default: hipLaunchKernelGGL((rmsmod_bwd_kernel<kRes, WPR, 8>), grid, dim3(256), 0, st, a); break;
   }
 #undef K2Q_RMB
+}
+
+template <bool kRes>
+void launch_norm_bwd(const NormBwdArgs& a, hipStream_t st) {
+  if (a.K <= 4096) launch_rmsmod_bwd<kRes, 1>(a, st);
+  else if (a.K <= 8192) launch_rmsmod_bwd<kRes, 2>(a, st);
+  else launch_rmsmod_bwd<kRes, 4>(a, st);
+}
+
+// Column sums of the residual norm's backward: the gradients of what is broadcast over the rows of a batch entry,
+//   dscale = sum_m dh n,  dshift = sum_m dh,  dgate = sum_m dR y,  and over every row  dw = sum_m dn x r,
+// with n and dn as in the forward and backward (dn unrounded in f32: dw is an f32 gradient).  Rows are cut into strips
+// of one batch entry each; a workgroup sums one strip of 512 columns (lane: 8 columns, its four waves: every fourth
+// row) into f32 partials, and a second launch adds the strips in order: no atomics, the same result every time.
+constexpr int CS_COLS = 512;
+
+struct ColSumArgs {
+  const uint16_t *dh, *x, *y, *dx;   // M x K bf16 (y: row stride ldy; null: no gate)
+  const float* rinv;                 // M
+  int64_t M, ldy, rpb;
+  int K, strips, strip_rows;         // strips per batch entry, rows per strip
+  const float* nw;
+  float nwadd;
+  const uint16_t* mscale;            // or null
+  int64_t ldm;
+  float* part;                       // strip-major: (entry * strips + strip) x 4 x K
+};
+
+enum { CS_W = 0, CS_SCALE = 1, CS_SHIFT = 2, CS_GATE = 3 };
+
+__global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
+  __shared__ float red[3][64][33];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int K = a.K;
+  const int col = blockIdx.x * CS_COLS + 8 * lane;
+  const int entry = blockIdx.y / a.strips, strip = blockIdx.y % a.strips;
+  const int64_t m0 = entry * a.rpb + (int64_t)strip * a.strip_rows;
+  const int64_t mend = (int64_t)(entry + 1) * a.rpb;
+  const int64_t m1 = m0 + a.strip_rows < mend ? m0 + a.strip_rows : mend;
+  const int cc = col < K ? col : 0;
+  float w[8], p1[8], acc[4][8] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = a.nw[cc + i] + a.nwadd;
+    p1[i] = a.mscale ? bf16r(1.f + bf16_bits_to_f32(a.mscale[entry * a.ldm + cc + i])) : 1.f;
+  }
+  for (int64_t m = m0 + wave; m < m1; m += 4) {
+    const float r = a.rinv[m];
+    const uint4 dv = *reinterpret_cast<const uint4*>(a.dh + m * K + cc);
+    const uint4 xv = *reinterpret_cast<const uint4*>(a.x + m * K + cc);
+    const uint32_t dw[4] = {dv.x, dv.y, dv.z, dv.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = i & 1 ? __uint_as_float(dw[i >> 1] & 0xffff0000u) : __uint_as_float(dw[i >> 1] << 16);
+      const float x = i & 1 ? __uint_as_float(xw[i >> 1] & 0xffff0000u) : __uint_as_float(xw[i >> 1] << 16);
+      const float xr = x * r;
+      acc[CS_W][i] = __builtin_fmaf(d * p1[i], xr, acc[CS_W][i]);
+      acc[CS_SCALE][i] = __builtin_fmaf(d, bf16r(xr * w[i]), acc[CS_SCALE][i]);
+      acc[CS_SHIFT][i] += d;
+    }
+    if (a.y) {
+      const uint4 yv = *reinterpret_cast<const uint4*>(a.y + m * a.ldy + cc);
+      const uint4 ev = *reinterpret_cast<const uint4*>(a.dx + m * K + cc);
+      const uint32_t yw[4] = {yv.x, yv.y, yv.z, yv.w}, ew[4] = {ev.x, ev.y, ev.z, ev.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = i & 1 ? __uint_as_float(yw[i >> 1] & 0xffff0000u) : __uint_as_float(yw[i >> 1] << 16);
+        const float e = i & 1 ? __uint_as_float(ew[i >> 1] & 0xffff0000u) : __uint_as_float(ew[i >> 1] << 16);
+        acc[CS_GATE][i] = __builtin_fmaf(e, y, acc[CS_GATE][i]);
+      }
+    }
+  }
+  if (wave)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) red[wave - 1][lane][i] = acc[i >> 3][i & 7];
+  __syncthreads();
+  if (wave || col >= K) return;
+  float* out = a.part + (int64_t)blockIdx.y * 4 * K + col;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      out[(int64_t)k * K + i] = ((acc[k][i] + red[0][lane][8 * k + i]) + red[1][lane][8 * k + i]) + red[2][lane][8 * k + i];
+}
+
+// One thread a column: the strips' partials in order.  Grid y: the batch entries (scale, shift and gate gradients,
+// bf16), then one more for the norm weight's (f32, over every entry).
+__global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* part, int K, int entries, int strips,
+                                                                  float* dnw, uint16_t* dscale, uint16_t* dshift,
+                                                                  uint16_t* dgate) {
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col >= K) return;
+  const int entry = blockIdx.y;
+  if (entry == entries) {
+    if (!dnw) return;
+    float f = 0.f;
+    for (int64_t i = 0; i < (int64_t)entries * strips; ++i) f += part[(i * 4 + CS_W) * K + col];
+    dnw[col] = f;
+    return;
+  }
+  float f[3] = {};
+  for (int64_t i = (int64_t)entry * strips; i < (int64_t)(entry + 1) * strips; ++i)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) f[k] += part[(i * 4 + CS_SCALE + k) * K + col];
+  const int64_t o = (int64_t)entry * K + col;
+  if (dscale) dscale[o] = (uint16_t)f32_to_bf16_bits(f[0]);
+  if (dshift) dshift[o] = (uint16_t)f32_to_bf16_bits(f[1]);
+  if (dgate) dgate[o] = (uint16_t)f32_to_bf16_bits(f[2]);
+}
+
+// Strips per batch entry: about two workgroups a CU over the column tiles, at least 32 rows each.
+int colsum_strips(int64_t rpb, int64_t K, int64_t entries, int cus) {
+  const int64_t tiles = (K + CS_COLS - 1) / CS_COLS * entries;
+  int64_t s = (2 * cus + tiles - 1) / tiles;
+  const int64_t most = (rpb + 31) / 32;
+  s = s < 1 ? 1 : s > most ? most : s;
+  const int64_t rows = (rpb + s - 1) / s;
+  return (int)((rpb + rows - 1) / rows);
 }
 
 }  // namespace
@@ -391,10 +597,19 @@ extern "C" int k2q_rmsmod_bwd(const uint16_t* dh, const uint16_t* x, int64_t M, 
       !k2q_aligned(norm_scale, 16) || !k2q_aligned(mod_scale, 16) || !k2q_aligned(dx, 16) || ld_mod < 0 ||
       ld_mod % 8 || rows_per_batch < 1 || !(eps >= 0.f))
     return K2Q_EINVAL;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  if (K <= 4096) launch_rmsmod_bwd<1>(dh, x, M, (int)K, norm_scale, eps, mod_scale, ld_mod, rows_per_batch, dx, st);
-  else if (K <= 8192) launch_rmsmod_bwd<2>(dh, x, M, (int)K, norm_scale, eps, mod_scale, ld_mod, rows_per_batch, dx, st);
-  else launch_rmsmod_bwd<4>(dh, x, M, (int)K, norm_scale, eps, mod_scale, ld_mod, rows_per_batch, dx, st);
+  NormBwdArgs a{};
+  a.dh = dh;
+  a.x = x;
+  a.M = M;
+  a.K = (int)K;
+  a.nw = norm_scale;
+  a.nwadd = 1.f;
+  a.eps = eps;
+  a.mscale = mod_scale;
+  a.ldm = ld_mod;
+  a.rpb = rows_per_batch;
+  a.dx = dx;
+  launch_norm_bwd<false>(a, static_cast<hipStream_t>(stream));
   return k2q_launch_status();
 }
 
@@ -430,9 +645,10 @@ extern "C" int k2q_rmsmod_rotquant(const uint16_t* x, int64_t ldx, int64_t M, in
   a.x0 = reinterpret_cast<const __bf16*>(x);
   a.ld0 = ldx;
   a.nw = norm_scale;
+  a.nwadd = 1.f;
   a.mscale = mod_scale;
   a.mshift = mod_shift;
-  a.ldm = ld_mod;
+  a.ldm = a.ldb = ld_mod;
   a.rpb = rows_per_batch;
   a.eps = eps;
   a.M = M;
@@ -441,6 +657,51 @@ extern "C" int k2q_rmsmod_rotquant(const uint16_t* x, int64_t ldx, int64_t M, in
   a.q = q;
   a.s = s;
   return launch_prod<PROD_RMSMOD>(a, static_cast<hipStream_t>(stream));
+}
+
+namespace {
+
+// A per-entry row vector (gate, modulation scale or shift): 16-byte aligned rows, row stride ld (0: one entry).
+bool rowvec_ok(const uint16_t* p, int64_t ld) { return k2q_aligned(p, 16) && ld >= 0 && ld % 8 == 0; }
+
+}  // namespace
+
+extern "C" int k2q_resnorm_rotquant(const uint16_t* x, int64_t ldx, const uint16_t* y, int64_t ldy,
+                                    const uint16_t* gate, int64_t ld_gate, int64_t M, int64_t K,
+                                    const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale,
+                                    int64_t ld_scale, const uint16_t* mod_shift, int64_t ld_shift,
+                                    int64_t rows_per_batch, uint16_t* r, uint16_t* h, int8_t* q, float* s,
+                                    void* stream) {
+  int rc = check_prod_common(M, K, h, q, s);
+  if (rc) return rc;
+  if (M > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  if (!x || !y || !norm_scale || !r || !k2q_aligned(x, 16) || !k2q_aligned(y, 16) || !k2q_aligned(norm_scale, 16) ||
+      !k2q_aligned(r, 16) || ldx < K || ldx % 8 || ldy < K || ldy % 8 || rows_per_batch < 1 || !(eps >= 0.f) ||
+      !rowvec_ok(gate, ld_gate) || !rowvec_ok(mod_scale, ld_scale) || !rowvec_ok(mod_shift, ld_shift) ||
+      !mod_scale != !mod_shift)
+    return K2Q_EINVAL;
+  ProdArgs a{};
+  a.x0 = reinterpret_cast<const __bf16*>(x);
+  a.x1 = reinterpret_cast<const __bf16*>(y);
+  a.ld0 = ldx;
+  a.ld1 = ldy;
+  a.nw = norm_scale;
+  a.nwadd = scale_add;
+  a.mscale = mod_scale;
+  a.mshift = mod_shift;
+  a.gate = gate;
+  a.ldm = ld_scale;
+  a.ldb = ld_shift;
+  a.ldg = ld_gate;
+  a.rpb = rows_per_batch;
+  a.eps = eps;
+  a.M = M;
+  a.K = (int)K;
+  a.r = r;
+  a.h = h;
+  a.q = q;
+  a.s = s;
+  return launch_prod<PROD_RESNORM>(a, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int k2q_swiglu_bwd(const uint16_t* dh, const uint16_t* gate, const uint16_t* up, int64_t n,
@@ -456,5 +717,75 @@ extern "C" int k2q_swiglu_bwd(const uint16_t* dh, const uint16_t* gate, const ui
                      reinterpret_cast<const uint4*>(dh), reinterpret_cast<const uint4*>(gate),
                      reinterpret_cast<const uint4*>(up), n8, reinterpret_cast<uint4*>(dgate),
                      reinterpret_cast<uint4*>(dup));
+  return k2q_launch_status();
+}
+
+extern "C" int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch) {
+  if (M < 1 || K < 8 || K % 8 || K > 16384 || rows_per_batch < 1 || M % rows_per_batch) return 0;
+  const int64_t entries = M / rows_per_batch;
+  return (M + entries * colsum_strips(rows_per_batch, K, entries, k2q_cu_count()) * 4 * K) * 4;
+}
+
+extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
+                               const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale,
+                               int64_t ld_scale, const uint16_t* gate, int64_t ld_gate, int64_t rows_per_batch,
+                               uint16_t* dx, uint16_t* dy, const uint16_t* y, int64_t ldy, float* dnorm,
+                               uint16_t* dscale, uint16_t* dshift, uint16_t* dgate, void* ws, int64_t ws_bytes,
+                               void* stream) {
+  if (M < 1 || K < 8 || K % 8) return K2Q_EINVAL;
+  if (K > 16384 || M > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  if (!dh || !r || !norm_scale || !dx || !k2q_aligned(dh, 16) || !k2q_aligned(dr, 16) || !k2q_aligned(r, 16) ||
+      !k2q_aligned(norm_scale, 16) || !k2q_aligned(dx, 16) || !k2q_aligned(dy, 16) || !rowvec_ok(mod_scale, ld_scale) ||
+      !rowvec_ok(gate, ld_gate) || rows_per_batch < 1 || !(eps >= 0.f) || !gate != !dy)
+    return K2Q_EINVAL;
+  const bool cols = dnorm || dscale || dshift || dgate;
+  const int64_t entries = M / rows_per_batch;
+  if (cols) {
+    if (M % rows_per_batch || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_resnorm_bwd_ws_bytes(M, K, rows_per_batch) ||
+        ((dscale || dshift) && !mod_scale) || (dgate && (!gate || !y || !k2q_aligned(y, 16) || ldy < K || ldy % 8)))
+      return K2Q_EINVAL;
+    if (entries > 32767) return K2Q_EUNSUPPORTED;   // launch extents: two bytes of entries and strips
+  }
+  NormBwdArgs a{};
+  a.dh = dh;
+  a.x = r;
+  a.M = M;
+  a.K = (int)K;
+  a.nw = norm_scale;
+  a.nwadd = scale_add;
+  a.eps = eps;
+  a.mscale = mod_scale;
+  a.ldm = ld_scale;
+  a.rpb = rows_per_batch;
+  a.dx = dx;
+  a.dr = dr;
+  a.gate = gate;
+  a.ldg = ld_gate;
+  a.dy = dy;
+  a.rinv = cols ? static_cast<float*>(ws) : nullptr;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  launch_norm_bwd<true>(a, st);
+  if (!cols) return k2q_launch_status();
+  ColSumArgs c{};
+  c.dh = dh;
+  c.x = r;
+  c.y = dgate ? y : nullptr;
+  c.dx = dx;
+  c.rinv = a.rinv;
+  c.M = M;
+  c.ldy = ldy;
+  c.rpb = rows_per_batch;
+  c.K = (int)K;
+  c.strips = colsum_strips(rows_per_batch, K, entries, k2q_cu_count());
+  c.strip_rows = (int)((rows_per_batch + c.strips - 1) / c.strips);
+  c.nw = norm_scale;
+  c.nwadd = scale_add;
+  c.mscale = mod_scale;
+  c.ldm = ld_scale;
+  c.part = a.rinv + M;
+  const dim3 grid((unsigned)((K + CS_COLS - 1) / CS_COLS), (unsigned)(entries * c.strips));
+  hipLaunchKernelGGL(resnorm_colsum_kernel, grid, dim3(256), 0, st, c);
+  hipLaunchKernelGGL(resnorm_colsum_join_kernel, dim3((unsigned)((K + 255) / 256), (unsigned)entries + 1), dim3(256), 0,
+                     st, c.part, (int)K, (int)entries, c.strips, dnorm, dscale, dshift, dgate);
   return k2q_launch_status();
 }

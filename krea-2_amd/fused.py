@@ -25,10 +25,16 @@ from . import _lib
 from .quantize import ConvRotLinear, shared_input_quant
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned: a contiguous view may start anywhere in its storage."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _rows(t: torch.Tensor, K: int) -> torch.Tensor:
     t2 = t.reshape(-1, K)
-    if t2.stride(1) != 1 or t2.stride(0) % 8 or t2.data_ptr() % 16:
-        t2 = t2.contiguous()
+    if t2.stride(1) != 1 or t2.stride(0) % 8 or t2.stride(0) < K or t2.data_ptr() % 16:
+        t2 = _aligned(t2)
     return t2
 
 
@@ -38,8 +44,7 @@ def _dense_grad(dh, like):
     no gradient (two fills per producer: an MLP half's training pass at 768 x 6144 x 16384 1070.3 -> 1064.6 us)."""
     if dh is None:
         return torch.zeros(like.shape, dtype=torch.bfloat16, device=like.device)
-    dh = dh.contiguous()
-    return dh if dh.dtype == torch.bfloat16 else dh.to(torch.bfloat16)
+    return _aligned(dh if dh.dtype == torch.bfloat16 else dh.to(torch.bfloat16))
 
 
 class _SwiGLUQuantFn(torch.autograd.Function):
@@ -104,10 +109,39 @@ class _RmsModQuantFn(torch.autograd.Function):
         return dx, None, None, None, None, None
 
 
-def _norm_scale_f32(norm: nn.Module) -> torch.Tensor:
-    """The norm's (frozen) scale as the kernels take it, f32 and contiguous, kept on the module and rebuilt when
-    the scale changes (in place: version; re-pointed, e.g. paged by block swap: pointer or device)."""
-    t = norm.scale
+class _ResNormQuantFn(torch.autograd.Function):
+    """Forward: the residual's addition and the (modulated) RMSNorm of ``mmdit.py:317-318`` with the codes of its output,
+    one gfx950 pass.  Backward ``k2q_resnorm_bwd``: the gradients of the stream and of what was added in one pass, and the
+    sums over the rows for the gate, the modulation and the norm's scale where they are asked for."""
+
+    @staticmethod
+    def forward(ctx, x2, y2, gate, w, scale, shift, add, eps, rows):
+        r, h, q, s = _lib.resnorm_rotquant(x2, y2, gate, w, add, eps, scale, shift, rows)
+        ctx.add, ctx.eps, ctx.rows = add, eps, rows
+        ctx.save_for_backward(r, w, scale, gate, y2 if gate is not None and ctx.needs_input_grad[2] else None)
+        ctx.mark_non_differentiable(q, s)
+        ctx.set_materialize_grads(False)
+        return r, h, q, s
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dr, dh, _dq, _ds):
+        if dr is None and dh is None:
+            return (None,) * 9
+        r, w, scale, gate, y2 = ctx.saved_tensors
+        nx, ny, ng, nw, ns, nb = ctx.needs_input_grad[:6]
+        dx, dy, dw, dscale, dshift, dgate = _lib.resnorm_bwd(
+            _dense_grad(dh, r), None if dr is None else _dense_grad(dr, r), r, w, ctx.add, ctx.eps, scale, gate,
+            ctx.rows, y2, nw, ns, nb)
+        if gate is None:
+            dy = dx
+        return dx if nx else None, dy if ny else None, dgate, dw, dscale, dshift, None, None, None
+
+
+def _norm_scale_f32(norm: nn.Module, name: str = "scale") -> torch.Tensor:
+    """The norm's (frozen) scale (or ``weight``) as the kernels take it, f32 and contiguous, kept on the module and rebuilt
+    when it changes (in place: version; re-pointed, e.g. paged by block swap: pointer or device)."""
+    t = getattr(norm, name)
     key = (t._version, t.data_ptr(), t.device, t.dtype, tuple(t.shape))
     kept = norm.__dict__.get("_k2q_scale_f32")
     if kept is None or kept[0] != key:
@@ -148,6 +182,92 @@ def modulated_rmsnorm(norm: nn.Module, x: torch.Tensor, scale: torch.Tensor, shi
     return h
 
 
+def _entry_rows(t: torch.Tensor, name: str, x: torch.Tensor):
+    """A gate or modulation vector of ``x`` (.., K) as rows: (1, K) for one entry, or (B, K) with one per batch row of
+    ``x``, broadcast over its tokens."""
+    K = x.shape[-1]
+    if t.shape[-1:] != (K,):
+        raise ValueError(f"{name} {tuple(t.shape)} does not match {K} features")
+    n = t.numel() // K
+    if n != 1 and (x.dim() < 2 or x.shape[0] != n or t.shape[0] != n or any(d != 1 for d in t.shape[1:-1])):
+        raise ValueError(f"{name} {tuple(t.shape)} does not broadcast over x {tuple(x.shape)} per batch row")
+    t = t.reshape(n, K)
+    if t.stride(1) != 1 or (n > 1 and t.stride(0) % 8) or t.data_ptr() % 16:
+        t = _aligned(t)
+    return t
+
+
+def _norm_weight(norm: nn.Module, train: bool):
+    """``(w, add)``: the norm's weight is ``w + add``, w f32.  A norm with a ``scale`` (``mmdit.py:146-161``) weighs by
+    ``scale + 1``, one with a ``weight`` by it."""
+    for name, add in (("scale", 1.0), ("weight", 0.0)):
+        t = getattr(norm, name, None)
+        if isinstance(t, torch.Tensor):
+            return (t.float().contiguous() if train and t.requires_grad else _norm_scale_f32(norm, name)), add
+    raise ValueError(f"{type(norm).__name__} has neither a scale nor a weight")
+
+
+def residual_rmsnorm(norm: nn.Module, x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None = None,
+                     scale: torch.Tensor | None = None, shift: torch.Tensor | None = None):
+    """``r = x + gate * y`` and ``h``, the norm of r (``mmdit.py:317-318``), in one pass with the int8 codes of ``h``, which
+    the ConvRot layers that receive it take.  Returns ``(r, h)``.
+
+    ``norm`` is an RMSNorm module with ``eps`` and a ``scale`` (weight ``scale + 1``, ``mmdit.py:146-161``) or a
+    ``weight``; ``h`` is modulated, ``(1 + scale) * norm(r) + shift``, where ``scale`` and ``shift`` are given.  ``x`` and
+    ``y`` (B, L, K) or (M, K) bf16; ``gate``, ``scale``, ``shift`` bf16, one entry or one per batch row of ``x`` ((B, 1,
+    K)).  Every tensor of the formula is rounded to bf16 where the eager bf16 operations round it, so ``r`` and ``h`` equal
+    theirs (and ``h`` that of :func:`modulated_rmsnorm` on ``r``) bit for bit; the mean square and every gradient's sum
+    over rows are float32.
+
+    Differentiable (once) in ``x``, ``y``, ``gate``, ``scale``, ``shift`` and the norm's parameter; the gradients of the
+    last four are sums over rows, added in a fixed order."""
+    given = [t for t in (x, y, gate, scale, shift) if t is not None]
+    if any(t.dtype != torch.bfloat16 for t in given):
+        raise NotImplementedError("the fused residual RMSNorm runs bf16 tensors (the DiT dtype)")
+    if x.shape != y.shape:
+        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} differ in shape")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift come together")
+    K = x.shape[-1]
+    grad = torch.is_grad_enabled()
+    w, add = _norm_weight(norm, grad)
+    if w.shape != (K,):
+        raise ValueError(f"the norm's weight {tuple(w.shape)} does not match {K} features")
+    g2, s2, b2 = (None if t is None else _entry_rows(t, name, x)
+                  for t, name in ((gate, "gate"), (scale, "scale"), (shift, "shift")))
+    _lib._check_k(K)
+    if x.numel() == 0:
+        _lib._device_check(x.device)
+        r = x + y if gate is None else x + gate.reshape(gate.shape[0] if g2.shape[0] > 1 else 1,
+                                                        *(1,) * (x.dim() - 2), K) * y
+        return r, torch.zeros_like(r)
+    x2, y2 = _rows(x, K), _rows(y, K)
+    M = x2.shape[0]
+    entries = max([t.shape[0] for t in (g2, s2, b2) if t is not None], default=1)
+    rows = M // entries
+    eps = float(norm.eps)
+    if _lib.observed() or (grad and any(t.requires_grad for t in (w, *given))):
+        if entries > 1:     # one gradient row per entry: autograd sums those of a vector given once
+            g2, s2, b2 = (t if t is None or t.shape[0] == entries else t.expand(entries, K) for t in (g2, s2, b2))
+        r, h, q, s = _ResNormQuantFn.apply(x2, y2, g2, w, s2, b2, add, eps, rows)
+    else:                   # nothing to differentiate: no autograd node
+        r, h, q, s = _lib.resnorm_rotquant(x2, y2, g2, w, add, eps, s2, b2, rows)
+    if x.dim() != 2:
+        r, h = r.reshape(x.shape), h.reshape(x.shape)
+    shared_input_quant.seed(h, q, s)
+    return r, h
+
+
+def input_codes(h: torch.Tensor):
+    """``(q, s)``: the int8 codes (rows, K) of ``h``'s rotated rows and their f32 scales (rows,), as the ConvRot layers
+    take them: a code stands for ``q * s``.  Those that the producer of this very tensor left, else computed now (and
+    kept for the next layer)."""
+    if h.dtype != torch.bfloat16:
+        raise NotImplementedError("the codes are those of a bf16 tensor (the DiT dtype)")
+    with torch.no_grad():
+        return shared_input_quant.lookup(h, _aligned(h.reshape(-1, h.shape[-1])))
+
+
 # ----------------------------------------------------------------------------------------------------------
 # In-place patch of a DiT's blocks
 # ----------------------------------------------------------------------------------------------------------
@@ -177,9 +297,20 @@ def _fused_block_forward(self, x, vec, freqs, mask=None):
     if _block_norms_train(self, vec):
         return type(self).forward(self, x, vec, freqs, mask)
     prescale, preshift, pregate, postscale, postshift, postgate = self.mod(vec)
-    x = x + pregate * self.attn(modulated_rmsnorm(self.prenorm, x, prescale, preshift), freqs, mask)
-    x = x + postgate * self.mlp(modulated_rmsnorm(self.postnorm, x, postscale, postshift))
-    return x
+    a = self.attn(modulated_rmsnorm(self.prenorm, x, prescale, preshift), freqs, mask)
+    if _takes_residual(x, a, pregate):
+        x, h = residual_rmsnorm(self.postnorm, x, a, pregate, postscale, postshift)
+    else:
+        x = x + pregate * a
+        h = modulated_rmsnorm(self.postnorm, x, postscale, postshift)
+    return x + postgate * self.mlp(h)
+
+
+def _takes_residual(x, a, gate) -> bool:
+    """Whether the gated residual is one that :func:`residual_rmsnorm` adds (else the block adds it eagerly)."""
+    n = gate.numel() // x.shape[-1]
+    return (a.dtype == gate.dtype == torch.bfloat16 and a.shape == x.shape and gate.shape[-1] == x.shape[-1]
+            and (n == 1 or (n == gate.shape[0] == x.shape[0] and x.dim() == gate.dim() == 3)))
 
 
 def fuse_producers(dit) -> int:

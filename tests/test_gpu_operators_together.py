@@ -1,0 +1,139 @@
+"""The operators as a decoder layer uses them: the residual norm's codes into quantized projections (int4 base, LoRA), rotary
+positions, attention, and the next residual norm, for a prompt, for single tokens and in training."""
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+FEAT, HEADS, KV, D, HID = 512, 8, 2, 64, 1024
+
+
+class Norm(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.eps, self.scale = 1e-5, nn.Parameter(torch.zeros(FEAT))
+
+
+class Layer(nn.Module):
+    def __init__(self, rope, mode):
+        super().__init__()
+        self.mode, self.rope = mode, rope
+        self.norm1, self.norm2 = Norm(), Norm()
+        for name, k, n in (("wq", FEAT, HEADS * D), ("wk", FEAT, KV * D), ("wv", FEAT, KV * D), ("wo", HEADS * D, FEAT),
+                           ("gate", FEAT, HID), ("up", FEAT, HID), ("down", HID, FEAT)):
+            setattr(self, name, nn.Linear(k, n, bias=False))
+
+    def attend(self, h, pos, cache):
+        B, L, _ = h.shape
+        q, k, v = (w(h).view(B, L, -1, D) for w in (self.wq, self.wk, self.wv))
+        q, k = self.rope(q, k, pos)
+        if cache is not None:
+            k, v = torch.cat([cache[0], k], 1), torch.cat([cache[1], v], 1)
+        q, kk, vv = q.transpose(1, 2).float(), *(t.transpose(1, 2).repeat_interleave(HEADS // KV, 1).float() for t in (k, v))
+        s = q @ kk.transpose(-1, -2).contiguous() * D ** -0.5
+        hide = torch.arange(kk.shape[2], device=h.device) > pos.expand(B, L).view(B, 1, L, 1)
+        o = s.masked_fill(hide, float("-inf")).softmax(-1) @ vv
+        return self.wo(o.to(h.dtype).transpose(1, 2).reshape(B, L, -1)), (k, v)
+
+    def forward(self, k2, x, add, pos, cache=None):
+        x, h = k2.residual_rmsnorm(self.norm1, x, add)
+        a, cache = self.attend(h, pos, cache)
+        x, h = k2.residual_rmsnorm(self.norm2, x, a)
+        return x, self.down(k2.swiglu(self.gate(h), self.up(h))), cache
+
+
+def _model(k2, dev, mode, n=2):
+    torch.manual_seed(1)
+    rope = k2.RotaryEmbedding(D, layout="half", scaling=k2.RotaryScaling("yarn", 2.0, 64))
+    m = nn.Module()
+    m.blocks = nn.ModuleList([Layer(rope, mode) for _ in range(n)]).to(dev).to(torch.bfloat16)
+    for b in m.blocks:
+        for nm in (b.norm1, b.norm2):
+            nm.float()
+            nm.scale.data.normal_(0, 0.1)
+    k2.quantize_dit_convrot(m, mode)
+    names = ("wq", "wk", "wv", "wo", "gate", "up", "down")
+    ad = k2.inject_lora(m, 16, targets=names, include_txtfusion=False, include_txtmlp=False)
+    for a in ad.values():
+        a.lora_B.data.normal_(0, 0.02)
+    return m, ad
+
+
+def _run(k2, m, x, pos, caches=None):
+    add, out = torch.zeros_like(x), []
+    for i, b in enumerate(m.blocks):
+        x, add, c = b(k2, x, add, pos, caches[i] if caches else None)
+        out.append(c)
+    return x + add, out
+
+
+@pytest.mark.parametrize("mode", ["w8a8", "w4a8"])
+def test_prompt_then_tokens(k2, dev, mode):
+    """Tokens served one at a time over a cache against the prompt in one call: the same operators at 1 row and at 24.  The
+    codes of a row do not depend on the rows beside it; the linears' sums differ in float32 and the attention's in order,
+    so a rounding of h may fall the other way and flip codes: the bf16 bar of 1e-2 applies."""
+    from krea2_amd.quantize import shared_input_quant
+    m, _ = _model(k2, dev, mode)
+    x = torch.randn(1, 24, FEAT, device=dev).bfloat16()
+    pos = torch.arange(24, device=dev)
+    with torch.no_grad():
+        whole, _ = _run(k2, m, x, pos)
+        caches = [(torch.empty(1, 0, KV, D, device=dev, dtype=torch.bfloat16),) * 2 for _ in m.blocks]
+        rows = []
+        for t in range(24):
+            misses = shared_input_quant.misses
+            y, caches = _run(k2, m, x[:, t:t + 1].clone(), pos[t:t + 1], caches)
+            assert shared_input_quant.misses - misses == len(m.blocks)      # the attention outputs alone are coded apart
+            rows.append(y)
+    got = torch.cat(rows, 1)
+    assert (got.double() - whole.double()).norm() <= 1e-2 * whole.double().norm()
+
+
+@pytest.mark.parametrize("mode", ["w8a8", "w4a8"])
+def test_training_step(k2, dev, mode):
+    """Gradients of the stream and every adapter against the same layer over the eager operations (float32 norm, complex
+    rotation), and a checkpointed step bit for bit."""
+    from torch.utils.checkpoint import checkpoint
+    m, ad = _model(k2, dev, mode)
+    x = torch.randn(2, 40, FEAT, device=dev).bfloat16()
+    dy = torch.randn_like(x)
+    pos = torch.arange(40, device=dev).expand(2, 40)
+    params = k2.lora_parameters(ad)
+
+    def step(run):
+        t = x.detach().clone().requires_grad_()
+        y = run(t)
+        return [y.detach(), *torch.autograd.grad(y, [t, *params], dy)]
+
+    fused = step(lambda t: _run(k2, m, t, pos)[0])
+    again = step(lambda t: checkpoint(lambda u: _run(k2, m, u, pos)[0], t, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(fused, again))
+
+    class Eager:
+        swiglu = staticmethod(lambda g, u: F.silu(g) * u)
+
+        @staticmethod
+        def residual_rmsnorm(norm, x, y):
+            r = x + y
+            return r, F.rms_norm(r.float(), (FEAT,), eps=norm.eps, weight=norm.scale.float() + 1.0).to(r.dtype)
+
+    def rotate(q, k, pos):
+        a = pos.double().unsqueeze(-1) * torch.tensor(m.blocks[0].rope.frequencies, device=dev, dtype=torch.float64)
+        c, s = ((f(a) * m.blocks[0].rope.factor).float().unsqueeze(2) for f in (torch.cos, torch.sin))
+
+        def one(t):
+            u, v = t.float().chunk(2, -1)
+            return torch.cat([u * c - v * s, u * s + v * c], -1).to(t.dtype)
+        return one(q), one(k)
+
+    ropes = [b._modules.pop("rope") for b in m.blocks]
+    for b in m.blocks:
+        object.__setattr__(b, "rope", rotate)
+    m.blocks[0].rope.__dict__.update(frequencies=ropes[0].frequencies, factor=ropes[0].factor)
+    eager = step(lambda t: _run(Eager, m, t, pos)[0])
+    # the eager norm and silu round an element of h the other way now and then, which flips codes: the bars of the blocks
+    bars = [1e-2, 1e-2] + [2e-2] * len(params)
+    for a, e, bar in zip(fused, eager, bars):
+        assert (a.double() - e.double()).norm() <= bar * e.double().norm()

@@ -1,0 +1,115 @@
+"""CPU tests of the arguments that the residual norm, the rotary positions and the W4A8 matrix-vector product refuse, and
+of the rotary frequencies."""
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+
+class _Norm(nn.Module):
+    def __init__(self, k):
+        super().__init__()
+        self.eps, self.scale = 1e-5, nn.Parameter(torch.zeros(k), requires_grad=False)
+
+
+def test_residual_norm_refuses_before_any_launch(k2):
+    x = torch.zeros(2, 3, 256, dtype=torch.bfloat16)
+    v = torch.zeros(2, 1, 256, dtype=torch.bfloat16)
+    f = k2.residual_rmsnorm
+    for bad in (lambda: f(_Norm(256), x, x[:, :2]), lambda: f(_Norm(256), x, x, v, v), lambda: f(_Norm(128), x, x),
+                lambda: f(_Norm(256), x, x, v[..., :128]), lambda: f(_Norm(256), x, x, v.expand(2, 3, 256)),
+                lambda: f(_Norm(256), x, x, torch.cat([v, v[:1]])), lambda: f(nn.Module(), x, x),
+                lambda: f(_Norm(64), x[..., :64], x[..., :64])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        f(_Norm(256), x, x.float())
+    with pytest.raises(NotImplementedError):
+        k2.input_codes(x.float())
+    with pytest.raises(RuntimeError):
+        f(_Norm(256), x, x, v)
+    with pytest.raises(RuntimeError):
+        f(_Norm(256), x[:, :0], x[:, :0])
+
+
+def test_entry_points_refuse_bad_arguments(k2):
+    """The C entries' own checks (addresses that are never read)."""
+    lib = k2._lib.load()
+    p, odd = 4096, 4100
+
+    def norm(x=p, ldx=256, y=p, gate=p, ldg=0, M=4, K=256, w=p, eps=1e-5, ms=p, ls=0, mb=p, lb=0, rows=4, r=p, h=p, q=p,
+             s=p):
+        return lib.k2q_resnorm_rotquant(x, ldx, y, 256, gate, ldg, M, K, w, 1.0, eps, ms, ls, mb, lb, rows, r, h, q, s, None)
+
+    for bad in ({"x": None}, {"x": odd}, {"ldx": 255}, {"ldx": 128}, {"y": None}, {"gate": odd}, {"ldg": 4}, {"M": 0},
+                {"K": 192}, {"w": None}, {"eps": float("nan")}, {"ms": None}, {"mb": None}, {"lb": -8}, {"rows": 0},
+                {"r": None}, {"h": odd}, {"q": None}, {"s": None}):
+        assert norm(**bad) == -1, bad
+    assert norm(K=16512, ldx=16512) == -4 and norm(M=1 << 31) == -4
+
+    def bwd(dh=p, r=p, M=4, K=256, ms=p, gate=p, rows=2, dx=p, dy=p, y=p, dw=p, ds=p, dg=p, ws=p, nws=1 << 30):
+        return lib.k2q_resnorm_bwd(dh, None, r, M, K, p, 1.0, 1e-5, ms, 0, gate, 0, rows, dx, dy, y, 256, dw, ds, None, dg,
+                                   ws, nws, None)
+
+    for bad in ({"dh": None}, {"r": odd}, {"M": 0}, {"K": 100}, {"ms": None}, {"gate": None}, {"dy": None}, {"rows": 3},
+                {"rows": 0}, {"dx": None}, {"y": None}, {"ws": None}, {"nws": 16}):
+        assert bwd(**bad) == -1, bad
+    assert bwd(M=40000, rows=1) == -4
+
+    heads = k2._lib.RotaryHeads(p, p, 4, 64 * 4 * 6, 256, 64, 64 * 4 * 6, 256, 64)
+
+    def rot(t=heads, n=1, dtype=0, B=1, L=6, D=64, dim=64, layout=0, pos=p, pt=0, turns=p):
+        return lib.k2q_rotary(ctypes.byref(t) if t is not None else None, n, dtype, B, L, D, dim, layout, pos, pt, 0, 1, 0,
+                              turns, None, 1.0, 0, None)
+
+    for bad in ({"t": None}, {"n": 0}, {"n": 3}, {"dtype": 3}, {"dtype": -1}, {"B": 0}, {"L": 0}, {"dim": 66}, {"dim": 63},
+                {"dim": 0}, {"layout": 2}, {"pos": None}, {"pos": odd}, {"pt": 4}, {"turns": None},
+                {"t": k2._lib.RotaryHeads(p, None, 4, 0, 0, 0, 0, 0, 0)}, {"t": k2._lib.RotaryHeads(p, p, 0, 0, 0, 0, 0, 0, 0)}):
+        assert rot(**bad) == -1, bad
+    assert rot(D=8192) == -4 and rot(D=4096, dim=2048) == -4 and rot(B=1 << 20, L=1 << 20) == -4
+
+
+def test_w4_gemv_needs_no_workspace(k2):
+    lib = k2._lib.load()
+    for M in range(1, 9):
+        assert lib.k2q_linear_fwd_ws_bytes(1, M, 1536, 16384, 0) == 0
+
+
+def test_rotary_module_refuses(k2):
+    R, S = k2.RotaryEmbedding, k2.RotaryScaling
+    for bad in (lambda: R(0), lambda: R(63), lambda: R(2048), lambda: R(64, layout="both"), lambda: R(64, axes=(32, 16)),
+                lambda: R(64, axes=(33, 31)), lambda: R(64, theta=1.0), lambda: S("other", 2.0), lambda: S("linear", 0.5),
+                lambda: S("linear", float("nan")), lambda: S("yarn", 4.0), lambda: S("yarn", 4.0, 2048, 1.0, 32.0),
+                lambda: R(2, scaling=S("ntk", 2.0))):
+        with pytest.raises(ValueError):
+            bad()
+    rope = R(64)
+    q = torch.zeros(1, 5, 2, 64)
+    with pytest.raises(RuntimeError):
+        rope(q, None, torch.arange(5))
+    with pytest.raises(ValueError):
+        rope(q[..., :32], None, torch.arange(5))
+    assert rope(q[:, :0], None, torch.arange(0))[0].shape == (1, 0, 2, 64)
+    assert not list(rope.parameters()) and not rope.state_dict()
+
+
+def test_rotary_frequencies(k2):
+    R, S = k2.RotaryEmbedding, k2.RotaryScaling
+    f = R(8, theta=10000.0).frequencies
+    assert all(math.isclose(a, b) for a, b in zip(f, (1.0, 0.1, 0.01, 0.001)))
+    assert R(8, axes=(4, 4)).frequencies == R(4).frequencies * 2
+    g = R(128, scaling=S("yarn", 4.0, 4096)).frequencies
+    p = R(128).frequencies
+    kept = [2 * math.pi / v * 32 <= 4096 for v in p]             # over 32 turns within the original length
+    slow = [2 * math.pi / v >= 4096 for v in p]                  # under one
+    assert any(kept) and any(slow)
+    for i, v in enumerate(p):
+        if kept[i] and i + 1 < len(p) and kept[i + 1]:
+            assert math.isclose(g[i], v)
+        elif slow[i] and slow[i - 1]:
+            assert math.isclose(g[i], v / 4)
+        else:
+            assert v / 4 <= g[i] * (1 + 1e-12) and g[i] <= v * (1 + 1e-12)
+    assert R(64, scaling=S("yarn", 4.0, 4096, attention_factor=1.5)).factor == 1.5
