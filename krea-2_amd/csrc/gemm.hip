@@ -2168,8 +2168,10 @@ extern "C" int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, i
   return launch_gemm<EPI_DXLIN>(p, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
+static bool w4_takes_gemv(int64_t M, int64_t K) { return M <= K2Q_GEMV_MAX_M && K <= 16384; }
+
 int64_t gemm_w4a8_ws_bytes(int64_t M, int64_t N, int64_t K) {
-  if (check_common(M, N, K) || M <= K2Q_GEMV_MAX_M) return 0;
+  if (check_common(M, N, K) || w4_takes_gemv(M, K)) return 0;
   return w4_piece_bytes(M, N, w4_plan(M, N, K, k2q_cu_count(), true));
 }
 
@@ -2197,7 +2199,7 @@ int gemm_w4a8_impl(const int8_t* qx, const float* sx, const uint8_t* qw4, const 
     return K2Q_EINVAL;
   if (bias && !k2q_aligned(bias, 16)) return K2Q_EINVAL;
   if ((rc = check_lora(u, lora_b, r))) return rc;
-  if (M <= K2Q_GEMV_MAX_M)
+  if (w4_takes_gemv(M, K))
     return k2q_launch_gemv_w4a8(qx, sx, qw4, sw4, bias, u, lora_b, (int)r, lora_scale, M, N, K, y, st);
   W4Args p{};
   p.a = qw4; p.s4 = sw4; p.b = qx; p.N = N; p.M = M; p.K = K;

@@ -135,6 +135,7 @@ struct Gemv4Args {
   int64_t N;
   int K;
   uint16_t* y;           // M x N bf16
+  int waves, teams;      // waves on one team's rows, teams per workgroup
 };
 
 // 32 weights of one row against 32 activation codes (x[0..7]: four codes a word, k ascending); 16 times the dot.
@@ -151,60 +152,117 @@ __device__ __forceinline__ int dot32_i4(const v4u& w, const v4i& x0, const v4i& 
   return d;
 }
 
-template <int MT>
-__global__ __launch_bounds__(64 * GV_WAVES) void gemv_w4_kernel(Gemv4Args p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n0 = ((int64_t)blockIdx.x * GV_WAVES + (threadIdx.x >> 6)) * GV_ROWS;
-  if (n0 >= p.N) return;   // N % 4 == 0: a wave's four rows are all there; no barriers
-  const int kb = p.K / 2;  // bytes per row
-  const uint8_t* w0 = p.qw + n0 * kb;
-  float acc[GV_ROWS][MT] = {};
+// v + its neighbour's v under a DPP permutation of 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
 
-  for (int b0 = 16 * lane; b0 < kb; b0 += 1024) {
-    v4u w[GV_ROWS];
+// Sums over the wave of NV values (NV even or 1): afterwards lane l holds in v[0..] the sums of the values that its
+// 32-lane half, then 16-lane row, took.  Each swap folds two values into one register (32 lanes apart, then 16), so a
+// value costs one add per stage for every two; the four stages inside a row are DPP adds.  The tree of one value is the
+// same for every NV.
+template <int NV>
+__device__ __forceinline__ void wave_sums(float (&v)[NV], float (&out)[(NV + 3) / 4]) {
+  constexpr int H = (NV + 1) / 2, Q = (H + 1) / 2;
+  float h[H];
 #pragma unroll
-    for (int i = 0; i < GV_ROWS; ++i)
-      w[i] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(w0 + (int64_t)i * kb + b0));
-    const int k = 2 * b0;
-    const v2u sv = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)(k >> 6) * p.N + n0);
-    const float sc[GV_ROWS] = {__uint_as_float(sv[0] << 16), __uint_as_float(sv[0] & 0xffff0000u),
-                               __uint_as_float(sv[1] << 16), __uint_as_float(sv[1] & 0xffff0000u)};
+  for (int i = 0; i < H; ++i) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(i + H < NV ? v[i + H] : v[i]),
+                                                    false, false);
+    h[i] = __uint_as_float(p[0]) + __uint_as_float(p[1]);      // lanes 0-31: value i, 32-63: value i + H
+  }
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[i]), __float_as_uint(i + Q < H ? h[i + Q] : h[i]),
+                                                    false, false);
+    float f = __uint_as_float(p[0]) + __uint_as_float(p[1]);   // odd 16-lane rows: h[i + Q]
+    f = dpp_add<0xB1>(f);      // quad_perm xor 1
+    f = dpp_add<0x4E>(f);      // quad_perm xor 2
+    f = dpp_add<0x141>(f);     // row_half_mirror
+    out[i] = dpp_add<0x140>(f);   // row_mirror
+  }
+}
+
+// A team of `waves` waves owns GV_ROWS rows; a wave takes every `waves`-th 2048-wide step of K (16 bytes a lane), at most
+// G4_STEPS of them, all loads issued before the first is used.  The team's sums meet in LDS.
+constexpr int G4_STEPS = 2;         // K <= 16384: four waves of two steps
+constexpr int G4_K = 2048;
+
+template <int MT>
+__global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
+  constexpr int NV = GV_ROWS * MT, NS = (NV + 3) / 4;
+  __shared__ float red[4][4 * NS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int team = wave / p.waves, part = wave % p.waves;
+  // workgroups of one XCD (dispatched round-robin over eight) take neighbouring rows: the 128-byte lines of the scales,
+  // 64 rows wide, are then read by one XCD's L2 instead of all eight
+  const uint32_t per = gridDim.x >> 3, rest = gridDim.x & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  const int64_t block = x * per + (x < rest ? x : rest) + i;
+  const int64_t n0 = (block * p.teams + team) * GV_ROWS;
+  const bool live = n0 < p.N;       // N % 4 == 0: a team's four rows are all there or none is
+  const int kb = p.K / 2;           // bytes per row
+  const uint8_t* w0 = p.qw + (live ? n0 : 0) * kb;
+  v4u w[G4_STEPS][GV_ROWS];
+  v2u sv[G4_STEPS];
+#pragma unroll
+  for (int s = 0; s < G4_STEPS; ++s) {
+    const int k = G4_K * (part + s * p.waves) + 32 * lane;
+    const bool ok = live && k < p.K;
+    sv[s] = v2u{0, 0};
+    if (ok) sv[s] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)(k >> 6) * p.N + n0);
+#pragma unroll
+    for (int r = 0; r < GV_ROWS; ++r) {
+      w[s][r] = v4u{0, 0, 0, 0};
+      if (ok) w[s][r] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(w0 + (int64_t)r * kb + (k >> 1)));
+    }
+  }
+  float acc[NV] = {};
+#pragma unroll
+  for (int s = 0; s < G4_STEPS; ++s) {
+    const int k = G4_K * (part + s * p.waves) + 32 * lane;
+    if (k >= p.K) break;
+    const float sc[GV_ROWS] = {__uint_as_float(sv[s][0] << 16), __uint_as_float(sv[s][0] & 0xffff0000u),
+                               __uint_as_float(sv[s][1] << 16), __uint_as_float(sv[s][1] & 0xffff0000u)};
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const v4i x0 = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k);
       const v4i x1 = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k + 16);
 #pragma unroll
-      for (int i = 0; i < GV_ROWS; ++i) acc[i][m] = __builtin_fmaf((float)dot32_i4(w[i], x0, x1), sc[i], acc[i][m]);
+      for (int r = 0; r < GV_ROWS; ++r)
+        acc[GV_ROWS * m + r] = __builtin_fmaf((float)dot32_i4(w[s][r], x0, x1), sc[r], acc[GV_ROWS * m + r]);
     }
   }
-
+  float sum[NS];
+  wave_sums<NV>(acc, sum);
+  if ((lane & 15) == 0) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1)
-#pragma unroll
-    for (int i = 0; i < GV_ROWS; ++i)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[i][m] += __shfl_xor(acc[i][m], off, 64);
-
-  // Lane i + GV_ROWS m writes y[m][n0 + i].
-  if (lane >= GV_ROWS * MT) return;
-  const int i = lane % GV_ROWS, m = lane / GV_ROWS;
-  const int64_t n = n0 + i;
+    for (int j = 0; j < NS; ++j) red[wave][(lane >> 4) * NS + j] = sum[j];
+  }
+  __syncthreads();
+  if (part || !live || lane >= NV) return;
+  // value `lane` = GV_ROWS m + r: row 2 (upper half of the values) + (second half of those) of red, in order
+  const int m = lane / GV_ROWS, r = lane % GV_ROWS;
+  constexpr int H = (NV + 1) / 2;
+  const int up = lane >= H, in = lane - up * H, odd = in >= NS;
+  const int at = (2 * up + odd) * NS + in - odd * NS;
   float a = 0.f;
-#pragma unroll
-  for (int ii = 0; ii < GV_ROWS; ++ii)
-#pragma unroll
-    for (int mm = 0; mm < MT; ++mm) a = (ii == i && mm == m) ? acc[ii][mm] : a;
+  for (int v = 0; v < p.waves; ++v) a += red[wave + v][at];
+  const int64_t n = n0 + r;
   float f = __builtin_fmaf(a, p.sx[m] * (0.0078125f * 0.0625f), p.bias ? p.bias[n] : 0.f);
   if (p.u) f += lora_dot(p.u + (int64_t)m * p.r, p.lora_b + n * p.r, p.r, p.lora_scale);
   p.y[(int64_t)m * p.N + n] = (uint16_t)f32_to_bf16_bits(f);
 }
 
 template <int MT>
-int launch4_mt(const Gemv4Args& p, hipStream_t st) {
-  const int64_t rows_per_wg = (int64_t)GV_ROWS * GV_WAVES;
+int launch4_mt(Gemv4Args p, hipStream_t st) {
+  const int steps = (p.K + G4_K - 1) / G4_K;
+  p.waves = steps < 4 ? steps : 4;
+  p.teams = 4 / p.waves;
+  const int64_t rows_per_wg = (int64_t)GV_ROWS * p.teams;
   const int64_t grid = (p.N + rows_per_wg - 1) / rows_per_wg;
   if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
-  hipLaunchKernelGGL(gemv_w4_kernel<MT>, dim3((unsigned)grid), dim3(64 * GV_WAVES), 0, st, p);
+  hipLaunchKernelGGL(gemv_w4_kernel<MT>, dim3((unsigned)grid), dim3(64 * p.waves * p.teams), 0, st, p);
   return k2q_launch_status();
 }
 
@@ -241,8 +299,8 @@ int k2q_launch_gemv_w8a8(const int8_t* qx, const float* sx, const int8_t* qw, co
 int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const uint16_t* sw4, const float* bias,
                          const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
                          int64_t K, uint16_t* y, hipStream_t st) {
-  if (K > 0x3fffffff) return K2Q_EUNSUPPORTED;
-  Gemv4Args p{qx, sx, qw4, sw4, bias, u, lora_b, u ? r : 0, lora_scale, N, (int)K, y};
+  if (K > 4 * G4_STEPS * G4_K) return K2Q_EUNSUPPORTED;
+  Gemv4Args p{qx, sx, qw4, sw4, bias, u, lora_b, u ? r : 0, lora_scale, N, (int)K, y, 1, 1};
   switch (M) {
     case 1: return launch4_mt<1>(p, st);
     case 2: return launch4_mt<2>(p, st);

@@ -19,12 +19,13 @@ constexpr int SK_T = 256;       // lanes per workgroup (four waves)
 constexpr int SK_CW = SK_T * 16;   // elements per chunk
 
 // Workgroups [0, ncode): row blockIdx.x's codes and scale (the row rotated in registers, one amax).
-// Workgroups [ncode, ncode + r): rank j = blockIdx.x - ncode: u[m, j] = x[m, :] . A[j, :] for the M rows, each
+// Workgroups [ncode, ..): rank j = (blockIdx.x - ncode) % r of the rows mper at a time: u[m, j] = x[m, :] . A[j, :], each
 // lane's 16 columns per chunk summed in column order, then the wave's lanes (shuffle tree), then the four
-// waves in order.  kNCH chunks of 4096 elements cover K.
+// waves in order.  kNCH chunks of 4096 elements cover K.  A workgroup's rows follow one another, a load latency each, so
+// few ranks take a workgroup per row (rereading A's row from L2: 16 ranks, 7 rows of 16384 9.7 -> 5.0 us).
 template <int kNCH>
 __global__ __launch_bounds__(SK_T) void skinny_prologue_kernel(const __bf16* __restrict__ x, int64_t ldx, int K,
-                                                               int M, const float* __restrict__ a, int r,
+                                                               int M, const float* __restrict__ a, int r, int mper,
                                                                float* __restrict__ u, int ncode,
                                                                int8_t* __restrict__ q, float* __restrict__ s) {
   __shared__ float red[2][4];
@@ -33,14 +34,15 @@ __global__ __launch_bounds__(SK_T) void skinny_prologue_kernel(const __bf16* __r
   const int off = lane_offset(t);
 
   if ((int)blockIdx.x >= ncode) {
-    const int j = (int)blockIdx.x - ncode;
+    const int j = ((int)blockIdx.x - ncode) % r, m0 = ((int)blockIdx.x - ncode) / r * mper;
+    const int m1 = m0 + mper < M ? m0 + mper : M;
     float w[kNCH][16];
 #pragma unroll
     for (int c = 0; c < kNCH; ++c) {
       const int col = c * SK_CW + off;
       load16<float>(a + (int64_t)j * K + col, col < K, w[c]);
     }
-    for (int m = 0; m < M; ++m) {
+    for (int m = m0; m < m1; ++m) {
       float v[kNCH][16];
 #pragma unroll
       for (int c = 0; c < kNCH; ++c) {
@@ -104,13 +106,16 @@ int launch_skinny(const uint16_t* x, int64_t ldx, int64_t M, int64_t K, const fl
   const __bf16* xp = reinterpret_cast<const __bf16*>(x);
   const int nch = (int)((K + SK_CW - 1) / SK_CW);
   const int ncode = q ? (int)M : 0;
-  const dim3 grid((unsigned)(ncode + (a ? r : 0)));
+  // row groups: about two workgroups a CU, one row each at most
+  const int64_t most = a ? 512 / r : 1, groups = most < 1 ? 1 : most < M ? most : M;
+  const int mper = (int)((M + groups - 1) / groups);
+  const dim3 grid((unsigned)(ncode + (a ? r * ((M + mper - 1) / mper) : 0)));
   if (grid.x == 0) return K2Q_OK;
   switch (nch) {
 #define K2Q_SK_CASE(NCH)                                                                                          \
   case NCH:                                                                                                      \
-    hipLaunchKernelGGL(skinny_prologue_kernel<NCH>, grid, dim3(SK_T), 0, st, xp, ldx, (int)K, (int)M, a, (int)r, u, \
-                       ncode, q, s);                                                                             \
+    hipLaunchKernelGGL(skinny_prologue_kernel<NCH>, grid, dim3(SK_T), 0, st, xp, ldx, (int)K, (int)M, a, (int)r,    \
+                       mper, u, ncode, q, s);                                                                             \
     break;
     K2Q_SK_CASE(1) K2Q_SK_CASE(2) K2Q_SK_CASE(3) K2Q_SK_CASE(4)
 #undef K2Q_SK_CASE
