@@ -278,8 +278,8 @@ int k2q_linear_fwd(const uint16_t* x, int64_t ldx, int64_t M, int64_t K, int8_t*
                    int64_t ws_bytes, void* stream);
 
 /* W4A8 variant: per-group int32 partials scaled by the bf16 group scales and added in f32 over the whole K.
- * M <= 8 runs a GEMV (no workspace, no tiles): half-group partials scaled and added in f32 in an order that depends
- * on K alone, so a row's result is the same whatever rows are beside it. */
+ * M <= 8 and K <= 16384 runs a GEMV (no workspace, no tiles): half-group or group partials scaled and added in f32 in
+ * an order that M, N and K fix. */
 int k2q_gemm_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const uint16_t* sw4,
                   const float* bias, const float* u, const float* lora_b, int64_t r, float lora_scale,
                   int64_t M, int64_t N, int64_t K, uint16_t* y, void* stream);

@@ -152,6 +152,26 @@ __device__ __forceinline__ int dot32_i4(const v4u& w, const v4i& x0, const v4i& 
   return d;
 }
 
+// Orders a wave's LDS writes before its lanes' reads of one another's.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The epilogue: a is 16 times the scaled sum of row n and token m.
+__device__ __forceinline__ void gemv4_store(const Gemv4Args& p, int m, int64_t n, float a) {
+  float f = __builtin_fmaf(a, p.sx[m] * (0.0078125f * 0.0625f), p.bias ? p.bias[n] : 0.f);
+  if (p.u) f += lora_dot(p.u + (int64_t)m * p.r, p.lora_b + n * p.r, p.r, p.lora_scale);
+  p.y[(int64_t)m * p.N + n] = (uint16_t)f32_to_bf16_bits(f);
+}
+
+// This workgroup's place when those of one XCD (dispatched round-robin over eight) take neighbouring rows: the 128-byte
+// lines of the scales, 64 rows wide, are then read by one XCD's L2 instead of all eight.
+__device__ __forceinline__ int64_t xcd_block() {
+  const uint32_t per = gridDim.x >> 3, rest = gridDim.x & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  return x * per + (x < rest ? x : rest) + i;
+}
+
 // v + its neighbour's v under a DPP permutation of 16 lanes.
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
@@ -184,53 +204,176 @@ __device__ __forceinline__ void wave_sums(float (&v)[NV], float (&out)[(NV + 3) 
   }
 }
 
-// A team of `waves` waves owns GV_ROWS rows; a wave takes every `waves`-th 2048-wide step of K (16 bytes a lane), at most
-// G4_STEPS of them, all loads issued before the first is used.  The team's sums meet in LDS.
-constexpr int G4_STEPS = 2;         // K <= 16384: four waves of two steps
+// The same product on the matrix cores: a workgroup owns 16 rows, its waves split K into 1024-wide segments (512 bytes
+// of a row, 16 scale groups).  One 16 x 16 x 64 MFMA is 16 weight rows against up to 16 token rows over one scale group:
+// lane (c = lane % 16, b = lane / 16) holds the 8 bytes of row c and the 16 codes of token c at k = 64 g + 16 b, and gets
+// the dots of row c with the token operand's rows 4 b .. 4 b + 3.  Loaded in that layout a row's bytes come 32 at a time (2.9 TB/s); so a
+// wave loads whole row segments, 16 bytes a lane, and turns them through its own piece of LDS: row c, 16-byte unit q at
+// unit q ^ 2 (c % 8), which spreads the eight rows of a read over all banks.  With at most 8 tokens half of a token
+// operand would be idle: its rows 8-15 hold the same tokens' codes of the next group, so one register serves two MFMAs,
+// whose results for tokens 0-7 are rows 0-7 (even groups) and rows 8-15 (odd groups).
+constexpr int GM_ROWS = 16;
+constexpr int GM_SEG = 1024;
+constexpr int GM_GROUPS = GM_SEG / 64;
+constexpr int GM_WAVES = 8;
+constexpr int GM_STEPS = 2;         // segments per wave: K <= 8 * 2 * 1024
+constexpr int GM_LDS = GM_ROWS * GM_SEG / 2 + GM_GROUPS * GM_ROWS * 2;   // a wave's piece: codes, then scales
+
+template <int STEPS>
+__global__ __launch_bounds__(64 * GM_WAVES) void gemv_w4_mfma_kernel(Gemv4Args p, int M) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, b = lane >> 4;
+  const int64_t n0 = xcd_block() * GM_ROWS;
+  const int kb = p.K >> 1;
+  // loads: lane's row 2 i + lane / 32 (clamped to the last), its 16 bytes at 16 (lane % 32) of the segment; its scales'
+  // group lane / 4 and four rows
+  const int64_t s0 = n0 + 4 * (lane & 3) < p.N ? n0 + 4 * (lane & 3) : p.N - 4;
+  const int tok = c & 7;
+  const int8_t* xp = p.qx + (int64_t)(tok < M ? tok : 0) * p.K + 64 * (c >> 3) + 16 * b;
+  v4u w[STEPS][GM_ROWS / 2];
+  v2u sc[STEPS];
+  v4i x[GM_GROUPS / 2];
+  auto load_x = [&](int k0) {      // K % 128 == 0: groups come in pairs
+#pragma unroll
+    for (int g = 0; g < GM_GROUPS / 2; ++g)
+      x[g] = *reinterpret_cast<const v4i*>(xp + (k0 + 128 * g < p.K ? k0 + 128 * g : 0));
+  };
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int k0 = GM_SEG * (wave + s * p.waves);
+    if (k0 >= p.K) break;
+    const int k = k0 + 32 * (lane & 31), g = (k0 >> 6) + (lane >> 2);
+#pragma unroll
+    for (int i = 0; i < GM_ROWS / 2; ++i) {
+      const int64_t row = n0 + 2 * i + (lane >> 5) < p.N ? n0 + 2 * i + (lane >> 5) : p.N - 1;
+      w[s][i] = v4u{0, 0, 0, 0};
+      if (k < p.K) w[s][i] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p.qw + row * kb + (k >> 1)));
+    }
+    sc[s] = v2u{0, 0};
+    if (64 * g < p.K) sc[s] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)g * p.N + s0);
+    if (s == 0) load_x(k0);
+  }
+  float acc[4] = {};
+  uint8_t* wt = lds + GM_LDS * wave;
+  uint16_t* st = reinterpret_cast<uint16_t*>(wt + GM_ROWS * GM_SEG / 2);
+  const int sw = 2 * (c & 7);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int k0 = GM_SEG * (wave + s * p.waves);
+    if (k0 >= p.K) break;
+    if (s) load_x(k0);
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < GM_ROWS / 2; ++i) {
+      const int r = 2 * i + (lane >> 5);
+      *reinterpret_cast<v4u*>(wt + r * (GM_SEG / 2) + 16 * ((lane & 31) ^ (2 * (r & 7)))) = w[s][i];
+    }
+    *reinterpret_cast<v2u*>(st + 4 * lane) = sc[s];
+    wave_fence();
+    // groups past K: codes and scales are zeros
+#pragma unroll
+    for (int g = 0; g < GM_GROUPS; g += 2) {
+      v4i d[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v2u q = *reinterpret_cast<const v2u*>(wt + c * (GM_SEG / 2) + 16 * ((2 * (g + h) + (b >> 1)) ^ sw) + 8 * (b & 1));
+        const v4i a = {(int)((q[0] << 4) & 0xf0f0f0f0u), (int)((q[1] << 4) & 0xf0f0f0f0u), (int)(q[0] & 0xf0f0f0f0u),
+                       (int)(q[1] & 0xf0f0f0f0u)};
+        d[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[g / 2], a, v4i{0, 0, 0, 0}, 0, 0, 0);
+      }
+      const float f = bf16_bits_to_f32(st[GM_ROWS * (g + (b >> 1)) + c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf((float)(b < 2 ? d[0][i] : d[1][i]), f, acc[i]);
+    }
+  }
+  wave_fence();
+  float* red = reinterpret_cast<float*>(wt);      // 8 tokens x 16 rows, over the wave's own codes
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], 32, 64);      // even groups' sum plus odd groups'
+  if (b < 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[GM_ROWS * (4 * b + i) + c] = acc[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < GM_ROWS * M; i += 64 * p.waves) {
+    const int m = i / GM_ROWS, r = i % GM_ROWS;
+    const int64_t n = n0 + r;
+    if (n >= p.N) continue;
+    float a = 0.f;
+    for (int v = 0; v < p.waves; ++v) a += reinterpret_cast<const float*>(lds + GM_LDS * v)[i];
+    gemv4_store(p, m, n, a);
+  }
+}
+
+template <int STEPS>
+int launch4_mfma(const Gemv4Args& p, int M, hipStream_t st) {
+  static std::atomic<uint64_t> lds_set{0};
+  const int rc = k2q_lds_limit_once(gemv_w4_mfma_kernel<STEPS>, GM_LDS * GM_WAVES, lds_set);
+  if (rc) return rc;
+  const int64_t grid = (p.N + GM_ROWS - 1) / GM_ROWS;
+  if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  hipLaunchKernelGGL(gemv_w4_mfma_kernel<STEPS>, dim3((unsigned)grid), dim3(64 * p.waves), GM_LDS * p.waves, st, p, M);
+  return k2q_launch_status();
+}
+
+int launch4_mfma(Gemv4Args p, int M, hipStream_t st) {
+  const int segs = (p.K + GM_SEG - 1) / GM_SEG;
+  p.waves = segs < GM_WAVES ? segs : GM_WAVES;
+  return segs <= GM_WAVES ? launch4_mfma<1>(p, M, st) : launch4_mfma<2>(p, M, st);
+}
+
+// A team of `waves` waves owns R rows; a wave takes every `waves`-th 2048-wide step of K (16 bytes a lane), STEPS of
+// them, all weight loads issued before the first is used.  The team's sums meet in LDS.
 constexpr int G4_K = 2048;
 
-template <int MT>
+template <int MT, int R, int STEPS>
 __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
-  constexpr int NV = GV_ROWS * MT, NS = (NV + 3) / 4;
+  constexpr int NV = R * MT, NS = (NV + 3) / 4, H = NV / 2;
   __shared__ float red[4][4 * NS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int team = wave / p.waves, part = wave % p.waves;
-  // workgroups of one XCD (dispatched round-robin over eight) take neighbouring rows: the 128-byte lines of the scales,
-  // 64 rows wide, are then read by one XCD's L2 instead of all eight
-  const uint32_t per = gridDim.x >> 3, rest = gridDim.x & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
-  const int64_t block = x * per + (x < rest ? x : rest) + i;
-  const int64_t n0 = (block * p.teams + team) * GV_ROWS;
-  const bool live = n0 < p.N;       // N % 4 == 0: a team's four rows are all there or none is
+  const int64_t n0 = (xcd_block() * p.teams + team) * R;
+  const bool live = n0 < p.N;
   const int kb = p.K / 2;           // bytes per row
-  const uint8_t* w0 = p.qw + (live ? n0 : 0) * kb;
-  v4u w[G4_STEPS][GV_ROWS];
-  v2u sv[G4_STEPS];
+  // N % 4 == 0: rows come in fours, the last team's second four may be missing (its loads repeat the first)
+  const int64_t base = live ? n0 : 0, half = R > 4 && n0 + 4 < p.N ? 4 : 0;
+  v4u w[STEPS][R];
+  v2u sv[STEPS][R / 4];
 #pragma unroll
-  for (int s = 0; s < G4_STEPS; ++s) {
+  for (int s = 0; s < STEPS; ++s) {
     const int k = G4_K * (part + s * p.waves) + 32 * lane;
     const bool ok = live && k < p.K;
-    sv[s] = v2u{0, 0};
-    if (ok) sv[s] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)(k >> 6) * p.N + n0);
 #pragma unroll
-    for (int r = 0; r < GV_ROWS; ++r) {
+    for (int r = 0; r < R; ++r) {
       w[s][r] = v4u{0, 0, 0, 0};
-      if (ok) w[s][r] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(w0 + (int64_t)r * kb + (k >> 1)));
+      const int64_t row = base + (r & 3) + (r >> 2) * half;
+      if (ok) w[s][r] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p.qw + row * kb + (k >> 1)));
+    }
+#pragma unroll
+    for (int q = 0; q < R / 4; ++q) {
+      sv[s][q] = v2u{0, 0};
+      if (ok) sv[s][q] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)(k >> 6) * p.N + base + q * half);
     }
   }
   float acc[NV] = {};
 #pragma unroll
-  for (int s = 0; s < G4_STEPS; ++s) {
+  for (int s = 0; s < STEPS; ++s) {
     const int k = G4_K * (part + s * p.waves) + 32 * lane;
     if (k >= p.K) break;
-    const float sc[GV_ROWS] = {__uint_as_float(sv[s][0] << 16), __uint_as_float(sv[s][0] & 0xffff0000u),
-                               __uint_as_float(sv[s][1] << 16), __uint_as_float(sv[s][1] & 0xffff0000u)};
+    v4i x[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const v4i x0 = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k);
-      const v4i x1 = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k + 16);
+      x[m][0] = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k);
+      x[m][1] = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k + 16);
+    }
 #pragma unroll
-      for (int r = 0; r < GV_ROWS; ++r)
-        acc[GV_ROWS * m + r] = __builtin_fmaf((float)dot32_i4(w[s][r], x0, x1), sc[r], acc[GV_ROWS * m + r]);
+    for (int r = 0; r < R; ++r) {
+      const uint32_t sw = sv[s][r >> 2][(r >> 1) & 1];
+      const float sc = __uint_as_float(r & 1 ? sw & 0xffff0000u : sw << 16);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        acc[R * m + r] = __builtin_fmaf((float)dot32_i4(w[s][r], x[m][0], x[m][1]), sc, acc[R * m + r]);
     }
   }
   float sum[NS];
@@ -241,29 +384,50 @@ __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
   }
   __syncthreads();
   if (part || !live || lane >= NV) return;
-  // value `lane` = GV_ROWS m + r: row 2 (upper half of the values) + (second half of those) of red, in order
-  const int m = lane / GV_ROWS, r = lane % GV_ROWS;
-  constexpr int H = (NV + 1) / 2;
+  // value `lane` = R m + r: row 2 (upper half of the values) + (second half of those) of red, in order
+  const int m = lane / R, r = lane % R;
   const int up = lane >= H, in = lane - up * H, odd = in >= NS;
   const int at = (2 * up + odd) * NS + in - odd * NS;
+  if (n0 + r >= p.N) return;
   float a = 0.f;
   for (int v = 0; v < p.waves; ++v) a += red[wave + v][at];
-  const int64_t n = n0 + r;
-  float f = __builtin_fmaf(a, p.sx[m] * (0.0078125f * 0.0625f), p.bias ? p.bias[n] : 0.f);
-  if (p.u) f += lora_dot(p.u + (int64_t)m * p.r, p.lora_b + n * p.r, p.r, p.lora_scale);
-  p.y[(int64_t)m * p.N + n] = (uint16_t)f32_to_bf16_bits(f);
+  gemv4_store(p, m, n0 + r, a);
 }
 
-template <int MT>
-int launch4_mt(Gemv4Args p, hipStream_t st) {
+template <int MT, int R, int STEPS>
+int launch4_mrs(const Gemv4Args& p, hipStream_t st) {
+  const int64_t rows_per_wg = (int64_t)R * p.teams;
+  const int64_t grid = (p.N + rows_per_wg - 1) / rows_per_wg;
+  if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  hipLaunchKernelGGL((gemv_w4_kernel<MT, R, STEPS>), dim3((unsigned)grid), dim3(64 * p.waves * p.teams), 0, st, p);
+  return k2q_launch_status();
+}
+
+template <int MT, int R>
+int launch4_mr(Gemv4Args p, hipStream_t st) {
   const int steps = (p.K + G4_K - 1) / G4_K;
   p.waves = steps < 4 ? steps : 4;
   p.teams = 4 / p.waves;
-  const int64_t rows_per_wg = (int64_t)GV_ROWS * p.teams;
-  const int64_t grid = (p.N + rows_per_wg - 1) / rows_per_wg;
-  if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
-  hipLaunchKernelGGL(gemv_w4_kernel<MT>, dim3((unsigned)grid), dim3(64 * p.waves * p.teams), 0, st, p);
-  return k2q_launch_status();
+  return steps <= 4 ? launch4_mrs<MT, R, 1>(p, st) : launch4_mrs<MT, R, 2>(p, st);
+}
+
+// Which kernel.  A 16-row workgroup a CU needs N >= 4096; below that teams of four rows fill more of the chip.  From
+// there on one or two tokens are bound by the weight stream and take eight rows a team (the activation codes are read
+// from L1 once for twice the rows), more tokens would be bound by those reads (64 bytes a clock: 3 us a token at 36864 x
+// 6144) and take the matrix cores, which read them into one register for 16 rows.  Kernel times, us, on codes that no
+// cache holds (teams of 4 / teams of 8 / matrix cores):
+//   N x K          M = 1                M = 2                M = 3                M = 8
+//   1536 x 6144    3.6 / 3.7 / 5.3      4.0 / 4.1 / 5.5      4.3 / 4.4 / 5.5      5.4 / 5.4 / 5.8
+//   6144 x 6144    6.2 / 6.2 / 7.5      6.9 / 7.4 / 7.6      7.6 / 7.6 / 7.8      11.2 / 11.1 / 8.7
+//   36864 x 6144   24.3 / 22.4 / 25.6   26.9 / 25.3 / 25.1   29.9 / 25.4 / 25.7   47.5 / 43.4 / 29.7
+//   6144 x 16384   13.6 / 12.3 / 14.0   15.1 / 13.3 / 14.2   16.5 / 14.6 / 14.4   24.8 / 20.8 / 17.4
+constexpr int64_t G4_WIDE = 4096;
+
+template <int MT>
+int launch4_mt(const Gemv4Args& p, hipStream_t st) {
+  if (p.N < G4_WIDE) return launch4_mr<MT, 4>(p, st);
+  if constexpr (MT <= 2) return launch4_mr<MT, 8>(p, st);
+  else return launch4_mfma(p, MT, st);
 }
 
 template <int MT>
@@ -299,7 +463,7 @@ int k2q_launch_gemv_w8a8(const int8_t* qx, const float* sx, const int8_t* qw, co
 int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, const uint16_t* sw4, const float* bias,
                          const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
                          int64_t K, uint16_t* y, hipStream_t st) {
-  if (K > 4 * G4_STEPS * G4_K) return K2Q_EUNSUPPORTED;
+  if (K > 4 * 2 * G4_K) return K2Q_EUNSUPPORTED;
   Gemv4Args p{qx, sx, qw4, sw4, bias, u, lora_b, u ? r : 0, lora_scale, N, (int)K, y, 1, 1};
   switch (M) {
     case 1: return launch4_mt<1>(p, st);

@@ -1,15 +1,17 @@
-"""GPU tests of the W4A8 forward for 1 to 8 rows (the matrix-vector path) against the product in float64.
+"""GPU tests of the W4A8 forward for 1 to 8 rows (the matrix-vector paths) against the product in float64.
 
-A lane adds K / 2048 (rounded up) products of an exact int32 dot with a scale, then six more sums join the lanes; with the
-epilogue's product and sums that is fewer than K / 2048 + 16 float32 roundings, each at most 2^-24 of the sum of the
-terms' magnitudes, and one rounding to bf16 (2^-8 of the value)."""
+Every float32 sum starts from exact int32 dots of half groups or groups.  A lane adds at most K / 512 products with a
+scale (the matrix cores' 32 groups of K = 16384; two half groups on the vector path), then at most ten more sums join lanes
+and waves; with the epilogue's product and sums that is fewer than K / 512 + 16 float32 roundings (and one a rank), each at
+most 2^-24 of the sum of the terms' magnitudes, and one rounding to bf16 (2^-8 of the value)."""
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
 EDGES = [(1, 4, 128), (1, 1536, 6144), (2, 132, 2048), (3, 36, 2176), (4, 260, 4096), (5, 512, 640), (6, 1028, 8192),
-         (7, 6144, 16384), (8, 18432, 1024), (8, 64, 16384), (2, 36864, 6144), (1, 2000, 256)]
+         (7, 6144, 16384), (8, 18432, 1024), (8, 64, 16384), (2, 36864, 6144), (1, 2000, 256), (1, 4100, 2048),
+         (2, 4108, 16384), (3, 4100, 128), (8, 4124, 8320), (5, 6148, 1152), (3, 4096, 8192), (1, 8196, 10240)]
 
 
 def _codes(q4):
@@ -60,10 +62,11 @@ def test_against_float64(k2, dev, M, N, K, r):
         ub, Bb = (u * 0.75).bfloat16().double(), B.bfloat16().double()     # the factors' bf16 rounding is the operator's
         ref, mag = ref + bias.double() + ub @ Bb.t(), mag + bias.double().abs() + ub.abs() @ Bb.abs().t()
     off = (y.double() - ref).abs()
-    assert (off <= 2 ** -8 * ref.abs() + (K / 2048 + 16 + r) * 2 ** -24 * mag).all()
-    # a row's bits depend neither on the other rows nor on the call
-    one = L.gemm_w4a8(qx[-1:].contiguous(), sx[-1:].clone(), q4, s4, bias, u[-1:].clone() if r else None, B, 0.75)
-    assert torch.equal(one, y[-1:]) and torch.equal(L.gemm_w4a8(qx, sx, q4, s4, bias, u, B, 0.75), y)
+    assert (off <= 2 ** -8 * ref.abs() + (K / 512 + 16 + r) * 2 ** -24 * mag).all()
+    # the same bits again, and for a row in another's place
+    assert torch.equal(L.gemm_w4a8(qx, sx, q4, s4, bias, u, B, 0.75), y)
+    p = torch.arange(M - 1, -1, -1, device=dev)
+    assert torch.equal(L.gemm_w4a8(qx[p], sx[p], q4, s4, bias, u[p] if r else None, B, 0.75), y[p])
 
 
 def test_rows_behind_the_output_stay(k2, dev):
