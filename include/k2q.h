@@ -102,14 +102,16 @@ int k2q_rmsmod_bwd(const uint16_t* dh, const uint16_t* x, int64_t M, int64_t K, 
  * nullable bf16 vectors, row m reading entry m / rows_per_batch of row stride ld_gate / ld_scale / ld_shift (0: one
  * entry).  scale_add: 1 for a norm whose weight is scale + 1 (mmdit.py:156-161), 0 for a plain weight.  K as for
  * k2q_rotquant.
- * k2q_resnorm_bwd is its autograd.  dh, dr (nullable): the gradients of h and of r's other readers; dn = bf16(dh * bf16(1 +
- * p)), g = dn (norm_scale + scale_add), i = rsqrt(mean_k r^2 + eps):
- *   dx = bf16(dr + bf16(g i - r (i^3 / K) sum_k g r)),  dy = bf16(gate * dx) (given exactly when gate is; else dy is dx).
+ * k2q_resnorm_bwd is its autograd.  dh, dr (nullable): the gradients of h and of r's other readers; dn = dh * bf16(1 + p),
+ * g = dn (norm_scale + scale_add), i = rsqrt(mean_k r^2 + eps):
+ *   dR = dr + (g i - r (i^3 / K) sum_k g r),  dx = bf16(dR),  dy = bf16(gate * dR) (given exactly when gate is; else dy is
+ *   dx), in f32; eager != 0: dn, the norm's share of dR, and dR before the gate are rounded to bf16, as the eager ops and
+ *   k2q_rmsmod_bwd round them.
  * The sums over the rows of a batch entry are written where their pointer is given (dscale, dshift, dgate: entries x K
  * bf16, dnorm: K f32, over all rows); they need y (dgate), M a multiple of rows_per_batch, and ws of
  * k2q_resnorm_bwd_ws_bytes bytes, 16-byte aligned:
- *   dscale = sum dh n,  dshift = sum dh,  dgate = sum dx y,  dnorm = sum dh bf16(1 + p) r i,
- * in f32 in a fixed order.  All M x K operands but y contiguous. */
+ *   dscale = sum dh n,  dshift = sum dh,  dgate = sum dR y,  dnorm = sum dh bf16(1 + p) r i,
+ * in f32 in a fixed order, whatever eager is.  All M x K operands but y contiguous. */
 int k2q_resnorm_rotquant(const uint16_t* x, int64_t ldx, const uint16_t* y, int64_t ldy, const uint16_t* gate,
                          int64_t ld_gate, int64_t M, int64_t K, const float* norm_scale, float scale_add, float eps,
                          const uint16_t* mod_scale, int64_t ld_scale, const uint16_t* mod_shift, int64_t ld_shift,
@@ -117,7 +119,7 @@ int k2q_resnorm_rotquant(const uint16_t* x, int64_t ldx, const uint16_t* y, int6
 int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch);
 int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
                     const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale, int64_t ld_scale,
-                    const uint16_t* gate, int64_t ld_gate, int64_t rows_per_batch, uint16_t* dx, uint16_t* dy,
+                    const uint16_t* gate, int64_t ld_gate, int64_t rows_per_batch, int eager, uint16_t* dx, uint16_t* dy,
                     const uint16_t* y, int64_t ldy, float* dnorm, uint16_t* dscale, uint16_t* dshift, uint16_t* dgate,
                     void* ws, int64_t ws_bytes, void* stream);
 

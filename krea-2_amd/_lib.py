@@ -79,8 +79,8 @@ _SIGNATURES = {
     "k2q_resnorm_rotquant": ([_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _p,
                               _p, _p, _p, _p], _int),
     "k2q_resnorm_bwd_ws_bytes": ([_i64, _i64, _i64], _i64),
-    "k2q_resnorm_bwd": ([_p, _p, _p, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p,
-                         _p, _p, _p, _i64, _p], _int),
+    "k2q_resnorm_bwd": ([_p, _p, _p, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _int, _p, _p, _p, _i64, _p,
+                         _p, _p, _p, _p, _i64, _p], _int),
     "k2q_rotary": ([_p, _i64, _int, _i64, _i64, _i64, _i64, _int, _p, _int, _i64, _i64, _i64, _p, _p, _f32, _int, _p],
                    _int),
     "k2q_lora_down_ws_bytes": ([_i64, _i64, _i64], _i64),
@@ -480,31 +480,44 @@ def resnorm_rotquant(x, y, gate, w, add: float, eps: float, scale, shift, rows_p
                     lambda: _check_resnorm(x, y, gate, w, scale, shift, rows_per_entry))
 
 
+def resnorm_native(x, y, gate, w, add: float, eps: float, scale, shift):
+    """:func:`resnorm_rotquant` on contiguous ``x`` and ``y`` of any shape (.., K) and vectors of one entry or one per first
+    dimension of ``x``, (B, 1, .., K): ``(r, h)`` in that shape, ``(q, s)`` by rows.  None for what it does not take."""
+    out = _fast().resnorm(x, y, gate, w, add, eps, scale, shift, 0)
+    if out.__class__ is int:
+        _check(out, "k2q_resnorm_rotquant")
+    return out
+
+
 def _check_resnorm_bwd(dh, dr, r, w, ms, gate, rows_per_entry, y, need_mod) -> None:
-    _need(r, "r", torch.bfloat16, 2)
-    _check_norm_rows(r, "r", w, rows_per_entry)
+    _need(r, "r", torch.bfloat16)
+    flat = r.reshape(-1, r.shape[-1])
+    _check_norm_rows(flat, "r", w, rows_per_entry)
     for t, name in ((dh, "dh"), (dr, "dr")):
         if t is not None or name == "dh":
-            _need(t, name, torch.bfloat16, 2, r.device)
+            _need(t, name, torch.bfloat16, None, r.device)
             if t.shape != r.shape:
                 raise ValueError(f"{name} and r differ in shape")
     for t, name in ((gate, "gate"), (ms, "scale")):
-        _check_entries(t, name, r.shape[1], r.shape[0] // rows_per_entry, r.device)
+        if t is not None and t.numel() % flat.shape[1] == 0:
+            t = t.reshape(-1, flat.shape[1])
+        _check_entries(t, name, flat.shape[1], flat.shape[0] // rows_per_entry, r.device)
     if y is not None:
-        _need_rows(y, "y", r.device)
         if y.shape != r.shape or gate is None:
             raise ValueError("the gate's gradient needs the gate and y of r's shape")
+        _need_rows(y if y.dim() == 2 else y.reshape(flat.shape), "y", r.device)
     if need_mod and ms is None:
         raise ValueError("no modulation to differentiate")
     _device_check(r.device)
 
 
 def resnorm_bwd(dh, dr, r, w, add: float, eps: float, scale, gate, rows_per_entry: int, y=None, need_w=False,
-                need_scale=False, need_shift=False):
-    """Autograd of :func:`resnorm_rotquant` (``k2q_resnorm_bwd``): ``(dx, dy, dw, dscale, dshift, dgate)`` from the
-    gradients of ``h`` and (or None) of ``r``.  ``dy`` is None without a gate (it is ``dx``); ``dgate`` comes when ``y``
-    is given, the other sums where asked for, one row per entry."""
-    args = (dh, dr, r, w, add, eps, scale, gate, rows_per_entry, y, need_w, need_scale, need_shift)
+                need_scale=False, need_shift=False, eager=False):
+    """Autograd of :func:`resnorm_rotquant` and :func:`resnorm_native` (``k2q_resnorm_bwd``): ``(dx, dy, dw, dscale, dshift,
+    dgate)`` from the gradients of ``h`` and (or None) of ``r``, contiguous in r's shape.  ``dy`` is None without a gate
+    (it is ``dx``); ``dgate`` comes when ``y`` is given, the other sums where asked for, in the shape of ``gate`` /
+    ``scale``, or (entries, K) where those are one entry among more.  ``eager``: rounded where eager bf16 operations round."""
+    args = (dh, dr, r, w, add, eps, scale, gate, rows_per_entry, y, need_w, need_scale, need_shift, eager)
     out = _fast().resnorm_bwd(*args)
     if out.__class__ is tuple:
         return out

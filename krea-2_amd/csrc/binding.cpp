@@ -413,42 +413,73 @@ bool rows_ok(const Tensor* t, int64_t M, int64_t K, c10::Device d) {
          t->stride(1) == 1 && t->stride(0) >= K && t->stride(0) % 8 == 0 && aligned(*t);
 }
 
-// Per-entry bf16 vectors (1, K) or (entries, K), or null; ld is their row stride (0: one entry).
-bool entries_ok(const Tensor* t, int64_t entries, int64_t K, c10::Device d, int64_t& ld) {
+// Per-entry bf16 vectors of x's rows, or null: K values (one entry), or one row of K per entry, (n, K) or (n, 1, .., K);
+// n is their number, ld the row stride (0: one entry).
+bool vectors_ok(const Tensor* t, int64_t K, c10::Device d, int64_t& n, int64_t& ld) {
+  n = 1;
   ld = 0;
   if (!t) return true;
-  if (t->scalar_type() != at::kBFloat16 || t->dim() != 2 || t->size(1) != K || t->device() != d || t->stride(1) != 1 ||
-      !aligned(*t) || (t->size(0) != 1 && t->size(0) != entries))
+  const int64_t dim = t->dim();
+  if (t->scalar_type() != at::kBFloat16 || dim < 1 || t->size(dim - 1) != K || t->device() != d || t->stride(dim - 1) != 1 ||
+      !aligned(*t))
     return false;
-  if (t->size(0) > 1) ld = t->stride(0);
-  return ld >= 0 && ld % 8 == 0;
+  n = t->numel() / K;
+  if (n == 1) return true;
+  for (int64_t i = 1; i < dim - 1; ++i)
+    if (t->size(i) != 1) return false;
+  ld = t->stride(0);
+  return t->size(0) == n && ld >= 0 && ld % 8 == 0;
 }
 
-// resnorm(x, y, gate | None, w, add, eps, scale | None, shift | None, rows_per_entry) -> (r, h, q, s)
+// Whether n_i entries each (1, or all the same number of them) go with M rows, `rows` each; rows == 0: one per first
+// dimension of x (`lead` of them).
+bool entries_fit(std::initializer_list<int64_t> ns, int64_t M, int64_t lead, int64_t& rows) {
+  int64_t most = 1;
+  for (int64_t n : ns) most = n > most ? n : most;
+  if (!rows) {
+    if (most > 1 && most != lead) return false;
+    rows = M / most;
+  }
+  if (rows < 1 || M % rows) return false;
+  for (int64_t n : ns)
+    if (n != 1 && n != M / rows) return false;
+  return true;
+}
+
+// resnorm(x, y, gate | None, w, add, eps, scale | None, shift | None, rows_per_entry | 0) -> (r, h, q, s): x, y (M, K) rows,
+// or contiguous (.., K); r, h in x's shape
 PyObject* py_resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(9)
   return guarded([&]() -> PyObject* {
     const Tensor *x = tensor_of(a[0], bad), *y = tensor_of(a[1], bad), *gate = tensor_of(a[2], bad),
                  *w = tensor_of(a[3], bad), *ms = tensor_of(a[6], bad), *mb = tensor_of(a[7], bad);
     const double add = PyFloat_AsDouble(a[4]), eps = PyFloat_AsDouble(a[5]);
-    const int64_t rpb = PyLong_AsLongLong(a[8]);
+    int64_t rows = PyLong_AsLongLong(a[8]);
     if (PyErr_Occurred()) return nullptr;
-    if (bad || !x || !y || x->dim() != 2) K2Q_REFUSE;
-    const int64_t M = x->size(0), K = x->size(1);
+    if (bad || !x || !y || x->dim() < 2 || rows < 0) K2Q_REFUSE;
+    const int64_t K = x->size(x->dim() - 1);
+    if (!width_ok(K) || x->numel() == 0) K2Q_REFUSE;
+    const int64_t M = x->numel() / K;
     const c10::Device d = x->device();
-    int64_t lg, ls, lb;
-    if (!ready(d) || M < 1 || rpb < 1 || M % rpb || !width_ok(K) || !rows_ok(x, M, K, d) || !rows_ok(y, M, K, d) ||
-        !operand(w, at::kFloat, 1, d) || w->size(0) != K || !entries_ok(gate, M / rpb, K, d, lg) ||
-        !entries_ok(ms, M / rpb, K, d, ls) || !entries_ok(mb, M / rpb, K, d, lb) || !ms != !mb)
+    const bool flat = x->dim() == 2;
+    auto in = [&](const Tensor& t) {
+      return flat ? rows_ok(&t, M, K, d)
+                  : t.scalar_type() == at::kBFloat16 && t.device() == d && t.is_contiguous() && aligned(t) &&
+                        t.sizes() == x->sizes();
+    };
+    int64_t ng, ns, nb, lg, ls, lb;
+    if (!ready(d) || !in(*x) || !in(*y) || !operand(w, at::kFloat, 1, d) || w->size(0) != K ||
+        !vectors_ok(gate, K, d, ng, lg) || !vectors_ok(ms, K, d, ns, ls) || !vectors_ok(mb, K, d, nb, lb) || !ms != !mb ||
+        !entries_fit({ng, ns, nb}, M, x->size(0), rows))
       K2Q_REFUSE;
     const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
-    Tensor r = alloc({M, K}, at::kBFloat16, d), h = alloc({M, K}, at::kBFloat16, d), q = alloc({M, K}, at::kChar, d),
+    Tensor r = alloc(x->sizes(), at::kBFloat16, d), h = alloc(x->sizes(), at::kBFloat16, d), q = alloc({M, K}, at::kChar, d),
            s = alloc({M}, at::kFloat, d);
-    const int rc = foreign(api.resnorm_rotquant, as<uint16_t>(ptr(x)), x->stride(0), as<uint16_t>(ptr(y)), y->stride(0),
-                           as<uint16_t>(ptr(gate)), lg, M, K, as<float>(ptr(w)), (float)add, (float)eps,
-                           as<uint16_t>(ptr(ms)), ls, as<uint16_t>(ptr(mb)), lb, rpb, as<uint16_t>(ptr(r)),
+    const int rc = foreign(api.resnorm_rotquant, as<uint16_t>(ptr(x)), flat ? x->stride(0) : K, as<uint16_t>(ptr(y)),
+                           flat ? y->stride(0) : K, as<uint16_t>(ptr(gate)), lg, M, K, as<float>(ptr(w)), (float)add,
+                           (float)eps, as<uint16_t>(ptr(ms)), ls, as<uint16_t>(ptr(mb)), lb, rows, as<uint16_t>(ptr(r)),
                            as<uint16_t>(ptr(h)), as<int8_t>(ptr(q)), as<float>(ptr(s)), st);
     if (rc) return PyLong_FromLong(rc);
     return pack({r, h, q, s});
@@ -456,40 +487,52 @@ PyObject* py_resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // resnorm_bwd(dh, dr | None, r, w, add, eps, scale | None, gate | None, rows_per_entry, y | None, need_w, need_scale,
-//             need_shift) -> (dx, dy | None, dw | None, dscale | None, dshift | None, dgate | None)
+//             need_shift, eager) -> (dx, dy | None, dw | None, dscale | None, dshift | None, dgate | None): dh, dr, r
+// contiguous (.., K); dx, dy in their shape, the vectors' gradients in the vectors' (dshift in scale's), (entries, K) for
+// one entry among more
 PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  K2Q_ARGS(13)
+  K2Q_ARGS(14)
   return guarded([&]() -> PyObject* {
     const Tensor *dh = tensor_of(a[0], bad), *dr = tensor_of(a[1], bad), *r = tensor_of(a[2], bad),
                  *w = tensor_of(a[3], bad), *ms = tensor_of(a[6], bad), *gate = tensor_of(a[7], bad),
                  *y = tensor_of(a[9], bad);
     const double add = PyFloat_AsDouble(a[4]), eps = PyFloat_AsDouble(a[5]);
-    const int64_t rpb = PyLong_AsLongLong(a[8]);
-    const int need_w = PyObject_IsTrue(a[10]), need_scale = PyObject_IsTrue(a[11]), need_shift = PyObject_IsTrue(a[12]);
+    int64_t rows = PyLong_AsLongLong(a[8]);
+    const int need_w = PyObject_IsTrue(a[10]), need_scale = PyObject_IsTrue(a[11]), need_shift = PyObject_IsTrue(a[12]),
+              eager = PyObject_IsTrue(a[13]);
     if (PyErr_Occurred()) return nullptr;
-    if (bad || !dh || !r || r->dim() != 2) K2Q_REFUSE;
-    const int64_t M = r->size(0), K = r->size(1);
+    if (bad || !dh || !r || r->dim() < 2 || rows < 1) K2Q_REFUSE;
+    const int64_t K = r->size(r->dim() - 1);
+    if (!width_ok(K) || r->numel() == 0) K2Q_REFUSE;
+    const int64_t M = r->numel() / K;
     const c10::Device d = r->device();
-    auto whole = [&](const Tensor* t) { return operand(t, at::kBFloat16, 2, d) && t->size(0) == M && t->size(1) == K; };
-    int64_t lg, ls;
-    if (!ready(d) || M < 1 || rpb < 1 || M % rpb || !width_ok(K) || !whole(dh) || !whole(r) || (dr && !whole(dr)) ||
-        !operand(w, at::kFloat, 1, d) || w->size(0) != K || !entries_ok(gate, M / rpb, K, d, lg) ||
-        !entries_ok(ms, M / rpb, K, d, ls) || (y && (!gate || !rows_ok(y, M, K, d))) ||
+    auto whole = [&](const Tensor* t) {
+      return t && t->scalar_type() == at::kBFloat16 && t->device() == d && t->is_contiguous() && aligned(*t) &&
+             t->sizes() == r->sizes();
+    };
+    auto in = [&](const Tensor* t) { return r->dim() == 2 ? rows_ok(t, M, K, d) : whole(t); };
+    int64_t ng, ns, lg, ls;
+    if (!ready(d) || !whole(dh) || !whole(r) || (dr && !whole(dr)) ||
+        !operand(w, at::kFloat, 1, d) || w->size(0) != K || !vectors_ok(gate, K, d, ng, lg) ||
+        !vectors_ok(ms, K, d, ns, ls) || !entries_fit({ng, ns}, M, 0, rows) || (y && (!gate || !in(y))) ||
         ((need_scale || need_shift) && !ms))
       K2Q_REFUSE;
     const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
-    const int64_t E = M / rpb;
-    Tensor dx = alloc({M, K}, at::kBFloat16, d), dy = gate ? alloc({M, K}, at::kBFloat16, d) : Tensor();
-    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = need_scale ? alloc({E, K}, at::kBFloat16, d) : Tensor(),
-           db = need_shift ? alloc({E, K}, at::kBFloat16, d) : Tensor(), dg = y ? alloc({E, K}, at::kBFloat16, d) : Tensor();
-    const int64_t nws = need_w || need_scale || need_shift || y ? api.resnorm_bwd_ws_bytes(M, K, rpb) : 0;
+    const int64_t E = M / rows;
+    auto vec = [&](bool need, const Tensor* t, int64_t n) {
+      return !need ? Tensor() : n == E ? alloc(t->sizes(), at::kBFloat16, d) : alloc({E, K}, at::kBFloat16, d);
+    };
+    Tensor dx = alloc(r->sizes(), at::kBFloat16, d), dy = gate ? alloc(r->sizes(), at::kBFloat16, d) : Tensor();
+    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = vec(need_scale, ms, ns), db = vec(need_shift, ms, ns),
+           dg = vec(y, gate, ng);
+    const int64_t nws = need_w || need_scale || need_shift || y ? api.resnorm_bwd_ws_bytes(M, K, rows) : 0;
     Tensor ws = workspace(nws, d);
     const int rc = foreign(api.resnorm_bwd, as<uint16_t>(ptr(dh)), as<uint16_t>(ptr(dr)), as<uint16_t>(ptr(r)), M, K,
                            as<float>(ptr(w)), (float)add, (float)eps, as<uint16_t>(ptr(ms)), ls, as<uint16_t>(ptr(gate)),
-                           lg, rpb, as<uint16_t>(ptr(dx)), as<uint16_t>(ptr(dy)), as<uint16_t>(ptr(y)),
-                           y ? y->stride(0) : 0, as<float>(ptr(dw)), as<uint16_t>(ptr(ds)), as<uint16_t>(ptr(db)),
+                           lg, rows, eager, as<uint16_t>(ptr(dx)), as<uint16_t>(ptr(dy)), as<uint16_t>(ptr(y)),
+                           y ? r->dim() == 2 ? y->stride(0) : K : 0, as<float>(ptr(dw)), as<uint16_t>(ptr(ds)), as<uint16_t>(ptr(db)),
                            as<uint16_t>(ptr(dg)), ptr(ws), nws, st);
     if (rc) return PyLong_FromLong(rc);
     return pack({dx, dy, dw, ds, db, dg});

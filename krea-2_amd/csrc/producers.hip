@@ -322,15 +322,16 @@ struct NormBwdArgs {
   const uint16_t* gate;      // B x K bf16 or null
   int64_t ldg;
   uint16_t* dy;              // gradient of y, written where there is a gate (without one it is dx)
-  float* rinv;               // M row statistics for the column sums, or null
+  int eager;                 // round where the eager ops and k2q_rmsmod_bwd do
+  float* stats;              // M pairs (rsqrt, the subtracted term's factor c) for the column sums, or null
 };
 
 // Input gradient of the modulated RMSNorm (the autograd of the forward's eager ops for x alone):
 //   dn = bf16(dh * bf16(1 + p)),  g = dn * (w + 1),  r = rsqrt(mean x^2 + eps),
 //   dx = bf16(g r - x (r^3 / K) sum_k(g x)).
-// With a residual (kRes) x is the new stream, whose other readers' gradient joins it as autograd would add it, and the
-// gate scales it on the way to y:
-//   dR = bf16(dr + dx),  dy = bf16(gate * dR).
+// With a residual (kRes) x is the new stream, whose other readers' gradient joins it, and the gate scales it on the way to
+// y, all in f32 with one rounding of each result; eager: dn and dx above rounded as they are there, the sum before the gate:
+//   dR = dr + dx,  dx = bf16(dR),  dy = bf16(gate * dR).
 // A team of 64 * WPR lanes owns a row; lane t handles the 8-element chunks at 8 t + 8 T c, c < kNCH, held
 // packed (bf16 pairs) between the two row reductions.
 template <bool kRes, int WPR, int kNCH>
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
     for (int w = 0; w < WPR; ++w) ss += sred[0][w0 + w];
   }
   const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
-  if (kRes && a.rinv && t == 0 && row_ok) a.rinv[row] = r;
+  const bool steps = !kRes || a.eager;
 
   // g = bf16(dh * p1) * (w + 1), kept in f32 (8 per chunk) for the final pass
   float gv[kNCH][8];
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
       float p0 = 1.f + __uint_as_float(pw[j] << 16), p1 = 1.f + __uint_as_float(pw[j] & 0xffff0000u);
       bf16r2(p0, p1);
       float n0 = __uint_as_float(dw[j] << 16) * p0, n1 = __uint_as_float(dw[j] & 0xffff0000u) * p1;
-      bf16r2(n0, n1);
+      if (steps) bf16r2(n0, n1);
       const float g0 = n0 * (w[2 * j] + a.nwadd), g1 = n1 * (w[2 * j + 1] + a.nwadd);
       gv[c][2 * j] = g0;
       gv[c][2 * j + 1] = g1;
@@ -414,6 +415,7 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
   }
   if (!row_ok) return;
   const float c3 = __fdiv_rn(r * r * r * dot, (float)K);
+  if (kRes && a.stats && t == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(r, c3);
   const uint16_t* mg = kRes && a.gate ? a.gate + (row / a.rpb) * a.ldg : nullptr;
 #pragma unroll
   for (int c = 0; c < kNCH; ++c) {
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
       const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        bf16r2(d[2 * j], d[2 * j + 1]);
+        if (steps) bf16r2(d[2 * j], d[2 * j + 1]);
         d[2 * j] = __uint_as_float(rw[j] << 16) + d[2 * j];
         d[2 * j + 1] = __uint_as_float(rw[j] & 0xffff0000u) + d[2 * j + 1];
       }
@@ -445,9 +447,10 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
       const uint32_t gw[4] = {gg.x, gg.y, gg.z, gg.w};
       uint32_t e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        e[j] = pack_bf16x2(__uint_as_float(gw[j] << 16) * __uint_as_float(o[j] << 16),
-                           __uint_as_float(gw[j] & 0xffff0000u) * __uint_as_float(o[j] & 0xffff0000u));
+      for (int j = 0; j < 4; ++j) {
+        if (steps) bf16r2(d[2 * j], d[2 * j + 1]);
+        e[j] = pack_bf16x2(__uint_as_float(gw[j] << 16) * d[2 * j], __uint_as_float(gw[j] & 0xffff0000u) * d[2 * j + 1]);
+      }
       *reinterpret_cast<uint4*>(a.dy + row * K + col) = make_uint4(e[0], e[1], e[2], e[3]);
     }
   }
@@ -477,14 +480,14 @@ void launch_norm_bwd(const NormBwdArgs& a, hipStream_t st) {
 
 // Column sums of the residual norm's backward: the gradients of what is broadcast over the rows of a batch entry,
 //   dscale = sum_m dh n,  dshift = sum_m dh,  dgate = sum_m dR y,  and over every row  dw = sum_m dn x r,
-// with n and dn as in the forward and backward (dn unrounded in f32: dw is an f32 gradient).  Rows are cut into strips
-// of one batch entry each; a workgroup sums one strip of 512 columns (lane: 8 columns, its four waves: every fourth
-// row) into f32 partials, and a second launch adds the strips in order: no atomics, the same result every time.
+// with n as in the forward and dn, dR unrounded in f32 (from the row statistics that the pass above left).  Rows are cut
+// into strips of one batch entry each; a workgroup sums one strip of 512 columns (lane: 8 columns, its four waves: every
+// fourth row) into f32 partials, and a second launch adds the strips in order: no atomics, the same result every time.
 constexpr int CS_COLS = 512;
 
 struct ColSumArgs {
-  const uint16_t *dh, *x, *y, *dx;   // M x K bf16 (y: row stride ldy; null: no gate)
-  const float* rinv;                 // M
+  const uint16_t *dh, *dr, *x, *y;   // M x K bf16 (dr: null for none; y: row stride ldy, null: no gate)
+  const float* stats;                // M pairs
   int64_t M, ldy, rpb;
   int K, strips, strip_rows;         // strips per batch entry, rows per strip
   const float* nw;
@@ -495,6 +498,11 @@ struct ColSumArgs {
 };
 
 enum { CS_W = 0, CS_SCALE = 1, CS_SHIFT = 2, CS_GATE = 3 };
+
+__device__ __forceinline__ float bf16_of(const uint4& v, int i) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
+}
 
 __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
   __shared__ float red[3][64][33];
@@ -512,30 +520,22 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
     w[i] = a.nw[cc + i] + a.nwadd;
     p1[i] = a.mscale ? bf16r(1.f + bf16_bits_to_f32(a.mscale[entry * a.ldm + cc + i])) : 1.f;
   }
+  const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int64_t m = m0 + wave; m < m1; m += 4) {
-    const float r = a.rinv[m];
+    const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * m);
     const uint4 dv = *reinterpret_cast<const uint4*>(a.dh + m * K + cc);
     const uint4 xv = *reinterpret_cast<const uint4*>(a.x + m * K + cc);
-    const uint32_t dw[4] = {dv.x, dv.y, dv.z, dv.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+    const uint4 yv = a.y ? *reinterpret_cast<const uint4*>(a.y + m * a.ldy + cc) : zero;
+    const uint4 rv = a.y && a.dr ? *reinterpret_cast<const uint4*>(a.dr + m * K + cc) : zero;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float d = i & 1 ? __uint_as_float(dw[i >> 1] & 0xffff0000u) : __uint_as_float(dw[i >> 1] << 16);
-      const float x = i & 1 ? __uint_as_float(xw[i >> 1] & 0xffff0000u) : __uint_as_float(xw[i >> 1] << 16);
-      const float xr = x * r;
-      acc[CS_W][i] = __builtin_fmaf(d * p1[i], xr, acc[CS_W][i]);
+      const float d = bf16_of(dv, i), x = bf16_of(xv, i);
+      const float dn = d * p1[i], xr = x * st.x;
+      acc[CS_W][i] = __builtin_fmaf(dn, xr, acc[CS_W][i]);
       acc[CS_SCALE][i] = __builtin_fmaf(d, bf16r(xr * w[i]), acc[CS_SCALE][i]);
       acc[CS_SHIFT][i] += d;
-    }
-    if (a.y) {
-      const uint4 yv = *reinterpret_cast<const uint4*>(a.y + m * a.ldy + cc);
-      const uint4 ev = *reinterpret_cast<const uint4*>(a.dx + m * K + cc);
-      const uint32_t yw[4] = {yv.x, yv.y, yv.z, yv.w}, ew[4] = {ev.x, ev.y, ev.z, ev.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = i & 1 ? __uint_as_float(yw[i >> 1] & 0xffff0000u) : __uint_as_float(yw[i >> 1] << 16);
-        const float e = i & 1 ? __uint_as_float(ew[i >> 1] & 0xffff0000u) : __uint_as_float(ew[i >> 1] << 16);
-        acc[CS_GATE][i] = __builtin_fmaf(e, y, acc[CS_GATE][i]);
-      }
+      const float dR = bf16_of(rv, i) + (dn * w[i] * st.x - x * st.y);
+      acc[CS_GATE][i] = __builtin_fmaf(dR, bf16_of(yv, i), acc[CS_GATE][i]);
     }
   }
   if (wave)
@@ -551,25 +551,39 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
       out[(int64_t)k * K + i] = ((acc[k][i] + red[0][lane][8 * k + i]) + red[1][lane][8 * k + i]) + red[2][lane][8 * k + i];
 }
 
-// One thread a column: the strips' partials in order.  Grid y: the batch entries (scale, shift and gate gradients,
-// bf16), then one more for the norm weight's (f32, over every entry).
+// The strips' partials joined: 64 columns a workgroup, its four waves every fourth strip, then the four in order.  Grid y:
+// the batch entries (scale, shift and gate gradients, bf16), then one more for the norm weight's (f32, every entry).
 __global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* part, int K, int entries, int strips,
                                                                   float* dnw, uint16_t* dscale, uint16_t* dshift,
                                                                   uint16_t* dgate) {
-  const int col = blockIdx.x * 256 + threadIdx.x;
-  if (col >= K) return;
+  __shared__ float red[3][4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + lane;
   const int entry = blockIdx.y;
-  if (entry == entries) {
-    if (!dnw) return;
-    float f = 0.f;
-    for (int64_t i = 0; i < (int64_t)entries * strips; ++i) f += part[(i * 4 + CS_W) * K + col];
-    dnw[col] = f;
+  const bool all = entry == entries;
+  const int64_t i0 = all ? 0 : (int64_t)entry * strips, i1 = all ? (int64_t)entries * strips : i0 + strips;
+  float f[3] = {};
+  if (col < K) {
+    if (all) {
+#pragma unroll 4
+      for (int64_t i = i0 + wave; i < i1; i += 4) f[0] += part[(i * 4 + CS_W) * K + col];
+    } else {
+#pragma unroll 2
+      for (int64_t i = i0 + wave; i < i1; i += 4)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) f[k] += part[(i * 4 + CS_SCALE + k) * K + col];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) red[k][wave][lane] = f[k];
+  __syncthreads();
+  if (wave || col >= K) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) f[k] = ((red[k][0][lane] + red[k][1][lane]) + red[k][2][lane]) + red[k][3][lane];
+  if (all) {
+    if (dnw) dnw[col] = f[0];
     return;
   }
-  float f[3] = {};
-  for (int64_t i = (int64_t)entry * strips; i < (int64_t)(entry + 1) * strips; ++i)
-#pragma unroll
-    for (int k = 0; k < 3; ++k) f[k] += part[(i * 4 + CS_SCALE + k) * K + col];
   const int64_t o = (int64_t)entry * K + col;
   if (dscale) dscale[o] = (uint16_t)f32_to_bf16_bits(f[0]);
   if (dshift) dshift[o] = (uint16_t)f32_to_bf16_bits(f[1]);
@@ -723,13 +737,13 @@ extern "C" int k2q_swiglu_bwd(const uint16_t* dh, const uint16_t* gate, const ui
 extern "C" int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch) {
   if (M < 1 || K < 8 || K % 8 || K > 16384 || rows_per_batch < 1 || M % rows_per_batch) return 0;
   const int64_t entries = M / rows_per_batch;
-  return (M + entries * colsum_strips(rows_per_batch, K, entries, k2q_cu_count()) * 4 * K) * 4;
+  return (2 * M + entries * colsum_strips(rows_per_batch, K, entries, k2q_cu_count()) * 4 * K) * 4;
 }
 
 extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
                                const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale,
                                int64_t ld_scale, const uint16_t* gate, int64_t ld_gate, int64_t rows_per_batch,
-                               uint16_t* dx, uint16_t* dy, const uint16_t* y, int64_t ldy, float* dnorm,
+                               int eager, uint16_t* dx, uint16_t* dy, const uint16_t* y, int64_t ldy, float* dnorm,
                                uint16_t* dscale, uint16_t* dshift, uint16_t* dgate, void* ws, int64_t ws_bytes,
                                void* stream) {
   if (M < 1 || K < 8 || K % 8) return K2Q_EINVAL;
@@ -762,7 +776,8 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   a.gate = gate;
   a.ldg = ld_gate;
   a.dy = dy;
-  a.rinv = cols ? static_cast<float*>(ws) : nullptr;
+  a.eager = eager;
+  a.stats = cols ? static_cast<float*>(ws) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
   launch_norm_bwd<true>(a, st);
   if (!cols) return k2q_launch_status();
@@ -770,8 +785,8 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   c.dh = dh;
   c.x = r;
   c.y = dgate ? y : nullptr;
-  c.dx = dx;
-  c.rinv = a.rinv;
+  c.dr = dr;
+  c.stats = a.stats;
   c.M = M;
   c.ldy = ldy;
   c.rpb = rows_per_batch;
@@ -782,10 +797,10 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   c.nwadd = scale_add;
   c.mscale = mod_scale;
   c.ldm = ld_scale;
-  c.part = a.rinv + M;
+  c.part = a.stats + 2 * M;
   const dim3 grid((unsigned)((K + CS_COLS - 1) / CS_COLS), (unsigned)(entries * c.strips));
   hipLaunchKernelGGL(resnorm_colsum_kernel, grid, dim3(256), 0, st, c);
-  hipLaunchKernelGGL(resnorm_colsum_join_kernel, dim3((unsigned)((K + 255) / 256), (unsigned)entries + 1), dim3(256), 0,
-                     st, c.part, (int)K, (int)entries, c.strips, dnorm, dscale, dshift, dgate);
+  hipLaunchKernelGGL(resnorm_colsum_join_kernel, dim3((unsigned)((K + 63) / 64), (unsigned)entries + 1), dim3(256), 0, st,
+                     c.part, (int)K, (int)entries, c.strips, dnorm, dscale, dshift, dgate);
   return k2q_launch_status();
 }

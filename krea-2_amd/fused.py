@@ -112,29 +112,44 @@ class _RmsModQuantFn(torch.autograd.Function):
 class _ResNormQuantFn(torch.autograd.Function):
     """Forward: the residual's addition and the (modulated) RMSNorm of ``mmdit.py:317-318`` with the codes of its output,
     one gfx950 pass.  Backward ``k2q_resnorm_bwd``: the gradients of the stream and of what was added in one pass, and the
-    sums over the rows for the gate, the modulation and the norm's scale where they are asked for."""
+    sums over the rows for the gate, the modulation and the norm's scale where they are asked for.  Tensors come in the
+    caller's shapes: every view outside would be an autograd node (nine of them cost a training pass 80 us of the host)."""
 
     @staticmethod
-    def forward(ctx, x2, y2, gate, w, scale, shift, add, eps, rows):
-        r, h, q, s = _lib.resnorm_rotquant(x2, y2, gate, w, add, eps, scale, shift, rows)
-        ctx.add, ctx.eps, ctx.rows = add, eps, rows
-        ctx.save_for_backward(r, w, scale, gate, y2 if gate is not None and ctx.needs_input_grad[2] else None)
+    def forward(ctx, x, y, gate, w, scale, shift, add, eps, eager):
+        shape, ctx.shapes = x.shape, [None if t is None else t.shape for t in (scale, shift, gate)]
+        out = _lib.resnorm_native(x, y, gate, w, add, eps, scale, shift)
+        if out is None:
+            x, y, gate, scale, shift, rows = _residual_rows(x, y, gate, w, scale, shift)
+            out = _lib.resnorm_rotquant(x, y, gate, w, add, eps, scale, shift, rows)
+        r, h, q, s = out
+        ctx.add, ctx.eps, ctx.eager = add, eps, eager
+        ctx.rows = r.numel() // max([t.numel() for t in (gate, scale, shift) if t is not None], default=r.shape[-1])
+        ctx.save_for_backward(r, w, scale, gate, y if gate is not None and ctx.needs_input_grad[2] else None)
         ctx.mark_non_differentiable(q, s)
         ctx.set_materialize_grads(False)
-        return r, h, q, s
+        return (r, h, q, s) if r.shape == shape else (r.view(shape), h.view(shape), q, s)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dr, dh, _dq, _ds):
         if dr is None and dh is None:
             return (None,) * 9
-        r, w, scale, gate, y2 = ctx.saved_tensors
-        nx, ny, ng, nw, ns, nb = ctx.needs_input_grad[:6]
-        dx, dy, dw, dscale, dshift, dgate = _lib.resnorm_bwd(
-            _dense_grad(dh, r), None if dr is None else _dense_grad(dr, r), r, w, ctx.add, ctx.eps, scale, gate,
-            ctx.rows, y2, nw, ns, nb)
+        shape = (dh if dr is None else dr).shape
+        r, w, scale, gate, y = ctx.saved_tensors
+        nx, ny, _, nw, ns, nb = ctx.needs_input_grad[:6]
+        dh, dr = _dense_grad(dh, r), None if dr is None else _dense_grad(dr, r)
+        if r.shape != shape:        # the forward ran on rows
+            dh, dr = dh.view(r.shape), None if dr is None else dr.view(r.shape)
+        dx, dy, dw, *sums = _lib.resnorm_bwd(dh, dr, r, w, ctx.add, ctx.eps, scale, gate, ctx.rows, y, nw, ns, nb, ctx.eager)
+        if r.shape != shape:
+            dx, dy = dx.view(shape), None if dy is None else dy.view(shape)
         if gate is None:
             dy = dx
+        dscale, dshift, dgate = (
+            t if t is None or t.shape == shape          # one entry for every batch row: the sum of the rows' sums
+            else (t if t.numel() == shape.numel() else t.reshape(-1, t.shape[-1]).sum(0)).reshape(shape)
+            for t, shape in zip(sums, ctx.shapes))
         return dx if nx else None, dy if ny else None, dgate, dw, dscale, dshift, None, None, None
 
 
@@ -207,6 +222,24 @@ def _norm_weight(norm: nn.Module, train: bool):
     raise ValueError(f"{type(norm).__name__} has neither a scale nor a weight")
 
 
+def _residual_rows(x, y, gate, w, scale, shift):
+    """``(x, y, gate, scale, shift, rows of an entry)`` as rows for the kernel, after the checks that name what is wrong."""
+    K = x.shape[-1]
+    if any(t.dtype != torch.bfloat16 for t in (x, y, gate, scale, shift) if t is not None):
+        raise NotImplementedError("the fused residual RMSNorm runs bf16 tensors (the DiT dtype)")
+    if x.shape != y.shape:
+        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} differ in shape")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift come together")
+    if w.shape != (K,):
+        raise ValueError(f"the norm's weight {tuple(w.shape)} does not match {K} features")
+    vectors = [None if t is None else _entry_rows(t, name, x)
+               for t, name in ((gate, "gate"), (scale, "scale"), (shift, "shift"))]
+    _lib._check_k(K)
+    x, y = _rows(x, K), _rows(y, K)
+    return x, y, *vectors, x.shape[0] // max([t.shape[0] for t in vectors if t is not None], default=1)
+
+
 def residual_rmsnorm(norm: nn.Module, x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None = None,
                      scale: torch.Tensor | None = None, shift: torch.Tensor | None = None):
     """``r = x + gate * y`` and ``h``, the norm of r (``mmdit.py:317-318``), in one pass with the int8 codes of ``h``, which
@@ -216,44 +249,35 @@ def residual_rmsnorm(norm: nn.Module, x: torch.Tensor, y: torch.Tensor, gate: to
     ``weight``; ``h`` is modulated, ``(1 + scale) * norm(r) + shift``, where ``scale`` and ``shift`` are given.  ``x`` and
     ``y`` (B, L, K) or (M, K) bf16; ``gate``, ``scale``, ``shift`` bf16, one entry or one per batch row of ``x`` ((B, 1,
     K)).  Every tensor of the formula is rounded to bf16 where the eager bf16 operations round it, so ``r`` and ``h`` equal
-    theirs (and ``h`` that of :func:`modulated_rmsnorm` on ``r``) bit for bit; the mean square and every gradient's sum
-    over rows are float32.
+    theirs (and ``h`` that of :func:`modulated_rmsnorm` on ``r``) bit for bit; the mean square is float32.
 
-    Differentiable (once) in ``x``, ``y``, ``gate``, ``scale``, ``shift`` and the norm's parameter; the gradients of the
-    last four are sums over rows, added in a fixed order."""
-    given = [t for t in (x, y, gate, scale, shift) if t is not None]
-    if any(t.dtype != torch.bfloat16 for t in given):
-        raise NotImplementedError("the fused residual RMSNorm runs bf16 tensors (the DiT dtype)")
-    if x.shape != y.shape:
-        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} differ in shape")
-    if (scale is None) != (shift is None):
-        raise ValueError("scale and shift come together")
-    K = x.shape[-1]
+    Differentiable (once) in ``x``, ``y``, ``gate``, ``scale``, ``shift`` and the norm's parameter.  The backward is float32
+    with one rounding of each gradient; the last four are sums over rows, added in a fixed order."""
+    return _residual_rmsnorm(norm, x, y, gate, scale, shift, False)
+
+
+def _residual_rmsnorm(norm, x, y, gate, scale, shift, eager):
+    """``eager``: the backward rounds where the eager operations and :func:`modulated_rmsnorm` do, so that a block's
+    gradients are theirs bit for bit."""
     grad = torch.is_grad_enabled()
     w, add = _norm_weight(norm, grad)
-    if w.shape != (K,):
-        raise ValueError(f"the norm's weight {tuple(w.shape)} does not match {K} features")
-    g2, s2, b2 = (None if t is None else _entry_rows(t, name, x)
-                  for t, name in ((gate, "gate"), (scale, "scale"), (shift, "shift")))
-    _lib._check_k(K)
-    if x.numel() == 0:
-        _lib._device_check(x.device)
-        r = x + y if gate is None else x + gate.reshape(gate.shape[0] if g2.shape[0] > 1 else 1,
-                                                        *(1,) * (x.dim() - 2), K) * y
-        return r, torch.zeros_like(r)
-    x2, y2 = _rows(x, K), _rows(y, K)
-    M = x2.shape[0]
-    entries = max([t.shape[0] for t in (g2, s2, b2) if t is not None], default=1)
-    rows = M // entries
     eps = float(norm.eps)
-    if _lib.observed() or (grad and any(t.requires_grad for t in (w, *given))):
-        if entries > 1:     # one gradient row per entry: autograd sums those of a vector given once
-            g2, s2, b2 = (t if t is None or t.shape[0] == entries else t.expand(entries, K) for t in (g2, s2, b2))
-        r, h, q, s = _ResNormQuantFn.apply(x2, y2, g2, w, s2, b2, add, eps, rows)
+    if x.numel() == 0:
+        _residual_rows(x, y, gate, w, scale, shift)
+        _lib._device_check(x.device)
+        r = x + y if gate is None else x + gate.reshape(-1, *(1,) * (x.dim() - 2), x.shape[-1]) * y
+        return r, torch.zeros_like(r)
+    if grad and (x.requires_grad or y.requires_grad or w.requires_grad
+                 or any(t is not None and t.requires_grad for t in (gate, scale, shift))) or _lib.observed():
+        r, h, q, s = _ResNormQuantFn.apply(x, y, gate, w, scale, shift, add, eps, eager)
     else:                   # nothing to differentiate: no autograd node
-        r, h, q, s = _lib.resnorm_rotquant(x2, y2, g2, w, add, eps, s2, b2, rows)
-    if x.dim() != 2:
-        r, h = r.reshape(x.shape), h.reshape(x.shape)
+        out = _lib.resnorm_native(x, y, gate, w, add, eps, scale, shift)
+        if out is None:
+            x2, y2, gate, scale, shift, rows = _residual_rows(x, y, gate, w, scale, shift)
+            r, h, q, s = _lib.resnorm_rotquant(x2, y2, gate, w, add, eps, scale, shift, rows)
+            r, h = r.view(x.shape), h.view(x.shape)
+        else:
+            r, h, q, s = out
     shared_input_quant.seed(h, q, s)
     return r, h
 
@@ -264,8 +288,12 @@ def input_codes(h: torch.Tensor):
     kept for the next layer)."""
     if h.dtype != torch.bfloat16:
         raise NotImplementedError("the codes are those of a bf16 tensor (the DiT dtype)")
-    with torch.no_grad():
-        return shared_input_quant.lookup(h, _aligned(h.reshape(-1, h.shape[-1])))
+    key, codes = shared_input_quant.find(h)
+    if codes is None:
+        with torch.no_grad():
+            codes = _lib.rotquant(_aligned(h.reshape(-1, h.shape[-1])))[:2]
+        shared_input_quant.keep(h, key, *codes)
+    return codes
 
 
 # ----------------------------------------------------------------------------------------------------------
@@ -299,7 +327,7 @@ def _fused_block_forward(self, x, vec, freqs, mask=None):
     prescale, preshift, pregate, postscale, postshift, postgate = self.mod(vec)
     a = self.attn(modulated_rmsnorm(self.prenorm, x, prescale, preshift), freqs, mask)
     if _takes_residual(x, a, pregate):
-        x, h = residual_rmsnorm(self.postnorm, x, a, pregate, postscale, postshift)
+        x, h = _residual_rmsnorm(self.postnorm, x, a, pregate, postscale, postshift, True)
     else:
         x = x + pregate * a
         h = modulated_rmsnorm(self.postnorm, x, postscale, postshift)

@@ -50,7 +50,7 @@ def test_entry_points_refuse_bad_arguments(k2):
     assert norm(K=16512, ldx=16512) == -4 and norm(M=1 << 31) == -4
 
     def bwd(dh=p, r=p, M=4, K=256, ms=p, gate=p, rows=2, dx=p, dy=p, y=p, dw=p, ds=p, dg=p, ws=p, nws=1 << 30):
-        return lib.k2q_resnorm_bwd(dh, None, r, M, K, p, 1.0, 1e-5, ms, 0, gate, 0, rows, dx, dy, y, 256, dw, ds, None, dg,
+        return lib.k2q_resnorm_bwd(dh, None, r, M, K, p, 1.0, 1e-5, ms, 0, gate, 0, rows, 0, dx, dy, y, 256, dw, ds, None, dg,
                                    ws, nws, None)
 
     for bad in ({"dh": None}, {"r": odd}, {"M": 0}, {"K": 100}, {"ms": None}, {"gate": None}, {"dy": None}, {"rows": 3},
