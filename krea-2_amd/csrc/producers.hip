@@ -12,6 +12,7 @@
 //       t = bf16(gate * y)  (t = y without a gate),  r = bf16(x + t),
 //     and the norm above of r, modulated or not.  r is written too: it is the residual stream.  The roundings are those
 //     of the eager bf16 ops, so r, h and the codes equal those of the separate ops and of the norm on r bit for bit.
+//     9 bytes an element: 2 x 4608 x 6144 in 110 us (4.6 TB/s; a copy of 4 GB runs at 4.9).
 // All write h (bf16, the tensor the next linear receives: its LoRA down-projection and the saved input of
 // the backward read it) and the int8 codes + scales of rotate/quant applied to h, computed from the same
 // registers, so the codes equal those of a separate rotate/quant call on h bit for bit.
@@ -43,12 +44,34 @@ struct ProdArgs {
   int64_t M;
   int K;
   uint16_t* r;               // residual norm: M x K bf16, the new residual stream
+  bool stream;               // residual norm: r and h are stored past the caches
   uint16_t* h;               // M x K bf16 (row stride K)
   int8_t* q;                 // M x K int8 codes of h R
   float* s;                  // M per-row scales
 };
 
 __device__ __forceinline__ float bf16r(float f) { return bf16_bits_to_f32(f32_to_bf16_bits(f)); }
+
+// 16 bf16 values, past the caches where `stream`.
+__device__ __forceinline__ void put16_bf16(uint16_t* p, const float (&v)[16], bool stream) {
+  if (!stream) {
+    store16_bf16(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v4u h;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = pack_bf16x2(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+    __builtin_nontemporal_store(h, reinterpret_cast<v4u*>(p) + i);
+  }
+}
+
+// Element i of eight bf16 values.
+__device__ __forceinline__ float bf16_of(const uint4& v, int i) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
+}
 
 // Two values rounded to bf16 by one v_cvt_pk_bf16_f32 (round to nearest even), unpacked in place.
 __device__ __forceinline__ void bf16r2(float& a, float& b) {
@@ -119,12 +142,21 @@ __global__ __launch_bounds__(256) void prodquant_kernel(ProdArgs a) {
     const int64_t b = rr / a.rpb;
     if (PROD == PROD_RESNORM) {
       const uint16_t* mg = a.gate ? a.gate + b * a.ldg : nullptr;
+      uint4 yv[kNCH][2];      // loaded whole: a load behind a store of r would wait for its turn
+#pragma unroll
+      for (int c = 0; c < kNCH; ++c) {
+        const int col = c * CW + off;
+        const uint4* yp = reinterpret_cast<const uint4*>(a.x1 + rr * a.ld1 + (!kTail || col < K ? col : 0));
+        yv[c][0] = yp[0];
+        yv[c][1] = yp[1];
+      }
 #pragma unroll
       for (int c = 0; c < kNCH; ++c) {
         const int col = c * CW + off;
         const bool ok = !kTail || col < K;
         float y[16];
-        load16<__bf16>(a.x1 + rr * a.ld1 + (ok ? col : 0), true, y);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = bf16_of(yv[c][i >> 3], i & 7);
         if (mg) {
           float g[16];
           load16<__bf16>(reinterpret_cast<const __bf16*>(mg) + (ok ? col : 0), true, g);
@@ -142,7 +174,7 @@ __global__ __launch_bounds__(256) void prodquant_kernel(ProdArgs a) {
           v[c][i] = ok ? r0 : 0.f;
           v[c][i + 1] = ok ? r1 : 0.f;
         }
-        if (row_ok && ok) store16_bf16(a.r + row * (int64_t)K + col, v[c]);
+        if (row_ok && ok) put16_bf16(a.r + row * (int64_t)K + col, v[c], a.stream);
       }
     }
     float ss = 0.f;
@@ -208,7 +240,10 @@ __global__ __launch_bounds__(256) void prodquant_kernel(ProdArgs a) {
 #pragma unroll
     for (int c = 0; c < kNCH; ++c) {
       const int col = c * CW + off;
-      if (col < K) store16_bf16(a.h + row * (int64_t)K + col, v[c]);
+      if (col < K) {
+        if (PROD == PROD_RESNORM) put16_bf16(a.h + row * (int64_t)K + col, v[c], a.stream);
+        else store16_bf16(a.h + row * (int64_t)K + col, v[c]);
+      }
     }
   }
 
@@ -322,7 +357,6 @@ struct NormBwdArgs {
   const uint16_t* gate;      // B x K bf16 or null
   int64_t ldg;
   uint16_t* dy;              // gradient of y, written where there is a gate (without one it is dx)
-  int eager;                 // round where the eager ops and k2q_rmsmod_bwd do
   float* stats;              // M pairs (rsqrt, the subtracted term's factor c) for the column sums, or null
 };
 
@@ -333,9 +367,14 @@ struct NormBwdArgs {
 // y, all in f32 with one rounding of each result; eager: dn and dx above rounded as they are there, the sum before the gate:
 //   dR = dr + dx,  dx = bf16(dR),  dy = bf16(gate * dR).
 // A team of 64 * WPR lanes owns a row; lane t handles the 8-element chunks at 8 t + 8 T c, c < kNCH, held
-// packed (bf16 pairs) between the two row reductions.
-template <bool kRes, int WPR, int kNCH>
+// packed (bf16 pairs) between the two row reductions.  Bound by its reads and writes.  The form that rounds once keeps
+// dr in registers from the start and spreads a row over more lanes (fewer registers each, more rows in flight): 4608 x
+// 6144 with a gate 62.5 -> 54.8 us, 5.2 TB/s; the other two keep the order of the row sums that their results have.
+enum { BWD_NORM = 0, BWD_EAGER = 1, BWD_ONCE = 2 };    // without a residual; with it, rounded as the eager ops; once
+
+template <int MODE, int WPR, int kNCH>
 __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
+  constexpr bool kRes = MODE != BWD_NORM, steps = MODE != BWD_ONCE;
   constexpr int T = 64 * WPR;
   constexpr int ROWS = 4 / WPR;
   __shared__ float sred[2][4];
@@ -349,7 +388,7 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
   const bool mod = !kRes || a.mscale;
   const uint16_t* ms = mod ? a.mscale + (rr / a.rpb) * a.ldm : nullptr;
 
-  uint4 xv[kNCH], dv[kNCH];
+  uint4 xv[kNCH], dv[kNCH], rv[kNCH];
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < kNCH; ++c) {
@@ -357,6 +396,7 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
     const bool ok = col < K;
     xv[c] = ok ? *reinterpret_cast<const uint4*>(a.x + rr * K + col) : make_uint4(0, 0, 0, 0);
     dv[c] = ok ? *reinterpret_cast<const uint4*>(a.dh + rr * K + col) : make_uint4(0, 0, 0, 0);
+    if (MODE == BWD_ONCE) rv[c] = ok && a.dr ? *reinterpret_cast<const uint4*>(a.dr + rr * K + col) : make_uint4(0, 0, 0, 0);
     const uint32_t w[4] = {xv[c].x, xv[c].y, xv[c].z, xv[c].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -375,8 +415,6 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
     for (int w = 0; w < WPR; ++w) ss += sred[0][w0 + w];
   }
   const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
-  const bool steps = !kRes || a.eager;
-
   // g = bf16(dh * p1) * (w + 1), kept in f32 (8 per chunk) for the final pass
   float gv[kNCH][8];
   float dot = 0.f;
@@ -429,8 +467,8 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
       d[2 * j + 1] = gv[c][2 * j + 1] * r - __uint_as_float(xw[j] & 0xffff0000u) * c3;
     }
     if (kRes && a.dr) {
-      const uint4 rv = *reinterpret_cast<const uint4*>(a.dr + row * K + col);
-      const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+      const uint4 rc = MODE == BWD_ONCE ? rv[c] : *reinterpret_cast<const uint4*>(a.dr + row * K + col);
+      const uint32_t rw[4] = {rc.x, rc.y, rc.z, rc.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (steps) bf16r2(d[2 * j], d[2 * j + 1]);
@@ -456,26 +494,27 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
   }
 }
 
-template <bool kRes, int WPR>
+template <int MODE, int WPR>
 void launch_rmsmod_bwd(const NormBwdArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((a.M + (4 / WPR) - 1) / (4 / WPR)));
   const int nch = (a.K + 512 * WPR - 1) / (512 * WPR);
 #define K2Q_RMB(N)                                                                             \
   case N:                                                                                      \
-    hipLaunchKernelGGL((rmsmod_bwd_kernel<kRes, WPR, N>), grid, dim3(256), 0, st, a);          \
+    hipLaunchKernelGGL((rmsmod_bwd_kernel<MODE, WPR, N>), grid, dim3(256), 0, st, a);          \
     break;
   switch (nch) {
     K2Q_RMB(1) K2Q_RMB(2) K2Q_RMB(3) K2Q_RMB(4) K2Q_RMB(5) K2Q_RMB(6) K2Q_RMB(7)
-    default: hipLaunchKernelGGL((rmsmod_bwd_kernel<kRes, WPR, 8>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((rmsmod_bwd_kernel<MODE, WPR, 8>), grid, dim3(256), 0, st, a); break;
   }
 #undef K2Q_RMB
 }
 
-template <bool kRes>
+template <int MODE>
 void launch_norm_bwd(const NormBwdArgs& a, hipStream_t st) {
-  if (a.K <= 4096) launch_rmsmod_bwd<kRes, 1>(a, st);
-  else if (a.K <= 8192) launch_rmsmod_bwd<kRes, 2>(a, st);
-  else launch_rmsmod_bwd<kRes, 4>(a, st);
+  constexpr int NARROW = MODE == BWD_ONCE ? 1024 : 4096;
+  if (a.K <= NARROW) launch_rmsmod_bwd<MODE, 1>(a, st);
+  else if (a.K <= 2 * NARROW) launch_rmsmod_bwd<MODE, 2>(a, st);
+  else launch_rmsmod_bwd<MODE, 4>(a, st);
 }
 
 // Column sums of the residual norm's backward: the gradients of what is broadcast over the rows of a batch entry,
@@ -498,11 +537,6 @@ struct ColSumArgs {
 };
 
 enum { CS_W = 0, CS_SCALE = 1, CS_SHIFT = 2, CS_GATE = 3 };
-
-__device__ __forceinline__ float bf16_of(const uint4& v, int i) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
-}
 
 __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
   __shared__ float red[3][64][33];
@@ -623,7 +657,7 @@ extern "C" int k2q_rmsmod_bwd(const uint16_t* dh, const uint16_t* x, int64_t M, 
   a.ldm = ld_mod;
   a.rpb = rows_per_batch;
   a.dx = dx;
-  launch_norm_bwd<false>(a, static_cast<hipStream_t>(stream));
+  launch_norm_bwd<BWD_NORM>(a, static_cast<hipStream_t>(stream));
   return k2q_launch_status();
 }
 
@@ -712,6 +746,9 @@ extern "C" int k2q_resnorm_rotquant(const uint16_t* x, int64_t ldx, const uint16
   a.M = M;
   a.K = (int)K;
   a.r = r;
+  // r and h of a pass that does not fit the 256 MB last-level cache leave it to the reads (same box, us, cached / streamed:
+  // 4608 x 6144, 255 MB, 59.3 / 61.4; 4608 x 8192 84.6 / 79.5; 9216 x 6144 118.1 / 112.8; 2304 x 16384 87.1 / 81.9)
+  a.stream = M * K * 9 > (int64_t)256 << 20;
   a.h = h;
   a.q = q;
   a.s = s;
@@ -776,10 +813,10 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   a.gate = gate;
   a.ldg = ld_gate;
   a.dy = dy;
-  a.eager = eager;
   a.stats = cols ? static_cast<float*>(ws) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  launch_norm_bwd<true>(a, st);
+  if (eager) launch_norm_bwd<BWD_EAGER>(a, st);
+  else launch_norm_bwd<BWD_ONCE>(a, st);
   if (!cols) return k2q_launch_status();
   ColSumArgs c{};
   c.dh = dh;
