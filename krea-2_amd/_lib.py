@@ -556,15 +556,21 @@ def _check_rotary(q, k, positions, turns, axis, axes: int, heads_first: bool) ->
     _device_check(dev)
 
 
+def rotary_native(*args):
+    """:func:`rotary` where the native wrapper takes the arguments as they are, else None."""
+    r = _fast().rotary(*args)
+    if r.__class__ is int:
+        _check(r, "k2q_rotary")
+    return r
+
+
 def rotary(q, k, positions, turns, axis, axes: int, half: bool, factor: float, inverse: bool, heads_first: bool):
     """Rotary positions (``k2q_rotary``): ``(q', k')`` with the strides of ``q`` and ``k`` (k may be None).  ``q``, ``k``
     (B,L,H,D), or (B,H,L,D) heads first; ``positions`` (L,) or (B,L), with ``axis`` a dimension of ``axes`` more behind;
     ``turns`` f64 revolutions per position of every pair, ``axis`` int32 their axis (below ``axes``) or None."""
     args = (q, k, positions, turns, axis, axes, half, factor, inverse, heads_first)
-    r = _fast().rotary(*args)
-    if r.__class__ is tuple:
-        return r
-    return _refused(r, "k2q_rotary", lambda: _native.rotary(*args),
+    r = rotary_native(*args)
+    return r if r is not None else _refused(r, "k2q_rotary", lambda: _native.rotary(*args),
                     lambda: _check_rotary(q, k, positions, turns, axis, axes, heads_first))
 
 
@@ -888,6 +894,17 @@ def linear_fwd(x2, qx, sx, codes_ready: bool, A, B, lora_scale: float, qw, sw, b
     return _refused(r, "k2q_linear_fwd", lambda: _native.linear_fwd(x2, qx, sx, codes_ready, A, B, lora_scale, qw, sw,
                                                                     bias, w4, need_u),
                     lambda: _check_linear_fwd(x2, qx, sx, A, B, qw, bias))
+
+
+def linear_infer(x, codes, A, B, lora_scale: float, qw, scale_bits, bias, w4: bool):
+    """:func:`linear_fwd` where nothing is differentiated, on contiguous ``x`` (.., K) as it is: ``(y (.., N), q_x, s_x)``, the
+    codes given (``codes``) or made.  ``scale_bits``: the layer's scales in the integers that hold them.  None for what it
+    does not take."""
+    qx, sx = codes or (None, None)
+    out = _fast().linear_infer(x, qx, sx, A, B, lora_scale, qw, scale_bits, bias, w4)
+    if out.__class__ is int:
+        _check(out, "k2q_linear_fwd")
+    return out
 
 
 def _check_linear_fwd(x2, qx, sx, A, B, qw, bias) -> None:

@@ -203,6 +203,58 @@ PyObject* py_linear_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// linear_infer(x, qx | None, sx | None, A | None, B | None, lora_scale, qw, scale bits, bias | None, w4) -> (y, qx, sx): the
+// forward over contiguous x (.., K) that nothing differentiates, y (.., N); the codes are x's where given, else made and
+// returned.  The scale bits are the layer's own integers (or the floats they stand for).
+PyObject* py_linear_infer(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(10)
+  return guarded([&]() -> PyObject* {
+    const Tensor *x = tensor_of(a[0], bad), *qx = tensor_of(a[1], bad), *sx = tensor_of(a[2], bad),
+                 *A = tensor_of(a[3], bad), *B = tensor_of(a[4], bad), *qw = tensor_of(a[6], bad),
+                 *sw = tensor_of(a[7], bad), *bias = tensor_of(a[8], bad);
+    const double scale = PyFloat_AsDouble(a[5]);
+    const int w4 = PyObject_IsTrue(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    if (bad || !x || !qw || !sw || x->dim() < 1 || qw->dim() != 2 || !qx != !sx) K2Q_REFUSE;
+    const int64_t K = x->size(x->dim() - 1), N = qw->size(0);
+    const c10::Device d = x->device();
+    const bool bits = sw->scalar_type() == (w4 ? at::kShort : at::kInt);
+    if (!ready(d) || !width_ok(K) || x->numel() == 0 || x->scalar_type() != at::kBFloat16 || !x->is_contiguous() ||
+        !aligned(*x) || !operand(qw, w4 ? at::kByte : at::kChar, 2, d) || qw->size(1) != (w4 ? K / 2 : K) || N % 64 ||
+        !operand(sw, bits ? sw->scalar_type() : w4 ? at::kBFloat16 : at::kFloat, w4 ? 2 : 1, d) ||
+        (w4 ? sw->size(0) != K / 64 || sw->size(1) != N : sw->size(0) != N))
+      K2Q_REFUSE;
+    const int64_t M = x->numel() / K;
+    if (qx && (!operand(qx, at::kChar, 2, d) || qx->size(0) != M || qx->size(1) != K ||
+               !operand(sx, at::kFloat, 1, d) || sx->size(0) != M))
+      K2Q_REFUSE;
+    int64_t r = 0;
+    if (A) {
+      if (!operand(A, at::kFloat, 2, d) || !operand(B, at::kFloat, 2, d)) K2Q_REFUSE;
+      r = A->size(0);
+      if (A->size(1) != K || B->size(0) != N || B->size(1) != r || !rank_ok(r)) K2Q_REFUSE;
+    }
+    if (bias && (!operand(bias, at::kFloat, 1, d) || bias->size(0) != N)) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    const int wmode = w4 ? K2Q_WMODE_W4 : K2Q_WMODE_W8;
+    at::DimVector shape(x->sizes());
+    shape[x->dim() - 1] = N;
+    Tensor y = alloc(shape, at::kBFloat16, d);
+    const Tensor q = qx ? *qx : alloc({M, K}, at::kChar, d), s = sx ? *sx : alloc({M}, at::kFloat, d);
+    Tensor u = r && M <= 8 ? alloc({M, r}, at::kFloat, d) : Tensor();
+    const int64_t nws = api.linear_fwd_ws_bytes(wmode, M, N, K, r);
+    Tensor ws = workspace(nws, d);
+    const int rc = foreign(api.linear_fwd, as<uint16_t>(ptr(x)), K, M, K, as<int8_t>(ptr(q)), as<float>(ptr(s)),
+                           qx ? 1 : 0, as<float>(ptr(A)), as<float>(A ? ptr(B) : nullptr), r, (float)scale,
+                           as<float>(ptr(u)), wmode, ptr(qw), ptr(sw), as<float>(ptr(bias)), N, as<uint16_t>(ptr(y)),
+                           ptr(ws), nws, st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({y, q, s});
+  });
+}
+
 // lora_grads(dy, x | None, u | None, B, lora_scale) -> (g, dA | None, dB | None)
 PyObject* py_lora_grads(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(5)
@@ -558,7 +610,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int dt = ty == at::kBFloat16 ? K2Q_DTYPE_BF16 : ty == at::kHalf ? K2Q_DTYPE_F16 : K2Q_DTYPE_F32;
     const auto pt = p->scalar_type();
     const int pos_type = pt == at::kLong ? K2Q_POS_I64 : pt == at::kInt ? K2Q_POS_I32 : pt == at::kFloat ? K2Q_POS_F32 : K2Q_POS_F64;
-    if (!ready(d) || (dt == K2Q_DTYPE_F32 && ty != at::kFloat) || (pos_type == K2Q_POS_F64 && pt != at::kDouble) ||
+    if (!ready(d) || (dt == K2Q_DTYPE_F32 && ty != at::kFloat) || (pos_type == K2Q_POS_F64 && pt != at::kDouble) || D > 4096 ||
         turns->scalar_type() != at::kDouble || !turns->is_contiguous() || turns->device() != d || 2 * nf > D ||
         p->device() != d ||
         (axis && (axis->scalar_type() != at::kInt || !axis->is_contiguous() || axis->numel() != nf || axis->device() != d)))
@@ -633,7 +685,8 @@ PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2
                          K2Q_METHOD(linear_fwd),  K2Q_METHOD(lora_grads),     K2Q_METHOD(lora_down),
                          K2Q_METHOD(dx_weight),   K2Q_METHOD(gemm_dx),        K2Q_METHOD(dequant_fp8),
                          K2Q_METHOD(gemm_bf16),   K2Q_METHOD(pad_factors),    K2Q_METHOD(resnorm),
-                         K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         {nullptr, nullptr, 0, nullptr}};
+                         K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         K2Q_METHOD(linear_infer),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

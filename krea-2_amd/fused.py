@@ -3,14 +3,15 @@
 In a Krea 2 block every ConvRot linear receives one of three tensors (reference ``mmdit.py:310-319``):
 the modulated RMSNorm output ``(1 + scale) * norm(x) + shift`` (read by ``wq/wk/wv/gate`` and by
 ``mlp.gate/up``), the attention output (read by ``wo``) and the SwiGLU product ``silu(gate) * up`` (read by
-``mlp.down``).  The two producers here compute that tensor AND its int8 codes in one gfx950 pass
-(``k2q_rmsmod_rotquant`` / ``k2q_swiglu_rotquant``), then hand the codes to the shared-input cache, so the
-layers that read the tensor run no rotate/quant of their own.  Outputs are the reference's eager bf16
-results (same rounding points), and the codes equal a separate rotate/quant of them bit for bit.
+``mlp.down``).  The producers here compute that tensor AND its int8 codes in one gfx950 pass
+(``k2q_rmsmod_rotquant``; ``k2q_resnorm_rotquant``, which adds the residual first; ``k2q_swiglu_rotquant``), then
+hand the codes to the shared-input cache, so the layers that read the tensor run no rotate/quant of their own.
+Outputs are the reference's eager bf16 results (same rounding points), and the codes equal a separate
+rotate/quant of them bit for bit.
 
 :func:`fuse_producers` patches a DiT's blocks in place (call it after ``quantize_dit_convrot`` and
-``inject_lora``); :func:`modulated_rmsnorm` and :func:`swiglu` are the two operations for model code that
-calls them directly.  :func:`group_siblings` makes the linears that read one tensor (``wq / wk / wv / gate``)
+``inject_lora``); :func:`modulated_rmsnorm`, :func:`residual_rmsnorm` and :func:`swiglu` are the operations for model code
+that calls them directly.  :func:`group_siblings` makes the linears that read one tensor (``wq / wk / wv / gate``)
 run as one grouped GEMM launch.
 """
 from __future__ import annotations
@@ -109,6 +110,22 @@ class _RmsModQuantFn(torch.autograd.Function):
         return dx, None, None, None, None, None
 
 
+def _stream_grads(dr, r, w, gate, y, ctx):
+    nx, ny, ng, nw, ns, nb = ctx.needs_input_grad[:6]
+    dy, dgate = dr, None
+    if gate is not None:
+        rows = dr.reshape(-1, ctx.rows, r.shape[-1])        # (entries, rows, K)
+        dy = (gate.reshape(-1, 1, r.shape[-1]) * rows).reshape(dr.shape)
+        if ng:
+            g = (rows.float() * y.reshape(rows.shape)).sum(1)
+            shape = ctx.shapes[2]
+            dgate = (g if g.numel() == shape.numel() else g.sum(0)).to(gate.dtype).reshape(shape)
+    dscale, dshift = (torch.zeros(shape, dtype=r.dtype, device=r.device) if need else None
+                      for need, shape in zip((ns, nb), ctx.shapes))
+    return (dr if nx else None, dy if ny else None, dgate, torch.zeros_like(w) if nw else None, dscale, dshift, None, None,
+            None)
+
+
 class _ResNormQuantFn(torch.autograd.Function):
     """Forward: the residual's addition and the (modulated) RMSNorm of ``mmdit.py:317-318`` with the codes of its output,
     one gfx950 pass.  Backward ``k2q_resnorm_bwd``: the gradients of the stream and of what was added in one pass, and the
@@ -138,6 +155,8 @@ class _ResNormQuantFn(torch.autograd.Function):
         shape = (dh if dr is None else dr).shape
         r, w, scale, gate, y = ctx.saved_tensors
         nx, ny, _, nw, ns, nb = ctx.needs_input_grad[:6]
+        if dh is None:      # nothing read h: the stream's gradient passes as it is
+            return _stream_grads(dr, r, w, gate, y, ctx)
         dh, dr = _dense_grad(dh, r), None if dr is None else _dense_grad(dr, r)
         if r.shape != shape:        # the forward ran on rows
             dh, dr = dh.view(r.shape), None if dr is None else dr.view(r.shape)
@@ -215,9 +234,13 @@ def _entry_rows(t: torch.Tensor, name: str, x: torch.Tensor):
 def _norm_weight(norm: nn.Module, train: bool):
     """``(w, add)``: the norm's weight is ``w + add``, w f32.  A norm with a ``scale`` (``mmdit.py:146-161``) weighs by
     ``scale + 1``, one with a ``weight`` by it."""
+    if isinstance(norm, nn.LayerNorm) or isinstance(getattr(norm, "bias", None), torch.Tensor):
+        raise ValueError(f"{type(norm).__name__} is not a root-mean-square norm: it has a mean or a bias")
     for name, add in (("scale", 1.0), ("weight", 0.0)):
         t = getattr(norm, name, None)
         if isinstance(t, torch.Tensor):
+            if t.dtype == torch.float32 and t.is_contiguous():
+                return t, add
             return (t.float().contiguous() if train and t.requires_grad else _norm_scale_f32(norm, name)), add
     raise ValueError(f"{type(norm).__name__} has neither a scale nor a weight")
 
@@ -236,6 +259,8 @@ def _residual_rows(x, y, gate, w, scale, shift):
     vectors = [None if t is None else _entry_rows(t, name, x)
                for t, name in ((gate, "gate"), (scale, "scale"), (shift, "shift"))]
     _lib._check_k(K)
+    if w.data_ptr() % 16:
+        raise ValueError("the norm's weight must be 16-byte aligned")
     x, y = _rows(x, K), _rows(y, K)
     return x, y, *vectors, x.shape[0] // max([t.shape[0] for t in vectors if t is not None], default=1)
 
@@ -261,6 +286,8 @@ def _residual_rmsnorm(norm, x, y, gate, scale, shift, eager):
     gradients are theirs bit for bit."""
     grad = torch.is_grad_enabled()
     w, add = _norm_weight(norm, grad)
+    if norm.eps is None:
+        raise ValueError(f"{type(norm).__name__} has no eps")
     eps = float(norm.eps)
     if x.numel() == 0:
         _residual_rows(x, y, gate, w, scale, shift)

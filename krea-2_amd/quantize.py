@@ -263,19 +263,27 @@ class ConvRotLinear(nn.Module):
             raise ValueError(f"x has {x.shape[-1]} features, layer expects {self.in_features}")
         if x.dtype != torch.bfloat16:
             raise NotImplementedError(f"ConvRotLinear runs bf16 activations (the DiT dtype); got {x.dtype}")
-        x2 = _token_rows(x, self.in_features)
-        if x2.shape[0] == 0:
+        if x.numel() == 0:
             return x.new_empty(*x.shape[:-1], self.out_features)
+        w4 = self.mode == "w4a8"
+        grad = torch.is_grad_enabled() and (x.requires_grad or (lora_A is not None and
+                                                                (lora_A.requires_grad or lora_B.requires_grad)))
         key, codes = shared_input_quant.find(x)
+        if not grad and not _lib.observed():    # nothing to differentiate: no autograd node, one native call
+            out = _lib.linear_infer(x, codes, lora_A, lora_B, float(lora_scale), self.qweight, self.wscale,
+                                    self._bias_f32(), w4)
+            if out is not None:
+                y, qx, sx = out
+                if codes is None:
+                    shared_input_quant.keep(x, key, qx, sx)
+                return y
+        x2 = _token_rows(x, self.in_features)
         ready = codes is not None
         qx, sx = codes if ready else _lib.alloc_codes(x2)
-        w4 = self.mode == "w4a8"
-        grad = torch.is_grad_enabled() and (x2.requires_grad or (lora_A is not None and
-                                                                  (lora_A.requires_grad or lora_B.requires_grad)))
         if grad or _lib.observed():
             y = _ConvRotLinearFn.apply(x2, lora_A, lora_B, self.qweight, self.weight_scale, self._bias_f32(), w4,
                                        float(lora_scale), qx, sx, ready, self)
-        else:   # nothing to differentiate: no autograd node, the one library call (u stays internal)
+        else:   # rows that are not contiguous, a device not checked yet (u stays internal)
             y, _ = _lib.linear_fwd(x2, qx, sx, ready, lora_A, lora_B, float(lora_scale), self.qweight,
                                    self.weight_scale, self._bias_f32(), w4, need_u=False)
         if not ready:

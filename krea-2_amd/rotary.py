@@ -155,6 +155,12 @@ class RotaryEmbedding(nn.Module):
         """``(q', k')``, with the strides of ``q`` and ``k``.  ``q`` (B, L, H, D), or with ``heads_first`` (B, H, L, D), or
         either without the batch; ``k`` the same with its own number of heads, or None.  ``positions``: int64, int32,
         float32 or float64, (L,) or (B, L), with ``axes`` a last dimension of one value per axis."""
+        grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _lib.observed()
+        table = self._tables.get(q.device)
+        if table is not None and not grad:      # the call as it is, where the kernel takes it
+            out = _lib.rotary_native(q, k, positions, *table, self.layout == "half", self.factor, False, heads_first)
+            if out is not None:
+                return out
         if q.dim() not in (3, 4) or (k is not None and k.dim() != q.dim()):
             raise ValueError(f"q {tuple(q.shape)} and k must have 4 dimensions, or 3 without a batch")
         if self.dim > q.shape[-1]:
@@ -171,6 +177,6 @@ class RotaryEmbedding(nn.Module):
         _lib._device_check(q.device)
         q, k = _heads(q), None if k is None else _heads(k)
         table, half = self._table(q.device), self.layout == "half"
-        if _lib.observed() or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        if grad:
             return _RotaryFn.apply(q, k, positions, table, half, self.factor, heads_first)
         return _lib.rotary(q, k, positions, *table, half, self.factor, False, heads_first)

@@ -255,6 +255,16 @@ def test_unused_and_broadcast_outputs(k2, dev):
     ref = (dr.double() * y.double()).sum((0, 1), keepdim=True)
     mag = (dr.double() * y.double()).abs().sum((0, 1), keepdim=True)
     assert gg.shape == one.shape and ((gg.double() - ref).abs() <= 2 ** -7 * mag).all()
+    full = [t.detach().clone().requires_grad_() for t in (x, y, gate, p, b)]
+    norm.scale.requires_grad_()
+    bad = x.detach().clone()
+    bad[1, 2, 5] = float("inf")                     # a row that the norm cannot take, whose norm nothing reads
+    full[0] = bad.requires_grad_()
+    gs = torch.autograd.grad(k2.residual_rmsnorm(norm, *full)[0], [*full, norm.scale], dr)
+    norm.scale.requires_grad_(False)
+    assert torch.equal(gs[0], dr) and torch.equal(gs[1], gate * dr)
+    assert ((gs[2].double() - (dr.double() * y.double()).sum(1, keepdim=True)).abs() <= 2 ** -8 * mag).all()
+    assert all((t == 0).all() and t.shape == u.shape for t, u in zip(gs[3:], [*full[3:], norm.scale]))
     gx2, = torch.autograd.grad(h, xs, dr)
     e = x.detach().clone().requires_grad_()
     ge, = torch.autograd.grad(k2.modulated_rmsnorm(norm, e + one.detach() * y, p, b), e, dr)
@@ -340,6 +350,8 @@ def test_refusals(k2, dev):
                 lambda: k2.residual_rmsnorm(norm, x, y, gate[..., :128]), lambda: k2.residual_rmsnorm(norm, x, y, p, b[:0], p),
                 lambda: k2.residual_rmsnorm(norm, x[..., :192], y[..., :192]), lambda: k2.residual_rmsnorm(nn.Module(), x, y),
                 lambda: k2.residual_rmsnorm(Norm(norm.scale[:128]), x, y),
+                lambda: k2.residual_rmsnorm(nn.LayerNorm(256, device=dev), x, y),
+                lambda: k2.residual_rmsnorm(nn.RMSNorm(256, device=dev), x, y),
                 lambda: k2._lib.resnorm_rotquant(x[0], y[0], None, norm.scale, 1.0, EPS, None, None, 3),
                 lambda: k2._lib.resnorm_bwd(x[0], None, x[0], norm.scale, 1.0, EPS, None, None, 4, y[0])):
         with pytest.raises(ValueError):
