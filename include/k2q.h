@@ -257,7 +257,8 @@ int k2q_gemm_w8a8_grouped(const int8_t* qx, const float* sx, int64_t M, int64_t 
  * and u (M x r f32, the LoRA factors the backward reuses) are caller buffers the call fills; y M x N bf16.
  * u may be NULL when nothing needs the factors afterwards (inference) and M > 8: then, for W8 and r <= 128,
  * the GEMM epilogue adds the down-projection's K-slice partials itself (no reduce launch; y is bit-identical).
- * M <= 8: one launch computes the codes and u, then the GEMV (two launches for the linear; u required).
+ * M <= 8: one launch computes the codes and u, then the GEMV (two launches for the linear; u required).  One token
+ * through a narrow W4 linear without LoRA, its codes not given, is one launch: the GEMV makes them.
  * Where k2q_linear_fwd_fuses_down(M, K, r) is 1 (codes not given, K <= 3072, a CU's worth or two of 16-row
  * tiles), the codes and u come from one k2q_rotquant_lora launch instead of k2q_rotquant + k2q_lora_down (u then
  * carries that kernel's summation order).

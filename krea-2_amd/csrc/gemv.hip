@@ -18,9 +18,11 @@
 // In a packed chunk of 8 bytes byte j holds code j in its low and code j + 8 in its high nibble: a 32-bit word shifted
 // left by 4 and masked, or masked alone, is four weights of consecutive k times 16, dotted as they are with four
 // consecutive activation codes; the factor 16 leaves in the epilogue (a power of two: exact).
-#include "k2q_common.h"
+#include "rotation.h"
 
 namespace {
+
+using namespace k2q_rot;
 
 constexpr int GV_ROWS = 4;    // weight rows per wave
 constexpr int GV_WAVES = 4;   // waves per workgroup
@@ -136,6 +138,9 @@ struct Gemv4Args {
   int K;
   uint16_t* y;           // M x N bf16
   int waves, teams;      // waves on one team's rows, teams per workgroup
+  const __bf16* x;       // kQuant: the token's row, whose codes and scale go to q and s
+  int8_t* q;
+  float* s;
 };
 
 // 32 weights of one row against 32 activation codes (x[0..7]: four codes a word, k ascending); 16 times the dot.
@@ -159,8 +164,8 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // The epilogue: a is 16 times the scaled sum of row n and token m.
-__device__ __forceinline__ void gemv4_store(const Gemv4Args& p, int m, int64_t n, float a) {
-  float f = __builtin_fmaf(a, p.sx[m] * (0.0078125f * 0.0625f), p.bias ? p.bias[n] : 0.f);
+__device__ __forceinline__ void gemv4_store(const Gemv4Args& p, int m, int64_t n, float a, float sx) {
+  float f = __builtin_fmaf(a, sx * (0.0078125f * 0.0625f), p.bias ? p.bias[n] : 0.f);
   if (p.u) f += lora_dot(p.u + (int64_t)m * p.r, p.lora_b + n * p.r, p.r, p.lora_scale);
   p.y[(int64_t)m * p.N + n] = (uint16_t)f32_to_bf16_bits(f);
 }
@@ -302,7 +307,7 @@ __global__ __launch_bounds__(64 * GM_WAVES) void gemv_w4_mfma_kernel(Gemv4Args p
     if (n >= p.N) continue;
     float a = 0.f;
     for (int v = 0; v < p.waves; ++v) a += reinterpret_cast<const float*>(lds + GM_LDS * v)[i];
-    gemv4_store(p, m, n, a);
+    gemv4_store(p, m, n, a, p.sx[m]);
   }
 }
 
@@ -327,10 +332,15 @@ int launch4_mfma(Gemv4Args p, int M, hipStream_t st) {
 // them, all weight loads issued before the first is used.  The team's sums meet in LDS.
 constexpr int G4_K = 2048;
 
-template <int MT, int R, int STEPS>
+//
+// kQuant: the codes are made here from x, by every workgroup for itself (rotated in registers, one row maximum over the
+// team, the arithmetic of rotquant_kernel bit for bit) while its weight loads are in flight; the first writes them out.
+template <int MT, int R, int STEPS, bool kQuant>
 __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
   constexpr int NV = R * MT, NS = (NV + 3) / 4, H = NV / 2;
   __shared__ float red[4][4 * NS];
+  static_assert(!kQuant || (MT == 1 && STEPS == 1), "codes are made for one token and one step");
+  __shared__ __attribute__((aligned(16))) int8_t codes[kQuant ? 4 : 1][kQuant ? G4_K : 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int team = wave / p.waves, part = wave % p.waves;
   const int64_t n0 = (xcd_block() * p.teams + team) * R;
@@ -356,6 +366,37 @@ __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
       if (ok) sv[s][q] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)(k >> 6) * p.N + base + q * half);
     }
   }
+  float sx = 0.f;
+  if constexpr (kQuant) {
+    const int off = G4_K * part + lane_offset(lane), l = lane & 15;
+    const float c1 = (l & 1) ? -1.f : 1.f, c2 = (l & 2) ? -1.f : 1.f, c8 = (l & 8) ? -1.f : 1.f;
+    float v[2][16], amax = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load16<__bf16>(p.x + off + 1024 * h, off + 1024 * h < p.K, v[h]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      rotate16(v[h], c1, c2, c8);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(v[h][i]));
+    }
+    amax = wave_max(amax);
+    if (lane == 0) red[wave][0] = amax;
+    __syncthreads();
+    for (int i = 0; i < p.waves; ++i) amax = fmaxf(amax, red[team * p.waves + i][0]);
+    __syncthreads();                                    // red is written again below
+    amax = fmaxf(amax, 1e-8f);
+    const float mul = __fdiv_rn(127.f, amax) * (c1 * c2 * c8);
+    sx = __fdiv_rn(amax, 127.f);
+    const bool write = blockIdx.x == 0 && team == 0;
+    if (write && part == 0 && lane == 0) p.s[0] = sx;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 c = pack_codes16(v[h], mul);
+      *reinterpret_cast<uint4*>(codes[wave] + lane_offset(lane) + 1024 * h) = c;
+      if (write && off + 1024 * h < p.K) *reinterpret_cast<uint4*>(p.q + off + 1024 * h) = c;
+    }
+    wave_fence();
+  }
   float acc[NV] = {};
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
@@ -364,8 +405,9 @@ __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
     v4i x[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      x[m][0] = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k);
-      x[m][1] = *reinterpret_cast<const v4i*>(p.qx + (int64_t)m * p.K + k + 16);
+      const int8_t* xp = kQuant ? codes[wave] + 32 * lane : p.qx + (int64_t)m * p.K + k;
+      x[m][0] = *reinterpret_cast<const v4i*>(xp);
+      x[m][1] = *reinterpret_cast<const v4i*>(xp + 16);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -391,24 +433,25 @@ __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
   if (n0 + r >= p.N) return;
   float a = 0.f;
   for (int v = 0; v < p.waves; ++v) a += red[wave + v][at];
-  gemv4_store(p, m, n0 + r, a);
+  gemv4_store(p, m, n0 + r, a, kQuant ? sx : p.sx[m]);
 }
 
-template <int MT, int R, int STEPS>
+template <int MT, int R, int STEPS, bool kQuant>
 int launch4_mrs(const Gemv4Args& p, hipStream_t st) {
   const int64_t rows_per_wg = (int64_t)R * p.teams;
   const int64_t grid = (p.N + rows_per_wg - 1) / rows_per_wg;
   if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
-  hipLaunchKernelGGL((gemv_w4_kernel<MT, R, STEPS>), dim3((unsigned)grid), dim3(64 * p.waves * p.teams), 0, st, p);
+  hipLaunchKernelGGL((gemv_w4_kernel<MT, R, STEPS, kQuant>), dim3((unsigned)grid), dim3(64 * p.waves * p.teams), 0, st, p);
   return k2q_launch_status();
 }
 
-template <int MT, int R>
+template <int MT, int R, bool kQuant = false>
 int launch4_mr(Gemv4Args p, hipStream_t st) {
   const int steps = (p.K + G4_K - 1) / G4_K;
   p.waves = steps < 4 ? steps : 4;
   p.teams = 4 / p.waves;
-  return steps <= 4 ? launch4_mrs<MT, R, 1>(p, st) : launch4_mrs<MT, R, 2>(p, st);
+  if constexpr (kQuant) return launch4_mrs<MT, R, 1, true>(p, st);
+  else return steps <= 4 ? launch4_mrs<MT, R, 1, false>(p, st) : launch4_mrs<MT, R, 2, false>(p, st);
 }
 
 // Which kernel.  A 16-row workgroup a CU needs N >= 4096; below that teams of four rows fill more of the chip.  From
@@ -464,7 +507,7 @@ int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, 
                          const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
                          int64_t K, uint16_t* y, hipStream_t st) {
   if (K > 4 * 2 * G4_K) return K2Q_EUNSUPPORTED;
-  Gemv4Args p{qx, sx, qw4, sw4, bias, u, lora_b, u ? r : 0, lora_scale, N, (int)K, y, 1, 1};
+  Gemv4Args p{qx, sx, qw4, sw4, bias, u, lora_b, u ? r : 0, lora_scale, N, (int)K, y, 1, 1, nullptr, nullptr, nullptr};
   switch (M) {
     case 1: return launch4_mt<1>(p, st);
     case 2: return launch4_mt<2>(p, st);
@@ -476,4 +519,17 @@ int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, 
     case 8: return launch4_mt<8>(p, st);
     default: return K2Q_EINVAL;
   }
+}
+
+// One token through a linear, its codes not given: one launch instead of two where every workgroup's own rotation hides
+// behind its weight loads.  Both launches against one, us: 512 x 512 4.7 / 3.3, 1536 x 6144 6.1 / 5.5, 4096 x 6144 7.8 / 7.1,
+// 6144 x 6144 8.7 / 8.7; no gain beyond, at two tokens (1536 x 6144 6.5 / 7.6) or two steps of K (2048 x 16384 9.7 / 9.6).
+bool k2q_gemv_w4a8_quantizes(int64_t M, int64_t N, int64_t K) { return M == 1 && N < 2 * G4_WIDE && K <= 4 * G4_K; }
+
+// Called by k2q_linear_fwd for such shapes, after the checks of k2q_gemm_w4a8: the codes of x are written to qx, sx.
+int k2q_launch_gemv_w4a8_quant(const uint16_t* x, int8_t* qx, float* sx, const uint8_t* qw4, const uint16_t* sw4,
+                               const float* bias, int64_t N, int64_t K, uint16_t* y, hipStream_t st) {
+  const Gemv4Args p{qx, sx, qw4, sw4, bias, nullptr, nullptr, 0, 0.f, N, (int)K, y, 1, 1,
+                    reinterpret_cast<const __bf16*>(x), qx, sx};
+  return N < G4_WIDE ? launch4_mr<1, 4, true>(p, st) : launch4_mr<1, 8, true>(p, st);
 }

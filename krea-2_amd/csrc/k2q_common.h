@@ -65,6 +65,11 @@ int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, 
                          const float* u, const float* lora_b, int r, float lora_scale, int64_t M, int64_t N,
                          int64_t K, uint16_t* y, hipStream_t st);
 
+// The W4A8 one for a token whose codes are made in the same launch, and the shapes where that pays.
+int k2q_launch_gemv_w4a8_quant(const uint16_t* x, int8_t* qx, float* sx, const uint8_t* qw4, const uint16_t* sw4,
+                               const float* bias, int64_t N, int64_t K, uint16_t* y, hipStream_t st);
+bool k2q_gemv_w4a8_quantizes(int64_t M, int64_t N, int64_t K);
+
 // LoRA down-projection u = x (scale F)^T (lora.hip); F is r x K row-major (a_kstride = 1) or given as its
 // K x r transpose (a_kstride = r).  k2q_lora_down is the a_kstride = 1, scale = 1 case.
 int lora_down_impl(const uint16_t* x, int64_t M, int64_t K, int64_t ldx, const float* a, int64_t a_kstride,

@@ -211,6 +211,12 @@ extern "C" int k2q_linear_fwd(const uint16_t* x, int64_t ldx, int64_t M, int64_t
   if (lora_ws && (!ws || ws_bytes < lay.total)) return K2Q_EINVAL;
   if (ws && !k2q_aligned(ws, 256)) return K2Q_EINVAL;
   if (skinny && lora_a && !u) return K2Q_EINVAL;      // the prologue writes u
+  if (skinny && !codes_ready && !lora_a && wmode == K2Q_WMODE_W4 && k2q_gemv_w4a8_quantizes(M, N, K)) {
+    if (N % 4 || !k2q_aligned(qw, 16) || !k2q_aligned(sw, 8) || !k2q_aligned(y, 8) || (bias && !k2q_aligned(bias, 16)))
+      return K2Q_EINVAL;      // as k2q_gemm_w4a8 checks them
+    return k2q_launch_gemv_w4a8_quant(x, qx, sx, static_cast<const uint8_t*>(qw), static_cast<const uint16_t*>(sw), bias,
+                                      N, K, y, st);
+  }
   uint8_t* w = static_cast<uint8_t*>(ws);
   // the GEMM's split pieces (without room for them it runs full-K tiles: the same output for W8, for W4 its f32 group
   // sums in another order)

@@ -69,6 +69,25 @@ def test_against_float64(k2, dev, M, N, K, r):
     assert torch.equal(L.gemm_w4a8(qx[p], sx[p], q4, s4, bias, u[p] if r else None, B, 0.75), y[p])
 
 
+@pytest.mark.parametrize("N,K", [(64, 128), (512, 512), (1536, 2048), (1536, 6144), (4092, 8192), (4100, 6272), (8188, 1024),
+                                 (8192, 1024), (1536, 8320)])
+def test_codes_made_on_the_way(k2, dev, N, K):
+    """One token whose codes are not given: the codes, scale and output of the separate launches, bit for bit; a row of
+    zeros, and the row's neighbours in a longer buffer untouched."""
+    L = k2._lib
+    g, _, _, q4, s4, _ = _inputs(1, N, K, dev, False)
+    bias = torch.randn(N, device=dev, generator=g)
+    x = torch.randn(2, K, device=dev, generator=g)
+    x[:, ::37] *= 20
+    x[1] = 0
+    for row in x.bfloat16().split(1):
+        qx, sx = torch.full((2, K), 99, dtype=torch.int8, device=dev), torch.full((2,), 7.0, device=dev)
+        y, _ = L.linear_fwd(row, qx[:1], sx[:1], False, None, None, 0.0, q4, s4, bias, True, need_u=False)
+        q0, s0, _ = L.rotquant(row)
+        assert torch.equal(qx[:1], q0) and torch.equal(sx[:1], s0) and (qx[1] == 99).all() and sx[1] == 7
+        assert torch.equal(y, L.gemm_w4a8(q0, s0, q4, s4, bias))
+
+
 def test_rows_behind_the_output_stay(k2, dev):
     """The last rows of a partly filled workgroup: nothing is written past y."""
     L = k2._lib
