@@ -42,16 +42,23 @@ struct GemvArgs {
   uint16_t* y;           // M x N bf16
 };
 
-// The LoRA term of one output: sum_j bf16(B[n, j]) bf16(scale u[m, j]) in f32, j ascending (r % 4 == 0).
+// The LoRA term of one output: sum_j bf16(B[n, j]) bf16(scale u[m, j]) in f32, j ascending (r % 16 == 0).  The loads of 16
+// ranks are issued together: their latency is all that a workgroup waits for at its end.
 __device__ __forceinline__ float lora_dot(const float* ub, const float* bb, int r, float scale) {
   float l = 0.f;
-  for (int j = 0; j < r; j += 4) {
-    const v4f uv = *reinterpret_cast<const v4f*>(ub + j);
-    const v4f bv = *reinterpret_cast<const v4f*>(bb + j);
+  for (int j = 0; j < r; j += 16) {
+    v4f uv[4], bv[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      l = __builtin_fmaf(bf16_bits_to_f32(f32_to_bf16_bits(bv[e])),
-                         bf16_bits_to_f32(f32_to_bf16_bits(uv[e] * scale)), l);
+    for (int i = 0; i < 4; ++i) {
+      bv[i] = *reinterpret_cast<const v4f*>(bb + j + 4 * i);
+      uv[i] = *reinterpret_cast<const v4f*>(ub + j + 4 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        l = __builtin_fmaf(bf16_bits_to_f32(f32_to_bf16_bits(bv[i][e])),
+                           bf16_bits_to_f32(f32_to_bf16_bits(uv[i][e] * scale)), l);
   }
   return l;
 }
