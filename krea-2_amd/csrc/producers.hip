@@ -542,10 +542,12 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
   __shared__ float red[3][64][33];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int K = a.K;
-  const int col = blockIdx.x * CS_COLS + 8 * lane;
-  const int entry = blockIdx.y / a.strips, strip = blockIdx.y % a.strips;
+  const uint32_t tiles = (uint32_t)(K + CS_COLS - 1) / CS_COLS, piece = blockIdx.x / tiles;
+  const int col = (int)(blockIdx.x % tiles) * CS_COLS + 8 * lane;
+  const int64_t entry = piece / a.strips;
+  const int strip = piece % a.strips;
   const int64_t m0 = entry * a.rpb + (int64_t)strip * a.strip_rows;
-  const int64_t mend = (int64_t)(entry + 1) * a.rpb;
+  const int64_t mend = (entry + 1) * a.rpb;
   const int64_t m1 = m0 + a.strip_rows < mend ? m0 + a.strip_rows : mend;
   const int cc = col < K ? col : 0;
   float w[8], p1[8], acc[4][8] = {};
@@ -577,7 +579,7 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
     for (int i = 0; i < 32; ++i) red[wave - 1][lane][i] = acc[i >> 3][i & 7];
   __syncthreads();
   if (wave || col >= K) return;
-  float* out = a.part + (int64_t)blockIdx.y * 4 * K + col;
+  float* out = a.part + (int64_t)piece * 4 * K + col;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -585,17 +587,19 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
       out[(int64_t)k * K + i] = ((acc[k][i] + red[0][lane][8 * k + i]) + red[1][lane][8 * k + i]) + red[2][lane][8 * k + i];
 }
 
-// The strips' partials joined: 64 columns a workgroup, its four waves every fourth strip, then the four in order.  Grid y:
-// the batch entries (scale, shift and gate gradients, bf16), then one more for the norm weight's (f32, every entry).
-__global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* part, int K, int entries, int strips,
+// The strips' partials joined: 64 columns a workgroup, its four waves every fourth strip, then the four in order.  Column
+// tiles of the batch entries (scale, shift and gate gradients, bf16), then those of the norm weight's (f32, every entry).
+__global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* part, int K, int64_t entries, int strips,
                                                                   float* dnw, uint16_t* dscale, uint16_t* dshift,
                                                                   uint16_t* dgate) {
   __shared__ float red[3][4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = blockIdx.x * 64 + lane;
-  const int entry = blockIdx.y;
+  const uint32_t tiles = (uint32_t)(K + 63) / 64;
+  const int col = (int)(blockIdx.x % tiles) * 64 + lane;
+  const int64_t entry = blockIdx.x / tiles;
   const bool all = entry == entries;
-  const int64_t i0 = all ? 0 : (int64_t)entry * strips, i1 = all ? (int64_t)entries * strips : i0 + strips;
+  if (all && !dnw) return;
+  const int64_t i0 = all ? 0 : entry * strips, i1 = all ? entries * strips : i0 + strips;
   float f[3] = {};
   if (col < K) {
     if (all) {
@@ -615,10 +619,10 @@ __global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* p
 #pragma unroll
   for (int k = 0; k < 3; ++k) f[k] = ((red[k][0][lane] + red[k][1][lane]) + red[k][2][lane]) + red[k][3][lane];
   if (all) {
-    if (dnw) dnw[col] = f[0];
+    dnw[col] = f[0];
     return;
   }
-  const int64_t o = (int64_t)entry * K + col;
+  const int64_t o = entry * K + col;
   if (dscale) dscale[o] = (uint16_t)f32_to_bf16_bits(f[0]);
   if (dshift) dshift[o] = (uint16_t)f32_to_bf16_bits(f[1]);
   if (dgate) dgate[o] = (uint16_t)f32_to_bf16_bits(f[2]);
@@ -795,8 +799,9 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
     if (M % rows_per_batch || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_resnorm_bwd_ws_bytes(M, K, rows_per_batch) ||
         ((dscale || dshift) && !mod_scale) || (dgate && (!gate || !y || !k2q_aligned(y, 16) || ldy < K || ldy % 8)))
       return K2Q_EINVAL;
-    if (entries > 32767) return K2Q_EUNSUPPORTED;   // launch extents: two bytes of entries and strips
   }
+  // launch extents: column tiles by entries and strips (fewer than 1024 strips in all beyond one an entry)
+  if (cols && (K + 63) / 64 * (entries + 1024) > 0x7fffffff) return K2Q_EUNSUPPORTED;
   NormBwdArgs a{};
   a.dh = dh;
   a.x = r;
@@ -835,9 +840,9 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   c.mscale = mod_scale;
   c.ldm = ld_scale;
   c.part = a.stats + 2 * M;
-  const dim3 grid((unsigned)((K + CS_COLS - 1) / CS_COLS), (unsigned)(entries * c.strips));
-  hipLaunchKernelGGL(resnorm_colsum_kernel, grid, dim3(256), 0, st, c);
-  hipLaunchKernelGGL(resnorm_colsum_join_kernel, dim3((unsigned)((K + 63) / 64), (unsigned)entries + 1), dim3(256), 0, st,
-                     c.part, (int)K, (int)entries, c.strips, dnorm, dscale, dshift, dgate);
+  const int64_t grid = (K + CS_COLS - 1) / CS_COLS * entries * c.strips, join = (K + 63) / 64 * (entries + 1);
+  hipLaunchKernelGGL(resnorm_colsum_kernel, dim3((unsigned)grid), dim3(256), 0, st, c);
+  hipLaunchKernelGGL(resnorm_colsum_join_kernel, dim3((unsigned)join), dim3(256), 0, st, c.part, (int)K, entries, c.strips,
+                     dnorm, dscale, dshift, dgate);
   return k2q_launch_status();
 }

@@ -34,7 +34,9 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor, K: int) -> torch.Tensor:
     t2 = t.reshape(-1, K)
-    if t2.stride(1) != 1 or t2.stride(0) % 8 or t2.stride(0) < K or t2.data_ptr() % 16:
+    if t2.stride(0) < K:        # rows that overlap, or one row of any stride
+        return t2.clone(memory_format=torch.contiguous_format)
+    if t2.stride(1) != 1 or t2.stride(0) % 8 or t2.data_ptr() % 16:
         t2 = _aligned(t2)
     return t2
 

@@ -243,6 +243,21 @@ def test_gradient_against_differences(k2, dev):
         assert abs(num - (gi.double() * d).sum().item()) <= 8 * 2 ** -8 * (gi.double().abs() * d.abs()).sum().item(), i
 
 
+def test_an_entry_per_row(k2, dev):
+    """Rows with a gate and a modulation of their own, more of them than a launch has workgroups in its second extent."""
+    M, K = 66000, 128
+    norm, x, y, (gate, p, b) = _inputs((M, K), dev, M)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, y, gate, p, b)]
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+    got = _grads(k2.residual_rmsnorm(norm, *leaves), leaves, dr, dh)
+    l64 = [t.detach().double().requires_grad_() for t in leaves]
+    ref = _grads(_separate(norm.scale.detach().double(), *l64), l64, dr.double(), dh.double())
+    for a, e in zip(got, ref):
+        assert a.shape == e.shape and (a.double() - e).norm() <= 1.25 * 2 ** -8 * e.norm()
+    one = torch.randn(K, device=dev).as_strided((1, K), (1, 1)).bfloat16().as_strided((1, K), (1, 1))
+    assert torch.equal(k2.residual_rmsnorm(norm, one, one)[0], one + one)
+
+
 def test_unused_and_broadcast_outputs(k2, dev):
     """Only r, only h, or neither used; a gate of one entry beside a modulation per batch row; a bf16 norm scale."""
     norm, x, y, (gate, p, b) = _inputs((3, 4, 256), dev, 3)

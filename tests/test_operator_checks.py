@@ -56,7 +56,7 @@ def test_entry_points_refuse_bad_arguments(k2):
     for bad in ({"dh": None}, {"r": odd}, {"M": 0}, {"K": 100}, {"ms": None}, {"gate": None}, {"dy": None}, {"rows": 3},
                 {"rows": 0}, {"dx": None}, {"y": None}, {"ws": None}, {"nws": 16}):
         assert bwd(**bad) == -1, bad
-    assert bwd(M=40000, rows=1) == -4
+    assert bwd(M=1 << 31) == -4 and bwd(M=1 << 30, rows=1, nws=1 << 62) == -4
 
     heads = k2._lib.RotaryHeads(p, p, 4, 64 * 4 * 6, 256, 64, 64 * 4 * 6, 256, 64)
 
