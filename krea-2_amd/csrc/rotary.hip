@@ -10,7 +10,8 @@
 //
 // Bound: reading and writing the heads once.  A workgroup takes a run of (token, head) rows, q's heads before k's in
 // every token; its threads first compute the cos / sin of the run's tokens into LDS, once for all heads, then a thread
-// turns 16-byte vectors of one head position, stepping through the run's rows.
+// turns vectors of one head position, stepping through the run's rows.  4608 x 60 heads of 128 bf16: 30 us (4.8 TB/s), 16896
+// of them 98 us (5.3).
 #include <hip/hip_fp16.h>
 
 #include "k2q_common.h"
@@ -36,7 +37,7 @@ struct RotArgs {
   const double* turns;
   const int* axis;         // null: one axis
   float m, sign;
-  int items, width, slots; // work items per row, threads side by side on a row, rows side by side
+  int turned, items, width, slots;   // a row's turned vectors, all its vectors, threads side by side on a row, rows side by side
   uint32_t run;            // rows per workgroup
   int dt, dh;              // slots / h, slots % h
 };
@@ -68,29 +69,23 @@ struct Cvt<_Float16> {
   static __device__ __forceinline__ _Float16 out(float v) { return (_Float16)v; }
 };
 
-// Eight elements as one or two 16-byte vectors.
+// V elements as one aligned load and store (two of 16 bytes for eight f32).
+template <typename T, int V>
+struct Vec {
+  typedef T Raw __attribute__((ext_vector_type(V)));
+  Raw v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = v; }
+  __device__ __forceinline__ float get(int i) const { return Cvt<T>::in(v[i]); }
+  __device__ __forceinline__ void put(int i, float f) { v[i] = Cvt<T>::out(f); }
+};
 template <typename T>
-struct Vec8 {
-  static constexpr int N = sizeof(T) / 2;
-  uint4 v[N];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void store(T* p) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const T* e = reinterpret_cast<const T*>(v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::in(e[i]);
-  }
-  __device__ __forceinline__ void put(const float (&f)[8]) {
-    T* e = reinterpret_cast<T*>(v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = Cvt<T>::out(f[i]);
-  }
+struct Vec<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ float get(int) const { return Cvt<T>::in(v); }
+  __device__ __forceinline__ void put(int, float f) { v = Cvt<T>::out(f); }
 };
 
 __device__ __forceinline__ void turn(float& a, float& b, const float2& cs) {
@@ -99,7 +94,7 @@ __device__ __forceinline__ void turn(float& a, float& b, const float2& cs) {
   b = x * cs.y + y * cs.x;
 }
 
-template <typename T, bool kHalf, bool kVec>
+template <typename T, bool kHalf, int V>
 __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotArgs a) {
   extern __shared__ float2 cs[];
   const uint32_t r0 = blockIdx.x * a.run;
@@ -134,46 +129,37 @@ __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotArgs a) {
     T* o = static_cast<T*>(a.o[w]) + (b * a.ob[w] + l * a.ol[w] + hh * a.oh[w]);
     const float2* c = cs + (tok - t0) * nf;
     for (int j = j0; j < a.items; j += a.width) {
-      if constexpr (!kVec) {          // an item: one pair, or one copied element
-        if (j >= nf) {
-          o[j + nf] = x[j + nf];
-          continue;
-        }
-        const int ia = kHalf ? j : 2 * j, ib = kHalf ? j + nf : 2 * j + 1;
-        float f0 = Cvt<T>::in(x[ia]), f1 = Cvt<T>::in(x[ib]);
-        turn(f0, f1, c[j]);
-        o[ia] = Cvt<T>::out(f0);
-        o[ib] = Cvt<T>::out(f1);
-      } else if constexpr (kHalf) {   // an item: eight pairs, or eight copied elements
-        Vec8<T> u, v;
-        if (8 * j >= nf) {
-          const int e = a.rd + 8 * j - nf;
-          u.load(x + e);
-          u.store(o + e);
-          continue;
-        }
-        u.load(x + 8 * j);
-        v.load(x + nf + 8 * j);
-        float f[8], g[8];
-        u.get(f);
-        v.get(g);
+      if (j >= a.turned) {                    // V copied elements
+        Vec<T, V> u;
+        const int e = a.rd + V * (j - a.turned);
+        u.load(x + e);
+        u.store(o + e);
+      } else if constexpr (kHalf || V == 1) { // V pairs from two vectors
+        constexpr bool kBeside = !kHalf;
+        const int ia = kBeside ? 2 * j : V * j, ib = kBeside ? 2 * j + 1 : nf + V * j;
+        Vec<T, V> u, v;
+        u.load(x + ia);
+        v.load(x + ib);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) turn(f[i], g[i], c[8 * j + i]);
-        u.put(f);
-        v.put(g);
-        u.store(o + 8 * j);
-        v.store(o + nf + 8 * j);
-      } else {                        // an item: four pairs, or eight copied elements
-        Vec8<T> u;
-        u.load(x + 8 * j);
-        if (8 * j < a.rd) {
-          float f[8];
-          u.get(f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) turn(f[2 * i], f[2 * i + 1], c[4 * j + i]);
-          u.put(f);
+        for (int i = 0; i < V; ++i) {
+          float f = u.get(i), g = v.get(i);
+          turn(f, g, c[V * j + i]);
+          u.put(i, f);
+          v.put(i, g);
         }
-        u.store(o + 8 * j);
+        u.store(o + ia);
+        v.store(o + ib);
+      } else {                                // V / 2 pairs from one
+        Vec<T, V> u;
+        u.load(x + V * j);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          float f = u.get(2 * i), g = u.get(2 * i + 1);
+          turn(f, g, c[V / 2 * j + i]);
+          u.put(2 * i, f);
+          u.put(2 * i + 1, g);
+        }
+        u.store(o + V * j);
       }
     }
     tok += a.dt;
@@ -192,13 +178,17 @@ __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotArgs a) {
 }
 
 template <typename T, bool kHalf>
-void launch(const RotArgs& a, bool vec, unsigned grid, int lds, hipStream_t st) {
-  if (vec) hipLaunchKernelGGL((rotary_kernel<T, kHalf, true>), dim3(grid), dim3(RT_THREADS), lds, st, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, kHalf, false>), dim3(grid), dim3(RT_THREADS), lds, st, a);
+void launch(const RotArgs& a, int vec, unsigned grid, int lds, hipStream_t st) {
+  switch (vec) {
+    case 8: hipLaunchKernelGGL((rotary_kernel<T, kHalf, 8>), dim3(grid), dim3(RT_THREADS), lds, st, a); break;
+    case 4: hipLaunchKernelGGL((rotary_kernel<T, kHalf, 4>), dim3(grid), dim3(RT_THREADS), lds, st, a); break;
+    case 2: hipLaunchKernelGGL((rotary_kernel<T, kHalf, 2>), dim3(grid), dim3(RT_THREADS), lds, st, a); break;
+    default: hipLaunchKernelGGL((rotary_kernel<T, kHalf, 1>), dim3(grid), dim3(RT_THREADS), lds, st, a); break;
+  }
 }
 
 template <typename T>
-void launch_t(const RotArgs& a, bool half, bool vec, unsigned grid, int lds, hipStream_t st) {
+void launch_t(const RotArgs& a, bool half, int vec, unsigned grid, int lds, hipStream_t st) {
   if (half) launch<T, true>(a, vec, grid, lds, st);
   else launch<T, false>(a, vec, grid, lds, st);
 }
@@ -218,16 +208,24 @@ extern "C" int k2q_rotary(const k2q_rotary_heads* t, int64_t n, int dtype, int64
   const int size = dtype == K2Q_DTYPE_F32 ? 4 : 2;
   const bool half = layout == K2Q_ROTARY_HALF;
   RotArgs a{};
-  // 16-byte vectors: whole vectors in the rotated part (of each half), the rest and every row's start
-  bool vec = half ? rotary_dim % 16 == 0 && (D - rotary_dim) % 8 == 0 : rotary_dim % 8 == 0 && D % 8 == 0;
+  // The widest vector that cuts the rotated part (each half of it), the rest and every row's start into whole ones
+  const int rest = (int)(D - rotary_dim);
+  int vec = 8;
+  auto narrow = [&](int64_t elements) {
+    while (elements % vec) vec >>= 1;
+  };
+  narrow(half ? rotary_dim / 2 : rotary_dim);
+  narrow(rest);
   int64_t heads = 0;
   for (int i = 0; i < 2; ++i) {
     const k2q_rotary_heads& s = t[i < n ? i : 0];
     const int64_t strides[6] = {s.x_b, s.x_l, s.x_h, s.o_b, s.o_l, s.o_h};
     if (!s.x || !s.o || s.heads < 1 || !k2q_aligned(s.x, size) || !k2q_aligned(s.o, size)) return K2Q_EINVAL;
-    vec = vec && k2q_aligned(s.x, 16) && k2q_aligned(s.o, 16);
     const int64_t extent[3] = {B, L, s.heads};
-    for (int d = 0; d < 6; ++d) vec = vec && (extent[d % 3] == 1 || strides[d] * size % 16 == 0);
+    for (int d = 0; d < 6; ++d)
+      if (extent[d % 3] > 1) narrow(strides[d]);
+    narrow((int64_t)(reinterpret_cast<uintptr_t>(s.x) / size));
+    narrow((int64_t)(reinterpret_cast<uintptr_t>(s.o) / size));
     a.x[i] = s.x;
     a.o[i] = s.o;
     a.xb[i] = s.x_b; a.xl[i] = s.x_l; a.xh[i] = s.x_h;
@@ -255,18 +253,21 @@ extern "C" int k2q_rotary(const k2q_rotary_heads* t, int64_t n, int dtype, int64
   a.axis = axis;
   a.m = factor;
   a.sign = inverse ? -1.f : 1.f;
-  const int nf = a.rd / 2, rest = a.D - a.rd;
-  a.items = !vec ? nf + rest : half ? (nf + rest) / 8 : a.D / 8;
+  const int nf = a.rd / 2;
+  a.turned = half || vec == 1 ? nf / vec : a.rd / vec;
+  a.items = a.turned + rest / vec;
   a.width = a.items < RT_THREADS ? a.items : RT_THREADS;
   a.slots = RT_THREADS / a.width;
-  a.dt = a.slots / a.h;
-  a.dh = a.slots % a.h;
-  // steps per workgroup: eight where the rows still give every CU four workgroups, and no more tokens than fit LDS
-  int64_t steps = (int64_t)a.rows / ((int64_t)a.slots * 4 * k2q_cu_count());
-  steps = steps < 1 ? 1 : steps > 8 ? 8 : steps;
+  // Rows per workgroup: 16 KB of heads, fewer where the rows would not give every CU four workgroups, no more tokens than
+  // fit LDS.  4608 x 60 heads of 128 bf16, us at 16 / 32 / 64 / 128 rows (interleaved) 41 / 33 / 30 / 32, at 32 / 64 / 128 /
+  // 256 (half) 32 / 32 / 34 / 38; below 16 KB the cos / sin of a token are made too often, above it the last ones wait.
+  int64_t steps = 16384 / ((int64_t)a.slots * a.D * size);
+  const int64_t fill = (int64_t)a.rows / ((int64_t)a.slots * 4 * k2q_cu_count());
+  steps = steps > fill ? fill : steps;
+  steps = steps < 1 ? 1 : steps;
   const int64_t most = RT_LDS / (8 * nf);                    // tokens whose cos / sin fit
   while (steps > 1 && (steps * a.slots - 1) / a.h + 2 > most) --steps;
-  if (steps == 1 && (a.slots - 1) / a.h + 2 > most) a.slots = (int)((most - 2) * a.h + 1 < a.slots ? (most - 2) * a.h + 1 : a.slots);
+  if ((a.slots - 1) / a.h + 2 > most) a.slots = (int)((most - 2) * a.h + 1);
   a.dt = a.slots / a.h;
   a.dh = a.slots % a.h;
   a.run = (uint32_t)(steps * a.slots);

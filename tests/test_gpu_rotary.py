@@ -139,6 +139,24 @@ def test_strides_views_and_positions_broadcast(k2, dev):
     assert strided.stride(0) == 2 and torch.equal(rope(q, None, strided)[0], ref)
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,D", [(64, 64), (24, 96), (20, 80), (12, 30), (6, 7)])
+@pytest.mark.parametrize("start", [0, 1, 2, 4, 8])
+def test_every_vector_width(k2, dev, dim, D, start, dtype, layout):
+    """Heads that start anywhere in their storage, and sizes that cut into vectors of eight, four, two or one: the bits of
+    aligned copies, values between the rows untouched."""
+    rope = k2.RotaryEmbedding(dim, layout=layout)
+    wide = torch.randn(2, 9, 3, D + start, device=dev).to(dtype)
+    q = wide[..., start:]
+    pos = torch.arange(9, device=dev) * 11
+    aligned = torch.zeros(2, 9, 3, (D + 15) // 16 * 16, device=dev, dtype=dtype)[..., :D]
+    aligned.copy_(q)
+    a, b = rope(q, None, pos)[0], rope(aligned, None, pos)[0]
+    assert torch.equal(a, b)
+    _check(rope, a, q, pos)
+
+
 def test_gradients_of_one_of_both_and_expanded(k2, dev):
     rope = k2.RotaryEmbedding(64)
     q, k = torch.randn(1, 9, 4, 64, device=dev), torch.randn(1, 9, 2, 64, device=dev, requires_grad=True)
