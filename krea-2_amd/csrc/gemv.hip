@@ -190,24 +190,22 @@ __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
 }
 
-// Sums over the wave of NV values (NV even or 1): afterwards lane l holds in v[0..] the sums of the values that its
-// 32-lane half, then 16-lane row, took.  Each swap folds two values into one register (32 lanes apart, then 16), so a
-// value costs one add per stage for every two; the four stages inside a row are DPP adds.  The tree of one value is the
-// same for every NV.
+// Sums over the wave of NV values (NV % 4 == 0): afterwards every lane of 16-lane row 2 u + o holds in out[i] the sum of
+// value i + u NV / 2 + o NV / 4.  Each swap folds two values into one register (32 lanes apart, then 16), so a stage costs
+// one add for two values; the four stages inside a row are DPP adds.  The tree of one value is the same for every NV.
 template <int NV>
-__device__ __forceinline__ void wave_sums(float (&v)[NV], float (&out)[(NV + 3) / 4]) {
-  constexpr int H = (NV + 1) / 2, Q = (H + 1) / 2;
+__device__ __forceinline__ void wave_sums(float (&v)[NV], float (&out)[NV / 4]) {
+  static_assert(NV % 4 == 0, "values fold in fours");
+  constexpr int H = NV / 2, Q = NV / 4;
   float h[H];
 #pragma unroll
   for (int i = 0; i < H; ++i) {
-    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(i + H < NV ? v[i + H] : v[i]),
-                                                    false, false);
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + H]), false, false);
     h[i] = __uint_as_float(p[0]) + __uint_as_float(p[1]);      // lanes 0-31: value i, 32-63: value i + H
   }
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
-    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[i]), __float_as_uint(i + Q < H ? h[i + Q] : h[i]),
-                                                    false, false);
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[i]), __float_as_uint(h[i + Q]), false, false);
     float f = __uint_as_float(p[0]) + __uint_as_float(p[1]);   // odd 16-lane rows: h[i + Q]
     f = dpp_add<0xB1>(f);      // quad_perm xor 1
     f = dpp_add<0x4E>(f);      // quad_perm xor 2
@@ -219,16 +217,15 @@ __device__ __forceinline__ void wave_sums(float (&v)[NV], float (&out)[(NV + 3) 
 // The same product on the matrix cores: a workgroup owns 16 rows, its waves split K into 1024-wide segments (512 bytes
 // of a row, 16 scale groups).  One 16 x 16 x 64 MFMA is 16 weight rows against up to 16 token rows over one scale group:
 // lane (c = lane % 16, b = lane / 16) holds the 8 bytes of row c and the 16 codes of token c at k = 64 g + 16 b, and gets
-// the dots of row c with the token operand's rows 4 b .. 4 b + 3.  Loaded in that layout a row's bytes come 32 at a time (2.9 TB/s); so a
-// wave loads whole row segments, 16 bytes a lane, and turns them through its own piece of LDS: row c, 16-byte unit q at
-// unit q ^ 2 (c % 8), which spreads the eight rows of a read over all banks.  With at most 8 tokens half of a token
-// operand would be idle: its rows 8-15 hold the same tokens' codes of the next group, so one register serves two MFMAs,
-// whose results for tokens 0-7 are rows 0-7 (even groups) and rows 8-15 (odd groups).
+// the dots of row c with the token operand's rows 4 b .. 4 b + 3.  Loaded in that layout a row's bytes come 32 at a time
+// (2.9 TB/s); so a wave loads whole row segments, 16 bytes a lane, and turns them through its own piece of LDS: row c,
+// 16-byte unit q at unit q ^ 2 (c % 8), which spreads the eight rows of a read over all banks.  With at most 8 tokens half
+// of a token operand would be idle: its rows 8-15 hold the same tokens' codes of the next group, so one register serves two
+// MFMAs, whose results for tokens 0-7 are rows 0-7 (even groups) and rows 8-15 (odd groups).
 constexpr int GM_ROWS = 16;
 constexpr int GM_SEG = 1024;
 constexpr int GM_GROUPS = GM_SEG / 64;
 constexpr int GM_WAVES = 8;
-constexpr int GM_STEPS = 2;         // segments per wave: K <= 8 * 2 * 1024
 constexpr int GM_LDS = GM_ROWS * GM_SEG / 2 + GM_GROUPS * GM_ROWS * 2;   // a wave's piece: codes, then scales
 
 template <int STEPS>
@@ -335,16 +332,16 @@ int launch4_mfma(Gemv4Args p, int M, hipStream_t st) {
   return segs <= GM_WAVES ? launch4_mfma<1>(p, M, st) : launch4_mfma<2>(p, M, st);
 }
 
-// A team of `waves` waves owns R rows; a wave takes every `waves`-th 2048-wide step of K (16 bytes a lane), STEPS of
-// them, all weight loads issued before the first is used.  The team's sums meet in LDS.
 constexpr int G4_K = 2048;
 
+// A team of `waves` waves owns R rows; a wave takes every `waves`-th 2048-wide step of K (16 bytes a lane), STEPS of
+// them, all weight loads issued before the first is used.  The team's sums meet in LDS.
 //
 // kQuant: the codes are made here from x, by every workgroup for itself (rotated in registers, one row maximum over the
 // team, the arithmetic of rotquant_kernel bit for bit) while its weight loads are in flight; the first writes them out.
 template <int MT, int R, int STEPS, bool kQuant>
 __global__ __launch_bounds__(256) void gemv_w4_kernel(Gemv4Args p) {
-  constexpr int NV = R * MT, NS = (NV + 3) / 4, H = NV / 2;
+  constexpr int NV = R * MT, NS = NV / 4, H = NV / 2;
   __shared__ float red[4][4 * NS];
   static_assert(!kQuant || (MT == 1 && STEPS == 1), "codes are made for one token and one step");
   __shared__ __attribute__((aligned(16))) int8_t codes[kQuant ? 4 : 1][kQuant ? G4_K : 16];
