@@ -109,19 +109,23 @@ int k2q_rmsmod_bwd(const uint16_t* dh, const uint16_t* x, int64_t M, int64_t K, 
  *   k2q_rmsmod_bwd round them.
  * The sums over the rows of a batch entry are written where their pointer is given (dscale, dshift, dgate: entries x K
  * bf16, dnorm: K f32, over all rows); they need y (dgate), M a multiple of rows_per_batch, and ws of
- * k2q_resnorm_bwd_ws_bytes bytes, 16-byte aligned:
+ * k2q_resnorm_bwd_ws_bytes bytes, 16-byte aligned.  shared: K2Q_SHARED_* bits of the vectors that every entry shares; their
+ * gradients are K values, over all rows:
  *   dscale = sum dh n,  dshift = sum dh,  dgate = sum dR y,  dnorm = sum dh bf16(1 + p) r i,
  * in f32 in a fixed order, whatever eager is.  All M x K operands but y contiguous. */
 int k2q_resnorm_rotquant(const uint16_t* x, int64_t ldx, const uint16_t* y, int64_t ldy, const uint16_t* gate,
                          int64_t ld_gate, int64_t M, int64_t K, const float* norm_scale, float scale_add, float eps,
                          const uint16_t* mod_scale, int64_t ld_scale, const uint16_t* mod_shift, int64_t ld_shift,
                          int64_t rows_per_batch, uint16_t* r, uint16_t* h, int8_t* q, float* s, void* stream);
+#define K2Q_SHARED_SCALE 1
+#define K2Q_SHARED_SHIFT 2
+#define K2Q_SHARED_GATE 4
 int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch);
 int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
                     const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale, int64_t ld_scale,
                     const uint16_t* gate, int64_t ld_gate, int64_t rows_per_batch, int eager, uint16_t* dx, uint16_t* dy,
                     const uint16_t* y, int64_t ldy, float* dnorm, uint16_t* dscale, uint16_t* dshift, uint16_t* dgate,
-                    void* ws, int64_t ws_bytes, void* stream);
+                    int shared, void* ws, int64_t ws_bytes, void* stream);
 
 /* Rotary positions of queries and keys (mmdit.py:13-30, between the projections and the attention): every pair (a, b) of
  * the first rotary_dim values of a head turns by its token's angle, the rest of the head is copied:

@@ -80,7 +80,7 @@ _SIGNATURES = {
                               _p, _p, _p, _p], _int),
     "k2q_resnorm_bwd_ws_bytes": ([_i64, _i64, _i64], _i64),
     "k2q_resnorm_bwd": ([_p, _p, _p, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _int, _p, _p, _p, _i64, _p,
-                         _p, _p, _p, _p, _i64, _p], _int),
+                         _p, _p, _p, _int, _p, _i64, _p], _int),
     "k2q_rotary": ([_p, _i64, _int, _i64, _i64, _i64, _i64, _int, _p, _int, _i64, _i64, _i64, _p, _p, _f32, _int, _p],
                    _int),
     "k2q_lora_down_ws_bytes": ([_i64, _i64, _i64], _i64),
@@ -489,7 +489,7 @@ def resnorm_native(x, y, gate, w, add: float, eps: float, scale, shift):
     return out
 
 
-def _check_resnorm_bwd(dh, dr, r, w, ms, gate, rows_per_entry, y, need_mod) -> None:
+def _check_resnorm_bwd(dh, dr, r, w, ms, gate, rows_per_entry, y, need_mod, shift_entries) -> None:
     _need(r, "r", torch.bfloat16)
     flat = r.reshape(-1, r.shape[-1])
     _check_norm_rows(flat, "r", w, rows_per_entry)
@@ -508,21 +508,25 @@ def _check_resnorm_bwd(dh, dr, r, w, ms, gate, rows_per_entry, y, need_mod) -> N
         _need_rows(y if y.dim() == 2 else y.reshape(flat.shape), "y", r.device)
     if need_mod and ms is None:
         raise ValueError("no modulation to differentiate")
+    if shift_entries not in (1, flat.shape[0] // rows_per_entry):
+        raise ValueError(f"shift_entries={shift_entries}, expected 1 or {flat.shape[0] // rows_per_entry}")
     _device_check(r.device)
 
 
 def resnorm_bwd(dh, dr, r, w, add: float, eps: float, scale, gate, rows_per_entry: int, y=None, need_w=False,
-                need_scale=False, need_shift=False, eager=False):
+                need_scale=False, need_shift=False, shift_entries: int = 1, eager=False):
     """Autograd of :func:`resnorm_rotquant` and :func:`resnorm_native` (``k2q_resnorm_bwd``): ``(dx, dy, dw, dscale, dshift,
     dgate)`` from the gradients of ``h`` and (or None) of ``r``, contiguous in r's shape.  ``dy`` is None without a gate
-    (it is ``dx``); ``dgate`` comes when ``y`` is given, the other sums where asked for, in the shape of ``gate`` /
-    ``scale``, or (entries, K) where those are one entry among more.  ``eager``: rounded where eager bf16 operations round."""
-    args = (dh, dr, r, w, add, eps, scale, gate, rows_per_entry, y, need_w, need_scale, need_shift, eager)
+    (it is ``dx``); ``dgate`` comes when ``y`` is given, the other sums where asked for: in the shape of ``gate`` /
+    ``scale`` (one entry among more: the sum over every row), ``dshift`` (shift_entries, K).  ``eager``: rounded where eager
+    bf16 operations round."""
+    args = (dh, dr, r, w, add, eps, scale, gate, rows_per_entry, y, need_w, need_scale, need_shift, shift_entries, eager)
     out = _fast().resnorm_bwd(*args)
     if out.__class__ is tuple:
         return out
     return _refused(out, "k2q_resnorm_bwd", lambda: _native.resnorm_bwd(*args),
-                    lambda: _check_resnorm_bwd(dh, dr, r, w, scale, gate, rows_per_entry, y, need_scale or need_shift))
+                    lambda: _check_resnorm_bwd(dh, dr, r, w, scale, gate, rows_per_entry, y, need_scale or need_shift,
+                                               shift_entries))
 
 
 MAX_HEAD, MAX_ROTARY = 4096, 1024       # k2q_rotary's largest head and rotated part

@@ -539,11 +539,10 @@ PyObject* py_resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // resnorm_bwd(dh, dr | None, r, w, add, eps, scale | None, gate | None, rows_per_entry, y | None, need_w, need_scale,
-//             need_shift, eager) -> (dx, dy | None, dw | None, dscale | None, dshift | None, dgate | None): dh, dr, r
-// contiguous (.., K); dx, dy in their shape, the vectors' gradients in the vectors' (dshift in scale's), (entries, K) for
-// one entry among more
+//             need_shift, shift_entries, eager) -> (dx, dy | None, dw | None, dscale | None, dshift | None, dgate | None): dh,
+// dr, r contiguous (.., K); dx, dy in their shape, dscale and dgate in scale's and gate's, dshift (shift_entries, K)
 PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  K2Q_ARGS(14)
+  K2Q_ARGS(15)
   return guarded([&]() -> PyObject* {
     const Tensor *dh = tensor_of(a[0], bad), *dr = tensor_of(a[1], bad), *r = tensor_of(a[2], bad),
                  *w = tensor_of(a[3], bad), *ms = tensor_of(a[6], bad), *gate = tensor_of(a[7], bad),
@@ -551,7 +550,8 @@ PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double add = PyFloat_AsDouble(a[4]), eps = PyFloat_AsDouble(a[5]);
     int64_t rows = PyLong_AsLongLong(a[8]);
     const int need_w = PyObject_IsTrue(a[10]), need_scale = PyObject_IsTrue(a[11]), need_shift = PyObject_IsTrue(a[12]),
-              eager = PyObject_IsTrue(a[13]);
+              eager = PyObject_IsTrue(a[14]);
+    const int64_t nb = PyLong_AsLongLong(a[13]);
     if (PyErr_Occurred()) return nullptr;
     if (bad || !dh || !r || r->dim() < 2 || rows < 1) K2Q_REFUSE;
     const int64_t K = r->size(r->dim() - 1);
@@ -566,26 +566,23 @@ PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t ng, ns, lg, ls;
     if (!ready(d) || !whole(dh) || !whole(r) || (dr && !whole(dr)) ||
         !operand(w, at::kFloat, 1, d) || w->size(0) != K || !vectors_ok(gate, K, d, ng, lg) ||
-        !vectors_ok(ms, K, d, ns, ls) || !entries_fit({ng, ns}, M, 0, rows) || (y && (!gate || !in(y))) ||
+        !vectors_ok(ms, K, d, ns, ls) || !entries_fit({ng, ns, nb}, M, 0, rows) || (y && (!gate || !in(y))) ||
         ((need_scale || need_shift) && !ms))
       K2Q_REFUSE;
     const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
-    const int64_t E = M / rows;
-    auto vec = [&](bool need, const Tensor* t, int64_t n) {
-      return !need ? Tensor() : n == E ? alloc(t->sizes(), at::kBFloat16, d) : alloc({E, K}, at::kBFloat16, d);
-    };
     Tensor dx = alloc(r->sizes(), at::kBFloat16, d), dy = gate ? alloc(r->sizes(), at::kBFloat16, d) : Tensor();
-    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = vec(need_scale, ms, ns), db = vec(need_shift, ms, ns),
-           dg = vec(y, gate, ng);
+    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = need_scale ? alloc(ms->sizes(), at::kBFloat16, d) : Tensor(),
+           db = need_shift ? alloc({nb, K}, at::kBFloat16, d) : Tensor(), dg = y ? alloc(gate->sizes(), at::kBFloat16, d) : Tensor();
+    const int shared = (ns == 1 ? K2Q_SHARED_SCALE : 0) | (nb == 1 ? K2Q_SHARED_SHIFT : 0) | (ng == 1 ? K2Q_SHARED_GATE : 0);
     const int64_t nws = need_w || need_scale || need_shift || y ? api.resnorm_bwd_ws_bytes(M, K, rows) : 0;
     Tensor ws = workspace(nws, d);
     const int rc = foreign(api.resnorm_bwd, as<uint16_t>(ptr(dh)), as<uint16_t>(ptr(dr)), as<uint16_t>(ptr(r)), M, K,
                            as<float>(ptr(w)), (float)add, (float)eps, as<uint16_t>(ptr(ms)), ls, as<uint16_t>(ptr(gate)),
                            lg, rows, eager, as<uint16_t>(ptr(dx)), as<uint16_t>(ptr(dy)), as<uint16_t>(ptr(y)),
-                           y ? r->dim() == 2 ? y->stride(0) : K : 0, as<float>(ptr(dw)), as<uint16_t>(ptr(ds)), as<uint16_t>(ptr(db)),
-                           as<uint16_t>(ptr(dg)), ptr(ws), nws, st);
+                           y ? r->dim() == 2 ? y->stride(0) : K : 0, as<float>(ptr(dw)), as<uint16_t>(ptr(ds)),
+                           as<uint16_t>(ptr(db)), as<uint16_t>(ptr(dg)), shared, ptr(ws), nws, st);
     if (rc) return PyLong_FromLong(rc);
     return pack({dx, dy, dw, ds, db, dg});
   });

@@ -119,9 +119,13 @@ def _stream_grads(dr, r, w, gate, y, ctx):
         rows = dr.reshape(-1, ctx.rows, r.shape[-1])        # (entries, rows, K)
         dy = (gate.reshape(-1, 1, r.shape[-1]) * rows).reshape(dr.shape)
         if ng:
-            g = (rows.float() * y.reshape(rows.shape)).sum(1)
             shape = ctx.shapes[2]
-            dgate = (g if g.numel() == shape.numel() else g.sum(0)).to(gate.dtype).reshape(shape)
+            g = (rows.float() * y.reshape(rows.shape)).view(shape.numel() // r.shape[-1], -1, r.shape[-1])
+            while g.shape[1] > 1:   # halves added in f32: a reduction over many blocks clears counters, which no captured
+                n = g.shape[1] // 2         # graph can hold
+                g[:, :n] += g[:, -n:]
+                g = g[:, :g.shape[1] - n]
+            dgate = g.to(gate.dtype).reshape(shape)
     dscale, dshift = (torch.zeros(shape, dtype=r.dtype, device=r.device) if need else None
                       for need, shape in zip((ns, nb), ctx.shapes))
     return (dr if nx else None, dy if ny else None, dgate, torch.zeros_like(w) if nw else None, dscale, dshift, None, None,
@@ -162,15 +166,14 @@ class _ResNormQuantFn(torch.autograd.Function):
         dh, dr = _dense_grad(dh, r), None if dr is None else _dense_grad(dr, r)
         if r.shape != shape:        # the forward ran on rows
             dh, dr = dh.view(r.shape), None if dr is None else dr.view(r.shape)
-        dx, dy, dw, *sums = _lib.resnorm_bwd(dh, dr, r, w, ctx.add, ctx.eps, scale, gate, ctx.rows, y, nw, ns, nb, ctx.eager)
+        entries = 1 if scale is None else ctx.shapes[1].numel() // r.shape[-1]
+        dx, dy, dw, *sums = _lib.resnorm_bwd(dh, dr, r, w, ctx.add, ctx.eps, scale, gate, ctx.rows, y, nw, ns, nb, entries,
+                                             ctx.eager)
         if r.shape != shape:
             dx, dy = dx.view(shape), None if dy is None else dy.view(shape)
         if gate is None:
             dy = dx
-        dscale, dshift, dgate = (
-            t if t is None or t.shape == shape          # one entry for every batch row: the sum of the rows' sums
-            else (t if t.numel() == shape.numel() else t.reshape(-1, t.shape[-1]).sum(0)).reshape(shape)
-            for t, shape in zip(sums, ctx.shapes))
+        dscale, dshift, dgate = (t if t is None else t.view(shape) for t, shape in zip(sums, ctx.shapes))
         return dx if nx else None, dy if ny else None, dgate, dw, dscale, dshift, None, None, None
 
 

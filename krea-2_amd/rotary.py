@@ -154,7 +154,9 @@ class RotaryEmbedding(nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, heads_first: bool = False):
         """``(q', k')``, with the strides of ``q`` and ``k``.  ``q`` (B, L, H, D), or with ``heads_first`` (B, H, L, D), or
         either without the batch; ``k`` the same with its own number of heads, or None.  ``positions``: int64, int32,
-        float32 or float64, (L,) or (B, L), with ``axes`` a last dimension of one value per axis."""
+        float32 or float64, (L,) or (B, L), with ``axes`` a last dimension of one value per axis; they get no gradient."""
+        if positions.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("positions get no gradient: detach them")
         grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _lib.observed()
         table = self._tables.get(q.device)
         if table is not None and not grad:      # the call as it is, where the kernel takes it

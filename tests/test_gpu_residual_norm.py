@@ -258,6 +258,60 @@ def test_an_entry_per_row(k2, dev):
     assert torch.equal(k2.residual_rmsnorm(norm, one, one)[0], one + one)
 
 
+@pytest.mark.parametrize("one", [(0,), (1,), (2,), (0, 1, 2)])
+def test_vectors_that_every_entry_shares(k2, dev, one):
+    """One gate, scale or shift beside others with an entry per batch row: the sum over every row, rounded once (2^-8 of
+    it; float32 sums of 640 terms in a row and 231 in a column, (640 + 231) 2^-24 < 2^-14 of the products' magnitudes), and
+    the same bits from a captured backward, also of r alone."""
+    norm, x, y, mods = _inputs((3, 77, 640), dev, 3, seed=2)
+    leaves = [t.detach().clone()[:1 if i in one else 3].requires_grad_() for i, t in enumerate(mods)]
+    leaves = [x.detach().clone().requires_grad_(), y.detach().clone().requires_grad_(), *leaves]
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+    got = _grads(k2.residual_rmsnorm(norm, *leaves), leaves, dr, dh)
+    l64 = [t.detach().double().requires_grad_() for t in leaves]
+    r64 = l64[0] + l64[2] * l64[1]
+    r64 = r64 + ((x + leaves[2].detach() * y).double() - r64).detach()              # the bf16 r, the gradient passed through
+    n64 = r64 * torch.rsqrt(r64.square().mean(-1, keepdim=True) + EPS) * (norm.scale.double() + 1)
+    nb = n64.float().bfloat16().double()
+    p64 = (1 + leaves[3].detach()).double() + (l64[3] - l64[3].detach())
+    h64 = n64 * p64 + l64[4] + (nb - n64).detach() * (l64[3] - l64[3].detach())
+    ref = _grads((r64, h64), l64, dr.double(), dh.double())
+    r = r64.detach()
+    inv = torch.rsqrt(r.square().mean(-1, keepdim=True) + EPS)
+    g = (dh.double() * p64.detach() * (norm.scale.double() + 1)).abs()
+    dR = dr.double().abs() + g * inv + r.abs() * inv ** 3 * (g * r.abs()).mean(-1, keepdim=True)
+    mags = dR * y.double().abs(), dh.double().abs() * nb.detach().abs(), dh.double().abs()
+    for i in range(3):
+        a, e, over = got[2 + i], ref[2 + i], (0, 1) if i in one else 1
+        bound = 2 ** -8 * e.abs() + 2 ** -13 * mags[i].sum(over, keepdim=True)
+        if i == 1:      # an n at a tie rounds to either side: two products of a column a step (2^-7) off
+            bound += 2 * 2 ** -7 * mags[i].amax(over, keepdim=True)
+        assert a.shape == e.shape and ((a.double() - e).abs() <= bound).all(), i
+    static = [t.detach().clone().requires_grad_() for t in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _grads(k2.residual_rmsnorm(norm, *static), static, dr, dh)
+    torch.cuda.current_stream().wait_stream(side)
+    graph, alone = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap = _grads(k2.residual_rmsnorm(norm, *static), static, dr, dh)
+    with torch.cuda.graph(alone):                                                   # the stream's gradient without h's
+        stream = torch.autograd.grad(k2.residual_rmsnorm(norm, *static)[0], static[:3], dr)
+    ref = (dr.double() * y.double()).sum((0, 1) if 0 in one else 1, keepdim=True)
+    mag = (dr.double() * y.double()).abs().sum((0, 1) if 0 in one else 1, keepdim=True)
+    for _ in range(3):
+        for t in (*cap, *stream[1:]):       # stream[0] is dr itself
+            t.zero_()
+        graph.replay()
+        alone.replay()
+        again = _grads(k2.residual_rmsnorm(norm, *leaves), leaves, dr, dh)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) and torch.equal(c, e) for a, c, e in zip(again, cap, got))
+        assert torch.equal(stream[0], dr) and stream[2].shape == static[2].shape
+        assert ((stream[2].double() - ref).abs() <= 2 ** -8 * ref.abs() + 2 ** -15 * mag).all()
+
+
 def test_unused_and_broadcast_outputs(k2, dev):
     """Only r, only h, or neither used; a gate of one entry beside a modulation per batch row; a bf16 norm scale."""
     norm, x, y, (gate, p, b) = _inputs((3, 4, 256), dev, 3)
@@ -312,13 +366,13 @@ def test_captured_and_other_stream(k2, dev):
         r, h = k2.residual_rmsnorm(norm, xs, ys, gate, p, b)
         flat = [t.reshape(-1, 1024) for t in (dh, dr, r, ys)]
         ent = [t.reshape(2, 1024) for t in (p, gate)]
-        grads = k2._lib.resnorm_bwd(flat[0], flat[1], flat[2], w, 1.0, EPS, ent[0], ent[1], 50, flat[3], True, True, True)
+        grads = k2._lib.resnorm_bwd(flat[0], flat[1], flat[2], w, 1.0, EPS, ent[0], ent[1], 50, flat[3], True, True, True, 2)
     for i in range(3):
         xs.copy_(x * (i + 1))
         graph.replay()
         er, eh = k2.residual_rmsnorm(norm, x * (i + 1), y, gate, p, b)
         ref = k2._lib.resnorm_bwd(flat[0], flat[1], er.reshape(-1, 1024), w, 1.0, EPS, ent[0], ent[1], 50, flat[3], True,
-                                  True, True)
+                                  True, True, 2)
         torch.cuda.synchronize()
         assert torch.equal(r, er) and torch.equal(h, eh), i
         assert all(torch.equal(a, e) for a, e in zip(grads, ref)), i
@@ -368,7 +422,8 @@ def test_refusals(k2, dev):
                 lambda: k2.residual_rmsnorm(nn.LayerNorm(256, device=dev), x, y),
                 lambda: k2.residual_rmsnorm(nn.RMSNorm(256, device=dev), x, y),
                 lambda: k2._lib.resnorm_rotquant(x[0], y[0], None, norm.scale, 1.0, EPS, None, None, 3),
-                lambda: k2._lib.resnorm_bwd(x[0], None, x[0], norm.scale, 1.0, EPS, None, None, 4, y[0])):
+                lambda: k2._lib.resnorm_bwd(x[0], None, x[0], norm.scale, 1.0, EPS, None, None, 4, y[0]),
+                lambda: k2._lib.resnorm_bwd(x[0], None, x[0], norm.scale, 1.0, EPS, p[0], None, 1, None, False, True, True, 3)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(NotImplementedError):

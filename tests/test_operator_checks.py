@@ -49,12 +49,13 @@ def test_entry_points_refuse_bad_arguments(k2):
         assert norm(**bad) == -1, bad
     assert norm(K=16512, ldx=16512) == -4 and norm(M=1 << 31) == -4
 
-    def bwd(dh=p, r=p, M=4, K=256, ms=p, gate=p, rows=2, dx=p, dy=p, y=p, dw=p, ds=p, dg=p, ws=p, nws=1 << 30):
+    def bwd(dh=p, r=p, M=4, K=256, ms=p, gate=p, rows=2, dx=p, dy=p, y=p, dw=p, ds=p, dg=p, ws=p, nws=1 << 30,
+            shared=0):
         return lib.k2q_resnorm_bwd(dh, None, r, M, K, p, 1.0, 1e-5, ms, 0, gate, 0, rows, 0, dx, dy, y, 256, dw, ds, None, dg,
-                                   ws, nws, None)
+                                   shared, ws, nws, None)
 
     for bad in ({"dh": None}, {"r": odd}, {"M": 0}, {"K": 100}, {"ms": None}, {"gate": None}, {"dy": None}, {"rows": 3},
-                {"rows": 0}, {"dx": None}, {"y": None}, {"ws": None}, {"nws": 16}):
+                {"rows": 0}, {"dx": None}, {"y": None}, {"ws": None}, {"nws": 16}, {"shared": 8}, {"shared": -1}):
         assert bwd(**bad) == -1, bad
     assert bwd(M=1 << 31) == -4 and bwd(M=1 << 30, rows=1, nws=1 << 62) == -4
 
@@ -91,6 +92,8 @@ def test_rotary_module_refuses(k2):
         rope(q, None, torch.arange(5))
     with pytest.raises(ValueError):
         rope(q[..., :32], None, torch.arange(5))
+    with pytest.raises(NotImplementedError):                    # a gradient that it would not give
+        rope(q, None, torch.zeros(5, requires_grad=True))
     assert rope(q[:, :0], None, torch.arange(0))[0].shape == (1, 0, 2, 64)
     assert not list(rope.parameters()) and not rope.state_dict()
 
