@@ -214,35 +214,39 @@ __device__ __forceinline__ void wave_sums(float (&v)[NV], float (&out)[NV / 4]) 
   }
 }
 
-// The same product on the matrix cores: a workgroup owns 16 rows, its waves split K into 1024-wide segments (512 bytes
-// of a row, 16 scale groups).  One 16 x 16 x 64 MFMA is 16 weight rows against up to 16 token rows over one scale group:
+// The same product on the matrix cores: a workgroup owns 16 or 32 rows, its waves split K into 1024-wide segments (512
+// bytes of a row, 16 scale groups).  One 16 x 16 x 64 MFMA is 16 weight rows against up to 16 token rows over a scale group:
 // lane (c = lane % 16, b = lane / 16) holds the 8 bytes of row c and the 16 codes of token c at k = 64 g + 16 b, and gets
 // the dots of row c with the token operand's rows 4 b .. 4 b + 3.  Loaded in that layout a row's bytes come 32 at a time
 // (2.9 TB/s); so a wave loads whole row segments, 16 bytes a lane, and turns them through its own piece of LDS: row c,
 // 16-byte unit q at unit q ^ 2 (c % 8), which spreads the eight rows of a read over all banks.  With at most 8 tokens half
 // of a token operand would be idle: its rows 8-15 hold the same tokens' codes of the next group, so one register serves two
-// MFMAs, whose results for tokens 0-7 are rows 0-7 (even groups) and rows 8-15 (odd groups).
+// MFMAs, whose results for tokens 0-7 are rows 0-7 (even groups) and rows 8-15 (odd groups): eight tokens over 36864 x 6144
+// in 29.7 us, 36.8 with a register each (112 of them instead of 78).
 constexpr int GM_ROWS = 16;
 constexpr int GM_SEG = 1024;
 constexpr int GM_GROUPS = GM_SEG / 64;
-constexpr int GM_WAVES = 8;
+constexpr int GM_WAVES = 8;         // K <= 16 segments: two a wave, or 16 waves
 constexpr int GM_LDS = GM_ROWS * GM_SEG / 2 + GM_GROUPS * GM_ROWS * 2;   // a wave's piece: codes, then scales
 
-template <int STEPS>
-__global__ __launch_bounds__(64 * GM_WAVES) void gemv_w4_mfma_kernel(Gemv4Args p, int M) {
+// A workgroup has RT tiles of 16 rows and up to 8 RT waves; a wave takes STEPS segments, its tiles in turn through its LDS.
+template <int STEPS, int RT>
+__global__ __launch_bounds__(64 * GM_WAVES * RT) void gemv_w4_mfma_kernel(Gemv4Args p, int M) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, b = lane >> 4;
-  const int64_t n0 = xcd_block() * GM_ROWS;
+  const int64_t n0 = xcd_block() * (GM_ROWS * RT);
   const int kb = p.K >> 1;
   // loads: lane's row 2 i + lane / 32 (clamped to the last), its 16 bytes at 16 (lane % 32) of the segment; its scales'
   // group lane / 4 and four rows
-  const int64_t s0 = n0 + 4 * (lane & 3) < p.N ? n0 + 4 * (lane & 3) : p.N - 4;
+  int64_t s0[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) s0[t] = n0 + 16 * t + 4 * (lane & 3) < p.N ? n0 + 16 * t + 4 * (lane & 3) : p.N - 4;
   const int tok = c & 7;
   const int8_t* xp = p.qx + (int64_t)(tok < M ? tok : 0) * p.K + 64 * (c >> 3) + 16 * b;
-  v4u w[STEPS][GM_ROWS / 2];
-  v2u sc[STEPS];
+  v4u w[STEPS][RT][GM_ROWS / 2];
+  v2u sc[STEPS][RT];
   v4i x[GM_GROUPS / 2];
   auto load_x = [&](int k0) {      // K % 128 == 0: groups come in pairs
 #pragma unroll
@@ -255,16 +259,19 @@ __global__ __launch_bounds__(64 * GM_WAVES) void gemv_w4_mfma_kernel(Gemv4Args p
     if (k0 >= p.K) break;
     const int k = k0 + 32 * (lane & 31), g = (k0 >> 6) + (lane >> 2);
 #pragma unroll
-    for (int i = 0; i < GM_ROWS / 2; ++i) {
-      const int64_t row = n0 + 2 * i + (lane >> 5) < p.N ? n0 + 2 * i + (lane >> 5) : p.N - 1;
-      w[s][i] = v4u{0, 0, 0, 0};
-      if (k < p.K) w[s][i] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p.qw + row * kb + (k >> 1)));
+    for (int t = 0; t < RT; ++t) {
+#pragma unroll
+      for (int i = 0; i < GM_ROWS / 2; ++i) {
+        const int64_t at = n0 + 16 * t + 2 * i + (lane >> 5), row = at < p.N ? at : p.N - 1;
+        w[s][t][i] = v4u{0, 0, 0, 0};
+        if (k < p.K) w[s][t][i] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p.qw + row * kb + (k >> 1)));
+      }
+      sc[s][t] = v2u{0, 0};
+      if (64 * g < p.K) sc[s][t] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)g * p.N + s0[t]);
     }
-    sc[s] = v2u{0, 0};
-    if (64 * g < p.K) sc[s] = *reinterpret_cast<const v2u*>(p.s4 + (int64_t)g * p.N + s0);
     if (s == 0) load_x(k0);
   }
-  float acc[4] = {};
+  float acc[RT][4] = {};
   uint8_t* wt = lds + GM_LDS * wave;
   uint16_t* st = reinterpret_cast<uint16_t*>(wt + GM_ROWS * GM_SEG / 2);
   const int sw = 2 * (c & 7);
@@ -273,40 +280,47 @@ __global__ __launch_bounds__(64 * GM_WAVES) void gemv_w4_mfma_kernel(Gemv4Args p
     const int k0 = GM_SEG * (wave + s * p.waves);
     if (k0 >= p.K) break;
     if (s) load_x(k0);
-    wave_fence();
 #pragma unroll
-    for (int i = 0; i < GM_ROWS / 2; ++i) {
-      const int r = 2 * i + (lane >> 5);
-      *reinterpret_cast<v4u*>(wt + r * (GM_SEG / 2) + 16 * ((lane & 31) ^ (2 * (r & 7)))) = w[s][i];
-    }
-    *reinterpret_cast<v2u*>(st + 4 * lane) = sc[s];
-    wave_fence();
-    // groups past K: codes and scales are zeros
+    for (int t = 0; t < RT; ++t) {
+      wave_fence();
 #pragma unroll
-    for (int g = 0; g < GM_GROUPS; g += 2) {
-      v4i d[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const v2u q = *reinterpret_cast<const v2u*>(wt + c * (GM_SEG / 2) + 16 * ((2 * (g + h) + (b >> 1)) ^ sw) + 8 * (b & 1));
-        const v4i a = {(int)((q[0] << 4) & 0xf0f0f0f0u), (int)((q[1] << 4) & 0xf0f0f0f0u), (int)(q[0] & 0xf0f0f0f0u),
-                       (int)(q[1] & 0xf0f0f0f0u)};
-        d[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[g / 2], a, v4i{0, 0, 0, 0}, 0, 0, 0);
+      for (int i = 0; i < GM_ROWS / 2; ++i) {
+        const int r = 2 * i + (lane >> 5);
+        *reinterpret_cast<v4u*>(wt + r * (GM_SEG / 2) + 16 * ((lane & 31) ^ (2 * (r & 7)))) = w[s][t][i];
       }
-      const float f = bf16_bits_to_f32(st[GM_ROWS * (g + (b >> 1)) + c]);
+      *reinterpret_cast<v2u*>(st + 4 * lane) = sc[s][t];
+      wave_fence();
+      // groups past K: codes and scales are zeros
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf((float)(b < 2 ? d[0][i] : d[1][i]), f, acc[i]);
+      for (int g = 0; g < GM_GROUPS; g += 2) {
+        v4i d[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int unit = (2 * (g + h) + (b >> 1)) ^ sw;
+          const v2u q = *reinterpret_cast<const v2u*>(wt + c * (GM_SEG / 2) + 16 * unit + 8 * (b & 1));
+          const v4i a = {(int)((q[0] << 4) & 0xf0f0f0f0u), (int)((q[1] << 4) & 0xf0f0f0f0u), (int)(q[0] & 0xf0f0f0f0u),
+                         (int)(q[1] & 0xf0f0f0f0u)};
+          d[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[g / 2], a, v4i{0, 0, 0, 0}, 0, 0, 0);
+        }
+        const float f = bf16_bits_to_f32(st[GM_ROWS * (g + (b >> 1)) + c]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf((float)(b < 2 ? d[0][i] : d[1][i]), f, acc[t][i]);
+      }
     }
   }
   wave_fence();
-  float* red = reinterpret_cast<float*>(wt);      // 8 tokens x 16 rows, over the wave's own codes
+  float* red = reinterpret_cast<float*>(wt);      // 8 tokens x the rows, over the wave's own codes
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], 32, 64);      // even groups' sum plus odd groups'
-  if (b < 2)
+  for (int t = 0; t < RT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[GM_ROWS * (4 * b + i) + c] = acc[i];
+    for (int i = 0; i < 4; ++i) acc[t][i] += __shfl_xor(acc[t][i], 32, 64);      // even groups' sum plus odd groups'
+    if (b < 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[GM_ROWS * RT * (4 * b + i) + 16 * t + c] = acc[t][i];
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < GM_ROWS * M; i += 64 * p.waves) {
-    const int m = i / GM_ROWS, r = i % GM_ROWS;
+  for (int i = threadIdx.x; i < GM_ROWS * RT * M; i += 64 * p.waves) {
+    const int m = i / (GM_ROWS * RT), r = i % (GM_ROWS * RT);
     const int64_t n = n0 + r;
     if (n >= p.N) continue;
     float a = 0.f;
@@ -315,21 +329,33 @@ __global__ __launch_bounds__(64 * GM_WAVES) void gemv_w4_mfma_kernel(Gemv4Args p
   }
 }
 
-template <int STEPS>
+template <int STEPS, int RT>
 int launch4_mfma(const Gemv4Args& p, int M, hipStream_t st) {
   static std::atomic<uint64_t> lds_set{0};
-  const int rc = k2q_lds_limit_once(gemv_w4_mfma_kernel<STEPS>, GM_LDS * GM_WAVES, lds_set);
+  const int rc = k2q_lds_limit_once(gemv_w4_mfma_kernel<STEPS, RT>, GM_LDS * GM_WAVES * RT, lds_set);
   if (rc) return rc;
-  const int64_t grid = (p.N + GM_ROWS - 1) / GM_ROWS;
+  const int64_t grid = (p.N + GM_ROWS * RT - 1) / (GM_ROWS * RT);
   if (grid > 0x7fffffff) return K2Q_EUNSUPPORTED;
-  hipLaunchKernelGGL(gemv_w4_mfma_kernel<STEPS>, dim3((unsigned)grid), dim3(64 * p.waves), GM_LDS * p.waves, st, p, M);
+  hipLaunchKernelGGL((gemv_w4_mfma_kernel<STEPS, RT>), dim3((unsigned)grid), dim3(64 * p.waves), GM_LDS * p.waves, st, p, M);
   return k2q_launch_status();
 }
 
+// 16 rows a workgroup, or 32 and a wave a segment where that is one workgroup a CU or less and 16 rows would be more than
+// one: the CUs with two then end last, and every workgroup reads all tokens' codes.  It takes a CU's LDS and registers
+// for itself, so it loses in more than one round and, with few segments, where it has little more in flight.  us, 16 rows /
+// 32 rows, M = 3, then M = 8:
+//   4096 x 16384   10.3 / 12.3   11.3 / 13.7       6144 x 12288   11.8 / 11.5   14.0 / 12.5
+//   4352 x 16384   13.8 / 12.3   16.9 / 13.8      12288 x 12288   18.4 / 23.2   20.4 / 23.4
+//   6144 x 16384   14.4 / 13.7   17.4 / 15.0       4352 x 9344     9.8 / 10.0   11.5 / 10.7
+//   8192 x 16384   15.7 / 15.7   18.5 / 16.6       8192 x 8320    10.2 / 10.8   11.3 / 11.5
 int launch4_mfma(Gemv4Args p, int M, hipStream_t st) {
-  const int segs = (p.K + GM_SEG - 1) / GM_SEG;
+  const int segs = (p.K + GM_SEG - 1) / GM_SEG, cus = k2q_cu_count();
+  if (segs > GM_WAVES + 1 && p.N > GM_ROWS * cus && p.N <= 2 * GM_ROWS * cus) {
+    p.waves = segs;
+    return launch4_mfma<1, 2>(p, M, st);
+  }
   p.waves = segs < GM_WAVES ? segs : GM_WAVES;
-  return segs <= GM_WAVES ? launch4_mfma<1>(p, M, st) : launch4_mfma<2>(p, M, st);
+  return segs <= GM_WAVES ? launch4_mfma<1, 1>(p, M, st) : launch4_mfma<2, 1>(p, M, st);
 }
 
 constexpr int G4_K = 2048;
@@ -467,7 +493,7 @@ int launch4_mr(Gemv4Args p, hipStream_t st) {
 //   1536 x 6144    3.6 / 3.7 / 5.3      4.0 / 4.1 / 5.5      4.3 / 4.4 / 5.5      5.4 / 5.4 / 5.8
 //   6144 x 6144    6.2 / 6.2 / 7.5      6.9 / 7.4 / 7.6      7.6 / 7.6 / 7.8      11.2 / 11.1 / 8.7
 //   36864 x 6144   24.3 / 22.4 / 25.6   26.9 / 25.3 / 25.1   29.9 / 25.4 / 25.7   47.5 / 43.4 / 29.7
-//   6144 x 16384   13.6 / 12.3 / 14.0   15.1 / 13.3 / 14.2   16.5 / 14.6 / 14.4   24.8 / 20.8 / 17.4
+//   6144 x 16384   13.6 / 12.3 / 14.0   15.1 / 13.3 / 14.2   16.5 / 14.6 / 13.7   24.8 / 20.8 / 15.0
 constexpr int64_t G4_WIDE = 4096;
 
 template <int MT>

@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 
 EDGES = [(1, 4, 128), (1, 1536, 6144), (2, 132, 2048), (3, 36, 2176), (4, 260, 4096), (5, 512, 640), (6, 1028, 8192),
          (7, 6144, 16384), (8, 18432, 1024), (8, 64, 16384), (2, 36864, 6144), (1, 2000, 256), (1, 4100, 2048),
-         (2, 4108, 16384), (3, 4100, 128), (8, 4124, 8320), (5, 6148, 1152), (3, 4096, 8192), (1, 8196, 10240)]
+         (2, 4108, 16384), (3, 4100, 128), (8, 4124, 8320), (5, 6148, 1152), (3, 4096, 8192), (1, 8196, 10240),
+         (3, 4100, 9344), (8, 8192, 16384), (5, 6148, 12288), (6, 8196, 10240), (4, 4104, 9216)]
 
 
 def _codes(q4):
