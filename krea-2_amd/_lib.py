@@ -508,18 +508,18 @@ def _check_resnorm_bwd(dh, dr, r, w, ms, gate, rows_per_entry, y, need_mod, shif
         _need_rows(y if y.dim() == 2 else y.reshape(flat.shape), "y", r.device)
     if need_mod and ms is None:
         raise ValueError("no modulation to differentiate")
-    if shift_entries not in (1, flat.shape[0] // rows_per_entry):
+    if shift_entries not in (None, 1, flat.shape[0] // rows_per_entry):
         raise ValueError(f"shift_entries={shift_entries}, expected 1 or {flat.shape[0] // rows_per_entry}")
     _device_check(r.device)
 
 
 def resnorm_bwd(dh, dr, r, w, add: float, eps: float, scale, gate, rows_per_entry: int, y=None, need_w=False,
-                need_scale=False, need_shift=False, shift_entries: int = 1, eager=False):
+                need_scale=False, need_shift=False, shift_entries: int | None = None, eager=False):
     """Autograd of :func:`resnorm_rotquant` and :func:`resnorm_native` (``k2q_resnorm_bwd``): ``(dx, dy, dw, dscale, dshift,
     dgate)`` from the gradients of ``h`` and (or None) of ``r``, contiguous in r's shape.  ``dy`` is None without a gate
     (it is ``dx``); ``dgate`` comes when ``y`` is given, the other sums where asked for: in the shape of ``gate`` /
-    ``scale`` (one entry among more: the sum over every row), ``dshift`` (shift_entries, K).  ``eager``: rounded where eager
-    bf16 operations round."""
+    ``scale`` (one entry among more: the sum over every row), ``dshift`` as ``scale`` or (shift_entries, K).  ``eager``:
+    rounded where eager bf16 operations round."""
     args = (dh, dr, r, w, add, eps, scale, gate, rows_per_entry, y, need_w, need_scale, need_shift, shift_entries, eager)
     out = _fast().resnorm_bwd(*args)
     if out.__class__ is tuple:

@@ -539,8 +539,9 @@ PyObject* py_resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // resnorm_bwd(dh, dr | None, r, w, add, eps, scale | None, gate | None, rows_per_entry, y | None, need_w, need_scale,
-//             need_shift, shift_entries, eager) -> (dx, dy | None, dw | None, dscale | None, dshift | None, dgate | None): dh,
-// dr, r contiguous (.., K); dx, dy in their shape, dscale and dgate in scale's and gate's, dshift (shift_entries, K)
+//             need_shift, shift_entries | None, eager) -> (dx, dy | None, dw | None, dscale | None, dshift | None,
+// dgate | None): dh, dr, r contiguous (.., K); dx, dy in their shape, dscale and dgate in scale's and gate's, dshift in
+// scale's or (shift_entries, K)
 PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(15)
   return guarded([&]() -> PyObject* {
@@ -551,7 +552,8 @@ PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t rows = PyLong_AsLongLong(a[8]);
     const int need_w = PyObject_IsTrue(a[10]), need_scale = PyObject_IsTrue(a[11]), need_shift = PyObject_IsTrue(a[12]),
               eager = PyObject_IsTrue(a[14]);
-    const int64_t nb = PyLong_AsLongLong(a[13]);
+    const bool as_scale = a[13] == Py_None;
+    int64_t nb = as_scale ? 1 : PyLong_AsLongLong(a[13]);
     if (PyErr_Occurred()) return nullptr;
     if (bad || !dh || !r || r->dim() < 2 || rows < 1) K2Q_REFUSE;
     const int64_t K = r->size(r->dim() - 1);
@@ -566,15 +568,17 @@ PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t ng, ns, lg, ls;
     if (!ready(d) || !whole(dh) || !whole(r) || (dr && !whole(dr)) ||
         !operand(w, at::kFloat, 1, d) || w->size(0) != K || !vectors_ok(gate, K, d, ng, lg) ||
-        !vectors_ok(ms, K, d, ns, ls) || !entries_fit({ng, ns, nb}, M, 0, rows) || (y && (!gate || !in(y))) ||
+        !vectors_ok(ms, K, d, ns, ls) || nb < 1 || !entries_fit({ng, ns, nb}, M, 0, rows) || (y && (!gate || !in(y))) ||
         ((need_scale || need_shift) && !ms))
       K2Q_REFUSE;
+    if (as_scale) nb = ns;
     const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     Tensor dx = alloc(r->sizes(), at::kBFloat16, d), dy = gate ? alloc(r->sizes(), at::kBFloat16, d) : Tensor();
-    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = need_scale ? alloc(ms->sizes(), at::kBFloat16, d) : Tensor(),
-           db = need_shift ? alloc({nb, K}, at::kBFloat16, d) : Tensor(), dg = y ? alloc(gate->sizes(), at::kBFloat16, d) : Tensor();
+    auto like = [&](bool need, const Tensor* t) { return need ? alloc(t->sizes(), at::kBFloat16, d) : Tensor(); };
+    Tensor dw = need_w ? alloc({K}, at::kFloat, d) : Tensor(), ds = like(need_scale, ms), dg = like(y, gate),
+           db = need_shift && !as_scale ? alloc({nb, K}, at::kBFloat16, d) : like(need_shift, ms);
     const int shared = (ns == 1 ? K2Q_SHARED_SCALE : 0) | (nb == 1 ? K2Q_SHARED_SHIFT : 0) | (ng == 1 ? K2Q_SHARED_GATE : 0);
     const int64_t nws = need_w || need_scale || need_shift || y ? api.resnorm_bwd_ws_bytes(M, K, rows) : 0;
     Tensor ws = workspace(nws, d);

@@ -142,6 +142,7 @@ class _ResNormQuantFn(torch.autograd.Function):
     def forward(ctx, x, y, gate, w, scale, shift, add, eps, eager):
         shape, ctx.shapes = x.shape, [None if t is None else t.shape for t in (scale, shift, gate)]
         out = _lib.resnorm_native(x, y, gate, w, add, eps, scale, shift)
+        ctx.whole = out is not None         # the tensors kept are the caller's, in their shapes
         if out is None:
             x, y, gate, scale, shift, rows = _residual_rows(x, y, gate, w, scale, shift)
             out = _lib.resnorm_rotquant(x, y, gate, w, add, eps, scale, shift, rows)
@@ -166,14 +167,16 @@ class _ResNormQuantFn(torch.autograd.Function):
         dh, dr = _dense_grad(dh, r), None if dr is None else _dense_grad(dr, r)
         if r.shape != shape:        # the forward ran on rows
             dh, dr = dh.view(r.shape), None if dr is None else dr.view(r.shape)
-        entries = 1 if scale is None else ctx.shapes[1].numel() // r.shape[-1]
-        dx, dy, dw, *sums = _lib.resnorm_bwd(dh, dr, r, w, ctx.add, ctx.eps, scale, gate, ctx.rows, y, nw, ns, nb, entries,
-                                             ctx.eager)
-        if r.shape != shape:
+        same = ctx.shapes[0] == ctx.shapes[1]
+        dx, dy, dw, dscale, dshift, dgate = _lib.resnorm_bwd(
+            dh, dr, r, w, ctx.add, ctx.eps, scale, gate, ctx.rows, y, nw, ns, nb,
+            None if same else ctx.shapes[1].numel() // r.shape[-1], ctx.eager)
+        if not (ctx.whole and same):
             dx, dy = dx.view(shape), None if dy is None else dy.view(shape)
+            dscale, dshift, dgate = (t if t is None else t.view(shape)
+                                     for t, shape in zip((dscale, dshift, dgate), ctx.shapes))
         if gate is None:
             dy = dx
-        dscale, dshift, dgate = (t if t is None else t.view(shape) for t, shape in zip(sums, ctx.shapes))
         return dx if nx else None, dy if ny else None, dgate, dw, dscale, dshift, None, None, None
 
 

@@ -366,13 +366,13 @@ def test_captured_and_other_stream(k2, dev):
         r, h = k2.residual_rmsnorm(norm, xs, ys, gate, p, b)
         flat = [t.reshape(-1, 1024) for t in (dh, dr, r, ys)]
         ent = [t.reshape(2, 1024) for t in (p, gate)]
-        grads = k2._lib.resnorm_bwd(flat[0], flat[1], flat[2], w, 1.0, EPS, ent[0], ent[1], 50, flat[3], True, True, True, 2)
+        grads = k2._lib.resnorm_bwd(flat[0], flat[1], flat[2], w, 1.0, EPS, ent[0], ent[1], 50, flat[3], True, True, True)
     for i in range(3):
         xs.copy_(x * (i + 1))
         graph.replay()
         er, eh = k2.residual_rmsnorm(norm, x * (i + 1), y, gate, p, b)
         ref = k2._lib.resnorm_bwd(flat[0], flat[1], er.reshape(-1, 1024), w, 1.0, EPS, ent[0], ent[1], 50, flat[3], True,
-                                  True, True, 2)
+                                  True, True)
         torch.cuda.synchronize()
         assert torch.equal(r, er) and torch.equal(h, eh), i
         assert all(torch.equal(a, e) for a, e in zip(grads, ref)), i
