@@ -184,10 +184,13 @@ def _norm_scale_f32(norm: nn.Module, name: str = "scale") -> torch.Tensor:
     """The norm's (frozen) scale (or ``weight``) as the kernels take it, f32 and contiguous, kept on the module and rebuilt
     when it changes (in place: version; re-pointed, e.g. paged by block swap: pointer or device)."""
     t = getattr(norm, name)
+    if t.is_inference():
+        return t.float().contiguous()
     key = (t._version, t.data_ptr(), t.device, t.dtype, tuple(t.shape))
     kept = norm.__dict__.get("_k2q_scale_f32")
     if kept is None or kept[0] != key:
-        kept = (key, t.detach().float().contiguous())
+        with torch.inference_mode(False), torch.no_grad():      # a training pass may save what this call keeps
+            kept = (key, t.detach().float().contiguous())
         norm.__dict__["_k2q_scale_f32"] = kept
     return kept[1]
 
@@ -525,6 +528,8 @@ class _SiblingGroup:
         return (x._version, x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.device, _lib._stream(x.device))
 
     def call(self, idx: int, x: torch.Tensor):
+        if x.is_inference():        # no version counter to know it by
+            return None
         key = self._key(x)
         if self.ref is not None and self.ref() is x and self.key == key and idx in self.kept:
             out, sk = self.kept.pop(idx)

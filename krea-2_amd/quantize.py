@@ -33,7 +33,8 @@ class _SharedInputQuant:
 
     A hit needs the same tensor object (held by weak reference, so a freed tensor never matches), the same
     version counter (any in-place write bumps it), data pointer, shape, strides and CUDA stream.  The
-    codes are a pure function of the input, so a hit returns exactly what a fresh call would."""
+    codes are a pure function of the input, so a hit returns exactly what a fresh call would.  Tensors of
+    ``torch.inference_mode`` have no version counter: nothing is kept for them (key None)."""
 
     enabled = True
 
@@ -45,30 +46,32 @@ class _SharedInputQuant:
 
     @staticmethod
     def _key(x: torch.Tensor):
+        if x.is_inference():
+            return None
         dev = x.device
         return (x._version, x.data_ptr(), x.shape, x.stride(), dev, _lib._stream(dev))
 
     def lookup(self, x: torch.Tensor, x2: torch.Tensor):
         key = self._key(x)
-        if self.enabled and self.ref is not None and self.ref() is x and self.key == key:
+        if key is not None and self.enabled and self.ref is not None and self.ref() is x and self.key == key:
             return self.val
         self.misses += 1
         qx, sx, _ = _lib.rotquant(x2)
-        if self.enabled:
+        if self.enabled and key is not None:
             self.ref, self.key, self.val = weakref.ref(x), key, (qx, sx)
         return qx, sx
 
     def find(self, x: torch.Tensor):
         """``(key, codes)``: the codes kept for exactly this tensor, or None; the key goes back to :meth:`keep`."""
         key = self._key(x)
-        if self.enabled and self.ref is not None and self.ref() is x and self.key == key:
+        if key is not None and self.enabled and self.ref is not None and self.ref() is x and self.key == key:
             return key, self.val
         self.misses += 1
         return key, None
 
     def keep(self, x: torch.Tensor, key, qx: torch.Tensor, sx: torch.Tensor) -> None:
         """Record the codes a fused forward wrote for ``x`` (``key`` from :meth:`find`, taken before that call)."""
-        if self.enabled:
+        if self.enabled and key is not None:
             self.ref, self.key, self.val = weakref.ref(x), key, (qx, sx)
 
     def clear(self) -> None:
@@ -78,8 +81,9 @@ class _SharedInputQuant:
     def seed(self, x: torch.Tensor, qx: torch.Tensor, sx: torch.Tensor) -> None:
         """Record codes a producer-fused kernel computed for ``x`` (exactly those ``rotquant`` gives), so the
         ConvRot layers that receive ``x`` next skip their own rotate/quant."""
-        if self.enabled:
-            self.ref, self.key, self.val = weakref.ref(x), self._key(x), (qx, sx)
+        key = self._key(x) if self.enabled else None
+        if key is not None:
+            self.ref, self.key, self.val = weakref.ref(x), key, (qx, sx)
 
 
 shared_input_quant = _SharedInputQuant()

@@ -137,3 +137,28 @@ def test_training_step(k2, dev, mode):
     bars = [1e-2, 1e-2] + [2e-2] * len(params)
     for a, e, bar in zip(fused, eager, bars):
         assert (a.double() - e.double()).norm() <= bar * e.double().norm()
+
+
+@pytest.mark.parametrize("mode", ["w8a8", "w4a8"])
+def test_inference_mode_then_training(k2, dev, mode):
+    """``torch.inference_mode`` tensors carry no version, so no codes are kept for them: the linears make their own, and a
+    later training step finds nothing that autograd cannot save (norm scales in bf16 are held in float32)."""
+    m, ad = _model(k2, dev, mode)
+    for b in m.blocks:
+        b.norm1.bfloat16(), b.norm2.bfloat16()
+        b.norm1.requires_grad_(False), b.norm2.requires_grad_(False)
+    x = torch.randn(1, 24, FEAT, device=dev).bfloat16()
+    pos = torch.arange(24, device=dev)
+    with torch.inference_mode():
+        served, caches = _run(k2, m, x, pos)
+        token, _ = _run(k2, m, x[:, -1:].clone(), pos[-1:], [(c[0][:, :-1], c[1][:, :-1]) for c in caches])
+        h = k2.residual_rmsnorm(m.blocks[0].norm1, x, x)[1]
+        q, s = k2.input_codes(h)
+        h.mul_(2)                                                   # a write that no counter shows
+        assert torch.equal(k2.input_codes(h)[1], 2 * s) and torch.equal(k2.input_codes(h)[0], q)
+    t = x.clone().requires_grad_()
+    y, _ = _run(k2, m, t, pos)
+    g = torch.autograd.grad(y, [t, *k2.lora_parameters(ad)], torch.randn_like(y))
+    assert all(v.isfinite().all() for v in g)
+    for a, e in ((served, y), (token, y[:, -1:])):
+        assert (a.double() - e.double()).norm() <= 1e-2 * e.double().norm()

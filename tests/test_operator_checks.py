@@ -116,3 +116,15 @@ def test_rotary_frequencies(k2):
         else:
             assert v / 4 <= g[i] * (1 + 1e-12) and g[i] <= v * (1 + 1e-12)
     assert R(64, scaling=S("yarn", 4.0, 4096, attention_factor=1.5)).factor == 1.5
+
+
+def test_no_codes_kept_in_inference_mode(k2):
+    """A tensor without a version counter is never known again, so an in-place write cannot leave stale codes."""
+    from krea2_amd.quantize import _SharedInputQuant
+    cache = _SharedInputQuant()
+    with torch.inference_mode():
+        h = torch.zeros(2, 128, dtype=torch.bfloat16)
+        cache.seed(h, None, None)
+        key, codes = cache.find(h)
+        cache.keep(h, key, None, None)
+    assert key is None and codes is None and cache.ref is None and cache.misses == 1
