@@ -10,8 +10,8 @@
 //
 // Bound: reading and writing the heads once.  A workgroup takes a run of (token, head) rows, q's heads before k's in
 // every token; its threads first compute the cos / sin of the run's tokens into LDS, once for all heads, then a thread
-// turns vectors of one head position, stepping through the run's rows.  4608 x 60 heads of 128 bf16: 30 us (4.8 TB/s), 16896
-// of them 98 us (5.3).
+// turns vectors of one head position, stepping through the run's rows.  4608 x 60 heads of 128 bf16: 31 us (4.6 TB/s), 16896
+// of them 99 us (5.2).
 #include <hip/hip_fp16.h>
 
 #include "k2q_common.h"
