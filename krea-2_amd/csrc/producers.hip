@@ -394,9 +394,11 @@ __global__ __launch_bounds__(256) void rmsmod_bwd_kernel(NormBwdArgs a) {
   for (int c = 0; c < kNCH; ++c) {
     const int col = 8 * t + 8 * T * c;
     const bool ok = col < K;
-    xv[c] = ok ? *reinterpret_cast<const uint4*>(a.x + rr * K + col) : make_uint4(0, 0, 0, 0);
-    dv[c] = ok ? *reinterpret_cast<const uint4*>(a.dh + rr * K + col) : make_uint4(0, 0, 0, 0);
-    if (MODE == BWD_ONCE) rv[c] = ok && a.dr ? *reinterpret_cast<const uint4*>(a.dr + rr * K + col) : make_uint4(0, 0, 0, 0);
+    const int cc = ok ? col : 0;
+    xv[c] = *reinterpret_cast<const uint4*>(a.x + rr * K + cc);
+    dv[c] = *reinterpret_cast<const uint4*>(a.dh + rr * K + cc);
+    if (MODE == BWD_ONCE) rv[c] = *reinterpret_cast<const uint4*>((a.dr ? a.dr : a.x) + rr * K + cc);
+    if (!ok) xv[c] = dv[c] = make_uint4(0, 0, 0, 0);
     const uint32_t w[4] = {xv[c].x, xv[c].y, xv[c].z, xv[c].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
