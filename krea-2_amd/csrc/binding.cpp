@@ -610,14 +610,20 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto ty = q->scalar_type();
     const int dt = ty == at::kBFloat16 ? K2Q_DTYPE_BF16 : ty == at::kHalf ? K2Q_DTYPE_F16 : K2Q_DTYPE_F32;
     const auto pt = p->scalar_type();
-    const int pos_type = pt == at::kLong ? K2Q_POS_I64 : pt == at::kInt ? K2Q_POS_I32 : pt == at::kFloat ? K2Q_POS_F32 : K2Q_POS_F64;
-    if (!ready(d) || (dt == K2Q_DTYPE_F32 && ty != at::kFloat) || (pos_type == K2Q_POS_F64 && pt != at::kDouble) || D > 4096 ||
+    const int pos_type = pt == at::kLong    ? K2Q_POS_I64
+                         : pt == at::kInt   ? K2Q_POS_I32
+                         : pt == at::kFloat ? K2Q_POS_F32
+                                            : K2Q_POS_F64;
+    if (!ready(d) || (dt == K2Q_DTYPE_F32 && ty != at::kFloat) || (pos_type == K2Q_POS_F64 && pt != at::kDouble) ||
+        D > 4096 ||
         turns->scalar_type() != at::kDouble || !turns->is_contiguous() || turns->device() != d || 2 * nf > D ||
         p->device() != d ||
         (axis && (axis->scalar_type() != at::kInt || !axis->is_contiguous() || axis->numel() != nf || axis->device() != d)))
       K2Q_REFUSE;
     const int lead = (int)p->dim() - (axis ? 1 : 0);      // positions' batch and token dimensions
-    if (lead < 1 || lead > 2 || p->size(lead - 1) != L || (axis && p->size(lead) != axes) || (lead == 2 && p->size(0) != 1 && p->size(0) != B)) K2Q_REFUSE;
+    if (lead < 1 || lead > 2 || p->size(lead - 1) != L || (axis && p->size(lead) != axes) ||
+        (lead == 2 && p->size(0) != 1 && p->size(0) != B))
+      K2Q_REFUSE;
     k2q_rotary_heads t[2] = {};
     Tensor out[2];
     const c10::DeviceGuard guard(d);

@@ -552,8 +552,9 @@ int k2q_launch_gemv_w4a8(const int8_t* qx, const float* sx, const uint8_t* qw4, 
 }
 
 // One token through a linear, its codes not given: one launch instead of two where every workgroup's own rotation hides
-// behind its weight loads.  Both launches against one, us: 512 x 512 4.7 / 3.3, 1536 x 6144 6.1 / 5.5, 4096 x 6144 7.8 / 7.1,
-// 6144 x 6144 8.7 / 8.7; no gain beyond, at two tokens (1536 x 6144 6.5 / 7.6) or two steps of K (2048 x 16384 9.7 / 9.6).
+// behind its weight loads.  Both launches against one, us: 512 x 512 4.7 / 3.3, 1536 x 6144 6.1 / 5.5, 4096 x 6144
+// 7.8 / 7.1, 6144 x 6144 8.7 / 8.7; no gain beyond, at two tokens (1536 x 6144 6.5 / 7.6) or two steps of K (2048 x 16384
+// 9.7 / 9.6).
 bool k2q_gemv_w4a8_quantizes(int64_t M, int64_t N, int64_t K) { return M == 1 && N < 2 * G4_WIDE && K <= 4 * G4_K; }
 
 // Called by k2q_linear_fwd for such shapes, after the checks of k2q_gemm_w4a8: the codes of x are written to qx, sx.

@@ -37,7 +37,8 @@ struct RotArgs {
   const double* turns;
   const int* axis;         // null: one axis
   float m, sign;
-  int turned, items, width, slots;   // a row's turned vectors, all its vectors, threads side by side on a row, rows side by side
+  int turned, items;       // a row's turned vectors, all its vectors
+  int width, slots;        // threads side by side on a row, rows side by side
   uint32_t run;            // rows per workgroup
   int dt, dh;              // slots / h, slots % h
 };
