@@ -430,3 +430,22 @@ def test_refusals(k2, dev):
         k2.residual_rmsnorm(norm, x.float(), y)
     with pytest.raises(ValueError):
         k2.residual_rmsnorm(norm, x, y.cpu())
+
+
+def test_offsets_past_32_bits(k2, dev):
+    """2^31 elements and more: the last rows are those of the same rows alone, forward and backward."""
+    M, K, n = 350208, 6144, 8
+    g = torch.Generator(device=dev).manual_seed(0)
+    x, y, dr, dh = (torch.empty(M, K, device=dev, dtype=torch.bfloat16).normal_(generator=g) for _ in range(4))
+    norm = Norm((torch.randn(K, generator=g, device=dev) * 0.1))
+    gate = torch.randn(1, K, generator=g, device=dev).bfloat16()
+
+    def run(rows):
+        leaves = [t[rows].requires_grad_() for t in (x, y)]
+        r, h = k2.residual_rmsnorm(norm, *leaves, gate)
+        q, s = k2.input_codes(h)
+        out = [r.detach(), h.detach(), q, s, *torch.autograd.grad([r, h], leaves, [dr[rows], dh[rows]])]
+        return [t[-n:].clone() for t in out]
+
+    for a, e in zip(run(slice(None)), run(slice(M - n, M))):
+        assert torch.equal(a, e)

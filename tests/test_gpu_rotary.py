@@ -228,3 +228,19 @@ def test_refusals(k2, dev):
         with pytest.raises(ValueError):
             bad()
     assert rope(q[:, :0], q[:, :0], pos[:0])[0].shape == (2, 0, 4, 64)
+
+
+def test_offsets_past_32_bits(k2, dev):
+    """2^31 elements and more in q: the last tokens are those of the same tokens alone, either way round."""
+    L, H, D, n = 350000, 48, 128, 4
+    q = torch.empty(1, L, H, D, device=dev, dtype=torch.bfloat16).normal_()
+    k = torch.empty(1, L, 2, D, device=dev, dtype=torch.bfloat16).normal_()
+    pos = torch.arange(L, device=dev)
+    rope = k2.RotaryEmbedding(D, layout="half")
+    a, e = rope(q, k, pos), rope(q[:, -n:], k[:, -n:], pos[-n:])
+    assert all(torch.equal(u[:, -n:], v) for u, v in zip(a, e))
+    t = q.requires_grad_()
+    got, = torch.autograd.grad(rope(t, None, pos)[0], t, a[0])
+    one = q[:, -n:].detach().requires_grad_()
+    ref, = torch.autograd.grad(rope(one, None, pos[-n:])[0], one, e[0])
+    assert torch.equal(got[:, -n:], ref)

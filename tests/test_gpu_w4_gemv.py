@@ -147,3 +147,15 @@ def test_refusals(k2, dev):
         L.gemm_w4a8(qx, sx, q4[:63].contiguous(), s4)
     with pytest.raises((ValueError, RuntimeError)):
         L.gemm_w4a8(qx, sx[:1].clone(), q4, s4)
+
+
+@pytest.mark.parametrize("M", [1, 2, 8])
+def test_offsets_past_32_bits(k2, dev, M):
+    """More than 2^31 bytes of packed weights: the last rows are those of the same rows alone (exact sums)."""
+    L, N, K, n = k2._lib, 263168, 16384, 64
+    g, qx, sx, q4, s4, _ = _inputs(M, n, K, dev, True)
+    big = torch.empty(N, K // 2, device=dev, dtype=torch.uint8)
+    big.random_(0, 256, generator=g)
+    scales = torch.ones(K // 64, N, device=dev, dtype=torch.bfloat16)
+    big[-n:], scales[:, -n:] = q4, s4
+    assert torch.equal(L.gemm_w4a8(qx, sx, big, scales)[:, -n:], L.gemm_w4a8(qx, sx, q4, s4))
