@@ -594,13 +594,14 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
       out[(int64_t)k * K + i] = ((acc[k][i] + red[0][lane][8 * k + i]) + red[1][lane][8 * k + i]) + red[2][lane][8 * k + i];
 }
 
-// The strips' partials joined: 64 columns a workgroup, its four waves every fourth strip, then the four in order.  Column
+// The strips' partials joined: 64 columns a workgroup, its NW waves every NW-th strip, then the waves in order.  Column
 // tiles of the batch entries (the bits of `per_entry`: scale, shift and gate gradients, bf16), then those of the sums over
 // every entry (`whole`: the norm weight's, f32, and those of a vector that every entry shares).
-__global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* part, int K, int64_t entries, int strips,
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void resnorm_colsum_join_kernel(const float* part, int K, int64_t entries, int strips,
                                                                   int per_entry, int whole, float* dnw, uint16_t* dscale,
                                                                   uint16_t* dshift, uint16_t* dgate) {
-  __shared__ float red[4][4][64];
+  __shared__ float red[4][NW][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t tiles = (uint32_t)(K + 63) / 64;
   const int col = (int)(blockIdx.x % tiles) * 64 + lane;
@@ -612,11 +613,11 @@ __global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* p
   float f[4] = {};
   if (col < K) {
     if (want == 1 << CS_W) {
-#pragma unroll 4
-      for (int64_t i = i0 + wave; i < i1; i += 4) f[CS_W] += part[(i * 4 + CS_W) * K + col];
+#pragma unroll 8
+      for (int64_t i = i0 + wave; i < i1; i += NW) f[CS_W] += part[(i * 4 + CS_W) * K + col];
     } else {
-#pragma unroll 2
-      for (int64_t i = i0 + wave; i < i1; i += 4)
+#pragma unroll 4
+      for (int64_t i = i0 + wave; i < i1; i += NW)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (k != CS_W || want & 1 << CS_W) f[k] += part[(i * 4 + k) * K + col];
@@ -627,12 +628,29 @@ __global__ __launch_bounds__(256) void resnorm_colsum_join_kernel(const float* p
   __syncthreads();
   if (wave || col >= K) return;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) f[k] = ((red[k][0][lane] + red[k][1][lane]) + red[k][2][lane]) + red[k][3][lane];
+  for (int k = 0; k < 4; ++k) {
+    f[k] = red[k][0][lane];
+#pragma unroll
+    for (int v = 1; v < NW; ++v) f[k] += red[k][v][lane];
+  }
   const int64_t o = all ? col : entry * K + col;
   if (want & 1 << CS_W) dnw[o] = f[CS_W];
   if (want & 1 << CS_SCALE) dscale[o] = (uint16_t)f32_to_bf16_bits(f[CS_SCALE]);
   if (want & 1 << CS_SHIFT) dshift[o] = (uint16_t)f32_to_bf16_bits(f[CS_SHIFT]);
   if (want & 1 << CS_GATE) dgate[o] = (uint16_t)f32_to_bf16_bits(f[CS_GATE]);
+}
+
+// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 256 strips of 6144 columns 101 / 87,
+// 300 entries of one strip and 4096 columns 97 / 142).
+void launch_join(const float* part, int64_t K, int64_t entries, int strips, int asked, int over, float* dnorm,
+                 uint16_t* dscale, uint16_t* dshift, uint16_t* dgate, hipStream_t st) {
+  const dim3 grid((unsigned)((K + 63) / 64 * (entries + 1)));
+  if (strips >= 16)
+    hipLaunchKernelGGL(resnorm_colsum_join_kernel<16>, grid, dim3(1024), 0, st, part, (int)K, entries, strips, asked & ~over,
+                       asked & over, dnorm, dscale, dshift, dgate);
+  else
+    hipLaunchKernelGGL(resnorm_colsum_join_kernel<4>, grid, dim3(256), 0, st, part, (int)K, entries, strips, asked & ~over,
+                       asked & over, dnorm, dscale, dshift, dgate);
 }
 
 // Strips per batch entry: about two workgroups a CU over the column tiles, at least 16 rows each (all three passes, us, at
@@ -642,6 +660,141 @@ int colsum_strips(int64_t rpb, int64_t K, int64_t entries, int cus) {
   int64_t s = (2 * cus + tiles - 1) / tiles;
   const int64_t most = (rpb + 15) / 16;
   s = s < 1 ? 1 : s > most ? most : s;
+  const int64_t rows = (rpb + s - 1) / s;
+  return (int)((rpb + rows - 1) / rows);
+}
+
+// The row pass that rounds once and its column sums in one, which reads dh, r, y and dr once: a workgroup a CU owns a strip
+// of one entry's rows, a lane the same columns of every row (those of the row pass with four waves, whose row sums and
+// results it repeats bit for bit), so its column sums stay in registers (one wave per SIMD has 512) and no wave meets
+// another over them.  Both row sums cross the waves behind one barrier (neither needs the other's result) while the next
+// row is loaded (without: 47.6 us for 42.0).  Two passes / this one, with the join, us: 2 x 768 x 6144 43.4 / 35.4, 4608 x
+// 6144 102 / 87, 9216 x 6144 211 / 151, 4096 x 8192 118 / 102, 1024 x 6144 30.3 / 30.5, 768 x 6144 26.4 / 27.2.
+template <int kNCH>
+__global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a, const uint16_t* y, int64_t ldy, int strips,
+                                                                  int strip_rows, int asked, float* part) {
+  __shared__ float2 sred[2][4];
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, K = a.K;
+  const int64_t entry = blockIdx.x / strips;
+  const int64_t m0 = entry * a.rpb + (int64_t)(blockIdx.x % strips) * strip_rows, mend = (entry + 1) * a.rpb;
+  const int64_t m1 = m0 + strip_rows < mend ? m0 + strip_rows : mend;
+  const uint16_t* mg = a.gate ? a.gate + entry * a.ldg : nullptr;
+  // what is absent is read as x
+  const uint16_t *yp = y ? y : a.x, *rp = a.dr ? a.dr : a.x;
+  const int64_t ly = y ? ldy : K;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  float w[kNCH][8], acc[kNCH][4][8] = {};
+  uint4 pv[kNCH], gg[kNCH];
+#pragma unroll
+  for (int c = 0; c < kNCH; ++c) {
+    const int col = 8 * t + 2048 * c, cc = col < K ? col : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[c][i] = a.nw[cc + i] + a.nwadd;
+    pv[c] = a.mscale ? *reinterpret_cast<const uint4*>(a.mscale + entry * a.ldm + cc) : zero;
+    gg[c] = mg ? *reinterpret_cast<const uint4*>(mg + cc) : zero;
+  }
+  uint4 xn[kNCH], dn[kNCH], rn[kNCH], yn[kNCH];
+  auto load = [&](int64_t m) {
+#pragma unroll
+    for (int c = 0; c < kNCH; ++c) {
+      const int col = 8 * t + 2048 * c, cc = col < K ? col : 0;
+      xn[c] = *reinterpret_cast<const uint4*>(a.x + m * K + cc);
+      dn[c] = *reinterpret_cast<const uint4*>(a.dh + m * K + cc);
+      rn[c] = *reinterpret_cast<const uint4*>(rp + m * K + cc);
+      yn[c] = *reinterpret_cast<const uint4*>(yp + m * ly + cc);
+    }
+  };
+  load(m0);
+  for (int64_t m = m0; m < m1; ++m) {
+    uint4 xv[kNCH], dv[kNCH], rv[kNCH], yv[kNCH];
+    float gv[kNCH][8], ss = 0.f, dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < kNCH; ++c) {
+      const bool ok = 8 * t + 2048 * c < K;
+      xv[c] = ok ? xn[c] : zero;
+      dv[c] = ok ? dn[c] : zero;
+      rv[c] = a.dr ? rn[c] : zero;
+      yv[c] = y ? yn[c] : zero;
+    }
+    load(m + 1 < m1 ? m + 1 : m);
+#pragma unroll
+    for (int c = 0; c < kNCH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float x0 = bf16_of(xv[c], i), x1 = bf16_of(xv[c], i + 1);
+        ss += x0 * x0;
+        ss += x1 * x1;
+        float p0 = 1.f + bf16_of(pv[c], i), p1 = 1.f + bf16_of(pv[c], i + 1);
+        bf16r2(p0, p1);
+        gv[c][i] = bf16_of(dv[c], i) * p0 * w[c][i];
+        gv[c][i + 1] = bf16_of(dv[c], i + 1) * p1 * w[c][i + 1];
+        dot += gv[c][i] * x0;
+        dot += gv[c][i + 1] * x1;
+      }
+    ss = wave_sum(ss);
+    dot = wave_sum(dot);
+    float2* red = sred[(m - m0) & 1];       // written again two rows later, behind the next row's barrier
+    if (lane == 0) red[wave] = make_float2(ss, dot);
+    __syncthreads();
+    ss = dot = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      ss += red[v].x;
+      dot += red[v].y;
+    }
+    const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
+    const float c3 = __fdiv_rn(r * r * r * dot, (float)K);
+#pragma unroll
+    for (int c = 0; c < kNCH; ++c) {
+      const int col = 8 * t + 2048 * c;
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = bf16_of(xv[c], i), dh = bf16_of(dv[c], i), xr = x * r;
+        d[i] = gv[c][i] * r - x * c3;
+        if (a.dr) d[i] = bf16_of(rv[c], i) + d[i];
+        const float dnv = dh * bf16r(1.f + bf16_of(pv[c], i));
+        acc[c][CS_W][i] = __builtin_fmaf(dnv, xr, acc[c][CS_W][i]);
+        acc[c][CS_SCALE][i] = __builtin_fmaf(dh, bf16r(xr * w[c][i]), acc[c][CS_SCALE][i]);
+        acc[c][CS_SHIFT][i] += dh;
+        acc[c][CS_GATE][i] = __builtin_fmaf(d[i], bf16_of(yv[c], i), acc[c][CS_GATE][i]);
+      }
+      if (col >= K) continue;
+      uint32_t o[4], e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j] = pack_bf16x2(d[2 * j], d[2 * j + 1]);
+        e[j] = pack_bf16x2(bf16_of(gg[c], 2 * j) * d[2 * j], bf16_of(gg[c], 2 * j + 1) * d[2 * j + 1]);
+      }
+      *reinterpret_cast<uint4*>(a.dx + m * K + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      if (mg) *reinterpret_cast<uint4*>(a.dy + m * K + col) = make_uint4(e[0], e[1], e[2], e[3]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kNCH; ++c) {
+    const int col = 8 * t + 2048 * c;
+    if (col >= K) continue;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (asked & 1 << k) {
+        float4* out = reinterpret_cast<float4*>(part + ((int64_t)blockIdx.x * 4 + k) * K + col);
+        out[0] = make_float4(acc[c][k][0], acc[c][k][1], acc[c][k][2], acc[c][k][3]);
+        out[1] = make_float4(acc[c][k][4], acc[c][k][5], acc[c][k][6], acc[c][k][7]);
+      }
+  }
+}
+
+// The workspace: row statistics, then the partials, 16-byte aligned.
+int64_t stats_floats(int64_t M) { return (2 * M + 3) / 4 * 4; }
+
+// Strips per entry of that pass, one workgroup a CU of at least four rows each; 0 (the two passes) where they would leave a
+// quarter of the CUs idle, or the columns are not the four-wave row pass's or too many for the registers.
+int fused_strips(int64_t rpb, int64_t K, int64_t entries, int cus) {
+  if (K <= 2048 || K > 8192) return 0;
+  int64_t s = cus / entries;
+  const int64_t most = rpb / 4;
+  s = s > most ? most : s;
+  if (s < 1 || 4 * entries * s < 3 * cus) return 0;
   const int64_t rows = (rpb + s - 1) / s;
   return (int)((rpb + rows - 1) / rows);
 }
@@ -786,7 +939,9 @@ extern "C" int k2q_swiglu_bwd(const uint16_t* dh, const uint16_t* gate, const ui
 extern "C" int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch) {
   if (M < 1 || K < 8 || K % 8 || K > 16384 || rows_per_batch < 1 || M % rows_per_batch) return 0;
   const int64_t entries = M / rows_per_batch;
-  return (2 * M + entries * colsum_strips(rows_per_batch, K, entries, k2q_cu_count()) * 4 * K) * 4;
+  const int cus = k2q_cu_count(), two = colsum_strips(rows_per_batch, K, entries, cus),
+            one = fused_strips(rows_per_batch, K, entries, cus);
+  return (stats_floats(M) + entries * (two > one ? two : one) * 4 * K) * 4;
 }
 
 extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
@@ -829,6 +984,25 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   a.dy = dy;
   a.stats = cols ? static_cast<float*>(ws) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const int asked = (dnorm ? 1 << CS_W : 0) | (dscale ? 1 << CS_SCALE : 0) | (dshift ? 1 << CS_SHIFT : 0) |
+                    (dgate ? 1 << CS_GATE : 0);
+  const int over = 1 << CS_W | (entries == 1 ? 0 : (shared & K2Q_SHARED_SCALE ? 1 << CS_SCALE : 0) |
+                                                       (shared & K2Q_SHARED_SHIFT ? 1 << CS_SHIFT : 0) |
+                                                       (shared & K2Q_SHARED_GATE ? 1 << CS_GATE : 0));
+  const int fs = cols && !eager ? fused_strips(rows_per_batch, K, entries, k2q_cu_count()) : 0;
+  if (fs) {
+    const int rows = (int)((rows_per_batch + fs - 1) / fs);
+    float* part = a.stats + stats_floats(M);
+#define K2Q_RBC(N)                                                                                                        \
+  hipLaunchKernelGGL(resnorm_bwd_cols_kernel<N>, dim3((unsigned)(entries * fs)), dim3(256), 0, st, a, dgate ? y : nullptr, \
+                     ldy, fs, rows, asked, part)
+    if (K <= 4096) K2Q_RBC(2);
+    else if (K <= 6144) K2Q_RBC(3);
+    else K2Q_RBC(4);
+#undef K2Q_RBC
+    launch_join(part, K, entries, fs, asked, over, dnorm, dscale, dshift, dgate, st);
+    return k2q_launch_status();
+  }
   if (eager) launch_norm_bwd<BWD_EAGER>(a, st);
   else launch_norm_bwd<BWD_ONCE>(a, st);
   if (!cols) return k2q_launch_status();
@@ -848,15 +1022,9 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   c.nwadd = scale_add;
   c.mscale = mod_scale;
   c.ldm = ld_scale;
-  c.part = a.stats + 2 * M;
-  const int64_t grid = (K + CS_COLS - 1) / CS_COLS * entries * c.strips, join = (K + 63) / 64 * (entries + 1);
-  const int asked = (dnorm ? 1 << CS_W : 0) | (dscale ? 1 << CS_SCALE : 0) | (dshift ? 1 << CS_SHIFT : 0) |
-                    (dgate ? 1 << CS_GATE : 0);
-  const int over = 1 << CS_W | (entries == 1 ? 0 : (shared & K2Q_SHARED_SCALE ? 1 << CS_SCALE : 0) |
-                                                       (shared & K2Q_SHARED_SHIFT ? 1 << CS_SHIFT : 0) |
-                                                       (shared & K2Q_SHARED_GATE ? 1 << CS_GATE : 0));
+  c.part = a.stats + stats_floats(M);
+  const int64_t grid = (K + CS_COLS - 1) / CS_COLS * entries * c.strips;
   hipLaunchKernelGGL(resnorm_colsum_kernel, dim3((unsigned)grid), dim3(256), 0, st, c);
-  hipLaunchKernelGGL(resnorm_colsum_join_kernel, dim3((unsigned)join), dim3(256), 0, st, c.part, (int)K, entries, c.strips,
-                     asked & ~over, asked & over, dnorm, dscale, dshift, dgate);
+  launch_join(c.part, K, entries, c.strips, asked, over, dnorm, dscale, dshift, dgate, st);
   return k2q_launch_status();
 }
