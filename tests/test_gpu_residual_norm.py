@@ -206,6 +206,33 @@ def test_gradients_against_float64(k2, dev, shape, entries, gated):
     assert all(torch.equal(a, e) for a, e in zip(again, got))
 
 
+@pytest.mark.parametrize("read", ["both", "h"])
+@pytest.mark.parametrize("shape", [(2, 9, 640), (2, 450, 2304)])
+def test_some_of_the_gradients(k2, dev, shape, read):
+    """Each input alone, and h alone read: the same bits as when every gradient is asked for."""
+    norm, x, y, mods = _inputs(shape, dev, 2, seed=3)
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+    base = [t.detach() for t in (x, y, *mods)]
+
+    def run(asked):
+        leaves = [t.clone().requires_grad_(i in asked) for i, t in enumerate(base)]
+        norm.scale.requires_grad_(5 in asked)
+        r, h = k2.residual_rmsnorm(norm, *leaves)
+        of = [t for i, t in enumerate((*leaves, norm.scale)) if i in asked]
+        g = torch.autograd.grad([r, h], of, [dr, dh]) if read == "both" else torch.autograd.grad(h, of, dh)
+        norm.scale.requires_grad_(False)
+        return g
+
+    full = run(range(6))
+    for i in range(6):
+        assert torch.equal(run([i])[0], full[i]), i
+    none = torch.zeros_like(dr)
+    if read == "h":             # r unread is r read with a gradient of zeros
+        leaves = [t.clone().requires_grad_() for t in base]
+        got = torch.autograd.grad(k2.residual_rmsnorm(norm, *leaves), leaves, [none, dh])
+        assert all(torch.equal(a, e) for a, e in zip(got, full))
+
+
 @pytest.mark.parametrize("K", [640, 6144, 8320])
 def test_eager_gradients_equal_the_separate_operations(k2, dev, K):
     """The block's form (gate, modulation and norm frozen): the gradients of the eager residual and the norm kernel; the
