@@ -320,16 +320,33 @@ def _residual_rmsnorm(norm, x, y, gate, scale, shift, eager):
     return r, h
 
 
+class _CodesFn(torch.autograd.Function):
+    """The codes of ``h`` as a node: what a tracer records and a forward-mode level refuses."""
+
+    @staticmethod
+    def forward(ctx, h):
+        q, s, _ = _lib.rotquant(_aligned(h.reshape(-1, h.shape[-1])))
+        ctx.mark_non_differentiable(q, s)
+        return q, s
+
+    @staticmethod
+    def backward(ctx, _dq, _ds):
+        return None
+
+
 def input_codes(h: torch.Tensor):
     """``(q, s)``: the int8 codes (rows, K) of ``h``'s rotated rows and their f32 scales (rows,), as the ConvRot layers
     take them: a code stands for ``q * s``.  Those that the producer of this very tensor left, else computed now (and
-    kept for the next layer)."""
+    kept for the next layer).  They are not differentiable."""
     if h.dtype != torch.bfloat16:
         raise NotImplementedError("the codes are those of a bf16 tensor (the DiT dtype)")
     key, codes = shared_input_quant.find(h)
     if codes is None:
-        with torch.no_grad():
-            codes = _lib.rotquant(_aligned(h.reshape(-1, h.shape[-1])))[:2]
+        if _lib.observed():
+            codes = _CodesFn.apply(h)
+        else:
+            with torch.no_grad():
+                codes = _lib.rotquant(_aligned(h.reshape(-1, h.shape[-1])))[:2]
         shared_input_quant.keep(h, key, *codes)
     return codes
 
