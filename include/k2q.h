@@ -47,6 +47,9 @@ extern "C" {
 /* Library version string and device check (K2Q_OK when the current device is gfx950). */
 const char* k2q_version(void);
 int k2q_check_device(void);
+/* The number of the graph capture that stream is in (positive, another for every capture), 0 outside one, K2Q_ELAUNCH
+ * where the stream cannot be asked.  Host only. */
+int64_t k2q_capture_id(void* stream);
 
 /* (1) Rotate + per-row int8 quantize.
  * Replaces the point where Fp8Linear.forward receives x (reference quantize.py:48); the rotation and

@@ -68,6 +68,7 @@ GROUP_ALIGN = 256      # each segment's out_features: a multiple of the GEMM til
 
 _SIGNATURES = {
     "k2q_version": ([], ctypes.c_char_p),
+    "k2q_capture_id": ([_p], _i64),
     "k2q_check_device": ([], _int),
     "k2q_rotquant": ([_p, _int, _i64, _i64, _i64, _p, _p, _p, _p], _int),
     "k2q_rotquant_lora": ([_p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p], _int),
@@ -180,6 +181,18 @@ def observed() -> bool:
     """Whether a tracer records the calls or a forward-mode level is open: calls then stay torch operations and autograd
     nodes (the trace holds them; a node refuses tangents, which a library call would drop)."""
     return torch._C._is_tracing() or forward_ad._current_level >= 0
+
+
+def recording(stream: int):
+    """What records the calls made now on the raw ``stream``: a tracer's state, or the number of the graph capture that it is
+    in, 0 for neither.  Results kept under one value are no results under another: a trace would hold them as constants,
+    and a graph would replay without the launch that made them, or before it."""
+    if torch._C._is_tracing():
+        return torch._C._get_tracing_state()
+    if not stream:          # the default stream is never captured
+        return 0
+    number = _fast().capture_id(stream)
+    return number if number >= 0 else object()      # equal to nothing
 
 
 def _refused(rc, name: str, call, *checks):

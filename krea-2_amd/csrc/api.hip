@@ -25,6 +25,16 @@ int k2q_cu_count() {
 
 extern "C" const char* k2q_version(void) { return "k2q 0.1.0 gfx950"; }
 
+extern "C" int64_t k2q_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();      // not the next launch's
+    return K2Q_ELAUNCH;
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id;
+}
+
 extern "C" int k2q_check_device(void) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return K2Q_EARCH;

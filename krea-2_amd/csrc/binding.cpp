@@ -38,6 +38,7 @@ struct Api {
   decltype(&k2q_resnorm_bwd) resnorm_bwd;
   decltype(&k2q_resnorm_bwd_ws_bytes) resnorm_bwd_ws_bytes;
   decltype(&k2q_rotary) rotary;
+  decltype(&k2q_capture_id) capture_id;
 } api{};
 
 PyObject* raw_stream_of = nullptr;   // torch._C._cuda_getCurrentRawStream
@@ -670,7 +671,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !get("k2q_dequant_fp8", api.dequant_fp8) || !get("k2q_gemm_bf16", api.gemm_bf16) ||
       !get("k2q_gemm_plan_ws_bytes", api.gemm_plan_ws_bytes) || !get("k2q_resnorm_rotquant", api.resnorm_rotquant) ||
       !get("k2q_resnorm_bwd", api.resnorm_bwd) || !get("k2q_resnorm_bwd_ws_bytes", api.resnorm_bwd_ws_bytes) ||
-      !get("k2q_rotary", api.rotary))
+      !get("k2q_rotary", api.rotary) || !get("k2q_capture_id", api.capture_id))
     return nullptr;
   Py_INCREF(a[1]);
   Py_XSETREF(raw_stream_of, a[1]);
@@ -687,13 +688,22 @@ PyObject* py_device_checked(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// capture_id(raw stream): the capture that the stream is in, 0 outside one, negative where it cannot be asked
+PyObject* py_capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(1)
+  (void)bad;
+  void* st = PyLong_AsVoidPtr(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  return PyLong_FromLongLong(api.capture_id(st));
+}
+
 #define K2Q_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2Q_METHOD(alloc_codes),
                          K2Q_METHOD(linear_fwd),  K2Q_METHOD(lora_grads),     K2Q_METHOD(lora_down),
                          K2Q_METHOD(dx_weight),   K2Q_METHOD(gemm_dx),        K2Q_METHOD(dequant_fp8),
                          K2Q_METHOD(gemm_bf16),   K2Q_METHOD(pad_factors),    K2Q_METHOD(resnorm),
                          K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         K2Q_METHOD(linear_infer),
-                         {nullptr, nullptr, 0, nullptr}};
+                         K2Q_METHOD(capture_id),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -515,7 +515,7 @@ class _SiblingGroup:
     """Linears that receive the same tensor (``wq / wk / wv / gate`` of ``Attention.forward``, ``mmdit.py:199``).
     The first member called with a tensor computes every member's output in one grouped launch and keeps the
     others; each later member called with that same tensor (same object, version, pointer, shape, strides and
-    stream) and an unchanged adapter takes its output.  Anything else runs the member's own forward.  Kept
+    stream, in the same graph capture or none) and an unchanged adapter takes its output.  Anything else runs the member's own forward.  Kept
     outputs a member never asks for stay referenced until the group's next launch replaces them."""
 
     def __init__(self, members):
@@ -542,7 +542,8 @@ class _SiblingGroup:
 
     @staticmethod
     def _key(x):
-        return (x._version, x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.device, _lib._stream(x.device))
+        stream = _lib._stream(x.device)
+        return (x._version, x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.device, stream, _lib.recording(stream))
 
     def call(self, idx: int, x: torch.Tensor):
         if x.is_inference():        # no version counter to know it by

@@ -32,9 +32,10 @@ class _SharedInputQuant:
     (``mmdit.py:178``), so the rotation + quantization runs once per input instead of 4 / 2 times.
 
     A hit needs the same tensor object (held by weak reference, so a freed tensor never matches), the same
-    version counter (any in-place write bumps it), data pointer, shape, strides and CUDA stream.  The
-    codes are a pure function of the input, so a hit returns exactly what a fresh call would.  Tensors of
-    ``torch.inference_mode`` have no version counter: nothing is kept for them (key None)."""
+    version counter (any in-place write bumps it), data pointer, shape, strides, CUDA stream, and the same graph
+    capture or trace, or neither (a graph replayed after its input changed would take codes that no replay
+    makes).  The codes are a pure function of the input, so a hit returns exactly what a fresh call would.
+    Tensors of ``torch.inference_mode`` have no version counter: nothing is kept for them (key None)."""
 
     enabled = True
 
@@ -49,7 +50,8 @@ class _SharedInputQuant:
         if x.is_inference():
             return None
         dev = x.device
-        return (x._version, x.data_ptr(), x.shape, x.stride(), dev, _lib._stream(dev))
+        stream = _lib._stream(dev)
+        return (x._version, x.data_ptr(), x.shape, x.stride(), dev, stream, _lib.recording(stream))
 
     def lookup(self, x: torch.Tensor, x2: torch.Tensor):
         key = self._key(x)

@@ -1,0 +1,79 @@
+"""GPU tests: what is kept between calls (an input's codes, siblings' outputs, float32 copies) and graph captures.  A graph
+follows its static input at every replay, whatever ran before its capture on the same stream, and eager calls after a capture
+take nothing that only a replay computes."""
+import pytest
+import torch
+import torch.nn as nn
+
+pytestmark = pytest.mark.gpu
+
+
+def make_x(M, K, seed):
+    return torch.randn(M, K, generator=torch.Generator().manual_seed(seed)).bfloat16()
+
+
+def _layer(k2, dev, mode="w8a8", K=512, N=256, seed=0):
+    lin = nn.Linear(K, N, bias=False, device=dev, dtype=torch.bfloat16)
+    with torch.no_grad():
+        lin.weight.copy_(make_x(N, K, seed=seed).to(dev) * 0.05)
+    return k2.ConvRotLinear(lin, mode)
+
+
+def _replays(graph, static, outs, call, values):
+    """Every replay against the eager result on the same values, with eager work between."""
+    for v in values:
+        static.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        want = call(v.clone())
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+@pytest.mark.parametrize("rows", [3, 64])
+@pytest.mark.parametrize("mode", ["w8a8", "w4a8"])
+def test_captured_after_a_call_on_the_same_stream(k2, dev, mode, rows):
+    layer = _layer(k2, dev, mode)
+    values = [make_x(rows, 512, seed=s).to(dev) for s in range(3)]
+
+    def call(x):
+        with torch.no_grad():
+            return (*k2.input_codes(x), layer(x))
+
+    for first in (layer, k2.input_codes):
+        static = values[0].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+        outs = []
+        with torch.cuda.stream(side), torch.no_grad():
+            first(static)                                       # its codes are kept for this tensor
+        torch.cuda.synchronize()
+        for g in graphs:                                        # the second capture finds the first one's codes
+            with torch.cuda.graph(g, stream=side):
+                outs.append(call(static))
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            eager = call(static)                                # before any replay
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(eager, call(values[0].clone())))
+        for g, o in zip(reversed(graphs), reversed(outs)):
+            _replays(g, static, o, call, values)
+
+
+def test_siblings_kept_before_a_capture(k2, dev):
+    from krea2_amd.fused import _SiblingGroup
+    layers = [_layer(k2, dev, N=256, seed=s) for s in range(2)]
+    group = _SiblingGroup(layers)
+    values = [make_x(64, 512, seed=s).to(dev) for s in range(3)]
+    static = values[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad():
+        with torch.cuda.stream(side):
+            group.call(0, static)                               # keeps the other member's output
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = group.call(1, static)
+        _replays(graph, static, [out], lambda x: [layers[1](x)], values)

@@ -41,3 +41,25 @@ def test_codes_refuse_a_tangent(codes):
         with pytest.raises((RuntimeError, NotImplementedError)):
             codes(forward_ad.make_dual(x, torch.ones_like(x)))
         assert all(torch.equal(a, e) for a, e in zip(codes(x.clone()), want))    # no tangent: taken
+
+
+def test_codes_kept_before_a_trace_are_no_part_of_it(codes):
+    x, other = torch.randn(2, 4, 128).to(torch.bfloat16)
+    codes(x)
+    traced = torch.jit.trace(lambda h: codes(h), x, check_trace=False)
+    again = torch.jit.trace(lambda h: codes(h), x, check_trace=False)
+    for t in (traced, again):
+        for a, e in zip(t(other), _codes(other)):
+            assert torch.equal(a, e)
+
+
+def test_codes_of_one_recording_are_no_part_of_another(k2, monkeypatch):
+    """On the CPU: a hit needs the stream's capture, or none, that the codes were kept in."""
+    cache, now = k2.quantize._SharedInputQuant(), 0
+    monkeypatch.setattr(k2._lib, "_stream", lambda dev: 16)
+    monkeypatch.setattr(k2._lib, "_native", type("Native", (), {"capture_id": staticmethod(lambda stream: now)}))
+    x = torch.zeros(2, 128)
+    for now in (0, 7, 8, 0, -3, -3):
+        assert cache.find(x)[1] is None
+        cache.seed(x, now, now)
+        assert cache.find(x)[1] == ((now, now) if now >= 0 else None)       # -3: the stream could not be asked
