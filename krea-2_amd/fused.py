@@ -282,7 +282,8 @@ def residual_rmsnorm(norm: nn.Module, x: torch.Tensor, y: torch.Tensor, gate: to
     the ConvRot layers that receive it take.  Returns ``(r, h)``.
 
     ``norm`` is an RMSNorm module with ``eps`` and a ``scale`` (weight ``scale + 1``, ``mmdit.py:146-161``) or a
-    ``weight``; ``h`` is modulated, ``(1 + scale) * norm(r) + shift``, where ``scale`` and ``shift`` are given.  ``x`` and
+    ``weight``, either of which multiplies in float32 before the norm is rounded, as ``nn.RMSNorm`` does (not for modules
+    that round the normalised value first); ``h`` is modulated, ``(1 + scale) * norm(r) + shift``, where ``scale`` and ``shift`` are given.  ``x`` and
     ``y`` (B, L, K) or (M, K) bf16; ``gate``, ``scale``, ``shift`` bf16, one entry or one per batch row of ``x`` ((B, 1,
     K)).  Every tensor of the formula is rounded to bf16 where the eager bf16 operations round it, so ``r`` and ``h`` equal
     theirs (and ``h`` that of :func:`modulated_rmsnorm` on ``r``) bit for bit; the mean square is float32.
@@ -297,9 +298,10 @@ def _residual_rmsnorm(norm, x, y, gate, scale, shift, eager):
     gradients are theirs bit for bit."""
     grad = torch.is_grad_enabled()
     w, add = _norm_weight(norm, grad)
-    if norm.eps is None:
+    eps = getattr(norm, "eps", None)
+    if eps is None:
         raise ValueError(f"{type(norm).__name__} has no eps")
-    eps = float(norm.eps)
+    eps = float(eps)
     if x.numel() == 0:
         _residual_rows(x, y, gate, w, scale, shift)
         _lib._device_check(x.device)

@@ -34,6 +34,18 @@ def test_residual_norm_refuses_before_any_launch(k2):
         f(_Norm(256), x[:, :0], x[:, :0])
 
 
+def test_residual_norm_refuses_a_module_without_eps(k2):
+    """A norm that names its eps otherwise is no argument of this function: the refusal says what is missing."""
+    class Other(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.weight, self.variance_epsilon = nn.Parameter(torch.ones(256)), 1e-6
+
+    x = torch.zeros(2, 3, 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="Other has no eps"):
+        k2.residual_rmsnorm(Other(), x, x)
+
+
 def test_entry_points_refuse_bad_arguments(k2):
     """The C entries' own checks (addresses that are never read)."""
     lib = k2._lib.load()
