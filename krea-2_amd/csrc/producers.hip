@@ -11,7 +11,8 @@
 //   * RMSNorm with the residual's addition (mmdit.py:317-318: `x = x + pregate * attn`, then the norm of x):
 //       t = bf16(gate * y)  (t = y without a gate),  r = bf16(x + t),
 //     and the norm above of r, modulated or not.  r is written too: it is the residual stream.  The roundings are those
-//     of the eager bf16 ops, so r, h and the codes equal those of the separate ops and of the norm on r bit for bit.
+//     of the eager bf16 ops: r equals theirs, h and the codes those of the norm above on r, bit for bit (the eager norm's
+//     mean square is summed in another order: one value of h in about 1e5 is a bf16 step from its).
 //     9 bytes an element: 2 x 4608 x 6144 in 110 us (4.6 TB/s; a copy of 4 GB runs at 4.9).
 // All write h (bf16, the tensor the next linear receives: its LoRA down-projection and the saved input of
 // the backward read it) and the int8 codes + scales of rotate/quant applied to h, computed from the same

@@ -6,8 +6,8 @@ the modulated RMSNorm output ``(1 + scale) * norm(x) + shift`` (read by ``wq/wk/
 ``mlp.down``).  The producers here compute that tensor AND its int8 codes in one gfx950 pass
 (``k2q_rmsmod_rotquant``; ``k2q_resnorm_rotquant``, which adds the residual first; ``k2q_swiglu_rotquant``), then
 hand the codes to the shared-input cache, so the layers that read the tensor run no rotate/quant of their own.
-Outputs are the reference's eager bf16 results (same rounding points), and the codes equal a separate
-rotate/quant of them bit for bit.
+Outputs have the rounding points of the reference's eager bf16 operations (a norm's float32 row sum has an order of its
+own: a value at a tie may round the other way), and the codes equal a separate rotate/quant of them bit for bit.
 
 :func:`fuse_producers` patches a DiT's blocks in place (call it after ``quantize_dit_convrot`` and
 ``inject_lora``); :func:`modulated_rmsnorm`, :func:`residual_rmsnorm` and :func:`swiglu` are the operations for model code
@@ -283,10 +283,12 @@ def residual_rmsnorm(norm: nn.Module, x: torch.Tensor, y: torch.Tensor, gate: to
 
     ``norm`` is an RMSNorm module with ``eps`` and a ``scale`` (weight ``scale + 1``, ``mmdit.py:146-161``) or a
     ``weight``, either of which multiplies in float32 before the norm is rounded, as ``nn.RMSNorm`` does (not for modules
-    that round the normalised value first); ``h`` is modulated, ``(1 + scale) * norm(r) + shift``, where ``scale`` and ``shift`` are given.  ``x`` and
-    ``y`` (B, L, K) or (M, K) bf16; ``gate``, ``scale``, ``shift`` bf16, one entry or one per batch row of ``x`` ((B, 1,
-    K)).  Every tensor of the formula is rounded to bf16 where the eager bf16 operations round it, so ``r`` and ``h`` equal
-    theirs (and ``h`` that of :func:`modulated_rmsnorm` on ``r``) bit for bit; the mean square is float32.
+    that round the normalised value first); ``h`` is modulated, ``(1 + scale) * norm(r) + shift``, where ``scale`` and
+    ``shift`` are given.  ``x`` and ``y`` (B, L, K) or (M, K) bf16; ``gate``, ``scale``, ``shift`` bf16, one entry or one
+    per batch row of ``x`` ((B, 1, K)).  Every tensor of the formula is rounded to bf16 where the eager bf16 operations
+    round it: ``r`` equals theirs, and ``h`` that of :func:`modulated_rmsnorm` on ``r``, bit for bit.  The mean square is
+    float32, summed in that function's order and not in torch's, so one value of ``h`` in about 1e5 lies a bf16 step from
+    the eager norm's, and codes with it.
 
     Differentiable (once) in ``x``, ``y``, ``gate``, ``scale``, ``shift`` and the norm's parameter.  The backward is float32
     with one rounding of each gradient; the last four are sums over rows, added in a fixed order."""
