@@ -170,7 +170,8 @@ class RotaryEmbedding(nn.Module):
         if q.shape[-1] > _lib.MAX_HEAD:
             raise ValueError(f"heads of {q.shape[-1]} values exceed the kernel's {_lib.MAX_HEAD}")
         if q.dim() == 3:
-            q2, k2 = self(q.unsqueeze(0), None if k is None else k.unsqueeze(0), positions, heads_first)
+            # forward itself: the module's hooks have run
+            q2, k2 = self.forward(q.unsqueeze(0), None if k is None else k.unsqueeze(0), positions, heads_first)
             return q2.squeeze(0), None if k2 is None else k2.squeeze(0)
         if q.numel() == 0 or (k is not None and k.numel() == 0):
             if q.numel() or (k is not None and k.numel()):

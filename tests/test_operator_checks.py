@@ -110,6 +110,20 @@ def test_rotary_module_refuses(k2):
     assert not list(rope.parameters()) and not rope.state_dict()
 
 
+@pytest.mark.parametrize("shape", [(5, 2, 64), (1, 5, 2, 64)])
+def test_rotary_hooks_run_once(k2, monkeypatch, shape):
+    """Also where the call has no batch: a hook of the module sees the caller's tensors, once."""
+    rope = k2.RotaryEmbedding(64)
+    monkeypatch.setattr(k2._lib, "_device_check", lambda dev: None)
+    monkeypatch.setattr(k2._lib, "rotary", lambda q, k, *rest: (q.clone(), None if k is None else k.clone()))
+    seen = []
+    rope.register_forward_pre_hook(lambda m, args: seen.append(args[0].shape))
+    rope.register_forward_hook(lambda m, args, out: seen.append(out[0].shape))
+    q = torch.zeros(shape)
+    rope(q, q, torch.arange(5))
+    assert seen == [q.shape, q.shape]
+
+
 def test_rotary_frequencies(k2):
     R, S = k2.RotaryEmbedding, k2.RotaryScaling
     f = R(8, theta=10000.0).frequencies
