@@ -4,9 +4,9 @@
 // head is copied.  The transpose (inverse != 0: t -> -t) is the backward pass.  Pairs lie side by side (interleaved:
 // 2 i, 2 i + 1) or half the rotated part apart (half: i, i + rotary_dim / 2).
 //
-// Angles are products in float64 less their whole turns (a position of 2^24 and more keeps the angle to 1e-8 turns; in
-// float32 it would have no digit left), cos and sin of the rest in float32, and every product and sum of the rotation in
-// float32, rounded once to the tensor's type.
+// Angles are products in float64 less their whole turns, cos and sin of the rest in float32, and every product and sum of
+// the rotation in float32, rounded once to the tensor's type.  The product keeps 2^-53 of |pos turns| (a position of 2^24
+// still has its angle to 3e-10 turns; in float32 it would have no digit left), the rest 2^-26 turns.
 //
 // Bound: reading and writing the heads once.  A workgroup takes a run of (token, head) rows, q's heads before k's in
 // every token; its threads first compute the cos / sin of the run's tokens into LDS, once for all heads, then a thread

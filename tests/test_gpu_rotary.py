@@ -3,6 +3,7 @@
 A rotated value is two products and a sum in float32, with cos and sin of the float64 angle in float32: fewer than six
 roundings of 2^-24 of the pair's length (times the factor), and one to the tensor's type (half its epsilon)."""
 import math
+from decimal import Decimal, localcontext
 
 import pytest
 import torch
@@ -95,6 +96,31 @@ def test_position_types_and_far_positions(k2, dev, dtype):
         length = lambda v: (v[..., :32].double() ** 2 + v[..., 32:].double() ** 2).sqrt()       # noqa: E731
         assert (length(got) - length(t)).abs().max() < 1e-5
     assert torch.equal(got[:, 0], t[:, 0])
+
+
+def _rest(position, frequency):
+    """``position * frequency`` radians less the whole turns, from exact integers and 60 digits of pi."""
+    with localcontext() as c:
+        c.prec = 90
+        turn = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        a = Decimal(position) * Decimal(frequency)          # both binary fractions: exact
+        return float(a - turn * (a / turn).to_integral_value())
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.float64])
+def test_angles_of_far_positions(k2, dev, dtype):
+    """Every angle within the documented bound of the exact one, to a position of 2^44: 3 * 2^-53 of the angle and 2^-26
+    turns; cos and sin in float32 are two units of 2^-24 more, their product with ones and zeros exact."""
+    rope = k2.RotaryEmbedding(64, layout="half")
+    far = [1, 4095, (1 << 20) + 1, (1 << 24) + 1, (1 << 28) - 3, -(1 << 31) + 5, (1 << 37) + 11, (1 << 44) + 3]
+    t = torch.zeros(1, len(far), 1, 64, device=dev)
+    t[..., :32] = 1
+    got = rope(t, None, torch.tensor(far, dtype=dtype, device=dev))[0][0, :, 0].double().cpu()
+    for i, p in enumerate(far):
+        for j, f in enumerate(rope.frequencies):
+            a = _rest(p, f)
+            bound = abs(p * f) * 3 * 2.0 ** -53 + 2 * math.pi * 2.0 ** -26 + 2 * 2.0 ** -24
+            assert abs(got[i, j] - math.cos(a)) <= bound and abs(got[i, j + 32] - math.sin(a)) <= bound, (p, j)
 
 
 @pytest.mark.parametrize("scaling", [("linear", 4.0, None), ("ntk", 8.0, None), ("yarn", 4.0, 2048), ("yarn", 16.0, 32768)])
