@@ -74,6 +74,11 @@ __device__ __forceinline__ float bf16_of(const uint4& v, int i) {
   return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
 }
 
+// v where keep, else zeros: by component (a select between two uint4 objects puts them in scratch memory).
+__device__ __forceinline__ uint4 keep_if(bool keep, uint4 v) {
+  return make_uint4(keep ? v.x : 0u, keep ? v.y : 0u, keep ? v.z : 0u, keep ? v.w : 0u);
+}
+
 // Two values rounded to bf16 by one v_cvt_pk_bf16_f32 (round to nearest even), unpacked in place.
 __device__ __forceinline__ void bf16r2(float& a, float& b) {
   const uint32_t u = pack_bf16x2(a, b);
@@ -512,157 +517,381 @@ void launch_rmsmod_bwd(const NormBwdArgs& a, hipStream_t st) {
 #undef K2Q_RMB
 }
 
+// Columns up to which a wave has a row of its own; twice as many take two waves, more four.
+constexpr int bwd_narrow(int mode) { return mode == BWD_ONCE ? 1024 : 4096; }
+
 template <int MODE>
 void launch_norm_bwd(const NormBwdArgs& a, hipStream_t st) {
-  constexpr int NARROW = MODE == BWD_ONCE ? 1024 : 4096;
+  constexpr int NARROW = bwd_narrow(MODE);
   if (a.K <= NARROW) launch_rmsmod_bwd<MODE, 1>(a, st);
   else if (a.K <= 2 * NARROW) launch_rmsmod_bwd<MODE, 2>(a, st);
   else launch_rmsmod_bwd<MODE, 4>(a, st);
+}
+
+// Whether a launch of the row pass holds M rows: HIP counts its threads in 32 bits.
+bool norm_bwd_fits(int64_t M, int64_t K, int mode) {
+  const int waves = K <= bwd_narrow(mode) ? 1 : K <= 2 * bwd_narrow(mode) ? 2 : 4;
+  return (M * waves + 3) / 4 * 256 <= 0xffffffffll;
 }
 
 // Column sums of the residual norm's backward: the gradients of what is broadcast over the rows of a batch entry,
 //   dscale = sum_m dh n,  dshift = sum_m dh,  dgate = sum_m dR y,  and over every row  dw = sum_m dn x r,
 // with n as in the forward and dn, dR unrounded in f32 (from the row statistics that the pass above left).  Rows are cut
 // into strips of one batch entry each; a workgroup sums one strip of 512 columns (lane: 8 columns, its four waves: every
-// fourth row) into f32 partials, and a second launch adds the strips in order: no atomics, the same result every time.
+// fourth row).  Where an entry is one strip its sums are the gradients and are written here; else they and the sums over
+// every row leave as f32 partials, which a second launch adds in order: no atomics, the same result every time.  Only the
+// sums asked for have partials, one after another in the order below.
+// Entries of a few rows (kFew) are a wave's own, several of them one after another: a strip is then the rows of four waves
+// and spans entries, so the partials of the sums over every row stay few (one strip an entry would leave 4 bytes a sum for
+// every 2 of a row), and no wave is without a row.
+// The form without h's gradient (kStream: dR = dr) also makes dy = bf16(gate dr): it reads every row and column once anyway.
 // Bound by reading dh, r, y and dr once more: 1536 x 6144 in 18.2 us (4.5 TB/s), the join 4.0.
 constexpr int CS_COLS = 512;
 
 struct ColSumArgs {
-  const uint16_t *dh, *dr, *x, *y;   // M x K bf16 (dr: null for none; y: row stride ldy, null: no gate)
+  const uint16_t *dh, *dr, *x, *y;   // M x K bf16 (dr: null for none; y: row stride ldy, null: no gate's gradient)
   const float* stats;                // M pairs
   int64_t M, ldy, rpb;
-  int K, strips, strip_rows;         // strips per batch entry, rows per strip
+  int K, strips, strip_rows;         // strips per batch entry, rows per strip; kFew: rows per wave
   const float* nw;
   float nwadd;
   const uint16_t* mscale;            // or null
   int64_t ldm;
-  float* part;                       // strip-major: (entry * strips + strip) x 4 x K
+  const uint16_t* gate;              // kStream
+  int64_t ldg;
+  uint16_t* dy;
+  int parts, direct;                 // bits of the sums that leave as partials, and of those that are written whole
+  float* part;                       // strip x (the sums of `parts`) x K
+  uint16_t *dscale, *dshift, *dgate; // entries x K
 };
 
 enum { CS_W = 0, CS_SCALE = 1, CS_SHIFT = 2, CS_GATE = 3 };
 
+// Where sum k lies among those of `bits`.
+__device__ __forceinline__ int cs_slot(int bits, int k) { return __popc(bits & ((1 << k) - 1)); }
+
+__device__ __forceinline__ void put8_bf16(uint16_t* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                            pack_bf16x2(v[6], v[7]));
+}
+
+__device__ __forceinline__ void put_direct(const ColSumArgs& a, int64_t entry, int col, const float (&acc)[4][8]) {
+  const int64_t o = entry * a.K + col;
+  if (a.direct & 1 << CS_SCALE) put8_bf16(a.dscale + o, acc[CS_SCALE]);
+  if (a.direct & 1 << CS_SHIFT) put8_bf16(a.dshift + o, acc[CS_SHIFT]);
+  if (a.direct & 1 << CS_GATE) put8_bf16(a.dgate + o, acc[CS_GATE]);
+}
+
+template <bool kStream, bool kFew>
 __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
   __shared__ float red[3][64][33];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int K = a.K;
   const uint32_t tiles = (uint32_t)(K + CS_COLS - 1) / CS_COLS, piece = blockIdx.x / tiles;
   const int col = (int)(blockIdx.x % tiles) * CS_COLS + 8 * lane;
-  const int64_t entry = piece / a.strips;
-  const int strip = piece % a.strips;
-  const int64_t m0 = entry * a.rpb + (int64_t)strip * a.strip_rows;
-  const int64_t mend = (entry + 1) * a.rpb;
-  const int64_t m1 = m0 + a.strip_rows < mend ? m0 + a.strip_rows : mend;
-  const int cc = col < K ? col : 0;
-  float w[8], p1[8], acc[4][8] = {};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = a.nw[cc + i] + a.nwadd;
-    p1[i] = a.mscale ? bf16r(1.f + bf16_bits_to_f32(a.mscale[entry * a.ldm + cc + i])) : 1.f;
+  const bool ok = col < K;
+  const int cc = ok ? col : 0;
+  int64_t entry, m0, m1;
+  if (kFew) {
+    m0 = ((int64_t)piece * 4 + wave) * a.strip_rows;      // a whole number of entries
+    m1 = m0 + a.strip_rows < a.M ? m0 + a.strip_rows : a.M;
+    entry = m0 / a.rpb;
+  } else {
+    entry = piece / a.strips;
+    m0 = entry * a.rpb + (int64_t)(piece % a.strips) * a.strip_rows;
+    const int64_t mend = (entry + 1) * a.rpb;
+    m1 = m0 + a.strip_rows < mend ? m0 + a.strip_rows : mend;
+    m0 += wave;
   }
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  // what is absent is read as x: no branch between a row's loads (45.7 -> 43.7 us with both passes, 1536 x 6144)
-  const uint16_t *yp = a.y ? a.y : a.x, *rp = a.y && a.dr ? a.dr : a.x;
+  float w[8], p1[8], acc[4][8] = {}, tot[4][8] = {};
+  const uint16_t* vec = kStream ? a.gate : a.mscale;      // the entries' vector
+  const int64_t ldv = kStream ? a.ldg : a.ldm;
+  if (!kStream)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = a.nw[cc + i] + a.nwadd;
+  auto set_entry = [&](const uint4& v) {      // p1: bf16(1 + the modulation), or the gate
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p1[i] = kStream ? bf16_of(v, i) : vec ? bf16r(1.f + bf16_of(v, i)) : 1.f;
+  };
+  // what is absent is read as x (dr): no branch between a row's loads (45.7 -> 43.7 us with both passes, 1536 x 6144)
+  const uint16_t* x = kStream ? a.dr : a.x;
+  const uint16_t *yp = a.y ? a.y : x, *rp = !kStream && a.y && a.dr ? a.dr : x;
   const int64_t ly = a.y ? a.ldy : K;
-  for (int64_t m = m0 + wave; m < m1; m += 4) {
-    const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * m);
-    const uint4 dv = *reinterpret_cast<const uint4*>(a.dh + m * K + cc);
-    const uint4 xv = *reinterpret_cast<const uint4*>(a.x + m * K + cc);
-    uint4 yv = *reinterpret_cast<const uint4*>(yp + m * ly + cc), rv = *reinterpret_cast<const uint4*>(rp + m * K + cc);
-    if (!a.y) yv = zero;
-    if (!a.y || !a.dr) rv = zero;
+  struct Row {
+    uint4 d, x, y, r, v;
+    float2 st;
+  };
+  auto load = [&](int64_t m, int64_t e) {
+    Row t;
+    t.x = *reinterpret_cast<const uint4*>(x + m * K + cc);
+    t.y = *reinterpret_cast<const uint4*>(yp + m * ly + cc);
+    if (!kStream) {
+      t.st = *reinterpret_cast<const float2*>(a.stats + 2 * m);
+      t.d = *reinterpret_cast<const uint4*>(a.dh + m * K + cc);
+      t.r = *reinterpret_cast<const uint4*>(rp + m * K + cc);
+    }
+    if (kFew && vec) t.v = *reinterpret_cast<const uint4*>(vec + e * ldv + cc);
+    return t;
+  };
+  auto add = [&](int64_t m, Row t) {
+    t.y = keep_if(a.y, t.y);
+    if (kStream) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float dR = bf16_of(t.x, i);
+        e[i] = p1[i] * dR;
+        acc[CS_GATE][i] = __builtin_fmaf(dR, bf16_of(t.y, i), acc[CS_GATE][i]);
+      }
+      if (a.dy && ok) put8_bf16(a.dy + m * K + col, e);
+      return;
+    }
+    t.r = keep_if(a.y && a.dr, t.r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float d = bf16_of(dv, i), x = bf16_of(xv, i);
-      const float dn = d * p1[i], xr = x * st.x;
+      const float d = bf16_of(t.d, i), xv = bf16_of(t.x, i);
+      const float dn = d * p1[i], xr = xv * t.st.x;
       acc[CS_W][i] = __builtin_fmaf(dn, xr, acc[CS_W][i]);
       acc[CS_SCALE][i] = __builtin_fmaf(d, bf16r(xr * w[i]), acc[CS_SCALE][i]);
       acc[CS_SHIFT][i] += d;
-      const float dR = bf16_of(rv, i) + (dn * w[i] * st.x - x * st.y);
-      acc[CS_GATE][i] = __builtin_fmaf(dR, bf16_of(yv, i), acc[CS_GATE][i]);
+      const float dR = bf16_of(t.r, i) + (dn * w[i] * t.st.x - xv * t.st.y);
+      acc[CS_GATE][i] = __builtin_fmaf(dR, bf16_of(t.y, i), acc[CS_GATE][i]);
     }
+  };
+  if (kFew) {
+    if (m0 < m1) {
+      Row next = load(m0, entry);
+      int64_t left = a.rpb;
+      for (int64_t m = m0; m < m1; ++m) {
+        const Row t = next;
+        const bool last = --left == 0;
+        if (m + 1 < m1) next = load(m + 1, last ? entry + 1 : entry);
+        set_entry(t.v);
+        add(m, t);
+        if (!last) continue;
+        if (ok) put_direct(a, entry, col, acc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            tot[k][i] += acc[k][i];
+            acc[k][i] = 0.f;
+          }
+        left = a.rpb;
+        ++entry;
+      }
+    }
+    if (!a.parts) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[k][i] = tot[k][i];
+  } else {
+    set_entry(vec ? *reinterpret_cast<const uint4*>(vec + entry * ldv + cc) : make_uint4(0, 0, 0, 0));
+    for (int64_t m = m0; m < m1; m += 4) add(m, load(m, entry));
+    if (!(a.parts | a.direct)) return;
   }
   if (wave)
 #pragma unroll
     for (int i = 0; i < 32; ++i) red[wave - 1][lane][i] = acc[i >> 3][i & 7];
   __syncthreads();
-  if (wave || col >= K) return;
-  float* out = a.part + (int64_t)piece * 4 * K + col;
+  if (wave || !ok) return;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      out[(int64_t)k * K + i] = ((acc[k][i] + red[0][lane][8 * k + i]) + red[1][lane][8 * k + i]) + red[2][lane][8 * k + i];
+      acc[k][i] = ((acc[k][i] + red[0][lane][8 * k + i]) + red[1][lane][8 * k + i]) + red[2][lane][8 * k + i];
+  if (!kFew) put_direct(a, entry, col, acc);
+  float* out = a.part + (int64_t)piece * __popc(a.parts) * K + col;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (a.parts & 1 << k) {
+      float4* o = reinterpret_cast<float4*>(out + (int64_t)cs_slot(a.parts, k) * K);
+      o[0] = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
+      o[1] = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+    }
+}
+
+// Many partials of the sums over every row: 64 of them folded into one, 64 columns of one sum a workgroup, its four waves
+// every fourth partial, then the waves in order.  With the join behind it a value passes 16 + 4 and then a sixteenth of
+// the folded ones' additions, however many entries there are.
+constexpr int CS_FOLD = 64;
+
+__global__ __launch_bounds__(256) void resnorm_colsum_fold_kernel(const float* part, int K, int64_t pieces, int sums,
+                                                                  float* out) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t tiles = (uint32_t)(K + 63) / 64, per = tiles * sums;
+  const uint32_t group = blockIdx.x / per;
+  const int sum = (int)(blockIdx.x % per / tiles), col = (int)(blockIdx.x % tiles) * 64 + lane;
+  const int64_t i0 = (int64_t)group * CS_FOLD, i1 = i0 + CS_FOLD < pieces ? i0 + CS_FOLD : pieces;
+  float f = 0.f;
+  if (col < K) {
+#pragma unroll 8
+    for (int64_t i = i0 + wave; i < i1; i += 4) f += part[(i * sums + sum) * K + col];
+  }
+  red[wave][lane] = f;
+  __syncthreads();
+  if (wave || col >= K) return;
+  out[((int64_t)group * sums + sum) * K + col] = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
 }
 
 // The strips' partials joined: 64 columns a workgroup, its NW waves every NW-th strip, then the waves in order.  Column
 // tiles of the batch entries (the bits of `per_entry`: scale, shift and gate gradients, bf16), then those of the sums over
-// every entry (`whole`: the norm weight's, f32, and those of a vector that every entry shares).
+// every entry (`whole`: the norm weight's, f32, and those of a vector that every entry shares), which are sums over
+// `pieces` partials.  `parts`: the sums that have partials.
+struct JoinArgs {
+  const float* part;
+  int K, strips, parts, per_entry, whole;
+  int64_t entries, pieces;            // entries: 0 where only `whole` is joined
+  float* dnw;
+  uint16_t *dscale, *dshift, *dgate;
+};
+
+// NS sums (at `off` of a strip's partials) of the strips from i in steps of NW: the loads of eight strips are issued
+// together (four by four waves, which have no more of an entry), those past the end repeat the first and add nothing.
+template <int NS, int NW>
+__device__ __forceinline__ void join_strips(const float* p, int64_t i, int64_t end, int64_t stride, const int (&off)[4],
+                                            float (&f)[4]) {
+  constexpr int U = NW < 16 ? 4 : 8, step = NW;
+  for (; i < end; i += U * step) {
+    float v[U][NS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* q = p + (i + u * step < end ? i + u * step : i) * stride;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) v[u][s] = q[off[s]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) f[s] += i + u * step < end ? v[u][s] : 0.f;
+  }
+}
+
 template <int NW>
-__global__ __launch_bounds__(64 * NW) void resnorm_colsum_join_kernel(const float* part, int K, int64_t entries, int strips,
-                                                                  int per_entry, int whole, float* dnw, uint16_t* dscale,
-                                                                  uint16_t* dshift, uint16_t* dgate) {
+__global__ __launch_bounds__(64 * NW) void resnorm_colsum_join_kernel(JoinArgs a) {
   __shared__ float red[4][NW][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = a.K;
   const uint32_t tiles = (uint32_t)(K + 63) / 64;
   const int col = (int)(blockIdx.x % tiles) * 64 + lane;
   const int64_t entry = blockIdx.x / tiles;
-  const bool all = entry == entries;
-  const int want = all ? whole : per_entry;
+  const bool all = entry == a.entries;
+  const int want = all ? a.whole : a.per_entry;
   if (!want) return;
-  const int64_t i0 = all ? 0 : entry * strips, i1 = all ? entries * strips : i0 + strips;
+  const int64_t i0 = (all ? 0 : entry * a.strips) + wave, i1 = all ? a.pieces : (entry + 1) * a.strips;
+  const int64_t stride = (int64_t)__popc(a.parts) * K;
+  const float* p = a.part + (col < K ? col : 0);
+  int off[4] = {};
   float f[4] = {};
-  if (col < K) {
-    if (want == 1 << CS_W) {
-#pragma unroll 8
-      for (int64_t i = i0 + wave; i < i1; i += NW) f[CS_W] += part[(i * 4 + CS_W) * K + col];
-    } else {
-#pragma unroll 4
-      for (int64_t i = i0 + wave; i < i1; i += NW)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k != CS_W || want & 1 << CS_W) f[k] += part[(i * 4 + k) * K + col];
-    }
+  for (int s = 0, rest = want; s < 4; ++s, rest &= rest - 1)
+    if (rest) off[s] = cs_slot(a.parts, __ffs(rest) - 1) * K;
+  switch (__popc(want)) {
+    case 1: join_strips<1, NW>(p, i0, i1, stride, off, f); break;
+    case 2: join_strips<2, NW>(p, i0, i1, stride, off, f); break;
+    case 3: join_strips<3, NW>(p, i0, i1, stride, off, f); break;
+    default: join_strips<4, NW>(p, i0, i1, stride, off, f);
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) red[k][wave][lane] = f[k];
+  for (int s = 0; s < 4; ++s) red[s][wave][lane] = f[s];
   __syncthreads();
   if (wave || col >= K) return;
+  const int64_t o = all ? col : entry * K + col;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    f[k] = red[k][0][lane];
+    if (!(want & 1 << k)) continue;
+    const int s = cs_slot(want, k);
+    float t = red[s][0][lane];
 #pragma unroll
-    for (int v = 1; v < NW; ++v) f[k] += red[k][v][lane];
+    for (int v = 1; v < NW; ++v) t += red[s][v][lane];
+    if (k == CS_W) a.dnw[o] = t;
+    else (k == CS_SCALE ? a.dscale : k == CS_SHIFT ? a.dshift : a.dgate)[o] = (uint16_t)f32_to_bf16_bits(t);
   }
-  const int64_t o = all ? col : entry * K + col;
-  if (want & 1 << CS_W) dnw[o] = f[CS_W];
-  if (want & 1 << CS_SCALE) dscale[o] = (uint16_t)f32_to_bf16_bits(f[CS_SCALE]);
-  if (want & 1 << CS_SHIFT) dshift[o] = (uint16_t)f32_to_bf16_bits(f[CS_SHIFT]);
-  if (want & 1 << CS_GATE) dgate[o] = (uint16_t)f32_to_bf16_bits(f[CS_GATE]);
 }
 
-// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 256 strips of 6144 columns 101 / 87,
-// 300 entries of one strip and 4096 columns 97 / 142).
-void launch_join(const float* part, int64_t K, int64_t entries, int strips, int asked, int over, float* dnorm,
-                 uint16_t* dscale, uint16_t* dshift, uint16_t* dgate, hipStream_t st) {
-  const dim3 grid((unsigned)((K + 63) / 64 * (entries + 1)));
-  if (strips >= 16)
-    hipLaunchKernelGGL(resnorm_colsum_join_kernel<16>, grid, dim3(1024), 0, st, part, (int)K, entries, strips, asked & ~over,
-                       asked & over, dnorm, dscale, dshift, dgate);
-  else
-    hipLaunchKernelGGL(resnorm_colsum_join_kernel<4>, grid, dim3(256), 0, st, part, (int)K, entries, strips, asked & ~over,
-                       asked & over, dnorm, dscale, dshift, dgate);
+// The gradients that are sums over rows: which are asked for, where they go, and the partials' memory.
+struct ColOut {
+  int asked, whole;                  // bits asked for; of those, the sums over every entry
+  float* dnw;
+  uint16_t *dscale, *dshift, *dgate;
+  float* part;
+};
+
+int64_t fold_groups(int64_t pieces) { return (pieces + CS_FOLD - 1) / CS_FOLD; }
+constexpr int64_t CS_MANY = 1024;    // partials that one join adds
+
+// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 256 strips of 6144 columns 101 / 87),
+// or where the strips' entries are written already (`direct`) and only the sums over every entry are left.  Which of the
+// gradients are asked for changes no order.
+void launch_join(const ColOut& c, int parts, bool direct, int64_t K, int64_t entries, int strips, int64_t pieces,
+                 hipStream_t st) {
+  const int per_entry = direct ? 0 : c.asked & ~c.whole;
+  JoinArgs a{c.part, (int)K, strips, parts, per_entry, c.asked & c.whole, per_entry ? entries : 0, pieces, c.dnw, c.dscale,
+             c.dshift, c.dgate};
+  const int64_t tiles = (K + 63) / 64;
+  if (direct && pieces > CS_MANY) {
+    const int sums = __builtin_popcount(parts);
+    const int64_t groups = fold_groups(pieces);
+    float* folded = c.part + pieces * sums * K;
+    hipLaunchKernelGGL(resnorm_colsum_fold_kernel, dim3((unsigned)(tiles * sums * groups)), dim3(256), 0, st, c.part, (int)K,
+                       pieces, sums, folded);
+    a.part = folded;
+    a.pieces = groups;
+  }
+  const dim3 grid((unsigned)(tiles * (a.entries + 1)));
+  if (strips >= 16 || direct) hipLaunchKernelGGL(resnorm_colsum_join_kernel<16>, grid, dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL(resnorm_colsum_join_kernel<4>, grid, dim3(256), 0, st, a);
 }
+
+struct ColPlan {
+  bool few;
+  int strips, rows;                  // per entry; rows per strip, or per wave where `few`
+  int64_t pieces;
+};
 
 // Strips per batch entry: about two workgroups a CU over the column tiles, at least 16 rows each (all three passes, us, at
 // 8 / 16 / 32 rows: 333 x 2560 17.3 / 16.3 / 17.5, 4 x 64 x 1024 11.6 / 11.8 / 13.6, 2 x 1000 x 512 23.3 / 18.9 / 18.5).
-int colsum_strips(int64_t rpb, int64_t K, int64_t entries, int cus) {
-  const int64_t tiles = (K + CS_COLS - 1) / CS_COLS * entries;
-  int64_t s = (2 * cus + tiles - 1) / tiles;
+// Entries of fewer rows than that, where every wave of a workgroup has one: as many workgroups, a wave's entries at least
+// four rows.
+ColPlan colsum_plan(int64_t rpb, int64_t K, int64_t entries, int cus) {
+  const int64_t tiles = (K + CS_COLS - 1) / CS_COLS;
+  if (rpb < 16 && entries >= 4) {
+    const int64_t wgs = (2 * cus + tiles - 1) / tiles, least = (3 + rpb) / rpb;
+    int64_t own = (entries + 4 * wgs - 1) / (4 * wgs);      // entries per wave
+    own = own < least ? least : own;
+    return {true, 1, (int)(own * rpb), (entries + 4 * own - 1) / (4 * own)};
+  }
+  int64_t s = (2 * cus + tiles * entries - 1) / (tiles * entries);
   const int64_t most = (rpb + 15) / 16;
   s = s < 1 ? 1 : s > most ? most : s;
-  const int64_t rows = (rpb + s - 1) / s;
-  return (int)((rpb + rows - 1) / rows);
+  int64_t rows = (rpb + s - 1) / s;
+  s = (rpb + rows - 1) / rows;
+  rows = (rpb + s - 1) / s;
+  return {false, (int)s, (int)rows, entries * s};
+}
+
+// Floats of partials, at most: every sum, folded ones behind them.
+int64_t colsum_floats(const ColPlan& p, int64_t K) {
+  return (p.pieces + (p.pieces > CS_MANY ? fold_groups(p.pieces) : 0)) * 4 * K;
+}
+
+// The column pass and its join.  `a` holds the operands.
+template <bool kStream>
+void launch_colsum(ColSumArgs a, const ColOut& c, const ColPlan& p, int64_t entries, hipStream_t st) {
+  const int per_entry = c.asked & ~c.whole, direct = p.strips == 1 ? per_entry : 0;
+  a.strips = p.strips;
+  a.strip_rows = p.rows;
+  a.direct = direct;
+  a.parts = c.asked & ~direct;
+  a.part = c.part;
+  a.dscale = c.dscale;
+  a.dshift = c.dshift;
+  a.dgate = c.dgate;
+  const dim3 grid((unsigned)((a.K + CS_COLS - 1) / CS_COLS * p.pieces));
+  if (p.few) hipLaunchKernelGGL((resnorm_colsum_kernel<kStream, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((resnorm_colsum_kernel<kStream, false>), grid, dim3(256), 0, st, a);
+  if (a.parts) launch_join(c, a.parts, p.strips == 1, a.K, entries, p.strips, p.pieces, st);
 }
 
 // The row pass that rounds once and its column sums in one, which reads dh, r, y and dr once: a workgroup a CU owns a strip
@@ -778,7 +1007,7 @@ __global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a,
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (asked & 1 << k) {
-        float4* out = reinterpret_cast<float4*>(part + ((int64_t)blockIdx.x * 4 + k) * K + col);
+        float4* out = reinterpret_cast<float4*>(part + ((int64_t)blockIdx.x * __popc(asked) + cs_slot(asked, k)) * K + col);
         out[0] = make_float4(acc[c][k][0], acc[c][k][1], acc[c][k][2], acc[c][k][3]);
         out[1] = make_float4(acc[c][k][4], acc[c][k][5], acc[c][k][6], acc[c][k][7]);
       }
@@ -940,10 +1169,27 @@ extern "C" int k2q_swiglu_bwd(const uint16_t* dh, const uint16_t* gate, const ui
 extern "C" int64_t k2q_resnorm_bwd_ws_bytes(int64_t M, int64_t K, int64_t rows_per_batch) {
   if (M < 1 || K < 8 || K % 8 || K > 16384 || rows_per_batch < 1 || M % rows_per_batch) return 0;
   const int64_t entries = M / rows_per_batch;
-  const int cus = k2q_cu_count(), two = colsum_strips(rows_per_batch, K, entries, cus),
-            one = fused_strips(rows_per_batch, K, entries, cus);
-  return (stats_floats(M) + entries * (two > one ? two : one) * 4 * K) * 4;
+  const int cus = k2q_cu_count();
+  const int64_t two = colsum_floats(colsum_plan(rows_per_batch, K, entries, cus), K),
+                one = entries * fused_strips(rows_per_batch, K, entries, cus) * 4 * K;
+  return (stats_floats(M) + (two > one ? two : one)) * 4;
 }
+
+namespace {
+
+// The sums asked for; those of `shared` vectors (and the norm weight's always) are over every entry.
+ColOut col_out(float* dnorm, uint16_t* dscale, uint16_t* dshift, uint16_t* dgate, int shared, int64_t entries, float* part) {
+  const int asked = (dnorm ? 1 << CS_W : 0) | (dscale ? 1 << CS_SCALE : 0) | (dshift ? 1 << CS_SHIFT : 0) |
+                    (dgate ? 1 << CS_GATE : 0);
+  const int whole = 1 << CS_W | (entries == 1 ? 0 : (shared & K2Q_SHARED_SCALE ? 1 << CS_SCALE : 0) |
+                                                        (shared & K2Q_SHARED_SHIFT ? 1 << CS_SHIFT : 0) |
+                                                        (shared & K2Q_SHARED_GATE ? 1 << CS_GATE : 0));
+  return {asked, whole, dnorm, dscale, dshift, dgate, part};
+}
+
+bool shared_ok(int shared) { return shared >= 0 && shared <= (K2Q_SHARED_SCALE | K2Q_SHARED_SHIFT | K2Q_SHARED_GATE); }
+
+}  // namespace
 
 extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, int64_t M, int64_t K,
                                const float* norm_scale, float scale_add, float eps, const uint16_t* mod_scale,
@@ -955,18 +1201,17 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   if (K > 16384 || M > 0x7fffffff) return K2Q_EUNSUPPORTED;
   if (!dh || !r || !norm_scale || !dx || !k2q_aligned(dh, 16) || !k2q_aligned(dr, 16) || !k2q_aligned(r, 16) ||
       !k2q_aligned(norm_scale, 16) || !k2q_aligned(dx, 16) || !k2q_aligned(dy, 16) || !rowvec_ok(mod_scale, ld_scale) ||
-      !rowvec_ok(gate, ld_gate) || rows_per_batch < 1 || !(eps >= 0.f) || !gate != !dy || shared < 0 ||
-      shared > (K2Q_SHARED_SCALE | K2Q_SHARED_SHIFT | K2Q_SHARED_GATE))
+      !rowvec_ok(gate, ld_gate) || rows_per_batch < 1 || !(eps >= 0.f) || !gate != !dy || !shared_ok(shared))
     return K2Q_EINVAL;
   const bool cols = dnorm || dscale || dshift || dgate;
   const int64_t entries = M / rows_per_batch;
   if (cols) {
     if (M % rows_per_batch || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_resnorm_bwd_ws_bytes(M, K, rows_per_batch) ||
-        ((dscale || dshift) && !mod_scale) || (dgate && (!gate || !y || !k2q_aligned(y, 16) || ldy < K || ldy % 8)))
+        ((dscale || dshift) && !mod_scale) || !k2q_aligned(dscale, 16) || !k2q_aligned(dshift, 16) ||
+        !k2q_aligned(dgate, 16) || (dgate && (!gate || !y || !k2q_aligned(y, 16) || ldy < K || ldy % 8)))
       return K2Q_EINVAL;
   }
-  // launch extents: column tiles by entries and strips (fewer than 1024 strips in all beyond one an entry)
-  if (cols && (K + 63) / 64 * (entries + 1024) > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  if (!norm_bwd_fits(M, K, eager ? BWD_EAGER : BWD_ONCE)) return K2Q_EUNSUPPORTED;
   NormBwdArgs a{};
   a.dh = dh;
   a.x = r;
@@ -985,23 +1230,18 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   a.dy = dy;
   a.stats = cols ? static_cast<float*>(ws) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int asked = (dnorm ? 1 << CS_W : 0) | (dscale ? 1 << CS_SCALE : 0) | (dshift ? 1 << CS_SHIFT : 0) |
-                    (dgate ? 1 << CS_GATE : 0);
-  const int over = 1 << CS_W | (entries == 1 ? 0 : (shared & K2Q_SHARED_SCALE ? 1 << CS_SCALE : 0) |
-                                                       (shared & K2Q_SHARED_SHIFT ? 1 << CS_SHIFT : 0) |
-                                                       (shared & K2Q_SHARED_GATE ? 1 << CS_GATE : 0));
+  const ColOut out = col_out(dnorm, dscale, dshift, dgate, shared, entries, cols ? a.stats + stats_floats(M) : nullptr);
   const int fs = cols && !eager ? fused_strips(rows_per_batch, K, entries, k2q_cu_count()) : 0;
   if (fs) {
     const int rows = (int)((rows_per_batch + fs - 1) / fs);
-    float* part = a.stats + stats_floats(M);
 #define K2Q_RBC(N)                                                                                                        \
   hipLaunchKernelGGL(resnorm_bwd_cols_kernel<N>, dim3((unsigned)(entries * fs)), dim3(256), 0, st, a, dgate ? y : nullptr, \
-                     ldy, fs, rows, asked, part)
+                     ldy, fs, rows, out.asked, out.part)
     if (K <= 4096) K2Q_RBC(2);
     else if (K <= 6144) K2Q_RBC(3);
     else K2Q_RBC(4);
 #undef K2Q_RBC
-    launch_join(part, K, entries, fs, asked, over, dnorm, dscale, dshift, dgate, st);
+    launch_join(out, out.asked, false, K, entries, fs, entries * fs, st);
     return k2q_launch_status();
   }
   if (eager) launch_norm_bwd<BWD_EAGER>(a, st);
@@ -1017,15 +1257,10 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   c.ldy = ldy;
   c.rpb = rows_per_batch;
   c.K = (int)K;
-  c.strips = colsum_strips(rows_per_batch, K, entries, k2q_cu_count());
-  c.strip_rows = (int)((rows_per_batch + c.strips - 1) / c.strips);
   c.nw = norm_scale;
   c.nwadd = scale_add;
   c.mscale = mod_scale;
   c.ldm = ld_scale;
-  c.part = a.stats + stats_floats(M);
-  const int64_t grid = (K + CS_COLS - 1) / CS_COLS * entries * c.strips;
-  hipLaunchKernelGGL(resnorm_colsum_kernel, dim3((unsigned)grid), dim3(256), 0, st, c);
-  launch_join(c.part, K, entries, c.strips, asked, over, dnorm, dscale, dshift, dgate, st);
+  launch_colsum<false>(c, out, colsum_plan(rows_per_batch, K, entries, k2q_cu_count()), entries, st);
   return k2q_launch_status();
 }

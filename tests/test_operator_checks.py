@@ -84,6 +84,20 @@ def test_entry_points_refuse_bad_arguments(k2):
     assert rot(D=8192) == -4 and rot(D=4096, dim=2048) == -4 and rot(B=1 << 20, L=1 << 20) == -4
 
 
+def test_residual_norm_workspace_is_small(k2):
+    """The partial sums never exceed the tensors that they are sums of (an entry per row: 16 bytes of four sums an element
+    once), however the rows are cut."""
+    lib = k2._lib.load()
+    for K in (128, 640, 2304, 6144, 16384):
+        for rpb in (1, 2, 3, 7, 15, 16, 17, 40, 333):
+            for entries in (1, 3, 64, 999, 9216):
+                M = rpb * entries
+                if M < 4096:
+                    continue
+                ws = lib.k2q_resnorm_bwd_ws_bytes(M, K, rpb)
+                assert ws <= 2 * M * K + 16 * M, (M, K, rpb, ws)
+
+
 def test_w4_gemv_needs_no_workspace(k2):
     lib = k2._lib.load()
     for M in range(1, 9):
