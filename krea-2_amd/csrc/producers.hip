@@ -912,7 +912,6 @@ __global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a,
   // what is absent is read as x
   const uint16_t *yp = y ? y : a.x, *rp = a.dr ? a.dr : a.x;
   const int64_t ly = y ? ldy : K;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
   float w[kNCH][8], acc[kNCH][4][8] = {};
   uint4 pv[kNCH], gg[kNCH];
 #pragma unroll
@@ -920,8 +919,8 @@ __global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a,
     const int col = 8 * t + 2048 * c, cc = col < K ? col : 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[c][i] = a.nw[cc + i] + a.nwadd;
-    pv[c] = a.mscale ? *reinterpret_cast<const uint4*>(a.mscale + entry * a.ldm + cc) : zero;
-    gg[c] = mg ? *reinterpret_cast<const uint4*>(mg + cc) : zero;
+    pv[c] = a.mscale ? *reinterpret_cast<const uint4*>(a.mscale + entry * a.ldm + cc) : make_uint4(0, 0, 0, 0);
+    gg[c] = mg ? *reinterpret_cast<const uint4*>(mg + cc) : make_uint4(0, 0, 0, 0);
   }
   uint4 xn[kNCH], dn[kNCH], rn[kNCH], yn[kNCH];
   auto load = [&](int64_t m) {
@@ -941,10 +940,10 @@ __global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a,
 #pragma unroll
     for (int c = 0; c < kNCH; ++c) {
       const bool ok = 8 * t + 2048 * c < K;
-      xv[c] = ok ? xn[c] : zero;
-      dv[c] = ok ? dn[c] : zero;
-      rv[c] = a.dr ? rn[c] : zero;
-      yv[c] = y ? yn[c] : zero;
+      xv[c] = keep_if(ok, xn[c]);
+      dv[c] = keep_if(ok, dn[c]);
+      rv[c] = keep_if(a.dr, rn[c]);
+      yv[c] = keep_if(y, yn[c]);
     }
     load(m + 1 < m1 ? m + 1 : m);
 #pragma unroll
