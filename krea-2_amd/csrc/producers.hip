@@ -749,12 +749,13 @@ struct JoinArgs {
 };
 
 // NS sums (at `off` of a strip's partials) of the strips from i in steps of NW: the loads of eight strips are issued
-// together (four by four waves, which have no more of an entry), those past the end repeat the first and add nothing.
+// together (four of several sums by four waves, which have no more of an entry), those past the end repeat the first and add nothing; a last one goes
+// alone (64 x 32 x 6144, a strip a wave: 47.6 us with the repeats).
 template <int NS, int NW>
 __device__ __forceinline__ void join_strips(const float* p, int64_t i, int64_t end, int64_t stride, const int (&off)[4],
                                             float (&f)[4]) {
-  constexpr int U = NW < 16 ? 4 : 8, step = NW;
-  for (; i < end; i += U * step) {
+  constexpr int U = NW < 16 && NS > 1 ? 4 : 8, step = NW;
+  for (; i + step < end; i += U * step) {
     float v[U][NS];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -767,6 +768,9 @@ __device__ __forceinline__ void join_strips(const float* p, int64_t i, int64_t e
 #pragma unroll
       for (int s = 0; s < NS; ++s) f[s] += i + u * step < end ? v[u][s] : 0.f;
   }
+  if (i < end)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) f[s] += p[i * stride + off[s]];
 }
 
 template <int NW>
@@ -898,8 +902,10 @@ void launch_colsum(ColSumArgs a, const ColOut& c, const ColPlan& p, int64_t entr
 // of one entry's rows, a lane the same columns of every row (those of the row pass with four waves, whose row sums and
 // results it repeats bit for bit), so its column sums stay in registers (one wave per SIMD has 512) and no wave meets
 // another over them.  Both row sums cross the waves behind one barrier (neither needs the other's result) while the next
-// row is loaded (without: 47.6 us for 42.0).  Two passes / this one, with the join, us: 2 x 768 x 6144 43.4 / 35.4, 4608 x
-// 6144 102 / 87, 9216 x 6144 211 / 151, 4096 x 8192 118 / 102, 1024 x 6144 30.3 / 30.5, 768 x 6144 26.4 / 27.2.
+// row is loaded (without: 47.6 us for 42.0).  Two passes / this one, with the join, us: 9216 x 6144 201 / 152, 4608 x 6144
+// 100 / 84, 2 x 768 x 6144 41.6 / 35.8, 1024 x 6144 30.1 / 28.6, 768 x 6144 25.7 / 25.6, 4096 x 8192 121 / 100, 768 x 8192
+// 30.1 / 31.0, 768 x 2560 18.1 / 18.1, 16 x 128 x 6144 50.9 / 46.3, 64 x 32 x 6144 49.5 / 44.6, 200 x 64 x 2560 118 / 108;
+// for the norm weight's gradient alone 2 x 768 x 6144 36.7 / 26.7, 768 x 6144 21.9 / 19.0.
 template <int kNCH>
 __global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a, const uint16_t* y, int64_t ldy, int strips,
                                                                   int strip_rows, int asked, float* part) {
@@ -1016,12 +1022,14 @@ __global__ __launch_bounds__(256, 1) void resnorm_bwd_cols_kernel(NormBwdArgs a,
 // The workspace: row statistics, then the partials, 16-byte aligned.
 int64_t stats_floats(int64_t M) { return (2 * M + 3) / 4 * 4; }
 
-// Strips per entry of that pass, one workgroup a CU of at least four rows each; 0 (the two passes) where they would leave a
-// quarter of the CUs idle, or the columns are not the four-wave row pass's or too many for the registers.
+// Strips per entry of that pass, one workgroup a CU of at least four rows each, eight where there are more than eight entries
+// (their partials are joined one by one, where the two passes write a short entry's sums at once: 64 x 16 x 6144 29.2 / 31.9
+// us, 128 x 8 x 6144 30.1 / 37.5, 200 x 8 x 6144 46.3 / 47.5); 0 (the two passes) where they would leave a quarter of the CUs
+// idle, or the columns are not the four-wave row pass's or too many for the registers.
 int fused_strips(int64_t rpb, int64_t K, int64_t entries, int cus) {
   if (K <= 2048 || K > 8192) return 0;
   int64_t s = cus / entries;
-  const int64_t most = rpb / 4;
+  const int64_t most = rpb / (entries > 8 ? 8 : 4);
   s = s > most ? most : s;
   if (s < 1 || 4 * entries * s < 3 * cus) return 0;
   const int64_t rows = (rpb + s - 1) / s;
