@@ -130,6 +130,12 @@ int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uint16_t* r, i
                     const uint16_t* y, int64_t ldy, float* dnorm, uint16_t* dscale, uint16_t* dshift, uint16_t* dgate,
                     int shared, void* ws, int64_t ws_bytes, void* stream);
 
+/* The same where h has no gradient: dx is dr itself, dscale, dshift and dnorm are zeros, and in one pass dy = bf16(gate * dr)
+ * (nullable) and dgate = sum dr y (nullable; y and ws, as above, where it is given).  M a multiple of rows_per_batch. */
+int k2q_resnorm_stream_bwd(const uint16_t* dr, int64_t M, int64_t K, const uint16_t* gate, int64_t ld_gate,
+                           int64_t rows_per_batch, uint16_t* dy, const uint16_t* y, int64_t ldy, uint16_t* dgate,
+                           int shared, void* ws, int64_t ws_bytes, void* stream);
+
 /* Rotary positions of queries and keys (mmdit.py:13-30, between the projections and the attention): every pair (a, b) of
  * the first rotary_dim values of a head turns by its token's angle, the rest of the head is copied:
  *   (a, b) -> factor (a cos t - b sin t, a sin t + b cos t),  t = 2 pi pos[axis[i]] turns[i],  i < rotary_dim / 2.

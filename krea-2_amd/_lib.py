@@ -82,6 +82,7 @@ _SIGNATURES = {
     "k2q_resnorm_bwd_ws_bytes": ([_i64, _i64, _i64], _i64),
     "k2q_resnorm_bwd": ([_p, _p, _p, _i64, _i64, _p, _f32, _f32, _p, _i64, _p, _i64, _i64, _int, _p, _p, _p, _i64, _p,
                          _p, _p, _p, _int, _p, _i64, _p], _int),
+    "k2q_resnorm_stream_bwd": ([_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _int, _p, _i64, _p], _int),
     "k2q_rotary": ([_p, _i64, _int, _i64, _i64, _i64, _i64, _int, _p, _int, _i64, _i64, _i64, _p, _p, _f32, _int, _p],
                    _int),
     "k2q_lora_down_ws_bytes": ([_i64, _i64, _i64], _i64),
@@ -540,6 +541,32 @@ def resnorm_bwd(dh, dr, r, w, add: float, eps: float, scale, gate, rows_per_entr
     return _refused(out, "k2q_resnorm_bwd", lambda: _native.resnorm_bwd(*args),
                     lambda: _check_resnorm_bwd(dh, dr, r, w, scale, gate, rows_per_entry, y, need_scale or need_shift,
                                                shift_entries))
+
+
+def _check_resnorm_stream(dr, gate, rows_per_entry, y) -> None:
+    _need(dr, "dr", torch.bfloat16)
+    K = dr.shape[-1]
+    flat = dr.reshape(-1, K)
+    _check_k(K)
+    if rows_per_entry < 1 or flat.shape[0] % rows_per_entry:
+        raise ValueError(f"{flat.shape[0]} rows do not split into entries of {rows_per_entry}")
+    _check_entries(gate.reshape(-1, K) if gate.numel() % K == 0 else gate, "gate", K, flat.shape[0] // rows_per_entry, dr.device)
+    if y is not None:
+        if y.shape != dr.shape:
+            raise ValueError("y and dr differ in shape")
+        _need_rows(y if y.dim() == 2 else y.reshape(flat.shape), "y", dr.device)
+    _device_check(dr.device)
+
+
+def resnorm_stream_bwd(dr, gate, rows_per_entry: int, y=None, need_dy=True):
+    """:func:`resnorm_bwd` where h has no gradient (``k2q_resnorm_stream_bwd``): ``(dy, dgate)`` from the gradient of r, dy (r's
+    shape) where asked for, dgate (the gate's shape) where ``y`` is given.  dx is ``dr``."""
+    args = (dr, gate, rows_per_entry, y, need_dy)
+    out = _fast().resnorm_stream_bwd(*args)
+    if out.__class__ is tuple:
+        return out
+    return _refused(out, "k2q_resnorm_stream_bwd", lambda: _native.resnorm_stream_bwd(*args),
+                    lambda: _check_resnorm_stream(dr, gate, rows_per_entry, y))
 
 
 MAX_HEAD, MAX_ROTARY = 4096, 1024       # k2q_rotary's largest head and rotated part

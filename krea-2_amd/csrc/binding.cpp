@@ -37,6 +37,7 @@ struct Api {
   decltype(&k2q_resnorm_rotquant) resnorm_rotquant;
   decltype(&k2q_resnorm_bwd) resnorm_bwd;
   decltype(&k2q_resnorm_bwd_ws_bytes) resnorm_bwd_ws_bytes;
+  decltype(&k2q_resnorm_stream_bwd) resnorm_stream_bwd;
   decltype(&k2q_rotary) rotary;
   decltype(&k2q_capture_id) capture_id;
 } api{};
@@ -593,6 +594,42 @@ PyObject* py_resnorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// resnorm_stream_bwd(dr, gate, rows_per_entry, y | None, need_dy) -> (dy | None, dgate | None): dr contiguous (.., K), dy in
+// its shape, dgate in the gate's
+PyObject* py_resnorm_stream_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(5)
+  return guarded([&]() -> PyObject* {
+    const Tensor *dr = tensor_of(a[0], bad), *gate = tensor_of(a[1], bad), *y = tensor_of(a[3], bad);
+    int64_t rows = PyLong_AsLongLong(a[2]);
+    const int need_dy = PyObject_IsTrue(a[4]);
+    if (PyErr_Occurred()) return nullptr;
+    if (bad || !dr || !gate || dr->dim() < 2 || rows < 1 || (!need_dy && !y)) K2Q_REFUSE;
+    const int64_t K = dr->size(dr->dim() - 1);
+    if (!width_ok(K) || dr->numel() == 0) K2Q_REFUSE;
+    const int64_t M = dr->numel() / K;
+    const c10::Device d = dr->device();
+    auto whole = [&](const Tensor& t) {
+      return t.scalar_type() == at::kBFloat16 && t.device() == d && t.is_contiguous() && aligned(t) && t.sizes() == dr->sizes();
+    };
+    int64_t ng, lg;
+    if (!ready(d) || !whole(*dr) || !vectors_ok(gate, K, d, ng, lg) || !entries_fit({ng}, M, 0, rows) ||
+        (y && !(dr->dim() == 2 ? rows_ok(y, M, K, d) : whole(*y))))
+      K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    Tensor dy = need_dy ? alloc(dr->sizes(), at::kBFloat16, d) : Tensor(),
+           dg = y ? alloc(gate->sizes(), at::kBFloat16, d) : Tensor();
+    const int64_t nws = y ? api.resnorm_bwd_ws_bytes(M, K, rows) : 0;
+    Tensor ws = workspace(nws, d);
+    const int rc = foreign(api.resnorm_stream_bwd, as<uint16_t>(ptr(dr)), M, K, as<uint16_t>(ptr(gate)), lg, rows,
+                           as<uint16_t>(ptr(dy)), as<uint16_t>(ptr(y)), y ? dr->dim() == 2 ? y->stride(0) : K : 0,
+                           as<uint16_t>(ptr(dg)), ng == 1 ? K2Q_SHARED_GATE : 0, ptr(ws), nws, st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({dy, dg});
+  });
+}
+
 // rotary(q, k | None, positions, turns, axis | None, axes, half, factor, inverse, heads_first) -> (q', k' | None): q, k (B,
 // L, H, D) or, heads first, (B, H, L, D); positions (L,) or (B, L), with an axis one dimension of `axes` more behind
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -671,6 +708,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !get("k2q_dequant_fp8", api.dequant_fp8) || !get("k2q_gemm_bf16", api.gemm_bf16) ||
       !get("k2q_gemm_plan_ws_bytes", api.gemm_plan_ws_bytes) || !get("k2q_resnorm_rotquant", api.resnorm_rotquant) ||
       !get("k2q_resnorm_bwd", api.resnorm_bwd) || !get("k2q_resnorm_bwd_ws_bytes", api.resnorm_bwd_ws_bytes) ||
+      !get("k2q_resnorm_stream_bwd", api.resnorm_stream_bwd) ||
       !get("k2q_rotary", api.rotary) || !get("k2q_capture_id", api.capture_id))
     return nullptr;
   Py_INCREF(a[1]);
@@ -703,7 +741,7 @@ PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2
                          K2Q_METHOD(dx_weight),   K2Q_METHOD(gemm_dx),        K2Q_METHOD(dequant_fp8),
                          K2Q_METHOD(gemm_bf16),   K2Q_METHOD(pad_factors),    K2Q_METHOD(resnorm),
                          K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         K2Q_METHOD(linear_infer),
-                         K2Q_METHOD(capture_id),  {nullptr, nullptr, 0, nullptr}};
+                         K2Q_METHOD(capture_id),  K2Q_METHOD(resnorm_stream_bwd), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -544,7 +544,7 @@ bool norm_bwd_fits(int64_t M, int64_t K, int mode) {
 // Entries of a few rows (kFew) are a wave's own, several of them one after another: a strip is then the rows of four waves
 // and spans entries, so the partials of the sums over every row stay few (one strip an entry would leave 4 bytes a sum for
 // every 2 of a row), and no wave is without a row.
-// The form without h's gradient (kStream: dR = dr) also makes dy = bf16(gate dr): it reads every row and column once anyway.
+// Where nothing read h (kStream) dR = dr: the same pass makes dy = bf16(gate dr) and the gate's gradient, and is all there is.
 // Bound by reading dh, r, y and dr once more: 1536 x 6144 in 18.2 us (4.5 TB/s), the join 4.0.
 constexpr int CS_COLS = 512;
 
@@ -1269,5 +1269,33 @@ extern "C" int k2q_resnorm_bwd(const uint16_t* dh, const uint16_t* dr, const uin
   c.mscale = mod_scale;
   c.ldm = ld_scale;
   launch_colsum<false>(c, out, colsum_plan(rows_per_batch, K, entries, k2q_cu_count()), entries, st);
+  return k2q_launch_status();
+}
+
+extern "C" int k2q_resnorm_stream_bwd(const uint16_t* dr, int64_t M, int64_t K, const uint16_t* gate, int64_t ld_gate,
+                                      int64_t rows_per_batch, uint16_t* dy, const uint16_t* y, int64_t ldy,
+                                      uint16_t* dgate, int shared, void* ws, int64_t ws_bytes, void* stream) {
+  if (M < 1 || K < 8 || K % 8) return K2Q_EINVAL;
+  if (K > 16384 || M > 0x7fffffff) return K2Q_EUNSUPPORTED;
+  if (!dr || !gate || (!dy && !dgate) || !k2q_aligned(dr, 16) || !k2q_aligned(dy, 16) || !rowvec_ok(gate, ld_gate) ||
+      rows_per_batch < 1 || M % rows_per_batch || !shared_ok(shared))
+    return K2Q_EINVAL;
+  if (dgate && (!y || !k2q_aligned(y, 16) || ldy < K || ldy % 8 || !k2q_aligned(dgate, 16) || !ws || !k2q_aligned(ws, 16) ||
+                ws_bytes < k2q_resnorm_bwd_ws_bytes(M, K, rows_per_batch)))
+    return K2Q_EINVAL;
+  const int64_t entries = M / rows_per_batch;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  ColSumArgs c{};
+  c.dr = dr;
+  c.y = dgate ? y : nullptr;
+  c.M = M;
+  c.ldy = ldy;
+  c.rpb = rows_per_batch;
+  c.K = (int)K;
+  c.gate = gate;
+  c.ldg = ld_gate;
+  c.dy = dy;
+  launch_colsum<true>(c, col_out(nullptr, nullptr, nullptr, dgate, shared, entries, static_cast<float*>(ws)),
+                      colsum_plan(rows_per_batch, K, entries, k2q_cu_count()), entries, st);
   return k2q_launch_status();
 }

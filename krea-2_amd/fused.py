@@ -113,19 +113,13 @@ class _RmsModQuantFn(torch.autograd.Function):
 
 
 def _stream_grads(dr, r, w, gate, y, ctx):
-    nx, ny, ng, nw, ns, nb = ctx.needs_input_grad[:6]
+    """The gradients where nothing read h: r's passes as it is, the gate scales it on the way to y."""
+    nx, ny, _, nw, ns, nb = ctx.needs_input_grad[:6]
     dy, dgate = dr, None
-    if gate is not None:
-        rows = dr.reshape(-1, ctx.rows, r.shape[-1])        # (entries, rows, K)
-        dy = (gate.reshape(-1, 1, r.shape[-1]) * rows).reshape(dr.shape)
-        if ng:
-            shape = ctx.shapes[2]
-            g = (rows.float() * y.reshape(rows.shape)).view(shape.numel() // r.shape[-1], -1, r.shape[-1])
-            while g.shape[1] > 1:   # halves added in f32: a reduction over many blocks clears counters, which no captured
-                n = g.shape[1] // 2         # graph can hold
-                g[:, :n] += g[:, -n:]
-                g = g[:, :g.shape[1] - n]
-            dgate = g.to(gate.dtype).reshape(shape)
+    if gate is not None and (ny or y is not None):
+        rows = _dense_grad(dr, r).view(r.shape)
+        dy, dgate = _lib.resnorm_stream_bwd(rows, gate, ctx.rows, y, ny)
+        dy, dgate = dy if dy is None else dy.view(dr.shape), dgate if dgate is None else dgate.view(ctx.shapes[2])
     dscale, dshift = (torch.zeros(shape, dtype=r.dtype, device=r.device) if need else None
                       for need, shape in zip((ns, nb), ctx.shapes))
     return (dr if nx else None, dy if ny else None, dgate, torch.zeros_like(w) if nw else None, dscale, dshift, None, None,

@@ -126,3 +126,40 @@ def test_sums_past_32_bits(k2, dev, M, K, entries):
         assert ((a[-few:].double() - one[2 + i].double()).abs() <= 2 * 2 ** -8 * ref[i].abs() + 128 * 2 ** -24 * mag[i]).all()
         assert not a[:-few].any()
     assert ((got[5] - one[5]).double().abs() <= 200 * 2 ** -24 * mag[3].sum((0, 1))).all()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("rows,entries,K", [*MANY, (4608, 1, 6144), (300, 2, 2560)])
+def test_stream_alone(k2, dev, rows, entries, K, shared):
+    """Nothing reads h: dx is r's gradient, dy its product with the gate rounded once, the gate's gradient the rows' sum of
+    dr y, exact products added in float32 (16 rows of a strip or 64 of a wave, and the joins: under 200) and rounded once."""
+    norm, x, y, vectors, dr, _ = _inputs(rows * entries, K, entries, dev, seed=5)
+    if shared:
+        vectors[0] = vectors[0][:1].contiguous()
+    leaves = [t.detach().clone().requires_grad_() for t in (x, y, *vectors)]
+    norm.scale.requires_grad_()
+    r, _ = k2.residual_rmsnorm(norm, *leaves)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    gx, gy, gg, gs, gb, gw = torch.autograd.grad(r, [*leaves, norm.scale], dr)
+    used = torch.cuda.max_memory_allocated() - before
+    # dy, the vectors' gradients and the sums' partials, in the allocator's blocks (each up to 2 MB larger): no copy of the
+    # stream in float32
+    ws = k2._lib.load().k2q_resnorm_bwd_ws_bytes(rows * entries, K, rows)
+    assert used <= 2 * x.numel() + 6 * gs.numel() + 4 * K + ws + 6 * (2 << 20)
+    assert torch.equal(gx, dr) and torch.equal(gy, vectors[0] * dr)
+    assert not (gs.any() or gb.any() or gw.any())
+    over = (0, 1) if shared else 1
+    e, m = (f(dr.double() * y.double()).sum(over, keepdim=True) for f in (lambda t: t, torch.abs))
+    assert gg.shape == vectors[0].shape and ((gg.double() - e).abs() <= 2 ** -8 * e.abs() + 200 * 2 ** -24 * m).all()
+    assert torch.equal(torch.autograd.grad(k2.residual_rmsnorm(norm, *leaves)[0], leaves[1], dr)[0], gy)
+    assert torch.equal(torch.autograd.grad(k2.residual_rmsnorm(norm, *leaves)[0], leaves[2], dr)[0], gg)
+
+
+def test_stream_refusals(k2, dev):
+    x, g = torch.zeros(2, 4, 256, device=dev, dtype=torch.bfloat16), torch.zeros(2, 1, 256, device=dev, dtype=torch.bfloat16)
+    f = k2._lib.resnorm_stream_bwd
+    for bad in (lambda: f(x.float(), g, 4), lambda: f(x, g, 3), lambda: f(x, g[..., :128], 4), lambda: f(x, g, 4, x[:1]),
+                lambda: f(x, g, 4, None, False), lambda: f(x, g.float(), 4), lambda: f(x, torch.cat([g, g]), 4)):
+        with pytest.raises(ValueError):
+            bad()

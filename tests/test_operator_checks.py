@@ -71,6 +71,15 @@ def test_entry_points_refuse_bad_arguments(k2):
         assert bwd(**bad) == -1, bad
     assert bwd(M=1 << 31) == -4 and bwd(M=1 << 30, rows=1, nws=1 << 62) == -4
 
+    def stream(dr=p, M=4, K=256, gate=p, ld=0, rows=2, dy=p, y=p, ldy=256, dg=p, shared=0, ws=p, nws=1 << 30):
+        return lib.k2q_resnorm_stream_bwd(dr, M, K, gate, ld, rows, dy, y, ldy, dg, shared, ws, nws, None)
+
+    for bad in ({"dr": None}, {"dr": odd}, {"M": 0}, {"K": 100}, {"gate": None}, {"gate": odd}, {"ld": 4}, {"rows": 3},
+                {"rows": 0}, {"dy": None, "dg": None}, {"dy": odd}, {"y": None}, {"y": odd}, {"ldy": 255}, {"dg": odd},
+                {"ws": None}, {"ws": odd}, {"nws": 16}, {"shared": 8}, {"shared": -1}):
+        assert stream(**bad) == -1, bad
+    assert stream(M=1 << 31) == -4 and stream(K=16512) == -4
+
     heads = k2._lib.RotaryHeads(p, p, 4, 64 * 4 * 6, 256, 64, 64 * 4 * 6, 256, 64)
 
     def rot(t=heads, n=1, dtype=0, B=1, L=6, D=64, dim=64, layout=0, pos=p, pt=0, turns=p):
