@@ -176,11 +176,14 @@ class _ResNormQuantFn(torch.autograd.Function):
 
 def _norm_scale_f32(norm: nn.Module, name: str = "scale") -> torch.Tensor:
     """The norm's (frozen) scale (or ``weight``) as the kernels take it, f32 and contiguous, kept on the module and rebuilt
-    when it changes (in place: version; re-pointed, e.g. paged by block swap: pointer or device)."""
+    when it changes (in place: version; re-pointed, e.g. paged by block swap: pointer or device) or when another stream
+    asks (nothing orders its reads behind the copy).  A graph capture or a trace makes its own: a kept copy can be let go
+    while the graph lives, and what a capture makes holds nothing before a replay."""
     t = getattr(norm, name)
-    if t.is_inference():
-        return t.float().contiguous()
-    key = (t._version, t.data_ptr(), t.device, t.dtype, tuple(t.shape))
+    stream = _lib._stream(t.device) if t.is_cuda else 0
+    if t.is_inference() or _lib.recording(stream):
+        return t.detach().float().contiguous()
+    key = (t._version, t.data_ptr(), t.device, t.dtype, tuple(t.shape), stream)
     kept = norm.__dict__.get("_k2q_scale_f32")
     if kept is None or kept[0] != key:
         with torch.inference_mode(False), torch.no_grad():      # a training pass may save what this call keeps

@@ -77,3 +77,47 @@ def test_siblings_kept_before_a_capture(k2, dev):
         with torch.cuda.graph(graph, stream=side):
             out = group.call(1, static)
         _replays(graph, static, [out], lambda x: [layers[1](x)], values)
+
+
+class Norm(nn.Module):
+    def __init__(self, dev, K=512):
+        super().__init__()
+        self.eps, self.scale = 1e-5, nn.Parameter(torch.randn(K, device=dev).bfloat16(), requires_grad=False)
+
+
+@pytest.mark.parametrize("entry", ["residual", "modulated"])
+def test_a_norm_scale_first_seen_or_changed_around_a_capture(k2, dev, entry):
+    """A bf16 norm scale is held in float32 between calls.  The copy that a capture makes belongs to its graph, and a graph
+    follows the scale as it follows every input, also where a later eager call has replaced the kept copy."""
+    norm, x = Norm(dev), make_x(33, 512, seed=4).to(dev)
+    zero = torch.zeros(1, 512, device=dev, dtype=torch.bfloat16)
+
+    def call(n):
+        with torch.no_grad():
+            return k2.residual_rmsnorm(n, x, x)[1] if entry == "residual" else k2.modulated_rmsnorm(n, x, zero, zero)
+
+    def fresh():                                                # nothing kept
+        n = Norm(dev)
+        n.scale.copy_(norm.scale)
+        return call(n)
+
+    call(Norm(dev))                                             # the device is known to the wrappers
+    torch.cuda.synchronize()
+    first = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        out = call(norm)
+    assert torch.equal(call(norm), fresh())                     # eager, before any replay
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        out2 = call(norm)
+    for i in range(3):
+        norm.scale.normal_()
+        want = fresh()
+        assert torch.equal(call(norm), want)
+        junk = torch.full((1 << 16,), float("nan"), device=dev)     # takes the memory of what was let go
+        for g, o in ((first, out), (second, out2)):
+            o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, want), i
+        del junk

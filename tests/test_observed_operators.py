@@ -53,6 +53,29 @@ def test_codes_kept_before_a_trace_are_no_part_of_it(codes):
             assert torch.equal(a, e)
 
 
+def test_a_norm_scale_kept_in_float32_is_no_part_of_a_recording(k2, monkeypatch):
+    """On the CPU: the copy is a stream's own, and a capture neither keeps one nor takes a kept one."""
+    from krea2_amd.fused import _norm_scale_f32
+    at, now = 0, 0
+
+    class Scale(torch.nn.Parameter):        # a parameter that says it is on the device
+        is_cuda = True
+
+    norm = torch.nn.Module()
+    norm.scale = Scale(torch.ones(8, dtype=torch.bfloat16), requires_grad=False)
+    monkeypatch.setattr(k2._lib, "_stream", lambda dev: at)
+    monkeypatch.setattr(k2._lib, "_native", type("Native", (), {"capture_id": staticmethod(lambda stream: now)}))
+    plain = _norm_scale_f32(norm)
+    assert _norm_scale_f32(norm) is plain
+    at = 16
+    other = _norm_scale_f32(norm)
+    assert other is not plain and _norm_scale_f32(norm) is other
+    now = 5
+    assert _norm_scale_f32(norm) is not other and _norm_scale_f32(norm) is not _norm_scale_f32(norm)
+    now = 0
+    assert _norm_scale_f32(norm) is other
+
+
 def test_codes_of_one_recording_are_no_part_of_another(k2, monkeypatch):
     """On the CPU: a hit needs the stream's capture, or none, that the codes were kept in."""
     cache, now = k2.quantize._SharedInputQuant(), 0
