@@ -528,14 +528,16 @@ class _SiblingGroup:
     def _a_stack(self, As):
         """The members' A factors stacked along the rank.  Kept while every factor is the adapter's own
         parameter (the module holds it, so its object, version and pointer identify its values: an optimizer
-        step or a re-pointed parameter rebuilds the stack); padded or converted factors are new tensors every
-        call, whose object and memory the next call's may take over, and are stacked every call."""
+        step or a re-pointed parameter rebuilds the stack) and the stream is the one that made it; padded or
+        converted factors are new tensors every call, whose object and memory the next call's may take over, and
+        are stacked every call, and so is what a graph capture or a trace records (its replays follow the factors)."""
         if not As:
             return None
-        if not all(isinstance(a, nn.Parameter) for a in As):
+        stream = _lib._stream(As[0].device) if As[0].is_cuda else 0
+        if _lib.recording(stream) or not all(isinstance(a, nn.Parameter) for a in As):
             with torch.no_grad():
                 return torch.cat(As) if len(As) > 1 else As[0].detach()
-        key = tuple((id(a), a._version, a.data_ptr(), a.device) for a in As)
+        key = (stream, *((id(a), a._version, a.data_ptr(), a.device) for a in As))
         if self.stack is None or self.stack[0] != key:
             with torch.no_grad():
                 self.stack = (key, torch.cat(As) if len(As) > 1 else As[0].detach())

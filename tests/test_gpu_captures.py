@@ -121,3 +121,31 @@ def test_a_norm_scale_first_seen_or_changed_around_a_capture(k2, dev, entry):
             torch.cuda.synchronize()
             assert torch.equal(o, want), i
         del junk
+
+
+def test_a_captured_grouped_step_follows_its_factors(k2, dev):
+    """Siblings with adapters: the stacked LoRA factors that eager calls keep are no part of a graph, whose replays follow
+    an update of the factors in place."""
+    from krea2_amd.fused import _SiblingGroup
+
+    def members():
+        return [k2.LoRALinear(_layer(k2, dev, N=256, seed=s), 16, 16.0) for s in range(2)]
+
+    layers = members()
+    group, x = _SiblingGroup(layers), make_x(64, 512, seed=7).to(dev)
+    for m in layers:
+        m.lora_B.data.normal_()
+    with torch.no_grad():
+        group.call(0, x.clone())                                # the stack is kept
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [group.call(0, x), group.call(1, x)]
+        for _ in range(3):
+            for m in layers:
+                m.lora_A.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            fresh = _SiblingGroup(layers)
+            y = x.clone()
+            assert all(torch.equal(a, fresh.call(i, y)) for i, a in enumerate(out))

@@ -76,6 +76,29 @@ def test_a_norm_scale_kept_in_float32_is_no_part_of_a_recording(k2, monkeypatch)
     assert _norm_scale_f32(norm) is other
 
 
+def test_stacked_factors_are_no_part_of_a_recording(k2, monkeypatch):
+    """On the CPU: a captured training step stacks the factors that its optimizer changes, and does not keep what only its
+    replays fill."""
+    from krea2_amd.fused import _SiblingGroup
+    at, now = 0, 0
+
+    class Factor(torch.nn.Parameter):
+        is_cuda = True
+
+    group, pair = _SiblingGroup([]), [Factor(torch.ones(16, 8)), Factor(torch.ones(16, 8))]
+    monkeypatch.setattr(k2._lib, "_stream", lambda dev: at)
+    monkeypatch.setattr(k2._lib, "_native", type("Native", (), {"capture_id": staticmethod(lambda stream: now)}))
+    kept = group._a_stack(pair)
+    assert group._a_stack(pair) is kept
+    at = 16
+    other = group._a_stack(pair)
+    assert other is not kept and group._a_stack(pair) is other
+    now = 5
+    assert group._a_stack(pair) is not other
+    now = 0
+    assert group._a_stack(pair) is other
+
+
 def test_codes_of_one_recording_are_no_part_of_another(k2, monkeypatch):
     """On the CPU: a hit needs the stream's capture, or none, that the codes were kept in."""
     cache, now = k2.quantize._SharedInputQuant(), 0
