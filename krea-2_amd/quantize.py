@@ -225,7 +225,8 @@ class ConvRotLinear(nn.Module):
         were paged out or re-pointed rebuilds it on its next backward, and every build first releases the
         weights kept for layers whose codes have left the device they were built on (a block paged out by
         block swap keeps nothing resident past the next backward of any layer).  An edit through ``.data``
-        that keeps the pointer bumps no version: turn the cache off and on after one."""
+        that keeps the pointer bumps no version: turn the cache off and on after one.  A graph capture takes a
+        kept weight (leave the cache on while the graph lives) and keeps none that it builds."""
         q, s = self.qweight, self.wscale
         if not getattr(self, "keep_dx_weight", False):
             self._dx_kept = None
@@ -234,6 +235,8 @@ class ConvRotLinear(nn.Module):
         kept = self._dx_kept
         if kept is not None and kept[0] == key:
             return kept[1]
+        if _lib.recording(_lib._stream(q.device) if q.is_cuda else 0):      # a capture's holds nothing before a replay
+            return _lib.dx_weight(q, self.weight_scale, w4=self.mode == "w4a8")
         self._dx_kept = None
         _release_stale_dx_weights()
         wt = _lib.dx_weight(q, self.weight_scale, w4=self.mode == "w4a8")

@@ -99,6 +99,21 @@ def test_stacked_factors_are_no_part_of_a_recording(k2, monkeypatch):
     assert group._a_stack(pair) is other
 
 
+def test_an_effective_weight_built_in_a_capture_is_not_kept(k2, monkeypatch):
+    now = 5
+    q = torch.zeros(64, 128, dtype=torch.int8)
+    layer = k2.ConvRotLinear.from_quantized(q, torch.zeros(64, dtype=torch.int32), None)
+    monkeypatch.setattr(k2._lib, "dx_weight", lambda q, s, w4=False: torch.zeros(128, 64))
+    monkeypatch.setattr(k2._lib, "recording", lambda stream: now)
+    k2.set_dx_weight_cache(layer, True)
+    layer.dx_weight()
+    assert layer.dx_weight_kept is None
+    now = 0
+    kept = layer.dx_weight()
+    now = 5
+    assert layer.dx_weight() is kept
+
+
 def test_codes_of_one_recording_are_no_part_of_another(k2, monkeypatch):
     """On the CPU: a hit needs the stream's capture, or none, that the codes were kept in."""
     cache, now = k2.quantize._SharedInputQuant(), 0
