@@ -516,13 +516,13 @@ class _SiblingGroup:
     """Linears that receive the same tensor (``wq / wk / wv / gate`` of ``Attention.forward``, ``mmdit.py:199``).
     The first member called with a tensor computes every member's output in one grouped launch and keeps the
     others; each later member called with that same tensor (same object, version, pointer, shape, strides and
-    stream, in the same graph capture or none) and an unchanged adapter takes its output.  Anything else runs the member's own forward.  Kept
-    outputs a member never asks for stay referenced until the group's next launch replaces them."""
+    stream, in the same graph capture or none) and an unchanged adapter takes its output.  Anything else runs
+    the member's own forward.  Kept outputs a member never asks for stay referenced until the group's next launch
+    replaces them."""
 
     def __init__(self, members):
         self.members = list(members)
-        self.ref = self.key = None
-        self.kept = {}
+        self.last = None    # (weak reference, key, the other members' outputs), replaced as one: threads see a whole one
         self.stack = None   # (key, the adapted members' stacked LoRA A rows)
 
     def _a_stack(self, As):
@@ -552,9 +552,10 @@ class _SiblingGroup:
         if x.is_inference():        # no version counter to know it by
             return None
         key = self._key(x)
-        if self.ref is not None and self.ref() is x and self.key == key and idx in self.kept:
-            out, sk = self.kept.pop(idx)
-            if sk == _state_key(self.members[idx]):
+        last = self.last
+        if last is not None and last[0]() is x and last[1] == key:
+            out, sk = last[2].pop(idx, (None, None))
+            if out is not None and sk == _state_key(self.members[idx]):
                 return out
         K = x.shape[-1]
         if x.dtype != torch.bfloat16 or x.numel() // max(K, 1) <= 8:
@@ -569,8 +570,8 @@ class _SiblingGroup:
                               self._a_stack(ab[0::2]), *ab)
         lead = x.shape[:-1]
         outs = [y.reshape(*lead, b.out_features) for y, b in zip(ys, bases)]
-        self.ref, self.key = weakref.ref(x), key
-        self.kept = {i: (o, _state_key(m)) for i, (o, m) in enumerate(zip(outs, self.members)) if i != idx}
+        kept = {i: (o, _state_key(m)) for i, (o, m) in enumerate(zip(outs, self.members)) if i != idx}
+        self.last = (weakref.ref(x), key, kept)
         return outs[idx]
 
 

@@ -40,10 +40,13 @@ class _SharedInputQuant:
     enabled = True
 
     def __init__(self):
-        self.ref = None
-        self.key = None
-        self.val = None
+        self._kept = None       # (weak reference, key, codes), replaced as one: threads see a whole one or none
         self.misses = 0
+
+    @property
+    def ref(self):
+        kept = self._kept
+        return None if kept is None else kept[0]
 
     @staticmethod
     def _key(x: torch.Tensor):
@@ -53,39 +56,39 @@ class _SharedInputQuant:
         stream = _lib._stream(dev)
         return (x._version, x.data_ptr(), x.shape, x.stride(), dev, stream, _lib.recording(stream))
 
-    def lookup(self, x: torch.Tensor, x2: torch.Tensor):
-        key = self._key(x)
-        if key is not None and self.enabled and self.ref is not None and self.ref() is x and self.key == key:
-            return self.val
+    def _codes(self, x: torch.Tensor, key):
+        kept = self._kept
+        if key is not None and self.enabled and kept is not None and kept[0]() is x and kept[1] == key:
+            return kept[2]
         self.misses += 1
-        qx, sx, _ = _lib.rotquant(x2)
-        if self.enabled and key is not None:
-            self.ref, self.key, self.val = weakref.ref(x), key, (qx, sx)
-        return qx, sx
+        return None
+
+    def lookup(self, x: torch.Tensor, x2: torch.Tensor):
+        key, codes = self.find(x)
+        if codes is None:
+            codes = _lib.rotquant(x2)[:2]
+            self.keep(x, key, *codes)
+        return codes
 
     def find(self, x: torch.Tensor):
         """``(key, codes)``: the codes kept for exactly this tensor, or None; the key goes back to :meth:`keep`."""
         key = self._key(x)
-        if key is not None and self.enabled and self.ref is not None and self.ref() is x and self.key == key:
-            return key, self.val
-        self.misses += 1
-        return key, None
+        return key, self._codes(x, key)
 
     def keep(self, x: torch.Tensor, key, qx: torch.Tensor, sx: torch.Tensor) -> None:
         """Record the codes a fused forward wrote for ``x`` (``key`` from :meth:`find`, taken before that call)."""
         if self.enabled and key is not None:
-            self.ref, self.key, self.val = weakref.ref(x), key, (qx, sx)
+            self._kept = (weakref.ref(x), key, (qx, sx))
 
     def clear(self) -> None:
         """Forget the kept codes (their memory returns to the allocator)."""
-        self.ref = self.key = self.val = None
+        self._kept = None
 
     def seed(self, x: torch.Tensor, qx: torch.Tensor, sx: torch.Tensor) -> None:
         """Record codes a producer-fused kernel computed for ``x`` (exactly those ``rotquant`` gives), so the
         ConvRot layers that receive ``x`` next skip their own rotate/quant."""
-        key = self._key(x) if self.enabled else None
-        if key is not None:
-            self.ref, self.key, self.val = weakref.ref(x), key, (qx, sx)
+        if self.enabled:
+            self.keep(x, self._key(x), qx, sx)
 
 
 shared_input_quant = _SharedInputQuant()

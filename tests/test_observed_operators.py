@@ -114,6 +114,23 @@ def test_an_effective_weight_built_in_a_capture_is_not_kept(k2, monkeypatch):
     assert layer.dx_weight() is kept
 
 
+def test_codes_kept_by_another_thread_in_between(k2, monkeypatch):
+    """Between a call's look at the kept tensor and its taking the codes another thread may keep others: the call takes the
+    codes of its own tensor."""
+    cache, x, y = k2.quantize._SharedInputQuant(), torch.zeros(2, 128), torch.ones(2, 128)
+
+    class Key:
+        def __eq__(self, other):            # what runs between the two
+            cache.keep(y, other, "qy", "sy")
+            return True
+
+    monkeypatch.setattr(cache, "_key", lambda t: Key())
+    cache.seed(x, "qx", "sx")
+    assert cache.find(x)[1] == ("qx", "sx")
+    cache.seed(x, "qx", "sx")
+    assert cache.lookup(x, x) == ("qx", "sx")
+
+
 def test_codes_of_one_recording_are_no_part_of_another(k2, monkeypatch):
     """On the CPU: a hit needs the stream's capture, or none, that the codes were kept in."""
     cache, now = k2.quantize._SharedInputQuant(), 0
