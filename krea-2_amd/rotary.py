@@ -142,6 +142,9 @@ class RotaryEmbedding(nn.Module):
         """``(turns, axis, axes)`` on ``dev``: revolutions per position of every pair, f64, and its axis."""
         t = self._tables.get(dev)
         if t is None:
+            if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the frequencies are not on {dev} yet and a capture cannot copy them there: call the "
+                                   "module once before it, or make it with device=")
             turns = torch.tensor([f / (2 * math.pi) for f in self.frequencies], dtype=torch.float64, device=dev)
             axis = None
             if self.axes is not None:

@@ -79,6 +79,24 @@ def test_siblings_kept_before_a_capture(k2, dev):
         _replays(graph, static, [out], lambda x: [layers[1](x)], values)
 
 
+def test_rotary_first_called_in_a_capture_says_what_it_needs(k2, dev):
+    """A refusal, before anything is launched: the capture goes on, and takes the module once it has its frequencies."""
+    rope, q, pos = k2.RotaryEmbedding(64), torch.randn(1, 5, 2, 64, device=dev), torch.arange(5, device=dev)
+    k2.RotaryEmbedding(64, device=dev)(q, None, pos)
+    ready = k2.RotaryEmbedding(64, device=dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before it"):
+            rope(q, None, pos)
+        out, _ = ready(q, None, pos)
+    for i in range(3):
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, rope(q, None, pos)[0])
+
+
 class Norm(nn.Module):
     def __init__(self, dev, K=512):
         super().__init__()
