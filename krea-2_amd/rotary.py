@@ -145,11 +145,16 @@ class RotaryEmbedding(nn.Module):
             if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"the frequencies are not on {dev} yet and a capture cannot copy them there: call the "
                                    "module once before it, or make it with device=")
-            turns = torch.tensor([f / (2 * math.pi) for f in self.frequencies], dtype=torch.float64, device=dev)
-            axis = None
-            if self.axes is not None:
-                axis = torch.tensor([a for a, d in enumerate(self.axes) for _ in range(d // 2)], dtype=torch.int32,
-                                    device=dev)
+            tracing = torch._C._get_tracing_state()
+            torch._C._set_tracing_state(None)       # the module's own, not values of a trace that ends before it
+            try:
+                turns = torch.tensor([f / (2 * math.pi) for f in self.frequencies], dtype=torch.float64, device=dev)
+                axis = None
+                if self.axes is not None:
+                    axis = torch.tensor([a for a, d in enumerate(self.axes) for _ in range(d // 2)], dtype=torch.int32,
+                                        device=dev)
+            finally:
+                torch._C._set_tracing_state(tracing)
             t = self._tables[dev] = (turns, axis, len(self.axes or ()))
         return t
 

@@ -141,3 +141,59 @@ def test_codes_of_one_recording_are_no_part_of_another(k2, monkeypatch):
         assert cache.find(x)[1] is None
         cache.seed(x, now, now)
         assert cache.find(x)[1] == ((now, now) if now >= 0 else None)       # -3: the stream could not be asked
+
+
+class _Norm(torch.nn.Module):
+    def __init__(self, k):
+        super().__init__()
+        self.eps, self.scale = 1e-5, torch.nn.Parameter(torch.zeros(k), requires_grad=False)
+
+
+@pytest.fixture
+def residual(k2, monkeypatch):
+    def native(x, y, gate, w, add, eps, scale, shift):
+        r = (_unseen(x) + (1 if gate is None else _unseen(gate)) * _unseen(y)).to(torch.bfloat16)
+        h = (r.float() * torch.rsqrt(r.float().square().mean(-1, keepdim=True) + eps) * (_unseen(w) + add)).to(torch.bfloat16)
+        return _unseen(r).to(r.dtype), _unseen(h).to(h.dtype), *_codes(h)
+
+    monkeypatch.setattr(k2._lib, "resnorm_native", native)
+    monkeypatch.setattr(k2._lib, "_stream", lambda dev: 0)
+    norm = _Norm(128)
+    yield lambda x, y: k2.residual_rmsnorm(norm, x, y)
+    k2.quantize.shared_input_quant.clear()
+
+
+@pytest.fixture
+def rotary(k2, monkeypatch):
+    def turned(q, k, positions, turns, axis, axes, half, factor, inverse, heads_first):
+        a = _unseen(positions)[:, None, None] * _unseen(turns) * 6.283185307179586
+        u, v = _unseen(q).chunk(2, -1)
+        return torch.tensor(torch.cat([u * a.cos() - v * a.sin(), u * a.sin() + v * a.cos()], -1).tolist()), None
+
+    monkeypatch.setattr(k2._lib, "rotary", turned)
+    monkeypatch.setattr(k2._lib, "_device_check", lambda dev: None)
+    rope = k2.RotaryEmbedding(16, layout="half")
+    return lambda q, pos: rope(q, None, pos)[0]
+
+
+def test_residual_norm_and_rotary_in_a_trace_follow_their_inputs(residual, rotary):
+    a, b, c, d = torch.randn(4, 2, 3, 128).to(torch.bfloat16)
+    with torch.no_grad():
+        traced = torch.jit.trace(residual, (a, b), check_trace=False)
+        for got, want in zip(traced(c, d), residual(c, d)):
+            assert torch.equal(got, want)
+        q, pos = torch.randn(1, 5, 2, 16), torch.arange(5.0)
+        traced = torch.jit.trace(rotary, (q, pos), check_trace=False)
+        assert torch.equal(traced(2 * q, pos + 3), rotary(2 * q, pos + 3))
+
+
+def test_residual_norm_and_rotary_refuse_a_tangent(residual, rotary):
+    x, q, pos = torch.randn(2, 3, 128).to(torch.bfloat16), torch.randn(1, 5, 2, 16), torch.arange(5.0)
+    with torch.no_grad():
+        want = residual(x, x)[1], rotary(q, pos)
+        with forward_ad.dual_level():
+            for call in (lambda: residual(forward_ad.make_dual(x, torch.ones_like(x)), x),
+                         lambda: rotary(forward_ad.make_dual(q, torch.ones_like(q)), pos)):
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    call()
+            assert torch.equal(residual(x, x)[1], want[0]) and torch.equal(rotary(q, pos), want[1])
