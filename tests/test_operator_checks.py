@@ -167,6 +167,23 @@ def test_rotary_frequencies(k2):
     assert R(64, scaling=S("yarn", 4.0, 4096, attention_factor=1.5)).factor == 1.5
 
 
+def test_scaled_frequencies_of_every_pair(k2):
+    """Each scaling's frequencies from its formula, every pair.  yarn at 128 values, theta 1e4 and 4096 positions: a pair i
+    turns 4096 f_i / 2 pi times, 32 times at i = 64 ln(4096 / 64 pi) / ln 1e4 = 20.94 and once at 64 ln(4096 / 2 pi) / ln 1e4
+    = 45.03, so the ramp runs from pair 20 to pair 46, a 26th a pair; at 8 positions no pair turns 32 times (from pair 0)
+    and one at i = 1.68 once."""
+    R, S = k2.RotaryEmbedding, k2.RotaryScaling
+    p = R(128).frequencies
+    for i, (lin, ntk, yarn, short) in enumerate(zip(*(R(128, scaling=s).frequencies for s in (
+            S("linear", 4.0), S("ntk", 8.0), S("yarn", 4.0, 4096), S("yarn", 16.0, 8))))):
+        base = math.exp(-2 * i / 128 * math.log(10000))
+        assert math.isclose(p[i], base, rel_tol=1e-12) and math.isclose(lin, base / 4, rel_tol=1e-12)
+        assert math.isclose(ntk, (10000 * 8 ** (128 / 126)) ** (-i / 64), rel_tol=1e-12)
+        r = min(max((i - 20) / 26, 0), 1)
+        assert math.isclose(yarn, base * (1 - 0.75 * r), rel_tol=1e-12)
+        assert math.isclose(short, base * (1 - 15 / 16 * min(i / 2, 1)), rel_tol=1e-12)
+
+
 def test_no_codes_kept_in_inference_mode(k2):
     """A tensor without a version counter is never known again, so an in-place write cannot leave stale codes."""
     from krea2_amd.quantize import _SharedInputQuant
