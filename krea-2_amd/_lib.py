@@ -12,6 +12,7 @@ the same arguments, allocates and calls the library; what it refuses comes back 
 from __future__ import annotations
 
 import ctypes
+import functools
 import importlib.util
 import sysconfig
 import threading
@@ -251,6 +252,22 @@ def _device_check(dev: torch.device) -> None:
         raise RuntimeError(f"device cuda:{idx} is not gfx950 (MI355X); the k2q kernels are built for gfx950 only")
 
 
+def _on_its_device(call):
+    """``call`` with the device of its first argument (a tensor, or a list whose first item is or begins with one) as the
+    current one: kernels are launched, and CUs counted, for the current device.  The native wrappers do the same."""
+    @functools.wraps(call)
+    def on(first, *args, **kwargs):
+        t = first
+        while t.__class__ in (list, tuple):
+            t = next((v for v in t if v is not None), None)
+        dev = getattr(t, "device", None)
+        if dev is None or dev.type != "cuda" or dev.index == torch.cuda.current_device():
+            return call(first, *args, **kwargs)
+        with torch.cuda.device(dev):
+            return call(first, *args, **kwargs)
+    return on
+
+
 def _need(t: torch.Tensor, name: str, dtype, ndim: int | None = None, dev: torch.device | None = None):
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
@@ -297,6 +314,7 @@ def _check_rank(r: int) -> None:
 # ----------------------------------------------------------------------------------------------------------
 # (1) rotate + quantize
 # ----------------------------------------------------------------------------------------------------------
+@_on_its_device
 def rotquant(x: torch.Tensor, want_xrot: bool = False):
     """Per-row FWHT-128 rotation + int8 quantization.  ``x`` (M,K) bf16 or f32, contiguous.
     Returns ``(q int8 (M,K), s f32 (M,), xrot bf16 (M,K) | None)``."""
@@ -322,6 +340,7 @@ def rotquant_lora_fits(K: int, r: int) -> bool:
     return 512 <= K <= 3072 and K % 512 == 0 and r in (16, 32, 48, 64) and 16 * (r // 16) * 1024 <= 16 * (K + 8) * 2
 
 
+@_on_its_device
 def rotquant_lora(x: torch.Tensor, A: torch.Tensor):
     """Rotate/quant of ``x`` (M,K) bf16 with the LoRA down-projection ``u = x A^T`` from the same pass
     (``k2q_rotquant_lora``; ``A`` (r,K) f32).  Returns ``(q int8 (M,K), s f32 (M,), u f32 (M,r))``; the codes
@@ -356,6 +375,7 @@ def _need_rows(t: torch.Tensor, name: str, dev: torch.device | None = None) -> N
         raise ValueError(f"{name} is on {t.device}, expected {dev}")
 
 
+@_on_its_device
 def swiglu_rotquant(g: torch.Tensor, u: torch.Tensor):
     """``h = bf16(bf16(silu(g)) * u)`` with the codes of ``rotquant(h)`` from the same pass.
     ``g``, ``u`` (M,K) bf16 with contiguous rows.  Returns ``(h bf16 (M,K), q int8 (M,K), s f32 (M,))``."""
@@ -376,6 +396,7 @@ def swiglu_rotquant(g: torch.Tensor, u: torch.Tensor):
     return h, q, s
 
 
+@_on_its_device
 def rmsmod_rotquant(x: torch.Tensor, norm_scale: torch.Tensor, eps: float, mod_scale: torch.Tensor,
                     mod_shift: torch.Tensor, rows_per_batch: int):
     """Modulated RMSNorm ``h = bf16(bf16(bf16(1 + p) * n) + b)``, ``n = bf16(rms_norm(x) * (norm_scale + 1))``,
@@ -415,6 +436,7 @@ def rmsmod_rotquant(x: torch.Tensor, norm_scale: torch.Tensor, eps: float, mod_s
     return h, q, s
 
 
+@_on_its_device
 def rmsmod_bwd(dh: torch.Tensor, x: torch.Tensor, norm_scale: torch.Tensor, eps: float, mod_scale: torch.Tensor,
                rows_per_batch: int) -> torch.Tensor:
     """Input gradient of :func:`rmsmod_rotquant`'s ``h`` for ``x``: ``dx`` (M,K) bf16.  ``dh``, ``x`` (M,K) bf16
@@ -618,6 +640,7 @@ def rotary(q, k, positions, turns, axis, axes: int, half: bool, factor: float, i
                     lambda: _check_rotary(q, k, positions, turns, axis, axes, heads_first))
 
 
+@_on_its_device
 def swiglu_bwd(dh: torch.Tensor, g: torch.Tensor, u: torch.Tensor):
     """Autograd of ``bf16(bf16(silu(g)) * u)``: ``(dg, du)``, bf16, shapes of ``g``; all contiguous."""
     _need(dh, "dh", torch.bfloat16)
@@ -642,6 +665,7 @@ def quant_weight_i8(w: torch.Tensor):
     return q, s
 
 
+@_on_its_device
 def quant_weight_i4(w: torch.Tensor):
     """int4 group-64 quantization of ``W R``: ``(q4 uint8 (N,K/2) packed, s4 bf16 (K/64,N) group-major)``."""
     if w.dtype not in (torch.bfloat16, torch.float32):
@@ -733,6 +757,7 @@ def _check_lora_grads(dy, x, u, lora_b) -> None:
 LORA_GROUP_MAX = 8     # members per k2q_lora_grads_grouped call
 
 
+@_on_its_device
 def lora_grads_grouped(dys, x, u, lora_bs, scales, want_db=None):
     """LoRA gradients of linears that read one input (``k2q_lora_grads_grouped``; the autograd of ``lora.py:47-48``
     for every member of a grouped node).  Member i: output gradient ``dys[i]`` (M,N_i) bf16, ``lora_bs[i]``
@@ -791,6 +816,7 @@ def lora_grads_grouped(dys, x, u, lora_bs, scales, want_db=None):
 SCRATCH_BYTES = 64 << 20     # K2Q_SCRATCH_BYTES: the library's own device scratch per GPU
 
 
+@_on_its_device
 def lora_grads_noalloc(dy, x, u, lora_b, lora_scale: float, g, dA=None, dB=None) -> None:
     """:func:`lora_grads` into caller-provided outputs with nothing allocated, by the library or here: the
     workspace is the library's device scratch (``SCRATCH_BYTES`` per GPU, shared by every call on that GPU, so
@@ -889,6 +915,7 @@ def gemm_w4a8_plan(M: int, N: int, K: int, cus: int = 256, workspace: bool = Tru
     return rc, pieces.value
 
 
+@_on_its_device
 def gemm_w8a8(qx, sx, qw, sw, bias=None, u=None, lora_b=None, lora_scale: float = 1.0, *,
               split: bool = True, tile: str = "auto") -> torch.Tensor:
     """``y = bf16(2^-7 s_x s_w acc + bias + lora_scale u lora_B^T)`` (M,N).  ``split=False`` runs every tile
@@ -973,6 +1000,7 @@ def alloc_codes(x2):
     return _fast().alloc_codes(x2)
 
 
+@_on_its_device
 def gemm_w8a8_grouped(qx, sx, segments, u=None):
     """Several W8A8 linears that read the same codes in one launch.  ``segments``: sequence of
     ``(q_w, s_w, bias, lora_b, u_col, lora_scale)`` (bias, lora_b nullable; a segment with ``lora_b`` uses
@@ -1031,6 +1059,7 @@ def gemm_w8a8_grouped(qx, sx, segments, u=None):
     return outs
 
 
+@_on_its_device
 def gemm_w4a8(qx, sx, q4, s4, bias=None, u=None, lora_b=None, lora_scale: float = 1.0) -> torch.Tensor:
     """W4A8 variant of :func:`gemm_w8a8` (packed int4 codes, group-major bf16 group scales)."""
     _need(q4, "q_w4", torch.uint8, 2)
@@ -1049,6 +1078,7 @@ def gemm_w4a8(qx, sx, q4, s4, bias=None, u=None, lora_b=None, lora_scale: float 
     return y
 
 
+@_on_its_device
 def gemm_w8a8_acc(qx, qw, *, split: bool = True, tile: str = "auto") -> torch.Tensor:
     """Debug: raw int32 accumulators ``qx @ qw^T`` (M,N), optionally with a forced tile shape (``TILES``)."""
     _need(qx, "q_x", torch.int8, 2)
@@ -1068,6 +1098,7 @@ def gemm_w8a8_acc(qx, qw, *, split: bool = True, tile: str = "auto") -> torch.Te
     return acc
 
 
+@_on_its_device
 def gemm_w4a8_f32(qx, q4, s4) -> torch.Tensor:
     """Debug: ``sum_g s4[g,n] * acc_g[m,n]`` in f32 (M,N), no s_x / 2^-7 / bias / LoRA."""
     _need(qx, "q_x", torch.int8, 2)
@@ -1118,6 +1149,7 @@ def _check_dx_weight(qw, sw, w4: bool) -> None:
     _device_check(dev)
 
 
+@_on_its_device
 def gemm_dx(dy, qw, sw, *, w4: bool = False, g=None, lora_a=None, split: bool = True,
             fold_rotation: bool = True, wt=None) -> torch.Tensor:
     """``dx = bf16(2^-7 (dy W_hat) R + g lora_A)`` (M,K); ``dy`` (M,N) bf16, ``g`` (M,r) f32 already
@@ -1181,6 +1213,7 @@ def gemm_dx(dy, qw, sw, *, w4: bool = False, g=None, lora_a=None, split: bool = 
     return dx
 
 
+@_on_its_device
 def gemm_dx_grouped(segments, g=None, lora_a=None) -> torch.Tensor:
     """Input gradient of linears that share their input, in one GEMM: ``dx = bf16(sum_i dy_i wt_i^T + g A)``.
     ``segments``: ``(dy_i, wt_i)`` with ``dy_i`` (M, N_i) bf16 (row stride a multiple of 8, unit column
@@ -1230,6 +1263,7 @@ def gemm_dx_grouped(segments, g=None, lora_a=None) -> torch.Tensor:
 # ----------------------------------------------------------------------------------------------------------
 # fp8-e4m3 weight-only base (the reference's Fp8Linear, quantize.py:23-51)
 # ----------------------------------------------------------------------------------------------------------
+@_on_its_device
 def quant_weight_fp8(w: torch.Tensor):
     """``Fp8Linear.__init__`` (``quantize.py:34-37``) on the GPU: ``(q float8_e4m3fn (N,K), scale bf16 (N,1))``."""
     if w.dtype not in (torch.bfloat16, torch.float32):
@@ -1272,6 +1306,7 @@ def _check_dequant_fp8(q, s, transpose: bool) -> None:
     _device_check(q.device)
 
 
+@_on_its_device
 def gemm_bf16(x, w, bias=None, u=None, lora_b=None, lora_scale: float = 1.0, *, split: bool = True) -> torch.Tensor:
     """``y = bf16(x w^T + bias) + LoRA`` (``quantize.py:51`` + ``lora.py:47-48``); x (M,K), w (N,K) bf16."""
     if split:
@@ -1308,6 +1343,7 @@ def gemm_bf16(x, w, bias=None, u=None, lora_b=None, lora_scale: float = 1.0, *, 
     return y
 
 
+@_on_its_device
 def gemm_dx_fp8(dy, q, s, *, g=None, lora_a=None, split: bool = True) -> torch.Tensor:
     """``dx = bf16(dy W_deq + g lora_A)`` for the fp8 base (``W_deq = bf16(q s)``)."""
     _need(dy, "dy", torch.bfloat16, 2)

@@ -185,6 +185,7 @@ PyObject* py_linear_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         K2Q_REFUSE;
     }
     if (bias && (bias->dim() != 1 || bias->size(0) != N || bias->scalar_type() != at::kFloat || bias->device() != d)) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     const int wmode = w4 ? K2Q_WMODE_W4 : K2Q_WMODE_W8;
@@ -276,6 +277,7 @@ PyObject* py_lora_grads(PyObject*, PyObject* const* a, Py_ssize_t n) {
       K = x->size(1);
     }
     if (u && (!operand(u, at::kFloat, 2, d) || u->size(0) != M || u->size(1) != r)) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     const int64_t nws = api.lora_grads_ws_bytes(M, N, K, r);
@@ -300,6 +302,7 @@ PyObject* py_lora_down(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!ready(d) || !operand(x, at::kBFloat16, 2, d) || !operand(A, at::kFloat, 2, d)) K2Q_REFUSE;
     const int64_t M = x->size(0), K = x->size(1), r = A->size(0);
     if (A->size(1) != K || !rank_ok(r)) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     const int64_t nws = api.lora_down_ws_bytes(M, K, r);
@@ -322,6 +325,7 @@ PyObject* py_pad_factors(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!ready(d) || !operand(A, at::kFloat, 2, d) || !operand(B, at::kFloat, 2, d)) K2Q_REFUSE;
     const int64_t r = A->size(0), K = A->size(1), N = B->size(0);
     if (B->size(1) != r || r < 1 || rp < r || !rank_ok(rp) || K % 4 || K < 4 || N < 1) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     Tensor ap = alloc({rp, K}, at::kFloat, d), bp = alloc({N, rp}, at::kFloat, d);
@@ -352,6 +356,7 @@ PyObject* py_dx_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::Device d = q->device();
     int64_t N, K;
     if (!ready(d) || !convrot_ok(q, s, w4, d, N, K)) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     Tensor wt = alloc({K, N}, at::kBFloat16, d);
@@ -397,6 +402,7 @@ PyObject* py_gemm_dx(PyObject*, PyObject* const* a, Py_ssize_t n) {
       K2Q_REFUSE;
     int64_t N, K;
     if (q && (!convrot_ok(q, s, w4, d, N, K) || N != dy->size(1) || K != wt->size(0))) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     return dx_lin(*dy, *wt, g, A, st);
@@ -420,6 +426,7 @@ PyObject* py_dequant_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!ready(d) || !fp8_ok(q, s, d)) K2Q_REFUSE;
     const int64_t N = q->size(0), K = q->size(1);
     if (tr && N % 8) K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     Tensor w = tr ? alloc({K, N}, at::kBFloat16, d) : alloc({N, K}, at::kBFloat16, d);
@@ -449,6 +456,7 @@ PyObject* py_gemm_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
       r = u->size(1);
       if (u->size(0) != M || B->size(0) != N || B->size(1) != r || !rank_ok(r)) K2Q_REFUSE;
     }
+    const c10::DeviceGuard guard(d);
     void* st;
     if (!stream_of(d, st)) return nullptr;
     Tensor y = alloc({M, N}, at::kBFloat16, d);

@@ -194,3 +194,32 @@ def test_no_codes_kept_in_inference_mode(k2):
         key, codes = cache.find(h)
         cache.keep(h, key, None, None)
     assert key is None and codes is None and cache.ref is None and cache.misses == 1
+
+
+def test_calls_run_on_their_tensors_device(k2, monkeypatch):
+    """The device of a call's tensors is the current one while it runs, and the caller's again afterwards."""
+    class There:
+        device = torch.device("cuda", 3)
+
+    now = [0]
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            now.append(self.dev.index)
+
+        def __exit__(self, *a):
+            now.pop()
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[-1])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(k2._lib, "load", lambda: 1 / 0)
+    call = k2._lib._on_its_device(lambda first, more=None: (now[-1], more))
+    assert call(There(), more=5) == (3, 5) and call([None, There()]) == (3, None) and call([(There(), 1)]) == (3, None)
+    assert call(torch.zeros(1)) == (0, None) and call(None) == (0, None) and call([]) == (0, None) and now == [0]
+    now[0] = 3
+    assert call(There()) == (3, None)
+    for name in ("rotquant", "rmsmod_rotquant", "swiglu_rotquant", "rmsmod_bwd", "swiglu_bwd", "gemm_w4a8", "gemm_dx_grouped"):
+        assert hasattr(getattr(k2._lib, name), "__wrapped__"), name
