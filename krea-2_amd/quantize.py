@@ -25,6 +25,8 @@ from . import _lib
 
 MODES = ("w8a8", "w4a8")
 
+_is_tracing = torch._C._is_tracing
+
 
 class _SharedInputQuant:
     """The last activation's int8 codes and scales, reused when the next ConvRot layer receives the very same
@@ -54,14 +56,8 @@ class _SharedInputQuant:
             return None
         dev = x.device
         stream = _lib._stream(dev)
-        return (x._version, x.data_ptr(), x.shape, x.stride(), dev, stream, _lib.recording(stream))
-
-    def _codes(self, x: torch.Tensor, key):
-        kept = self._kept
-        if key is not None and self.enabled and kept is not None and kept[0]() is x and kept[1] == key:
-            return kept[2]
-        self.misses += 1
-        return None
+        recorded = _lib.recording(stream) if stream or _is_tracing() else 0
+        return (x._version, x.data_ptr(), x.shape, x.stride(), dev, stream, recorded)
 
     def lookup(self, x: torch.Tensor, x2: torch.Tensor):
         key, codes = self.find(x)
@@ -72,8 +68,11 @@ class _SharedInputQuant:
 
     def find(self, x: torch.Tensor):
         """``(key, codes)``: the codes kept for exactly this tensor, or None; the key goes back to :meth:`keep`."""
-        key = self._key(x)
-        return key, self._codes(x, key)
+        key, kept = self._key(x), self._kept
+        if kept is not None and key is not None and self.enabled and kept[0]() is x and kept[1] == key:
+            return key, kept[2]
+        self.misses += 1
+        return key, None
 
     def keep(self, x: torch.Tensor, key, qx: torch.Tensor, sx: torch.Tensor) -> None:
         """Record the codes a fused forward wrote for ``x`` (``key`` from :meth:`find`, taken before that call)."""
@@ -87,8 +86,9 @@ class _SharedInputQuant:
     def seed(self, x: torch.Tensor, qx: torch.Tensor, sx: torch.Tensor) -> None:
         """Record codes a producer-fused kernel computed for ``x`` (exactly those ``rotquant`` gives), so the
         ConvRot layers that receive ``x`` next skip their own rotate/quant."""
-        if self.enabled:
-            self.keep(x, self._key(x), qx, sx)
+        key = self._key(x) if self.enabled else None
+        if key is not None:
+            self._kept = (weakref.ref(x), key, (qx, sx))
 
 
 shared_input_quant = _SharedInputQuant()
