@@ -375,7 +375,7 @@ struct NormBwdArgs {
 // A team of 64 * WPR lanes owns a row; lane t handles the 8-element chunks at 8 t + 8 T c, c < kNCH, held
 // packed (bf16 pairs) between the two row reductions.  Bound by its reads and writes.  The form that rounds once keeps
 // dr in registers from the start and spreads a row over more lanes (fewer registers each, more rows in flight): 4608 x
-// 6144 with a gate 62.5 -> 54.8 us, 5.2 TB/s; the other two keep the order of the row sums that their results have.
+// 6144 with a gate in 51.8 us alone (5.5 TB/s) and 57 in a training pass (4.9), with the eager roundings 60.4; the other two keep the order of the row sums that their results have.
 enum { BWD_NORM = 0, BWD_EAGER = 1, BWD_ONCE = 2 };    // without a residual; with it, rounded as the eager ops; once
 
 template <int MODE, int WPR, int kNCH>
@@ -545,7 +545,8 @@ bool norm_bwd_fits(int64_t M, int64_t K, int mode) {
 // and spans entries, so the partials of the sums over every row stay few (one strip an entry would leave 4 bytes a sum for
 // every 2 of a row), and no wave is without a row.
 // Where nothing read h (kStream) dR = dr: the same pass makes dy = bf16(gate dr) and the gate's gradient, and is all there is.
-// Bound by reading dh, r, y and dr once more: 1536 x 6144 in 18.2 us (4.5 TB/s), the join 4.0.
+// Bound by reading dh, r, y and dr once more: 2304 x 16384 in 58.5 us (5.2 TB/s), kFew with a gate and a modulation a row
+// 9216 x 6144 in 201 (4.2 TB/s with those and the gradients of them), kStream 9216 x 6144 in 81 (4.2); the join 4 to 5.
 constexpr int CS_COLS = 512;
 
 struct ColSumArgs {
@@ -613,7 +614,7 @@ __global__ __launch_bounds__(256) void resnorm_colsum_kernel(ColSumArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) p1[i] = kStream ? bf16_of(v, i) : vec ? bf16r(1.f + bf16_of(v, i)) : 1.f;
   };
-  // what is absent is read as x (dr): no branch between a row's loads (45.7 -> 43.7 us with both passes, 1536 x 6144)
+  // what is absent is read as x (dr): no branch between a row's loads (with: 5 % of both passes, 1536 x 6144)
   const uint16_t* x = kStream ? a.dr : a.x;
   const uint16_t *yp = a.y ? a.y : x, *rp = !kStream && a.y && a.dr ? a.dr : x;
   const int64_t ly = a.y ? a.ldy : K;
@@ -825,7 +826,7 @@ struct ColOut {
 int64_t fold_groups(int64_t pieces) { return (pieces + CS_FOLD - 1) / CS_FOLD; }
 constexpr int64_t CS_MANY = 1024;    // partials that one join adds
 
-// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 256 strips of 6144 columns 101 / 87),
+// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 9216 x 6144 156 / 150, 4608 x 2048 41.3 / 38.8),
 // or where the strips' entries are written already (`direct`) and only the sums over every entry are left.  Which of the
 // gradients are asked for changes no order.
 void launch_join(const ColOut& c, int parts, bool direct, int64_t K, int64_t entries, int strips, int64_t pieces,
@@ -854,10 +855,11 @@ struct ColPlan {
   int64_t pieces;
 };
 
-// Strips per batch entry: about two workgroups a CU over the column tiles, at least 16 rows each (all three passes, us, at
-// 8 / 16 / 32 rows: 333 x 2560 17.3 / 16.3 / 17.5, 4 x 64 x 1024 11.6 / 11.8 / 13.6, 2 x 1000 x 512 23.3 / 18.9 / 18.5).
-// Entries of fewer rows than that, where every wave of a workgroup has one: as many workgroups, a wave's entries at least
-// four rows.
+// Strips per batch entry: about two workgroups a CU over the column tiles, at least 8 rows each (all three passes, us, at
+// 8 / 16 / 32 rows: 333 x 2560 14.9 / 15.1 / 17.0, 4 x 64 x 1024 10.6 / 12.0 / 14.6, 2 x 1000 x 512 14.5 / 15.3 / 17.5).
+// Entries of fewer than 16 rows, where every wave of a workgroup has one: as many workgroups, a wave's entries at least four
+// rows (one strip an entry / this, all three passes, us: 4099 x 1 x 640 129 / 24, 1000 x 13 x 2048 142 / 96, 9216 x 1 x 6144
+// 1568 / 343).
 ColPlan colsum_plan(int64_t rpb, int64_t K, int64_t entries, int cus) {
   const int64_t tiles = (K + CS_COLS - 1) / CS_COLS;
   if (rpb < 16 && entries >= 4) {
@@ -867,7 +869,7 @@ ColPlan colsum_plan(int64_t rpb, int64_t K, int64_t entries, int cus) {
     return {true, 1, (int)(own * rpb), (entries + 4 * own - 1) / (4 * own)};
   }
   int64_t s = (2 * cus + tiles * entries - 1) / (tiles * entries);
-  const int64_t most = (rpb + 15) / 16;
+  const int64_t most = (rpb + 7) / 8;
   s = s < 1 ? 1 : s > most ? most : s;
   int64_t rows = (rpb + s - 1) / s;
   s = (rpb + rows - 1) / rows;
