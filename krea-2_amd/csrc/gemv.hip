@@ -494,6 +494,8 @@ int launch4_mr(Gemv4Args p, hipStream_t st) {
 //   6144 x 6144    6.2 / 6.2 / 7.5      6.9 / 7.4 / 7.6      7.6 / 7.6 / 7.8      11.2 / 11.1 / 8.7
 //   36864 x 6144   24.3 / 22.4 / 25.6   26.9 / 25.3 / 25.1   29.9 / 25.4 / 25.7   47.5 / 43.4 / 29.7
 //   6144 x 16384   13.6 / 12.3 / 14.0   15.1 / 13.3 / 14.2   16.5 / 14.6 / 13.7   24.8 / 20.8 / 15.0
+// Below 4096 the first row alone is measured on both; just below it a deep K would be faster on the matrix cores too (eight
+// tokens: 4032 x 16384 on teams of four 17.4, 4096 x 16384 on the matrix cores 11.6).
 constexpr int64_t G4_WIDE = 4096;
 
 template <int MT>
