@@ -23,4 +23,5 @@ from .rotary import RotaryEmbedding, RotaryScaling
 __all__ = ["ConvRotLinear", "quantize_dit_convrot", "set_dx_weight_cache", "MODES", "Fp8Linear", "quantize_dit_fp8",
            "save_quantized_base", "load_quantized_base", "fuse_producers", "group_siblings", "modulated_rmsnorm",
            "residual_rmsnorm", "input_codes", "swiglu", "RotaryEmbedding", "RotaryScaling", "LoRALinear", "inject_lora",
-           "inject_lora_te", "QWEN_TE_TARGETS", "lora_scaled", "lora_disabled", "lora_parameters", "save_lora", "load_lora_weights", "load_lora", "DEFAULT_TARGETS", "_lib"]
+           "inject_lora_te", "QWEN_TE_TARGETS", "lora_scaled", "lora_disabled", "lora_parameters", "save_lora",
+           "load_lora_weights", "load_lora", "DEFAULT_TARGETS", "_lib"]

@@ -572,7 +572,8 @@ def _check_resnorm_stream(dr, gate, rows_per_entry, y) -> None:
     _check_k(K)
     if rows_per_entry < 1 or flat.shape[0] % rows_per_entry:
         raise ValueError(f"{flat.shape[0]} rows do not split into entries of {rows_per_entry}")
-    _check_entries(gate.reshape(-1, K) if gate.numel() % K == 0 else gate, "gate", K, flat.shape[0] // rows_per_entry, dr.device)
+    gate = gate.reshape(-1, K) if gate.numel() % K == 0 else gate
+    _check_entries(gate, "gate", K, flat.shape[0] // rows_per_entry, dr.device)
     if y is not None:
         if y.shape != dr.shape:
             raise ValueError("y and dr differ in shape")
@@ -581,8 +582,8 @@ def _check_resnorm_stream(dr, gate, rows_per_entry, y) -> None:
 
 
 def resnorm_stream_bwd(dr, gate, rows_per_entry: int, y=None, need_dy=True):
-    """:func:`resnorm_bwd` where h has no gradient (``k2q_resnorm_stream_bwd``): ``(dy, dgate)`` from the gradient of r, dy (r's
-    shape) where asked for, dgate (the gate's shape) where ``y`` is given.  dx is ``dr``."""
+    """:func:`resnorm_bwd` where h has no gradient (``k2q_resnorm_stream_bwd``): ``(dy, dgate)`` from the gradient of r, dy
+    (r's shape) where asked for, dgate (the gate's shape) where ``y`` is given.  dx is ``dr``."""
     args = (dr, gate, rows_per_entry, y, need_dy)
     out = _fast().resnorm_stream_bwd(*args)
     if out.__class__ is tuple:

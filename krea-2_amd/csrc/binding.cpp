@@ -617,7 +617,8 @@ PyObject* py_resnorm_stream_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t M = dr->numel() / K;
     const c10::Device d = dr->device();
     auto whole = [&](const Tensor& t) {
-      return t.scalar_type() == at::kBFloat16 && t.device() == d && t.is_contiguous() && aligned(t) && t.sizes() == dr->sizes();
+      return t.scalar_type() == at::kBFloat16 && t.device() == d && t.is_contiguous() && aligned(t) &&
+             t.sizes() == dr->sizes();
     };
     int64_t ng, lg;
     if (!ready(d) || !whole(*dr) || !vectors_ok(gate, K, d, ng, lg) || !entries_fit({ng}, M, 0, rows) ||

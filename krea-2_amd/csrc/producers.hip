@@ -375,7 +375,8 @@ struct NormBwdArgs {
 // A team of 64 * WPR lanes owns a row; lane t handles the 8-element chunks at 8 t + 8 T c, c < kNCH, held
 // packed (bf16 pairs) between the two row reductions.  Bound by its reads and writes.  The form that rounds once keeps
 // dr in registers from the start and spreads a row over more lanes (fewer registers each, more rows in flight): 4608 x
-// 6144 with a gate in 51.8 us alone (5.5 TB/s) and 57 in a training pass (4.9), with the eager roundings 60.4; the other two keep the order of the row sums that their results have.
+// 6144 with a gate in 51.8 us alone (5.5 TB/s) and 57 in a training pass (4.9), with the eager roundings 60.4; the other
+// two keep the order of the row sums that their results have.
 enum { BWD_NORM = 0, BWD_EAGER = 1, BWD_ONCE = 2 };    // without a residual; with it, rounded as the eager ops; once
 
 template <int MODE, int WPR, int kNCH>
@@ -544,9 +545,10 @@ bool norm_bwd_fits(int64_t M, int64_t K, int mode) {
 // Entries of a few rows (kFew) are a wave's own, several of them one after another: a strip is then the rows of four waves
 // and spans entries, so the partials of the sums over every row stay few (one strip an entry would leave 4 bytes a sum for
 // every 2 of a row), and no wave is without a row.
-// Where nothing read h (kStream) dR = dr: the same pass makes dy = bf16(gate dr) and the gate's gradient, and is all there is.
+// Where nothing read h (kStream) dR = dr: the same pass makes dy = bf16(gate dr) and the gate's gradient, and is all there
+// is.
 // Bound by reading dh, r, y and dr once more: 2304 x 16384 in 58.5 us (5.2 TB/s), kFew with a gate and a modulation a row
-// 9216 x 6144 in 201 (4.2 TB/s with those and the gradients of them), kStream 9216 x 6144 in 81 (4.2); the join 4 to 5.
+// 9216 x 6144 in 201 (4.5 TB/s with the modulation and the gradients of the vectors), kStream 9216 x 6144 in 81 (4.2); the join 4 to 5.
 constexpr int CS_COLS = 512;
 
 struct ColSumArgs {
@@ -750,8 +752,8 @@ struct JoinArgs {
 };
 
 // NS sums (at `off` of a strip's partials) of the strips from i in steps of NW: the loads of eight strips are issued
-// together (four of several sums by four waves, which have no more of an entry), those past the end repeat the first and add nothing; a last one goes
-// alone (64 x 32 x 6144, a strip a wave: 47.6 us with the repeats).
+// together (four of several sums by four waves, which have no more of an entry), those past the end repeat the first and
+// add nothing; a last one goes alone (64 x 32 x 6144, a strip a wave: 44.6 us, with the repeats 47.6).
 template <int NS, int NW>
 __device__ __forceinline__ void join_strips(const float* p, int64_t i, int64_t end, int64_t stride, const int (&off)[4],
                                             float (&f)[4]) {
@@ -826,9 +828,9 @@ struct ColOut {
 int64_t fold_groups(int64_t pieces) { return (pieces + CS_FOLD - 1) / CS_FOLD; }
 constexpr int64_t CS_MANY = 1024;    // partials that one join adds
 
-// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 9216 x 6144 156 / 150, 4608 x 2048 41.3 / 38.8),
-// or where the strips' entries are written already (`direct`) and only the sums over every entry are left.  Which of the
-// gradients are asked for changes no order.
+// 16 waves where an entry has as many strips (the whole backward, us, four waves / 16: 9216 x 6144 156 / 150, 4608 x 2048
+// 41.3 / 38.8), or where the strips' entries are written already (`direct`) and only the sums over every entry are left.
+// Which of the gradients are asked for changes no order.
 void launch_join(const ColOut& c, int parts, bool direct, int64_t K, int64_t entries, int strips, int64_t pieces,
                  hipStream_t st) {
   const int per_entry = direct ? 0 : c.asked & ~c.whole;

@@ -114,8 +114,10 @@ class RotaryEmbedding(nn.Module):
     Angles are products in float64 and the rotation is float32, rounded once to the tensors' type (bf16, float16 or
     float32).  An angle of ``position * f_i`` radians is off by at most ``3 * 2^-53`` of itself (the rounded revolutions
     per position and one product) and 2^-26 turns (the rest behind the whole turns, in float32): the first is the smaller
-    up to 2^28 radians, 1e-4 turns at 2^41, and a whole turn, so that nothing is left, near 2^54.  It holds no parameters and no state: the frequencies of a device are built at its
-    first call there (before a graph captures one), or for ``device`` at once."""
+    up to 2^28 radians, 1e-4 turns at 2^41, and a whole turn, so that nothing is left, near 2^54.
+
+    It holds no parameters and no state: the frequencies of a device are built at its first call there (before a graph
+    captures one), or for ``device`` at once."""
 
     def __init__(self, dim: int, theta: float = 10000.0, layout: str = "interleaved", axes=None,
                  scaling: RotaryScaling | None = None, device=None):

@@ -51,8 +51,8 @@ def _sums64(norm, x, y, vectors, dr, dh):
             [m.abs().amax(1, keepdim=True) for _, m in terms])
 
 
-# (rows of an entry, entries, K): a wave's own entries (fewer than 16 rows; a last wave and workgroup that are short), one strip
-# an entry (their partials folded above 1024), strips of an entry
+# (rows of an entry, entries, K): a wave's own entries (fewer than 16 rows; a last wave and workgroup that are short), one
+# strip an entry (their partials folded above 1024), strips of an entry
 MANY = [(1, 5, 128), (1, 4099, 640), (3, 1003, 384), (15, 77, 1152), (7, 4, 8320), (1, 66000, 128), (13, 2500, 256),
         (17, 1100, 128), (16, 4200, 256), (33, 129, 2304), (40, 3, 640), (2, 2, 512)]
 

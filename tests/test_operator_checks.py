@@ -221,5 +221,6 @@ def test_calls_run_on_their_tensors_device(k2, monkeypatch):
     assert call(torch.zeros(1)) == (0, None) and call(None) == (0, None) and call([]) == (0, None) and now == [0]
     now[0] = 3
     assert call(There()) == (3, None)
-    for name in ("rotquant", "rmsmod_rotquant", "swiglu_rotquant", "rmsmod_bwd", "swiglu_bwd", "gemm_w4a8", "gemm_dx_grouped"):
+    for name in ("rotquant", "rmsmod_rotquant", "swiglu_rotquant", "rmsmod_bwd", "swiglu_bwd", "gemm_w4a8",
+                 "gemm_dx_grouped"):
         assert hasattr(getattr(k2._lib, name), "__wrapped__"), name
