@@ -433,11 +433,11 @@ def _lora_state(m):
 
 
 def _state_key(m):
-    """Identity of what a member's adapter would add now: its parameters (object and version) and scale."""
+    """Identity of what a member's adapter would add now: its parameters (object, version, whether they train) and scale."""
     if isinstance(m, ConvRotLinear) or m.scale * m.scale_mul == 0.0:
         return None
     A, B = m.lora_A, m.lora_B
-    return (id(A), A._version, id(B), B._version, float(m.scale * m.scale_mul))
+    return (id(A), A._version, A.requires_grad, id(B), B._version, B.requires_grad, float(m.scale * m.scale_mul))
 
 
 class _GroupedFn(torch.autograd.Function):
@@ -516,8 +516,8 @@ class _SiblingGroup:
     """Linears that receive the same tensor (``wq / wk / wv / gate`` of ``Attention.forward``, ``mmdit.py:199``).
     The first member called with a tensor computes every member's output in one grouped launch and keeps the
     others; each later member called with that same tensor (same object, version, pointer, shape, strides and
-    stream, in the same graph capture or none) and an unchanged adapter takes its output.  Anything else runs
-    the member's own forward.  Kept outputs a member never asks for stay referenced until the group's next launch
+    stream, in the same graph capture or none, gradients asked for alike) and an unchanged adapter takes its
+    output.  Anything else runs the member's own forward.  Kept outputs a member never asks for stay referenced until the group's next launch
     replaces them."""
 
     def __init__(self, members):
@@ -546,7 +546,8 @@ class _SiblingGroup:
     @staticmethod
     def _key(x):
         stream = _lib._stream(x.device)
-        return (x._version, x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.device, stream, _lib.recording(stream))
+        return (x._version, x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.device, stream, _lib.recording(stream),
+                torch.is_grad_enabled(), x.requires_grad)
 
     def call(self, idx: int, x: torch.Tensor):
         if x.is_inference():        # no version counter to know it by

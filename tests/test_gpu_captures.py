@@ -167,3 +167,29 @@ def test_a_captured_grouped_step_follows_its_factors(k2, dev):
             fresh = _SiblingGroup(layers)
             y = x.clone()
             assert all(torch.equal(a, fresh.call(i, y)) for i, a in enumerate(out))
+
+
+def test_siblings_kept_without_gradients_are_not_taken_with_them(k2, dev):
+    """An output kept under no_grad, for an input or an adapter that did not ask for a gradient, has none to give: a call
+    that asks runs its own forward."""
+    from krea2_amd.fused import _SiblingGroup
+    layers = [k2.LoRALinear(_layer(k2, dev, N=256, seed=s), 16, 16.0) for s in range(2)]
+    for m in layers:
+        m.lora_B.data.normal_()
+    x = make_x(64, 512, seed=8).to(dev)
+    group = _SiblingGroup(layers)
+    with torch.no_grad():
+        group.call(0, x)
+    y = group.call(1, x)
+    gA, = torch.autograd.grad(y.float().sum(), layers[1].lora_A)
+    assert gA.any()
+    group.call(0, x)
+    x.requires_grad_()
+    gx, = torch.autograd.grad(group.call(1, x).float().sum(), x)
+    assert gx.any()
+    x.requires_grad_(False)
+    layers[1].lora_A.requires_grad_(False)
+    group.call(0, x)
+    layers[1].lora_A.requires_grad_()
+    gA2, = torch.autograd.grad(group.call(1, x).float().sum(), layers[1].lora_A)
+    assert torch.equal(gA2, gA)
