@@ -254,7 +254,8 @@ def _device_check(dev: torch.device) -> None:
 
 def _on_its_device(call):
     """``call`` with the device of its first argument (a tensor, or a list whose first item is or begins with one) as the
-    current one: kernels are launched, and CUs counted, for the current device.  The native wrappers do the same."""
+    current one: kernels are launched, and CUs counted, for the current device.  The native wrappers do the same, and what
+    calls them first asks here behind them (a microsecond on autograd's thread is ten of a host-bound step)."""
     @functools.wraps(call)
     def on(first, *args, **kwargs):
         t = first
@@ -1150,7 +1151,6 @@ def _check_dx_weight(qw, sw, w4: bool) -> None:
     _device_check(dev)
 
 
-@_on_its_device
 def gemm_dx(dy, qw, sw, *, w4: bool = False, g=None, lora_a=None, split: bool = True,
             fold_rotation: bool = True, wt=None) -> torch.Tensor:
     """``dx = bf16(2^-7 (dy W_hat) R + g lora_A)`` (M,K); ``dy`` (M,N) bf16, ``g`` (M,r) f32 already
@@ -1163,6 +1163,11 @@ def gemm_dx(dy, qw, sw, *, w4: bool = False, g=None, lora_a=None, split: bool = 
             return dx
         if dx.__class__ is int:
             _check(dx, "k2q_gemm_dx")
+    return _gemm_dx_checked(dy, qw, sw, w4, g, lora_a, split, fold_rotation, wt)
+
+
+@_on_its_device
+def _gemm_dx_checked(dy, qw, sw, w4, g, lora_a, split, fold_rotation, wt):
     _need(dy, "dy", torch.bfloat16, 2)
     dev = dy.device
     M, N = dy.shape
@@ -1307,7 +1312,6 @@ def _check_dequant_fp8(q, s, transpose: bool) -> None:
     _device_check(q.device)
 
 
-@_on_its_device
 def gemm_bf16(x, w, bias=None, u=None, lora_b=None, lora_scale: float = 1.0, *, split: bool = True) -> torch.Tensor:
     """``y = bf16(x w^T + bias) + LoRA`` (``quantize.py:51`` + ``lora.py:47-48``); x (M,K), w (N,K) bf16."""
     if split:
@@ -1316,6 +1320,11 @@ def gemm_bf16(x, w, bias=None, u=None, lora_b=None, lora_scale: float = 1.0, *, 
             return y
         if y.__class__ is int:
             _check(y, "k2q_gemm_bf16")
+    return _gemm_bf16_checked(x, w, bias, u, lora_b, lora_scale, split)
+
+
+@_on_its_device
+def _gemm_bf16_checked(x, w, bias, u, lora_b, lora_scale, split):
     _need(x, "x", torch.bfloat16, 2)
     dev = x.device
     _need(w, "w", torch.bfloat16, 2, dev)
@@ -1344,7 +1353,6 @@ def gemm_bf16(x, w, bias=None, u=None, lora_b=None, lora_scale: float = 1.0, *, 
     return y
 
 
-@_on_its_device
 def gemm_dx_fp8(dy, q, s, *, g=None, lora_a=None, split: bool = True) -> torch.Tensor:
     """``dx = bf16(dy W_deq + g lora_A)`` for the fp8 base (``W_deq = bf16(q s)``)."""
     _need(dy, "dy", torch.bfloat16, 2)
@@ -1362,8 +1370,6 @@ def gemm_dx_fp8(dy, q, s, *, g=None, lora_a=None, split: bool = True) -> torch.T
             raise ValueError("LoRA gradient shapes mismatch")
         _check_rank(r)
     _device_check(dev)
-    lib = load()
-    st = _stream(dev)
     wt = dequant_fp8(q, s, transpose=True)
     if split:
         dx = _native.gemm_dx(dy, wt, g, lora_a, None, None, False)
@@ -1371,8 +1377,14 @@ def gemm_dx_fp8(dy, q, s, *, g=None, lora_a=None, split: bool = True) -> torch.T
             return dx
         if dx.__class__ is int:
             _check(dx, "k2q_gemm_dx_lin")
+    return _gemm_dx_lin(dy, wt, g, lora_a if r else None, r, split)
+
+
+@_on_its_device
+def _gemm_dx_lin(dy, wt, g, lora_a, r, split):
+    (M, N), K, dev = dy.shape, wt.shape[0], dy.device
     dx = torch.empty((M, K), dtype=torch.bfloat16, device=dev)
     ws, nws = _workspace(gemm_plan_ws_bytes(GEMM_DX_LIN, M, N, K) if split else 0, dev)
-    _check(lib.k2q_gemm_dx_lin(_ptr(dy), _ptr(wt), M, N, K, _ptr(g), _ptr(lora_a) if r else None, r, _ptr(dx),
-                               _ptr(ws), nws, st), "k2q_gemm_dx_lin")
+    _check(load().k2q_gemm_dx_lin(_ptr(dy), _ptr(wt), M, N, K, _ptr(g), _ptr(lora_a), r, _ptr(dx), _ptr(ws), nws,
+                                  _stream(dev)), "k2q_gemm_dx_lin")
     return dx
