@@ -42,7 +42,7 @@ extern "C" {
 
 #define K2Q_DTYPE_BF16 0
 #define K2Q_DTYPE_F32 1
-#define K2Q_DTYPE_F16 2      /* k2q_rotary alone */
+#define K2Q_DTYPE_F16 2      /* k2q_rotary and the optimizer step alone */
 
 /* Library version string and device check (K2Q_OK when the current device is gfx950). */
 const char* k2q_version(void);
@@ -394,6 +394,46 @@ int k2q_gemm_dx_grouped(const k2q_dx_segment* seg, int64_t nseg, int64_t M, int6
  * k2q_gemm_plan_ws_bytes(K2Q_GEMM_DX_GROUPED, M, sum_i N_i, K) bytes.  ws NULL or too small: full-reduction tiles only, what k2q_gemm_dx_grouped runs. */
 int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, int64_t M, int64_t K, const float* g, int64_t ldg,
                            const float* lora_a, int64_t r, uint16_t* dx, void* ws, int64_t ws_bytes, void* stream);
+
+
+/* The step behind a backward pass, over a list of tensors (no counterpart in the reference's kernels; its trainer calls
+ * torch's clip_grad_norm_ and AdamW, train_t2i_lora_cached.py:329-332).  t: host array, count tensors of n contiguous elements
+ * of type dtype (bf16, f32, f16), g their gradients in the same type; read before the call returns.
+ * k2q_grad_norm: out[0] = the 2-norm over all gradients (sums in f64, in a fixed order), out[1] = min(1, max_norm /
+ * (norm + 1e-6)).  k2q_scale_grads: every gradient times by[0], rounded once.
+ * k2q_adamw: steps[index] += 1 (= T), and with g the gradient times norm[1] where norm is given,
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^T) m / (sqrt(v) / sqrt(1 - beta2^T) + eps)
+ * in f32.  lr_of (nullable): the learning rate in device memory, in place of lr.  A norm[0] that is not finite: nothing
+ * changes.  p is rounded to its type to nearest; stochastic != 0 rounds bf16 (not f16) at random: 16 random bits are added
+ * below the kept ones and the rest is cut off.
+ * m and v of a tensor begin at element `at` (a multiple of K2Q_MOMENT_BLOCK) of exp_avg and exp_avg_sq and reach to the end
+ * of its last block.  state_bits 32: f32.  8: one byte each and an f32 scale for every block in avg_scale / sq_scale.  m =
+ * e4m3(code) scale; v = (u(code) scale)^2 with u(c) = c / 16 below 16 and (16 + c % 16) 2^(c / 16 - 5) from there on; a scale is
+ * the block's largest |m| / 448 or sqrt(v) / 31744, a block whose largest is under 2^-100 holds zeros, and a code is rounded at
+ * random between its neighbours, roots above zero to 1 at least.  Random bits are a function of seed, T and the element's
+ * place at + i.  Values of m that are not finite stay so (code 0x7F); a root that is not finite has code 255.
+ * t[i].index strictly increasing; ws of k2q_adamw_ws_bytes(count) bytes, 16-byte aligned.
+ * k2q_moments: m and v (f32 or bf16) of n codes, n a multiple of K2Q_MOMENT_BLOCK. */
+#define K2Q_MOMENT_BLOCK 256
+typedef struct {
+  void* p;              /* the tensor (k2q_adamw alone) */
+  void* g;              /* its gradient */
+  int64_t n;
+  int64_t at;           /* k2q_adamw: place of its first element in the moments' buffers */
+  int32_t index;        /* k2q_adamw: its count in steps */
+  int32_t dtype;
+} k2q_step_tensor;
+int64_t k2q_grad_norm_ws_bytes(const k2q_step_tensor* t, int64_t count);
+int k2q_grad_norm(const k2q_step_tensor* t, int64_t count, double max_norm, void* ws, int64_t ws_bytes, float* out,
+                  void* stream);
+int k2q_scale_grads(const k2q_step_tensor* t, int64_t count, const float* by, void* stream);
+int64_t k2q_adamw_ws_bytes(int64_t count);
+int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits, void* exp_avg, void* exp_avg_sq, float* avg_scale,
+              float* sq_scale, float* steps, double lr, const float* lr_of, double beta1, double beta2, double eps,
+              double weight_decay, const float* norm, int stochastic, uint32_t seed, void* ws, int64_t ws_bytes, void* stream);
+int k2q_moments(const uint8_t* avg, const float* avg_scale, const uint8_t* sq, const float* sq_scale, int64_t n, int dtype,
+                void* m, void* v, void* stream);
 
 
 #ifdef __cplusplus

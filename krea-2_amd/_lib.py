@@ -38,6 +38,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 
 class DxSegment(ctypes.Structure):
@@ -49,6 +50,12 @@ class RotaryHeads(ctypes.Structure):
     """``k2q_rotary_heads`` of ``include/k2q.h``: one tensor of heads, its result, and their strides in elements."""
     _fields_ = [("x", ctypes.c_void_p), ("o", ctypes.c_void_p), ("heads", ctypes.c_int64)] + [
         (name, ctypes.c_int64) for name in ("x_b", "x_l", "x_h", "o_b", "o_l", "o_h")]
+
+
+class StepTensor(ctypes.Structure):
+    """``k2q_step_tensor`` of ``include/k2q.h``: one tensor of an optimizer's step."""
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("n", ctypes.c_int64), ("at", ctypes.c_int64),
+                ("index", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
 class LoraMember(ctypes.Structure):
@@ -118,6 +125,13 @@ _SIGNATURES = {
     "k2q_gemm_dx_ws_bytes": ([_i64, _i64, _i64], _i64),
     "k2q_gemm_dx": ([_p, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _p], _int),
     "k2q_gemm_dx_grouped": ([_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p], _int),
+    "k2q_grad_norm_ws_bytes": ([_p, _i64], _i64),
+    "k2q_grad_norm": ([_p, _i64, _f64, _p, _i64, _p, _p], _int),
+    "k2q_scale_grads": ([_p, _i64, _p, _p], _int),
+    "k2q_adamw_ws_bytes": ([_i64], _i64),
+    "k2q_adamw": ([_p, _i64, _int, _p, _p, _p, _p, _p, _f64, _p, _f64, _f64, _f64, _f64, _p, _int, ctypes.c_uint32, _p, _i64,
+                   _p], _int),
+    "k2q_moments": ([_p, _p, _p, _p, _i64, _int, _p, _p, _p], _int),
     "k2q_gemm_dx_grouped_ws": ([_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p], _int),
 }
 EXPORTS = tuple(_SIGNATURES)
@@ -1388,3 +1402,86 @@ def _gemm_dx_lin(dy, wt, g, lora_a, r, split):
     _check(load().k2q_gemm_dx_lin(_ptr(dy), _ptr(wt), M, N, K, _ptr(g), _ptr(lora_a), r, _ptr(dx), _ptr(ws), nws,
                                   _stream(dev)), "k2q_gemm_dx_lin")
     return dx
+
+
+# ----------------------------------------------------------------------------------------------------------
+# The optimizer's step over many tensors
+# ----------------------------------------------------------------------------------------------------------
+STEP_DTYPES = (torch.bfloat16, torch.float32, torch.float16)
+MOMENT_BLOCK = 256      # K2Q_MOMENT_BLOCK: elements of a moment in 8 bits that share a scale
+
+
+def _check_gradients(params, in_place: bool) -> None:
+    dev, seen = None, set()
+    for i, p in enumerate(params):
+        if not isinstance(p, torch.Tensor):
+            raise ValueError(f"parameter {i} must be a tensor, got {type(p).__name__}")
+        g = p.grad
+        if g is None or g.numel() == 0:
+            continue
+        if g.layout != torch.strided:
+            raise ValueError(f"parameter {i} has a sparse gradient")
+        if g.dtype not in STEP_DTYPES:
+            raise ValueError(f"parameter {i}'s gradient is {g.dtype}, not one of {STEP_DTYPES}")
+        dev = g.device if dev is None else dev
+        if g.device != dev or p.device != dev:
+            raise ValueError(f"parameter {i} or its gradient is on {g.device}, others are on {dev}")
+        if p.is_inference() or g.is_inference():
+            raise ValueError(f"parameter {i} or its gradient was made under torch.inference_mode")
+        if in_place and not torch.ops.aten.is_non_overlapping_and_dense.default(g):
+            raise ValueError(f"parameter {i}'s gradient has gaps or elements twice: it cannot be scaled in place")
+        if in_place and g.data_ptr() in seen:
+            raise ValueError(f"parameter {i}'s gradient is in the list twice")
+        seen.add(g.data_ptr())
+    if dev is not None:
+        _device_check(dev)
+
+
+def grad_norm(params: list, max_norm: float, scale: bool):
+    """``{norm, factor}`` of the parameters' gradients (``k2q_grad_norm``), which ``scale`` multiplies by the factor in
+    place; None where none has a gradient."""
+    call = lambda: _native.grad_norm(params, max_norm, scale)   # noqa: E731
+    r = _fast().grad_norm(params, max_norm, scale)
+    if r.__class__ is not tuple:
+        r = _refused(r, "k2q_grad_norm", call, lambda: _check_gradients(params, scale))
+    return r[0] if r else None
+
+
+def _check_adamw(params, starts, exp_avg, steps, stochastic) -> None:
+    if len(params) != len(starts) or steps.numel() != len(starts):
+        raise ValueError(f"the group has {len(params)} parameters now, and had {len(starts)} when its moments were laid out")
+    for i, p in enumerate(params):
+        if p.grad is None:
+            continue
+        if p.device != exp_avg.device:
+            raise ValueError(f"parameter {i} is on {p.device}, its moments are on {exp_avg.device}")
+        if not p.is_contiguous():
+            raise ValueError(f"parameter {i} must be contiguous")
+        if p.grad.dtype != p.dtype or p.grad.shape != p.shape:
+            raise ValueError(f"parameter {i} is {p.dtype} {tuple(p.shape)}, its gradient {p.grad.dtype} "
+                             f"{tuple(p.grad.shape)}")
+        if starts[i] + p.numel() > (starts[i + 1] if i + 1 < len(starts) else exp_avg.numel()):
+            raise ValueError(f"parameter {i} has grown to {p.numel()} elements")
+        if stochastic and p.dtype == torch.float16:
+            raise ValueError(f"parameter {i} is float16: only bfloat16 is rounded at random")
+    _check_gradients(params, False)
+
+
+def adamw(params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale, sq_scale, steps, lr, lr_of, beta1, beta2, eps,
+          weight_decay, norm, stochastic, seed) -> None:
+    """A step (``k2q_adamw``) of the parameters that have a gradient; ``starts`` are the places of all of them in the
+    moments' flat buffers."""
+    args = (params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale, sq_scale, steps, lr, lr_of, beta1, beta2, eps,
+            weight_decay, norm, stochastic, seed)
+    r = _fast().adamw(*args)
+    if r.__class__ is not tuple:
+        _refused(r, "k2q_adamw", lambda: _native.adamw(*args),
+                 lambda: _check_adamw(params, starts, exp_avg, steps, stochastic))
+
+
+def moments(exp_avg, avg_scale, exp_avg_sq, sq_scale, dtype):
+    """What the moments' codes stand for (``k2q_moments``), flat, in float32 or bfloat16."""
+    args = (exp_avg, avg_scale, exp_avg_sq, sq_scale, dtype == torch.bfloat16)
+    r = _fast().moments(*args)
+    return r if r.__class__ is tuple else _refused(r, "k2q_moments", lambda: _native.moments(*args),
+                                                   lambda: _device_check(exp_avg.device))

@@ -15,6 +15,9 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <unordered_set>
+#include <vector>
+
 #include "../../include/k2q.h"
 
 namespace {
@@ -40,6 +43,12 @@ struct Api {
   decltype(&k2q_resnorm_stream_bwd) resnorm_stream_bwd;
   decltype(&k2q_rotary) rotary;
   decltype(&k2q_capture_id) capture_id;
+  decltype(&k2q_grad_norm) grad_norm;
+  decltype(&k2q_grad_norm_ws_bytes) grad_norm_ws_bytes;
+  decltype(&k2q_scale_grads) scale_grads;
+  decltype(&k2q_adamw) adamw;
+  decltype(&k2q_adamw_ws_bytes) adamw_ws_bytes;
+  decltype(&k2q_moments) moments;
 } api{};
 
 PyObject* raw_stream_of = nullptr;   // torch._C._cuda_getCurrentRawStream
@@ -696,6 +705,158 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The tensors of an optimizer's step that have a gradient: what the library takes of them, and the gradients (copies of
+// those that do not lie one element behind another, which hold the memory until the call returns).
+struct Stepped {
+  std::vector<k2q_step_tensor> t;
+  std::vector<Tensor> grads, params;
+  std::unordered_set<void*> written;
+  c10::Device device = c10::Device(at::kCPU);
+
+  // False where an argument is not what the kernels take.  in_place: the gradients are written, so a copy will not do.
+  bool add(const Tensor& p, bool in_place) {
+    const Tensor& g = p.grad();
+    if (!g.defined() || g.numel() == 0) return true;
+    const auto ty = g.scalar_type();
+    const int dt = ty == at::kBFloat16 ? K2Q_DTYPE_BF16 : ty == at::kHalf ? K2Q_DTYPE_F16 : K2Q_DTYPE_F32;
+    if (g.layout() != at::kStrided || (dt == K2Q_DTYPE_F32 && ty != at::kFloat) || g.device() != p.device()) return false;
+    if (t.empty()) device = g.device();
+    if (!ready(g.device()) || g.device() != device || p.is_inference() || g.is_inference()) return false;
+    Tensor flat = g;
+    if (in_place ? !g.is_non_overlapping_and_dense() : !g.is_contiguous()) {
+      if (in_place) return false;
+      flat = g.detach().contiguous();
+    }
+    if (in_place && !written.insert(flat.data_ptr()).second) return false;     // scaled twice, in no order
+    t.push_back({p.data_ptr(), flat.data_ptr(), flat.numel(), 0, 0, dt});
+    grads.push_back(flat);
+    params.push_back(p);
+    return true;
+  }
+};
+
+// Runs f(tensor, its place in the list) over a list of tensors; false where it is none or f says so.
+template <class F>
+bool each_of(PyObject* list, F&& f) {
+  if (!PyList_Check(list)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    if (!THPVariable_Check(o) || !f(THPVariable_Unpack(o), (int64_t)i)) return false;
+  }
+  return true;
+}
+
+void changed(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
+// grad_norm(params, max_norm, scale) -> (out,): {norm, factor} of the parameters' gradients, which `scale` multiplies by the
+// factor; () where none has a gradient
+PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(3)
+  return guarded([&]() -> PyObject* {
+    const double most = PyFloat_AsDouble(a[1]);
+    const int scale = PyObject_IsTrue(a[2]);
+    if (PyErr_Occurred()) return nullptr;
+    Stepped s;
+    if (bad || !each_of(a[0], [&](const Tensor& p, int64_t) { return s.add(p, scale); })) K2Q_REFUSE;
+    if (s.t.empty()) return PyTuple_New(0);
+    const c10::DeviceGuard guard(s.device);
+    void* st;
+    if (!stream_of(s.device, st)) return nullptr;
+    const int64_t count = (int64_t)s.t.size(), nws = api.grad_norm_ws_bytes(s.t.data(), count);
+    Tensor out = alloc({2}, at::kFloat, s.device), ws = workspace(nws, s.device);
+    int rc = foreign(api.grad_norm, s.t.data(), count, most, ptr(ws), nws, as<float>(ptr(out)), st);
+    if (!rc && scale) {
+      rc = foreign(api.scale_grads, s.t.data(), count, as<float>(ptr(out)) + 1, st);
+      for (const Tensor& g : s.grads) changed(g);
+    }
+    if (rc) return PyLong_FromLong(rc);
+    return pack({out});
+  });
+}
+
+// adamw(params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale | None, sq_scale | None, steps, lr, lr_of | None, beta1,
+// beta2, eps, weight_decay, norm | None, stochastic, seed) -> (): a step of the parameters that have a gradient; starts: their
+// places in the moments' buffers
+PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(17)
+  return guarded([&]() -> PyObject* {
+    const Tensor *m = tensor_of(a[3], bad), *v = tensor_of(a[4], bad), *ms = tensor_of(a[5], bad), *vs = tensor_of(a[6], bad),
+                 *steps = tensor_of(a[7], bad), *lr_of = tensor_of(a[9], bad), *norm = tensor_of(a[14], bad);
+    const long bits = PyLong_AsLong(a[2]);
+    const double lr = PyFloat_AsDouble(a[8]), beta1 = PyFloat_AsDouble(a[10]), beta2 = PyFloat_AsDouble(a[11]),
+                 eps = PyFloat_AsDouble(a[12]), decay = PyFloat_AsDouble(a[13]);
+    const int stochastic = PyObject_IsTrue(a[15]);
+    const unsigned long seed = PyLong_AsUnsignedLong(a[16]);
+    if (PyErr_Occurred()) return nullptr;
+    if (bad || !m || !v || !steps || !PyList_Check(a[1]) || (bits == 8) != (ms && vs)) K2Q_REFUSE;
+    const c10::Device d = m->device();
+    auto held = [&](const Tensor* t, at::ScalarType ty, int64_t size) {
+      return operand(t, ty, 1, d) && t->numel() == size;
+    };
+    const int64_t size = m->numel(), places = PyList_GET_SIZE(a[1]);
+    if (!ready(d) || size % K2Q_MOMENT_BLOCK || !operand(steps, at::kFloat, 1, d) || steps->numel() != places ||
+        !held(m, bits == 8 ? at::kFloat8_e4m3fn : at::kFloat, size) || !held(v, bits == 8 ? at::kByte : at::kFloat, size) ||
+        (bits == 8 && (!held(ms, at::kFloat, size / K2Q_MOMENT_BLOCK) || !held(vs, at::kFloat, size / K2Q_MOMENT_BLOCK))) ||
+        (lr_of && (lr_of->scalar_type() != at::kFloat || lr_of->numel() != 1 || lr_of->device() != d)) ||
+        (norm && !(norm->scalar_type() == at::kFloat && norm->numel() == 2 && norm->device() == d)))
+      K2Q_REFUSE;
+    Stepped s;
+    const bool fits = each_of(a[0], [&](const Tensor& p, int64_t i) {
+      const size_t before = s.t.size();
+      if (i >= places || !s.add(p, false)) return false;
+      if (s.t.size() == before) return true;
+      const int64_t at = PyLong_AsLongLong(PyList_GET_ITEM(a[1], i));
+      s.t.back().at = at;
+      s.t.back().index = (int32_t)i;
+      return !(at == -1 && PyErr_Occurred()) && p.is_contiguous() && p.scalar_type() == s.grads.back().scalar_type() &&
+             p.sizes() == p.grad().sizes() && p.device() == d && at >= 0 && at % K2Q_MOMENT_BLOCK == 0 &&
+             at + p.numel() <= size && !(stochastic && p.scalar_type() == at::kHalf);
+    });
+    if (PyErr_Occurred()) return nullptr;
+    if (!fits) K2Q_REFUSE;
+    if (s.t.empty()) return PyTuple_New(0);
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    const int64_t count = (int64_t)s.t.size(), nws = api.adamw_ws_bytes(count);
+    Tensor ws = workspace(nws, d);
+    const int rc = foreign(api.adamw, s.t.data(), count, (int)bits, m->data_ptr(), v->data_ptr(), as<float>(ptr(ms)),
+                           as<float>(ptr(vs)), as<float>(ptr(steps)), lr, as<float>(ptr(lr_of)), beta1, beta2, eps, decay,
+                           as<float>(ptr(norm)), stochastic, (uint32_t)seed, ptr(ws), nws, st);
+    if (rc) return PyLong_FromLong(rc);
+    for (const Tensor& p : s.params) changed(p);
+    for (const Tensor* t : {m, v, ms, vs, steps})
+      if (t) changed(*t);
+    return PyTuple_New(0);
+  });
+}
+
+// moments(exp_avg, avg_scale, exp_avg_sq, sq_scale, bf16) -> (m, v): what codes stand for
+PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(5)
+  return guarded([&]() -> PyObject* {
+    const Tensor *m = tensor_of(a[0], bad), *ms = tensor_of(a[1], bad), *v = tensor_of(a[2], bad), *vs = tensor_of(a[3], bad);
+    const int bf16 = PyObject_IsTrue(a[4]);
+    if (bad || !m || !ms || !v || !vs) K2Q_REFUSE;
+    const c10::Device d = m->device();
+    const int64_t size = m->numel();
+    if (!ready(d) || size < K2Q_MOMENT_BLOCK || size % K2Q_MOMENT_BLOCK || !operand(m, at::kFloat8_e4m3fn, 1, d) ||
+        !operand(v, at::kByte, 1, d) || v->numel() != size || !operand(ms, at::kFloat, 1, d) ||
+        !operand(vs, at::kFloat, 1, d) || ms->numel() * K2Q_MOMENT_BLOCK != size || vs->numel() * K2Q_MOMENT_BLOCK != size)
+      K2Q_REFUSE;
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    const auto ty = bf16 ? at::kBFloat16 : at::kFloat;
+    Tensor om = alloc({size}, ty, d), ov = alloc({size}, ty, d);
+    const int rc = foreign(api.moments, as<uint8_t>(ptr(m)), as<float>(ptr(ms)), as<uint8_t>(ptr(v)), as<float>(ptr(vs)), size,
+                           bf16 ? K2Q_DTYPE_BF16 : K2Q_DTYPE_F32, ptr(om), ptr(ov), st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({om, ov});
+  });
+}
+
 // bind(dict of entry point addresses, raw stream getter)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(2)
@@ -718,7 +879,10 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !get("k2q_gemm_plan_ws_bytes", api.gemm_plan_ws_bytes) || !get("k2q_resnorm_rotquant", api.resnorm_rotquant) ||
       !get("k2q_resnorm_bwd", api.resnorm_bwd) || !get("k2q_resnorm_bwd_ws_bytes", api.resnorm_bwd_ws_bytes) ||
       !get("k2q_resnorm_stream_bwd", api.resnorm_stream_bwd) ||
-      !get("k2q_rotary", api.rotary) || !get("k2q_capture_id", api.capture_id))
+      !get("k2q_rotary", api.rotary) || !get("k2q_capture_id", api.capture_id) ||
+      !get("k2q_grad_norm", api.grad_norm) || !get("k2q_grad_norm_ws_bytes", api.grad_norm_ws_bytes) ||
+      !get("k2q_scale_grads", api.scale_grads) || !get("k2q_adamw", api.adamw) ||
+      !get("k2q_adamw_ws_bytes", api.adamw_ws_bytes) || !get("k2q_moments", api.moments))
     return nullptr;
   Py_INCREF(a[1]);
   Py_XSETREF(raw_stream_of, a[1]);
@@ -750,7 +914,9 @@ PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2
                          K2Q_METHOD(dx_weight),   K2Q_METHOD(gemm_dx),        K2Q_METHOD(dequant_fp8),
                          K2Q_METHOD(gemm_bf16),   K2Q_METHOD(pad_factors),    K2Q_METHOD(resnorm),
                          K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         K2Q_METHOD(linear_infer),
-                         K2Q_METHOD(capture_id),  K2Q_METHOD(resnorm_stream_bwd), {nullptr, nullptr, 0, nullptr}};
+                         K2Q_METHOD(capture_id),  K2Q_METHOD(resnorm_stream_bwd),
+                         K2Q_METHOD(grad_norm),   K2Q_METHOD(adamw),          K2Q_METHOD(moments),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

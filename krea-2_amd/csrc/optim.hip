@@ -1,0 +1,527 @@
+// The step behind a backward pass, over many tensors in few launches: the gradients' norm and their scaling to a largest
+// one (the trainer's clip_grad_norm_, reference train_t2i_lora_cached.py:329), and AdamW (the line after it) with moments in
+// 32 bits or in 8.
+//
+// A launch takes up to TENSORS tensors by value, in its argument block: pointers move from step to step (autograd allocates
+// gradients anew), and nothing has to be copied to the device or kept there.  A workgroup finds its tensor by bisecting the
+// workgroups' prefix sums, on the scalar unit.
+#include <math.h>
+
+#include "k2q_common.h"
+#include "rotation.h"
+
+namespace {
+
+constexpr int TENSORS = 64;           // 40 bytes each: 2.8 KB of arguments
+constexpr int THREADS = 256;
+constexpr int BLOCK = K2Q_MOMENT_BLOCK;
+
+struct Item {
+  void* p;
+  void* g;
+  int64_t n;
+  int64_t at;         // the tensor's place in the moments' buffers
+  int32_t slot;       // its scalars
+  int32_t vec;        // p and g take vector loads
+};
+
+struct Table {
+  Item t[TENSORS];
+  uint32_t first[TENSORS];    // a tensor's first workgroup
+  int32_t count;
+  uint32_t blocks;
+};
+
+__device__ __forceinline__ int tensor_of(const Table& a, uint32_t wg) {
+  int lo = 0;
+#pragma unroll
+  for (int s = TENSORS / 2; s; s >>= 1)
+    if (lo + s < a.count && a.first[lo + s] <= wg) lo += s;
+  return lo;
+}
+
+// V values of a tensor from element e on; what lies past its end reads as zero and is not written.
+template <int V>
+__device__ __forceinline__ void load(const float* p, int64_t e, int64_t n, bool vec, float (&v)[V]) {
+  if (vec && e + V <= n) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const v4f q = *reinterpret_cast<const v4f*>(p + e + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + j] = q[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = e + i < n ? p[e + i] : 0.f;
+  }
+}
+
+template <int V, typename T>
+__device__ __forceinline__ void load(const T* p, int64_t e, int64_t n, bool vec, float (&v)[V]) {
+  typedef T VecT __attribute__((ext_vector_type(4)));
+  if (vec && e + V <= n) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const VecT q = *reinterpret_cast<const VecT*>(p + e + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + j] = (float)q[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = e + i < n ? (float)p[e + i] : 0.f;
+  }
+}
+
+template <int V, typename T>
+__device__ __forceinline__ void store(T* p, int64_t e, int64_t n, bool vec, const T (&v)[V]) {
+  typedef T VecT __attribute__((ext_vector_type(4)));
+  if (vec && e + V <= n) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<VecT*>(p + e + i) = VecT{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e + i < n) p[e + i] = v[i];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Norm and scaling
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ double wave_add(double v) {
+#pragma unroll
+  for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
+  return v;
+}
+
+// Sums of squares of runs of `chunk` elements, one a workgroup.  The sums are in 64 bits: squares of 32-bit values neither
+// overflow nor vanish there, and the card adds them at half the 32-bit rate, ten times what the reads need.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void sumsq_kernel(Table a, int64_t chunk, double* part) {
+  __shared__ double sums[THREADS / 64];
+  const int i = tensor_of(a, blockIdx.x);
+  const Item& it = a.t[i];
+  const T* g = static_cast<const T*>(it.g);
+  const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
+  const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
+  double s = 0;
+#pragma unroll 4
+  for (int64_t e = begin + threadIdx.x * 4; e < end; e += THREADS * 4) {
+    float v[4];
+    load<4>(g, e, n, it.vec, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = __builtin_fma((double)v[j], (double)v[j], s);
+  }
+  s = wave_add(s);
+  if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+// The norm and the factor that brings it to max_norm: partials in a fixed order.
+__global__ __launch_bounds__(1024) void norm_kernel(const double* part, int64_t n, double max_norm, float* out) {
+  __shared__ double sums[16];
+  double s = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
+  s = wave_add(s);
+  if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0;
+  for (int i = 0; i < 16; ++i) s += sums[i];
+  const double norm = sqrt(s), by = max_norm / (norm + 1e-6);
+  out[0] = (float)norm;
+  out[1] = by > 1.0 ? 1.f : (float)by;      // a norm that is no number gives a factor that is none
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void scale_kernel(Table a, int64_t chunk, const float* by) {
+  const int i = tensor_of(a, blockIdx.x);
+  const Item& it = a.t[i];
+  T* g = static_cast<T*>(it.g);
+  const float f = by[0];
+  const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
+  const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
+#pragma unroll 4
+  for (int64_t e = begin + threadIdx.x * 4; e < end; e += THREADS * 4) {
+    float v[4];
+    T o[4];
+    load<4>(g, e, n, it.vec, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (T)(v[j] * f);
+    store<4>(g, e, n, it.vec, o);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------------------------------------------
+// 32 random bits: two rounds of a shift and a product modulo 2^32, with constants of low bias found by C. Wellons (public
+// domain).  Every element of a step has its own: its place, mixed with the seed's and the step's.
+__device__ __forceinline__ uint32_t mix(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x7FEB352Du;
+  h = (h ^ (h >> 15)) * 0x846CA68Bu;
+  return h ^ (h >> 16);
+}
+
+struct Scalars {
+  float decay;      // 1 - lr weight_decay
+  float size;       // lr / (1 - beta1^t)
+  float root;       // 1 / sqrt(1 - beta2^t)
+  uint32_t key;
+};
+
+// A step's scalars for every tensor, in 64 bits (1 - beta^t loses digits in 32), and the count of steps one further.  A norm
+// that is not finite stops the step: nothing of the tensors changes.
+__global__ __launch_bounds__(THREADS) void begin_kernel(float* steps, int n, double lr, const float* lr_of, double beta1,
+                                                        double beta2, double decay, const float* norm, uint32_t seed,
+                                                        Scalars* out) {
+  const int i = blockIdx.x * THREADS + threadIdx.x;
+  if (i >= n || (norm && !(fabsf(norm[0]) <= 3.402823466e38f))) return;
+  const float t = steps[i] + 1.f;
+  steps[i] = t;
+  if (lr_of) lr = (double)lr_of[0];
+  Scalars s;
+  s.decay = (float)(1.0 - lr * decay);
+  s.size = (float)(lr / (1.0 - pow(beta1, (double)t)));
+  s.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
+  s.key = mix(mix(seed) ^ (uint32_t)t);
+  out[i] = s;
+}
+
+// Numbers in 8 bits.  The first moment: sign, 4 bits of exponent and 3 of fraction (OCP e4m3, so a state is a
+// float8_e4m3fn tensor), scaled so that the block's largest magnitude is 448.  The root of the second: 4 bits of each, no
+// sign, scaled so that the largest is 31744 (code 255).  The step between neighbours is 2^-3 and 2^-4 of a value at most, over
+// 17 and 19 binary orders below the largest, and evenly spaced below those.  A moment moves by a tenth (a thousandth) of its
+// distance to the gradient, less than half a code, so that rounding to the nearest would leave it where it is: the code is
+// chosen at random between the two neighbours, with the chances that make its mean the value.  No root above zero becomes
+// zero: the parameter would move by m / eps.
+constexpr float M_TOP = 448.f, V_TOP = 31744.f;
+constexpr float SMALLEST = 0x1p-100f;     // a block whose largest value is under this holds zeros: 448 / it stays finite
+
+__device__ __forceinline__ uint32_t code_m(float m, float by, uint32_t random) {
+  const float a = fminf(fabsf(m) * by, M_TOP);
+  const bool small = a < 0x1p-6f;
+  const uint32_t bits = __float_as_uint(small ? a + 0x1p-6f : a) + (random << 4);
+  const uint32_t code = (bits >> 20) - (small ? 121u * 8 : 120u * 8);
+  return fabsf(m) <= 3.402823466e38f ? code | (__float_as_uint(m) >> 31 << 7) : 0x7Fu;
+}
+
+__device__ __forceinline__ uint32_t code_v(float r, float by, uint32_t random) {
+  const float a = fminf(r * by, V_TOP);
+  const bool small = a < 1.f;
+  const uint32_t bits = __float_as_uint(small ? a + 1.f : a) + (random << 3);
+  const uint32_t code = (bits >> 19) - (small ? 127u * 16 : 126u * 16);
+  return !(r <= 3.402823466e38f) ? 255u : a > 0.f && code == 0 ? 1u : code;
+}
+
+__device__ __forceinline__ float value_v(uint32_t c) {
+  const bool small = c < 16;
+  return __uint_as_float((c + (small ? 127u * 16 : 126u * 16)) << 19) - (small ? 1.f : 0.f);
+}
+
+template <int I>
+__device__ __forceinline__ float value_m(uint32_t w) {
+  return __builtin_amdgcn_cvt_f32_fp8((int)w, I);
+}
+
+__device__ __forceinline__ float decode_m(uint32_t w, int i) {
+  switch (i) {
+    case 0: return value_m<0>(w);
+    case 1: return value_m<1>(w);
+    case 2: return value_m<2>(w);
+    default: return value_m<3>(w);
+  }
+}
+
+// The largest of a value's 32 neighbours (half a wave).
+__device__ __forceinline__ float half_max(float m) {
+  m = fmaxf(m, k2q_rot::dpp_f<0xB1>(m));
+  m = fmaxf(m, k2q_rot::dpp_f<0x4E>(m));
+  m = fmaxf(m, k2q_rot::dpp_f<0x141>(m));
+  m = fmaxf(m, k2q_rot::dpp_f<0x140>(m));
+  return fmaxf(m, __shfl_xor(m, 16));
+}
+
+struct Step {
+  void* m;            // 32 bits: floats; 8 bits: codes
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  const Scalars* scalars;
+  const float* norm;  // {norm, factor}, or null
+  float beta1, alpha1, beta2, alpha2, eps;
+  int stochastic;
+};
+
+// Parameters in 16 bits that are rounded at random: 16 random bits below the kept ones, then the rest is cut off.
+template <typename T>
+__device__ __forceinline__ T rounded(float p, int stochastic, uint32_t random) {
+  if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) {
+    if (stochastic) {
+      const uint32_t bits = __float_as_uint(p);
+      const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+      return __builtin_bit_cast(T, (uint16_t)((finite ? bits + (random & 0xFFFFu) : bits | (bits & 0xFFFFu ? 0x400000u : 0u)) >> 16));
+    }
+  }
+  return (T)p;
+}
+
+constexpr int64_t CHUNK = 8192;       // elements of a workgroup
+
+// One element's moments and parameter, each operation rounded once in 32 bits:
+//   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  p = decay p - size m / (root sqrt(v) + eps)
+__device__ __forceinline__ void element(const Step& a, const Scalars& s, float g, float& m, float& v, float& r, float& p) {
+  m = m * a.beta1 + g * a.alpha1;
+  v = v * a.beta2 + g * g * a.alpha2;
+  r = sqrtf(v);
+  p = p * s.decay - m / (r * s.root + a.eps) * s.size;
+}
+
+template <typename T, bool kCodes>
+__global__ __launch_bounds__(THREADS) void adamw_kernel(Table a, Step st) {
+  float by = 1.f;
+  if (st.norm) {
+    if (!(fabsf(st.norm[0]) <= 3.402823466e38f)) return;
+    by = st.norm[1];
+  }
+  const int i = tensor_of(a, blockIdx.x);
+  const Item& it = a.t[i];
+  const Scalars s = st.scalars[it.slot];
+  T* P = static_cast<T*>(it.p);
+  const T* G = static_cast<const T*>(it.g);
+  const int64_t n = it.n, at = it.at, begin = (int64_t)(blockIdx.x - a.first[i]) * CHUNK;
+  // moments reach to the end of the last block
+  const int64_t end = begin + CHUNK < n ? begin + CHUNK : (n + BLOCK - 1) / BLOCK * BLOCK;
+  constexpr int V = kCodes ? 8 : 4;
+  for (int64_t e = begin + threadIdx.x * V; e < end; e += THREADS * V) {
+    float p[V], g[V], m[V], v[V], r[V];
+    T o[V];
+    load<V>(P, e, n, it.vec, p);
+    load<V>(G, e, n, it.vec, g);
+    uint32_t random[V];
+    const uint64_t place = (uint64_t)(at + e);
+    const uint32_t key = s.key ^ (uint32_t)(place >> 32) * 0x9E3779B9u;
+    if (kCodes || st.stochastic) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) random[j] = mix((uint32_t)(place + j) ^ key);
+    }
+    if constexpr (kCodes) {
+      v2u* cm = reinterpret_cast<v2u*>(static_cast<uint8_t*>(st.m) + place);
+      v2u* cv = reinterpret_cast<v2u*>(static_cast<uint8_t*>(st.v) + place);
+      const v2u wm = *cm, wv = *cv;
+      const float sm = st.m_scale[place / BLOCK], sv = st.v_scale[place / BLOCK];
+      float am = 0.f, av = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        m[j] = decode_m(wm[j / 4], j % 4) * sm;
+        const float root = value_v(wv[j / 4] >> (8 * (j % 4)) & 0xFFu) * sv;
+        v[j] = root * root;
+        element(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
+        am = fmaxf(am, fabsf(m[j]) <= 3.402823466e38f ? fabsf(m[j]) : 0.f);
+        av = fmaxf(av, r[j] <= 3.402823466e38f ? r[j] : 0.f);
+      }
+      am = half_max(am);
+      av = half_max(av);
+      am = am < SMALLEST ? 0.f : am;
+      av = av < SMALLEST ? 0.f : av;
+      const float fm = am > 0.f ? M_TOP / am : 0.f, fv = av > 0.f ? V_TOP / av : 0.f;
+      v2u nm = {0, 0}, nv = {0, 0};
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        nm[j / 4] |= code_m(m[j], fm, random[j] & 0xFFFFu) << (8 * (j % 4));
+        nv[j / 4] |= code_v(r[j], fv, random[j] >> 16) << (8 * (j % 4));
+      }
+      *cm = nm;
+      *cv = nv;
+      if (threadIdx.x % 32 == 0) {
+        st.m_scale[place / BLOCK] = am / M_TOP;
+        st.v_scale[place / BLOCK] = av / V_TOP;
+      }
+    } else {
+      v4f* fm = reinterpret_cast<v4f*>(static_cast<float*>(st.m) + place);
+      v4f* fv = reinterpret_cast<v4f*>(static_cast<float*>(st.v) + place);
+      v4f wm = *fm, wv = *fv;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        m[j] = wm[j];
+        v[j] = wv[j];
+        element(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
+        wm[j] = m[j];
+        wv[j] = v[j];
+      }
+      *fm = wm;
+      *fv = wv;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = rounded<T>(p[j], st.stochastic, st.stochastic ? mix(random[j] ^ 0x9E3779B9u) : 0u);
+    store<V>(P, e, n, it.vec, o);
+  }
+}
+
+// What codes stand for: m and v, in 32 bits or bf16.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void moments_kernel(const uint8_t* cm, const float* m_scale, const uint8_t* cv,
+                                                          const float* v_scale, int64_t n, T* m, T* v) {
+  const int64_t e = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 8;
+  if (e >= n) return;
+  const v2u wm = *reinterpret_cast<const v2u*>(cm + e), wv = *reinterpret_cast<const v2u*>(cv + e);
+  const float sm = m_scale[e / BLOCK], sv = v_scale[e / BLOCK];
+  T om[8], ov[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    om[j] = (T)(decode_m(wm[j / 4], j % 4) * sm);
+    const float root = value_v(wv[j / 4] >> (8 * (j % 4)) & 0xFFu) * sv;
+    ov[j] = (T)(root * root);
+  }
+  store<8>(m, e, n, true, om);
+  store<8>(v, e, n, true, ov);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------------------------
+int size_of(int dtype) { return dtype == K2Q_DTYPE_F32 ? 4 : 2; }
+
+int check(const k2q_step_tensor* t, int64_t count, bool params) {
+  if (!t || count < 1) return K2Q_EINVAL;
+  for (int64_t i = 0; i < count; ++i) {
+    if (t[i].dtype < K2Q_DTYPE_BF16 || t[i].dtype > K2Q_DTYPE_F16 || t[i].n < 1 || !t[i].g ||
+        !k2q_aligned(t[i].g, size_of(t[i].dtype)) ||
+        (params && (!t[i].p || !k2q_aligned(t[i].p, size_of(t[i].dtype)) || t[i].at < 0 || t[i].at % BLOCK || t[i].index < 0)))
+      return K2Q_EINVAL;
+    if (t[i].n > (int64_t)1 << 42 || t[i].at > (int64_t)1 << 46) return K2Q_EUNSUPPORTED;    // 2^29 workgroups
+  }
+  return K2Q_OK;
+}
+
+// Elements of a workgroup, for at most about 16384 partial sums: 8192 at least, which a small step spreads over CUs.
+int64_t norm_chunk(const k2q_step_tensor* t, int64_t count) {
+  int64_t total = 0, chunk = CHUNK;
+  for (int64_t i = 0; i < count; ++i) total += t[i].n;
+  while (total / chunk > 16384) chunk *= 2;
+  return chunk;
+}
+
+// f(table) over the tensors of one type, TENSORS and 2^30 workgroups at a time.
+template <class F>
+void each_table(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, F&& f) {
+  Table a{};
+  for (int64_t i = 0; i < count; ++i) {
+    if (t[i].dtype != dtype) continue;
+    const uint32_t blocks = (uint32_t)((t[i].n + chunk - 1) / chunk);
+    if (a.count == TENSORS || (a.count && (int64_t)a.blocks + blocks > 1 << 30)) {
+      f(a);
+      a.count = 0;
+      a.blocks = 0;
+    }
+    const uintptr_t both = (uintptr_t)t[i].p | (uintptr_t)t[i].g;
+    a.t[a.count] = {t[i].p, t[i].g, t[i].n, t[i].at, (int32_t)i, both % (4 * size_of(dtype)) == 0};
+    a.first[a.count++] = a.blocks;
+    a.blocks += blocks;
+  }
+  if (a.count) f(a);
+}
+
+template <class F>
+void by_type(F&& f) {
+  f(K2Q_DTYPE_BF16, __bf16{});
+  f(K2Q_DTYPE_F32, float{});
+  f(K2Q_DTYPE_F16, _Float16{});
+}
+
+}  // namespace
+
+extern "C" int64_t k2q_grad_norm_ws_bytes(const k2q_step_tensor* t, int64_t count) {
+  if (check(t, count, false) != K2Q_OK) return 0;
+  const int64_t chunk = norm_chunk(t, count);
+  int64_t parts = 0;
+  for (int64_t i = 0; i < count; ++i) parts += (t[i].n + chunk - 1) / chunk;
+  return parts * 8;
+}
+
+extern "C" int k2q_grad_norm(const k2q_step_tensor* t, int64_t count, double max_norm, void* ws, int64_t ws_bytes, float* out,
+                             void* stream) {
+  int rc = check(t, count, false);
+  if (rc != K2Q_OK) return rc;
+  const int64_t need = k2q_grad_norm_ws_bytes(t, count);
+  if (!(max_norm >= 0) || !ws || ws_bytes < need || !k2q_aligned(ws, 16) || !out || !k2q_aligned(out, 8)) return K2Q_EINVAL;
+  const int64_t chunk = norm_chunk(t, count);
+  double* part = static_cast<double*>(ws);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  by_type([&](int dtype, auto T) {
+    each_table(t, count, dtype, chunk, [&](const Table& a) {
+      hipLaunchKernelGGL(sumsq_kernel<decltype(T)>, dim3(a.blocks), dim3(THREADS), 0, st, a, chunk, part);
+      part += a.blocks;
+    });
+  });
+  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(1024), 0, st, static_cast<const double*>(ws), need / 8, max_norm, out);
+  return k2q_launch_status();
+}
+
+extern "C" int k2q_scale_grads(const k2q_step_tensor* t, int64_t count, const float* by, void* stream) {
+  int rc = check(t, count, false);
+  if (rc != K2Q_OK) return rc;
+  if (!by || !k2q_aligned(by, 4)) return K2Q_EINVAL;
+  by_type([&](int dtype, auto T) {
+    each_table(t, count, dtype, CHUNK, [&](const Table& a) {
+      hipLaunchKernelGGL(scale_kernel<decltype(T)>, dim3(a.blocks), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a,
+                         CHUNK, by);
+    });
+  });
+  return k2q_launch_status();
+}
+
+extern "C" int64_t k2q_adamw_ws_bytes(int64_t count) { return count < 1 ? 0 : count * (int64_t)sizeof(Scalars); }
+
+extern "C" int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits, void* exp_avg, void* exp_avg_sq,
+                         float* avg_scale, float* sq_scale, float* steps, double lr, const float* lr_of, double beta1,
+                         double beta2, double eps, double weight_decay, const float* norm, int stochastic, uint32_t seed,
+                         void* ws, int64_t ws_bytes, void* stream) {
+  int rc = check(t, count, true);
+  if (rc != K2Q_OK) return rc;
+  if ((state_bits != 32 && state_bits != 8) || !exp_avg || !exp_avg_sq || !k2q_aligned(exp_avg, 16) ||
+      !k2q_aligned(exp_avg_sq, 16) || (state_bits == 8 && (!avg_scale || !sq_scale)) || !k2q_aligned(avg_scale, 4) ||
+      !k2q_aligned(sq_scale, 4) || !steps || !k2q_aligned(steps, 4) || !(beta1 >= 0 && beta1 < 1) ||
+      !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(lr == lr) || !(weight_decay >= 0) || !k2q_aligned(lr_of, 4) ||
+      !k2q_aligned(norm, 8) || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_adamw_ws_bytes(count) || count > 0x7fffffff)
+    return K2Q_EINVAL;
+  for (int64_t i = 0; i < count; ++i)
+    if ((stochastic && t[i].dtype == K2Q_DTYPE_F16) || (i && t[i].index <= t[i - 1].index)) return K2Q_EINVAL;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  Scalars* scalars = static_cast<Scalars*>(ws);
+  for (int64_t i = 0, j; i < count; i = j) {      // counts of neighbouring places in one launch
+    for (j = i + 1; j < count && t[j].index == t[j - 1].index + 1;) ++j;
+    hipLaunchKernelGGL(begin_kernel, dim3((unsigned)((j - i + THREADS - 1) / THREADS)), dim3(THREADS), 0, st,
+                       steps + t[i].index, (int)(j - i), lr, lr_of, beta1, beta2, weight_decay, norm, seed, scalars + i);
+  }
+  const Step s{exp_avg, exp_avg_sq, avg_scale, sq_scale, scalars, norm, (float)beta1, (float)(1 - beta1), (float)beta2,
+               (float)(1 - beta2), (float)eps, stochastic};
+  by_type([&](int dtype, auto T) {
+    each_table(t, count, dtype, CHUNK, [&](const Table& a) {
+      if (state_bits == 8)
+        hipLaunchKernelGGL((adamw_kernel<decltype(T), true>), dim3(a.blocks), dim3(THREADS), 0, st, a, s);
+      else
+        hipLaunchKernelGGL((adamw_kernel<decltype(T), false>), dim3(a.blocks), dim3(THREADS), 0, st, a, s);
+    });
+  });
+  return k2q_launch_status();
+}
+
+extern "C" int k2q_moments(const uint8_t* avg, const float* avg_scale, const uint8_t* sq, const float* sq_scale, int64_t n,
+                           int dtype, void* m, void* v, void* stream) {
+  if (!avg || !avg_scale || !sq || !sq_scale || !m || !v || n < BLOCK || n % BLOCK || !k2q_aligned(avg, 8) ||
+      !k2q_aligned(sq, 8) || !k2q_aligned(avg_scale, 4) || !k2q_aligned(sq_scale, 4) || !k2q_aligned(m, 16) ||
+      !k2q_aligned(v, 16) || (dtype != K2Q_DTYPE_BF16 && dtype != K2Q_DTYPE_F32))
+    return K2Q_EINVAL;
+  if (n > (int64_t)THREADS * 8 << 30) return K2Q_EUNSUPPORTED;
+  const dim3 grid((unsigned)((n / 8 + THREADS - 1) / THREADS));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == K2Q_DTYPE_BF16)
+    hipLaunchKernelGGL(moments_kernel<__bf16>, grid, dim3(THREADS), 0, st, avg, avg_scale, sq, sq_scale, n,
+                       static_cast<__bf16*>(m), static_cast<__bf16*>(v));
+  else
+    hipLaunchKernelGGL(moments_kernel<float>, grid, dim3(THREADS), 0, st, avg, avg_scale, sq, sq_scale, n,
+                       static_cast<float*>(m), static_cast<float*>(v));
+  return k2q_launch_status();
+}

@@ -1,0 +1,220 @@
+"""The step behind a LoRA training step's backward pass, over every factor in a few launches: ``clip_grad_norm_`` and AdamW,
+the two lines that the reference's trainer takes from torch (``train_t2i_lora_cached.py:329-332``).
+
+:class:`AdamW` keeps its moments in 32 bits, or in 8 bits with a scale for every 256 elements: 2 bytes for an element in
+place of 8, and 16 bytes moved by a step in place of 28.  A group's moments lie in flat buffers, each parameter's at a
+multiple of 256 elements; ``state[p]`` holds views of them.
+"""
+from __future__ import annotations
+
+import math
+from types import SimpleNamespace
+
+import torch
+
+from . import _lib
+
+_BLOCK = _lib.MOMENT_BLOCK
+
+
+def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
+    """Scale the gradients of ``parameters`` (a tensor, or an iterable of them) in place so that their 2-norm, taken over all
+    together, is at most ``max_norm``: ``torch.nn.utils.clip_grad_norm_`` of the 2-norm.  Returns the norm before, a float32
+    tensor on the gradients' device (nothing waits for it).  The factor is ``min(1, max_norm / (norm + 1e-6))`` and each
+    gradient is rounded once; a norm that is infinite or NaN gives the gradients that torch's gives."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be 0 or above, got {max_norm}")
+    out = _lib.grad_norm(params, max_norm, True)
+    return torch.zeros(()) if out is None else out[0]
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (Loshchilov and Hutter, "Decoupled weight decay regularization", 2019) with the update of ``torch.optim.AdamW``,
+    in float32, over parameters in float32, bfloat16 or float16 whose gradients have their type.
+
+    ``max_norm``: the gradients, over all groups together, are first brought to this 2-norm at most, as ``clip_grad_norm_``
+    does it, but they are not written: the step multiplies them as it reads them.  :attr:`grad_norm` holds the norm of the
+    last step.  A norm that is infinite or NaN skips the step on the device: parameters, moments and counts stay.
+
+    ``state_bits=8``: the first moment in e4m3, the root of the second in 4 bits of exponent and 4 of fraction, both scaled
+    by the largest of 256 neighbours.  ``stochastic=True`` rounds bfloat16 parameters to one of their two neighbours at
+    random instead of to the nearest, so that updates below half a step are not lost (the reference's full fine-tune does
+    that, ``fused_adamw.py:44-56``).  Codes and such parameters are rounded by chance, with bits that are a function of
+    ``seed``, the step and the element's place in its group: equal runs give equal results.
+
+    ``lr`` may be a float32 tensor of one element on the device (read there, for captured graphs).  Without ``max_norm``, a
+    gradient that is infinite or NaN spoils its own element, as in torch.  Make a step, or load a state, before a graph
+    capture: the moments are made at the first."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 max_norm: float | None = None, state_bits: int = 32, stochastic: bool = False, seed: int = 0):
+        defaults = {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay, "state_bits": state_bits,
+                    "stochastic": stochastic, "seed": seed}
+        if max_norm is not None and not float(max_norm) >= 0:
+            raise ValueError(f"max_norm must be 0 or above, got {max_norm}")
+        self.max_norm = None if max_norm is None else float(max_norm)
+        self.grad_norm = None
+        self._held = {}         # group number -> its moments' buffers
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group: dict) -> None:
+        for name, value in self.defaults.items():
+            param_group.setdefault(name, value)
+        _check_options(param_group)
+        super().add_param_group(param_group)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.setdefault("max_norm", None)
+        self.grad_norm, self._held = None, {}       # laid out again from the states at the next step
+        super().__setstate__(state)
+        for group in self.param_groups:
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+            _check_options(group)
+
+    # -- moments -------------------------------------------------------------------------------------------------
+    def _moments_of(self, i: int) -> SimpleNamespace:
+        """Group ``i``'s buffers, made when they are not there: zeros, or the states that its parameters have."""
+        held = self._held.get(i)
+        if held is not None:
+            return held
+        group = self.param_groups[i]
+        params = group["params"]
+        devices = {p.device for p in params}
+        if len(devices) != 1 or next(iter(devices)).type != "cuda":
+            raise RuntimeError(f"k2q kernels need a group's parameters on one gfx950 GPU, got {sorted(map(str, devices))}")
+        dev = next(iter(devices))
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the moments are not made yet and a graph capture would make them at every replay: make a "
+                               "step, or load a state, before it")
+        for k, p in enumerate(params):
+            if p.dtype not in _lib.STEP_DTYPES:
+                raise ValueError(f"parameter {k} of group {i} is {p.dtype}, not one of {_lib.STEP_DTYPES}")
+        starts, total = [], 0
+        for p in params:
+            starts.append(total)
+            total += -(-p.numel() // _BLOCK) * _BLOCK
+        held = SimpleNamespace(starts=starts, steps=torch.zeros(len(params), device=dev))
+        kinds = _kinds(group["state_bits"])
+        for name, (dtype, per) in kinds.items():
+            setattr(held, name, torch.zeros(total // per, device=dev, dtype=torch.uint8).view(dtype)
+                    if dtype.itemsize == 1 else torch.zeros(total // per, device=dev, dtype=dtype))
+        with torch.no_grad():
+            for k, (p, start) in enumerate(zip(params, starts)):
+                old, new = self.state.get(p), {"step": held.steps[k]}
+                for name, (dtype, per) in kinds.items():
+                    flat = getattr(held, name)
+                    new[name] = flat[start:start + p.numel()].view(p.shape) if per == 1 else \
+                        flat[start // per:start // per - (-p.numel() // per)]
+                if old:
+                    for name, view in new.items():
+                        _copy(view, old[name])
+                self.state[p] = new
+        self._held[i] = held
+        return held
+
+    def moments(self, group: int = 0, dtype: torch.dtype = torch.float32):
+        """``(exp_avg, exp_avg_sq)`` of a group's parameters as numbers, flat, each parameter's from a multiple of 256
+        elements on: its own buffers where they are held in ``dtype``, else what they hold in ``dtype`` (float32 or
+        bfloat16)."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
+        held = self._moments_of(group)
+        if self.param_groups[group]["state_bits"] == 32:
+            return held.exp_avg.to(dtype), held.exp_avg_sq.to(dtype)
+        return _lib.moments(held.exp_avg, held.exp_avg_scale, held.exp_avg_sq, held.exp_avg_sq_scale, dtype)
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """A state of this class, or, in 32 bits, of ``torch.optim.AdamW`` (without ``amsgrad`` or ``maximize``).  The values
+        are copied, in their own types."""
+        super().load_state_dict({**state_dict, "state": {}})
+        numbers = [n for g in state_dict["param_groups"] for n in g["params"]]
+        for n, p in zip(numbers, (p for g in self.param_groups for p in g["params"])):
+            if n in state_dict["state"]:
+                self.state[p] = dict(state_dict["state"][n])
+        try:
+            for i, group in enumerate(self.param_groups):
+                for p in group["params"]:
+                    _check_state(self.state.get(p), p, group["state_bits"])
+                if any(p in self.state for p in group["params"]):
+                    self._moments_of(i)
+        except BaseException:
+            self.state.clear()
+            self._held.clear()
+            raise
+
+    # -- the step ------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups, norm = self.param_groups, None
+        if self.max_norm is not None:
+            every = groups[0]["params"] if len(groups) == 1 else [p for g in groups for p in g["params"]]
+            norm = _lib.grad_norm(every, self.max_norm, False)
+            self.grad_norm = None if norm is None else norm[0]
+        for i, g in enumerate(groups):
+            held = self._held.get(i) or self._moments_of(i)
+            lr, lr_of = g["lr"], None
+            if isinstance(lr, torch.Tensor):
+                lr, lr_of = (0.0, lr) if lr.is_cuda else (float(lr), None)
+            scales = (held.exp_avg_scale, held.exp_avg_sq_scale) if g["state_bits"] == 8 else (None, None)
+            _lib.adamw(g["params"], held.starts, g["state_bits"], held.exp_avg, held.exp_avg_sq, *scales, held.steps, lr,
+                       lr_of, *g["betas"], g["eps"], g["weight_decay"], norm, g["stochastic"], g["seed"])
+        return loss
+
+
+def _kinds(bits: int) -> dict:
+    """A parameter's states but the count of steps: (type, elements that share one)."""
+    if bits == 32:
+        return {"exp_avg": (torch.float32, 1), "exp_avg_sq": (torch.float32, 1)}
+    return {"exp_avg": (torch.float8_e4m3fn, 1), "exp_avg_sq": (torch.uint8, 1), "exp_avg_scale": (torch.float32, _BLOCK),
+            "exp_avg_sq_scale": (torch.float32, _BLOCK)}
+
+
+def _copy(view: torch.Tensor, value) -> None:
+    if not isinstance(value, torch.Tensor):
+        view.fill_(value)
+    elif view.dtype.itemsize == 1:
+        view.view(torch.uint8).copy_(value.contiguous().view(torch.uint8))
+    else:
+        view.copy_(value)
+
+
+def _check_options(g: dict) -> None:
+    lr, (beta1, beta2) = g["lr"], g["betas"]
+    if isinstance(lr, torch.Tensor):
+        if lr.numel() != 1 or lr.dtype != torch.float32:
+            raise ValueError(f"lr as a tensor must be one float32 element, got {tuple(lr.shape)} {lr.dtype}")
+    elif not (lr >= 0 and math.isfinite(lr)):
+        raise ValueError(f"lr must be 0 or above, got {lr}")
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
+        raise ValueError(f"betas must be from 0 to below 1, got {g['betas']}")
+    if not g["eps"] >= 0 or not g["weight_decay"] >= 0:
+        raise ValueError(f"eps and weight_decay must be 0 or above, got {g['eps']} and {g['weight_decay']}")
+    if g["state_bits"] not in (32, 8):
+        raise ValueError(f"state_bits must be 32 or 8, got {g['state_bits']}")
+    if not (isinstance(g["seed"], int) and 0 <= g["seed"] < 1 << 32):
+        raise ValueError(f"seed must be an integer of 32 bits, got {g['seed']}")
+    for name in ("amsgrad", "maximize"):
+        if g.get(name):
+            raise ValueError(f"{name} is not offered")
+
+
+def _check_state(state: dict | None, p: torch.Tensor, bits: int) -> None:
+    if state is None:
+        return
+    kinds = _kinds(bits)
+    if set(state) != {"step", *kinds}:
+        raise ValueError(f"a state in {bits} bits holds {sorted(('step', *kinds))}, got {sorted(state)}")
+    for name, (dtype, per) in kinds.items():
+        shape = tuple(p.shape) if per == 1 else (-(-p.numel() // per),)
+        if state[name].dtype != dtype or tuple(state[name].shape) != shape:
+            raise ValueError(f"{name} must be {dtype} {shape}, got {state[name].dtype} {tuple(state[name].shape)}")
