@@ -396,6 +396,38 @@ int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, int64_t M, i
                            const float* lora_a, int64_t r, uint16_t* dx, void* ws, int64_t ws_bytes, void* stream);
 
 
+/* Low-rank adapters of many requests beside one projection (LoRALinear.forward, lora.py:43-48, with an adapter of its own
+ * for every row).  Row t of T has the adapter a = ids[t / per] of a bank (T a multiple of per), none where that is outside
+ * 0 .. count - 1; A count x R x K and B count x N x R, both bf16 or f32; of adapter a the first ranks[a] (NULL: R; rounded up
+ * to 16) ranks count, f = scale * scales[a] (NULL: scale):
+ *   u[t] = f x[t] A_a^T,  out[t] = bf16(y[t] + u[t] B_a^T)   (y[t] for a row without adapter; y NULL: zeros; out may be y)
+ * u (T x R f32, nullable) is what the backward reads; ranks past an adapter's, and rows without one, are not written.
+ * k2q_bank_bwd: g[t] = f dy[t] B_a,  dx[t] = bf16(base[t] + g[t] A_a) (base nullable: zeros; dx may be base),
+ *   dA_a = sum_t g[t]^T x[t] and dB_a = sum_t dy[t]^T u[t] over the adapter's rows, in the factors' type, zeros for an adapter
+ *   without rows and for ranks past its own.  dx, dA (with x), dB (with u) are nullable; one at least is given.
+ * x T x K, y, out and dy T x N, dx T x K: bf16, contiguous.  Sums are f32 in a fixed order; f32 factors, u and g enter the
+ * products in 16 bits of precision.  K and N multiples of 64, R of 16, count <= K2Q_MAX_ADAPTERS, T < 2^31 - 256.
+ * ws: *_ws_bytes bytes, 16-byte aligned (need_factors: dA or dB is given). */
+#define K2Q_MAX_ADAPTERS 1024
+typedef struct {
+  const void* A;
+  const void* B;
+  const void* ids;          /* int32 or int64 */
+  const int32_t* ranks;
+  const float* scales;
+  float scale;
+  int32_t ids64;
+  int32_t dtype;            /* of A and B */
+  int32_t count, R;
+  int32_t K, N;
+} k2q_bank;
+int64_t k2q_bank_fwd_ws_bytes(const k2q_bank* b, int64_t T, int64_t per);
+int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* x, const uint16_t* y, uint16_t* out, float* u,
+                 void* ws, int64_t ws_bytes, void* stream);
+int64_t k2q_bank_bwd_ws_bytes(const k2q_bank* b, int64_t T, int64_t per, int need_factors);
+int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* dy, const uint16_t* x, const float* u,
+                 const uint16_t* base, uint16_t* dx, void* dA, void* dB, void* ws, int64_t ws_bytes, void* stream);
+
 /* The step behind a backward pass, over a list of tensors (no counterpart in the reference's kernels; its trainer calls
  * torch's clip_grad_norm_ and AdamW, train_t2i_lora_cached.py:329-332).  t: host array, count tensors of n contiguous elements
  * of type dtype (bf16, f32, f16), g their gradients in the same type; read before the call returns.

@@ -52,6 +52,12 @@ class RotaryHeads(ctypes.Structure):
         (name, ctypes.c_int64) for name in ("x_b", "x_l", "x_h", "o_b", "o_l", "o_h")]
 
 
+class Bank(ctypes.Structure):
+    """``k2q_bank`` of ``include/k2q.h``: a bank of adapters and the ids of the rows that have them."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("A", "B", "ids", "ranks", "scales")] + [("scale", ctypes.c_float)] + [
+        (name, ctypes.c_int32) for name in ("ids64", "dtype", "count", "R", "K", "N")]
+
+
 class StepTensor(ctypes.Structure):
     """``k2q_step_tensor`` of ``include/k2q.h``: one tensor of an optimizer's step."""
     _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("n", ctypes.c_int64), ("at", ctypes.c_int64),
@@ -125,6 +131,10 @@ _SIGNATURES = {
     "k2q_gemm_dx_ws_bytes": ([_i64, _i64, _i64], _i64),
     "k2q_gemm_dx": ([_p, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _p], _int),
     "k2q_gemm_dx_grouped": ([_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p], _int),
+    "k2q_bank_fwd_ws_bytes": ([_p, _i64, _i64], _i64),
+    "k2q_bank_fwd": ([_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p], _int),
+    "k2q_bank_bwd_ws_bytes": ([_p, _i64, _i64, _int], _i64),
+    "k2q_bank_bwd": ([_p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p], _int),
     "k2q_grad_norm_ws_bytes": ([_p, _i64], _i64),
     "k2q_grad_norm": ([_p, _i64, _f64, _p, _i64, _p, _p], _int),
     "k2q_scale_grads": ([_p, _i64, _p, _p], _int),
@@ -1485,3 +1495,68 @@ def moments(exp_avg, avg_scale, exp_avg_sq, sq_scale, dtype):
     r = _fast().moments(*args)
     return r if r.__class__ is tuple else _refused(r, "k2q_moments", lambda: _native.moments(*args),
                                                    lambda: _device_check(exp_avg.device))
+
+
+# ----------------------------------------------------------------------------------------------------------
+# Adapters of many requests beside one projection
+# ----------------------------------------------------------------------------------------------------------
+MAX_ADAPTERS = 1024     # K2Q_MAX_ADAPTERS
+BANK_ALIGN = 64         # in and out features of a bank
+
+
+def check_bank(t, width: int, A, B, ids, scales, ranks) -> None:
+    """What the bank's kernels take: ``t`` is a tensor of the batch, of this width."""
+    dev = t.device
+    if A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2]:
+        raise ValueError(f"lora_A {tuple(A.shape)} and lora_B {tuple(B.shape)} must be (count, rank, in) and "
+                         "(count, out, rank)")
+    (count, R, K), N = A.shape, B.shape[1]
+    if A.dtype not in (torch.float32, torch.bfloat16) or B.dtype != A.dtype:
+        raise ValueError(f"the factors must be both float32 or both bfloat16, got {A.dtype} and {B.dtype}")
+    _check_rank(R)
+    if not 1 <= count <= MAX_ADAPTERS:
+        raise ValueError(f"{count} adapters: a bank holds 1 to {MAX_ADAPTERS}")
+    if K < BANK_ALIGN or K % BANK_ALIGN or N < BANK_ALIGN or N % BANK_ALIGN or max(K, N) > 1 << 24:
+        raise ValueError(f"a bank's in and out features must be multiples of {BANK_ALIGN}, got {K} -> {N}")
+    _need(A, "lora_A", A.dtype, 3, dev)
+    _need(B, "lora_B", A.dtype, 3, dev)
+    if t.dim() < 2 or t.shape[-1] != width:
+        raise ValueError(f"a tensor of shape {tuple(t.shape)} where (.., {width}) is wanted")
+    _need(t, "a tensor of the batch", torch.bfloat16)
+    if ids.dtype not in (torch.int32, torch.int64) or ids.device != dev or not ids.is_contiguous():
+        raise ValueError(f"adapters must be contiguous int32 or int64 on {dev}, got {ids.dtype} on {ids.device}")
+    if not 1 <= ids.dim() < t.dim() or ids.shape != t.shape[:ids.dim()]:
+        raise ValueError(f"adapters {tuple(ids.shape)} must be one for each of x's first dimensions, got {tuple(t.shape)}")
+    for v, name, dtype in ((scales, "scales", torch.float32), (ranks, "ranks", torch.int32)):
+        if v is not None and (v.dtype != dtype or v.numel() != count or v.device != dev or not v.is_contiguous()):
+            raise ValueError(f"{name} must be {count} contiguous {dtype} values on {dev}, got {tuple(v.shape)} {v.dtype} on "
+                             f"{v.device}")
+    if t.numel() // width > 0x7fffff00:
+        raise ValueError(f"{t.numel() // width} rows: 2^31 - 256 are the most")
+    _device_check(dev)
+
+
+def _check_bank_fwd(y, x, A, B, ids, scales, ranks) -> None:
+    for t, name in ((y, "y"), (x, "x")):
+        if t.dtype != torch.bfloat16:
+            raise NotImplementedError(f"adapters run on bf16 activations (the DiT dtype); {name} is {t.dtype}")
+    if y.shape[:-1] != x.shape[:-1] or y.device != x.device:
+        raise ValueError(f"y {tuple(y.shape)} on {y.device} and x {tuple(x.shape)} on {x.device} differ in their rows")
+    check_bank(x, A.shape[-1], A, B, ids, scales, ranks)
+    check_bank(y, B.shape[1], A, B, ids, scales, ranks)
+
+
+def bank_fwd(y, x, A, B, ids, scales, ranks, scale: float, need_u: bool):
+    """``(out, u | None)`` of :func:`add_adapters` (``k2q_bank_fwd``)."""
+    args = (y, x, A, B, ids, scales, ranks, scale, need_u)
+    r = _fast().bank_fwd(*args)
+    return r if r.__class__ is tuple else _refused(r, "k2q_bank_fwd", lambda: _native.bank_fwd(*args),
+                                                   lambda: _check_bank_fwd(*args[:7]))
+
+
+def bank_bwd(dy, x, u, A, B, ids, scales, ranks, scale: float, base, need_x: bool, need_A: bool, need_B: bool):
+    """``(dx, dA, dB)``, each as it is needed (``k2q_bank_bwd``); ``base``: a gradient of x that dx is added to in place."""
+    args = (dy, x, u, A, B, ids, scales, ranks, scale, base, need_x, need_A, need_B)
+    r = _fast().bank_bwd(*args)
+    return r if r.__class__ is tuple else _refused(r, "k2q_bank_bwd", lambda: _native.bank_bwd(*args),
+                                                   lambda: check_bank(dy, B.shape[1], A, B, ids, scales, ranks))

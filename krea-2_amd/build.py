@@ -17,7 +17,7 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 LIB = HERE / "libk2q.so"
 SOURCES = ("api.hip", "rotquant.hip", "producers.hip", "gemm.hip", "gemv.hip", "lora.hip", "lora_grad.hip", "fp8.hip",
-           "linear.hip", "rotary.hip", "optim.hip")
+           "linear.hip", "rotary.hip", "optim.hip", "lora_bank.hip")
 # bench.py's same-run MFMA ceiling: a measurement aid, built into its own library, not into the product's
 PROBE_SOURCES = ("probe.hip",)
 PROBE_LIB = HERE / "libk2q_probe.so"

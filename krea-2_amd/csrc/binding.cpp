@@ -49,6 +49,10 @@ struct Api {
   decltype(&k2q_adamw) adamw;
   decltype(&k2q_adamw_ws_bytes) adamw_ws_bytes;
   decltype(&k2q_moments) moments;
+  decltype(&k2q_bank_fwd) bank_fwd;
+  decltype(&k2q_bank_fwd_ws_bytes) bank_fwd_ws_bytes;
+  decltype(&k2q_bank_bwd) bank_bwd;
+  decltype(&k2q_bank_bwd_ws_bytes) bank_bwd_ws_bytes;
 } api{};
 
 PyObject* raw_stream_of = nullptr;   // torch._C._cuda_getCurrentRawStream
@@ -857,6 +861,116 @@ PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// A bank of adapters and the rows that have them.
+struct BankRows {
+  k2q_bank b;
+  int64_t T, per;
+};
+
+// False where the arguments are not what the kernels take.  t: a tensor of the batch, (.., width of which is of no account);
+// ids has its first dimensions.
+bool bank_of(const Tensor* A, const Tensor* B, const Tensor* ids, const Tensor* scales, const Tensor* ranks, double scale,
+             const Tensor& t, BankRows& o) {
+  const c10::Device d = t.device();
+  if (!A || !B || !ids || !ready(d) || A->dim() != 3 || B->dim() != 3) return false;
+  const auto ty = A->scalar_type(), it = ids->scalar_type();
+  const int64_t count = A->size(0), R = A->size(1), K = A->size(2), N = B->size(1), lead = ids->dim();
+  if ((ty != at::kFloat && ty != at::kBFloat16) || !operand(A, ty, 3, d) || !operand(B, ty, 3, d) || B->size(0) != count ||
+      B->size(2) != R || count < 1 || count > K2Q_MAX_ADAPTERS || R < 16 || R % 16 || R > K2Q_MAX_RANK || K % 64 || N % 64 ||
+      K < 64 || N < 64 || K > 1 << 24 || N > 1 << 24)
+    return false;
+  if ((it != at::kInt && it != at::kLong) || ids->device() != d || !ids->is_contiguous() || lead < 1 || lead > t.dim() - 1 ||
+      t.numel() == 0)
+    return false;
+  for (int64_t i = 0; i < lead; ++i)
+    if (ids->size(i) != t.size(i)) return false;
+  if ((scales && (!scales->is_contiguous() || scales->scalar_type() != at::kFloat || scales->numel() != count ||
+                  scales->device() != d)) ||
+      (ranks && (!ranks->is_contiguous() || ranks->scalar_type() != at::kInt || ranks->numel() != count ||
+                 ranks->device() != d)))
+    return false;
+  o.T = t.numel() / t.size(t.dim() - 1);
+  o.per = o.T / ids->numel();
+  if (o.T > 0x7fffff00) return false;
+  o.b = {A->data_ptr(), B->data_ptr(), ids->data_ptr(), as<int32_t>(ptr(ranks)), as<float>(ptr(scales)), (float)scale,
+         it == at::kLong, ty == at::kFloat ? K2Q_DTYPE_F32 : K2Q_DTYPE_BF16, (int32_t)count, (int32_t)R, (int32_t)K,
+         (int32_t)N};
+  return true;
+}
+
+// A contiguous, aligned bf16 tensor of the batch with this width.
+bool batch(const Tensor* t, const Tensor& like, int64_t width) {
+  if (!t || t->scalar_type() != at::kBFloat16 || t->device() != like.device() || !t->is_contiguous() || !aligned(*t) ||
+      t->dim() != like.dim() || t->size(t->dim() - 1) != width)
+    return false;
+  for (int64_t i = 0; i + 1 < t->dim(); ++i)
+    if (t->size(i) != like.size(i)) return false;
+  return true;
+}
+
+// bank_fwd(y, x, A, B, ids, scales | None, ranks | None, scale, need_u) -> (out, u | None)
+PyObject* py_bank_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(9)
+  return guarded([&]() -> PyObject* {
+    const Tensor *y = tensor_of(a[0], bad), *x = tensor_of(a[1], bad), *A = tensor_of(a[2], bad), *B = tensor_of(a[3], bad),
+                 *ids = tensor_of(a[4], bad), *scales = tensor_of(a[5], bad), *ranks = tensor_of(a[6], bad);
+    const double scale = PyFloat_AsDouble(a[7]);
+    const int need_u = PyObject_IsTrue(a[8]);
+    if (PyErr_Occurred()) return nullptr;
+    BankRows r;
+    if (bad || !x || !y || x->dim() < 2 || !bank_of(A, B, ids, scales, ranks, scale, *x, r) || !batch(x, *x, r.b.K) ||
+        !batch(y, *x, r.b.N))
+      K2Q_REFUSE;
+    const c10::Device d = x->device();
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    Tensor out = alloc(y->sizes(), at::kBFloat16, d), u = need_u ? alloc({r.T, r.b.R}, at::kFloat, d) : Tensor();
+    const int64_t nws = api.bank_fwd_ws_bytes(&r.b, r.T, r.per);
+    Tensor ws = workspace(nws, d);
+    const int rc = foreign(api.bank_fwd, static_cast<const k2q_bank*>(&r.b), r.T, r.per, as<uint16_t>(ptr(x)),
+                           as<uint16_t>(ptr(y)), as<uint16_t>(ptr(out)), as<float>(ptr(u)), ptr(ws), nws, st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({out, u});
+  });
+}
+
+// bank_bwd(dy, x | None, u | None, A, B, ids, scales | None, ranks | None, scale, base | None, need_dx, need_dA, need_dB) ->
+// (dx | None, dA | None, dB | None); base: what dx is added to, in place
+PyObject* py_bank_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(13)
+  return guarded([&]() -> PyObject* {
+    const Tensor *dy = tensor_of(a[0], bad), *x = tensor_of(a[1], bad), *u = tensor_of(a[2], bad), *A = tensor_of(a[3], bad),
+                 *B = tensor_of(a[4], bad), *ids = tensor_of(a[5], bad), *scales = tensor_of(a[6], bad),
+                 *ranks = tensor_of(a[7], bad), *base = tensor_of(a[9], bad);
+    const double scale = PyFloat_AsDouble(a[8]);
+    const int need_x = PyObject_IsTrue(a[10]), need_A = PyObject_IsTrue(a[11]), need_B = PyObject_IsTrue(a[12]);
+    if (PyErr_Occurred()) return nullptr;
+    BankRows r;
+    if (bad || !dy || dy->dim() < 2 || !bank_of(A, B, ids, scales, ranks, scale, *dy, r) || !batch(dy, *dy, r.b.N) ||
+        (need_A && !batch(x, *dy, r.b.K)) || (base && !batch(base, *dy, r.b.K)) ||
+        (need_B && !(operand(u, at::kFloat, 2, dy->device()) && u->size(0) == r.T && u->size(1) == r.b.R)) ||
+        !(need_x || need_A || need_B))
+      K2Q_REFUSE;
+    const c10::Device d = dy->device();
+    const c10::DeviceGuard guard(d);
+    void* st;
+    if (!stream_of(d, st)) return nullptr;
+    std::vector<int64_t> shape(dy->sizes().begin(), dy->sizes().end());
+    shape.back() = r.b.K;
+    Tensor dx = need_x ? base ? *base : alloc(shape, at::kBFloat16, d) : Tensor(),
+           dA = need_A ? alloc(A->sizes(), A->scalar_type(), d) : Tensor(),
+           dB = need_B ? alloc(B->sizes(), B->scalar_type(), d) : Tensor();
+    const int64_t nws = api.bank_bwd_ws_bytes(&r.b, r.T, r.per, need_A || need_B);
+    Tensor ws = workspace(nws, d);
+    const int rc = foreign(api.bank_bwd, static_cast<const k2q_bank*>(&r.b), r.T, r.per, as<uint16_t>(ptr(dy)),
+                           as<uint16_t>(need_A ? ptr(x) : nullptr), as<float>(need_B ? ptr(u) : nullptr),
+                           as<uint16_t>(ptr(base)), as<uint16_t>(ptr(dx)), ptr(dA), ptr(dB), ptr(ws), nws, st);
+    if (rc) return PyLong_FromLong(rc);
+    return pack({dx, dA, dB});
+  });
+}
+
 // bind(dict of entry point addresses, raw stream getter)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(2)
@@ -882,7 +996,9 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !get("k2q_rotary", api.rotary) || !get("k2q_capture_id", api.capture_id) ||
       !get("k2q_grad_norm", api.grad_norm) || !get("k2q_grad_norm_ws_bytes", api.grad_norm_ws_bytes) ||
       !get("k2q_scale_grads", api.scale_grads) || !get("k2q_adamw", api.adamw) ||
-      !get("k2q_adamw_ws_bytes", api.adamw_ws_bytes) || !get("k2q_moments", api.moments))
+      !get("k2q_adamw_ws_bytes", api.adamw_ws_bytes) || !get("k2q_moments", api.moments) ||
+      !get("k2q_bank_fwd", api.bank_fwd) || !get("k2q_bank_fwd_ws_bytes", api.bank_fwd_ws_bytes) ||
+      !get("k2q_bank_bwd", api.bank_bwd) || !get("k2q_bank_bwd_ws_bytes", api.bank_bwd_ws_bytes))
     return nullptr;
   Py_INCREF(a[1]);
   Py_XSETREF(raw_stream_of, a[1]);
@@ -916,6 +1032,7 @@ PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2
                          K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         K2Q_METHOD(linear_infer),
                          K2Q_METHOD(capture_id),  K2Q_METHOD(resnorm_stream_bwd),
                          K2Q_METHOD(grad_norm),   K2Q_METHOD(adamw),          K2Q_METHOD(moments),
+                         K2Q_METHOD(bank_fwd),    K2Q_METHOD(bank_bwd),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,758 @@
+// Low-rank adapters of many requests beside one projection: row t of a batch has adapter a = ids[t / per] of a bank of factors
+// A (count x R x K) and B (count x N x R), or none, and
+//   out[t] = y[t] + u[t] B_a^T,  u[t] = s_a x[t] A_a^T              (LoRALinear.forward, reference lora.py:43-48, by row)
+// with the gradients g = s_a dy B_a, dx = g A_a (+ the base's), dA_a = sum_t g[t]^T x[t], dB_a = sum_t dy[t]^T u[t].
+//
+// Two forms of product make all of it.  "Down" reduces wide rows to an adapter's rank (u from x and A, g from dy and B),
+// "up" widens them again and adds (out from u and B, dx from g and A); each takes its factor with the wide index contiguous
+// (A) or the rank contiguous (B).  The third form, "sums", reduces over an adapter's rows (dA from g and x, dB from u and
+// dy).  All run on 16x16x32 bf16 MFMAs with f32 sums: what is in f32 (factors, u, g) goes in as its bf16 rounding and the
+// rounding of the rest, 2^-17 of it, so a product is that of 16 bits of each; y, x, dy are bf16 as they are.
+//
+// Rows may come in any order.  A tile of 64 rows goes over the adapters that it finds in it, one after another: rows of one
+// request lie together, so that is one adapter, or two, in all but the smallest batches.
+#include "k2q_common.h"
+
+namespace {
+
+constexpr int ROWS = 64;              // rows of a tile
+constexpr int THREADS = 256;          // 4 waves
+constexpr int RANKS = 128;            // most ranks that an "up" workgroup holds at once
+
+struct Rows {
+  const void* ids;
+  const int32_t* ranks;     // nullable
+  const float* scales;      // nullable
+  float mul;
+  int32_t wide;             // ids are 64-bit
+  int32_t per;              // rows of an id
+  int32_t T;
+  int32_t count;
+  int32_t R;                // rank of the bank's storage
+};
+
+// The adapter of a row: -1 for none, and for numbers that are no adapter's.
+__device__ __forceinline__ int adapter_of(const Rows& a, int row) {
+  if (row >= a.T) return -2;
+  const int i = row / a.per;
+  const int64_t id = a.wide ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
+  return id < 0 || id >= a.count ? -1 : (int)id;
+}
+
+// Ranks of an adapter that hold something, in whole MFMA tiles.
+__device__ __forceinline__ int rank_of(const Rows& a, int id) {
+  if (id < 0) return 0;
+  if (!a.ranks) return a.R;
+  const int r = (a.ranks[id] + 15) & ~15;
+  return r < 0 ? 0 : r > a.R ? a.R : r;
+}
+
+__device__ __forceinline__ float scale_of(const Rows& a, int id) { return a.scales ? a.mul * a.scales[id] : a.mul; }
+
+// 8 values as bf16 and, where they are f32, the bf16 of what that leaves.
+struct Split {
+  v8bf hi, lo;
+};
+
+__device__ __forceinline__ Split split(const float (&v)[8]) {
+  v4u h, l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    l[i] = pack_bf16x2(v[2 * i] - __uint_as_float(h[i] << 16), v[2 * i + 1] - __uint_as_float(h[i] & 0xffff0000u));
+  }
+  return {__builtin_bit_cast(v8bf, h), __builtin_bit_cast(v8bf, l)};
+}
+
+__device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+template <typename F>
+constexpr bool kF32 = sizeof(F) == 4;
+
+// Fragments of a factor for one MFMA step of 32: Q tiles, a lane's 8 values of the reduction each.
+template <typename F, int Q>
+struct Frag {
+  v8bf hi[Q], lo[Q];      // lo: f32 factors alone
+};
+
+// Reduction contiguous: value e of tile q is p[q * tile + e].
+template <typename F, int Q>
+__device__ __forceinline__ void load_contiguous(const F* p, int64_t tile, const bool (&ok)[Q], Frag<F, Q>& f) {
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    if constexpr (kF32<F>) {
+      v4f a = {0.f, 0.f, 0.f, 0.f}, b = a;
+      if (ok[q]) {
+        a = *reinterpret_cast<const v4f*>(p + q * tile);
+        b = *reinterpret_cast<const v4f*>(p + q * tile + 4);
+      }
+      const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      const Split s = split(v);
+      f.hi[q] = s.hi;
+      f.lo[q] = s.lo;
+    } else {
+      v4u a = {0, 0, 0, 0};
+      if (ok[q]) a = *reinterpret_cast<const v4u*>(p + q * tile);
+      f.hi[q] = __builtin_bit_cast(v8bf, a);
+    }
+  }
+}
+
+// Reduction strided: value e of tile q is p[e * step + q], so that Q tiles come with one vector load a value.
+template <typename F, int Q>
+__device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, Frag<F, Q>& f) {
+  typedef F VecT __attribute__((ext_vector_type(Q > 1 ? Q : 2)));
+  if constexpr (kF32<F>) {
+    float v[Q][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (Q == 1) {
+        v[0][e] = ok ? p[e * step] : 0.f;
+      } else {
+        VecT t = {};
+        if (ok) t = *reinterpret_cast<const VecT*>(p + e * step);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) v[q][e] = t[q];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const Split s = split(v[q]);
+      f.hi[q] = s.hi;
+      f.lo[q] = s.lo;
+    }
+  } else {
+    typedef uint16_t VecU __attribute__((ext_vector_type(Q > 1 ? Q : 2)));
+    uint32_t v[Q][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (Q == 1) {
+        v[0][e] = ok ? reinterpret_cast<const uint16_t*>(p)[e * step] : 0;
+      } else {
+        VecU t = {};
+        if (ok) t = *reinterpret_cast<const VecU*>(reinterpret_cast<const uint16_t*>(p) + e * step);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) v[q][e] = t[q];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      v4u w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = v[q][2 * i] | v[q][2 * i + 1] << 16;
+      f.hi[q] = __builtin_bit_cast(v8bf, w);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Down: part[slice][t][j] = sum over the slice's columns c of x[t][c] F_a[j][c]
+// ---------------------------------------------------------------------------------------------------------------
+// A workgroup: 64 rows, a slice of columns, Q tiles of 16 ranks.  Its waves take 64 columns in turn (a row's 128 bytes of x),
+// all 64 rows and all ranks, so that a factor's fragment serves four MFMAs; their sums meet in LDS.
+template <typename F, bool kWide, int Q>
+__global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
+                                                       int slice_cols, float* part) {
+  constexpr int RS = 16 * Q + 4;        // a row of sums in LDS
+  extern __shared__ float sums[];       // 4 waves x 64 rows x RS
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
+  const int row0 = blockIdx.x * ROWS, j0 = blockIdx.z * 16 * Q;
+  const int begin = blockIdx.y * slice_cols, end = min(C, begin + slice_cols);
+  const int id = adapter_of(rows, row0 + lane);
+  const uint16_t* xr[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) xr[t] = x + (int64_t)min(row0 + 16 * t + m, rows.T - 1) * C + 8 * g;
+  uint64_t left = __ballot(id >= 0);
+  while (left) {
+    const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    const uint64_t mask = __ballot(id == a);
+    left &= ~mask;
+    const int r = rank_of(rows, a);
+    if (j0 >= r) continue;
+    v4f acc[4][Q] = {};
+    bool ok[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) ok[q] = j0 + 16 * q + m < r;
+    const bool some = j0 + Q * m < r;
+    const F* f = factor + a * one;
+    for (int c0 = begin + 64 * wave; c0 < end; c0 += 64 * 4) {
+      v8bf xv[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) xv[h][t] = *reinterpret_cast<const v8bf*>(xr[t] + c0 + 32 * h);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = c0 + 32 * h + 8 * g;
+        Frag<F, Q> fr;
+        if constexpr (kWide) load_contiguous<F, Q>(f + (int64_t)(j0 + m) * C + c, 16 * (int64_t)C, ok, fr);
+        else load_strided<F, Q>(f + (int64_t)c * rows.R + j0 + Q * m, rows.R, some, fr);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            acc[t][q] = mfma(fr.hi[q], xv[h][t], acc[t][q]);
+            if constexpr (kF32<F>) acc[t][q] = mfma(fr.lo[q], xv[h][t], acc[t][q]);
+          }
+      }
+    }
+    // a lane's sums: token 16 t + m, ranks 16 q + 4 g + i, or (strided) Q (4 g + i) + q
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        float* s = sums + (wave * ROWS + 16 * t + m) * RS;
+        if constexpr (kWide) {
+          *reinterpret_cast<v4f*>(s + 16 * q + 4 * g) = acc[t][q];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[Q * (4 * g + i) + q] = acc[t][q][i];
+        }
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * 4 * Q; i += THREADS) {
+      const int row = i / (4 * Q), j = 4 * (i % (4 * Q));
+      if (!(mask >> row & 1) || j0 + j >= r) continue;
+      v4f v = *reinterpret_cast<const v4f*>(sums + row * RS + j);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + (w * ROWS + row) * RS + j);
+      *reinterpret_cast<v4f*>(part + ((int64_t)blockIdx.y * rows.T + row0 + row) * rows.R + j0 + j) = v;
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Up: out[t][c] = y[t][c] + sum_j u[t][j] F_a[j][c],  u = s_a sum over slices of part
+// ---------------------------------------------------------------------------------------------------------------
+// A workgroup: 64 rows, 256 columns at a time.  It adds up the slices once, scaled, and holds u in LDS in two bf16 halves; a
+// wave takes 64 columns of all rows.  The order of a tile's columns among MFMA rows is chosen so that a lane ends with 16
+// columns of a row in two pieces of 8, and 4 lanes with 64 bytes in one: y comes and goes in vectors.
+template <typename F, bool kWide>
+__global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* part, int slices, float* sum, const uint16_t* y,
+                                                     int C, const F* factor, int64_t one, int passes, uint16_t* out) {
+  constexpr int RS = RANKS + 8;         // a row of halves in LDS (bf16): 16 bytes off the banks' turn
+  __shared__ uint16_t hi[ROWS * RS], lo[ROWS * RS];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
+  const int row0 = blockIdx.x * ROWS;
+  const int id = adapter_of(rows, row0 + lane);
+  uint64_t left = __ballot(id >= -1);
+  while (left) {
+    const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    const uint64_t mask = __ballot(id == a);
+    left &= ~mask;
+    const int r = rank_of(rows, a);
+    const float scale = a >= 0 ? scale_of(rows, a) : 0.f;
+    const F* f = factor + (int64_t)max(a, 0) * one;
+    for (int p = 0; p < passes; ++p) {
+      const int c0 = (blockIdx.y * passes + p) * 256 + 64 * wave;
+      const bool in = c0 < C;
+      v4f acc[4][4] = {};
+      for (int j0 = 0; j0 < r; j0 += RANKS) {
+        const int n = min(RANKS, r - j0), n32 = (n + 31) & ~31;
+        if (p == 0 || r > RANKS) {
+          __syncthreads();
+          for (int i = threadIdx.x; i < ROWS * (n32 / 8); i += THREADS) {
+            const int row = i / (n32 / 8), j = 8 * (i % (n32 / 8));
+            float v[8] = {};
+            if ((mask >> row & 1) && j < n) {
+              const int64_t at = (int64_t)(row0 + row) * rows.R + j0 + j;
+              for (int s = 0; s < slices; ++s) {
+                const float* q = part + (int64_t)s * rows.T * rows.R + at;
+                const v4f b = *reinterpret_cast<const v4f*>(q), c = *reinterpret_cast<const v4f*>(q + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  v[e] += b[e];
+                  v[e + 4] += c[e];
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] *= scale;
+              if (sum && blockIdx.y == 0 && p == 0) {
+                *reinterpret_cast<v4f*>(sum + at) = v4f{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<v4f*>(sum + at + 4) = v4f{v[4], v[5], v[6], v[7]};
+              }
+            }
+            const Split s = split(v);
+            *reinterpret_cast<v8bf*>(hi + row * RS + j) = s.hi;
+            *reinterpret_cast<v8bf*>(lo + row * RS + j) = s.lo;
+          }
+          __syncthreads();
+        }
+        if (in) {
+          for (int j = 0; j < n; j += 32) {
+            Frag<F, 4> fr;
+            const bool some = j + 8 * g < n;
+            if constexpr (kWide) {
+              // MFMA row m of tile q is column 8 (m / 4 % ..): a lane loads 4 neighbouring columns, one for each tile
+              const int col = 32 * (m % 4 / 2) + 8 * (m / 4) + 4 * (m % 2);
+              load_strided<F, 4>(f + (int64_t)(j0 + j + 8 * g) * C + c0 + col, C, some, fr);
+            } else {
+              // row m of tile q: column 32 (q / 2) + 8 (m / 4) + 4 (q % 2) + m % 4
+              const bool ok[2] = {some, some};
+              const F* b = f + (int64_t)(c0 + 8 * (m / 4) + m % 4) * rows.R + j0 + j + 8 * g;
+              Frag<F, 2> half[2];
+              load_contiguous<F, 2>(b, 4 * (int64_t)rows.R, ok, half[0]);
+              load_contiguous<F, 2>(b + 32 * (int64_t)rows.R, 4 * (int64_t)rows.R, ok, half[1]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                fr.hi[q] = half[q / 2].hi[q % 2];
+                if constexpr (kF32<F>) fr.lo[q] = half[q / 2].lo[q % 2];
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const v8bf uh = *reinterpret_cast<const v8bf*>(hi + (16 * t + m) * RS + j + 8 * g);
+              const v8bf ul = *reinterpret_cast<const v8bf*>(lo + (16 * t + m) * RS + j + 8 * g);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                acc[t][q] = mfma(fr.hi[q], uh, acc[t][q]);
+                acc[t][q] = mfma(fr.hi[q], ul, acc[t][q]);
+                if constexpr (kF32<F>) acc[t][q] = mfma(fr.lo[q], uh, acc[t][q]);
+              }
+            }
+          }
+        }
+      }
+      if (!in) continue;
+      // a lane: row 16 t + m, columns 32 h + 8 g + e
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (!(mask >> (16 * t + m) & 1)) continue;
+        const int64_t at = (int64_t)(row0 + 16 * t + m) * C + c0 + 8 * g;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          v4u b = {0, 0, 0, 0}, o;
+          if (y) b = *reinterpret_cast<const v4u*>(y + at + 32 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int e = 2 * i + k;      // of 8
+              // strided: tile e % 4 holds column 4 (e / 4) + e % 4 of the piece in its MFMA row 2 h + e / 4
+              const float d = kWide ? acc[t][e % 4][2 * h + e / 4] : acc[t][2 * h + e / 4][e % 4];
+              v[k] = d + (k ? __uint_as_float(b[i] & 0xffff0000u) : __uint_as_float(b[i] << 16));
+            }
+            o[i] = pack_bf16x2(v[0], v[1]);
+          }
+          *reinterpret_cast<v4u*>(out + at + 32 * h) = o;
+        }
+      }
+    }
+  }
+}
+
+// The slices' sums, scaled, where no "up" is wanted.
+__global__ __launch_bounds__(THREADS) void join_kernel(Rows rows, const float* part, int slices, float* sum) {
+  const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
+  const int row = (int)(i / rows.R), j = (int)(i % rows.R);
+  const int a = adapter_of(rows, row);
+  if (a < 0 || j >= rank_of(rows, a)) return;
+  v4f v = *reinterpret_cast<const v4f*>(part + i);
+  for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const v4f*>(part + (int64_t)s * rows.T * rows.R + i);
+  *reinterpret_cast<v4f*>(sum + i) = v * scale_of(rows, a);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Sums over an adapter's rows
+// ---------------------------------------------------------------------------------------------------------------
+// Rows by adapter: the batch's ids sorted (stably), and the pieces of at most `chunk` rows that workgroups take.
+struct Item {
+  int32_t a, begin, end;      // rows begin .. end of the adapter's, in the order of the batch
+  int32_t slot;               // where its partial sums go: -1, the adapter has no other piece
+};
+
+struct Plan {
+  int32_t* head;      // pieces
+  int32_t* start;     // count + 1: an adapter's first place in order
+  int32_t* first;     // count + 1: its first piece
+  int32_t* order;     // ids in the order of their adapters
+  Item* items;
+};
+
+constexpr int PLAN = 1024;            // threads: one an adapter
+
+__device__ __forceinline__ void scan(int32_t* s, int n) {      // inclusive, over PLAN entries
+  for (int d = 1; d < n; d *= 2) {
+    const int v = (int)threadIdx.x >= d ? s[threadIdx.x - d] : 0;
+    __syncthreads();
+    s[threadIdx.x] += v;
+    __syncthreads();
+  }
+}
+
+// One workgroup: every wave counts a run of ids, then places it; no atomics, so the order is the batch's.
+__global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chunk, Plan plan) {
+  extern __shared__ int32_t lds[];      // 16 waves x count, then PLAN
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = rows.count;
+  int32_t* mine = lds + wave * n;
+  int32_t* line = lds + 16 * n;
+  for (int i = threadIdx.x; i < 16 * n; i += PLAN) lds[i] = 0;
+  __syncthreads();
+  const int run = (ids + 15) / 16, begin = min(ids, wave * run), end = min(ids, begin + run);
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i = begin; i < end; i += 64) {
+      const int id = i + lane < end ? adapter_of(rows, (i + lane) * rows.per) : -1;
+      uint64_t left = __ballot(id >= 0);
+      while (left) {
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const uint64_t mask = __ballot(id == a);
+        left &= ~mask;
+        const int at = mine[a];
+        if (pass && id == a) plan.order[at + __popcll(mask & ((uint64_t(1) << lane) - 1))] = i + lane;
+        if (lane == 0) mine[a] = at + __popcll(mask);
+      }
+    }
+    __syncthreads();
+    if (pass) break;
+    const int a = threadIdx.x;
+    int total = 0;
+    if (a < n)
+      for (int w = 0; w < 16; ++w) total += lds[w * n + a];
+    line[a] = total;
+    __syncthreads();
+    scan(line, PLAN);
+    int at = line[a] - total;
+    if (a < n) {
+      plan.start[a] = at;
+      for (int w = 0; w < 16; ++w) {
+        const int c = lds[w * n + a];
+        lds[w * n + a] = at;
+        at += c;
+      }
+    }
+    if (a == n - 1) plan.start[n] = at;
+    const int of = total * rows.per, pieces = (of + chunk - 1) / chunk;
+    __syncthreads();
+    line[a] = pieces;
+    __syncthreads();
+    scan(line, PLAN);
+    const int first = line[a] - pieces, all = line[PLAN - 1];
+    __syncthreads();
+    line[a] = pieces > 1 ? pieces : 0;
+    __syncthreads();
+    scan(line, PLAN);
+    const int slot = line[a] - (pieces > 1 ? pieces : 0);
+    if (a < n) {
+      plan.first[a] = first;
+      for (int p = 0; p < pieces; ++p)
+        plan.items[first + p] = Item{a, p * chunk, min(of, (p + 1) * chunk), pieces > 1 ? slot + p : -1};
+    }
+    if (a == 0) {
+      plan.head[0] = all;
+      plan.first[n] = all;
+    }
+    __syncthreads();
+  }
+}
+
+struct Job {
+  const uint16_t* x;      // T x C
+  const float* p;         // T x R, scaled
+  int C;
+  int blocks;             // of 128 columns
+  int swapped;            // the result is C x R (dB), else R x C (dA)
+  int64_t one;            // R C
+  void* out;
+  float* part;            // slots of R C
+};
+
+constexpr int COLS = 128;
+constexpr int JOBS = 2;
+
+struct Jobs {
+  Job j[JOBS];
+  int32_t blocks;         // of all
+};
+
+// A workgroup: 128 columns of a piece's rows, Q tiles of 16 ranks.  Its waves take 32 rows in turn; both operands come with
+// the wide index contiguous and the rows strided, so a lane loads 8 rows of 8 columns (and of Q ranks) and turns them in
+// registers: each 16-byte load of x serves 8 MFMA tiles.  The waves' sums are added in LDS in their order.
+template <typename F, int Q>
+__global__ __launch_bounds__(THREADS) void sums_kernel(Rows rows, Plan plan, Jobs jobs) {
+  constexpr int RR = 16 * Q;
+  __shared__ float sums[RR * (COLS + 4) > COLS * (RR + 4) ? RR * (COLS + 4) : COLS * (RR + 4)];
+  if ((int)blockIdx.y >= plan.head[0]) return;
+  const Item it = plan.items[blockIdx.y];
+  const int second = (int)blockIdx.x >= jobs.j[0].blocks;
+  const Job job = jobs.j[second];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
+  const int c0 = ((int)blockIdx.x - (second ? jobs.j[0].blocks : 0)) * COLS, j0 = blockIdx.z * RR;
+  const int r = rank_of(rows, it.a), C = job.C;
+  const bool some = j0 + Q * m < r, in = c0 + 8 * m < C;
+  const int32_t* order = plan.order + plan.start[it.a];
+  const uint16_t* x = job.x + c0 + (in ? 8 * m : 0);
+  const float* p = job.p + j0 + (some ? Q * m : 0);
+  typedef float VecT __attribute__((ext_vector_type(Q > 1 ? Q : 2)));
+  v4f acc[8][Q] = {};
+  if (j0 < r)
+    for (int b = it.begin + 32 * wave; b < it.end; b += 32 * 4) {
+      // lane l finds row b + l; past the piece's end the last one, whose factor is zero
+      const int at = min(b + lane % 32, it.end - 1), q = at / rows.per;
+      const int row = order[q] * rows.per + (at - q * rows.per);
+      v4u xv[8];
+      float pv[Q][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t of = __shfl(row, 8 * g + e);
+        xv[e] = *reinterpret_cast<const v4u*>(x + of * C);
+        const bool live = some && b + 8 * g + e < it.end;
+        if constexpr (Q == 1) {
+          pv[0][e] = live ? p[of * rows.R] : 0.f;
+        } else {
+          VecT t = {};
+          if (live) t = *reinterpret_cast<const VecT*>(p + of * rows.R);
+#pragma unroll
+          for (int k = 0; k < Q; ++k) pv[k][e] = t[k];
+        }
+      }
+      Split ps[Q];
+#pragma unroll
+      for (int k = 0; k < Q; ++k) ps[k] = split(pv[k]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v4u w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = __builtin_amdgcn_perm(xv[2 * i + 1][k / 2], xv[2 * i][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
+        const v8bf xf = __builtin_bit_cast(v8bf, w);
+#pragma unroll
+        for (int t = 0; t < Q; ++t) {
+          acc[k][t] = mfma(xf, ps[t].hi, acc[k][t]);
+          acc[k][t] = mfma(xf, ps[t].lo, acc[k][t]);
+        }
+      }
+    }
+  // a lane: columns 8 (4 g + i) + k, ranks Q m + t
+  const int lc = job.swapped ? RR + 4 : 1, lr = job.swapped ? 1 : COLS + 4;
+  for (int w = 0; w < 4; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int t = 0; t < Q; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float* s = sums + (8 * (4 * g + i) + k) * lc + (Q * m + t) * lr;
+            *s = w ? *s + acc[k][t][i] : acc[k][t][i];
+          }
+    }
+    __syncthreads();
+  }
+  // rows of the result of 4 neighbours each
+  const int inner = job.swapped ? RR : COLS, outer = job.swapped ? COLS : RR;
+  const int64_t ld = job.swapped ? rows.R : C;
+  const int64_t at0 = job.swapped ? (int64_t)c0 * rows.R + j0 : (int64_t)j0 * C + c0;
+  const int ends = job.swapped ? min(COLS, C - c0) : min(RR, rows.R - j0);
+  const int ende = job.swapped ? min(RR, rows.R - j0) : min(COLS, C - c0);
+  for (int i = threadIdx.x; i < outer * (inner / 4); i += THREADS) {
+    const int o = i / (inner / 4), e = 4 * (i % (inner / 4));
+    if (o >= ends || e >= ende) continue;
+    const v4f v = *reinterpret_cast<const v4f*>(sums + o * (inner + 4) + e);
+    const int64_t at = at0 + o * ld + e;
+    if (it.slot >= 0) {
+      *reinterpret_cast<v4f*>(job.part + it.slot * job.one + at) = v;
+    } else if constexpr (kF32<F>) {
+      *reinterpret_cast<v4f*>(static_cast<float*>(job.out) + it.a * job.one + at) = v;
+    } else {
+      *reinterpret_cast<v2u*>(static_cast<uint16_t*>(job.out) + it.a * job.one + at) =
+          v2u{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+  }
+}
+
+// What pieces left: the sum of an adapter's in their order, and zeros for an adapter without rows.
+template <typename F>
+__global__ __launch_bounds__(THREADS) void pieces_kernel(Plan plan, Jobs jobs) {
+  const int a = blockIdx.y, second = (int)blockIdx.x >= jobs.j[0].blocks;
+  const Job job = jobs.j[second];
+  const int first = plan.first[a], n = plan.first[a + 1] - first;
+  const int64_t i = ((int64_t)((int)blockIdx.x - (second ? jobs.j[0].blocks : 0)) * THREADS + threadIdx.x) * 4;
+  if (n == 1 || i >= job.one) return;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  if (n) {
+    const float* p = job.part + plan.items[first].slot * job.one + i;
+    v = *reinterpret_cast<const v4f*>(p);
+    for (int s = 1; s < n; ++s) v += *reinterpret_cast<const v4f*>(p + s * job.one);
+  }
+  if constexpr (kF32<F>)
+    *reinterpret_cast<v4f*>(static_cast<float*>(job.out) + a * job.one + i) = v;
+  else
+    *reinterpret_cast<v2u*>(static_cast<uint16_t*>(job.out) + a * job.one + i) =
+        v2u{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------------------------
+int64_t up16(int64_t n) { return (n + 15) & ~int64_t(15); }
+
+int check(const k2q_bank* b, int64_t T, int64_t per) {
+  if (!b || !b->A || !b->B || !k2q_aligned(b->A, 16) || !k2q_aligned(b->B, 16) || b->count < 1 || b->R < 16 || b->R % 16 ||
+      b->K < 64 || b->K % 64 || b->N < 64 || b->N % 64 || (b->dtype != K2Q_DTYPE_BF16 && b->dtype != K2Q_DTYPE_F32) ||
+      !b->ids || !k2q_aligned(b->ids, b->ids64 ? 8 : 4) || !k2q_aligned(b->ranks, 4) || !k2q_aligned(b->scales, 4) || T < 1 ||
+      per < 1 || T % per)
+    return K2Q_EINVAL;
+  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > 0x7fffff00 || b->K > 1 << 24 || b->N > 1 << 24)
+    return K2Q_EUNSUPPORTED;
+  return K2Q_OK;
+}
+
+Rows rows_of(const k2q_bank* b, int64_t T, int64_t per) {
+  return {b->ids, b->ranks, b->scales, b->scale, b->ids64, (int32_t)per, (int32_t)T, b->count, b->R};
+}
+
+int tiles_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+
+// Slices of a "down" over C columns: as many as give every CU four workgroups, of 256 columns or more.
+int down_slices(int64_t T, int64_t C, int64_t R) {
+  const int64_t groups = ((T + ROWS - 1) / ROWS) * ((R + 16 * tiles_of(R) - 1) / (16 * tiles_of(R)));
+  int64_t s = (4 * (int64_t)k2q_cu_count() + groups - 1) / groups;
+  const int64_t most = (C + 255) / 256;
+  s = s > most ? most : s;
+  const int64_t cols = ((C + s - 1) / s + 255) / 256 * 256;
+  return (int)((C + cols - 1) / cols);
+}
+
+template <typename F, bool kWide>
+void launch_down(const Rows& rows, const uint16_t* x, int64_t C, const void* f, int slices, float* part, hipStream_t st) {
+  const int64_t cols = ((C + slices - 1) / slices + 255) / 256 * 256, one = (int64_t)rows.R * C;
+  const int q = tiles_of(rows.R);
+  const dim3 grid((unsigned)((rows.T + ROWS - 1) / ROWS), (unsigned)slices, (unsigned)((rows.R + 16 * q - 1) / (16 * q)));
+  const int lds = 4 * ROWS * (16 * q + 4) * 4;
+  const F* factor = static_cast<const F*>(f);
+  auto go = [&](auto kernel, std::atomic<uint64_t>& once) {
+    (void)k2q_lds_limit_once(kernel, lds, once);
+    hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, st, rows, x, (int)C, factor, one, (int)cols, part);
+  };
+  static std::atomic<uint64_t> once[3];
+  if (q == 1) go(down_kernel<F, kWide, 1>, once[0]);
+  else if (q == 2) go(down_kernel<F, kWide, 2>, once[1]);
+  else go(down_kernel<F, kWide, 4>, once[2]);
+}
+
+template <typename F, bool kWide>
+void launch_up(const Rows& rows, const float* part, int slices, float* sum, const uint16_t* y, int64_t C, const void* f,
+               uint16_t* out, hipStream_t st) {
+  const int64_t tiles = (rows.T + ROWS - 1) / ROWS, blocks = (C + 255) / 256;
+  int64_t passes = tiles * blocks / (4 * (int64_t)k2q_cu_count());
+  passes = passes < 1 ? 1 : passes > 8 ? 8 : passes;
+  const dim3 grid((unsigned)tiles, (unsigned)((blocks + passes - 1) / passes));
+  hipLaunchKernelGGL((up_kernel<F, kWide>), grid, dim3(THREADS), 0, st, rows, part, slices, sum, y, (int)C,
+                     static_cast<const F*>(f), (int64_t)rows.R * C, (int)passes, out);
+}
+
+struct Sums {
+  int64_t chunk, items, slots;
+  int64_t plan_bytes;
+};
+
+// Rows of a piece: all pieces together give every CU four workgroups, and a piece 256 rows or more.
+Sums sums_plan(const k2q_bank* b, int64_t T, int64_t per) {
+  const int64_t blocks = ((b->K + COLS - 1) / COLS + (b->N + COLS - 1) / COLS) * ((b->R + 16 * tiles_of(b->R) - 1) / (16 * tiles_of(b->R)));
+  const int64_t want = (4 * (int64_t)k2q_cu_count() + blocks - 1) / blocks;
+  int64_t chunk = ((T + want - 1) / want + 127) / 128 * 128;
+  chunk = chunk < 256 ? 256 : chunk;
+  const int64_t whole = T / chunk;
+  return {chunk, whole + b->count, 2 * whole, 4 * up16(1 + 2 * (b->count + 1)) + 16 * (whole + b->count) + 4 * up16(T / per)};
+}
+
+}  // namespace
+
+extern "C" int64_t k2q_bank_fwd_ws_bytes(const k2q_bank* b, int64_t T, int64_t per) {
+  if (check(b, T, per) != K2Q_OK) return 0;
+  return (int64_t)down_slices(T, b->K, b->R) * T * b->R * 4;
+}
+
+extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* x, const uint16_t* y, uint16_t* out,
+                            float* u, void* ws, int64_t ws_bytes, void* stream) {
+  const int rc = check(b, T, per);
+  if (rc != K2Q_OK) return rc;
+  if (!x || !out || !ws || !k2q_aligned(x, 16) || !k2q_aligned(y, 16) || !k2q_aligned(out, 16) || !k2q_aligned(u, 16) ||
+      !k2q_aligned(ws, 16) || ws_bytes < k2q_bank_fwd_ws_bytes(b, T, per))
+    return K2Q_EINVAL;
+  const Rows rows = rows_of(b, T, per);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int slices = down_slices(T, b->K, b->R);
+  float* part = static_cast<float*>(ws);
+  if (b->dtype == K2Q_DTYPE_F32) {
+    launch_down<float, true>(rows, x, b->K, b->A, slices, part, st);
+    launch_up<float, false>(rows, part, slices, u, y, b->N, b->B, out, st);
+  } else {
+    launch_down<uint16_t, true>(rows, x, b->K, b->A, slices, part, st);
+    launch_up<uint16_t, false>(rows, part, slices, u, y, b->N, b->B, out, st);
+  }
+  return k2q_launch_status();
+}
+
+extern "C" int64_t k2q_bank_bwd_ws_bytes(const k2q_bank* b, int64_t T, int64_t per, int need_factors) {
+  if (check(b, T, per) != K2Q_OK) return 0;
+  const int64_t down = (int64_t)down_slices(T, b->N, b->R) * T * b->R * 4;
+  if (!need_factors) return down;
+  const Sums s = sums_plan(b, T, per);
+  return down + T * b->R * 4 + s.plan_bytes + s.slots * b->R * (b->K + b->N) * 4;
+}
+
+extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* dy, const uint16_t* x, const float* u,
+                            const uint16_t* base, uint16_t* dx, void* dA, void* dB, void* ws, int64_t ws_bytes, void* stream) {
+  const int rc = check(b, T, per);
+  if (rc != K2Q_OK) return rc;
+  if (!dy || (!dx && !dA && !dB) || (dA && !x) || (dB && !u) || !k2q_aligned(dy, 16) || !k2q_aligned(x, 16) ||
+      !k2q_aligned(u, 16) || !k2q_aligned(base, 16) || !k2q_aligned(dx, 16) || !k2q_aligned(dA, 16) || !k2q_aligned(dB, 16) ||
+      !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_bank_bwd_ws_bytes(b, T, per, dA || dB))
+    return K2Q_EINVAL;
+  const Rows rows = rows_of(b, T, per);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int slices = down_slices(T, b->N, b->R);
+  const bool f32 = b->dtype == K2Q_DTYPE_F32;
+  float* part = static_cast<float*>(ws);
+  float* g = part + slices * T * b->R;
+  if (dx || dA) {
+    if (f32) launch_down<float, false>(rows, dy, b->N, b->B, slices, part, st);
+    else launch_down<uint16_t, false>(rows, dy, b->N, b->B, slices, part, st);
+    if (dx) {
+      if (f32) launch_up<float, true>(rows, part, slices, dA ? g : nullptr, base, b->K, b->A, dx, st);
+      else launch_up<uint16_t, true>(rows, part, slices, dA ? g : nullptr, base, b->K, b->A, dx, st);
+    } else {
+      hipLaunchKernelGGL(join_kernel, dim3((unsigned)((T * b->R / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0, st, rows,
+                         part, slices, g);
+    }
+  }
+  if (!dA && !dB) return k2q_launch_status();
+  const Sums s = sums_plan(b, T, per);
+  const int ids = (int)(T / per), n = b->count;
+  Plan plan;
+  plan.items = reinterpret_cast<Item*>(g + T * b->R);
+  plan.head = reinterpret_cast<int32_t*>(plan.items + s.items);
+  plan.start = plan.head + 1;
+  plan.first = plan.start + n + 1;
+  plan.order = plan.head + up16(1 + 2 * (n + 1));
+  float* pieces = reinterpret_cast<float*>(plan.order + up16(ids));
+  const int lds = (16 * n + PLAN) * 4;
+  static std::atomic<uint64_t> once;
+  int rl = k2q_lds_limit_once(plan_kernel, (16 * K2Q_MAX_ADAPTERS + PLAN) * 4, once);
+  if (rl != K2Q_OK) return rl;
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(PLAN), lds, st, rows, ids, (int)s.chunk, plan);
+  Jobs jobs{};
+  int k = 0;
+  auto job = [&](const uint16_t* t, const float* p, int64_t C, int swapped, void* out) {
+    jobs.j[k] = {t, p, (int)C, (int)((C + COLS - 1) / COLS), swapped, (int64_t)b->R * C, out, pieces};
+    jobs.blocks += jobs.j[k++].blocks;
+    pieces += s.slots * b->R * C;
+  };
+  if (dA) job(x, g, b->K, 0, dA);
+  if (dB) job(dy, u, b->N, 1, dB);
+  const int q = tiles_of(b->R);
+  const dim3 grid((unsigned)jobs.blocks, (unsigned)s.items, (unsigned)((b->R + 16 * q - 1) / (16 * q)));
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, st, rows, plan, jobs); };
+  if (q == 1) f32 ? go(sums_kernel<float, 1>) : go(sums_kernel<uint16_t, 1>);
+  else if (q == 2) f32 ? go(sums_kernel<float, 2>) : go(sums_kernel<uint16_t, 2>);
+  else f32 ? go(sums_kernel<float, 4>) : go(sums_kernel<uint16_t, 4>);
+  for (int i = 0; i < k; ++i) jobs.j[i].blocks = (int)((jobs.j[i].one / 4 + THREADS - 1) / THREADS);
+  jobs.blocks = jobs.j[0].blocks + (k > 1 ? jobs.j[1].blocks : 0);
+  const dim3 rest((unsigned)jobs.blocks, (unsigned)n);
+  if (f32) hipLaunchKernelGGL(pieces_kernel<float>, rest, dim3(THREADS), 0, st, plan, jobs);
+  else hipLaunchKernelGGL(pieces_kernel<uint16_t>, rest, dim3(THREADS), 0, st, plan, jobs);
+  return k2q_launch_status();
+}

@@ -123,8 +123,12 @@ class LoRALinear(nn.Module):
         return y + s * ((x.to(self.lora_A.dtype) @ self.lora_A.t()) @ self.lora_B.t()).to(y.dtype)
 
 
-def _adapters_in(model: nn.Module) -> list[LoRALinear]:
-    return [m for m in model.modules() if isinstance(m, LoRALinear)]
+# the modules whose strength lora_scaled sets (their scale_mul); the bank's module adds its own
+_SCALED: tuple = (LoRALinear,)
+
+
+def _adapters_in(model: nn.Module) -> list[nn.Module]:
+    return [m for m in model.modules() if isinstance(m, _SCALED)]
 
 
 @contextlib.contextmanager
@@ -181,6 +185,10 @@ def inject_lora(dit, rank: int, alpha: float | None = None, *, targets=DEFAULT_T
     layerwise / refiner blocks, plus every linear of ``dit.txtmlp``.  Returns ``{module path: adapter}``;
     raises ``RuntimeError`` when nothing matched.  ``alpha`` defaults to ``rank`` (scale 1)."""
     alpha = float(rank) if alpha is None else alpha
+    return _inject(dit, lambda base: LoRALinear(base, rank, alpha), targets, include_txtfusion, include_txtmlp, "inject_lora")
+
+
+def _inject(dit, make, targets, include_txtfusion: bool, include_txtmlp: bool, caller: str) -> dict:
     dit.requires_grad_(False)
     sites = list(_target_sites("blocks", dit.blocks, targets))
     fusion = getattr(dit, "txtfusion", None) if include_txtfusion else None
@@ -191,10 +199,10 @@ def inject_lora(dit, rank: int, alpha: float | None = None, *, targets=DEFAULT_T
     if txtmlp is not None:
         sites += _module_sites("txtmlp", txtmlp)
     if not sites:
-        raise RuntimeError(f"inject_lora: no linear of {type(dit).__name__} matches the targets {tuple(targets)}")
+        raise RuntimeError(f"{caller}: no linear of {type(dit).__name__} matches the targets {tuple(targets)}")
     adapters = {}
     for site in sites:
-        adapter = LoRALinear(site.base, rank, alpha)
+        adapter = make(site.base)
         setattr(site.owner, site.attr, adapter)
         adapters[site.name] = adapter
     return adapters
@@ -239,6 +247,13 @@ def inject_lora_te(qwen: nn.Module, rank: int, alpha: float | None = None, *, ta
         setattr(site.owner, site.attr, adapter)
         adapters[site.name] = adapter
     return adapters
+
+
+class _Factors:
+    """Two factors, as :func:`save_lora` reads them of an adapter."""
+
+    def __init__(self, lora_A, lora_B):
+        self.lora_A, self.lora_B = lora_A, lora_B
 
 
 def _key(prefix: str, name: str, which: str) -> str:

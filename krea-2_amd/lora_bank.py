@@ -1,0 +1,210 @@
+"""Adapters of many requests over one base: a bank of LoRA factors beside a projection, a row of the batch using the adapter
+that its request names, or none.
+
+:class:`LoRALinear` holds one adapter, whose arithmetic is ``lora.py:43-48`` of the reference.  :class:`LoRABank` holds
+``count`` of them over the same frozen base, so that requests with different adapters run in one batch, and several adapters
+train at once: each gets the gradients of its own rows.  :func:`add_adapters` is the operator behind it.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from . import lora as _lora
+from .lora import DEFAULT_TARGETS
+
+
+class _AddAdaptersFn(torch.autograd.Function):
+    """Backward: ``g = s dy B_a``, ``dx = g A_a``, ``dA_a = sum g^T x`` and ``dB_a = sum dy^T u`` over the adapter's rows.
+    Fixed order of sums, no atomics."""
+
+    @staticmethod
+    def forward(ctx, y, x, A, B, ids, scales, ranks, scale):
+        out, u = _lib.bank_fwd(y, x, A, B, ids, scales, ranks, scale, ctx.needs_input_grad[3])
+        need_A = ctx.needs_input_grad[2]
+        ctx.save_for_backward(x if need_A else None, u, A, B, ids, scales, ranks)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, u, A, B, ids, scales, ranks = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        d = _rows(dy)
+        grads = _lib.bank_bwd(d, x, u, A, B, ids, scales, ranks, ctx.scale, None, *need[1:4]) if any(need[1:4]) else (None,) * 3
+        return (dy if need[0] else None, *grads, None, None, None, None)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous, 16-byte aligned and in bf16 (itself when it is that)."""
+    if t.dtype != torch.bfloat16:
+        t = t.to(torch.bfloat16)
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def add_adapters(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B: torch.Tensor, adapters: torch.Tensor,
+                 scales: torch.Tensor | None = None, ranks: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
+    """``y + s_a (x A_a^T) B_a^T``, the adapter ``a`` of every row from ``adapters``; rows without one (a number outside
+    ``0 .. count - 1``, such as -1) keep ``y``.
+
+    ``x`` (.., in) and ``y`` (.., out) bf16 with the same leading dimensions; ``lora_A`` (count, rank, in) and ``lora_B``
+    (count, out, rank), float32 or bfloat16, the rank a multiple of 16; ``adapters`` int32 or int64, one number for each of
+    ``x``'s first dimension, or first dimensions (a request's rows, or every row), on the device, where nothing waits for it.
+    ``s_a = scale * scales[a]`` (``scales`` float32, default 1).  ``ranks`` (int32): the ranks of each adapter that count; the
+    rest, zeros in a bank whose adapters differ, is not read and gets zero gradients.
+
+    Sums are float32 and ``out`` is rounded once.  Float32 factors (and the sums between the products) enter the matrix
+    units as two bf16 parts, 2^-17 of a value off at most.  Rows may have any order; rows of one adapter that lie together
+    are faster.  Differentiable in ``y``, ``x`` and both factors.  A value that is infinite or NaN spoils its own row, and the
+    gradients of its row's adapter."""
+    if x.dim() < 2 or y.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"y {tuple(y.shape)} and x {tuple(x.shape)} differ in their rows")
+    if any(t is not None and t.requires_grad for t in (scales,)) and torch.is_grad_enabled():
+        raise NotImplementedError("scales get no gradient: detach them")
+    if x.numel() == 0 and x.shape[-1] == lora_A.shape[-1] and y.shape[-1] == lora_B.shape[1]:
+        return y.clone()
+    if x.dtype == y.dtype == torch.bfloat16:
+        x, y = _rows(x), _rows(y)
+    A, B, ids = lora_A.contiguous(), lora_B.contiguous(), adapters.contiguous()
+    if _lib.observed() or torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, A, B)):
+        return _AddAdaptersFn.apply(y, x, A, B, ids, scales, ranks, float(scale))
+    return _lib.bank_fwd(y, x, A, B, ids, scales, ranks, float(scale), False)[0]
+
+
+class LoRABank(nn.Module):
+    """``base(x) + s_a (x A_a^T) B_a^T`` over a bank of ``count`` adapters of up to ``rank`` ranks: ``lora_A`` (count, rank, in),
+    ``lora_B`` (count, out, rank), with the rank rounded up to a multiple of 16 (zero ranks, which training leaves zero).
+    Initialised as ``LoRALinear`` (``lora.py:30-41``): ``A`` kaiming-uniform, ``B`` zeros, ``scale = alpha / rank``.
+
+    Which rows use which adapter comes with the call, or from :func:`lora_requests` around the model's; without either the
+    output is ``base(x)``.  ``scale_mul`` and ``lora_scaled`` act on all adapters."""
+
+    def __init__(self, base: nn.Module, count: int, rank: int, alpha: float | None = None, dtype: torch.dtype = torch.float32):
+        super().__init__()
+        if not 1 <= count <= _lib.MAX_ADAPTERS:
+            raise ValueError(f"{count} adapters: a bank holds 1 to {_lib.MAX_ADAPTERS}")
+        if not 1 <= rank <= _lib.MAX_RANK:
+            raise ValueError(f"LoRA rank must be 1 to {_lib.MAX_RANK}, got {rank}")
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"the factors must be float32 or bfloat16, got {dtype}")
+        K, N = base.in_features, base.out_features
+        if K % _lib.BANK_ALIGN or N % _lib.BANK_ALIGN:
+            raise ValueError(f"a bank needs in/out features that are multiples of {_lib.BANK_ALIGN}, got {K} -> {N}")
+        self.base = base
+        base.requires_grad_(False)
+        self.count, self.rank, self.scale_mul = count, rank, 1.0
+        self.adapters = None
+        home = base.weight.device
+        held = rank + -rank % _lib.RANK_ALIGN
+        self.lora_A = nn.Parameter(torch.zeros(count, held, K, device=home, dtype=dtype))
+        self.lora_B = nn.Parameter(torch.zeros(count, N, held, device=home, dtype=dtype))
+        with torch.no_grad():
+            for A in self.lora_A:
+                nn.init.kaiming_uniform_(A[:rank], a=math.sqrt(5))
+        # the scales as f32 bits: Module.to(dtype) casts floating buffers and leaves integer ones alone
+        scale = torch.full((count,), (rank if alpha is None else alpha) / rank, dtype=torch.float32, device=home)
+        self.register_buffer("scale_bits", scale.view(torch.int32))
+        self.register_buffer("ranks", torch.full((count,), rank, dtype=torch.int32, device=home))
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """Every adapter's ``alpha / rank`` (a view)."""
+        return self.scale_bits.view(torch.float32)
+
+    @torch.no_grad()
+    def set_adapter(self, index: int, A: torch.Tensor, B: torch.Tensor, alpha: float | None = None) -> None:
+        """Put an adapter's factors (rank, in) and (out, rank) in place ``index``; ``alpha`` defaults to their rank."""
+        r = A.shape[0]
+        if not 0 <= index < self.count:
+            raise ValueError(f"adapter {index} of {self.count}")
+        if A.shape != (r, self.lora_A.shape[2]) or B.shape != (self.lora_B.shape[1], r) or not 1 <= r <= self.lora_A.shape[1]:
+            raise ValueError(f"factors {tuple(A.shape)} and {tuple(B.shape)} do not fit a bank of rank {self.lora_A.shape[1]}, "
+                             f"{self.lora_A.shape[2]} -> {self.lora_B.shape[1]}")
+        for held, t in ((self.lora_A[index], A), (self.lora_B[index].t(), B.t())):
+            held[:r].copy_(t)
+            held[r:].zero_()
+        self.scales[index] = (r if alpha is None else alpha) / r
+        self.ranks[index] = r
+
+    def adapter(self, index: int):
+        """``(A, B, alpha)`` of an adapter, without the zero ranks (views; waits for the device)."""
+        if not 0 <= index < self.count:
+            raise ValueError(f"adapter {index} of {self.count}")
+        r = int(self.ranks[index])
+        return self.lora_A[index, :r], self.lora_B[index, :, :r], float(self.scales[index]) * r
+
+    def extra_repr(self) -> str:
+        return f"count={self.count}, rank={self.rank}"
+
+    def forward(self, x: torch.Tensor, adapters: torch.Tensor | None = None) -> torch.Tensor:
+        ids = self.adapters if adapters is None else adapters
+        y = self.base(x)
+        if ids is None or self.scale_mul == 0.0:
+            return y
+        return add_adapters(y, x, self.lora_A, self.lora_B, ids, self.scales, self.ranks, self.scale_mul)
+
+
+_lora._SCALED += (LoRABank,)
+
+
+@contextlib.contextmanager
+def lora_requests(model: nn.Module, adapters: torch.Tensor | None):
+    """Within the ``with`` body the rows of every bank's input in ``model`` use the adapters of ``adapters``: one number for
+    each entry of the input's first dimension (the requests of a batch), or of its first dimensions; None: the base alone."""
+    banks = [m for m in model.modules() if isinstance(m, LoRABank)]
+    saved = [m.adapters for m in banks]
+    for m in banks:
+        m.adapters = adapters
+    try:
+        yield
+    finally:
+        for m, v in zip(banks, saved):
+            m.adapters = v
+
+
+def inject_lora_bank(dit, count: int, rank: int, alpha: float | None = None, *, targets=DEFAULT_TARGETS,
+                     include_txtfusion: bool = False, include_txtmlp: bool = False, dtype: torch.dtype = torch.float32) -> dict:
+    """Freeze ``dit`` and put a :class:`LoRABank` around every linear that :func:`inject_lora` would wrap with these
+    arguments.  The stages outside the blocks are left out by default: their inputs need the batch as their first dimension.
+    Returns ``{module path: bank}``; raises ``RuntimeError`` when nothing matched."""
+    return _lora._inject(dit, lambda base: LoRABank(base, count, rank, alpha, dtype), targets, include_txtfusion,
+                         include_txtmlp, "inject_lora_bank")
+
+
+def load_lora_into(banks: dict, index: int, path: str, *, key_prefix: str = "diffusion_model") -> int:
+    """Load a saved adapter (:func:`save_lora`) into place ``index`` of ``banks``, its scale ``alpha / rank`` from the file's
+    metadata (1 without).  A bank that the file does not name gets no adapter there (zero factors).  Returns how many of the
+    file's adapters have no bank (0: everything loaded)."""
+    from safetensors import safe_open
+
+    with safe_open(path, framework="pt") as f:
+        meta = f.metadata() or {}
+        saved = {k: f.get_tensor(k) for k in f.keys()}
+    names = {k[len(key_prefix) + 1:].rsplit(".lora_", 1)[0] for k in saved if k.startswith(key_prefix + ".")}
+    if not names:
+        raise ValueError(f"{path} holds no adapters under {key_prefix!r}")
+    ratio = float(meta["alpha"]) / float(meta["rank"]) if "alpha" in meta and "rank" in meta else 1.0
+    for name, bank in banks.items():
+        A, B = (saved.get(_lora._key(key_prefix, name, w)) for w in ("A", "B"))
+        if A is None or B is None:
+            A, B = torch.zeros(1, bank.lora_A.shape[2]), torch.zeros(bank.lora_B.shape[1], 1)
+        bank.set_adapter(index, A, B, ratio * A.shape[0])
+    return len(names - set(banks))
+
+
+def save_lora_from(banks: dict, index: int, path: str, *, metadata: dict | None = None,
+                   key_prefix: str = "diffusion_model") -> None:
+    """Write adapter ``index`` of ``banks`` as a file of its own, as :func:`save_lora` writes one.  All banks must hold one rank
+    and one alpha there."""
+    parts = {name: bank.adapter(index) for name, bank in banks.items()}
+    kinds = {(A.shape[0], alpha) for A, _, alpha in parts.values()}
+    if len(kinds) != 1:
+        raise ValueError(f"the banks' ranks and alphas differ at {index}: {sorted(kinds)}")
+    (rank, alpha), = kinds
+    held = {name: _lora._Factors(A, B) for name, (A, B, _) in parts.items()}
+    _lora.save_lora(held, path, rank=rank, alpha=alpha, metadata=metadata, key_prefix=key_prefix)

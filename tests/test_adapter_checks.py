@@ -1,8 +1,10 @@
-"""CPU tests of what the optimizer's step refuses, and of its options and states."""
+"""CPU tests of what the optimizer's step and the banks of adapters refuse, of their options and states, and of what walks a
+model to place banks, files and requests."""
 import ctypes
 
 import pytest
 import torch
+import torch.nn as nn
 
 
 def _p(*shape, dtype=torch.float32, grad=True):
@@ -107,3 +109,149 @@ def test_step_entries_refuse_bad_arguments(k2):
     assert lib.k2q_scale_grads(addr, 2, None, None) == -1
     for args in ((None, a, a, a, 256, 0, a, a), (a, a, a, a, 255, 0, a, a), (a, a, a, a, 256, 2, a, a), (a, a, a, a, 0, 0, a, a)):
         assert lib.k2q_moments(*args, None) == -1
+
+
+def test_bank_entries_refuse_bad_arguments(k2):
+    """The C entries' own checks (addresses that are never read)."""
+    lib, a = k2._lib.load(), 4096
+
+    def bank(**kw):
+        return k2._lib.Bank(**{"A": a, "B": a, "ids": a, "scale": 1.0, "ids64": 1, "dtype": 1, "count": 3, "R": 16, "K": 64, "N": 128,
+                               **kw})
+
+    def fwd(b, T=12, per=4, x=a, y=a, out=a, u=a, ws=a, nws=1 << 30):
+        return lib.k2q_bank_fwd(ctypes.addressof(b), T, per, x, y, out, u, ws, nws, None)
+
+    def bwd(b, T=12, per=4, dy=a, x=a, u=a, base=None, dx=a, dA=a, dB=a, ws=a, nws=1 << 30):
+        return lib.k2q_bank_bwd(ctypes.addressof(b), T, per, dy, x, u, base, dx, dA, dB, ws, nws, None)
+
+    for bad in ({"A": None}, {"B": a + 4}, {"ids": None}, {"ids": a + 4}, {"dtype": 2}, {"count": 0}, {"R": 8}, {"R": 24},
+                {"K": 32}, {"K": 96}, {"N": 0}, {"N": 100}, {"ranks": a + 2}, {"scales": a + 2}):
+        b = bank(**bad)
+        assert fwd(b) == -1 and bwd(b) == -1, bad
+        assert lib.k2q_bank_fwd_ws_bytes(ctypes.addressof(b), 12, 4) == 0
+        assert lib.k2q_bank_bwd_ws_bytes(ctypes.addressof(b), 12, 4, 1) == 0
+    for bad in ({"count": 1025}, {"R": 4112}, {"K": (1 << 24) + 64}):
+        assert fwd(bank(**bad)) == -4 and bwd(bank(**bad)) == -4, bad
+    assert fwd(bank(), T=0x7fffff04, per=4) == -4
+    for bad in ({"T": 0}, {"per": 0}, {"T": 13}, {"ws": None}, {"ws": a + 8}, {"nws": 0}):
+        assert fwd(bank(), **bad) == -1 and bwd(bank(), **bad) == -1, bad
+    for bad in ({"x": None}, {"x": a + 2}, {"y": a + 2}, {"out": None}, {"u": a + 4}):
+        assert fwd(bank(), **bad) == -1, bad
+    for bad in ({"dy": None}, {"dy": a + 2}, {"x": None}, {"u": None}, {"base": a + 2}, {"dA": a + 4},
+                {"dx": None, "dA": None, "dB": None}):
+        assert bwd(bank(), **bad) == -1, bad
+    b = bank()
+    need = lib.k2q_bank_bwd_ws_bytes(ctypes.addressof(b), 12, 4, 1)
+    assert need > lib.k2q_bank_bwd_ws_bytes(ctypes.addressof(b), 12, 4, 0) > 0
+    assert bwd(b, nws=need - 1) == -1
+
+
+def test_add_adapters_refuses(k2):
+    x, y = torch.zeros(2, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 3, 128, dtype=torch.bfloat16)
+    A, B, ids = torch.zeros(4, 16, 64), torch.zeros(4, 128, 16), torch.zeros(2, dtype=torch.int64)
+    f = k2.add_adapters
+    for bad in (lambda: f(y[:1], x, A, B, ids), lambda: f(y, x, A[:3], B, ids), lambda: f(y, x, A, B[..., :8], ids),
+                lambda: f(y, x, A[:, :8], B[..., :8], ids), lambda: f(y, x, A.half(), B.half(), ids),
+                lambda: f(y, x, A, B.bfloat16(), ids), lambda: f(y, x, A, B, ids.float()), lambda: f(y, x, A, B, ids[:1]),
+                lambda: f(y, x, A, B, torch.zeros(2, 3, 64, dtype=torch.int64)), lambda: f(y, x, A, B, ids.sum()),
+                lambda: f(y, x, A, B, ids, torch.zeros(3)), lambda: f(y, x, A, B, ids, ranks=torch.zeros(4)),
+                lambda: f(y, x, A[..., :32], B, ids), lambda: f(y[0, 0], x[0, 0], A, B, ids),
+                lambda: f(y, x[..., :32], A[..., :32], B, ids), lambda: f(y, x, A[0], B[0], ids)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        f(y.float(), x.float(), A, B, ids)
+    with pytest.raises(NotImplementedError):
+        f(y, x, A, B, ids, torch.zeros(4, requires_grad=True))
+    with pytest.raises(RuntimeError):
+        f(y, x, A, B, ids)                  # arguments that fit, on a device that does not
+    assert torch.equal(f(y[:0], x[:0], A, B, ids[:0]), y[:0])
+
+
+@pytest.mark.parametrize("bad", [{"count": 0}, {"count": 1025}, {"rank": 0}, {"rank": 4097}, {"dtype": torch.float16},
+                                 {"base": (96, 128)}, {"base": (128, 96)}])
+def test_bank_refuses(k2, bad):
+    args = {"base": (128, 192), "count": 2, "rank": 16, **bad}
+    base = nn.Linear(*args.pop("base"))
+    with pytest.raises(ValueError):
+        k2.LoRABank(base, **args)
+
+
+class _Block(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.attn, self.mlp = nn.Module(), nn.Module()
+        for n in ("wq", "wo"):
+            setattr(self.attn, n, nn.Linear(64, 128 if n == "wq" else 64, bias=False))
+        self.mlp.up = nn.Linear(64, 64, bias=False)
+
+
+class _Dit(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.blocks = nn.ModuleList(_Block() for _ in range(2))
+        self.txtmlp = nn.Sequential(nn.Linear(64, 64))
+
+
+def test_banks_hold_adapters_of_files(k2, tmp_path):
+    """Adapters saved one by one fill a bank, in their own ranks and scales, and a bank's adapter is a file like any."""
+    files = []
+    for i, (rank, alpha) in enumerate(((4, 8.0), (16, 16.0), (20, 5.0))):
+        dit = _Dit()
+        adapters = k2.inject_lora(dit, rank, alpha, include_txtmlp=i == 1)
+        with torch.no_grad():
+            for m in adapters.values():
+                m.lora_A.copy_(m.lora_A.bfloat16())
+                m.lora_B.copy_(torch.randn(m.lora_B.shape).bfloat16())
+        files.append((str(tmp_path / f"{i}.safetensors"), adapters, rank, alpha))
+        k2.save_lora(adapters, files[-1][0], rank=rank, alpha=alpha)
+    dit = _Dit()
+    banks = k2.inject_lora_bank(dit, 3, 20)
+    assert len(banks) == 6 and all(b.lora_A.shape[:2] == (3, 32) for b in banks.values())
+    assert not any(p.requires_grad for n, p in dit.named_parameters() if "lora_" not in n)
+    for i, (path, adapters, rank, alpha) in enumerate(files):
+        assert k2.load_lora_into(banks, i, path) == (1 if i == 1 else 0)
+        for name, bank in banks.items():
+            A, B, a = bank.adapter(i)
+            assert torch.equal(A, adapters[name].lora_A) and torch.equal(B, adapters[name].lora_B) and abs(a - alpha) < 1e-5
+            assert float(bank.scales[i]) == torch.tensor(alpha / rank)
+            assert not int(bank.lora_A[i, rank:].count_nonzero()) and not int(bank.lora_B[i, :, rank:].count_nonzero())
+    out = str(tmp_path / "out.safetensors")
+    k2.save_lora_from(banks, 2, out, metadata={"step": 3})
+    again = k2.load_lora(_Dit(), out)
+    assert all(torch.equal(again[n].lora_A, files[2][1][n].lora_A) for n in banks)
+    # a file without some of the banks: those have no adapter there
+    part = str(tmp_path / "part.safetensors")
+    k2.save_lora({n: m for n, m in files[0][1].items() if "attn" in n}, part, rank=4, alpha=8.0)
+    assert k2.load_lora_into(banks, 1, part) == 0
+    assert not int(banks["blocks.0.mlp.up"].lora_B[1].count_nonzero())
+    with pytest.raises(ValueError, match="no adapters"):
+        k2.load_lora_into(banks, 0, part, key_prefix="text_encoder")
+    with pytest.raises(ValueError, match="fit a bank"):
+        next(iter(banks.values())).set_adapter(0, torch.zeros(33, 64), torch.zeros(128, 33))
+    for bad in (3, -1):
+        with pytest.raises(ValueError):
+            next(iter(banks.values())).adapter(bad)
+        with pytest.raises(ValueError):
+            k2.load_lora_into(banks, bad, part)
+    with pytest.raises(RuntimeError, match="inject_lora_bank"):
+        k2.inject_lora_bank(_Dit(), 1, 4, targets=("attn.none",))
+
+
+def test_requests_and_scales_reach_every_bank(k2):
+    dit = _Dit()
+    banks = k2.inject_lora_bank(dit, 2, 4)
+    x = torch.randn(3, 5, 64)
+    bank = banks["blocks.1.mlp.up"]
+    assert torch.equal(bank(x), bank.base(x))
+    ids = torch.tensor([0, 1, -1])
+    with pytest.raises(RuntimeError):
+        with k2.lora_requests(dit, ids):
+            assert all(b.adapters is ids for b in banks.values())
+            with k2.lora_disabled(dit):
+                assert torch.equal(bank(x), bank.base(x))
+            bank.base.bfloat16()
+            bank(x.bfloat16())              # there is no kernel off the GPU
+    assert all(b.adapters is None and b.scale_mul == 1.0 for b in banks.values())
+
