@@ -12,6 +12,7 @@
 // Rows may come in any order.  A tile of 64 rows goes over the adapters that it finds in it, one after another: rows of one
 // request lie together, so that is one adapter, or two, in all but the smallest batches.
 #include "k2q_common.h"
+#include "rotation.h"
 
 namespace {
 
@@ -146,7 +147,7 @@ __device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Down: part[slice][t][j] = sum over the slice's columns c of x[t][c] F_a[j][c]
+// Down: part[slice][t][j] = sum over the slice's columns c of x[t][c] F_a[j][c], scaled where one slice is all
 // ---------------------------------------------------------------------------------------------------------------
 // A workgroup: 64 rows, a slice of columns, Q tiles of 16 ranks.  Its waves take 64 columns in turn (a row's 128 bytes of x),
 // all 64 rows and all ranks, so that a factor's fragment serves four MFMAs; their sums meet in LDS.
@@ -169,6 +170,7 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
     left &= ~mask;
     const int r = rank_of(rows, a);
     if (j0 >= r) continue;
+    const float scale = scale_of(rows, a);
     v4f acc[4][Q] = {};
     bool ok[Q];
 #pragma unroll
@@ -216,6 +218,7 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
       v4f v = *reinterpret_cast<const v4f*>(sums + row * RS + j);
 #pragma unroll
       for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + (w * ROWS + row) * RS + j);
+      if (gridDim.y == 1) v *= scale;
       *reinterpret_cast<v4f*>(part + ((int64_t)blockIdx.y * rows.T + row0 + row) * rows.R + j0 + j) = v;
     }
     __syncthreads();
@@ -223,18 +226,21 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Up: out[t][c] = y[t][c] + sum_j u[t][j] F_a[j][c],  u = s_a sum over slices of part
+// Up: out[t][c] = y[t][c] + sum_j u[t][j] F_a[j][c]
 // ---------------------------------------------------------------------------------------------------------------
-// A workgroup: 64 rows, 256 columns at a time.  It adds up the slices once, scaled, and holds u in LDS in two bf16 halves; a
-// wave takes 64 columns of all rows.  The order of a tile's columns among MFMA rows is chosen so that a lane ends with 16
+// A workgroup: 64 rows, 256 columns at a time.  It holds u in LDS in two bf16 halves; a wave takes 64 columns of all rows, and
+// y's vectors are on their way while it computes.  The order of a tile's columns among MFMA rows is chosen so that a lane ends with 16
 // columns of a row in two pieces of 8, and 4 lanes with 64 bytes in one: y comes and goes in vectors.
-template <typename F, bool kWide>
-__global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* part, int slices, float* sum, const uint16_t* y,
-                                                     int C, const F* factor, int64_t one, int passes, uint16_t* out) {
-  constexpr int RS = RANKS + 8;         // a row of halves in LDS (bf16): 16 bytes off the banks' turn
-  __shared__ uint16_t hi[ROWS * RS], lo[ROWS * RS];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
-  const int row0 = blockIdx.x * ROWS;
+template <typename F, bool kWide, int TR>
+__global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, const uint16_t* y, int C, const F* factor,
+                                                     int64_t one, int held, int passes, int groups, int past, uint16_t* out) {
+  constexpr int WC = TR;                // waves side by side: 64 columns each; 4 / WC below one another, 16 TR rows each
+  extern __shared__ uint16_t halves[];  // u in two halves of ROWS x RS
+  const int RS = held + 8;              // 16 bytes off the banks' turn
+  uint16_t *hi = halves, *lo = halves + ROWS * RS;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16, r0 = wave / WC * 16 * TR;
+  // a row's columns on neighbouring workgroups
+  const int row0 = blockIdx.x / groups * ROWS, first = blockIdx.x % groups * passes;
   const int id = adapter_of(rows, row0 + lane);
   uint64_t left = __ballot(id >= -1);
   while (left) {
@@ -242,35 +248,35 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* par
     const uint64_t mask = __ballot(id == a);
     left &= ~mask;
     const int r = rank_of(rows, a);
-    const float scale = a >= 0 ? scale_of(rows, a) : 0.f;
     const F* f = factor + (int64_t)max(a, 0) * one;
     for (int p = 0; p < passes; ++p) {
-      const int c0 = (blockIdx.y * passes + p) * 256 + 64 * wave;
+      const int c0 = ((first + p) * WC + wave % WC) * 64;
       const bool in = c0 < C;
-      v4f acc[4][4] = {};
-      for (int j0 = 0; j0 < r; j0 += RANKS) {
-        const int n = min(RANKS, r - j0), n32 = (n + 31) & ~31;
-        if (p == 0 || r > RANKS) {
+      v4u old[TR][2] = {};
+      if (y && in) {
+#pragma unroll
+        for (int t = 0; t < TR; ++t) {
+          if (!(mask >> (r0 + 16 * t + m) & 1)) continue;
+          const uint16_t* b = y + (int64_t)(row0 + r0 + 16 * t + m) * C + c0 + 8 * g;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) old[t][h] = *reinterpret_cast<const v4u*>(b + 32 * h);
+        }
+      }
+      v4f acc[TR][4] = {};
+      for (int j0 = 0; j0 < r; j0 += held) {
+        const int n = min(held, r - j0), n32 = (n + 31) & ~31;
+        if (p == 0 || r > held) {
           __syncthreads();
           for (int i = threadIdx.x; i < ROWS * (n32 / 8); i += THREADS) {
             const int row = i / (n32 / 8), j = 8 * (i % (n32 / 8));
             float v[8] = {};
             if ((mask >> row & 1) && j < n) {
-              const int64_t at = (int64_t)(row0 + row) * rows.R + j0 + j;
-              for (int s = 0; s < slices; ++s) {
-                const float* q = part + (int64_t)s * rows.T * rows.R + at;
-                const v4f b = *reinterpret_cast<const v4f*>(q), c = *reinterpret_cast<const v4f*>(q + 4);
+              const float* q = u + (int64_t)(row0 + row) * rows.R + j0 + j;
+              const v4f b = *reinterpret_cast<const v4f*>(q), c = *reinterpret_cast<const v4f*>(q + 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  v[e] += b[e];
-                  v[e + 4] += c[e];
-                }
-              }
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] *= scale;
-              if (sum && blockIdx.y == 0 && p == 0) {
-                *reinterpret_cast<v4f*>(sum + at) = v4f{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<v4f*>(sum + at + 4) = v4f{v[4], v[5], v[6], v[7]};
+              for (int e = 0; e < 4; ++e) {
+                v[e] = b[e];
+                v[e + 4] = c[e];
               }
             }
             const Split s = split(v);
@@ -284,7 +290,7 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* par
             Frag<F, 4> fr;
             const bool some = j + 8 * g < n;
             if constexpr (kWide) {
-              // MFMA row m of tile q is column 8 (m / 4 % ..): a lane loads 4 neighbouring columns, one for each tile
+              // MFMA row m of tile q: column 32 (m / 2 % 2) + 8 (m / 4) + 4 (m % 2) + q, four tiles with one load
               const int col = 32 * (m % 4 / 2) + 8 * (m / 4) + 4 * (m % 2);
               load_strided<F, 4>(f + (int64_t)(j0 + j + 8 * g) * C + c0 + col, C, some, fr);
             } else {
@@ -301,9 +307,9 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* par
               }
             }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const v8bf uh = *reinterpret_cast<const v8bf*>(hi + (16 * t + m) * RS + j + 8 * g);
-              const v8bf ul = *reinterpret_cast<const v8bf*>(lo + (16 * t + m) * RS + j + 8 * g);
+            for (int t = 0; t < TR; ++t) {
+              const int at = (r0 + 16 * t + m) * RS + j + 8 * g;
+              const v8bf uh = *reinterpret_cast<const v8bf*>(hi + at), ul = *reinterpret_cast<const v8bf*>(lo + at);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 acc[t][q] = mfma(fr.hi[q], uh, acc[t][q]);
@@ -317,13 +323,13 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* par
       if (!in) continue;
       // a lane: row 16 t + m, columns 32 h + 8 g + e
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (!(mask >> (16 * t + m) & 1)) continue;
-        const int64_t at = (int64_t)(row0 + 16 * t + m) * C + c0 + 8 * g;
+      for (int t = 0; t < TR; ++t) {
+        if (!(mask >> (r0 + 16 * t + m) & 1)) continue;
+        uint16_t* to = out + (int64_t)(row0 + r0 + 16 * t + m) * C + c0 + 8 * g;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          v4u b = {0, 0, 0, 0}, o;
-          if (y) b = *reinterpret_cast<const v4u*>(y + at + 32 * h);
+          const v4u b = old[t][h];
+          v4u o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float v[2];
@@ -336,20 +342,159 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* par
             }
             o[i] = pack_bf16x2(v[0], v[1]);
           }
-          *reinterpret_cast<v4u*>(out + at + 32 * h) = o;
+          if (past) __builtin_nontemporal_store(o, reinterpret_cast<v4u*>(to + 32 * h));
+          else *reinterpret_cast<v4u*>(to + 32 * h) = o;
         }
       }
     }
   }
 }
 
-// The slices' sums, scaled, where no "up" is wanted.
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows
+// ---------------------------------------------------------------------------------------------------------------
+// One row a workgroup: its adapter's factors are read as they lie, once, by vectors, on the vector unit; a row of another
+// request on another workgroup.  Rows that share an adapter read it again from L2.
+template <typename F>
+__device__ __forceinline__ void load8(const F* p, float (&v)[8]) {
+  if constexpr (kF32<F>) {
+    const v4f a = *reinterpret_cast<const v4f*>(p), b = *reinterpret_cast<const v4f*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = a[i];
+      v[4 + i] = b[i];
+    }
+  } else {
+    const v4u w = *reinterpret_cast<const v4u*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+// Workgroups in the order that the hardware deals to its 8 dies, one each in turn: the same part of the columns for all rows
+// goes to one die, row after row, so that rows of one adapter find its factors in that die's L2 (64 rows of 32 adapters: up
+// 23 -> 15 us).  With fewer than 8 parts a row's parts follow each other.
+struct RowPart {
+  int row, part;
+};
+
+__device__ __forceinline__ RowPart row_part(int T, int parts) {
+  const int id = blockIdx.x;
+  if (parts < 8) return {id / parts, id % parts};
+  return {id / 8 % T, id / 8 / T * 8 + id % 8};
+}
+
+int64_t row_parts(int64_t T, int64_t parts) { return T * (parts < 8 ? parts : (parts + 7) / 8 * 8); }
+
+// Down: a wave takes 4 ranks over the slice's columns, a workgroup 16.
+template <typename F>
+__global__ __launch_bounds__(THREADS) void down_row_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
+                                                           int slice_cols, int slices, float* part) {
+  const RowPart at = row_part(rows.T, slices * (rows.R / 16));
+  const int row = at.row, slice = at.part % slices, lane = threadIdx.x % 64;
+  const int j = at.part / slices * 16 + threadIdx.x / 64 * 4;
+  const int a = __builtin_amdgcn_readfirstlane(adapter_of(rows, row));
+  if (j >= rank_of(rows, a)) return;
+  const int begin = slice * slice_cols, end = min(C, begin + slice_cols);
+  const F* f = factor + a * one + (int64_t)j * C;
+  const uint16_t* xr = x + (int64_t)row * C;
+  float acc[4] = {};
+#pragma unroll 2
+  for (int c = begin + 8 * lane; c < end; c += 512) {
+    float xv[8], fv[4][8];
+    load8(xr + c, xv);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load8(f + (int64_t)q * C + c, fv[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[q] = __builtin_fmaf(xv[e], fv[q][e], acc[q]);
+  }
+  v4f sum;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sum[q] = k2q_rot::wave_sum(acc[q]);
+  if (lane == 0) *reinterpret_cast<v4f*>(part + ((int64_t)slice * rows.T + row) * rows.R + j) = sum;
+}
+
+// Up, from B: L lanes share a column's ranks, 16 bytes each, and a wave's 64 columns come in L steps; then every lane has one
+// column's sum.
+template <typename F, int L>
+__global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float* part, int slices, float* sum, const uint16_t* y,
+                                                         int C, const F* factor, int64_t one, uint16_t* out) {
+  constexpr int E = 16 / sizeof(F);
+  extern __shared__ float u[];          // R
+  const RowPart of = row_part(rows.T, (C + THREADS - 1) / THREADS);
+  const int row = of.row, lane = threadIdx.x % 64, sub = E * (lane % L);
+  const int a = __builtin_amdgcn_readfirstlane(adapter_of(rows, row));
+  const int r = rank_of(rows, a);
+  const int c0 = of.part * THREADS + threadIdx.x / 64 * 64, mine = c0 + lane % L * (64 / L) + lane / L;
+  const bool in = c0 < C;
+  // the columns' factors are on their way before u is added up
+  const F* f = factor + max(a, 0) * one + (int64_t)(c0 + lane / L) * rows.R + sub;
+  v4u w[L] = {};
+  auto fetch = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (in && j + sub < r) w[i] = *reinterpret_cast<const v4u*>(f + (int64_t)i * (64 / L) * rows.R + j);
+  };
+  fetch(0);
+  const float base = y && in ? bf16_bits_to_f32(y[(int64_t)row * C + mine]) : 0.f;
+  if (r) {
+    const float scale = scale_of(rows, a);
+    for (int j = threadIdx.x; j < r; j += THREADS) {
+      const float* p = part + (int64_t)row * rows.R + j;
+      float v = *p;
+#pragma unroll 4
+      for (int s = 1; s < slices; ++s) v += p[(int64_t)s * rows.T * rows.R];
+      v *= scale;
+      u[j] = v;
+      if (sum && of.part == 0) sum[(int64_t)row * rows.R + j] = v;
+    }
+    __syncthreads();
+  }
+  if (!in) return;
+  float d[L] = {};
+  for (int j = 0; j < r; j += L * E) {
+    if (j) fetch(j);
+    if (j + sub < r) {
+      float uv[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) uv[e] = u[j + sub + e];
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float v = kF32<F> ? __uint_as_float(w[i][e % 4])
+                                  : e % 2 ? __uint_as_float(w[i][e / 2 % 4] & 0xffff0000u) : __uint_as_float(w[i][e / 2 % 4] << 16);
+          d[i] = __builtin_fmaf(v, uv[e], d[i]);
+        }
+    }
+  }
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    float t = d[i];
+    t += k2q_rot::dpp_f<0xB1>(t);
+    if constexpr (L > 2) t += k2q_rot::dpp_f<0x4E>(t);
+    if constexpr (L > 4) t += k2q_rot::dpp_f<0x141>(t);
+    if constexpr (L > 8) t += k2q_rot::dpp_f<0x140>(t);
+    v = lane % L == i ? t : v;
+  }
+  out[(int64_t)row * C + mine] = (uint16_t)f32_to_bf16_bits(base + v);
+}
+
+// The slices' sums, scaled: once, ahead of an "up" whose workgroups would each add them up (64 x 6 of them read a row's 22
+// slices of 64 ranks in 57 us; added up once, both take 25), or where no "up" is wanted.
 __global__ __launch_bounds__(THREADS) void join_kernel(Rows rows, const float* part, int slices, float* sum) {
   const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
   const int row = (int)(i / rows.R), j = (int)(i % rows.R);
   const int a = adapter_of(rows, row);
   if (a < 0 || j >= rank_of(rows, a)) return;
   v4f v = *reinterpret_cast<const v4f*>(part + i);
+#pragma unroll 4
   for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const v4f*>(part + (int64_t)s * rows.T * rows.R + i);
   *reinterpret_cast<v4f*>(sum + i) = v * scale_of(rows, a);
 }
@@ -372,36 +517,57 @@ struct Plan {
 };
 
 constexpr int PLAN = 1024;            // threads: one an adapter
+constexpr int AHEAD = 16;             // ids of a lane
 
-__device__ __forceinline__ void scan(int32_t* s, int n) {      // inclusive, over PLAN entries
-  for (int d = 1; d < n; d *= 2) {
-    const int v = (int)threadIdx.x >= d ? s[threadIdx.x - d] : 0;
-    __syncthreads();
-    s[threadIdx.x] += v;
-    __syncthreads();
+// Inclusive sums of three values over the workgroup's threads; waves: 3 x 16 in LDS.
+__device__ __forceinline__ void scan(int (&v)[3], int32_t* waves) {
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    for (int d = 1; d < 64; d *= 2) {
+      const int t = __shfl_up(v[k], d);
+      if (lane >= d) v[k] += t;
+    }
+  if (lane == 63)
+    for (int k = 0; k < 3; ++k) waves[16 * k + wave] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    int t = lane < wave ? waves[16 * k + lane] : 0;      // the waves before this one
+#pragma unroll
+    for (int d = 8; d; d /= 2) t += __shfl_xor(t, d);
+    v[k] += __shfl(t, 0);
   }
 }
 
 // One workgroup: every wave counts a run of ids, then places it; no atomics, so the order is the batch's.
 __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chunk, Plan plan) {
-  extern __shared__ int32_t lds[];      // 16 waves x count, then PLAN
+  extern __shared__ int32_t lds[];      // 16 waves x count, then 48
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = rows.count;
   int32_t* mine = lds + wave * n;
-  int32_t* line = lds + 16 * n;
   for (int i = threadIdx.x; i < 16 * n; i += PLAN) lds[i] = 0;
   __syncthreads();
   const int run = (ids + 15) / 16, begin = min(ids, wave * run), end = min(ids, begin + run);
   for (int pass = 0; pass < 2; ++pass) {
-    for (int i = begin; i < end; i += 64) {
-      const int id = i + lane < end ? adapter_of(rows, (i + lane) * rows.per) : -1;
-      uint64_t left = __ballot(id >= 0);
-      while (left) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const uint64_t mask = __ballot(id == a);
-        left &= ~mask;
-        const int at = mine[a];
-        if (pass && id == a) plan.order[at + __popcll(mask & ((uint64_t(1) << lane) - 1))] = i + lane;
-        if (lane == 0) mine[a] = at + __popcll(mask);
+    for (int i0 = begin; i0 < end; i0 += 64 * AHEAD) {
+      int some[AHEAD];        // on their way together
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + 64 * k + lane;
+        some[k] = i < end ? adapter_of(rows, i * rows.per) : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int id = some[k];
+        uint64_t left = __ballot(id >= 0);
+        while (left) {
+          const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+          const uint64_t mask = __ballot(id == a);
+          left &= ~mask;
+          const int at = mine[a];
+          if (pass && id == a) plan.order[at + __popcll(mask & ((uint64_t(1) << lane) - 1))] = i0 + 64 * k + lane;
+          if (lane == 0) mine[a] = at + __popcll(mask);
+        }
       }
     }
     __syncthreads();
@@ -410,10 +576,11 @@ __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chun
     int total = 0;
     if (a < n)
       for (int w = 0; w < 16; ++w) total += lds[w * n + a];
-    line[a] = total;
-    __syncthreads();
-    scan(line, PLAN);
-    int at = line[a] - total;
+    const int of = total * rows.per, pieces = (of + chunk - 1) / chunk, shared = pieces > 1 ? pieces : 0;
+    int sums[3] = {total, pieces, shared};
+    scan(sums, lds + 16 * n);
+    const int first = sums[1] - pieces, slot = sums[2] - shared;
+    int at = sums[0] - total;
     if (a < n) {
       plan.start[a] = at;
       for (int w = 0; w < 16; ++w) {
@@ -422,26 +589,14 @@ __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chun
         at += c;
       }
     }
-    if (a == n - 1) plan.start[n] = at;
-    const int of = total * rows.per, pieces = (of + chunk - 1) / chunk;
-    __syncthreads();
-    line[a] = pieces;
-    __syncthreads();
-    scan(line, PLAN);
-    const int first = line[a] - pieces, all = line[PLAN - 1];
-    __syncthreads();
-    line[a] = pieces > 1 ? pieces : 0;
-    __syncthreads();
-    scan(line, PLAN);
-    const int slot = line[a] - (pieces > 1 ? pieces : 0);
     if (a < n) {
       plan.first[a] = first;
       for (int p = 0; p < pieces; ++p)
         plan.items[first + p] = Item{a, p * chunk, min(of, (p + 1) * chunk), pieces > 1 ? slot + p : -1};
     }
-    if (a == 0) {
-      plan.head[0] = all;
-      plan.first[n] = all;
+    if (a == n - 1) {
+      plan.start[n] = sums[0];
+      plan.head[0] = plan.first[n] = sums[1];
     }
     __syncthreads();
   }
@@ -470,9 +625,10 @@ struct Jobs {
 // the wide index contiguous and the rows strided, so a lane loads 8 rows of 8 columns (and of Q ranks) and turns them in
 // registers: each 16-byte load of x serves 8 MFMA tiles.  The waves' sums are added in LDS in their order.
 template <typename F, int Q>
-__global__ __launch_bounds__(THREADS) void sums_kernel(Rows rows, Plan plan, Jobs jobs) {
+__global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, Jobs jobs) {
   constexpr int RR = 16 * Q;
-  __shared__ float sums[RR * (COLS + 4) > COLS * (RR + 4) ? RR * (COLS + 4) : COLS * (RR + 4)];
+  constexpr int HALF = COLS / 2, PART = RR * HALF + 4 * (RR > HALF ? RR : HALF);
+  extern __shared__ float sums[];       // 4 waves x PART
   if ((int)blockIdx.y >= plan.head[0]) return;
   const Item it = plan.items[blockIdx.y];
   const int second = (int)blockIdx.x >= jobs.j[0].blocks;
@@ -524,41 +680,54 @@ __global__ __launch_bounds__(THREADS) void sums_kernel(Rows rows, Plan plan, Job
         }
       }
     }
-  // a lane: columns 8 (4 g + i) + k, ranks Q m + t
-  const int lc = job.swapped ? RR + 4 : 1, lr = job.swapped ? 1 : COLS + 4;
-  for (int w = 0; w < 4; ++w) {
-    if (wave == w) {
+  // a lane: columns 8 (4 g + i) + k, ranks Q m + t.  Half of the columns (k below 4, then the rest) of all waves meet in LDS,
+  // with the index that the result has inside inside; the sums leave in vectors of 4.
+  const int inner = job.swapped ? RR : HALF, ld = inner + 4;
+  for (int h = 0; h < 2; ++h) {
+    float* s = sums + wave * PART;
+    if (job.swapped) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int t = 0; t < Q; ++t)
+        for (int i = 0; i < 4; ++i) {
+          VecT v;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float* s = sums + (8 * (4 * g + i) + k) * lc + (Q * m + t) * lr;
-            *s = w ? *s + acc[k][t][i] : acc[k][t][i];
-          }
+          for (int t = 0; t < Q; ++t) v[t] = h ? acc[4 + k][t][i] : acc[k][t][i];
+          float* to = s + (4 * (4 * g + i) + k) * ld + Q * m;
+          if constexpr (Q == 1) *to = v[0];
+          else *reinterpret_cast<VecT*>(to) = v;
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < Q; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v4f v;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = h ? acc[4 + k][t][i] : acc[k][t][i];
+          *reinterpret_cast<v4f*>(s + (Q * m + t) * ld + 4 * (4 * g + i)) = v;
+        }
     }
     __syncthreads();
-  }
-  // rows of the result of 4 neighbours each
-  const int inner = job.swapped ? RR : COLS, outer = job.swapped ? COLS : RR;
-  const int64_t ld = job.swapped ? rows.R : C;
-  const int64_t at0 = job.swapped ? (int64_t)c0 * rows.R + j0 : (int64_t)j0 * C + c0;
-  const int ends = job.swapped ? min(COLS, C - c0) : min(RR, rows.R - j0);
-  const int ende = job.swapped ? min(RR, rows.R - j0) : min(COLS, C - c0);
-  for (int i = threadIdx.x; i < outer * (inner / 4); i += THREADS) {
-    const int o = i / (inner / 4), e = 4 * (i % (inner / 4));
-    if (o >= ends || e >= ende) continue;
-    const v4f v = *reinterpret_cast<const v4f*>(sums + o * (inner + 4) + e);
-    const int64_t at = at0 + o * ld + e;
-    if (it.slot >= 0) {
-      *reinterpret_cast<v4f*>(job.part + it.slot * job.one + at) = v;
-    } else if constexpr (kF32<F>) {
-      *reinterpret_cast<v4f*>(static_cast<float*>(job.out) + it.a * job.one + at) = v;
-    } else {
-      *reinterpret_cast<v2u*>(static_cast<uint16_t*>(job.out) + it.a * job.one + at) =
-          v2u{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    for (int i = threadIdx.x; i < RR * HALF / 4; i += THREADS) {
+      const int o = i / (inner / 4), e = 4 * (i % (inner / 4));
+      const int lc = job.swapped ? o : e;
+      const int c = c0 + lc / 4 * 8 + 4 * h + lc % 4, j = j0 + (job.swapped ? e : o);
+      if (c >= C || j >= rows.R) continue;
+      v4f v = *reinterpret_cast<const v4f*>(sums + o * ld + e);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + w * PART + o * ld + e);
+      const int64_t at = job.swapped ? (int64_t)c * rows.R + j : (int64_t)j * C + c;
+      if (it.slot >= 0) {
+        *reinterpret_cast<v4f*>(job.part + it.slot * job.one + at) = v;
+      } else if constexpr (kF32<F>) {
+        *reinterpret_cast<v4f*>(static_cast<float*>(job.out) + it.a * job.one + at) = v;
+      } else {
+        *reinterpret_cast<v2u*>(static_cast<uint16_t*>(job.out) + it.a * job.one + at) =
+            v2u{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -594,7 +763,8 @@ int check(const k2q_bank* b, int64_t T, int64_t per) {
       !b->ids || !k2q_aligned(b->ids, b->ids64 ? 8 : 4) || !k2q_aligned(b->ranks, 4) || !k2q_aligned(b->scales, 4) || T < 1 ||
       per < 1 || T % per)
     return K2Q_EINVAL;
-  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > 0x7fffff00 || b->K > 1 << 24 || b->N > 1 << 24)
+  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > 0x7fffff00 || b->K > 1 << 24 || b->N > 1 << 24 ||
+      T * (b->K > b->N ? b->K : b->N) > (int64_t)1 << 40)      // more than any card holds, and 2^24 workgroups
     return K2Q_EUNSUPPORTED;
   return K2Q_OK;
 }
@@ -632,15 +802,55 @@ void launch_down(const Rows& rows, const uint16_t* x, int64_t C, const void* f, 
   else go(down_kernel<F, kWide, 4>, once[2]);
 }
 
+// past: the output goes past the last-level cache (256 MB), which what the call reads next fills.
 template <typename F, bool kWide>
-void launch_up(const Rows& rows, const float* part, int slices, float* sum, const uint16_t* y, int64_t C, const void* f,
-               uint16_t* out, hipStream_t st) {
-  const int64_t tiles = (rows.T + ROWS - 1) / ROWS, blocks = (C + 255) / 256;
-  int64_t passes = tiles * blocks / (4 * (int64_t)k2q_cu_count());
-  passes = passes < 1 ? 1 : passes > 8 ? 8 : passes;
-  const dim3 grid((unsigned)tiles, (unsigned)((blocks + passes - 1) / passes));
-  hipLaunchKernelGGL((up_kernel<F, kWide>), grid, dim3(THREADS), 0, st, rows, part, slices, sum, y, (int)C,
-                     static_cast<const F*>(f), (int64_t)rows.R * C, (int)passes, out);
+void launch_up(const Rows& rows, const float* u, const uint16_t* y, int64_t C, const void* f, uint16_t* out, bool past,
+               hipStream_t st) {
+  constexpr int TR = kF32<F> && !kWide ? 4 : 2;
+  const int64_t tiles = (rows.T + ROWS - 1) / ROWS, blocks = (C + 64 * TR - 1) / (64 * TR);
+  int64_t passes = tiles * blocks / (6 * (int64_t)k2q_cu_count());
+  passes = passes < 1 ? 1 : passes > 4 ? 4 : passes;
+  const int64_t groups = (blocks + passes - 1) / passes;
+  const int held = rows.R < RANKS ? (rows.R + 31) & ~31 : RANKS;
+  hipLaunchKernelGGL((up_kernel<F, kWide, TR>), dim3((unsigned)(tiles * groups)), dim3(THREADS), 2 * ROWS * (held + 8) * 2,
+                     st, rows, u, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups,
+                     (int)past, out);
+}
+
+void launch_join(const Rows& rows, const float* part, int slices, float* sum, hipStream_t st) {
+  if (slices == 1) return;      // scaled already
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(((int64_t)rows.T * rows.R / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0,
+                     st, rows, part, slices, sum);
+}
+
+constexpr int FEW = 128;
+
+// Few rows: slices that give every CU four workgroups, of 512 columns or more.
+int row_slices(int64_t T, int64_t C, int64_t R) {
+  const int64_t groups = T * (R / 16), most = (C + 511) / 512;
+  int64_t s = (4 * (int64_t)k2q_cu_count() + groups - 1) / groups;
+  s = s > most ? most : s;
+  const int64_t cols = ((C + s - 1) / s + 511) / 512 * 512;
+  return (int)((C + cols - 1) / cols);
+}
+
+template <typename F>
+void launch_rows(const Rows& rows, const uint16_t* x, int64_t K, const void* A, float* part, float* sum, const uint16_t* y,
+                 int64_t N, const void* B, uint16_t* out, hipStream_t st) {
+  const int slices = row_slices(rows.T, K, rows.R);
+  const int64_t cols = ((K + slices - 1) / slices + 511) / 512 * 512;
+  hipLaunchKernelGGL(down_row_kernel<F>, dim3((unsigned)row_parts(rows.T, slices * (rows.R / 16))), dim3(THREADS), 0, st, rows,
+                     x, (int)K, static_cast<const F*>(A), (int64_t)rows.R * K, (int)cols, slices, part);
+  const dim3 grid((unsigned)row_parts(rows.T, (N + THREADS - 1) / THREADS));
+  const int lanes = (int)(rows.R * sizeof(F) / 16);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(THREADS), (size_t)rows.R * 4, st, rows, part, slices, sum, y, (int)N,
+                       static_cast<const F*>(B), (int64_t)rows.R * N, out);
+  };
+  if (lanes <= 2) go(up_row_kernel<F, 2>);
+  else if (lanes <= 4) go(up_row_kernel<F, 4>);
+  else if (lanes <= 8) go(up_row_kernel<F, 8>);
+  else go(up_row_kernel<F, 16>);
 }
 
 struct Sums {
@@ -662,7 +872,7 @@ Sums sums_plan(const k2q_bank* b, int64_t T, int64_t per) {
 
 extern "C" int64_t k2q_bank_fwd_ws_bytes(const k2q_bank* b, int64_t T, int64_t per) {
   if (check(b, T, per) != K2Q_OK) return 0;
-  return (int64_t)down_slices(T, b->K, b->R) * T * b->R * 4;
+  return (int64_t)(T <= FEW ? row_slices(T, b->K, b->R) : down_slices(T, b->K, b->R)) * T * b->R * 4;
 }
 
 extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* x, const uint16_t* y, uint16_t* out,
@@ -674,14 +884,23 @@ extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uin
     return K2Q_EINVAL;
   const Rows rows = rows_of(b, T, per);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int slices = down_slices(T, b->K, b->R);
   float* part = static_cast<float*>(ws);
+  if (T <= FEW) {
+    if (b->dtype == K2Q_DTYPE_F32) launch_rows<float>(rows, x, b->K, b->A, part, u, y, b->N, b->B, out, st);
+    else launch_rows<uint16_t>(rows, x, b->K, b->A, part, u, y, b->N, b->B, out, st);
+    return k2q_launch_status();
+  }
+  const int slices = down_slices(T, b->K, b->R);
+  if (!u) u = part;       // the first slice's place
+  const bool past = T * b->N * 4 > (int64_t)256 << 20;
   if (b->dtype == K2Q_DTYPE_F32) {
-    launch_down<float, true>(rows, x, b->K, b->A, slices, part, st);
-    launch_up<float, false>(rows, part, slices, u, y, b->N, b->B, out, st);
+    launch_down<float, true>(rows, x, b->K, b->A, slices, slices == 1 ? u : part, st);
+    launch_join(rows, part, slices, u, st);
+    launch_up<float, false>(rows, u, y, b->N, b->B, out, past, st);
   } else {
-    launch_down<uint16_t, true>(rows, x, b->K, b->A, slices, part, st);
-    launch_up<uint16_t, false>(rows, part, slices, u, y, b->N, b->B, out, st);
+    launch_down<uint16_t, true>(rows, x, b->K, b->A, slices, slices == 1 ? u : part, st);
+    launch_join(rows, part, slices, u, st);
+    launch_up<uint16_t, false>(rows, u, y, b->N, b->B, out, past, st);
   }
   return k2q_launch_status();
 }
@@ -707,19 +926,21 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   const int slices = down_slices(T, b->N, b->R);
   const bool f32 = b->dtype == K2Q_DTYPE_F32;
   float* part = static_cast<float*>(ws);
-  float* g = part + slices * T * b->R;
+  float* g = dA || dB ? part + slices * T * b->R : part;
   if (dx || dA) {
-    if (f32) launch_down<float, false>(rows, dy, b->N, b->B, slices, part, st);
-    else launch_down<uint16_t, false>(rows, dy, b->N, b->B, slices, part, st);
-    if (dx) {
-      if (f32) launch_up<float, true>(rows, part, slices, dA ? g : nullptr, base, b->K, b->A, dx, st);
-      else launch_up<uint16_t, true>(rows, part, slices, dA ? g : nullptr, base, b->K, b->A, dx, st);
-    } else {
-      hipLaunchKernelGGL(join_kernel, dim3((unsigned)((T * b->R / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0, st, rows,
-                         part, slices, g);
-    }
+    if (f32) launch_down<float, false>(rows, dy, b->N, b->B, slices, slices == 1 ? g : part, st);
+    else launch_down<uint16_t, false>(rows, dy, b->N, b->B, slices, slices == 1 ? g : part, st);
+    launch_join(rows, part, slices, g, st);
   }
-  if (!dA && !dB) return k2q_launch_status();
+  // dx last: dy is still in the last-level cache for dB, and what dx would push out of it is read no more
+  auto input = [&] {
+    if (!dx) return k2q_launch_status();
+    const bool past = T * (2 * b->K + b->N) * 2 > (int64_t)256 << 20;
+    if (f32) launch_up<float, true>(rows, g, base, b->K, b->A, dx, past, st);
+    else launch_up<uint16_t, true>(rows, g, base, b->K, b->A, dx, past, st);
+    return k2q_launch_status();
+  };
+  if (!dA && !dB) return input();
   const Sums s = sums_plan(b, T, per);
   const int ids = (int)(T / per), n = b->count;
   Plan plan;
@@ -729,9 +950,9 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   plan.first = plan.start + n + 1;
   plan.order = plan.head + up16(1 + 2 * (n + 1));
   float* pieces = reinterpret_cast<float*>(plan.order + up16(ids));
-  const int lds = (16 * n + PLAN) * 4;
+  const int lds = (16 * n + 48) * 4;
   static std::atomic<uint64_t> once;
-  int rl = k2q_lds_limit_once(plan_kernel, (16 * K2Q_MAX_ADAPTERS + PLAN) * 4, once);
+  int rl = k2q_lds_limit_once(plan_kernel, (16 * K2Q_MAX_ADAPTERS + 48) * 4, once);
   if (rl != K2Q_OK) return rl;
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(PLAN), lds, st, rows, ids, (int)s.chunk, plan);
   Jobs jobs{};
@@ -741,18 +962,25 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
     jobs.blocks += jobs.j[k++].blocks;
     pieces += s.slots * b->R * C;
   };
-  if (dA) job(x, g, b->K, 0, dA);
   if (dB) job(dy, u, b->N, 1, dB);
+  if (dA) job(x, g, b->K, 0, dA);
   const int q = tiles_of(b->R);
   const dim3 grid((unsigned)jobs.blocks, (unsigned)s.items, (unsigned)((b->R + 16 * q - 1) / (16 * q)));
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, st, rows, plan, jobs); };
-  if (q == 1) f32 ? go(sums_kernel<float, 1>) : go(sums_kernel<uint16_t, 1>);
-  else if (q == 2) f32 ? go(sums_kernel<float, 2>) : go(sums_kernel<uint16_t, 2>);
-  else f32 ? go(sums_kernel<float, 4>) : go(sums_kernel<uint16_t, 4>);
+  const int sums_lds = 4 * (16 * q * (COLS / 2) + 4 * (16 * q > COLS / 2 ? 16 * q : COLS / 2)) * 4;
+  static std::atomic<uint64_t> sums_once[6];
+  int sl = K2Q_OK;
+  auto go = [&](auto kernel, int i) {
+    sl = k2q_lds_limit_once(kernel, sums_lds, sums_once[i]);
+    if (sl == K2Q_OK) hipLaunchKernelGGL(kernel, grid, dim3(THREADS), sums_lds, st, rows, plan, jobs);
+  };
+  if (q == 1) f32 ? go(sums_kernel<float, 1>, 0) : go(sums_kernel<uint16_t, 1>, 1);
+  else if (q == 2) f32 ? go(sums_kernel<float, 2>, 2) : go(sums_kernel<uint16_t, 2>, 3);
+  else f32 ? go(sums_kernel<float, 4>, 4) : go(sums_kernel<uint16_t, 4>, 5);
+  if (sl != K2Q_OK) return sl;
   for (int i = 0; i < k; ++i) jobs.j[i].blocks = (int)((jobs.j[i].one / 4 + THREADS - 1) / THREADS);
   jobs.blocks = jobs.j[0].blocks + (k > 1 ? jobs.j[1].blocks : 0);
   const dim3 rest((unsigned)jobs.blocks, (unsigned)n);
   if (f32) hipLaunchKernelGGL(pieces_kernel<float>, rest, dim3(THREADS), 0, st, plan, jobs);
   else hipLaunchKernelGGL(pieces_kernel<uint16_t>, rest, dim3(THREADS), 0, st, plan, jobs);
-  return k2q_launch_status();
+  return input();
 }
