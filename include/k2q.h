@@ -432,11 +432,13 @@ int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* dy, 
  * torch's clip_grad_norm_ and AdamW, train_t2i_lora_cached.py:329-332).  t: host array, count tensors of n contiguous elements
  * of type dtype (bf16, f32, f16), g their gradients in the same type; read before the call returns.
  * k2q_grad_norm: out[0] = the 2-norm over all gradients (sums in f64, in a fixed order), out[1] = min(1, max_norm /
- * (norm + 1e-6)).  k2q_scale_grads: every gradient times by[0], rounded once.
- * k2q_adamw: steps[index] += 1 (= T), and with g the gradient times norm[1] where norm is given,
+ * (norm + 1e-6)); ws holds the partial sums of squares, k2q_grad_norm_ws_bytes / 8 of them, and with out NULL that is all.
+ * k2q_scale_grads: every gradient times by[0], rounded once.
+ * k2q_adamw: steps[index] += 1 (= T), and with g the gradient, times the factor of the norm that n_squares partial sums
+ * (nullable: no factor) give with max_norm, both written to norm[0] and norm[1],
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^T) m / (sqrt(v) / sqrt(1 - beta2^T) + eps)
- * in f32.  lr_of (nullable): the learning rate in device memory, in place of lr.  A norm[0] that is not finite: nothing
+ * in f32.  lr_of (nullable): the learning rate in device memory, in place of lr.  A norm that is not finite: nothing else
  * changes.  p is rounded to its type to nearest; stochastic != 0 rounds bf16 (not f16) at random: 16 random bits are added
  * below the kept ones and the rest is cut off.
  * m and v of a tensor begin at element `at` (a multiple of K2Q_MOMENT_BLOCK) of exp_avg and exp_avg_sq and reach to the end
@@ -463,7 +465,8 @@ int k2q_scale_grads(const k2q_step_tensor* t, int64_t count, const float* by, vo
 int64_t k2q_adamw_ws_bytes(int64_t count);
 int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits, void* exp_avg, void* exp_avg_sq, float* avg_scale,
               float* sq_scale, float* steps, double lr, const float* lr_of, double beta1, double beta2, double eps,
-              double weight_decay, const float* norm, int stochastic, uint32_t seed, void* ws, int64_t ws_bytes, void* stream);
+              double weight_decay, const double* squares, int64_t n_squares, double max_norm, float* norm, int stochastic,
+              uint32_t seed, void* ws, int64_t ws_bytes, void* stream);
 int k2q_moments(const uint8_t* avg, const float* avg_scale, const uint8_t* sq, const float* sq_scale, int64_t n, int dtype,
                 void* m, void* v, void* stream);
 

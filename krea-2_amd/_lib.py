@@ -139,8 +139,8 @@ _SIGNATURES = {
     "k2q_grad_norm": ([_p, _i64, _f64, _p, _i64, _p, _p], _int),
     "k2q_scale_grads": ([_p, _i64, _p, _p], _int),
     "k2q_adamw_ws_bytes": ([_i64], _i64),
-    "k2q_adamw": ([_p, _i64, _int, _p, _p, _p, _p, _p, _f64, _p, _f64, _f64, _f64, _f64, _p, _int, ctypes.c_uint32, _p, _i64,
-                   _p], _int),
+    "k2q_adamw": ([_p, _i64, _int, _p, _p, _p, _p, _p, _f64, _p, _f64, _f64, _f64, _f64, _p, _i64, _f64, _p, _int,
+                   ctypes.c_uint32, _p, _i64, _p], _int),
     "k2q_moments": ([_p, _p, _p, _p, _i64, _int, _p, _p, _p], _int),
     "k2q_gemm_dx_grouped_ws": ([_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p], _int),
 }
@@ -1448,8 +1448,8 @@ def _check_gradients(params, in_place: bool) -> None:
 
 
 def grad_norm(params: list, max_norm: float, scale: bool):
-    """``{norm, factor}`` of the parameters' gradients (``k2q_grad_norm``), which ``scale`` multiplies by the factor in
-    place; None where none has a gradient."""
+    """``{norm, factor}`` of the parameters' gradients (``k2q_grad_norm``), which are multiplied by the factor in place; with
+    ``scale`` false the partial sums of squares for :func:`adamw`.  None where none has a gradient."""
     call = lambda: _native.grad_norm(params, max_norm, scale)   # noqa: E731
     r = _fast().grad_norm(params, max_norm, scale)
     if r.__class__ is not tuple:
@@ -1478,11 +1478,12 @@ def _check_adamw(params, starts, exp_avg, steps, stochastic) -> None:
 
 
 def adamw(params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale, sq_scale, steps, lr, lr_of, beta1, beta2, eps,
-          weight_decay, norm, stochastic, seed) -> None:
+          weight_decay, squares, max_norm, norm, stochastic, seed) -> None:
     """A step (``k2q_adamw``) of the parameters that have a gradient; ``starts`` are the places of all of them in the
-    moments' flat buffers."""
+    moments' flat buffers.  With ``squares`` (:func:`grad_norm`'s) gradients are brought to ``max_norm`` at most, and ``norm``
+    receives the norm and the factor."""
     args = (params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale, sq_scale, steps, lr, lr_of, beta1, beta2, eps,
-            weight_decay, norm, stochastic, seed)
+            weight_decay, squares, max_norm, norm, stochastic, seed)
     r = _fast().adamw(*args)
     if r.__class__ is not tuple:
         _refused(r, "k2q_adamw", lambda: _native.adamw(*args),

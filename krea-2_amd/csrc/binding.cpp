@@ -753,8 +753,8 @@ bool each_of(PyObject* list, F&& f) {
 
 void changed(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
-// grad_norm(params, max_norm, scale) -> (out,): {norm, factor} of the parameters' gradients, which `scale` multiplies by the
-// factor; () where none has a gradient
+// grad_norm(params, max_norm, scale) -> (out,): {norm, factor} of the parameters' gradients, which are multiplied by the
+// factor; with scale false the partial sums of squares that adamw takes; () where none has a gradient
 PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(3)
   return guarded([&]() -> PyObject* {
@@ -768,30 +768,32 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st;
     if (!stream_of(s.device, st)) return nullptr;
     const int64_t count = (int64_t)s.t.size(), nws = api.grad_norm_ws_bytes(s.t.data(), count);
-    Tensor out = alloc({2}, at::kFloat, s.device), ws = workspace(nws, s.device);
+    Tensor out = scale ? alloc({2}, at::kFloat, s.device) : Tensor(), ws = alloc({nws / 8}, at::kDouble, s.device);
     int rc = foreign(api.grad_norm, s.t.data(), count, most, ptr(ws), nws, as<float>(ptr(out)), st);
     if (!rc && scale) {
       rc = foreign(api.scale_grads, s.t.data(), count, as<float>(ptr(out)) + 1, st);
       for (const Tensor& g : s.grads) changed(g);
     }
     if (rc) return PyLong_FromLong(rc);
-    return pack({out});
+    return pack({scale ? out : ws});
   });
 }
 
 // adamw(params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale | None, sq_scale | None, steps, lr, lr_of | None, beta1,
-// beta2, eps, weight_decay, norm | None, stochastic, seed) -> (): a step of the parameters that have a gradient; starts: their
-// places in the moments' buffers
+// beta2, eps, weight_decay, squares | None, max_norm, norm | None, stochastic, seed) -> (): a step of the parameters that have
+// a gradient; starts: their places in the moments' buffers
 PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  K2Q_ARGS(17)
+  K2Q_ARGS(19)
   return guarded([&]() -> PyObject* {
     const Tensor *m = tensor_of(a[3], bad), *v = tensor_of(a[4], bad), *ms = tensor_of(a[5], bad), *vs = tensor_of(a[6], bad),
-                 *steps = tensor_of(a[7], bad), *lr_of = tensor_of(a[9], bad), *norm = tensor_of(a[14], bad);
+                 *steps = tensor_of(a[7], bad), *lr_of = tensor_of(a[9], bad), *squares = tensor_of(a[14], bad),
+                 *norm = tensor_of(a[16], bad);
     const long bits = PyLong_AsLong(a[2]);
     const double lr = PyFloat_AsDouble(a[8]), beta1 = PyFloat_AsDouble(a[10]), beta2 = PyFloat_AsDouble(a[11]),
-                 eps = PyFloat_AsDouble(a[12]), decay = PyFloat_AsDouble(a[13]);
-    const int stochastic = PyObject_IsTrue(a[15]);
-    const unsigned long seed = PyLong_AsUnsignedLong(a[16]);
+                 eps = PyFloat_AsDouble(a[12]), decay = PyFloat_AsDouble(a[13]),
+                 most = PyFloat_AsDouble(a[15]);
+    const int stochastic = PyObject_IsTrue(a[17]);
+    const unsigned long seed = PyLong_AsUnsignedLong(a[18]);
     if (PyErr_Occurred()) return nullptr;
     if (bad || !m || !v || !steps || !PyList_Check(a[1]) || (bits == 8) != (ms && vs)) K2Q_REFUSE;
     const c10::Device d = m->device();
@@ -803,7 +805,7 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !held(m, bits == 8 ? at::kFloat8_e4m3fn : at::kFloat, size) || !held(v, bits == 8 ? at::kByte : at::kFloat, size) ||
         (bits == 8 && (!held(ms, at::kFloat, size / K2Q_MOMENT_BLOCK) || !held(vs, at::kFloat, size / K2Q_MOMENT_BLOCK))) ||
         (lr_of && (lr_of->scalar_type() != at::kFloat || lr_of->numel() != 1 || lr_of->device() != d)) ||
-        (norm && !(norm->scalar_type() == at::kFloat && norm->numel() == 2 && norm->device() == d)))
+        (squares && (!operand(squares, at::kDouble, 1, d) || !operand(norm, at::kFloat, 1, d) || norm->numel() != 2)))
       K2Q_REFUSE;
     Stepped s;
     const bool fits = each_of(a[0], [&](const Tensor& p, int64_t i) {
@@ -827,7 +829,8 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor ws = workspace(nws, d);
     const int rc = foreign(api.adamw, s.t.data(), count, (int)bits, m->data_ptr(), v->data_ptr(), as<float>(ptr(ms)),
                            as<float>(ptr(vs)), as<float>(ptr(steps)), lr, as<float>(ptr(lr_of)), beta1, beta2, eps, decay,
-                           as<float>(ptr(norm)), stochastic, (uint32_t)seed, ptr(ws), nws, st);
+                           as<double>(ptr(squares)), squares ? squares->numel() : 0, most, as<float>(ptr(norm)), stochastic,
+                           (uint32_t)seed, ptr(ws), nws, st);
     if (rc) return PyLong_FromLong(rc);
     for (const Tensor& p : s.params) changed(p);
     for (const Tensor* t : {m, v, ms, vs, steps})

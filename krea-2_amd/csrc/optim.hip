@@ -4,17 +4,22 @@
 //
 // A launch takes up to TENSORS tensors by value, in its argument block: pointers move from step to step (autograd allocates
 // gradients anew), and nothing has to be copied to the device or kept there.  A workgroup finds its tensor by bisecting the
-// workgroups' prefix sums, on the scalar unit.
+// workgroups' prefix sums, on the scalar unit.  A list of a few tensors goes in a block of FEW, which the host writes faster.
 #include <math.h>
+
+#include <type_traits>
 
 #include "k2q_common.h"
 #include "rotation.h"
 
 namespace {
 
-constexpr int TENSORS = 64;           // 40 bytes each: 2.8 KB of arguments
+constexpr int TENSORS = 64;           // 40 bytes each and 4: 2.8 KB of arguments
+constexpr int FEW = 8;
 constexpr int THREADS = 256;
 constexpr int BLOCK = K2Q_MOMENT_BLOCK;
+
+constexpr int64_t CHUNK = 8192;       // most elements of a step's workgroup
 
 struct Item {
   void* p;
@@ -25,63 +30,67 @@ struct Item {
   int32_t vec;        // p and g take vector loads
 };
 
+template <int N>
 struct Table {
-  Item t[TENSORS];
-  uint32_t first[TENSORS];    // a tensor's first workgroup
+  Item t[N];
+  uint32_t first[N];          // a tensor's first workgroup
   int32_t count;
   uint32_t blocks;
 };
 
-__device__ __forceinline__ int tensor_of(const Table& a, uint32_t wg) {
+template <int N>
+__device__ __forceinline__ int tensor_of(const Table<N>& a, uint32_t wg) {
   int lo = 0;
 #pragma unroll
-  for (int s = TENSORS / 2; s; s >>= 1)
+  for (int s = N / 2; s; s >>= 1)
     if (lo + s < a.count && a.first[lo + s] <= wg) lo += s;
   return lo;
 }
 
-// V values of a tensor from element e on; what lies past its end reads as zero and is not written.
-template <int V>
-__device__ __forceinline__ void load(const float* p, int64_t e, int64_t n, bool vec, float (&v)[V]) {
-  if (vec && e + V <= n) {
+// V values of a tensor from element e on.  kWhole: all of them are the tensor's, and vectors are aligned, so that the loads of
+// several turns of a loop leave together; else what lies past its end reads as zero and is not written.
+template <bool kWhole, int V, typename T>
+__device__ __forceinline__ void load(const T* p, int64_t e, int64_t n, float (&v)[V]) {
+  typedef T VecT __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const v4f q = *reinterpret_cast<const v4f*>(p + e + i);
+  for (int i = 0; i < V; i += 4) {
+    VecT q;
+    if constexpr (kWhole) {
+      q = *reinterpret_cast<const VecT*>(p + e + i);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i + j] = q[j];
+      for (int j = 0; j < 4; ++j) q[j] = e + i + j < n ? p[e + i + j] : (T)0.f;
     }
-  } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = e + i < n ? p[e + i] : 0.f;
+    for (int j = 0; j < 4; ++j) v[i + j] = (float)q[j];
   }
 }
 
-template <int V, typename T>
-__device__ __forceinline__ void load(const T* p, int64_t e, int64_t n, bool vec, float (&v)[V]) {
+template <bool kWhole, int V, typename T>
+__device__ __forceinline__ void store(T* p, int64_t e, int64_t n, const T (&v)[V]) {
   typedef T VecT __attribute__((ext_vector_type(4)));
-  if (vec && e + V <= n) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const VecT q = *reinterpret_cast<const VecT*>(p + e + i);
+  for (int i = 0; i < V; i += 4) {
+    if constexpr (kWhole) {
+      *reinterpret_cast<VecT*>(p + e + i) = VecT{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i + j] = (float)q[j];
+      for (int j = 0; j < 4; ++j)
+        if (e + i + j < n) p[e + i + j] = v[i + j];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = e + i < n ? (float)p[e + i] : 0.f;
   }
 }
 
-template <int V, typename T>
-__device__ __forceinline__ void store(T* p, int64_t e, int64_t n, bool vec, const T (&v)[V]) {
-  typedef T VecT __attribute__((ext_vector_type(4)));
-  if (vec && e + V <= n) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) *reinterpret_cast<VecT*>(p + e + i) = VecT{v[i], v[i + 1], v[i + 2], v[i + 3]};
+// f(e, whole) for a workgroup's vectors of V elements; whole: a std::bool_constant, as above.
+template <int V, class F>
+__device__ __forceinline__ void each_vector(const Item& it, int64_t begin, int64_t end, F&& f) {
+  const bool whole = it.vec && end <= it.n && (end - begin) % (THREADS * V) == 0;
+  if (whole) {
+    const int turns = (int)((end - begin) / (THREADS * V));       // a chunk is whole turns
+#pragma unroll 4
+    for (int i = 0; i < turns; ++i) f(begin + i * (THREADS * V) + threadIdx.x * V, std::true_type{});
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (e + i < n) p[e + i] = v[i];
+    for (int64_t e = begin + threadIdx.x * V; e < end; e += THREADS * V) f(e, std::false_type{});
   }
 }
 
@@ -96,8 +105,8 @@ __device__ __forceinline__ double wave_add(double v) {
 
 // Sums of squares of runs of `chunk` elements, one a workgroup.  The sums are in 64 bits: squares of 32-bit values neither
 // overflow nor vanish there, and the card adds them at half the 32-bit rate, ten times what the reads need.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void sumsq_kernel(Table a, int64_t chunk, double* part) {
+template <typename T, int N>
+__global__ __launch_bounds__(THREADS) void sumsq_kernel(Table<N> a, int64_t chunk, double* part) {
   __shared__ double sums[THREADS / 64];
   const int i = tensor_of(a, blockIdx.x);
   const Item& it = a.t[i];
@@ -105,52 +114,63 @@ __global__ __launch_bounds__(THREADS) void sumsq_kernel(Table a, int64_t chunk, 
   const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
   double s = 0;
-#pragma unroll 4
-  for (int64_t e = begin + threadIdx.x * 4; e < end; e += THREADS * 4) {
+  each_vector<4>(it, begin, end, [&](int64_t e, auto whole) {
     float v[4];
-    load<4>(g, e, n, it.vec, v);
+    load<whole>(g, e, n, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s = __builtin_fma((double)v[j], (double)v[j], s);
-  }
+  });
   s = wave_add(s);
   if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = s;
   __syncthreads();
   if (threadIdx.x == 0) part[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
-// The norm and the factor that brings it to max_norm: partials in a fixed order.
-__global__ __launch_bounds__(1024) void norm_kernel(const double* part, int64_t n, double max_norm, float* out) {
+// The norm and the factor that brings it to max_norm, from the partial sums in a fixed order; for every thread of a workgroup.
+struct Norm {
+  float norm, by;
+};
+
+__device__ __forceinline__ Norm norm_of(const double* part, int64_t n, double max_norm) {
   __shared__ double sums[16];
   double s = 0;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
   s = wave_add(s);
   if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = s;
   __syncthreads();
-  if (threadIdx.x) return;
   s = 0;
+#pragma unroll
   for (int i = 0; i < 16; ++i) s += sums[i];
   const double norm = sqrt(s), by = max_norm / (norm + 1e-6);
-  out[0] = (float)norm;
-  out[1] = by > 1.0 ? 1.f : (float)by;      // a norm that is no number gives a factor that is none
+  return {(float)norm, by > 1.0 ? 1.f : (float)by};      // a norm that is no number gives a factor that is none
 }
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void scale_kernel(Table a, int64_t chunk, const float* by) {
+__global__ __launch_bounds__(1024) void norm_kernel(const double* part, int64_t n, double max_norm, float* out) {
+  const Norm v = norm_of(part, n, max_norm);
+  if (threadIdx.x) return;
+  out[0] = v.norm;
+  out[1] = v.by;
+}
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+template <typename T, int N>
+__global__ __launch_bounds__(THREADS) void scale_kernel(Table<N> a, int64_t chunk, const float* by) {
   const int i = tensor_of(a, blockIdx.x);
   const Item& it = a.t[i];
   T* g = static_cast<T*>(it.g);
   const float f = by[0];
   const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
-#pragma unroll 4
-  for (int64_t e = begin + threadIdx.x * 4; e < end; e += THREADS * 4) {
+  each_vector<4>(it, begin, end, [&](int64_t e, auto whole) {
     float v[4];
     T o[4];
-    load<4>(g, e, n, it.vec, v);
+    load<whole>(g, e, n, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (T)(v[j] * f);
-    store<4>(g, e, n, it.vec, o);
-  }
+    store<whole>(g, e, n, o);
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -171,13 +191,21 @@ struct Scalars {
   uint32_t key;
 };
 
-// A step's scalars for every tensor, in 64 bits (1 - beta^t loses digits in 32), and the count of steps one further.  A norm
-// that is not finite stops the step: nothing of the tensors changes.
-__global__ __launch_bounds__(THREADS) void begin_kernel(float* steps, int n, double lr, const float* lr_of, double beta1,
-                                                        double beta2, double decay, const float* norm, uint32_t seed,
-                                                        Scalars* out) {
-  const int i = blockIdx.x * THREADS + threadIdx.x;
-  if (i >= n || (norm && !(fabsf(norm[0]) <= 3.402823466e38f))) return;
+// A step's scalars for every tensor, in 64 bits (1 - beta^t loses digits in 32), the count of steps one further, and the norm.
+// One that is not finite stops the step: nothing of the tensors changes.
+__global__ __launch_bounds__(1024) void begin_kernel(float* steps, int n, double lr, const float* lr_of, double beta1,
+                                                     double beta2, double decay, const double* squares, int64_t count,
+                                                     double max_norm, float* norm, uint32_t seed, Scalars* out) {
+  const int i = blockIdx.x * 1024 + threadIdx.x;
+  if (squares) {
+    const Norm v = norm_of(squares, count, max_norm);
+    if (i == 0) {
+      norm[0] = v.norm;
+      norm[1] = v.by;
+    }
+    if (!finite(v.norm)) return;
+  }
+  if (i >= n) return;
   const float t = steps[i] + 1.f;
   steps[i] = t;
   if (lr_of) lr = (double)lr_of[0];
@@ -199,25 +227,26 @@ __global__ __launch_bounds__(THREADS) void begin_kernel(float* steps, int n, dou
 constexpr float M_TOP = 448.f, V_TOP = 31744.f;
 constexpr float SMALLEST = 0x1p-100f;     // a block whose largest value is under this holds zeros: 448 / it stays finite
 
+constexpr uint32_t INFINITE = 0x7F800000u;
+
+// A value a of 0 to the format's top.  Where numbers are evenly spaced, below 2^-6 (1 for roots), x = (a + 2^-6) / 2 lies in
+// the binary order below and has a's steps there; from 2^-6 on a is the larger of the two.  The code is then the exponent and
+// the kept bits of x, less those of x at a = 0.
 __device__ __forceinline__ uint32_t code_m(float m, float by, uint32_t random) {
-  const float a = fminf(fabsf(m) * by, M_TOP);
-  const bool small = a < 0x1p-6f;
-  const uint32_t bits = __float_as_uint(small ? a + 0x1p-6f : a) + (random << 4);
-  const uint32_t code = (bits >> 20) - (small ? 121u * 8 : 120u * 8);
-  return fabsf(m) <= 3.402823466e38f ? code | (__float_as_uint(m) >> 31 << 7) : 0x7Fu;
+  const float a = fminf(fabsf(m) * by, M_TOP), x = fmaxf(a, __builtin_fmaf(a, 0.5f, 0x1p-7f));
+  const uint32_t code = (__float_as_uint(x) + (random & 0xFFFFu) * 16u - (120u << 23)) >> 20;
+  return code | (__float_as_uint(m) >> 24 & 0x80u);
 }
 
 __device__ __forceinline__ uint32_t code_v(float r, float by, uint32_t random) {
-  const float a = fminf(r * by, V_TOP);
-  const bool small = a < 1.f;
-  const uint32_t bits = __float_as_uint(small ? a + 1.f : a) + (random << 3);
-  const uint32_t code = (bits >> 19) - (small ? 127u * 16 : 126u * 16);
-  return !(r <= 3.402823466e38f) ? 255u : a > 0.f && code == 0 ? 1u : code;
+  const float a = fminf(r * by, V_TOP), x = fmaxf(a, __builtin_fmaf(a, 0.5f, 0.5f));
+  const uint32_t code = (__float_as_uint(x) + (random >> 16) * 8u - (126u << 23)) >> 19;
+  return max(code, min(__float_as_uint(a), 1u));
 }
 
 __device__ __forceinline__ float value_v(uint32_t c) {
-  const bool small = c < 16;
-  return __uint_as_float((c + (small ? 127u * 16 : 126u * 16)) << 19) - (small ? 1.f : 0.f);
+  const float x = __uint_as_float((c << 19) + (126u << 23));
+  return fminf(x, __builtin_fmaf(x, 2.f, -1.f));
 }
 
 template <int I>
@@ -234,13 +263,15 @@ __device__ __forceinline__ float decode_m(uint32_t w, int i) {
   }
 }
 
-// The largest of a value's 32 neighbours (half a wave).
-__device__ __forceinline__ float half_max(float m) {
-  m = fmaxf(m, k2q_rot::dpp_f<0xB1>(m));
-  m = fmaxf(m, k2q_rot::dpp_f<0x4E>(m));
-  m = fmaxf(m, k2q_rot::dpp_f<0x141>(m));
-  m = fmaxf(m, k2q_rot::dpp_f<0x140>(m));
-  return fmaxf(m, __shfl_xor(m, 16));
+// The largest of a value's 32 neighbours (half a wave), of the bits of values of 0 and more: what is not finite is largest.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+
+__device__ __forceinline__ uint32_t half_max(uint32_t v) {
+  v = dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));
+  return max(v, (uint32_t)__shfl_xor((int)v, 16));
 }
 
 struct Step {
@@ -267,22 +298,26 @@ __device__ __forceinline__ T rounded(float p, int stochastic, uint32_t random) {
   return (T)p;
 }
 
-constexpr int64_t CHUNK = 8192;       // elements of a workgroup
 
-// One element's moments and parameter, each operation rounded once in 32 bits:
+// One element's moments and parameter, in 32 bits:
 //   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  p = decay p - size m / (root sqrt(v) + eps)
+// Moments in 32 bits are bound by memory, and their root and quotient are rounded correctly.  With codes the vector unit is as
+// busy as memory (about 75 operations an element, 90 with random rounding of the parameter): the hardware's root and
+// reciprocal, 1 ulp off each, take 8 where the exact ones take 25.
+template <bool kFast>
 __device__ __forceinline__ void element(const Step& a, const Scalars& s, float g, float& m, float& v, float& r, float& p) {
-  m = m * a.beta1 + g * a.alpha1;
-  v = v * a.beta2 + g * g * a.alpha2;
-  r = sqrtf(v);
-  p = p * s.decay - m / (r * s.root + a.eps) * s.size;
+  m = __builtin_fmaf(m, a.beta1, g * a.alpha1);
+  v = __builtin_fmaf(v, a.beta2, g * g * a.alpha2);
+  r = kFast ? __builtin_amdgcn_sqrtf(v) : sqrtf(v);
+  const float d = __builtin_fmaf(r, s.root, a.eps), u = kFast ? m * __builtin_amdgcn_rcpf(d) : m / d;
+  p = __builtin_fmaf(p, s.decay, -s.size * u);
 }
 
-template <typename T, bool kCodes>
-__global__ __launch_bounds__(THREADS) void adamw_kernel(Table a, Step st) {
+template <typename T, bool kCodes, int N>
+__global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chunk, Step st) {
   float by = 1.f;
   if (st.norm) {
-    if (!(fabsf(st.norm[0]) <= 3.402823466e38f)) return;
+    if (!finite(st.norm[0])) return;
     by = st.norm[1];
   }
   const int i = tensor_of(a, blockIdx.x);
@@ -290,15 +325,15 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table a, Step st) {
   const Scalars s = st.scalars[it.slot];
   T* P = static_cast<T*>(it.p);
   const T* G = static_cast<const T*>(it.g);
-  const int64_t n = it.n, at = it.at, begin = (int64_t)(blockIdx.x - a.first[i]) * CHUNK;
+  const int64_t n = it.n, at = it.at, begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   // moments reach to the end of the last block
-  const int64_t end = begin + CHUNK < n ? begin + CHUNK : (n + BLOCK - 1) / BLOCK * BLOCK;
+  const int64_t end = begin + chunk < n ? begin + chunk : (n + BLOCK - 1) / BLOCK * BLOCK;
   constexpr int V = kCodes ? 8 : 4;
-  for (int64_t e = begin + threadIdx.x * V; e < end; e += THREADS * V) {
+  each_vector<V>(it, begin, end, [&](int64_t e, auto whole) {
     float p[V], g[V], m[V], v[V], r[V];
     T o[V];
-    load<V>(P, e, n, it.vec, p);
-    load<V>(G, e, n, it.vec, g);
+    load<whole>(P, e, n, p);
+    load<whole>(G, e, n, g);
     uint32_t random[V];
     const uint64_t place = (uint64_t)(at + e);
     const uint32_t key = s.key ^ (uint32_t)(place >> 32) * 0x9E3779B9u;
@@ -311,26 +346,44 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table a, Step st) {
       v2u* cv = reinterpret_cast<v2u*>(static_cast<uint8_t*>(st.v) + place);
       const v2u wm = *cm, wv = *cv;
       const float sm = st.m_scale[place / BLOCK], sv = st.v_scale[place / BLOCK];
-      float am = 0.f, av = 0.f;
+      uint32_t bm = 0, bv = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         m[j] = decode_m(wm[j / 4], j % 4) * sm;
         const float root = value_v(wv[j / 4] >> (8 * (j % 4)) & 0xFFu) * sv;
         v[j] = root * root;
-        element(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
-        am = fmaxf(am, fabsf(m[j]) <= 3.402823466e38f ? fabsf(m[j]) : 0.f);
-        av = fmaxf(av, r[j] <= 3.402823466e38f ? r[j] : 0.f);
+        element<true>(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
+        bm = max(bm, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+        bv = max(bv, __float_as_uint(r[j]) & 0x7FFFFFFFu);
       }
-      am = half_max(am);
-      av = half_max(av);
+      bm = half_max(bm);
+      bv = half_max(bv);
+      const bool spoilt = bm >= INFINITE || bv >= INFINITE;
+      if (spoilt) {       // the scales are those of the rest
+        bm = bv = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const uint32_t am = __float_as_uint(m[j]) & 0x7FFFFFFFu, ar = __float_as_uint(r[j]) & 0x7FFFFFFFu;
+          bm = max(bm, am < INFINITE ? am : 0);
+          bv = max(bv, ar < INFINITE ? ar : 0);
+        }
+        bm = half_max(bm);
+        bv = half_max(bv);
+      }
+      float am = __uint_as_float(bm), av = __uint_as_float(bv);
       am = am < SMALLEST ? 0.f : am;
       av = av < SMALLEST ? 0.f : av;
       const float fm = am > 0.f ? M_TOP / am : 0.f, fv = av > 0.f ? V_TOP / av : 0.f;
       v2u nm = {0, 0}, nv = {0, 0};
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        nm[j / 4] |= code_m(m[j], fm, random[j] & 0xFFFFu) << (8 * (j % 4));
-        nv[j / 4] |= code_v(r[j], fv, random[j] >> 16) << (8 * (j % 4));
+        uint32_t cm = code_m(m[j], fm, random[j]), cr = code_v(r[j], fv, random[j]);
+        if (spoilt) {
+          cm = (__float_as_uint(m[j]) & 0x7FFFFFFFu) >= INFINITE ? 0x7Fu : cm;
+          cr = (__float_as_uint(r[j]) & 0x7FFFFFFFu) >= INFINITE ? 255u : cr;
+        }
+        nm[j / 4] |= cm << (8 * (j % 4));
+        nv[j / 4] |= cr << (8 * (j % 4));
       }
       *cm = nm;
       *cv = nv;
@@ -346,7 +399,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table a, Step st) {
       for (int j = 0; j < V; ++j) {
         m[j] = wm[j];
         v[j] = wv[j];
-        element(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
+        element<false>(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
         wm[j] = m[j];
         wv[j] = v[j];
       }
@@ -355,8 +408,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table a, Step st) {
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = rounded<T>(p[j], st.stochastic, st.stochastic ? mix(random[j] ^ 0x9E3779B9u) : 0u);
-    store<V>(P, e, n, it.vec, o);
-  }
+    store<whole>(P, e, n, o);
+  });
 }
 
 // What codes stand for: m and v, in 32 bits or bf16.
@@ -374,8 +427,8 @@ __global__ __launch_bounds__(THREADS) void moments_kernel(const uint8_t* cm, con
     const float root = value_v(wv[j / 4] >> (8 * (j % 4)) & 0xFFu) * sv;
     ov[j] = (T)(root * root);
   }
-  store<8>(m, e, n, true, om);
-  store<8>(v, e, n, true, ov);
+  store<true>(m, e, n, om);
+  store<true>(v, e, n, ov);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -395,22 +448,39 @@ int check(const k2q_step_tensor* t, int64_t count, bool params) {
   return K2Q_OK;
 }
 
-// Elements of a workgroup, for at most about 16384 partial sums: 8192 at least, which a small step spreads over CUs.
-int64_t norm_chunk(const k2q_step_tensor* t, int64_t count) {
+// Elements of a workgroup: CHUNK, or less, down to one turn of its threads, where a CU would not get four workgroups.
+int64_t step_chunk(const k2q_step_tensor* t, int64_t count, int64_t least) {
   int64_t total = 0, chunk = CHUNK;
+  for (int64_t i = 0; i < count; ++i) total += t[i].n;
+  while (chunk > least && total / chunk < 4 * (int64_t)k2q_cu_count()) chunk /= 2;
+  return chunk;
+}
+
+// The same for the norm, which has at most about 16384 partial sums.
+int64_t norm_chunk(const k2q_step_tensor* t, int64_t count) {
+  int64_t total = 0, chunk = step_chunk(t, count, 4 * THREADS);
   for (int64_t i = 0; i < count; ++i) total += t[i].n;
   while (total / chunk > 16384) chunk *= 2;
   return chunk;
 }
 
-// f(table) over the tensors of one type, TENSORS and 2^30 workgroups at a time.
-template <class F>
-void each_table(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, F&& f) {
-  Table a{};
-  for (int64_t i = 0; i < count; ++i) {
+int64_t norm_parts(const k2q_step_tensor* t, int64_t count) {
+  const int64_t chunk = norm_chunk(t, count);
+  int64_t parts = 0;
+  for (int64_t i = 0; i < count; ++i) parts += (t[i].n + chunk - 1) / chunk;
+  return parts;
+}
+
+// f(table) over the tensors of one type, N and 2^30 workgroups at a time.  Behind a pass over the gradients they go backwards:
+// what that pass read last is still in the last-level cache.
+template <int N, class F>
+void tables(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, bool backwards, F&& f) {
+  Table<N> a{};
+  for (int64_t k = 0; k < count; ++k) {
+    const int64_t i = backwards ? count - 1 - k : k;
     if (t[i].dtype != dtype) continue;
     const uint32_t blocks = (uint32_t)((t[i].n + chunk - 1) / chunk);
-    if (a.count == TENSORS || (a.count && (int64_t)a.blocks + blocks > 1 << 30)) {
+    if (a.count == N || (a.count && (int64_t)a.blocks + blocks > 1 << 30)) {
       f(a);
       a.count = 0;
       a.blocks = 0;
@@ -424,6 +494,12 @@ void each_table(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chun
 }
 
 template <class F>
+void each_table(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, bool backwards, F&& f) {
+  if (count <= FEW) tables<FEW>(t, count, dtype, chunk, backwards, f);
+  else tables<TENSORS>(t, count, dtype, chunk, backwards, f);
+}
+
+template <class F>
 void by_type(F&& f) {
   f(K2Q_DTYPE_BF16, __bf16{});
   f(K2Q_DTYPE_F32, float{});
@@ -433,29 +509,25 @@ void by_type(F&& f) {
 }  // namespace
 
 extern "C" int64_t k2q_grad_norm_ws_bytes(const k2q_step_tensor* t, int64_t count) {
-  if (check(t, count, false) != K2Q_OK) return 0;
-  const int64_t chunk = norm_chunk(t, count);
-  int64_t parts = 0;
-  for (int64_t i = 0; i < count; ++i) parts += (t[i].n + chunk - 1) / chunk;
-  return parts * 8;
+  return check(t, count, false) != K2Q_OK ? 0 : 8 * norm_parts(t, count);
 }
 
 extern "C" int k2q_grad_norm(const k2q_step_tensor* t, int64_t count, double max_norm, void* ws, int64_t ws_bytes, float* out,
                              void* stream) {
   int rc = check(t, count, false);
   if (rc != K2Q_OK) return rc;
-  const int64_t need = k2q_grad_norm_ws_bytes(t, count);
-  if (!(max_norm >= 0) || !ws || ws_bytes < need || !k2q_aligned(ws, 16) || !out || !k2q_aligned(out, 8)) return K2Q_EINVAL;
-  const int64_t chunk = norm_chunk(t, count);
+  const int64_t parts = norm_parts(t, count), chunk = norm_chunk(t, count);
+  if (!(max_norm >= 0) || !ws || ws_bytes < 8 * parts || !k2q_aligned(ws, 16) || !k2q_aligned(out, 8)) return K2Q_EINVAL;
   double* part = static_cast<double*>(ws);
   hipStream_t st = static_cast<hipStream_t>(stream);
   by_type([&](int dtype, auto T) {
-    each_table(t, count, dtype, chunk, [&](const Table& a) {
-      hipLaunchKernelGGL(sumsq_kernel<decltype(T)>, dim3(a.blocks), dim3(THREADS), 0, st, a, chunk, part);
+    each_table(t, count, dtype, chunk, false, [&](const auto& a) {
+      hipLaunchKernelGGL((sumsq_kernel<decltype(T), std::extent_v<decltype(a.first)>>), dim3(a.blocks), dim3(THREADS), 0, st, a, chunk, part);
       part += a.blocks;
     });
   });
-  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(1024), 0, st, static_cast<const double*>(ws), need / 8, max_norm, out);
+  if (out)
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(1024), 0, st, static_cast<const double*>(ws), parts, max_norm, out);
   return k2q_launch_status();
 }
 
@@ -463,10 +535,11 @@ extern "C" int k2q_scale_grads(const k2q_step_tensor* t, int64_t count, const fl
   int rc = check(t, count, false);
   if (rc != K2Q_OK) return rc;
   if (!by || !k2q_aligned(by, 4)) return K2Q_EINVAL;
+  const int64_t chunk = step_chunk(t, count, 4 * THREADS);
   by_type([&](int dtype, auto T) {
-    each_table(t, count, dtype, CHUNK, [&](const Table& a) {
-      hipLaunchKernelGGL(scale_kernel<decltype(T)>, dim3(a.blocks), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a,
-                         CHUNK, by);
+    each_table(t, count, dtype, chunk, true, [&](const auto& a) {
+      hipLaunchKernelGGL((scale_kernel<decltype(T), std::extent_v<decltype(a.first)>>), dim3(a.blocks), dim3(THREADS), 0,
+                         static_cast<hipStream_t>(stream), a, chunk, by);
     });
   });
   return k2q_launch_status();
@@ -476,15 +549,16 @@ extern "C" int64_t k2q_adamw_ws_bytes(int64_t count) { return count < 1 ? 0 : co
 
 extern "C" int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits, void* exp_avg, void* exp_avg_sq,
                          float* avg_scale, float* sq_scale, float* steps, double lr, const float* lr_of, double beta1,
-                         double beta2, double eps, double weight_decay, const float* norm, int stochastic, uint32_t seed,
-                         void* ws, int64_t ws_bytes, void* stream) {
+                         double beta2, double eps, double weight_decay, const double* squares, int64_t n_squares,
+                         double max_norm, float* norm, int stochastic, uint32_t seed, void* ws, int64_t ws_bytes,
+                         void* stream) {
   int rc = check(t, count, true);
   if (rc != K2Q_OK) return rc;
   if ((state_bits != 32 && state_bits != 8) || !exp_avg || !exp_avg_sq || !k2q_aligned(exp_avg, 16) ||
       !k2q_aligned(exp_avg_sq, 16) || (state_bits == 8 && (!avg_scale || !sq_scale)) || !k2q_aligned(avg_scale, 4) ||
       !k2q_aligned(sq_scale, 4) || !steps || !k2q_aligned(steps, 4) || !(beta1 >= 0 && beta1 < 1) ||
       !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(lr == lr) || !(weight_decay >= 0) || !k2q_aligned(lr_of, 4) ||
-      !k2q_aligned(norm, 8) || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_adamw_ws_bytes(count) || count > 0x7fffffff)
+      (squares && (n_squares < 1 || !k2q_aligned(squares, 8) || !(max_norm >= 0) || !norm || !k2q_aligned(norm, 8))) || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_adamw_ws_bytes(count) || count > 0x7fffffff)
     return K2Q_EINVAL;
   for (int64_t i = 0; i < count; ++i)
     if ((stochastic && t[i].dtype == K2Q_DTYPE_F16) || (i && t[i].index <= t[i - 1].index)) return K2Q_EINVAL;
@@ -492,17 +566,20 @@ extern "C" int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits
   Scalars* scalars = static_cast<Scalars*>(ws);
   for (int64_t i = 0, j; i < count; i = j) {      // counts of neighbouring places in one launch
     for (j = i + 1; j < count && t[j].index == t[j - 1].index + 1;) ++j;
-    hipLaunchKernelGGL(begin_kernel, dim3((unsigned)((j - i + THREADS - 1) / THREADS)), dim3(THREADS), 0, st,
-                       steps + t[i].index, (int)(j - i), lr, lr_of, beta1, beta2, weight_decay, norm, seed, scalars + i);
+    hipLaunchKernelGGL(begin_kernel, dim3((unsigned)((j - i + 1023) / 1024)), dim3(1024), 0, st, steps + t[i].index,
+                       (int)(j - i), lr, lr_of, beta1, beta2, weight_decay, squares, n_squares, max_norm, norm, seed,
+                       scalars + i);
   }
-  const Step s{exp_avg, exp_avg_sq, avg_scale, sq_scale, scalars, norm, (float)beta1, (float)(1 - beta1), (float)beta2,
+  const int64_t chunk = step_chunk(t, count, (state_bits == 8 ? 8 : 4) * THREADS);
+  const Step s{exp_avg, exp_avg_sq, avg_scale, sq_scale, scalars, squares ? norm : nullptr, (float)beta1, (float)(1 - beta1), (float)beta2,
                (float)(1 - beta2), (float)eps, stochastic};
   by_type([&](int dtype, auto T) {
-    each_table(t, count, dtype, CHUNK, [&](const Table& a) {
+    each_table(t, count, dtype, chunk, squares != nullptr, [&](const auto& a) {
+      constexpr int N = std::extent_v<decltype(a.first)>;
       if (state_bits == 8)
-        hipLaunchKernelGGL((adamw_kernel<decltype(T), true>), dim3(a.blocks), dim3(THREADS), 0, st, a, s);
+        hipLaunchKernelGGL((adamw_kernel<decltype(T), true, N>), dim3(a.blocks), dim3(THREADS), 0, st, a, chunk, s);
       else
-        hipLaunchKernelGGL((adamw_kernel<decltype(T), false>), dim3(a.blocks), dim3(THREADS), 0, st, a, s);
+        hipLaunchKernelGGL((adamw_kernel<decltype(T), false, N>), dim3(a.blocks), dim3(THREADS), 0, st, a, chunk, s);
     });
   });
   return k2q_launch_status();

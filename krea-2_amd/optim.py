@@ -7,6 +7,7 @@ multiple of 256 elements; ``state[p]`` holds views of them.
 """
 from __future__ import annotations
 
+import importlib
 import math
 from types import SimpleNamespace
 
@@ -15,6 +16,10 @@ import torch
 from . import _lib
 
 _BLOCK = _lib.MOMENT_BLOCK
+
+# what torch.optim.optimizer.register_optimizer_step_pre_hook and its post form register, for every optimizer
+_torch_optimizer = importlib.import_module("torch.optim.optimizer")
+_EVERY = (_torch_optimizer._global_optimizer_pre_hooks, _torch_optimizer._global_optimizer_post_hooks)
 
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
@@ -149,16 +154,37 @@ class AdamW(torch.optim.Optimizer):
             raise
 
     # -- the step ------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None):
+        """One step of every parameter that has a gradient; ``closure``, if given, is called first and its value returned."""
+        hooks = _hooks(self)
+        args, kwargs = (closure,) if closure is not None else (), {}
+        for hook in hooks[0]:
+            given = hook(self, args, kwargs)
+            if given is not None:
+                args, kwargs = given
+        closure = args[0] if args else kwargs.get("closure")
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, norm = self.param_groups, None
+        if torch.autograd._profiler_enabled():
+            with torch.autograd.profiler.record_function("Optimizer.step#AdamW.step"):
+                self._step()
+        else:
+            self._step()
+        for hook in hooks[1]:
+            hook(self, args, kwargs)
+        return loss
+
+    step.hooked = True      # hooks and the profiler's label are above: torch's own wrapper takes 12 of a small step's 28 us
+
+    def _step(self) -> None:
+        groups, squares, norm = self.param_groups, None, None
         if self.max_norm is not None:
             every = groups[0]["params"] if len(groups) == 1 else [p for g in groups for p in g["params"]]
-            norm = _lib.grad_norm(every, self.max_norm, False)
+            squares = _lib.grad_norm(every, self.max_norm, False)
+            if squares is not None:
+                norm = torch.empty(2, device=squares.device)
             self.grad_norm = None if norm is None else norm[0]
         for i, g in enumerate(groups):
             held = self._held.get(i) or self._moments_of(i)
@@ -167,8 +193,14 @@ class AdamW(torch.optim.Optimizer):
                 lr, lr_of = (0.0, lr) if lr.is_cuda else (float(lr), None)
             scales = (held.exp_avg_scale, held.exp_avg_sq_scale) if g["state_bits"] == 8 else (None, None)
             _lib.adamw(g["params"], held.starts, g["state_bits"], held.exp_avg, held.exp_avg_sq, *scales, held.steps, lr,
-                       lr_of, *g["betas"], g["eps"], g["weight_decay"], norm, g["stochastic"], g["seed"])
-        return loss
+                       lr_of, *g["betas"], g["eps"], g["weight_decay"], squares, self.max_norm or 0.0, norm, g["stochastic"],
+                       g["seed"])
+
+
+def _hooks(opt: torch.optim.Optimizer):
+    """What is registered to run ahead of a step and behind it: for every optimizer, and for this one."""
+    return ([*_EVERY[0].values(), *opt._optimizer_step_pre_hooks.values()],
+            [*opt._optimizer_step_post_hooks.values(), *_EVERY[1].values()])
 
 
 def _kinds(bits: int) -> dict:

@@ -25,6 +25,37 @@ def test_adamw_refuses_options(k2, bad):
         k2.AdamW([{"params": [_p(4)], **bad}]) if "max_norm" not in bad else k2.AdamW([_p(4)], **bad)
 
 
+def test_hooks_closures_and_schedulers(k2):
+    """What torch runs around a step: hooks of all optimizers and of one, the closure with gradients on, a scheduler's count,
+    and its label under the profiler."""
+    import importlib
+    every = importlib.import_module("torch.optim.optimizer")
+    opt, seen = k2.AdamW([_p(4, grad=False)]), []
+    opt._step = lambda: seen.append("step")
+    handles = [every.register_optimizer_step_pre_hook(lambda o, a, k: seen.append("all before")),
+               every.register_optimizer_step_post_hook(lambda o, a, k: seen.append("all behind")),
+               opt.register_step_pre_hook(lambda o, a, k: seen.append("before")),
+               opt.register_step_post_hook(lambda o, a, k: seen.append("behind"))]
+
+    def closure():
+        seen.append(torch.is_grad_enabled())
+        return 3.0
+
+    with torch.no_grad():
+        assert opt.step(closure) == 3.0
+    assert seen == ["all before", "before", True, "step", "behind", "all behind"]
+    for h in handles:
+        h.remove()
+    scheduler = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    del seen[:]
+    assert opt.step() is None and seen == ["step"]
+    scheduler.step()
+    assert opt.param_groups[0]["lr"] == 5e-4
+    with torch.profiler.profile() as p:
+        opt.step()
+    assert any(e.key == "Optimizer.step#AdamW.step" for e in p.key_averages())
+
+
 def test_steps_run_on_the_gpu_alone(k2):
     opt = k2.AdamW([_p(4)])
     with pytest.raises(RuntimeError):
@@ -85,26 +116,27 @@ def test_step_entries_refuse_bad_arguments(k2):
     def one(**kw):
         return k2._lib.StepTensor(**{"p": a, "g": a, "n": 4, "at": 0, "index": 0, "dtype": 1, **kw})
 
-    def call(t=None, count=None, bits=32, m=a, v=a, ms=None, vs=None, steps=a, lr=1e-3, b1=0.9, b2=0.9, eps=0.0, wd=0.0, norm=None,
-             stochastic=0, ws=a, nws=1 << 20):
+    def call(t=None, count=None, bits=32, m=a, v=a, ms=None, vs=None, steps=a, lr=1e-3, b1=0.9, b2=0.9, eps=0.0, wd=0.0, sq=None,
+             nsq=1, most=1.0, norm=a, stochastic=0, ws=a, nws=1 << 20):
         t = [one()] if t is None else t
         arr = (k2._lib.StepTensor * max(len(t), 1))(*t)
         return lib.k2q_adamw(ctypes.addressof(arr), len(t) if count is None else count, bits, m, v, ms, vs, steps, lr, None, b1,
-                             b2, eps, wd, norm, stochastic, 0, ws, nws, None)
+                             b2, eps, wd, sq, nsq, most, norm, stochastic, 0, ws, nws, None)
 
     for bad in ({"count": 0}, {"t": [one(p=None)]}, {"t": [one(g=None)]}, {"t": [one(n=0)]}, {"t": [one(at=8)]},
                 {"t": [one(at=-256)]}, {"t": [one(index=-1)]}, {"t": [one(dtype=3)]}, {"t": [one(p=a + 2)]},
                 {"t": [one(), one()]}, {"bits": 4}, {"m": None}, {"v": a + 4}, {"bits": 8}, {"steps": None},
-                {"lr": float("nan")}, {"b1": 1.0}, {"b2": -0.5}, {"eps": -1.0}, {"wd": float("nan")}, {"norm": a + 4},
+                {"lr": float("nan")}, {"b1": 1.0}, {"b2": -0.5}, {"eps": -1.0}, {"wd": float("nan")}, {"sq": a, "norm": a + 4},
+                {"sq": a + 4}, {"sq": a, "nsq": 0}, {"sq": a, "most": -1.0}, {"sq": a, "norm": None},
                 {"ws": None}, {"nws": 8}, {"stochastic": 1, "t": [one(dtype=2)]}):
         assert call(**bad) == -1, bad
     assert call(t=[one(n=1 << 43)]) == -4
     arr = (k2._lib.StepTensor * 2)(one(), one(n=100000))
     addr = ctypes.addressof(arr)
     need = lib.k2q_grad_norm_ws_bytes(addr, 2)
-    assert need == 8 * (1 + 13) and lib.k2q_grad_norm_ws_bytes(addr, 0) == 0
+    assert need == 8 * (1 + 98) and lib.k2q_grad_norm_ws_bytes(addr, 0) == 0
     for args in ((addr, 2, -1.0, a, need, a), (addr, 2, 1.0, None, need, a), (addr, 2, 1.0, a, need - 1, a),
-                 (addr, 2, 1.0, a, need, None), (addr, 0, 1.0, a, need, a), (None, 2, 1.0, a, need, a)):
+                 (addr, 2, 1.0, a, need, a + 4), (addr, 0, 1.0, a, need, a), (None, 2, 1.0, a, need, a)):
         assert lib.k2q_grad_norm(*args, None) == -1
     assert lib.k2q_scale_grads(addr, 2, None, None) == -1
     for args in ((None, a, a, a, 256, 0, a, a), (a, a, a, a, 255, 0, a, a), (a, a, a, a, 256, 2, a, a), (a, a, a, a, 0, 0, a, a)):
