@@ -19,7 +19,10 @@ constexpr int FEW = 8;
 constexpr int THREADS = 256;
 constexpr int BLOCK = K2Q_MOMENT_BLOCK;
 
-constexpr int64_t CHUNK = 8192;       // most elements of a step's workgroup
+// Elements of a workgroup.  A step streams: nothing that it reads or writes is wanted again before a whole training step has
+// gone by, so all of it passes by the last-level cache.  214.7M parameters in f32, us at 2048 / 4096 / 8192 / 32768 elements
+// 1136 / 1160 / 1177 / 1249 through that cache, 1029 at 2048 past it (5.8 TB/s, as much as torch.add of large operands).
+constexpr int64_t CHUNK = 2048;
 
 struct Item {
   void* p;
@@ -47,50 +50,43 @@ __device__ __forceinline__ int tensor_of(const Table<N>& a, uint32_t wg) {
   return lo;
 }
 
-// V values of a tensor from element e on.  kWhole: all of them are the tensor's, and vectors are aligned, so that the loads of
+// 4 values of a tensor from element e on.  kWhole: all of them are the tensor's, and vectors are aligned, so that the loads of
 // several turns of a loop leave together; else what lies past its end reads as zero and is not written.
-template <bool kWhole, int V, typename T>
-__device__ __forceinline__ void load(const T* p, int64_t e, int64_t n, float (&v)[V]) {
+template <bool kWhole, bool kPast, typename T>
+__device__ __forceinline__ v4f load(const T* p, int64_t e, int64_t n) {
   typedef T VecT __attribute__((ext_vector_type(4)));
-#pragma unroll
-  for (int i = 0; i < V; i += 4) {
-    VecT q;
-    if constexpr (kWhole) {
-      q = *reinterpret_cast<const VecT*>(p + e + i);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = e + i + j < n ? p[e + i + j] : (T)0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[i + j] = (float)q[j];
-  }
-}
-
-template <bool kWhole, int V, typename T>
-__device__ __forceinline__ void store(T* p, int64_t e, int64_t n, const T (&v)[V]) {
-  typedef T VecT __attribute__((ext_vector_type(4)));
-#pragma unroll
-  for (int i = 0; i < V; i += 4) {
-    if constexpr (kWhole) {
-      *reinterpret_cast<VecT*>(p + e + i) = VecT{v[i], v[i + 1], v[i + 2], v[i + 3]};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (e + i + j < n) p[e + i + j] = v[i + j];
-    }
-  }
-}
-
-// f(e, whole) for a workgroup's vectors of V elements; whole: a std::bool_constant, as above.
-template <int V, class F>
-__device__ __forceinline__ void each_vector(const Item& it, int64_t begin, int64_t end, F&& f) {
-  const bool whole = it.vec && end <= it.n && (end - begin) % (THREADS * V) == 0;
-  if (whole) {
-    const int turns = (int)((end - begin) / (THREADS * V));       // a chunk is whole turns
-#pragma unroll 4
-    for (int i = 0; i < turns; ++i) f(begin + i * (THREADS * V) + threadIdx.x * V, std::true_type{});
+  VecT q;
+  if constexpr (kWhole) {
+    const VecT* at = reinterpret_cast<const VecT*>(p + e);
+    q = kPast ? __builtin_nontemporal_load(at) : *at;
   } else {
-    for (int64_t e = begin + threadIdx.x * V; e < end; e += THREADS * V) f(e, std::false_type{});
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = e + j < n ? p[e + j] : (T)0.f;
+  }
+  return v4f{(float)q[0], (float)q[1], (float)q[2], (float)q[3]};
+}
+
+template <bool kWhole, typename T>
+__device__ __forceinline__ void store(T* p, int64_t e, int64_t n, const T (&v)[4]) {
+  typedef T VecT __attribute__((ext_vector_type(4)));
+  if constexpr (kWhole) {
+    __builtin_nontemporal_store((VecT{v[0], v[1], v[2], v[3]}), reinterpret_cast<VecT*>(p + e));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (e + j < n) p[e + j] = v[j];
+  }
+}
+
+// f(first element of a turn, whole) for a workgroup's turns of THREADS x V elements; whole: a bool constant, as above.
+template <int V, class F>
+__device__ __forceinline__ void each_turn(const Item& it, int64_t begin, int64_t end, F&& f) {
+  const int turns = (int)((end - begin + THREADS * V - 1) / (THREADS * V));
+  if (it.vec && end <= it.n && (end - begin) % (THREADS * V) == 0) {
+#pragma unroll 4
+    for (int i = 0; i < turns; ++i) f(begin + i * (THREADS * V), std::true_type{});
+  } else {
+    for (int i = 0; i < turns; ++i) f(begin + i * (THREADS * V), std::false_type{});
   }
 }
 
@@ -114,9 +110,10 @@ __global__ __launch_bounds__(THREADS) void sumsq_kernel(Table<N> a, int64_t chun
   const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
   double s = 0;
-  each_vector<4>(it, begin, end, [&](int64_t e, auto whole) {
-    float v[4];
-    load<whole>(g, e, n, v);
+  each_turn<4>(it, begin, end, [&](int64_t e, auto whole) {
+    e += threadIdx.x * 4;
+    if (!whole && e >= end) return;
+    const v4f v = load<whole, false>(g, e, n);      // kept: the step reads it next
 #pragma unroll
     for (int j = 0; j < 4; ++j) s = __builtin_fma((double)v[j], (double)v[j], s);
   });
@@ -163,10 +160,11 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(Table<N> a, int64_t chun
   const float f = by[0];
   const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
-  each_vector<4>(it, begin, end, [&](int64_t e, auto whole) {
-    float v[4];
+  each_turn<4>(it, begin, end, [&](int64_t e, auto whole) {
+    e += threadIdx.x * 4;
+    if (!whole && e >= end) return;
+    const v4f v = load<whole, true>(g, e, n);
     T o[4];
-    load<whole>(g, e, n, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (T)(v[j] * f);
     store<whole>(g, e, n, o);
@@ -328,33 +326,55 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
   const int64_t n = it.n, at = it.at, begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   // moments reach to the end of the last block
   const int64_t end = begin + chunk < n ? begin + chunk : (n + BLOCK - 1) / BLOCK * BLOCK;
-  constexpr int V = kCodes ? 8 : 4;
-  each_vector<V>(it, begin, end, [&](int64_t e, auto whole) {
-    float p[V], g[V], m[V], v[V], r[V];
-    T o[V];
-    load<whole>(P, e, n, p);
-    load<whole>(G, e, n, g);
-    uint32_t random[V];
+  // A thread has one quad of neighbours, or, with codes, two, and 32 threads a block.  Two quads of 4-byte values lie 128 apart,
+  // so that each vector instruction takes whole lines; of 2-byte values side by side, 16 bytes.
+  constexpr int QUADS = kCodes ? 2 : 1, V = 4 * QUADS;
+  constexpr int GAP = sizeof(T) == 4 ? 128 : 4, NEXT = !kCodes || sizeof(T) == 4 ? 4 : 8;
+  each_turn<V>(it, begin, end, [&](int64_t e, auto whole) {
+    const int t = threadIdx.x;
+    e += kCodes ? t / 32 * BLOCK + t % 32 * NEXT : t * NEXT;
+    if (!whole && e >= end) return;
     const uint64_t place = (uint64_t)(at + e);
-    const uint32_t key = s.key ^ (uint32_t)(place >> 32) * 0x9E3779B9u;
-    if (kCodes || st.stochastic) {
+    v4f p[QUADS], g[QUADS], m[QUADS], v[QUADS], r[QUADS];
 #pragma unroll
-      for (int j = 0; j < V; ++j) random[j] = mix((uint32_t)(place + j) ^ key);
+    for (int q = 0; q < QUADS; ++q) {
+      p[q] = load<whole, true>(P, e + q * GAP, n);
+      g[q] = load<whole, true>(G, e + q * GAP, n);
+    }
+    uint32_t random[V];
+    if (kCodes || st.stochastic) {
+      const uint32_t key = s.key ^ (uint32_t)(place >> 32) * 0x9E3779B9u;     // a block does not straddle 2^32
+#pragma unroll
+      for (int j = 0; j < V; ++j) random[j] = mix((uint32_t)(place + j / 4 * GAP + j % 4) ^ key);
     }
     if constexpr (kCodes) {
-      v2u* cm = reinterpret_cast<v2u*>(static_cast<uint8_t*>(st.m) + place);
-      v2u* cv = reinterpret_cast<v2u*>(static_cast<uint8_t*>(st.v) + place);
-      const v2u wm = *cm, wv = *cv;
+      uint8_t *cm = static_cast<uint8_t*>(st.m) + place, *cv = static_cast<uint8_t*>(st.v) + place;
+      uint32_t wm[2], wv[2];
+      if constexpr (GAP == 4) {
+        const v2u a = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(cm));
+        const v2u b = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(cv));
+        wm[0] = a[0], wm[1] = a[1], wv[0] = b[0], wv[1] = b[1];
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          wm[q] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(cm + q * GAP));
+          wv[q] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(cv + q * GAP));
+        }
+      }
       const float sm = st.m_scale[place / BLOCK], sv = st.v_scale[place / BLOCK];
       uint32_t bm = 0, bv = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        m[j] = decode_m(wm[j / 4], j % 4) * sm;
-        const float root = value_v(wv[j / 4] >> (8 * (j % 4)) & 0xFFu) * sv;
-        v[j] = root * root;
-        element<true>(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
-        bm = max(bm, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-        bv = max(bv, __float_as_uint(r[j]) & 0x7FFFFFFFu);
+        const int q = j / 4, i = j % 4;
+        m[q][i] = decode_m(wm[q], i) * sm;
+        const float root = value_v(wv[q] >> (8 * i) & 0xFFu) * sv;
+        float mj = m[q][i], vj = root * root, rj, pj = p[q][i];
+        element<true>(st, s, g[q][i] * by, mj, vj, rj, pj);
+        m[q][i] = mj;
+        r[q][i] = rj;
+        p[q][i] = pj;
+        bm = max(bm, __float_as_uint(mj) & 0x7FFFFFFFu);
+        bv = max(bv, __float_as_uint(rj) & 0x7FFFFFFFu);
       }
       bm = half_max(bm);
       bv = half_max(bv);
@@ -363,7 +383,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
         bm = bv = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const uint32_t am = __float_as_uint(m[j]) & 0x7FFFFFFFu, ar = __float_as_uint(r[j]) & 0x7FFFFFFFu;
+          const uint32_t am = __float_as_uint(m[j / 4][j % 4]) & 0x7FFFFFFFu, ar = __float_as_uint(r[j / 4][j % 4]) & 0x7FFFFFFFu;
           bm = max(bm, am < INFINITE ? am : 0);
           bv = max(bv, ar < INFINITE ? ar : 0);
         }
@@ -374,41 +394,58 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
       am = am < SMALLEST ? 0.f : am;
       av = av < SMALLEST ? 0.f : av;
       const float fm = am > 0.f ? M_TOP / am : 0.f, fv = av > 0.f ? V_TOP / av : 0.f;
-      v2u nm = {0, 0}, nv = {0, 0};
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        uint32_t cm = code_m(m[j], fm, random[j]), cr = code_v(r[j], fv, random[j]);
-        if (spoilt) {
-          cm = (__float_as_uint(m[j]) & 0x7FFFFFFFu) >= INFINITE ? 0x7Fu : cm;
-          cr = (__float_as_uint(r[j]) & 0x7FFFFFFFu) >= INFINITE ? 255u : cr;
+      for (int q = 0; q < 2; ++q) {
+        wm[q] = wv[q] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float mj = m[q][i], rj = r[q][i];
+          uint32_t dm = code_m(mj, fm, random[4 * q + i]), dv = code_v(rj, fv, random[4 * q + i]);
+          if (spoilt) {
+            dm = (__float_as_uint(mj) & 0x7FFFFFFFu) >= INFINITE ? 0x7Fu : dm;
+            dv = (__float_as_uint(rj) & 0x7FFFFFFFu) >= INFINITE ? 255u : dv;
+          }
+          wm[q] |= dm << (8 * i);
+          wv[q] |= dv << (8 * i);
         }
-        nm[j / 4] |= cm << (8 * (j % 4));
-        nv[j / 4] |= cr << (8 * (j % 4));
       }
-      *cm = nm;
-      *cv = nv;
-      if (threadIdx.x % 32 == 0) {
+      if constexpr (GAP == 4) {
+        __builtin_nontemporal_store((v2u{wm[0], wm[1]}), reinterpret_cast<v2u*>(cm));
+        __builtin_nontemporal_store((v2u{wv[0], wv[1]}), reinterpret_cast<v2u*>(cv));
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          __builtin_nontemporal_store(wm[q], reinterpret_cast<uint32_t*>(cm + q * GAP));
+          __builtin_nontemporal_store(wv[q], reinterpret_cast<uint32_t*>(cv + q * GAP));
+        }
+      }
+      if (t % 32 == 0) {
         st.m_scale[place / BLOCK] = am / M_TOP;
         st.v_scale[place / BLOCK] = av / V_TOP;
       }
     } else {
       v4f* fm = reinterpret_cast<v4f*>(static_cast<float*>(st.m) + place);
       v4f* fv = reinterpret_cast<v4f*>(static_cast<float*>(st.v) + place);
-      v4f wm = *fm, wv = *fv;
+      v4f wm = __builtin_nontemporal_load(fm), wv = __builtin_nontemporal_load(fv);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        m[j] = wm[j];
-        v[j] = wv[j];
-        element<false>(st, s, g[j] * by, m[j], v[j], r[j], p[j]);
-        wm[j] = m[j];
-        wv[j] = v[j];
+      for (int i = 0; i < 4; ++i) {
+        float mj = wm[i], vj = wv[i], rj, pj = p[0][i];
+        element<false>(st, s, g[0][i] * by, mj, vj, rj, pj);
+        wm[i] = mj;
+        wv[i] = vj;
+        p[0][i] = pj;
       }
-      *fm = wm;
-      *fv = wv;
+      __builtin_nontemporal_store(wm, fm);
+      __builtin_nontemporal_store(wv, fv);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = rounded<T>(p[j], st.stochastic, st.stochastic ? mix(random[j] ^ 0x9E3779B9u) : 0u);
-    store<whole>(P, e, n, o);
+    for (int q = 0; q < QUADS; ++q) {
+      T o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o[i] = rounded<T>(p[q][i], st.stochastic, st.stochastic ? mix(random[4 * q + i] ^ 0x9E3779B9u) : 0u);
+      store<whole>(P, e + q * GAP, n, o);
+    }
   });
 }
 
@@ -418,17 +455,19 @@ __global__ __launch_bounds__(THREADS) void moments_kernel(const uint8_t* cm, con
                                                           const float* v_scale, int64_t n, T* m, T* v) {
   const int64_t e = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 8;
   if (e >= n) return;
-  const v2u wm = *reinterpret_cast<const v2u*>(cm + e), wv = *reinterpret_cast<const v2u*>(cv + e);
+  const v2u wm = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(cm + e));
+  const v2u wv = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(cv + e));
   const float sm = m_scale[e / BLOCK], sv = v_scale[e / BLOCK];
-  T om[8], ov[8];
+  typedef T Vec8 __attribute__((ext_vector_type(8)));
+  Vec8 om, ov;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     om[j] = (T)(decode_m(wm[j / 4], j % 4) * sm);
     const float root = value_v(wv[j / 4] >> (8 * (j % 4)) & 0xFFu) * sv;
     ov[j] = (T)(root * root);
   }
-  store<true>(m, e, n, om);
-  store<true>(v, e, n, ov);
+  *reinterpret_cast<Vec8*>(m + e) = om;
+  *reinterpret_cast<Vec8*>(v + e) = ov;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
