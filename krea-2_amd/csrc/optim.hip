@@ -242,6 +242,12 @@ __device__ __forceinline__ uint32_t code_v(float r, float by, uint32_t random) {
   return max(code, min(__float_as_uint(a), 1u));
 }
 
+// A value's bits without the sign, 0 for one that is not finite.
+__device__ __forceinline__ uint32_t below_infinite(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b < INFINITE ? b : 0;
+}
+
 __device__ __forceinline__ float value_v(uint32_t c) {
   const float x = __uint_as_float((c << 19) + (126u << 23));
   return fminf(x, __builtin_fmaf(x, 2.f, -1.f));
@@ -287,10 +293,9 @@ struct Step {
 template <typename T>
 __device__ __forceinline__ T rounded(float p, int stochastic, uint32_t random) {
   if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) {
-    if (stochastic) {
-      const uint32_t bits = __float_as_uint(p);
-      const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
-      return __builtin_bit_cast(T, (uint16_t)((finite ? bits + (random & 0xFFFFu) : bits | (bits & 0xFFFFu ? 0x400000u : 0u)) >> 16));
+    if (stochastic) {     // infinite bits end with zeros and stay; those of a NaN could carry past its sign
+      const uint32_t bits = __float_as_uint(p) + (random & 0xFFFFu);
+      return __builtin_bit_cast(T, (uint16_t)((p != p ? 0x7FC00000u : bits) >> 16));
     }
   }
   return (T)p;
@@ -300,8 +305,8 @@ __device__ __forceinline__ T rounded(float p, int stochastic, uint32_t random) {
 // One element's moments and parameter, in 32 bits:
 //   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  p = decay p - size m / (root sqrt(v) + eps)
 // Moments in 32 bits are bound by memory, and their root and quotient are rounded correctly.  With codes the vector unit is as
-// busy as memory (about 75 operations an element, 90 with random rounding of the parameter): the hardware's root and
-// reciprocal, 1 ulp off each, take 8 where the exact ones take 25.
+// busy as memory (about 60 operations an element, 80 with random rounding of the parameter): the hardware's root and
+// reciprocals, 1 ulp off each, take a third of what the exact ones take.
 template <bool kFast>
 __device__ __forceinline__ void element(const Step& a, const Scalars& s, float g, float& m, float& v, float& r, float& p) {
   m = __builtin_fmaf(m, a.beta1, g * a.alpha1);
@@ -378,14 +383,14 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
       }
       bm = half_max(bm);
       bv = half_max(bv);
-      const bool spoilt = bm >= INFINITE || bv >= INFINITE;
-      if (spoilt) {       // the scales are those of the rest
+      // A block with a value that is not finite, on a branch that no other takes: the scales are those of the rest
+      const bool spoilt = __ballot(bm >= INFINITE || bv >= INFINITE);
+      if (spoilt) {
         bm = bv = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const uint32_t am = __float_as_uint(m[j / 4][j % 4]) & 0x7FFFFFFFu, ar = __float_as_uint(r[j / 4][j % 4]) & 0x7FFFFFFFu;
-          bm = max(bm, am < INFINITE ? am : 0);
-          bv = max(bv, ar < INFINITE ? ar : 0);
+          bm = max(bm, below_infinite(m[j / 4][j % 4]));
+          bv = max(bv, below_infinite(r[j / 4][j % 4]));
         }
         bm = half_max(bm);
         bv = half_max(bv);
@@ -393,20 +398,23 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
       float am = __uint_as_float(bm), av = __uint_as_float(bv);
       am = am < SMALLEST ? 0.f : am;
       av = av < SMALLEST ? 0.f : av;
-      const float fm = am > 0.f ? M_TOP / am : 0.f, fv = av > 0.f ? V_TOP / av : 0.f;
+      const float fm = am > 0.f ? M_TOP * __builtin_amdgcn_rcpf(am) : 0.f;
+      const float fv = av > 0.f ? V_TOP * __builtin_amdgcn_rcpf(av) : 0.f;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         wm[q] = wv[q] = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float mj = m[q][i], rj = r[q][i];
-          uint32_t dm = code_m(mj, fm, random[4 * q + i]), dv = code_v(rj, fv, random[4 * q + i]);
-          if (spoilt) {
-            dm = (__float_as_uint(mj) & 0x7FFFFFFFu) >= INFINITE ? 0x7Fu : dm;
-            dv = (__float_as_uint(rj) & 0x7FFFFFFFu) >= INFINITE ? 255u : dv;
-          }
-          wm[q] |= dm << (8 * i);
-          wv[q] |= dv << (8 * i);
+          wm[q] |= code_m(m[q][i], fm, random[4 * q + i]) << (8 * i);
+          wv[q] |= code_v(r[q][i], fv, random[4 * q + i]) << (8 * i);
+        }
+      }
+      if (spoilt) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int q = j / 4, i = j % 4;
+          if (__float_as_uint(m[q][i]) * 2 >= INFINITE * 2) wm[q] = (wm[q] & ~(0xFFu << (8 * i))) | 0x7Fu << (8 * i);
+          if (__float_as_uint(r[q][i]) * 2 >= INFINITE * 2) wv[q] |= 0xFFu << (8 * i);
         }
       }
       if constexpr (GAP == 4) {
@@ -420,8 +428,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
         }
       }
       if (t % 32 == 0) {
-        st.m_scale[place / BLOCK] = am / M_TOP;
-        st.v_scale[place / BLOCK] = av / V_TOP;
+        st.m_scale[place / BLOCK] = am * (1.f / M_TOP);
+        st.v_scale[place / BLOCK] = av * (1.f / V_TOP);
       }
     } else {
       v4f* fm = reinterpret_cast<v4f*>(static_cast<float*>(st.m) + place);
