@@ -200,17 +200,21 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
     }
     // a lane's sums: token 16 t + m, ranks 16 q + 4 g + i, or (strided) Q (4 g + i) + q
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t) {
+      float* s = sums + (wave * ROWS + 16 * t + m) * RS;
+      if constexpr (kWide) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        float* s = sums + (wave * ROWS + 16 * t + m) * RS;
-        if constexpr (kWide) {
-          *reinterpret_cast<v4f*>(s + 16 * q + 4 * g) = acc[t][q];
-        } else {
+        for (int q = 0; q < Q; ++q) *reinterpret_cast<v4f*>(s + 16 * q + 4 * g) = acc[t][q];
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[Q * (4 * g + i) + q] = acc[t][q][i];
+        for (int k = 0; k < Q; ++k) {       // a lane's 4 Q ranks follow each other
+          v4f v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[t][(4 * k + e) % Q][(4 * k + e) / Q];
+          *reinterpret_cast<v4f*>(s + 4 * Q * g + 4 * k) = v;
         }
       }
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < ROWS * 4 * Q; i += THREADS) {
       const int row = i / (4 * Q), j = 4 * (i % (4 * Q));
@@ -228,17 +232,19 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 // ---------------------------------------------------------------------------------------------------------------
 // Up: out[t][c] = y[t][c] + sum_j u[t][j] F_a[j][c]
 // ---------------------------------------------------------------------------------------------------------------
-// A workgroup: 64 rows, 256 columns at a time.  It holds u in LDS in two bf16 halves; a wave takes 64 columns of all rows, and
-// y's vectors are on their way while it computes.  The order of a tile's columns among MFMA rows is chosen so that a lane ends with 16
-// columns of a row in two pieces of 8, and 4 lanes with 64 bytes in one: y comes and goes in vectors.
-template <typename F, bool kWide, int TR>
+// A workgroup: 64 rows, 256 columns at a time.  It holds u in LDS in two bf16 halves; a wave takes 64 columns of all rows, so
+// that a factor's fragment (in f32 split on its way) serves four tiles, and y's vectors are on their way while it computes.  The
+// order of a tile's columns among MFMA rows is chosen so that a lane ends with 16 columns of a row in two pieces of 8, and 4
+// lanes with 64 bytes in one: y comes and goes in vectors.  (Whole lines at once, 16 lanes to 256 bytes, want the factor's rows
+// 8 apart in a fragment and measured slower: 95 -> 135 us at 3072 x 6144 -> 16384 with rank 64 in f32.)
+template <typename F, bool kWide>
 __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, const uint16_t* y, int C, const F* factor,
-                                                     int64_t one, int held, int passes, int groups, int past, uint16_t* out) {
-  constexpr int WC = TR;                // waves side by side: 64 columns each; 4 / WC below one another, 16 TR rows each
+                                                     int64_t one, int held, int passes, int groups, uint16_t* out) {
+  constexpr int TR = 4;                 // tiles of 16 rows
   extern __shared__ uint16_t halves[];  // u in two halves of ROWS x RS
   const int RS = held + 8;              // 16 bytes off the banks' turn
   uint16_t *hi = halves, *lo = halves + ROWS * RS;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16, r0 = wave / WC * 16 * TR;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
   // a row's columns on neighbouring workgroups
   const int row0 = blockIdx.x / groups * ROWS, first = blockIdx.x % groups * passes;
   const int id = adapter_of(rows, row0 + lane);
@@ -250,14 +256,14 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
     const int r = rank_of(rows, a);
     const F* f = factor + (int64_t)max(a, 0) * one;
     for (int p = 0; p < passes; ++p) {
-      const int c0 = ((first + p) * WC + wave % WC) * 64;
+      const int c0 = (first + p) * 256 + 64 * wave;
       const bool in = c0 < C;
       v4u old[TR][2] = {};
       if (y && in) {
 #pragma unroll
         for (int t = 0; t < TR; ++t) {
-          if (!(mask >> (r0 + 16 * t + m) & 1)) continue;
-          const uint16_t* b = y + (int64_t)(row0 + r0 + 16 * t + m) * C + c0 + 8 * g;
+          if (!(mask >> (16 * t + m) & 1)) continue;
+          const uint16_t* b = y + (int64_t)(row0 + 16 * t + m) * C + c0 + 8 * g;
 #pragma unroll
           for (int h = 0; h < 2; ++h) old[t][h] = *reinterpret_cast<const v4u*>(b + 32 * h);
         }
@@ -308,7 +314,7 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
             }
 #pragma unroll
             for (int t = 0; t < TR; ++t) {
-              const int at = (r0 + 16 * t + m) * RS + j + 8 * g;
+              const int at = (16 * t + m) * RS + j + 8 * g;
               const v8bf uh = *reinterpret_cast<const v8bf*>(hi + at), ul = *reinterpret_cast<const v8bf*>(lo + at);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
@@ -324,8 +330,8 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
       // a lane: row 16 t + m, columns 32 h + 8 g + e
 #pragma unroll
       for (int t = 0; t < TR; ++t) {
-        if (!(mask >> (r0 + 16 * t + m) & 1)) continue;
-        uint16_t* to = out + (int64_t)(row0 + r0 + 16 * t + m) * C + c0 + 8 * g;
+        if (!(mask >> (16 * t + m) & 1)) continue;
+        uint16_t* to = out + (int64_t)(row0 + 16 * t + m) * C + c0 + 8 * g;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const v4u b = old[t][h];
@@ -342,8 +348,7 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
             }
             o[i] = pack_bf16x2(v[0], v[1]);
           }
-          if (past) __builtin_nontemporal_store(o, reinterpret_cast<v4u*>(to + 32 * h));
-          else *reinterpret_cast<v4u*>(to + 32 * h) = o;
+          *reinterpret_cast<v4u*>(to + 32 * h) = o;
         }
       }
     }
@@ -517,7 +522,7 @@ struct Plan {
 };
 
 constexpr int PLAN = 1024;            // threads: one an adapter
-constexpr int AHEAD = 16;             // ids of a lane
+constexpr int HELD = 32768;           // ids in LDS: both passes over 16896 ids 29 -> 10 us
 
 // Inclusive sums of three values over the workgroup's threads; waves: 3 x 16 in LDS.
 __device__ __forceinline__ void scan(int (&v)[3], int32_t* waves) {
@@ -542,32 +547,27 @@ __device__ __forceinline__ void scan(int (&v)[3], int32_t* waves) {
 
 // One workgroup: every wave counts a run of ids, then places it; no atomics, so the order is the batch's.
 __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chunk, Plan plan) {
-  extern __shared__ int32_t lds[];      // 16 waves x count, then 48
+  extern __shared__ int32_t lds[];      // 16 waves x count, then 48, then as many ids as fit
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = rows.count;
   int32_t* mine = lds + wave * n;
+  int16_t* held = reinterpret_cast<int16_t*>(lds + 16 * n + 48);
+  const int most = min(ids, HELD);
   for (int i = threadIdx.x; i < 16 * n; i += PLAN) lds[i] = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < most; i += PLAN) held[i] = (int16_t)adapter_of(rows, i * rows.per);
   __syncthreads();
   const int run = (ids + 15) / 16, begin = min(ids, wave * run), end = min(ids, begin + run);
   for (int pass = 0; pass < 2; ++pass) {
-    for (int i0 = begin; i0 < end; i0 += 64 * AHEAD) {
-      int some[AHEAD];        // on their way together
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int i = i0 + 64 * k + lane;
-        some[k] = i < end ? adapter_of(rows, i * rows.per) : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int id = some[k];
-        uint64_t left = __ballot(id >= 0);
-        while (left) {
-          const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-          const uint64_t mask = __ballot(id == a);
-          left &= ~mask;
-          const int at = mine[a];
-          if (pass && id == a) plan.order[at + __popcll(mask & ((uint64_t(1) << lane) - 1))] = i0 + 64 * k + lane;
-          if (lane == 0) mine[a] = at + __popcll(mask);
-        }
+    for (int i0 = begin; i0 < end; i0 += 64) {
+      const int i = i0 + lane, id = i >= end ? -1 : i < most ? held[i] : adapter_of(rows, i * rows.per);
+      uint64_t left = __ballot(id >= 0);
+      while (left) {
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const uint64_t mask = __ballot(id == a);
+        left &= ~mask;
+        const int at = mine[a];
+        if (pass && id == a) plan.order[at + __popcll(mask & ((uint64_t(1) << lane) - 1))] = i;
+        if (lane == 0) mine[a] = at + __popcll(mask);
       }
     }
     __syncthreads();
@@ -652,7 +652,7 @@ __global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int64_t of = __shfl(row, 8 * g + e);
-        xv[e] = *reinterpret_cast<const v4u*>(x + of * C);
+        xv[e] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(x + of * C));      // read no more
         const bool live = some && b + 8 * g + e < it.end;
         if constexpr (Q == 1) {
           pv[0][e] = live ? p[of * rows.R] : 0.f;
@@ -802,19 +802,19 @@ void launch_down(const Rows& rows, const uint16_t* x, int64_t C, const void* f, 
   else go(down_kernel<F, kWide, 4>, once[2]);
 }
 
-// past: the output goes past the last-level cache (256 MB), which what the call reads next fills.
+// Passes over 256 columns with one staging of u: two (four where the factor's rows are long and its loads wider), fewer
+// where a CU would not get six workgroups.  4 x 4608 rows x 6144 at 1 / 2 / 4 passes 182 / 172 / 177 us, 16896 x 16384 (dx, with
+// the factors' sums) 432 / 409 / 396.
 template <typename F, bool kWide>
-void launch_up(const Rows& rows, const float* u, const uint16_t* y, int64_t C, const void* f, uint16_t* out, bool past,
+void launch_up(const Rows& rows, const float* u, const uint16_t* y, int64_t C, const void* f, uint16_t* out,
                hipStream_t st) {
-  constexpr int TR = kF32<F> && !kWide ? 4 : 2;
-  const int64_t tiles = (rows.T + ROWS - 1) / ROWS, blocks = (C + 64 * TR - 1) / (64 * TR);
+  const int64_t tiles = (rows.T + ROWS - 1) / ROWS, blocks = (C + 255) / 256, most = kWide ? 4 : 2;
   int64_t passes = tiles * blocks / (6 * (int64_t)k2q_cu_count());
-  passes = passes < 1 ? 1 : passes > 4 ? 4 : passes;
+  passes = passes < 1 ? 1 : passes > most ? most : passes;
   const int64_t groups = (blocks + passes - 1) / passes;
   const int held = rows.R < RANKS ? (rows.R + 31) & ~31 : RANKS;
-  hipLaunchKernelGGL((up_kernel<F, kWide, TR>), dim3((unsigned)(tiles * groups)), dim3(THREADS), 2 * ROWS * (held + 8) * 2,
-                     st, rows, u, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups,
-                     (int)past, out);
+  hipLaunchKernelGGL((up_kernel<F, kWide>), dim3((unsigned)(tiles * groups)), dim3(THREADS), 2 * ROWS * (held + 8) * 2, st,
+                     rows, u, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups, out);
 }
 
 void launch_join(const Rows& rows, const float* part, int slices, float* sum, hipStream_t st) {
@@ -858,10 +858,10 @@ struct Sums {
   int64_t plan_bytes;
 };
 
-// Rows of a piece: all pieces together give every CU four workgroups, and a piece 256 rows or more.
+// Rows of a piece: all pieces together give every CU two workgroups, and a piece 256 rows or more.
 Sums sums_plan(const k2q_bank* b, int64_t T, int64_t per) {
   const int64_t blocks = ((b->K + COLS - 1) / COLS + (b->N + COLS - 1) / COLS) * ((b->R + 16 * tiles_of(b->R) - 1) / (16 * tiles_of(b->R)));
-  const int64_t want = (4 * (int64_t)k2q_cu_count() + blocks - 1) / blocks;
+  const int64_t want = (2 * (int64_t)k2q_cu_count() + blocks - 1) / blocks;
   int64_t chunk = ((T + want - 1) / want + 127) / 128 * 128;
   chunk = chunk < 256 ? 256 : chunk;
   const int64_t whole = T / chunk;
@@ -892,15 +892,14 @@ extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   }
   const int slices = down_slices(T, b->K, b->R);
   if (!u) u = part;       // the first slice's place
-  const bool past = T * b->N * 4 > (int64_t)256 << 20;
   if (b->dtype == K2Q_DTYPE_F32) {
     launch_down<float, true>(rows, x, b->K, b->A, slices, slices == 1 ? u : part, st);
     launch_join(rows, part, slices, u, st);
-    launch_up<float, false>(rows, u, y, b->N, b->B, out, past, st);
+    launch_up<float, false>(rows, u, y, b->N, b->B, out, st);
   } else {
     launch_down<uint16_t, true>(rows, x, b->K, b->A, slices, slices == 1 ? u : part, st);
     launch_join(rows, part, slices, u, st);
-    launch_up<uint16_t, false>(rows, u, y, b->N, b->B, out, past, st);
+    launch_up<uint16_t, false>(rows, u, y, b->N, b->B, out, st);
   }
   return k2q_launch_status();
 }
@@ -935,9 +934,8 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   // dx last: dy is still in the last-level cache for dB, and what dx would push out of it is read no more
   auto input = [&] {
     if (!dx) return k2q_launch_status();
-    const bool past = T * (2 * b->K + b->N) * 2 > (int64_t)256 << 20;
-    if (f32) launch_up<float, true>(rows, g, base, b->K, b->A, dx, past, st);
-    else launch_up<uint16_t, true>(rows, g, base, b->K, b->A, dx, past, st);
+    if (f32) launch_up<float, true>(rows, g, base, b->K, b->A, dx, st);
+    else launch_up<uint16_t, true>(rows, g, base, b->K, b->A, dx, st);
     return k2q_launch_status();
   };
   if (!dA && !dB) return input();
@@ -950,9 +948,9 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   plan.first = plan.start + n + 1;
   plan.order = plan.head + up16(1 + 2 * (n + 1));
   float* pieces = reinterpret_cast<float*>(plan.order + up16(ids));
-  const int lds = (16 * n + 48) * 4;
+  const int lds = (16 * n + 48) * 4 + 2 * (int)(ids < HELD ? up16(ids) : HELD);
   static std::atomic<uint64_t> once;
-  int rl = k2q_lds_limit_once(plan_kernel, (16 * K2Q_MAX_ADAPTERS + 48) * 4, once);
+  int rl = k2q_lds_limit_once(plan_kernel, (16 * K2Q_MAX_ADAPTERS + 48) * 4 + 2 * HELD, once);
   if (rl != K2Q_OK) return rl;
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(PLAN), lds, st, rows, ids, (int)s.chunk, plan);
   Jobs jobs{};
