@@ -32,13 +32,13 @@ struct Rows {
   int32_t R;                // rank of the bank's storage
 };
 
-// The adapter of a row: -1 for none, and for numbers that are no adapter's.
-__device__ __forceinline__ int adapter_of(const Rows& a, int row) {
-  if (row >= a.T) return -2;
-  const int i = row / a.per;
+// The adapter of an id: -1 for none, and for numbers that are no adapter's.
+__device__ __forceinline__ int adapter_at(const Rows& a, int i) {
   const int64_t id = a.wide ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
   return id < 0 || id >= a.count ? -1 : (int)id;
 }
+
+__device__ __forceinline__ int adapter_of(const Rows& a, int row) { return row >= a.T ? -2 : adapter_at(a, row / a.per); }
 
 // Ranks of an adapter that hold something, in whole MFMA tiles.
 __device__ __forceinline__ int rank_of(const Rows& a, int id) {
@@ -553,13 +553,23 @@ __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chun
   int16_t* held = reinterpret_cast<int16_t*>(lds + 16 * n + 48);
   const int most = min(ids, HELD);
   for (int i = threadIdx.x; i < 16 * n; i += PLAN) lds[i] = 0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < most; i += PLAN) held[i] = (int16_t)adapter_of(rows, i * rows.per);
+  auto hold = [&](auto* p) {        // a branch on the type inside would wait for each load by itself: 20 us at 16896 ids
+    for (int i0 = threadIdx.x; i0 < most; i0 += 8 * PLAN) {
+      int64_t id[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) id[k] = p[min(i0 + k * PLAN, most - 1)];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i0 + k * PLAN < most) held[i0 + k * PLAN] = (int16_t)(id[k] < 0 || id[k] >= n ? -1 : id[k]);
+    }
+  };
+  if (rows.wide) hold(static_cast<const int64_t*>(rows.ids));
+  else hold(static_cast<const int32_t*>(rows.ids));
   __syncthreads();
   const int run = (ids + 15) / 16, begin = min(ids, wave * run), end = min(ids, begin + run);
   for (int pass = 0; pass < 2; ++pass) {
     for (int i0 = begin; i0 < end; i0 += 64) {
-      const int i = i0 + lane, id = i >= end ? -1 : i < most ? held[i] : adapter_of(rows, i * rows.per);
+      const int i = i0 + lane, id = i >= end ? -1 : i < most ? held[i] : adapter_at(rows, i);
       uint64_t left = __ballot(id >= 0);
       while (left) {
         const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
@@ -775,12 +785,17 @@ Rows rows_of(const k2q_bank* b, int64_t T, int64_t per) {
 
 int tiles_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 
-// Slices of a "down" over C columns: as many as give every CU four workgroups, of 256 columns or more.
+// Slices of a "down" over C columns: up to 16 workgroups a CU, so that the last ones end together, of 1024 columns or more (a
+// workgroup's sums in LDS cost as much as 500 columns); where that leaves fewer than two a CU, slices down to 256 columns.
+// 16896 x 16384, rank 16, us at 1 / 3 / 5 / 10 / 16 slices (with the "up") 337 / 265 / 258 / 248 / 244; 18432 x 6144, rank 32
+// 191 / 177 / 170 / 172 / 177; 1000 x 2560 at 1 / 3 / 5 / 10 58 / 37 / 30 / 26.
 int down_slices(int64_t T, int64_t C, int64_t R) {
   const int64_t groups = ((T + ROWS - 1) / ROWS) * ((R + 16 * tiles_of(R) - 1) / (16 * tiles_of(R)));
-  int64_t s = (4 * (int64_t)k2q_cu_count() + groups - 1) / groups;
-  const int64_t most = (C + 255) / 256;
-  s = s > most ? most : s;
+  const int64_t cus = k2q_cu_count(), large = C / 1024, most = (C + 255) / 256;
+  int64_t s = 16 * cus / groups;
+  s = s > large ? large : s;
+  if (groups * s < 2 * cus) s = (2 * cus + groups - 1) / groups;
+  s = s > most ? most : s < 1 ? 1 : s;
   const int64_t cols = ((C + s - 1) / s + 255) / 256 * 256;
   return (int)((C + cols - 1) / cols);
 }
