@@ -40,6 +40,28 @@ class _AddAdaptersFn(torch.autograd.Function):
         return (dy if need[0] else None, *grads, None, None, None, None)
 
 
+class _BankLinearFn(torch.autograd.Function):
+    """``add_adapters`` over the output of a frozen quantized base, as one node: the base's input gradient is what the adapters'
+    is added to, in place (autograd would make both tensors, and a third)."""
+
+    @staticmethod
+    def forward(ctx, x, A, B, ids, scales, ranks, scale, base):
+        out, u = _lib.bank_fwd(_rows(base(x)), x, A, B, ids, scales, ranks, scale, ctx.needs_input_grad[2])
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, u, A, B, ids, scales, ranks)
+        ctx.scale, ctx.base = scale, base
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, u, A, B, ids, scales, ranks = ctx.saved_tensors
+        need = ctx.needs_input_grad[:3]
+        d, dx = _rows(dy), None
+        if need[0]:
+            dx = ctx.base.input_grad(d.view(-1, d.shape[-1])).view(*d.shape[:-1], -1)
+        return (*_lib.bank_bwd(d, x, u, A, B, ids, scales, ranks, ctx.scale, dx, *need), None, None, None, None, None)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous, 16-byte aligned and in bf16 (itself when it is that)."""
     if t.dtype != torch.bfloat16:
@@ -142,11 +164,16 @@ class LoRABank(nn.Module):
         return f"count={self.count}, rank={self.rank}"
 
     def forward(self, x: torch.Tensor, adapters: torch.Tensor | None = None) -> torch.Tensor:
-        ids = self.adapters if adapters is None else adapters
-        y = self.base(x)
+        ids, base = self.adapters if adapters is None else adapters, self.base
         if ids is None or self.scale_mul == 0.0:
-            return y
-        return add_adapters(y, x, self.lora_A, self.lora_B, ids, self.scales, self.ranks, self.scale_mul)
+            return base(x)
+        A, B = self.lora_A, self.lora_B
+        grad = torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad)
+        if (grad and isinstance(base, _lora._HIP_BASES) and "_k2q_group" not in base.__dict__ and not _lib.observed()
+                and x.dtype == torch.bfloat16 and x.dim() > 1 and x.numel()):
+            return _BankLinearFn.apply(_rows(x), A.contiguous(), B.contiguous(), ids.contiguous(), self.scales, self.ranks,
+                                       float(self.scale_mul), base)
+        return add_adapters(base(x), x, A, B, ids, self.scales, self.ranks, self.scale_mul)
 
 
 _lora._SCALED += (LoRABank,)
@@ -155,7 +182,8 @@ _lora._SCALED += (LoRABank,)
 @contextlib.contextmanager
 def lora_requests(model: nn.Module, adapters: torch.Tensor | None):
     """Within the ``with`` body the rows of every bank's input in ``model`` use the adapters of ``adapters``: one number for
-    each entry of the input's first dimension (the requests of a batch), or of its first dimensions; None: the base alone."""
+    each entry of the input's first dimension (the requests of a batch), or of its first dimensions; None: the base alone.
+    A checkpointed forward runs again in its backward pass: keep that inside the body too."""
     banks = [m for m in model.modules() if isinstance(m, LoRABank)]
     saved = [m.adapters for m in banks]
     for m in banks:

@@ -305,6 +305,10 @@ class ConvRotLinear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.forward_lora(x, None, None, 0.0)
 
+    def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
+        """The gradient of the layer's input, (rows, in) bf16, from that of its output (contiguous (rows, out) bf16)."""
+        return _lib.gemm_dx(dy, self.qweight, self.weight_scale, w4=self.mode == "w4a8", wt=self.dx_weight())
+
 
 def quantize_dit_convrot(dit, mode: str = "w8a8") -> int:
     """Replace the transformer blocks' ``nn.Linear`` with :class:`ConvRotLinear` in place.
@@ -478,6 +482,10 @@ class Fp8Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.forward_lora(x, None, None, 0.0)
+
+    def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
+        """The gradient of the layer's input, (rows, in) bf16, from that of its output (contiguous (rows, out) bf16)."""
+        return _lib.gemm_dx_fp8(dy, self.weight_fp8, self.scale.to(torch.bfloat16).contiguous())
 
 
 def quantize_dit_fp8(dit) -> int:
