@@ -6,8 +6,8 @@
 // Two forms of product make all of it.  "Down" reduces wide rows to an adapter's rank (u from x and A, g from dy and B),
 // "up" widens them again and adds (out from u and B, dx from g and A); each takes its factor with the wide index contiguous
 // (A) or the rank contiguous (B).  The third form, "sums", reduces over an adapter's rows (dA from g and x, dB from u and
-// dy).  All run on 16x16x32 bf16 MFMAs with f32 sums: what is in f32 (factors, u, g) goes in as its bf16 rounding and the
-// rounding of the rest, 2^-17 of it, so a product is that of 16 bits of each; y, x, dy are bf16 as they are.
+// dy).  All run on 16x16x32 bf16 MFMAs with f32 sums: what is in f32 (factors, u, g) goes in as two bf16 parts, or three on the
+// way to a gradient in f32; y, x, dy are bf16 as they are.
 //
 // Rows may come in any order.  A tile of 64 rows goes over the adapters that it finds in it, one after another: rows of one
 // request lie together, so that is one adapter, or two, in all but the smallest batches.
@@ -50,19 +50,31 @@ __device__ __forceinline__ int rank_of(const Rows& a, int id) {
 
 __device__ __forceinline__ float scale_of(const Rows& a, int id) { return a.scales ? a.mul * a.scales[id] : a.mul; }
 
-// 8 values as bf16 and, where they are f32, the bf16 of what that leaves.
-struct Split {
-  v8bf hi, lo;
+// 8 values in f32 as N bf16 parts: their rounding, that of the rest, that of the rest's rest.  Two are 2^-17 of a value off at
+// most, for products that end in bf16; three hold all 24 bits, for gradients that end in f32.
+template <int N>
+struct Parts {
+  v8bf p[N];
 };
 
-__device__ __forceinline__ Split split(const float (&v)[8]) {
-  v4u h, l;
+template <int N>
+__device__ __forceinline__ Parts<N> split(const float (&v)[8]) {
+  Parts<N> s;
+  float r[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    h[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    l[i] = pack_bf16x2(v[2 * i] - __uint_as_float(h[i] << 16), v[2 * i + 1] - __uint_as_float(h[i] & 0xffff0000u));
+  for (int i = 0; i < 8; ++i) r[i] = v[i];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    v4u h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      r[2 * i] -= __uint_as_float(h[i] << 16);
+      r[2 * i + 1] -= __uint_as_float(h[i] & 0xffff0000u);
+    }
+    s.p[n] = __builtin_bit_cast(v8bf, h);
   }
-  return {__builtin_bit_cast(v8bf, h), __builtin_bit_cast(v8bf, l)};
+  return s;
 }
 
 __device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -70,15 +82,15 @@ __device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) { return __builtin_am
 template <typename F>
 constexpr bool kF32 = sizeof(F) == 4;
 
-// Fragments of a factor for one MFMA step of 32: Q tiles, a lane's 8 values of the reduction each.
-template <typename F, int Q>
+// Fragments of a factor for one MFMA step of 32: Q tiles, a lane's 8 values of the reduction each, in N parts (1: bf16).
+template <typename F, int Q, int N>
 struct Frag {
-  v8bf hi[Q], lo[Q];      // lo: f32 factors alone
+  v8bf p[N][Q];
 };
 
 // Reduction contiguous: value e of tile q is p[q * tile + e].
-template <typename F, int Q>
-__device__ __forceinline__ void load_contiguous(const F* p, int64_t tile, const bool (&ok)[Q], Frag<F, Q>& f) {
+template <typename F, int Q, int N>
+__device__ __forceinline__ void load_contiguous(const F* p, int64_t tile, const bool (&ok)[Q], Frag<F, Q, N>& f) {
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     if constexpr (kF32<F>) {
@@ -88,20 +100,20 @@ __device__ __forceinline__ void load_contiguous(const F* p, int64_t tile, const 
         b = *reinterpret_cast<const v4f*>(p + q * tile + 4);
       }
       const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      const Split s = split(v);
-      f.hi[q] = s.hi;
-      f.lo[q] = s.lo;
+      const Parts<N> s = split<N>(v);
+#pragma unroll
+      for (int n = 0; n < N; ++n) f.p[n][q] = s.p[n];
     } else {
       v4u a = {0, 0, 0, 0};
       if (ok[q]) a = *reinterpret_cast<const v4u*>(p + q * tile);
-      f.hi[q] = __builtin_bit_cast(v8bf, a);
+      f.p[0][q] = __builtin_bit_cast(v8bf, a);
     }
   }
 }
 
 // Reduction strided: value e of tile q is p[e * step + q], so that Q tiles come with one vector load a value.
-template <typename F, int Q>
-__device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, Frag<F, Q>& f) {
+template <typename F, int Q, int N>
+__device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, Frag<F, Q, N>& f) {
   typedef F VecT __attribute__((ext_vector_type(Q > 1 ? Q : 2)));
   if constexpr (kF32<F>) {
     float v[Q][8];
@@ -118,9 +130,9 @@ __device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, 
     }
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const Split s = split(v[q]);
-      f.hi[q] = s.hi;
-      f.lo[q] = s.lo;
+      const Parts<N> s = split<N>(v[q]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) f.p[n][q] = s.p[n];
     }
   } else {
     typedef uint16_t VecU __attribute__((ext_vector_type(Q > 1 ? Q : 2)));
@@ -141,7 +153,7 @@ __device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, 
       v4u w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = v[q][2 * i] | v[q][2 * i + 1] << 16;
-      f.hi[q] = __builtin_bit_cast(v8bf, w);
+      f.p[0][q] = __builtin_bit_cast(v8bf, w);
     }
   }
 }
@@ -155,6 +167,7 @@ template <typename F, bool kWide, int Q>
 __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
                                                        int slice_cols, float* part) {
   constexpr int RS = 16 * Q + 4;        // a row of sums in LDS
+  constexpr int N = kF32<F> ? 3 : 1;    // u and g go into gradients in f32, and a served row has a trained one's bits
   extern __shared__ float sums[];       // 4 waves x 64 rows x RS
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
   const int row0 = blockIdx.x * ROWS, j0 = blockIdx.z * 16 * Q;
@@ -186,16 +199,15 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c = c0 + 32 * h + 8 * g;
-        Frag<F, Q> fr;
-        if constexpr (kWide) load_contiguous<F, Q>(f + (int64_t)(j0 + m) * C + c, 16 * (int64_t)C, ok, fr);
-        else load_strided<F, Q>(f + (int64_t)c * rows.R + j0 + Q * m, rows.R, some, fr);
+        Frag<F, Q, N> fr;
+        if constexpr (kWide) load_contiguous<F, Q, N>(f + (int64_t)(j0 + m) * C + c, 16 * (int64_t)C, ok, fr);
+        else load_strided<F, Q, N>(f + (int64_t)c * rows.R + j0 + Q * m, rows.R, some, fr);
 #pragma unroll
         for (int q = 0; q < Q; ++q)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            acc[t][q] = mfma(fr.hi[q], xv[h][t], acc[t][q]);
-            if constexpr (kF32<F>) acc[t][q] = mfma(fr.lo[q], xv[h][t], acc[t][q]);
-          }
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int n = 0; n < N; ++n) acc[t][q] = mfma(fr.p[n][q], xv[h][t], acc[t][q]);
       }
     }
     // a lane's sums: token 16 t + m, ranks 16 q + 4 g + i, or (strided) Q (4 g + i) + q
@@ -285,32 +297,32 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
                 v[e + 4] = c[e];
               }
             }
-            const Split s = split(v);
-            *reinterpret_cast<v8bf*>(hi + row * RS + j) = s.hi;
-            *reinterpret_cast<v8bf*>(lo + row * RS + j) = s.lo;
+            const Parts<2> s = split<2>(v);
+            *reinterpret_cast<v8bf*>(hi + row * RS + j) = s.p[0];
+            *reinterpret_cast<v8bf*>(lo + row * RS + j) = s.p[1];
           }
           __syncthreads();
         }
         if (in) {
           for (int j = 0; j < n; j += 32) {
-            Frag<F, 4> fr;
+            constexpr int N = kF32<F> ? 2 : 1;
+            Frag<F, 4, N> fr;
             const bool some = j + 8 * g < n;
             if constexpr (kWide) {
               // MFMA row m of tile q: column 32 (m / 2 % 2) + 8 (m / 4) + 4 (m % 2) + q, four tiles with one load
               const int col = 32 * (m % 4 / 2) + 8 * (m / 4) + 4 * (m % 2);
-              load_strided<F, 4>(f + (int64_t)(j0 + j + 8 * g) * C + c0 + col, C, some, fr);
+              load_strided<F, 4, N>(f + (int64_t)(j0 + j + 8 * g) * C + c0 + col, C, some, fr);
             } else {
               // row m of tile q: column 32 (q / 2) + 8 (m / 4) + 4 (q % 2) + m % 4
               const bool ok[2] = {some, some};
               const F* b = f + (int64_t)(c0 + 8 * (m / 4) + m % 4) * rows.R + j0 + j + 8 * g;
-              Frag<F, 2> half[2];
-              load_contiguous<F, 2>(b, 4 * (int64_t)rows.R, ok, half[0]);
-              load_contiguous<F, 2>(b + 32 * (int64_t)rows.R, 4 * (int64_t)rows.R, ok, half[1]);
+              Frag<F, 2, N> half[2];
+              load_contiguous<F, 2, N>(b, 4 * (int64_t)rows.R, ok, half[0]);
+              load_contiguous<F, 2, N>(b + 32 * (int64_t)rows.R, 4 * (int64_t)rows.R, ok, half[1]);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                fr.hi[q] = half[q / 2].hi[q % 2];
-                if constexpr (kF32<F>) fr.lo[q] = half[q / 2].lo[q % 2];
-              }
+              for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int k = 0; k < N; ++k) fr.p[k][q] = half[q / 2].p[k][q % 2];
             }
 #pragma unroll
             for (int t = 0; t < TR; ++t) {
@@ -318,9 +330,9 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
               const v8bf uh = *reinterpret_cast<const v8bf*>(hi + at), ul = *reinterpret_cast<const v8bf*>(lo + at);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                acc[t][q] = mfma(fr.hi[q], uh, acc[t][q]);
-                acc[t][q] = mfma(fr.hi[q], ul, acc[t][q]);
-                if constexpr (kF32<F>) acc[t][q] = mfma(fr.lo[q], uh, acc[t][q]);
+                acc[t][q] = mfma(fr.p[0][q], uh, acc[t][q]);
+                acc[t][q] = mfma(fr.p[0][q], ul, acc[t][q]);
+                if constexpr (N > 1) acc[t][q] = mfma(fr.p[1][q], uh, acc[t][q]);
               }
             }
           }
@@ -673,9 +685,10 @@ __global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, 
           for (int k = 0; k < Q; ++k) pv[k][e] = t[k];
         }
       }
-      Split ps[Q];
+      constexpr int N = kF32<F> ? 3 : 2;
+      Parts<N> ps[Q];
 #pragma unroll
-      for (int k = 0; k < Q; ++k) ps[k] = split(pv[k]);
+      for (int k = 0; k < Q; ++k) ps[k] = split<N>(pv[k]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         v4u w;
@@ -684,10 +697,9 @@ __global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, 
           w[i] = __builtin_amdgcn_perm(xv[2 * i + 1][k / 2], xv[2 * i][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
         const v8bf xf = __builtin_bit_cast(v8bf, w);
 #pragma unroll
-        for (int t = 0; t < Q; ++t) {
-          acc[k][t] = mfma(xf, ps[t].hi, acc[k][t]);
-          acc[k][t] = mfma(xf, ps[t].lo, acc[k][t]);
-        }
+        for (int t = 0; t < Q; ++t)
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[k][t] = mfma(xf, ps[t].p[n], acc[k][t]);
       }
     }
   // a lane: columns 8 (4 g + i) + k, ranks Q m + t.  Half of the columns (k below 4, then the rest) of all waves meet in LDS,
