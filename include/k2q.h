@@ -406,7 +406,7 @@ int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, int64_t M, i
  *   dA_a = sum_t g[t]^T x[t] and dB_a = sum_t dy[t]^T u[t] over the adapter's rows, in the factors' type, zeros for an adapter
  *   without rows and for ranks past its own.  dx, dA (with x), dB (with u) are nullable; one at least is given.
  * x T x K, y, out and dy T x N, dx T x K: bf16, contiguous.  Sums are f32 in a fixed order; f32 factors, u and g enter the
- * products in 16 bits of precision.  K and N multiples of 64, R of 16, count <= K2Q_MAX_ADAPTERS, T < 2^31 - 256.
+ * products in 16 bits of precision where the result is bf16, in 24 where it is f32.  K and N multiples of 64, R of 16, count <= K2Q_MAX_ADAPTERS, T < 2^31 - 256.
  * ws: *_ws_bytes bytes, 16-byte aligned (need_factors: dA or dB is given). */
 #define K2Q_MAX_ADAPTERS 1024
 typedef struct {
@@ -433,7 +433,7 @@ int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* dy, 
  * of type dtype (bf16, f32, f16), g their gradients in the same type; read before the call returns.
  * k2q_grad_norm: out[0] = the 2-norm over all gradients (sums in f64, in a fixed order), out[1] = min(1, max_norm /
  * (norm + 1e-6)); ws holds the partial sums of squares, k2q_grad_norm_ws_bytes / 8 of them, and with out NULL that is all.
- * k2q_scale_grads: every gradient times by[0], rounded once.
+ * scale != 0: every gradient (no memory twice) is multiplied by out[1], rounded once.
  * k2q_adamw: steps[index] += 1 (= T), and with g the gradient, times the factor of the norm that n_squares partial sums
  * (nullable: no factor) give with max_norm, both written to norm[0] and norm[1],
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
@@ -459,9 +459,8 @@ typedef struct {
   int32_t dtype;
 } k2q_step_tensor;
 int64_t k2q_grad_norm_ws_bytes(const k2q_step_tensor* t, int64_t count);
-int k2q_grad_norm(const k2q_step_tensor* t, int64_t count, double max_norm, void* ws, int64_t ws_bytes, float* out,
+int k2q_grad_norm(const k2q_step_tensor* t, int64_t count, double max_norm, void* ws, int64_t ws_bytes, float* out, int scale,
                   void* stream);
-int k2q_scale_grads(const k2q_step_tensor* t, int64_t count, const float* by, void* stream);
 int64_t k2q_adamw_ws_bytes(int64_t count);
 int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits, void* exp_avg, void* exp_avg_sq, float* avg_scale,
               float* sq_scale, float* steps, double lr, const float* lr_of, double beta1, double beta2, double eps,

@@ -136,8 +136,7 @@ _SIGNATURES = {
     "k2q_bank_bwd_ws_bytes": ([_p, _i64, _i64, _int], _i64),
     "k2q_bank_bwd": ([_p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p], _int),
     "k2q_grad_norm_ws_bytes": ([_p, _i64], _i64),
-    "k2q_grad_norm": ([_p, _i64, _f64, _p, _i64, _p, _p], _int),
-    "k2q_scale_grads": ([_p, _i64, _p, _p], _int),
+    "k2q_grad_norm": ([_p, _i64, _f64, _p, _i64, _p, _int, _p], _int),
     "k2q_adamw_ws_bytes": ([_i64], _i64),
     "k2q_adamw": ([_p, _i64, _int, _p, _p, _p, _p, _p, _f64, _p, _f64, _f64, _f64, _f64, _p, _i64, _f64, _p, _int,
                    ctypes.c_uint32, _p, _i64, _p], _int),
@@ -1478,16 +1477,18 @@ def _check_adamw(params, starts, exp_avg, steps, stochastic) -> None:
 
 
 def adamw(params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale, sq_scale, steps, lr, lr_of, beta1, beta2, eps,
-          weight_decay, squares, max_norm, norm, stochastic, seed) -> None:
+          weight_decay, squares, max_norm, norm, stochastic, seed):
     """A step (``k2q_adamw``) of the parameters that have a gradient; ``starts`` are the places of all of them in the
-    moments' flat buffers.  With ``squares`` (:func:`grad_norm`'s) gradients are brought to ``max_norm`` at most, and ``norm``
-    receives the norm and the factor."""
+    moments' flat buffers.  With ``max_norm`` gradients are brought to that norm at most: that of ``squares``
+    (:func:`grad_norm`'s, ``norm`` receives it and the factor), or without it of these parameters' gradients.  Returns the
+    norm and the factor, or None."""
     args = (params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale, sq_scale, steps, lr, lr_of, beta1, beta2, eps,
             weight_decay, squares, max_norm, norm, stochastic, seed)
     r = _fast().adamw(*args)
     if r.__class__ is not tuple:
-        _refused(r, "k2q_adamw", lambda: _native.adamw(*args),
-                 lambda: _check_adamw(params, starts, exp_avg, steps, stochastic))
+        r = _refused(r, "k2q_adamw", lambda: _native.adamw(*args),
+                     lambda: _check_adamw(params, starts, exp_avg, steps, stochastic))
+    return r[0] if r else None
 
 
 def moments(exp_avg, avg_scale, exp_avg_sq, sq_scale, dtype):
@@ -1547,11 +1548,19 @@ def _check_bank_fwd(y, x, A, B, ids, scales, ranks) -> None:
     check_bank(y, B.shape[1], A, B, ids, scales, ranks)
 
 
+def bank_native(*args):
+    """:func:`bank_fwd` where the native wrapper takes the arguments as they are, else None."""
+    r = _fast().bank_fwd(*args)
+    if r.__class__ is int:
+        _check(r, "k2q_bank_fwd")
+    return r
+
+
 def bank_fwd(y, x, A, B, ids, scales, ranks, scale: float, need_u: bool):
     """``(out, u | None)`` of :func:`add_adapters` (``k2q_bank_fwd``)."""
     args = (y, x, A, B, ids, scales, ranks, scale, need_u)
-    r = _fast().bank_fwd(*args)
-    return r if r.__class__ is tuple else _refused(r, "k2q_bank_fwd", lambda: _native.bank_fwd(*args),
+    r = bank_native(*args)
+    return r if r is not None else _refused(r, "k2q_bank_fwd", lambda: _native.bank_fwd(*args),
                                                    lambda: _check_bank_fwd(*args[:7]))
 
 

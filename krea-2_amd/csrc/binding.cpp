@@ -45,7 +45,6 @@ struct Api {
   decltype(&k2q_capture_id) capture_id;
   decltype(&k2q_grad_norm) grad_norm;
   decltype(&k2q_grad_norm_ws_bytes) grad_norm_ws_bytes;
-  decltype(&k2q_scale_grads) scale_grads;
   decltype(&k2q_adamw) adamw;
   decltype(&k2q_adamw_ws_bytes) adamw_ws_bytes;
   decltype(&k2q_moments) moments;
@@ -769,19 +768,18 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!stream_of(s.device, st)) return nullptr;
     const int64_t count = (int64_t)s.t.size(), nws = api.grad_norm_ws_bytes(s.t.data(), count);
     Tensor out = scale ? alloc({2}, at::kFloat, s.device) : Tensor(), ws = alloc({nws / 8}, at::kDouble, s.device);
-    int rc = foreign(api.grad_norm, s.t.data(), count, most, ptr(ws), nws, as<float>(ptr(out)), st);
-    if (!rc && scale) {
-      rc = foreign(api.scale_grads, s.t.data(), count, as<float>(ptr(out)) + 1, st);
+    const int rc = foreign(api.grad_norm, s.t.data(), count, most, ptr(ws), nws, as<float>(ptr(out)), scale, st);
+    if (scale)
       for (const Tensor& g : s.grads) changed(g);
-    }
     if (rc) return PyLong_FromLong(rc);
     return pack({scale ? out : ws});
   });
 }
 
 // adamw(params, starts, state_bits, exp_avg, exp_avg_sq, avg_scale | None, sq_scale | None, steps, lr, lr_of | None, beta1,
-// beta2, eps, weight_decay, squares | None, max_norm, norm | None, stochastic, seed) -> (): a step of the parameters that have
-// a gradient; starts: their places in the moments' buffers
+// beta2, eps, weight_decay, squares | None, max_norm | None, norm | None, stochastic, seed) -> (norm,): a step of the parameters
+// that have a gradient; starts: their places in the moments' buffers.  With a largest norm and no squares this call takes the
+// norm of its own gradients, else norm is the argument
 PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   K2Q_ARGS(19)
   return guarded([&]() -> PyObject* {
@@ -791,7 +789,7 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long bits = PyLong_AsLong(a[2]);
     const double lr = PyFloat_AsDouble(a[8]), beta1 = PyFloat_AsDouble(a[10]), beta2 = PyFloat_AsDouble(a[11]),
                  eps = PyFloat_AsDouble(a[12]), decay = PyFloat_AsDouble(a[13]),
-                 most = PyFloat_AsDouble(a[15]);
+                 most = a[15] == Py_None ? -1.0 : PyFloat_AsDouble(a[15]);
     const int stochastic = PyObject_IsTrue(a[17]);
     const unsigned long seed = PyLong_AsUnsignedLong(a[18]);
     if (PyErr_Occurred()) return nullptr;
@@ -826,16 +824,24 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st;
     if (!stream_of(d, st)) return nullptr;
     const int64_t count = (int64_t)s.t.size(), nws = api.adamw_ws_bytes(count);
-    Tensor ws = workspace(nws, d);
-    const int rc = foreign(api.adamw, s.t.data(), count, (int)bits, m->data_ptr(), v->data_ptr(), as<float>(ptr(ms)),
-                           as<float>(ptr(vs)), as<float>(ptr(steps)), lr, as<float>(ptr(lr_of)), beta1, beta2, eps, decay,
-                           as<double>(ptr(squares)), squares ? squares->numel() : 0, most, as<float>(ptr(norm)), stochastic,
-                           (uint32_t)seed, ptr(ws), nws, st);
+    Tensor ws = workspace(nws, d), sums = squares ? *squares : Tensor(), out = squares ? *norm : Tensor();
+    int rc = K2Q_OK;
+    if (!squares && most >= 0) {
+      const int64_t bytes = api.grad_norm_ws_bytes(s.t.data(), count);
+      sums = alloc({bytes / 8}, at::kDouble, d);
+      out = alloc({2}, at::kFloat, d);
+      rc = foreign(api.grad_norm, s.t.data(), count, most, ptr(sums), bytes, nullptr, 0, st);
+    }
+    if (!rc)
+      rc = foreign(api.adamw, s.t.data(), count, (int)bits, m->data_ptr(), v->data_ptr(), as<float>(ptr(ms)),
+                   as<float>(ptr(vs)), as<float>(ptr(steps)), lr, as<float>(ptr(lr_of)), beta1, beta2, eps, decay,
+                   as<double>(ptr(sums)), sums.defined() ? sums.numel() : 0, most, as<float>(ptr(out)), stochastic,
+                   (uint32_t)seed, ptr(ws), nws, st);
     if (rc) return PyLong_FromLong(rc);
     for (const Tensor& p : s.params) changed(p);
     for (const Tensor* t : {m, v, ms, vs, steps})
       if (t) changed(*t);
-    return PyTuple_New(0);
+    return pack({out});
   });
 }
 
@@ -998,7 +1004,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !get("k2q_resnorm_stream_bwd", api.resnorm_stream_bwd) ||
       !get("k2q_rotary", api.rotary) || !get("k2q_capture_id", api.capture_id) ||
       !get("k2q_grad_norm", api.grad_norm) || !get("k2q_grad_norm_ws_bytes", api.grad_norm_ws_bytes) ||
-      !get("k2q_scale_grads", api.scale_grads) || !get("k2q_adamw", api.adamw) ||
+      !get("k2q_adamw", api.adamw) ||
       !get("k2q_adamw_ws_bytes", api.adamw_ws_bytes) || !get("k2q_moments", api.moments) ||
       !get("k2q_bank_fwd", api.bank_fwd) || !get("k2q_bank_fwd_ws_bytes", api.bank_fwd_ws_bytes) ||
       !get("k2q_bank_bwd", api.bank_bwd) || !get("k2q_bank_bwd_ws_bytes", api.bank_bwd_ws_bytes))

@@ -123,28 +123,30 @@ __global__ __launch_bounds__(THREADS) void sumsq_kernel(Table<N> a, int64_t chun
   if (threadIdx.x == 0) part[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
-// The norm and the factor that brings it to max_norm, from the partial sums in a fixed order; for every thread of a workgroup.
+// The norm and the factor that brings it to max_norm, from the partial sums in a fixed order; for every thread of a workgroup
+// of N.
 struct Norm {
   float norm, by;
 };
 
+template <int N>
 __device__ __forceinline__ Norm norm_of(const double* part, int64_t n, double max_norm) {
-  __shared__ double sums[16];
+  __shared__ double sums[N / 64];
   double s = 0;
 #pragma unroll 4
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
+  for (int64_t i = threadIdx.x; i < n; i += N) s += part[i];
   s = wave_add(s);
   if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = s;
   __syncthreads();
   s = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s += sums[i];
+  for (int i = 0; i < N / 64; ++i) s += sums[i];
   const double norm = sqrt(s), by = max_norm / (norm + 1e-6);
   return {(float)norm, by > 1.0 ? 1.f : (float)by};      // a norm that is no number gives a factor that is none
 }
 
 __global__ __launch_bounds__(1024) void norm_kernel(const double* part, int64_t n, double max_norm, float* out) {
-  const Norm v = norm_of(part, n, max_norm);
+  const Norm v = norm_of<1024>(part, n, max_norm);
   if (threadIdx.x) return;
   out[0] = v.norm;
   out[1] = v.by;
@@ -152,12 +154,25 @@ __global__ __launch_bounds__(1024) void norm_kernel(const double* part, int64_t 
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
+// Gradients times norm[1]; with few partial sums (parts) every workgroup adds them up itself and the first writes the norm,
+// which saves a launch.
 template <typename T, int N>
-__global__ __launch_bounds__(THREADS) void scale_kernel(Table<N> a, int64_t chunk, const float* by) {
+__global__ __launch_bounds__(THREADS) void scale_kernel(Table<N> a, int64_t chunk, const double* part, int64_t parts,
+                                                        double max_norm, float* norm) {
   const int i = tensor_of(a, blockIdx.x);
   const Item& it = a.t[i];
   T* g = static_cast<T*>(it.g);
-  const float f = by[0];
+  float f;
+  if (part) {
+    const Norm v = norm_of<THREADS>(part, parts, max_norm);
+    f = v.by;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      norm[0] = v.norm;
+      norm[1] = v.by;
+    }
+  } else {
+    f = norm[1];
+  }
   const int64_t begin = (int64_t)(blockIdx.x - a.first[i]) * chunk;
   const int64_t n = it.n, end = begin + chunk < n ? begin + chunk : n;
   each_turn<4>(it, begin, end, [&](int64_t e, auto whole) {
@@ -196,7 +211,7 @@ __global__ __launch_bounds__(1024) void begin_kernel(float* steps, int n, double
                                                      double max_norm, float* norm, uint32_t seed, Scalars* out) {
   const int i = blockIdx.x * 1024 + threadIdx.x;
   if (squares) {
-    const Norm v = norm_of(squares, count, max_norm);
+    const Norm v = norm_of<1024>(squares, count, max_norm);
     if (i == 0) {
       norm[0] = v.norm;
       norm[1] = v.by;
@@ -560,33 +575,31 @@ extern "C" int64_t k2q_grad_norm_ws_bytes(const k2q_step_tensor* t, int64_t coun
 }
 
 extern "C" int k2q_grad_norm(const k2q_step_tensor* t, int64_t count, double max_norm, void* ws, int64_t ws_bytes, float* out,
-                             void* stream) {
+                             int scale, void* stream) {
   int rc = check(t, count, false);
   if (rc != K2Q_OK) return rc;
-  const int64_t parts = norm_parts(t, count), chunk = norm_chunk(t, count);
-  if (!(max_norm >= 0) || !ws || ws_bytes < 8 * parts || !k2q_aligned(ws, 16) || !k2q_aligned(out, 8)) return K2Q_EINVAL;
+  const int64_t parts = norm_parts(t, count);
+  int64_t chunk = norm_chunk(t, count);
+  if (!(max_norm >= 0) || !ws || ws_bytes < 8 * parts || !k2q_aligned(ws, 16) || !k2q_aligned(out, 8) || (scale && !out))
+    return K2Q_EINVAL;
   double* part = static_cast<double*>(ws);
+  const double* sums = part;
   hipStream_t st = static_cast<hipStream_t>(stream);
   by_type([&](int dtype, auto T) {
     each_table(t, count, dtype, chunk, false, [&](const auto& a) {
-      hipLaunchKernelGGL((sumsq_kernel<decltype(T), std::extent_v<decltype(a.first)>>), dim3(a.blocks), dim3(THREADS), 0, st, a, chunk, part);
+      hipLaunchKernelGGL((sumsq_kernel<decltype(T), std::extent_v<decltype(a.first)>>), dim3(a.blocks), dim3(THREADS), 0, st,
+                         a, chunk, part);
       part += a.blocks;
     });
   });
-  if (out)
-    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(1024), 0, st, static_cast<const double*>(ws), parts, max_norm, out);
-  return k2q_launch_status();
-}
-
-extern "C" int k2q_scale_grads(const k2q_step_tensor* t, int64_t count, const float* by, void* stream) {
-  int rc = check(t, count, false);
-  if (rc != K2Q_OK) return rc;
-  if (!by || !k2q_aligned(by, 4)) return K2Q_EINVAL;
-  const int64_t chunk = step_chunk(t, count, 4 * THREADS);
+  const bool itself = scale && parts <= 2 * THREADS;
+  if (out && !itself) hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(1024), 0, st, sums, parts, max_norm, out);
+  if (!scale) return k2q_launch_status();
+  chunk = step_chunk(t, count, 4 * THREADS);
   by_type([&](int dtype, auto T) {
     each_table(t, count, dtype, chunk, true, [&](const auto& a) {
-      hipLaunchKernelGGL((scale_kernel<decltype(T), std::extent_v<decltype(a.first)>>), dim3(a.blocks), dim3(THREADS), 0,
-                         static_cast<hipStream_t>(stream), a, chunk, by);
+      hipLaunchKernelGGL((scale_kernel<decltype(T), std::extent_v<decltype(a.first)>>), dim3(a.blocks), dim3(THREADS), 0, st,
+                         a, chunk, itself ? sums : nullptr, parts, max_norm, out);
     });
   });
   return k2q_launch_status();

@@ -81,19 +81,24 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B:
     rest, zeros in a bank whose adapters differ, is not read and gets zero gradients.
 
     Sums are float32 and ``out`` is rounded once.  Float32 factors (and the sums between the products) enter the matrix
-    units as two bf16 parts, 2^-17 of a value off at most.  Rows may have any order; rows of one adapter that lie together
+    units as two bf16 parts, 2^-17 of a value off at most, or on the way to a float32 gradient as three, which hold it.  Rows may have any order; rows of one adapter that lie together
     are faster.  Differentiable in ``y``, ``x`` and both factors.  A value that is infinite or NaN spoils its own row, and the
     gradients of its row's adapter."""
+    grad = torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or lora_A.requires_grad or lora_B.requires_grad)
+    if not grad and not _lib.observed() and not (scales is not None and scales.requires_grad):
+        out = _lib.bank_native(y, x, lora_A, lora_B, adapters, scales, ranks, scale, False)
+        if out is not None:
+            return out[0]
     if x.dim() < 2 or y.shape[:-1] != x.shape[:-1]:
         raise ValueError(f"y {tuple(y.shape)} and x {tuple(x.shape)} differ in their rows")
-    if any(t is not None and t.requires_grad for t in (scales,)) and torch.is_grad_enabled():
+    if scales is not None and scales.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("scales get no gradient: detach them")
     if x.numel() == 0 and x.shape[-1] == lora_A.shape[-1] and y.shape[-1] == lora_B.shape[1]:
         return y.clone()
     if x.dtype == y.dtype == torch.bfloat16:
         x, y = _rows(x), _rows(y)
     A, B, ids = lora_A.contiguous(), lora_B.contiguous(), adapters.contiguous()
-    if _lib.observed() or torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, A, B)):
+    if _lib.observed() or grad:
         return _AddAdaptersFn.apply(y, x, A, B, ids, scales, ranks, float(scale))
     return _lib.bank_fwd(y, x, A, B, ids, scales, ranks, float(scale), False)[0]
 

@@ -180,21 +180,21 @@ class AdamW(torch.optim.Optimizer):
 
     def _step(self) -> None:
         groups, squares, norm = self.param_groups, None, None
-        if self.max_norm is not None:
-            every = groups[0]["params"] if len(groups) == 1 else [p for g in groups for p in g["params"]]
-            squares = _lib.grad_norm(every, self.max_norm, False)
+        if self.max_norm is not None and len(groups) > 1:       # of one group, the step's own call takes it
+            squares = _lib.grad_norm([p for g in groups for p in g["params"]], self.max_norm, False)
             if squares is not None:
                 norm = torch.empty(2, device=squares.device)
-            self.grad_norm = None if norm is None else norm[0]
         for i, g in enumerate(groups):
             held = self._held.get(i) or self._moments_of(i)
             lr, lr_of = g["lr"], None
             if isinstance(lr, torch.Tensor):
                 lr, lr_of = (0.0, lr) if lr.is_cuda else (float(lr), None)
             scales = (held.exp_avg_scale, held.exp_avg_sq_scale) if g["state_bits"] == 8 else (None, None)
-            _lib.adamw(g["params"], held.starts, g["state_bits"], held.exp_avg, held.exp_avg_sq, *scales, held.steps, lr,
-                       lr_of, *g["betas"], g["eps"], g["weight_decay"], squares, self.max_norm or 0.0, norm, g["stochastic"],
-                       g["seed"])
+            out = _lib.adamw(g["params"], held.starts, g["state_bits"], held.exp_avg, held.exp_avg_sq, *scales, held.steps, lr,
+                             lr_of, *g["betas"], g["eps"], g["weight_decay"], squares, self.max_norm, norm, g["stochastic"],
+                             g["seed"])
+            norm = out if len(groups) == 1 else norm
+        self.grad_norm = None if norm is None else norm[0]
 
 
 def _hooks(opt: torch.optim.Optimizer):

@@ -137,8 +137,8 @@ def test_step_entries_refuse_bad_arguments(k2):
     assert need == 8 * (1 + 98) and lib.k2q_grad_norm_ws_bytes(addr, 0) == 0
     for args in ((addr, 2, -1.0, a, need, a), (addr, 2, 1.0, None, need, a), (addr, 2, 1.0, a, need - 1, a),
                  (addr, 2, 1.0, a, need, a + 4), (addr, 0, 1.0, a, need, a), (None, 2, 1.0, a, need, a)):
-        assert lib.k2q_grad_norm(*args, None) == -1
-    assert lib.k2q_scale_grads(addr, 2, None, None) == -1
+        assert lib.k2q_grad_norm(*args, 0, None) == -1
+    assert lib.k2q_grad_norm(addr, 2, 1.0, a, need, None, 1, None) == -1
     for args in ((None, a, a, a, 256, 0, a, a), (a, a, a, a, 255, 0, a, a), (a, a, a, a, 256, 2, a, a), (a, a, a, a, 0, 0, a, a)):
         assert lib.k2q_moments(*args, None) == -1
 
