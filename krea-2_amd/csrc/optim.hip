@@ -461,13 +461,16 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
       __builtin_nontemporal_store(wm, fm);
       __builtin_nontemporal_store(wv, fv);
     }
+    T o[V];
 #pragma unroll
-    for (int q = 0; q < QUADS; ++q) {
-      T o[4];
+    for (int j = 0; j < V; ++j)
+      o[j] = rounded<T>(p[j / 4][j % 4], st.stochastic, st.stochastic ? mix(random[j] ^ 0x9E3779B9u) : 0u);
+    if constexpr (whole && QUADS == 2 && GAP == 4) {      // one store: half ones past the cache write lines twice
+      typedef T Vec8 __attribute__((ext_vector_type(8)));
+      __builtin_nontemporal_store((Vec8{o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]}), reinterpret_cast<Vec8*>(P + e));
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[i] = rounded<T>(p[q][i], st.stochastic, st.stochastic ? mix(random[4 * q + i] ^ 0x9E3779B9u) : 0u);
-      store<whole>(P, e + q * GAP, n, o);
+      for (int q = 0; q < QUADS; ++q) store<whole>(P, e + q * GAP, n, {o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]});
     }
   });
 }
@@ -548,7 +551,7 @@ void tables(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, b
       a.blocks = 0;
     }
     const uintptr_t both = (uintptr_t)t[i].p | (uintptr_t)t[i].g;
-    a.t[a.count] = {t[i].p, t[i].g, t[i].n, t[i].at, (int32_t)i, both % (4 * size_of(dtype)) == 0};
+    a.t[a.count] = {t[i].p, t[i].g, t[i].n, t[i].at, (int32_t)i, both % 16 == 0};
     a.first[a.count++] = a.blocks;
     a.blocks += blocks;
   }
