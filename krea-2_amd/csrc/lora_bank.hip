@@ -44,8 +44,8 @@ __device__ __forceinline__ int adapter_of(const Rows& a, int row) { return row >
 __device__ __forceinline__ int rank_of(const Rows& a, int id) {
   if (id < 0) return 0;
   if (!a.ranks) return a.R;
-  const int r = (a.ranks[id] + 15) & ~15;
-  return r < 0 ? 0 : r > a.R ? a.R : r;
+  const int r = min(a.ranks[id], a.R);
+  return r <= 0 ? 0 : (r + 15) & ~15;
 }
 
 __device__ __forceinline__ float scale_of(const Rows& a, int id) { return a.scales ? a.mul * a.scales[id] : a.mul; }
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 // that a factor's fragment (in f32 split on its way) serves four tiles, and y's vectors are on their way while it computes.  The
 // order of a tile's columns among MFMA rows is chosen so that a lane ends with 16 columns of a row in two pieces of 8, and 4
 // lanes with 64 bytes in one: y comes and goes in vectors.  (Whole lines at once, 16 lanes to 256 bytes, want the factor's rows
-// 8 apart in a fragment and measured slower: 95 -> 135 us at 3072 x 6144 -> 16384 with rank 64 in f32.)
+// 8 apart in a fragment and measured slower: 95 -> 135 us at 4 x 768 rows x 6144 -> 16384 with rank 64 in f32.)
 template <typename F, bool kWide>
 __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, const uint16_t* y, int C, const F* factor,
                                                      int64_t one, int held, int passes, int groups, uint16_t* out) {
@@ -503,8 +503,8 @@ __global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float*
   out[(int64_t)row * C + mine] = (uint16_t)f32_to_bf16_bits(base + v);
 }
 
-// The slices' sums, scaled: once, ahead of an "up" whose workgroups would each add them up (64 x 6 of them read a row's 22
-// slices of 64 ranks in 57 us; added up once, both take 25), or where no "up" is wanted.
+// The slices' sums, scaled: once, ahead of an "up" whose workgroups would each add them up (4 x 768 rows, 22 slices of 64
+// ranks, 24 workgroups a row: 57 us; added up once, both take 24), or where no "up" is wanted.
 __global__ __launch_bounds__(THREADS) void join_kernel(Rows rows, const float* part, int slices, float* sum) {
   const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
   const int row = (int)(i / rows.R), j = (int)(i % rows.R);
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chun
     int total = 0;
     if (a < n)
       for (int w = 0; w < 16; ++w) total += lds[w * n + a];
-    const int of = total * rows.per, pieces = (of + chunk - 1) / chunk, shared = pieces > 1 ? pieces : 0;
+    const int of = total * rows.per, pieces = of / chunk + (of % chunk != 0), shared = pieces > 1 ? pieces : 0;
     int sums[3] = {total, pieces, shared};
     scan(sums, lds + 16 * n);
     const int first = sums[1] - pieces, slot = sums[2] - shared;
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chun
     if (a < n) {
       plan.first[a] = first;
       for (int p = 0; p < pieces; ++p)
-        plan.items[first + p] = Item{a, p * chunk, min(of, (p + 1) * chunk), pieces > 1 ? slot + p : -1};
+        plan.items[first + p] = Item{a, p * chunk, p + 1 < pieces ? (p + 1) * chunk : of, pieces > 1 ? slot + p : -1};
     }
     if (a == n - 1) {
       plan.start[n] = sums[0];
@@ -785,8 +785,11 @@ int check(const k2q_bank* b, int64_t T, int64_t per) {
       !b->ids || !k2q_aligned(b->ids, b->ids64 ? 8 : 4) || !k2q_aligned(b->ranks, 4) || !k2q_aligned(b->scales, 4) || T < 1 ||
       per < 1 || T % per)
     return K2Q_EINVAL;
-  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > 0x7fffff00 || b->K > 1 << 24 || b->N > 1 << 24 ||
-      T * (b->K > b->N ? b->K : b->N) > (int64_t)1 << 40)      // more than any card holds, and 2^24 workgroups
+  // The row numbers of a piece, up to T + its length, fit 32 bits; and so do the threads of a launch: T C / 64 of "up",
+  // T R / 4 of the join, R (K + N) / 4 of the gradients' join.
+  const int64_t most = b->K > b->N ? b->K : b->N;
+  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > 1 << 30 || most > 1 << 24 || T * most > (int64_t)1 << 37 ||
+      T * b->R > (int64_t)1 << 33 || b->R * most > (int64_t)1 << 31)
     return K2Q_EUNSUPPORTED;
   return K2Q_OK;
 }
@@ -850,7 +853,19 @@ void launch_join(const Rows& rows, const float* part, int slices, float* sum, hi
                      st, rows, part, slices, sum);
 }
 
-constexpr int FEW = 128;
+// Few rows: the form of single rows, whose time grows with the rows, where that of tiles grows with the adapters that a tile
+// meets, e at most.  us of rows / tiles, 6144 -> 16384 in f32 with rank 64; 6144 -> 6144 in f32 with rank 16:
+//   one adapter       64 rows   23 / 20;  8.4 / 15      128 rows  37 / 20;  11 / 14     256 rows  71 / 22;  17 / 15
+//   4 in any order    96 rows   38 / 51;  9.9 / 30      192 rows  59 / 53;  15 / 30     512 rows  137 / 60;  29 / 30
+//   16 in any order   256 rows  80 / 170;  18 / 91      512 rows  152 / 193;  31 / 90   1024 rows  292 / 318;  59 / 110
+//   16 that lie together                                 256 rows  77 / 69;  18 / 37    512 rows  140 / 48;  31 / 29
+//   64 in any order   384 rows  174 / 486;  37 / 215    768 rows  321 / 768;  56 / 258  1024 rows  422 / 827;  77 / 268
+//   64 that lie together                                 384 rows  156 / 161;  38 / 73  768 rows  267 / 151;  46 / 50
+// Only the device knows which it is: the bound lies between the two orders' own.
+bool few_rows(const k2q_bank* b, int64_t T, int64_t per) {
+  const int64_t of_tile = (ROWS + per - 1) / per, e = of_tile < b->count ? of_tile : b->count;
+  return T <= 768 && T <= 64 + 16 * e;
+}
 
 // Few rows: slices that give every CU four workgroups, of 512 columns or more.
 int row_slices(int64_t T, int64_t C, int64_t R) {
@@ -887,7 +902,8 @@ struct Sums {
 
 // Rows of a piece: all pieces together give every CU two workgroups, and a piece 256 rows or more.
 Sums sums_plan(const k2q_bank* b, int64_t T, int64_t per) {
-  const int64_t blocks = ((b->K + COLS - 1) / COLS + (b->N + COLS - 1) / COLS) * ((b->R + 16 * tiles_of(b->R) - 1) / (16 * tiles_of(b->R)));
+  const int ranks = 16 * tiles_of(b->R);
+  const int64_t blocks = ((b->K + COLS - 1) / COLS + (b->N + COLS - 1) / COLS) * ((b->R + ranks - 1) / ranks);
   const int64_t want = (2 * (int64_t)k2q_cu_count() + blocks - 1) / blocks;
   int64_t chunk = ((T + want - 1) / want + 127) / 128 * 128;
   chunk = chunk < 256 ? 256 : chunk;
@@ -899,7 +915,7 @@ Sums sums_plan(const k2q_bank* b, int64_t T, int64_t per) {
 
 extern "C" int64_t k2q_bank_fwd_ws_bytes(const k2q_bank* b, int64_t T, int64_t per) {
   if (check(b, T, per) != K2Q_OK) return 0;
-  return (int64_t)(T <= FEW ? row_slices(T, b->K, b->R) : down_slices(T, b->K, b->R)) * T * b->R * 4;
+  return (int64_t)(few_rows(b, T, per) ? row_slices(T, b->K, b->R) : down_slices(T, b->K, b->R)) * T * b->R * 4;
 }
 
 extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* x, const uint16_t* y, uint16_t* out,
@@ -912,7 +928,7 @@ extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   const Rows rows = rows_of(b, T, per);
   hipStream_t st = static_cast<hipStream_t>(stream);
   float* part = static_cast<float*>(ws);
-  if (T <= FEW) {
+  if (few_rows(b, T, per)) {
     if (b->dtype == K2Q_DTYPE_F32) launch_rows<float>(rows, x, b->K, b->A, part, u, y, b->N, b->B, out, st);
     else launch_rows<uint16_t>(rows, x, b->K, b->A, part, u, y, b->N, b->B, out, st);
     return k2q_launch_status();

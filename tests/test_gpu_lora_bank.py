@@ -97,7 +97,10 @@ def _ids(shape, count, how, seed=1):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("case", list(CASES))
 def test_values_and_gradients(k2, dev, case, dtype, how):
-    lead, of, count, R, K, N = CASES[case]
+    _values_and_gradients(k2, dev, *CASES[case], dtype, how)
+
+
+def _values_and_gradients(k2, dev, lead, of, count, R, K, N, dtype, how):
     ids = _ids(of, count, how)
     x, y, A, B, ids, scales, _, dy = _make(dev, lead, ids, count, R, K, N, DTYPES[dtype])
     want, size = _formula(x, y, A, B, ids, scales, dy)
@@ -116,6 +119,18 @@ def test_values_and_gradients(k2, dev, case, dtype, how):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
     if how == "none":
         assert torch.equal(out, y) and not any(int(g.count_nonzero()) for g in grads[1:])
+
+
+@pytest.mark.parametrize("how", ["sorted", "mixed"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("lead, of, count, R, K, N", [
+    ((80,), (80,), 1, 32, 192, 320), ((81,), (81,), 1, 32, 192, 320),           # single rows and tiles, either side of the
+    ((176,), (176,), 7, 48, 320, 64), ((177,), (177,), 7, 48, 320, 64),         # rule between them
+    ((768,), (768,), 64, 16, 64, 192), ((769,), (769,), 64, 16, 64, 192),
+    ((5, 20), (5,), 5, 64, 128, 64), ((3, 50), (3,), 5, 64, 128, 64),
+    ((1000,), (1000,), 40, 64, 1088, 576), ((300,), (300,), 6, 144, 64, 128), ((11, 40), (11,), 9, 272, 128, 1344)])
+def test_single_rows_and_tiles(k2, dev, lead, of, count, R, K, N, dtype, how):
+    _values_and_gradients(k2, dev, lead, of, count, R, K, N, dtype, how)
 
 
 @pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 63, 64, 65, 127, 255, 256, 257, 300, 513])
@@ -233,7 +248,8 @@ def test_forms_of_arguments(k2, dev):
     plain = [t.clone().requires_grad_() for t in (y, x, A)]
     far = torch.empty(3, 20, 193, device=dev, dtype=torch.bfloat16)[..., :-1]
     far.copy_(dy)
-    for a, b in zip(torch.autograd.grad(out, leaves, far), torch.autograd.grad(k2.add_adapters(*plain, B, ids, scales), plain, dy)):
+    near = torch.autograd.grad(k2.add_adapters(*plain, B, ids, scales), plain, dy)
+    for a, b in zip(torch.autograd.grad(out, leaves, far), near):
         assert torch.equal(a, b)
     none = k2.add_adapters(y[:0], x[:0], A, B, ids[:0], scales)
     assert none.shape == (0, 20, 192)
@@ -408,3 +424,27 @@ def test_bank_gradients_beside_every_base(k2, dev, kind):
     _check(dA, want[2], size[2], 384 + 120, "f32")
     _check(dB, want[3], size[3], 256 + 120, "f32")
     assert not int(dA[2].count_nonzero()) and not int(dB[2].count_nonzero())
+
+
+def test_two_streams_at_once(k2, dev):
+    """Calls on two streams share no workspace: each gives what it gives alone."""
+    a = _make(dev, (300,), _ids((300,), 5, "mixed"), 5, 32, 256, 320, torch.float32)
+    b = _make(dev, (70,), _ids((70,), 5, "mixed", seed=2), 5, 32, 256, 320, torch.float32, seed=7)
+
+    def call(x, y, A, B, ids, scales, _, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, A, B)]
+        out = k2.add_adapters(y, *leaves, ids, scales)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dy))
+
+    want = [call(*a), call(*b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(10):
+        for s, args in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(call(*args))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(p, q) for p, q in zip(g, want[i % 2])), i
