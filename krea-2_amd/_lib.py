@@ -1421,7 +1421,7 @@ MOMENT_BLOCK = 256      # K2Q_MOMENT_BLOCK: elements of a moment in 8 bits that 
 
 
 def _check_gradients(params, in_place: bool) -> None:
-    dev, seen = None, set()
+    dev, written = None, []
     for i, p in enumerate(params):
         if not isinstance(p, torch.Tensor):
             raise ValueError(f"parameter {i} must be a tensor, got {type(p).__name__}")
@@ -1439,9 +1439,13 @@ def _check_gradients(params, in_place: bool) -> None:
             raise ValueError(f"parameter {i} or its gradient was made under torch.inference_mode")
         if in_place and not torch.ops.aten.is_non_overlapping_and_dense.default(g):
             raise ValueError(f"parameter {i}'s gradient has gaps or elements twice: it cannot be scaled in place")
-        if in_place and g.data_ptr() in seen:
-            raise ValueError(f"parameter {i}'s gradient is in the list twice")
-        seen.add(g.data_ptr())
+        w = g if in_place else p
+        written.append((w.data_ptr(), w.data_ptr() + w.nbytes, i))
+    written.sort()
+    for (_, end, i), (start, _, j) in zip(written, written[1:]):
+        if start < end:
+            what = "gradients" if in_place else "values"
+            raise ValueError(f"the {what} of parameters {min(i, j)} and {max(i, j)} share memory, which would be written twice")
     if dev is not None:
         _device_check(dev)
 
@@ -1533,8 +1537,10 @@ def check_bank(t, width: int, A, B, ids, scales, ranks) -> None:
         if v is not None and (v.dtype != dtype or v.numel() != count or v.device != dev or not v.is_contiguous()):
             raise ValueError(f"{name} must be {count} contiguous {dtype} values on {dev}, got {tuple(v.shape)} {v.dtype} on "
                              f"{v.device}")
-    if t.numel() // width > 0x7fffff00:
-        raise ValueError(f"{t.numel() // width} rows: 2^31 - 256 are the most")
+    T, most = t.numel() // width, max(K, N)
+    if T > 1 << 30 or T * most > 1 << 37 or T * R > 1 << 33 or R * most > 1 << 31:
+        raise ValueError(f"{T} rows of {K} -> {N} features and rank {R}: the most are 2^30 rows, 2^37 elements of a tensor of "
+                         "the batch, 2^33 of rows x rank and 2^31 of a factor")
     _device_check(dev)
 
 

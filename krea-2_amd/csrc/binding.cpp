@@ -15,7 +15,8 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 
-#include <unordered_set>
+#include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "../../include/k2q.h"
@@ -713,7 +714,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
 struct Stepped {
   std::vector<k2q_step_tensor> t;
   std::vector<Tensor> grads, params;
-  std::unordered_set<void*> written;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;     // what the call writes, from and to
   c10::Device device = c10::Device(at::kCPU);
 
   // False where an argument is not what the kernels take.  in_place: the gradients are written, so a copy will not do.
@@ -730,10 +731,20 @@ struct Stepped {
       if (in_place) return false;
       flat = g.detach().contiguous();
     }
-    if (in_place && !written.insert(flat.data_ptr()).second) return false;     // scaled twice, in no order
+    const Tensor& w = in_place ? flat : p;
+    const uintptr_t from = (uintptr_t)w.data_ptr();
+    written.emplace_back(from, from + w.nbytes());
     t.push_back({p.data_ptr(), flat.data_ptr(), flat.numel(), 0, 0, dt});
     grads.push_back(flat);
     params.push_back(p);
+    return true;
+  }
+
+  // Nothing is written twice: it would be, in no order.
+  bool apart() {
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i].first < written[i - 1].second) return false;
     return true;
   }
 };
@@ -761,7 +772,7 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int scale = PyObject_IsTrue(a[2]);
     if (PyErr_Occurred()) return nullptr;
     Stepped s;
-    if (bad || !each_of(a[0], [&](const Tensor& p, int64_t) { return s.add(p, scale); })) K2Q_REFUSE;
+    if (bad || !each_of(a[0], [&](const Tensor& p, int64_t) { return s.add(p, scale); }) || (scale && !s.apart())) K2Q_REFUSE;
     if (s.t.empty()) return PyTuple_New(0);
     const c10::DeviceGuard guard(s.device);
     void* st;
@@ -810,15 +821,16 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const size_t before = s.t.size();
       if (i >= places || !s.add(p, false)) return false;
       if (s.t.size() == before) return true;
-      const int64_t at = PyLong_AsLongLong(PyList_GET_ITEM(a[1], i));
+      const int64_t at = PyLong_AsLongLong(PyList_GET_ITEM(a[1], i)),
+                    end = i + 1 < places ? PyLong_AsLongLong(PyList_GET_ITEM(a[1], i + 1)) : size;
       s.t.back().at = at;
       s.t.back().index = (int32_t)i;
       return !(at == -1 && PyErr_Occurred()) && p.is_contiguous() && p.scalar_type() == s.grads.back().scalar_type() &&
              p.sizes() == p.grad().sizes() && p.device() == d && at >= 0 && at % K2Q_MOMENT_BLOCK == 0 &&
-             at + p.numel() <= size && !(stochastic && p.scalar_type() == at::kHalf);
+             end <= size && at + p.numel() <= end && !(stochastic && p.scalar_type() == at::kHalf);
     });
     if (PyErr_Occurred()) return nullptr;
-    if (!fits) K2Q_REFUSE;
+    if (!fits || !s.apart()) K2Q_REFUSE;
     if (s.t.empty()) return PyTuple_New(0);
     const c10::DeviceGuard guard(d);
     void* st;
@@ -900,7 +912,9 @@ bool bank_of(const Tensor* A, const Tensor* B, const Tensor* ids, const Tensor* 
     return false;
   o.T = t.numel() / t.size(t.dim() - 1);
   o.per = o.T / ids->numel();
-  if (o.T > 0x7fffff00) return false;
+  const int64_t most = K > N ? K : N;
+  if (o.T > 1 << 30 || o.T * most > (int64_t)1 << 37 || o.T * R > (int64_t)1 << 33 || R * most > (int64_t)1 << 31)
+    return false;
   o.b = {A->data_ptr(), B->data_ptr(), ids->data_ptr(), as<int32_t>(ptr(ranks)), as<float>(ptr(scales)), (float)scale,
          it == at::kLong, ty == at::kFloat ? K2Q_DTYPE_F32 : K2Q_DTYPE_BF16, (int32_t)count, (int32_t)R, (int32_t)K,
          (int32_t)N};

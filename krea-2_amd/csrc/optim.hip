@@ -499,6 +499,8 @@ __global__ __launch_bounds__(THREADS) void moments_kernel(const uint8_t* cm, con
 // ---------------------------------------------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int64_t MOST = (int64_t)1 << 34;      // elements of a tensor: 2^23 workgroups, for a launch's threads fit 32 bits
+
 int size_of(int dtype) { return dtype == K2Q_DTYPE_F32 ? 4 : 2; }
 
 int check(const k2q_step_tensor* t, int64_t count, bool params) {
@@ -508,7 +510,7 @@ int check(const k2q_step_tensor* t, int64_t count, bool params) {
         !k2q_aligned(t[i].g, size_of(t[i].dtype)) ||
         (params && (!t[i].p || !k2q_aligned(t[i].p, size_of(t[i].dtype)) || t[i].at < 0 || t[i].at % BLOCK || t[i].index < 0)))
       return K2Q_EINVAL;
-    if (t[i].n > (int64_t)1 << 42 || t[i].at > (int64_t)1 << 46) return K2Q_EUNSUPPORTED;    // 2^29 workgroups
+    if (t[i].n > MOST || t[i].at > (int64_t)1 << 46) return K2Q_EUNSUPPORTED;
   }
   return K2Q_OK;
 }
@@ -536,7 +538,7 @@ int64_t norm_parts(const k2q_step_tensor* t, int64_t count) {
   return parts;
 }
 
-// f(table) over the tensors of one type, N and 2^30 workgroups at a time.  Behind a pass over the gradients they go backwards:
+// f(table) over the tensors of one type, N and fewer than 2^24 workgroups at a time.  Behind a pass over the gradients they go backwards:
 // what that pass read last is still in the last-level cache.
 template <int N, class F>
 void tables(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, bool backwards, F&& f) {
@@ -545,7 +547,7 @@ void tables(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, b
     const int64_t i = backwards ? count - 1 - k : k;
     if (t[i].dtype != dtype) continue;
     const uint32_t blocks = (uint32_t)((t[i].n + chunk - 1) / chunk);
-    if (a.count == N || (a.count && (int64_t)a.blocks + blocks > 1 << 30)) {
+    if (a.count == N || (a.count && a.blocks + blocks >= 1u << 24)) {
       f(a);
       a.count = 0;
       a.blocks = 0;
@@ -621,7 +623,8 @@ extern "C" int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits
       !k2q_aligned(exp_avg_sq, 16) || (state_bits == 8 && (!avg_scale || !sq_scale)) || !k2q_aligned(avg_scale, 4) ||
       !k2q_aligned(sq_scale, 4) || !steps || !k2q_aligned(steps, 4) || !(beta1 >= 0 && beta1 < 1) ||
       !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(lr == lr) || !(weight_decay >= 0) || !k2q_aligned(lr_of, 4) ||
-      (squares && (n_squares < 1 || !k2q_aligned(squares, 8) || !(max_norm >= 0) || !norm || !k2q_aligned(norm, 8))) || !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_adamw_ws_bytes(count) || count > 0x7fffffff)
+      (squares && (n_squares < 1 || !k2q_aligned(squares, 8) || !(max_norm >= 0) || !norm || !k2q_aligned(norm, 8))) ||
+      !ws || !k2q_aligned(ws, 16) || ws_bytes < k2q_adamw_ws_bytes(count) || count > 0x7fffffff)
     return K2Q_EINVAL;
   for (int64_t i = 0; i < count; ++i)
     if ((stochastic && t[i].dtype == K2Q_DTYPE_F16) || (i && t[i].index <= t[i - 1].index)) return K2Q_EINVAL;
@@ -634,8 +637,8 @@ extern "C" int k2q_adamw(const k2q_step_tensor* t, int64_t count, int state_bits
                        scalars + i);
   }
   const int64_t chunk = step_chunk(t, count, (state_bits == 8 ? 8 : 4) * THREADS);
-  const Step s{exp_avg, exp_avg_sq, avg_scale, sq_scale, scalars, squares ? norm : nullptr, (float)beta1, (float)(1 - beta1), (float)beta2,
-               (float)(1 - beta2), (float)eps, stochastic};
+  const Step s{exp_avg, exp_avg_sq, avg_scale, sq_scale, scalars, squares ? norm : nullptr, (float)beta1, (float)(1 - beta1),
+               (float)beta2, (float)(1 - beta2), (float)eps, stochastic};
   by_type([&](int dtype, auto T) {
     each_table(t, count, dtype, chunk, squares != nullptr, [&](const auto& a) {
       constexpr int N = std::extent_v<decltype(a.first)>;
@@ -654,7 +657,7 @@ extern "C" int k2q_moments(const uint8_t* avg, const float* avg_scale, const uin
       !k2q_aligned(sq, 8) || !k2q_aligned(avg_scale, 4) || !k2q_aligned(sq_scale, 4) || !k2q_aligned(m, 16) ||
       !k2q_aligned(v, 16) || (dtype != K2Q_DTYPE_BF16 && dtype != K2Q_DTYPE_F32))
     return K2Q_EINVAL;
-  if (n > (int64_t)THREADS * 8 << 30) return K2Q_EUNSUPPORTED;
+  if (n > MOST) return K2Q_EUNSUPPORTED;
   const dim3 grid((unsigned)((n / 8 + THREADS - 1) / THREADS));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == K2Q_DTYPE_BF16)

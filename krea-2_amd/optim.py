@@ -61,7 +61,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"max_norm must be 0 or above, got {max_norm}")
         self.max_norm = None if max_norm is None else float(max_norm)
         self.grad_norm = None
-        self._held = {}         # group number -> its moments' buffers
+        self._held = {}         # id of a group's list of parameters -> its moments' buffers (which hold the list)
         super().__init__(params, defaults)
 
     def add_param_group(self, param_group: dict) -> None:
@@ -83,13 +83,12 @@ class AdamW(torch.optim.Optimizer):
             _check_options(group)
 
     # -- moments -------------------------------------------------------------------------------------------------
-    def _moments_of(self, i: int) -> SimpleNamespace:
-        """Group ``i``'s buffers, made when they are not there: zeros, or the states that its parameters have."""
-        held = self._held.get(i)
+    def _moments_of(self, group: dict) -> SimpleNamespace:
+        """A group's buffers, made when they are not there: zeros, or the states that its parameters have."""
+        params = group["params"]
+        held = self._held.get(id(params))
         if held is not None:
             return held
-        group = self.param_groups[i]
-        params = group["params"]
         devices = {p.device for p in params}
         if len(devices) != 1 or next(iter(devices)).type != "cuda":
             raise RuntimeError(f"k2q kernels need a group's parameters on one gfx950 GPU, got {sorted(map(str, devices))}")
@@ -99,13 +98,14 @@ class AdamW(torch.optim.Optimizer):
                                "step, or load a state, before it")
         for k, p in enumerate(params):
             if p.dtype not in _lib.STEP_DTYPES:
-                raise ValueError(f"parameter {k} of group {i} is {p.dtype}, not one of {_lib.STEP_DTYPES}")
+                raise ValueError(f"parameter {k} is {p.dtype}, not one of {_lib.STEP_DTYPES}")
         starts, total = [], 0
         for p in params:
             starts.append(total)
             total += -(-p.numel() // _BLOCK) * _BLOCK
-        held = SimpleNamespace(starts=starts, steps=torch.zeros(len(params), device=dev))
-        kinds = _kinds(group["state_bits"])
+        held = SimpleNamespace(params=params, bits=group["state_bits"], starts=starts,
+                               steps=torch.zeros(len(params), device=dev))
+        kinds = _kinds(held.bits)
         for name, (dtype, per) in kinds.items():
             setattr(held, name, torch.zeros(total // per, device=dev, dtype=torch.uint8).view(dtype)
                     if dtype.itemsize == 1 else torch.zeros(total // per, device=dev, dtype=dtype))
@@ -120,7 +120,7 @@ class AdamW(torch.optim.Optimizer):
                     for name, view in new.items():
                         _copy(view, old[name])
                 self.state[p] = new
-        self._held[i] = held
+        self._held[id(params)] = held
         return held
 
     def moments(self, group: int = 0, dtype: torch.dtype = torch.float32):
@@ -129,29 +129,29 @@ class AdamW(torch.optim.Optimizer):
         bfloat16)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
-        held = self._moments_of(group)
-        if self.param_groups[group]["state_bits"] == 32:
+        held = self._moments_of(self.param_groups[group])
+        if held.bits == 32 or not held.exp_avg.numel():
             return held.exp_avg.to(dtype), held.exp_avg_sq.to(dtype)
         return _lib.moments(held.exp_avg, held.exp_avg_scale, held.exp_avg_sq, held.exp_avg_sq_scale, dtype)
 
     def load_state_dict(self, state_dict: dict) -> None:
         """A state of this class, or, in 32 bits, of ``torch.optim.AdamW`` (without ``amsgrad`` or ``maximize``).  The values
         are copied, in their own types."""
-        super().load_state_dict({**state_dict, "state": {}})
-        numbers = [n for g in state_dict["param_groups"] for n in g["params"]]
-        for n, p in zip(numbers, (p for g in self.param_groups for p in g["params"])):
-            if n in state_dict["state"]:
-                self.state[p] = dict(state_dict["state"][n])
-        try:
-            for i, group in enumerate(self.param_groups):
-                for p in group["params"]:
-                    _check_state(self.state.get(p), p, group["state_bits"])
-                if any(p in self.state for p in group["params"]):
-                    self._moments_of(i)
-        except BaseException:
-            self.state.clear()
-            self._held.clear()
-            raise
+        saved, states = state_dict["param_groups"], state_dict["state"]
+        # options that a state does not name stay; what does not fit is refused before anything changes
+        own = [{k: g[k] for k in self.defaults} for g in self.param_groups]
+        saved = [{**g, **s} for g, s in zip(own, saved)] + saved[len(own):]
+        for s, g in zip(saved, self.param_groups):
+            _check_options(s)
+            for n, p in zip(s["params"], g["params"]):
+                _check_state(states.get(n), p, s["state_bits"])
+        super().load_state_dict({**state_dict, "state": {}, "param_groups": saved})
+        for s, g in zip(saved, self.param_groups):
+            for n, p in zip(s["params"], g["params"]):
+                if n in states:
+                    self.state[p] = dict(states[n])
+            if any(p in self.state for p in g["params"]):
+                self._moments_of(g)
 
     # -- the step ------------------------------------------------------------------------------------------------
     def step(self, closure=None):
@@ -184,13 +184,15 @@ class AdamW(torch.optim.Optimizer):
             squares = _lib.grad_norm([p for g in groups for p in g["params"]], self.max_norm, False)
             if squares is not None:
                 norm = torch.empty(2, device=squares.device)
-        for i, g in enumerate(groups):
-            held = self._held.get(i) or self._moments_of(i)
+        for g in groups:
+            if not g["params"]:
+                continue
+            held = self._held.get(id(g["params"])) or self._moments_of(g)
             lr, lr_of = g["lr"], None
             if isinstance(lr, torch.Tensor):
                 lr, lr_of = (0.0, lr) if lr.is_cuda else (float(lr), None)
-            scales = (held.exp_avg_scale, held.exp_avg_sq_scale) if g["state_bits"] == 8 else (None, None)
-            out = _lib.adamw(g["params"], held.starts, g["state_bits"], held.exp_avg, held.exp_avg_sq, *scales, held.steps, lr,
+            scales = (held.exp_avg_scale, held.exp_avg_sq_scale) if held.bits == 8 else (None, None)
+            out = _lib.adamw(g["params"], held.starts, held.bits, held.exp_avg, held.exp_avg_sq, *scales, held.steps, lr,
                              lr_of, *g["betas"], g["eps"], g["weight_decay"], squares, self.max_norm, norm, g["stochastic"],
                              g["seed"])
             norm = out if len(groups) == 1 else norm

@@ -131,6 +131,8 @@ def test_step_entries_refuse_bad_arguments(k2):
                 {"ws": None}, {"nws": 8}, {"stochastic": 1, "t": [one(dtype=2)]}):
         assert call(**bad) == -1, bad
     assert call(t=[one(n=1 << 43)]) == -4
+    assert call(t=[one(n=(1 << 34) + 1)]) == -4 and call(t=[one(at=(1 << 46) + 256)]) == -4     # a launch's threads
+    assert lib.k2q_moments(a, a, a, a, (1 << 34) + 256, 1, a, a, None) == -4
     arr = (k2._lib.StepTensor * 2)(one(), one(n=100000))
     addr = ctypes.addressof(arr)
     need = lib.k2q_grad_norm_ws_bytes(addr, 2)
@@ -148,8 +150,8 @@ def test_bank_entries_refuse_bad_arguments(k2):
     lib, a = k2._lib.load(), 4096
 
     def bank(**kw):
-        return k2._lib.Bank(**{"A": a, "B": a, "ids": a, "scale": 1.0, "ids64": 1, "dtype": 1, "count": 3, "R": 16, "K": 64, "N": 128,
-                               **kw})
+        return k2._lib.Bank(**{"A": a, "B": a, "ids": a, "scale": 1.0, "ids64": 1, "dtype": 1, "count": 3, "R": 16, "K": 64,
+                               "N": 128, **kw})
 
     def fwd(b, T=12, per=4, x=a, y=a, out=a, u=a, ws=a, nws=1 << 30):
         return lib.k2q_bank_fwd(ctypes.addressof(b), T, per, x, y, out, u, ws, nws, None)
@@ -166,6 +168,14 @@ def test_bank_entries_refuse_bad_arguments(k2):
     for bad in ({"count": 1025}, {"R": 4112}, {"K": (1 << 24) + 64}):
         assert fwd(bank(**bad)) == -4 and bwd(bank(**bad)) == -4, bad
     assert fwd(bank(), T=0x7fffff04, per=4) == -4
+    for T, bad in (((1 << 30) + 4, {"K": 64, "N": 64}), (1 << 30, {"K": 192, "N": 64}), (1 << 30, {"R": 16, "K": 64, "N": 192}),
+                   (1 << 26, {"R": 144, "K": 64, "N": 64}), (12, {"R": 4096, "K": (1 << 19) + 64}),
+                   (12, {"R": 4096, "N": 1 << 20})):      # the grids' threads, a piece's row numbers
+        b = bank(**bad)
+        assert fwd(b, T=T, per=4, nws=1 << 62) == -4 and bwd(b, T=T, per=4, nws=1 << 62) == -4, (T, bad)
+        assert lib.k2q_bank_fwd_ws_bytes(ctypes.addressof(b), T, 4) == 0
+    b = bank(R=16, K=64, N=64)
+    assert lib.k2q_bank_fwd_ws_bytes(ctypes.addressof(b), 1 << 29, 4) >= (1 << 29) * 16 * 4     # at the limits
     for bad in ({"T": 0}, {"per": 0}, {"T": 13}, {"ws": None}, {"ws": a + 8}, {"nws": 0}):
         assert fwd(bank(), **bad) == -1 and bwd(bank(), **bad) == -1, bad
     for bad in ({"x": None}, {"x": a + 2}, {"y": a + 2}, {"out": None}, {"u": a + 4}):
@@ -287,3 +297,11 @@ def test_requests_and_scales_reach_every_bank(k2):
             bank(x.bfloat16())              # there is no kernel off the GPU
     assert all(b.adapters is None and b.scale_mul == 1.0 for b in banks.values())
 
+
+def test_gradients_that_overlap_are_not_scaled(k2):
+    flat = torch.ones(100)
+    p, q = _p(60), _p(40)
+    p.grad, q.grad = flat[:60], flat[59:99]
+    with pytest.raises(ValueError, match="parameters 0 and 1 share memory"):
+        k2.clip_grad_norm_([p, q], 1.0)
+    assert bool((flat == 1).all())

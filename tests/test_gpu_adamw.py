@@ -465,3 +465,95 @@ def test_places_past_32_bits(k2, dev):
     have = opt.state[p]["exp_avg"][first:].double().abs() * scale
     off = (have - want).abs() > 64 * 2.0 ** -24 * want
     assert int(off.sum()) <= 2 and at.numel() == tail
+
+
+def test_groups_that_move(k2, dev):
+    """A group taken out or put elsewhere keeps its parameters' moments with the others; an empty one is passed over; one
+    that grows is refused."""
+    a, b = (_params(dev, [(16, 24), (40,), (300,)], torch.float32) for _ in range(2))
+    oa = k2.AdamW([{"params": [a[0]]}, {"params": []}, {"params": [a[1]], "lr": 1e-2}, {"params": [a[2]]}], max_norm=1e9)
+    ob = k2.AdamW([{"params": [b[0]]}, {"params": [b[1]], "lr": 1e-2}, {"params": [b[2]]}], max_norm=1e9)
+    _three(oa, a)
+    _three(ob, b)
+    oa.param_groups.reverse()
+    ob.param_groups[0]["params"][0].grad = None
+    oa.param_groups.pop()
+    for p, q in zip(a[1:], b[1:]):
+        p.grad = q.grad = torch.ones_like(p)
+    b[0].grad = None
+    oa.step()
+    ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    oa.param_groups[0]["params"].append(_params(dev, [(4,)], torch.float32)[0])
+    with pytest.raises(ValueError, match="the group has 2 parameters"):
+        oa.step()
+
+
+def test_a_state_that_does_not_fit_changes_nothing(k2, dev):
+    a = _params(dev, [(16, 24)], torch.float32)
+    opt = k2.AdamW([{"params": a, "state_bits": 8, "lr": 3e-3}])
+    _three(opt, a)
+    before = copy.deepcopy(opt.state_dict())
+    torch_opt = torch.optim.AdamW(a, lr=1.0)
+    torch_opt.step()
+    with pytest.raises(ValueError, match="8 bits"):         # the group's own bits, which the state does not name
+        opt.load_state_dict(torch_opt.state_dict())
+    after = opt.state_dict()
+    assert after["param_groups"] == before["param_groups"] and opt.param_groups[0]["lr"] == 3e-3
+    assert all(_same(after["state"][0][n], before["state"][0][n]) for n in before["state"][0])
+    _three(opt, a)
+
+
+@pytest.mark.parametrize("bits", [0x7FFFFFFF, -1, 0x7FC00000, 0x7F800000])
+def test_values_that_are_not_finite_are_rounded_at_random_to_what_they_are(k2, dev, bits):
+    """A NaN stays one whatever its bits (16 random ones must not carry past its sign), an infinity stays infinite."""
+    p = torch.nn.Parameter(torch.zeros(512, device=dev, dtype=torch.bfloat16))
+    value = torch.tensor([bits >> 16 & 0xFFFF], dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    with torch.no_grad():
+        p[100:200] = value.to(dev)
+    opt = k2.AdamW([p], lr=1e-3, stochastic=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert torch.isfinite(p[:100]).all() and torch.isfinite(p[200:]).all()
+    want = torch.isnan if math.isnan(float(value)) else torch.isinf
+    assert want(p[100:200]).all()
+
+
+def test_memory_written_twice_is_refused(k2, dev):
+    """Parameters or gradients that share memory, and a parameter that outgrew its moments: refused, nothing changes."""
+    flat = torch.zeros(600, device=dev)
+    a, b, c = (torch.nn.Parameter(t) for t in (flat[:300], flat[299:400], flat[400:]))
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="parameters 0 and 1 share memory"):
+        k2.AdamW([a, b, c]).step()
+    assert not int(flat.count_nonzero())
+    k2.AdamW([a, c]).step()             # neighbours
+    assert bool((flat[:300] != 0).all()) and bool((flat[400:] != 0).all()) and not int(flat[300:400].count_nonzero())
+    with pytest.warns(UserWarning, match="duplicate"):
+        opt = k2.AdamW([c, c])
+    with pytest.raises(ValueError, match="parameters 0 and 1 share memory"):
+        opt.step()
+    grads = torch.ones(600, device=dev)
+    a.grad, b.grad = grads[:300], grads[200:301]
+    with pytest.raises(ValueError, match="parameters 0 and 1 share memory"):
+        k2.clip_grad_norm_([a, b, c], 1e-3)
+    assert bool((grads == 1).all())
+    opt = k2.AdamW([a, c])
+    opt.step()                          # gradients that share memory are only read
+    kept = [t.clone() for t in opt.moments()]
+    a.data = torch.zeros(513, device=dev)
+    a.grad = torch.ones(513, device=dev)
+    with pytest.raises(ValueError, match="grown to 513"):
+        opt.step()
+    assert all(torch.equal(x, y) for x, y in zip(opt.moments(), kept)) and not int(a.count_nonzero())
+
+
+def test_empty_parameters(k2, dev):
+    p = torch.nn.Parameter(torch.zeros(0, 4, device=dev))
+    p.grad = torch.zeros(0, 4, device=dev)
+    for bits in (32, 8):
+        opt = k2.AdamW([p], state_bits=bits, max_norm=1.0)
+        opt.step()
+        assert opt.grad_norm is None and all(t.numel() == 0 for t in opt.moments(dtype=torch.bfloat16))
+    assert float(k2.clip_grad_norm_([p], 1.0)) == 0.0
