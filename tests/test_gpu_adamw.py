@@ -557,3 +557,25 @@ def test_empty_parameters(k2, dev):
         opt.step()
         assert opt.grad_norm is None and all(t.numel() == 0 for t in opt.moments(dtype=torch.bfloat16))
     assert float(k2.clip_grad_norm_([p], 1.0)) == 0.0
+
+
+@pytest.mark.parametrize("gap", [2, 7])
+def test_many_parameters_without_gradients_between(k2, dev, gap):
+    """Counts and values of the others stay; those with a gradient move as in a list of their own, beyond 512 of them too."""
+    n = 560 * gap
+    a = _params(dev, [(5,)] * n, torch.float32)
+    for p in a:
+        p.grad = None
+    few = [torch.nn.Parameter(p.detach().clone()) for p in a[::gap]]
+    oa, ob = k2.AdamW(a, max_norm=1.0), k2.AdamW(few, max_norm=1.0)
+    for k in range(3):
+        for i, p in enumerate(few):
+            p.grad = torch.full_like(p, (i % 13 - 6) * 0.25 + k)
+            a[i * gap].grad = p.grad.clone()
+        before = [p.detach().clone() for p in a]
+        oa.step()
+        ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a[::gap], few))
+    assert all(torch.equal(p, q) for i, (p, q) in enumerate(zip(a, before)) if i % gap)
+    counts = torch.stack([oa.state[p]["step"] for p in a]).view(-1, gap)
+    assert bool((counts[:, 0] == 3).all()) and not int(counts[:, 1:].count_nonzero())
