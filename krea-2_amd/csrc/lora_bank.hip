@@ -162,16 +162,22 @@ __device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, 
 // Down: part[slice][t][j] = sum over the slice's columns c of x[t][c] F_a[j][c], scaled where one slice is all
 // ---------------------------------------------------------------------------------------------------------------
 // A workgroup: 64 rows, a slice of columns, Q tiles of 16 ranks.  Its waves take 64 columns in turn (a row's 128 bytes of x),
-// all 64 rows and all ranks, so that a factor's fragment serves four MFMAs; their sums meet in LDS.
+// all 64 rows and all ranks, so that a factor's fragment serves four MFMAs; their sums meet in LDS.  Neighbouring workgroups go
+// to different dies, 8 of them: each die takes the row tiles of a slice, then those of the next, so that a slice's part of the
+// factors comes into one die's cache and not into all (4 x 4608 rows x 6144, rank 32, 171 -> 166 us with the "up"; 16896 x
+// 16384 backward 389 -> 382; 4 x 768 x 6144 -> 16384 backward 139.8 -> 137.5).
 template <typename F, bool kWide, int Q>
 __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
-                                                       int slice_cols, float* part) {
+                                                       int slice_cols, int slices, float* part) {
   constexpr int RS = 16 * Q + 4;        // a row of sums in LDS
   constexpr int N = kF32<F> ? 3 : 1;    // u and g go into gradients in f32, and a served row has a trained one's bits
   extern __shared__ float sums[];       // 4 waves x 64 rows x RS
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
-  const int row0 = blockIdx.x * ROWS, j0 = blockIdx.z * 16 * Q;
-  const int begin = blockIdx.y * slice_cols, end = min(C, begin + slice_cols);
+  const int eighth = (rows.T + 8 * ROWS - 1) / (8 * ROWS), job = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  const int slice = job / (8 * eighth), i = job % (8 * eighth);
+  const int row0 = (i % eighth * 8 + i / eighth) * ROWS, j0 = blockIdx.y * 16 * Q;
+  if (row0 >= rows.T) return;
+  const int begin = slice * slice_cols, end = min(C, begin + slice_cols);
   const int id = adapter_of(rows, row0 + lane);
   const uint16_t* xr[4];
 #pragma unroll
@@ -234,8 +240,8 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
       v4f v = *reinterpret_cast<const v4f*>(sums + row * RS + j);
 #pragma unroll
       for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + (w * ROWS + row) * RS + j);
-      if (gridDim.y == 1) v *= scale;
-      *reinterpret_cast<v4f*>(part + ((int64_t)blockIdx.y * rows.T + row0 + row) * rows.R + j0 + j) = v;
+      if (slices == 1) v *= scale;
+      *reinterpret_cast<v4f*>(part + ((int64_t)slice * rows.T + row0 + row) * rows.R + j0 + j) = v;
     }
     __syncthreads();
   }
@@ -534,7 +540,7 @@ struct Plan {
 };
 
 constexpr int PLAN = 1024;            // threads: one an adapter
-constexpr int HELD = 32768;           // ids in LDS: both passes over 16896 ids 29 -> 10 us
+constexpr int HELD = 32768;           // ids in LDS, for both passes: 16896 ids 26 -> 14 us
 
 // Inclusive sums of three values over the workgroup's threads; waves: 3 x 16 in LDS.
 __device__ __forceinline__ void scan(int (&v)[3], int32_t* waves) {
@@ -598,7 +604,9 @@ __global__ __launch_bounds__(PLAN) void plan_kernel(Rows rows, int ids, int chun
     int total = 0;
     if (a < n)
       for (int w = 0; w < 16; ++w) total += lds[w * n + a];
-    const int of = total * rows.per, pieces = of / chunk + (of % chunk != 0), shared = pieces > 1 ? pieces : 0;
+    // one at least, without rows: its sums are zeros
+    const int of = total * rows.per, pieces = a < n ? max(of / chunk + (of % chunk != 0), 1) : 0;
+    const int shared = pieces > 1 ? pieces : 0;
     int sums[3] = {total, pieces, shared};
     scan(sums, lds + 16 * n);
     const int first = sums[1] - pieces, slot = sums[2] - shared;
@@ -753,7 +761,7 @@ __global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, 
   }
 }
 
-// What pieces left: the sum of an adapter's in their order, and zeros for an adapter without rows.
+// What pieces left: the sum of an adapter's in their order.
 template <typename F>
 __global__ __launch_bounds__(THREADS) void pieces_kernel(Plan plan, Jobs jobs) {
   const int a = blockIdx.y, second = (int)blockIdx.x >= jobs.j[0].blocks;
@@ -761,12 +769,9 @@ __global__ __launch_bounds__(THREADS) void pieces_kernel(Plan plan, Jobs jobs) {
   const int first = plan.first[a], n = plan.first[a + 1] - first;
   const int64_t i = ((int64_t)((int)blockIdx.x - (second ? jobs.j[0].blocks : 0)) * THREADS + threadIdx.x) * 4;
   if (n == 1 || i >= job.one) return;
-  v4f v = {0.f, 0.f, 0.f, 0.f};
-  if (n) {
-    const float* p = job.part + plan.items[first].slot * job.one + i;
-    v = *reinterpret_cast<const v4f*>(p);
-    for (int s = 1; s < n; ++s) v += *reinterpret_cast<const v4f*>(p + s * job.one);
-  }
+  const float* p = job.part + plan.items[first].slot * job.one + i;
+  v4f v = *reinterpret_cast<const v4f*>(p);
+  for (int s = 1; s < n; ++s) v += *reinterpret_cast<const v4f*>(p + s * job.one);
   if constexpr (kF32<F>)
     *reinterpret_cast<v4f*>(static_cast<float*>(job.out) + a * job.one + i) = v;
   else
@@ -819,12 +824,12 @@ template <typename F, bool kWide>
 void launch_down(const Rows& rows, const uint16_t* x, int64_t C, const void* f, int slices, float* part, hipStream_t st) {
   const int64_t cols = ((C + slices - 1) / slices + 255) / 256 * 256, one = (int64_t)rows.R * C;
   const int q = tiles_of(rows.R);
-  const dim3 grid((unsigned)((rows.T + ROWS - 1) / ROWS), (unsigned)slices, (unsigned)((rows.R + 16 * q - 1) / (16 * q)));
+  const dim3 grid((unsigned)((rows.T + 8 * ROWS - 1) / (8 * ROWS) * 8 * slices), (unsigned)((rows.R + 16 * q - 1) / (16 * q)));
   const int lds = 4 * ROWS * (16 * q + 4) * 4;
   const F* factor = static_cast<const F*>(f);
   auto go = [&](auto kernel, std::atomic<uint64_t>& once) {
     (void)k2q_lds_limit_once(kernel, lds, once);
-    hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, st, rows, x, (int)C, factor, one, (int)cols, part);
+    hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, st, rows, x, (int)C, factor, one, (int)cols, slices, part);
   };
   static std::atomic<uint64_t> once[3];
   if (q == 1) go(down_kernel<F, kWide, 1>, once[0]);
@@ -1018,6 +1023,7 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   else if (q == 2) f32 ? go(sums_kernel<float, 2>, 2) : go(sums_kernel<uint16_t, 2>, 3);
   else f32 ? go(sums_kernel<float, 4>, 4) : go(sums_kernel<uint16_t, 4>, 5);
   if (sl != K2Q_OK) return sl;
+  if (!s.slots) return input();
   for (int i = 0; i < k; ++i) jobs.j[i].blocks = (int)((jobs.j[i].one / 4 + THREADS - 1) / THREADS);
   jobs.blocks = jobs.j[0].blocks + (k > 1 ? jobs.j[1].blocks : 0);
   const dim3 rest((unsigned)jobs.blocks, (unsigned)n);
