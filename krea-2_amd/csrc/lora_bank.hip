@@ -162,22 +162,18 @@ __device__ __forceinline__ void load_strided(const F* p, int64_t step, bool ok, 
 // Down: part[slice][t][j] = sum over the slice's columns c of x[t][c] F_a[j][c], scaled where one slice is all
 // ---------------------------------------------------------------------------------------------------------------
 // A workgroup: 64 rows, a slice of columns, Q tiles of 16 ranks.  Its waves take 64 columns in turn (a row's 128 bytes of x),
-// all 64 rows and all ranks, so that a factor's fragment serves four MFMAs; their sums meet in LDS.  Neighbouring workgroups go
-// to different dies, 8 of them: each die takes the row tiles of a slice, then those of the next, so that a slice's part of the
-// factors comes into one die's cache and not into all (4 x 4608 rows x 6144, rank 32, 171 -> 166 us with the "up"; 16896 x
-// 16384 backward 389 -> 382; 4 x 768 x 6144 -> 16384 backward 139.8 -> 137.5).
+// all 64 rows and all ranks, so that a factor's fragment serves four MFMAs; their sums meet in LDS.  (A slice's row
+// tiles on one die, so that its part of the factors comes into one cache: 171 -> 166 us at 4 x 4608 rows x 6144 with the "up",
+// but 156 -> 160 where a quarter of the rows has no adapter, and with the tiles spread over them 245 -> 278 at 16896 x 16384.)
 template <typename F, bool kWide, int Q>
 __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
-                                                       int slice_cols, int slices, float* part) {
+                                                       int slice_cols, float* part) {
   constexpr int RS = 16 * Q + 4;        // a row of sums in LDS
   constexpr int N = kF32<F> ? 3 : 1;    // u and g go into gradients in f32, and a served row has a trained one's bits
   extern __shared__ float sums[];       // 4 waves x 64 rows x RS
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
-  const int eighth = (rows.T + 8 * ROWS - 1) / (8 * ROWS), job = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
-  const int slice = job / (8 * eighth), i = job % (8 * eighth);
-  const int row0 = (i % eighth * 8 + i / eighth) * ROWS, j0 = blockIdx.y * 16 * Q;
-  if (row0 >= rows.T) return;
-  const int begin = slice * slice_cols, end = min(C, begin + slice_cols);
+  const int row0 = blockIdx.x * ROWS, j0 = blockIdx.z * 16 * Q;
+  const int begin = blockIdx.y * slice_cols, end = min(C, begin + slice_cols);
   const int id = adapter_of(rows, row0 + lane);
   const uint16_t* xr[4];
 #pragma unroll
@@ -240,8 +236,8 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
       v4f v = *reinterpret_cast<const v4f*>(sums + row * RS + j);
 #pragma unroll
       for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + (w * ROWS + row) * RS + j);
-      if (slices == 1) v *= scale;
-      *reinterpret_cast<v4f*>(part + ((int64_t)slice * rows.T + row0 + row) * rows.R + j0 + j) = v;
+      if (gridDim.y == 1) v *= scale;
+      *reinterpret_cast<v4f*>(part + ((int64_t)blockIdx.y * rows.T + row0 + row) * rows.R + j0 + j) = v;
     }
     __syncthreads();
   }
@@ -824,12 +820,12 @@ template <typename F, bool kWide>
 void launch_down(const Rows& rows, const uint16_t* x, int64_t C, const void* f, int slices, float* part, hipStream_t st) {
   const int64_t cols = ((C + slices - 1) / slices + 255) / 256 * 256, one = (int64_t)rows.R * C;
   const int q = tiles_of(rows.R);
-  const dim3 grid((unsigned)((rows.T + 8 * ROWS - 1) / (8 * ROWS) * 8 * slices), (unsigned)((rows.R + 16 * q - 1) / (16 * q)));
+  const dim3 grid((unsigned)((rows.T + ROWS - 1) / ROWS), (unsigned)slices, (unsigned)((rows.R + 16 * q - 1) / (16 * q)));
   const int lds = 4 * ROWS * (16 * q + 4) * 4;
   const F* factor = static_cast<const F*>(f);
   auto go = [&](auto kernel, std::atomic<uint64_t>& once) {
     (void)k2q_lds_limit_once(kernel, lds, once);
-    hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, st, rows, x, (int)C, factor, one, (int)cols, slices, part);
+    hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, st, rows, x, (int)C, factor, one, (int)cols, part);
   };
   static std::atomic<uint64_t> once[3];
   if (q == 1) go(down_kernel<F, kWide, 1>, once[0]);
