@@ -253,7 +253,8 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 // 8 apart in a fragment and measured slower: 95 -> 135 us at 4 x 768 rows x 6144 -> 16384 with rank 64 in f32.)
 template <typename F, bool kWide>
 __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, const uint16_t* y, int C, const F* factor,
-                                                     int64_t one, int held, int passes, int groups, uint16_t* out) {
+                                                     int64_t one, int held, int passes, int groups, int slices, float* sum,
+                                                     uint16_t* out) {
   constexpr int TR = 4;                 // tiles of 16 rows
   extern __shared__ uint16_t halves[];  // u in two halves of ROWS x RS
   const int RS = held + 8;              // 16 bytes off the banks' turn
@@ -269,6 +270,7 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
     left &= ~mask;
     const int r = rank_of(rows, a);
     const F* f = factor + (int64_t)max(a, 0) * one;
+    const float scale = slices > 1 && a >= 0 ? scale_of(rows, a) : 1.f;
     for (int p = 0; p < passes; ++p) {
       const int c0 = (first + p) * 256 + 64 * wave;
       const bool in = c0 < C;
@@ -292,7 +294,22 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
             float v[8] = {};
             if ((mask >> row & 1) && j < n) {
               const float* q = u + (int64_t)(row0 + row) * rows.R + j0 + j;
-              const v4f b = *reinterpret_cast<const v4f*>(q), c = *reinterpret_cast<const v4f*>(q + 4);
+              v4f b = *reinterpret_cast<const v4f*>(q), c = *reinterpret_cast<const v4f*>(q + 4);
+              if (slices > 1) {       // as join_kernel does it
+                const int64_t next = (int64_t)rows.T * rows.R;
+#pragma unroll 4
+                for (int s = 1; s < slices; ++s) {
+                  b += *reinterpret_cast<const v4f*>(q + s * next);
+                  c += *reinterpret_cast<const v4f*>(q + s * next + 4);
+                }
+                b *= scale;
+                c *= scale;
+                if (sum && first + p == 0) {
+                  float* to = sum + (int64_t)(row0 + row) * rows.R + j0 + j;
+                  *reinterpret_cast<v4f*>(to) = b;
+                  *reinterpret_cast<v4f*>(to + 4) = c;
+                }
+              }
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 v[e] = b[e];
@@ -506,7 +523,7 @@ __global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float*
 }
 
 // The slices' sums, scaled: once, ahead of an "up" whose workgroups would each add them up (4 x 768 rows, 22 slices of 64
-// ranks, 24 workgroups a row: 57 us; added up once, both take 24), or where no "up" is wanted.
+// ranks, 24 workgroups a row: 57 us; added up once, both take 24), or where the sums over rows want them.
 __global__ __launch_bounds__(THREADS) void join_kernel(Rows rows, const float* part, int slices, float* sum) {
   const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
   const int row = (int)(i / rows.R), j = (int)(i % rows.R);
@@ -833,25 +850,38 @@ void launch_down(const Rows& rows, const uint16_t* x, int64_t C, const void* f, 
   else go(down_kernel<F, kWide, 4>, once[2]);
 }
 
+void launch_join(const Rows& rows, const float* part, int slices, float* sum, hipStream_t st) {
+  if (slices == 1) return;      // scaled already
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(((int64_t)rows.T * rows.R / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0,
+                     st, rows, part, slices, sum);
+}
+
+// Slices that the "up" adds up itself, in the order of the join: where all of its workgroups together read 32 MB or less of
+// them, which costs less than a launch.  us of the forward with and without the join, by what they read: 685 x 640 -> 448, rank
+// 16 (0.3 MB) 12.6 / 10.2; 1000 x 2560 -> 6144, rank 16 (15 MB) 26.0 / 25.3; 546 x 1600 -> 8384, rank 64 (32 MB) 20.8 / 19.6;
+// 4000 x 6144 -> 16384, rank 16 (66 MB) 81.8 / 84.9; 4 x 768 x 6144 -> 16384, rank 64 (201 MB) 92.8 / 99.6.
+constexpr int64_t JOIN = 32 << 20;
+
 // Passes over 256 columns with one staging of u: two (four where the factor's rows are long and its loads wider), fewer
 // where a CU would not get six workgroups.  4 x 4608 rows x 6144 at 1 / 2 / 4 passes 182 / 172 / 177 us, 16896 x 16384 (dx, with
 // the factors' sums) 432 / 409 / 396.
 template <typename F, bool kWide>
-void launch_up(const Rows& rows, const float* u, const uint16_t* y, int64_t C, const void* f, uint16_t* out,
-               hipStream_t st) {
+void launch_up(const Rows& rows, const float* part, int slices, float* sum, const uint16_t* y, int64_t C, const void* f,
+               uint16_t* out, hipStream_t st) {
   const int64_t tiles = (rows.T + ROWS - 1) / ROWS, blocks = (C + 255) / 256, most = kWide ? 4 : 2;
   int64_t passes = tiles * blocks / (6 * (int64_t)k2q_cu_count());
   passes = passes < 1 ? 1 : passes > most ? most : passes;
   const int64_t groups = (blocks + passes - 1) / passes;
   const int held = rows.R < RANKS ? (rows.R + 31) & ~31 : RANKS;
+  if (slices > 1 && (int64_t)slices * rows.T * rows.R * 4 * groups > JOIN) {
+    float* to = sum ? sum : const_cast<float*>(part);       // or the first slice's place
+    launch_join(rows, part, slices, to, st);
+    part = to;
+    slices = 1;
+  }
   hipLaunchKernelGGL((up_kernel<F, kWide>), dim3((unsigned)(tiles * groups)), dim3(THREADS), 2 * ROWS * (held + 8) * 2, st,
-                     rows, u, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups, out);
-}
-
-void launch_join(const Rows& rows, const float* part, int slices, float* sum, hipStream_t st) {
-  if (slices == 1) return;      // scaled already
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(((int64_t)rows.T * rows.R / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0,
-                     st, rows, part, slices, sum);
+                     rows, part, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups,
+                     slices, sum, out);
 }
 
 // Few rows: the form of single rows, whose time grows with the rows, where that of tiles grows with the adapters that a tile
@@ -935,15 +965,13 @@ extern "C" int k2q_bank_fwd(const k2q_bank* b, int64_t T, int64_t per, const uin
     return k2q_launch_status();
   }
   const int slices = down_slices(T, b->K, b->R);
-  if (!u) u = part;       // the first slice's place
+  if (slices == 1 && u) part = u;
   if (b->dtype == K2Q_DTYPE_F32) {
-    launch_down<float, true>(rows, x, b->K, b->A, slices, slices == 1 ? u : part, st);
-    launch_join(rows, part, slices, u, st);
-    launch_up<float, false>(rows, u, y, b->N, b->B, out, st);
+    launch_down<float, true>(rows, x, b->K, b->A, slices, part, st);
+    launch_up<float, false>(rows, part, slices, u, y, b->N, b->B, out, st);
   } else {
-    launch_down<uint16_t, true>(rows, x, b->K, b->A, slices, slices == 1 ? u : part, st);
-    launch_join(rows, part, slices, u, st);
-    launch_up<uint16_t, false>(rows, u, y, b->N, b->B, out, st);
+    launch_down<uint16_t, true>(rows, x, b->K, b->A, slices, part, st);
+    launch_up<uint16_t, false>(rows, part, slices, u, y, b->N, b->B, out, st);
   }
   return k2q_launch_status();
 }
@@ -970,16 +998,20 @@ extern "C" int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uin
   const bool f32 = b->dtype == K2Q_DTYPE_F32;
   float* part = static_cast<float*>(ws);
   float* g = dA || dB ? part + slices * T * b->R : part;
+  int left = slices;        // of g, for the "up"
   if (dx || dA) {
     if (f32) launch_down<float, false>(rows, dy, b->N, b->B, slices, slices == 1 ? g : part, st);
     else launch_down<uint16_t, false>(rows, dy, b->N, b->B, slices, slices == 1 ? g : part, st);
-    launch_join(rows, part, slices, g, st);
+    if (dA || slices == 1) {
+      launch_join(rows, part, slices, g, st);
+      left = 1;
+    }
   }
   // dx last: dy is still in the last-level cache for dB, and what dx would push out of it is read no more
   auto input = [&] {
     if (!dx) return k2q_launch_status();
-    if (f32) launch_up<float, true>(rows, g, base, b->K, b->A, dx, st);
-    else launch_up<uint16_t, true>(rows, g, base, b->K, b->A, dx, st);
+    if (f32) launch_up<float, true>(rows, left > 1 ? part : g, left, nullptr, base, b->K, b->A, dx, st);
+    else launch_up<uint16_t, true>(rows, left > 1 ? part : g, left, nullptr, base, b->K, b->A, dx, st);
     return k2q_launch_status();
   };
   if (!dA && !dB) return input();
