@@ -19,6 +19,7 @@ namespace {
 constexpr int ROWS = 64;              // rows of a tile
 constexpr int THREADS = 256;          // 4 waves
 constexpr int RANKS = 128;            // most ranks that an "up" workgroup holds at once
+constexpr int LS = 72;                // a wave's 64 columns of a row in LDS, 16 bytes off the banks' turn
 
 struct Rows {
   const void* ids;
@@ -248,18 +249,22 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 // ---------------------------------------------------------------------------------------------------------------
 // A workgroup: 64 rows, 256 columns at a time.  It holds u in LDS in two bf16 halves; a wave takes 64 columns of all rows, so
 // that a factor's fragment (in f32 split on its way) serves four tiles, and y's vectors are on their way while it computes.  The
-// order of a tile's columns among MFMA rows is chosen so that a lane ends with 16 columns of a row in two pieces of 8, and 4
-// lanes with 64 bytes in one: y comes and goes in vectors.  (Whole lines at once, 16 lanes to 256 bytes, want the factor's rows
-// 8 apart in a fragment and measured slower: 95 -> 135 us at 4 x 768 rows x 6144 -> 16384 with rank 64 in f32.)
+// order of a tile's columns among MFMA rows is chosen so that a lane ends with 16 columns of a row in two pieces of 8.  y comes
+// and out goes in whole lines of 128 bytes, 8 rows an instruction, past the cache, and changes places with the lanes' pieces in
+// LDS.  In pieces (4 lanes to 64 bytes of a row) and through the cache the forward took 172 us for 153 at 4 x 4608 rows x 6144 (226
+// MB of y and of out: now 5.4 TB/s), 246 for 221 at 16896 x 16384 -> 6144, 93 for 83 at 4 x 768 x 6144 -> 16384 with rank 64 in f32,
+// and the long dx 127 for 86; a call between the base's product and a reader of out gains as much (57 MB 91.5 -> 83, 12 MB 30.3 ->
+// 29.6 with both).
 template <typename F, bool kWide>
 __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, const uint16_t* y, int C, const F* factor,
                                                      int64_t one, int held, int passes, int groups, int slices, float* sum,
                                                      uint16_t* out) {
   constexpr int TR = 4;                 // tiles of 16 rows
-  extern __shared__ uint16_t halves[];  // u in two halves of ROWS x RS
+  extern __shared__ uint16_t halves[];  // u in two halves of ROWS x RS, then a place of ROWS x LS for each wave
   const int RS = held + 8;              // 16 bytes off the banks' turn
-  uint16_t *hi = halves, *lo = halves + ROWS * RS;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
+  uint16_t *hi = halves, *lo = halves + ROWS * RS, *mine = halves + 2 * ROWS * RS + wave * ROWS * LS;
+  const int at = lane / 8 * LS + 8 * (lane % 8);      // a lane's 16 bytes of a line
   // a row's columns on neighbouring workgroups
   const int row0 = blockIdx.x / groups * ROWS, first = blockIdx.x % groups * passes;
   const int id = adapter_of(rows, row0 + lane);
@@ -271,18 +276,20 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
     const int r = rank_of(rows, a);
     const F* f = factor + (int64_t)max(a, 0) * one;
     const float scale = slices > 1 && a >= 0 ? scale_of(rows, a) : 1.f;
+    uint32_t live = 0;      // a lane's rows of lines, 8 k + lane / 8
+#pragma unroll
+    for (int k = 0; k < 8; ++k) live |= (uint32_t)(mask >> (8 * k + lane / 8) & 1) << k;
     for (int p = 0; p < passes; ++p) {
       const int c0 = (first + p) * 256 + 64 * wave;
       const bool in = c0 < C;
-      v4u old[TR][2] = {};
+      const int64_t line = (int64_t)(row0 + lane / 8) * C + c0 + 8 * (lane % 8);
+      v4u old[8] = {};
+      asm volatile("" : "+v"(live));      // tested where it is wanted: eight masks held through the loop spill scalars
       if (y && in) {
+        const uint16_t* from = y + line;
 #pragma unroll
-        for (int t = 0; t < TR; ++t) {
-          if (!(mask >> (16 * t + m) & 1)) continue;
-          const uint16_t* b = y + (int64_t)(row0 + 16 * t + m) * C + c0 + 8 * g;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) old[t][h] = *reinterpret_cast<const v4u*>(b + 32 * h);
-        }
+        for (int k = 0; k < 8; ++k, from += 8 * (int64_t)C)
+          if (live >> k & 1) old[k] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(from));
       }
       v4f acc[TR][4] = {};
       for (int j0 = 0; j0 < r; j0 += held) {
@@ -345,8 +352,8 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
             }
 #pragma unroll
             for (int t = 0; t < TR; ++t) {
-              const int at = (16 * t + m) * RS + j + 8 * g;
-              const v8bf uh = *reinterpret_cast<const v8bf*>(hi + at), ul = *reinterpret_cast<const v8bf*>(lo + at);
+              const int e = (16 * t + m) * RS + j + 8 * g;
+              const v8bf uh = *reinterpret_cast<const v8bf*>(hi + e), ul = *reinterpret_cast<const v8bf*>(lo + e);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 acc[t][q] = mfma(fr.p[0][q], uh, acc[t][q]);
@@ -358,14 +365,24 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
         }
       }
       if (!in) continue;
-      // a lane: row 16 t + m, columns 32 h + 8 g + e
+      // a lane: row 16 t + m, columns 32 h + 8 g + e.  The wave's own place: its LDS operations stay in order
+      v4u pieces[TR][2] = {};
+      uint16_t* place = mine + m * LS + 8 * g;
+      if (y) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) *reinterpret_cast<v4u*>(mine + at + 8 * k * LS) = old[k];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < TR; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) pieces[t][h] = *reinterpret_cast<const v4u*>(place + 16 * t * LS + 32 * h);
+        __builtin_amdgcn_wave_barrier();
+      }
 #pragma unroll
       for (int t = 0; t < TR; ++t) {
-        if (!(mask >> (16 * t + m) & 1)) continue;
-        uint16_t* to = out + (int64_t)(row0 + 16 * t + m) * C + c0 + 8 * g;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const v4u b = old[t][h];
+          const v4u b = pieces[t][h];
           v4u o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -379,9 +396,17 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
             }
             o[i] = pack_bf16x2(v[0], v[1]);
           }
-          *reinterpret_cast<v4u*>(to + 32 * h) = o;
+          *reinterpret_cast<v4u*>(place + 16 * t * LS + 32 * h) = o;
         }
       }
+      __builtin_amdgcn_wave_barrier();
+      uint16_t* to = out + line;
+#pragma unroll
+      for (int k = 0; k < 8; ++k, to += 8 * (int64_t)C) {
+        const v4u o = *reinterpret_cast<const v4u*>(mine + at + 8 * k * LS);
+        if (live >> k & 1) __builtin_nontemporal_store(o, reinterpret_cast<v4u*>(to));
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -863,8 +888,8 @@ void launch_join(const Rows& rows, const float* part, int slices, float* sum, hi
 constexpr int64_t JOIN = 32 << 20;
 
 // Passes over 256 columns with one staging of u: two (four where the factor's rows are long and its loads wider), fewer
-// where a CU would not get six workgroups.  4 x 4608 rows x 6144 at 1 / 2 / 4 passes 182 / 172 / 177 us, 16896 x 16384 (dx, with
-// the factors' sums) 432 / 409 / 396.
+// where a CU would not get six workgroups.  4 x 4608 rows x 6144 at 1 / 2 / 4 passes 163 / 154 / 154 us, 16896 x 16384 (dx, with
+// the factors' sums) 388 / 365 / 355.
 template <typename F, bool kWide>
 void launch_up(const Rows& rows, const float* part, int slices, float* sum, const uint16_t* y, int64_t C, const void* f,
                uint16_t* out, hipStream_t st) {
@@ -879,9 +904,12 @@ void launch_up(const Rows& rows, const float* part, int slices, float* sum, cons
     part = to;
     slices = 1;
   }
-  hipLaunchKernelGGL((up_kernel<F, kWide>), dim3((unsigned)(tiles * groups)), dim3(THREADS), 2 * ROWS * (held + 8) * 2, st,
-                     rows, part, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups,
-                     slices, sum, out);
+  static std::atomic<uint64_t> once;
+  (void)k2q_lds_limit_once(up_kernel<F, kWide>, (2 * ROWS * (RANKS + 8) + 4 * ROWS * LS) * 2, once);
+  const int lds = (2 * ROWS * (held + 8) + 4 * ROWS * LS) * 2;
+  hipLaunchKernelGGL((up_kernel<F, kWide>), dim3((unsigned)(tiles * groups)), dim3(THREADS), lds, st, rows,
+                     part, y, (int)C, static_cast<const F*>(f), (int64_t)rows.R * C, held, (int)passes, (int)groups, slices, sum,
+                     out);
 }
 
 // Few rows: the form of single rows, whose time grows with the rows, where that of tiles grows with the adapters that a tile
