@@ -11,6 +11,8 @@
 //
 // Rows may come in any order.  A tile of 64 rows goes over the adapters that it finds in it, one after another: rows of one
 // request lie together, so that is one adapter, or two, in all but the smallest batches.
+#include <type_traits>
+
 #include "k2q_common.h"
 #include "rotation.h"
 
@@ -252,9 +254,9 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
 // order of a tile's columns among MFMA rows is chosen so that a lane ends with 16 columns of a row in two pieces of 8.  y comes
 // and out goes in whole lines of 128 bytes, 8 rows an instruction, past the cache, and changes places with the lanes' pieces in
 // LDS.  In pieces (4 lanes to 64 bytes of a row) and through the cache the forward took 172 us for 153 at 4 x 4608 rows x 6144 (226
-// MB of y and of out: now 5.4 TB/s), 246 for 221 at 16896 x 16384 -> 6144, 93 for 83 at 4 x 768 x 6144 -> 16384 with rank 64 in f32,
-// and the long dx 127 for 86; a call between the base's product and a reader of out gains as much (57 MB 91.5 -> 83, 12 MB 30.3 ->
-// 29.6 with both).
+// MB of y and of out: 86 us, 5.4 TB/s), 246 for 222 at 16896 x 16384 -> 6144 with 389 for 346 in the backward, 93 for 83 at
+// 4 x 768 x 6144 -> 16384 with rank 64 in f32; a call between the base's product and a reader of out gains as much (57 MB 91.5 ->
+// 83, 12 MB 30.3 -> 29.6 with both).
 template <typename F, bool kWide>
 __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, const uint16_t* y, int C, const F* factor,
                                                      int64_t one, int held, int passes, int groups, int slices, float* sum,
@@ -330,18 +332,22 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
           __syncthreads();
         }
         if (in) {
-          for (int j = 0; j < n; j += 32) {
-            constexpr int N = kF32<F> ? 2 : 1;
+          constexpr int N = kF32<F> ? 2 : 1;
+          // 32 ranks of the reduction, or the last 16, of which lanes g and g + 2 then have the same ones: those below 2 the
+          // factor's (f32) or u's (bf16 factors) upper parts, the others the lower, and a product fewer does (dx of 16896 x 16384,
+          // rank 16 in f32, with its "down": 127 -> 120 us)
+          auto step = [&](int j, auto last) {
+            const int of = j + 8 * (last ? g % 2 : g);
+            const bool upper = g < 2;
             Frag<F, 4, N> fr;
-            const bool some = j + 8 * g < n;
             if constexpr (kWide) {
               // MFMA row m of tile q: column 32 (m / 2 % 2) + 8 (m / 4) + 4 (m % 2) + q, four tiles with one load
               const int col = 32 * (m % 4 / 2) + 8 * (m / 4) + 4 * (m % 2);
-              load_strided<F, 4, N>(f + (int64_t)(j0 + j + 8 * g) * C + c0 + col, C, some, fr);
+              load_strided<F, 4, N>(f + (int64_t)(j0 + of) * C + c0 + col, C, true, fr);
             } else {
               // row m of tile q: column 32 (q / 2) + 8 (m / 4) + 4 (q % 2) + m % 4
-              const bool ok[2] = {some, some};
-              const F* b = f + (int64_t)(c0 + 8 * (m / 4) + m % 4) * rows.R + j0 + j + 8 * g;
+              const bool ok[2] = {of < n, of < n};      // always: a step later than without it, 83 us for 87 at rank 64 in f32
+              const F* b = f + (int64_t)(c0 + 8 * (m / 4) + m % 4) * rows.R + j0 + of;
               Frag<F, 2, N> half[2];
               load_contiguous<F, 2, N>(b, 4 * (int64_t)rows.R, ok, half[0]);
               load_contiguous<F, 2, N>(b + 32 * (int64_t)rows.R, 4 * (int64_t)rows.R, ok, half[1]);
@@ -350,18 +356,30 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
 #pragma unroll
                 for (int k = 0; k < N; ++k) fr.p[k][q] = half[q / 2].p[k][q % 2];
             }
+            if constexpr (last && N > 1) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) fr.p[0][q] = upper ? fr.p[0][q] : fr.p[1][q];
+            }
 #pragma unroll
             for (int t = 0; t < TR; ++t) {
-              const int e = (16 * t + m) * RS + j + 8 * g;
+              const int e = (16 * t + m) * RS + of;
+              if constexpr (last && N == 1) {
+                const v8bf u = *reinterpret_cast<const v8bf*>((upper ? hi : lo) + e);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[t][q] = mfma(fr.p[0][q], u, acc[t][q]);
+                continue;
+              }
               const v8bf uh = *reinterpret_cast<const v8bf*>(hi + e), ul = *reinterpret_cast<const v8bf*>(lo + e);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 acc[t][q] = mfma(fr.p[0][q], uh, acc[t][q]);
                 acc[t][q] = mfma(fr.p[0][q], ul, acc[t][q]);
-                if constexpr (N > 1) acc[t][q] = mfma(fr.p[1][q], uh, acc[t][q]);
+                if constexpr (!last && N > 1) acc[t][q] = mfma(fr.p[1][q], uh, acc[t][q]);
               }
             }
-          }
+          };
+          for (int j = 0; j + 32 <= n; j += 32) step(j, std::false_type{});
+          if (n % 32) step(n / 32 * 32, std::true_type{});
         }
       }
       if (!in) continue;
