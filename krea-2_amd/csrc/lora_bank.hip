@@ -468,23 +468,14 @@ __device__ __forceinline__ RowPart row_part(int T, int parts) {
 
 int64_t row_parts(int64_t T, int64_t parts) { return T * (parts < 8 ? parts : (parts + 7) / 8 * 8); }
 
-// Down: a wave takes 4 ranks over the slice's columns, a workgroup 16.
+// A wave's sums of four ranks over columns begin .. end of a row; f: the first of them.
 template <typename F>
-__global__ __launch_bounds__(THREADS) void down_row_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
-                                                           int slice_cols, int slices, float* part) {
-  const RowPart at = row_part(rows.T, slices * (rows.R / 16));
-  const int row = at.row, slice = at.part % slices, lane = threadIdx.x % 64;
-  const int j = at.part / slices * 16 + threadIdx.x / 64 * 4;
-  const int a = __builtin_amdgcn_readfirstlane(adapter_of(rows, row));
-  if (j >= rank_of(rows, a)) return;
-  const int begin = slice * slice_cols, end = min(C, begin + slice_cols);
-  const F* f = factor + a * one + (int64_t)j * C;
-  const uint16_t* xr = x + (int64_t)row * C;
+__device__ __forceinline__ v4f four_ranks(const uint16_t* x, const F* f, int C, int begin, int end) {
   float acc[4] = {};
 #pragma unroll 2
-  for (int c = begin + 8 * lane; c < end; c += 512) {
+  for (int c = begin + 8 * (int)(threadIdx.x % 64); c < end; c += 512) {
     float xv[8], fv[4][8];
-    load8(xr + c, xv);
+    load8(x + c, xv);
 #pragma unroll
     for (int q = 0; q < 4; ++q) load8(f + (int64_t)q * C + c, fv[q]);
 #pragma unroll
@@ -495,14 +486,29 @@ __global__ __launch_bounds__(THREADS) void down_row_kernel(Rows rows, const uint
   v4f sum;
 #pragma unroll
   for (int q = 0; q < 4; ++q) sum[q] = k2q_rot::wave_sum(acc[q]);
+  return sum;
+}
+
+// Down: a wave takes 4 ranks over the slice's columns, a workgroup 16.
+template <typename F>
+__global__ __launch_bounds__(THREADS) void down_row_kernel(Rows rows, const uint16_t* x, int C, const F* factor, int64_t one,
+                                                           int slice_cols, int slices, float* part) {
+  const RowPart at = row_part(rows.T, slices * (rows.R / 16));
+  const int row = at.row, slice = at.part % slices, lane = threadIdx.x % 64;
+  const int j = at.part / slices * 16 + threadIdx.x / 64 * 4;
+  const int a = __builtin_amdgcn_readfirstlane(adapter_of(rows, row));
+  if (j >= rank_of(rows, a)) return;
+  const int begin = slice * slice_cols, end = min(C, begin + slice_cols);
+  const v4f sum = four_ranks(x + (int64_t)row * C, factor + a * one + (int64_t)j * C, C, begin, end);
   if (lane == 0) *reinterpret_cast<v4f*>(part + ((int64_t)slice * rows.T + row) * rows.R + j) = sum;
 }
 
 // Up, from B: L lanes share a column's ranks, 16 bytes each, and a wave's 64 columns come in L steps; then every lane has one
-// column's sum.
-template <typename F, int L>
+// column's sum.  kBoth: the workgroup makes the row's u itself, as the "down" does it in one slice.
+template <typename F, int L, bool kBoth>
 __global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float* part, int slices, float* sum, const uint16_t* y,
-                                                         int C, const F* factor, int64_t one, uint16_t* out) {
+                                                         int C, const F* factor, int64_t one, const uint16_t* x, int K,
+                                                         const F* A, uint16_t* out) {
   constexpr int E = 16 / sizeof(F);
   extern __shared__ float u[];          // R
   const RowPart of = row_part(rows.T, (C + THREADS - 1) / THREADS);
@@ -523,14 +529,24 @@ __global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float*
   const float base = y && in ? bf16_bits_to_f32(y[(int64_t)row * C + mine]) : 0.f;
   if (r) {
     const float scale = scale_of(rows, a);
-    for (int j = threadIdx.x; j < r; j += THREADS) {
-      const float* p = part + (int64_t)row * rows.R + j;
-      float v = *p;
+    if constexpr (kBoth) {
+      const F* from = A + (int64_t)a * rows.R * K;
+      for (int j = threadIdx.x / 64 * 4; j < r; j += 16) {
+        const v4f v = four_ranks(x + (int64_t)row * K, from + (int64_t)j * K, K, 0, K) * scale;
+        if (lane) continue;
+        *reinterpret_cast<v4f*>(u + j) = v;
+        if (sum && of.part == 0) *reinterpret_cast<v4f*>(sum + (int64_t)row * rows.R + j) = v;
+      }
+    } else {
+      for (int j = threadIdx.x; j < r; j += THREADS) {
+        const float* p = part + (int64_t)row * rows.R + j;
+        float v = *p;
 #pragma unroll 4
-      for (int s = 1; s < slices; ++s) v += p[(int64_t)s * rows.T * rows.R];
-      v *= scale;
-      u[j] = v;
-      if (sum && of.part == 0) sum[(int64_t)row * rows.R + j] = v;
+        for (int s = 1; s < slices; ++s) v += p[(int64_t)s * rows.T * rows.R];
+        v *= scale;
+        u[j] = v;
+        if (sum && of.part == 0) sum[(int64_t)row * rows.R + j] = v;
+      }
     }
     __syncthreads();
   }
@@ -953,23 +969,37 @@ int row_slices(int64_t T, int64_t C, int64_t R) {
   return (int)((C + cols - 1) / cols);
 }
 
+// One launch, whose workgroups each make their row's u: where an adapter's A has 192 KB at most, and all workgroups together
+// read 32 MB at most.  us in a graph, two launches / one, bf16: 512 -> 1024 (f32), 1 and 64 rows 4.7 / 3.1, 5.3 / 3.5; 2560 ->
+// 2560, 1, 32 (26 MB) and 64 rows (52 MB) 4.9 / 3.9, 5.3 / 4.8, 6.1 / 6.9; 6144 -> 1536, rank 16 (192 KB) 5.6 / 5.6, and the host
+// makes one launch less; 1024 -> 4096, rank 64 in f32 (256 KB) 5.9 / 7.3; 6144 -> 16384, 8 rows (101 MB) 6.1 / 7.1.
+constexpr int64_t ONE = 192 << 10, ALL = 32 << 20;
+
 template <typename F>
 void launch_rows(const Rows& rows, const uint16_t* x, int64_t K, const void* A, float* part, float* sum, const uint16_t* y,
                  int64_t N, const void* B, uint16_t* out, hipStream_t st) {
+  const int64_t parts = (N + THREADS - 1) / THREADS;
+  const int64_t read = rows.R * K * (int64_t)sizeof(F);
+  const bool both = read <= ONE && rows.T * parts * read <= ALL;
   const int slices = row_slices(rows.T, K, rows.R);
   const int64_t cols = ((K + slices - 1) / slices + 511) / 512 * 512;
-  hipLaunchKernelGGL(down_row_kernel<F>, dim3((unsigned)row_parts(rows.T, slices * (rows.R / 16))), dim3(THREADS), 0, st, rows,
-                     x, (int)K, static_cast<const F*>(A), (int64_t)rows.R * K, (int)cols, slices, part);
-  const dim3 grid((unsigned)row_parts(rows.T, (N + THREADS - 1) / THREADS));
-  const int lanes = (int)(rows.R * sizeof(F) / 16);
+  if (!both)
+    hipLaunchKernelGGL(down_row_kernel<F>, dim3((unsigned)row_parts(rows.T, slices * (rows.R / 16))), dim3(THREADS), 0, st,
+                       rows, x, (int)K, static_cast<const F*>(A), (int64_t)rows.R * K, (int)cols, slices, part);
+  const dim3 grid((unsigned)row_parts(rows.T, parts));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(THREADS), (size_t)rows.R * 4, st, rows, part, slices, sum, y, (int)N,
-                       static_cast<const F*>(B), (int64_t)rows.R * N, out);
+                       static_cast<const F*>(B), (int64_t)rows.R * N, x, (int)K, static_cast<const F*>(A), out);
   };
-  if (lanes <= 2) go(up_row_kernel<F, 2>);
-  else if (lanes <= 4) go(up_row_kernel<F, 4>);
-  else if (lanes <= 8) go(up_row_kernel<F, 8>);
-  else go(up_row_kernel<F, 16>);
+  auto of = [&](auto b) {
+    const int lanes = (int)(rows.R * sizeof(F) / 16);
+    if (lanes <= 2) go(up_row_kernel<F, 2, b.value>);
+    else if (lanes <= 4) go(up_row_kernel<F, 4, b.value>);
+    else if (lanes <= 8) go(up_row_kernel<F, 8, b.value>);
+    else go(up_row_kernel<F, 16, b.value>);
+  };
+  if (both) of(std::true_type{});
+  else of(std::false_type{});
 }
 
 struct Sums {

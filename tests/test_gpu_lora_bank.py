@@ -128,6 +128,8 @@ def _values_and_gradients(k2, dev, lead, of, count, R, K, N, dtype, how):
     ((176,), (176,), 7, 48, 320, 64), ((177,), (177,), 7, 48, 320, 64),         # rule between them
     ((768,), (768,), 64, 16, 64, 192), ((769,), (769,), 64, 16, 64, 192),
     ((5, 20), (5,), 5, 64, 128, 64), ((3, 50), (3,), 5, 64, 128, 64),
+    ((2, 30), (2,), 3, 32, 1536, 320), ((2, 30), (2,), 3, 32, 1600, 320),       # single rows in one launch, or in two
+    ((3,), (3,), 2, 16, 3008, 256), ((1,), (1,), 1, 16, 6144, 64), ((700,), (700,), 50, 16, 64, 8192),
     ((300,), (300,), 6, 144, 1088, 192), ((4, 500), (4,), 3, 64, 1088, 5120),   # slices that "up" adds up, and the join
     ((1000,), (1000,), 40, 64, 1088, 576), ((300,), (300,), 6, 144, 64, 128), ((11, 40), (11,), 9, 272, 128, 1344)])
 def test_single_rows_and_tiles(k2, dev, lead, of, count, R, K, N, dtype, how):
