@@ -398,10 +398,11 @@ int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, int64_t M, i
 
 /* Low-rank adapters of many requests beside one projection (LoRALinear.forward, lora.py:43-48, with an adapter of its own
  * for every row).  Row t of T has the adapter a = ids[t / per] of a bank (T a multiple of per), none where that is outside
- * 0 .. count - 1; A count x R x K and B count x N x R, both bf16 or f32; of adapter a the first ranks[a] (NULL: R; rounded up
- * to 16) ranks count, f = scale * scales[a] (NULL: scale):
+ * 0 .. count - 1; A count x R x K and B count x N x R, both bf16 or f32; of adapter a the first ranks[a] (NULL: R) ranks count,
+ * whatever the storage behind them holds, f = scale * scales[a] (NULL: scale):
  *   u[t] = f x[t] A_a^T,  out[t] = bf16(y[t] + u[t] B_a^T)   (y[t] for a row without adapter; y NULL: zeros; out may be y)
- * u (T x R f32, nullable) is what the backward reads; ranks past an adapter's, and rows without one, are not written.
+ * u (T x R f32, nullable) is what the backward reads; rows without an adapter, and ranks past its own rounded up to 16, are not
+ * written.
  * k2q_bank_bwd: g[t] = f dy[t] B_a,  dx[t] = bf16(base[t] + g[t] A_a) (base nullable: zeros; dx may be base),
  *   dA_a = sum_t g[t]^T x[t] and dB_a = sum_t dy[t]^T u[t] over the adapter's rows, in the factors' type, zeros for an adapter
  *   without rows and for ranks past its own.  dx, dA (with x), dB (with u) are nullable; one at least is given.

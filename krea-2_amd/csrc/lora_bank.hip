@@ -43,12 +43,30 @@ __device__ __forceinline__ int adapter_at(const Rows& a, int i) {
 
 __device__ __forceinline__ int adapter_of(const Rows& a, int row) { return row >= a.T ? -2 : adapter_at(a, row / a.per); }
 
-// Ranks of an adapter that hold something, in whole MFMA tiles.
+// Ranks of an adapter that count.
 __device__ __forceinline__ int rank_of(const Rows& a, int id) {
   if (id < 0) return 0;
   if (!a.ranks) return a.R;
-  const int r = min(a.ranks[id], a.R);
-  return r <= 0 ? 0 : (r + 15) & ~15;
+  return max(0, min(a.ranks[id], a.R));
+}
+
+// The same in whole MFMA tiles: what u and g hold, zeros behind the adapter's own ranks.  Storage between the two may hold
+// anything (zeros would not do: 0 x NaN is NaN), so the sums there are dropped and a factor's values taken out.
+__device__ __forceinline__ int whole(int rank) { return (rank + 15) & ~15; }
+
+// A vector of ranks j .. j + 3, of which those below r count.
+__device__ __forceinline__ v4f counted(v4f v, int j, int r) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = j + e < r ? v[e] : 0.f;
+  return v;
+}
+
+// 8 bf16 values, of which the first n count.
+__device__ __forceinline__ v8bf counted(v8bf v, int n) {
+  v4u w = __builtin_bit_cast(v4u, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] &= (2 * i < n ? 0xffffu : 0u) | (2 * i + 1 < n ? 0xffff0000u : 0u);
+  return __builtin_bit_cast(v8bf, w);
 }
 
 __device__ __forceinline__ float scale_of(const Rows& a, int id) { return a.scales ? a.mul * a.scales[id] : a.mul; }
@@ -235,11 +253,12 @@ __global__ __launch_bounds__(THREADS) void down_kernel(Rows rows, const uint16_t
     __syncthreads();
     for (int i = threadIdx.x; i < ROWS * 4 * Q; i += THREADS) {
       const int row = i / (4 * Q), j = 4 * (i % (4 * Q));
-      if (!(mask >> row & 1) || j0 + j >= r) continue;
+      if (!(mask >> row & 1) || j0 + j >= whole(r)) continue;
       v4f v = *reinterpret_cast<const v4f*>(sums + row * RS + j);
 #pragma unroll
       for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + (w * ROWS + row) * RS + j);
       if (gridDim.y == 1) v *= scale;
+      if constexpr (!kWide) v = counted(v, j0 + j, r);      // else nothing was loaded there
       *reinterpret_cast<v4f*>(part + ((int64_t)blockIdx.y * rows.T + row0 + row) * rows.R + j0 + j) = v;
     }
     __syncthreads();
@@ -275,7 +294,7 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
     const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
     const uint64_t mask = __ballot(id == a);
     left &= ~mask;
-    const int r = rank_of(rows, a);
+    const int own = rank_of(rows, a), r = whole(own);
     const F* f = factor + (int64_t)max(a, 0) * one;
     const float scale = slices > 1 && a >= 0 ? scale_of(rows, a) : 1.f;
     uint32_t live = 0;      // a lane's rows of lines, 8 k + lane / 8
@@ -355,6 +374,12 @@ __global__ __launch_bounds__(THREADS) void up_kernel(Rows rows, const float* u, 
               for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int k = 0; k < N; ++k) fr.p[k][q] = half[q / 2].p[k][q % 2];
+            }
+            if (j0 + j + (last ? 16 : 32) > own) {      // the adapter's last ranks
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int k = 0; k < N; ++k) fr.p[k][q] = counted(fr.p[k][q], own - j0 - of);
             }
             if constexpr (last && N > 1) {
 #pragma unroll
@@ -497,10 +522,11 @@ __global__ __launch_bounds__(THREADS) void down_row_kernel(Rows rows, const uint
   const int row = at.row, slice = at.part % slices, lane = threadIdx.x % 64;
   const int j = at.part / slices * 16 + threadIdx.x / 64 * 4;
   const int a = __builtin_amdgcn_readfirstlane(adapter_of(rows, row));
-  if (j >= rank_of(rows, a)) return;
+  const int r = rank_of(rows, a);
+  if (j >= whole(r)) return;
   const int begin = slice * slice_cols, end = min(C, begin + slice_cols);
   const v4f sum = four_ranks(x + (int64_t)row * C, factor + a * one + (int64_t)j * C, C, begin, end);
-  if (lane == 0) *reinterpret_cast<v4f*>(part + ((int64_t)slice * rows.T + row) * rows.R + j) = sum;
+  if (lane == 0) *reinterpret_cast<v4f*>(part + ((int64_t)slice * rows.T + row) * rows.R + j) = counted(sum, j, r);
 }
 
 // Up, from B: L lanes share a column's ranks, 16 bytes each, and a wave's 64 columns come in L steps; then every lane has one
@@ -531,14 +557,14 @@ __global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float*
     const float scale = scale_of(rows, a);
     if constexpr (kBoth) {
       const F* from = A + (int64_t)a * rows.R * K;
-      for (int j = threadIdx.x / 64 * 4; j < r; j += 16) {
-        const v4f v = four_ranks(x + (int64_t)row * K, from + (int64_t)j * K, K, 0, K) * scale;
+      for (int j = threadIdx.x / 64 * 4; j < whole(r); j += 16) {
+        const v4f v = counted(four_ranks(x + (int64_t)row * K, from + (int64_t)j * K, K, 0, K) * scale, j, r);
         if (lane) continue;
         *reinterpret_cast<v4f*>(u + j) = v;
         if (sum && of.part == 0) *reinterpret_cast<v4f*>(sum + (int64_t)row * rows.R + j) = v;
       }
     } else {
-      for (int j = threadIdx.x; j < r; j += THREADS) {
+      for (int j = threadIdx.x; j < whole(r); j += THREADS) {
         const float* p = part + (int64_t)row * rows.R + j;
         float v = *p;
 #pragma unroll 4
@@ -555,6 +581,15 @@ __global__ __launch_bounds__(THREADS) void up_row_kernel(Rows rows, const float*
   for (int j = 0; j < r; j += L * E) {
     if (j) fetch(j);
     if (j + sub < r) {
+      if (r % E) {      // of the adapter's last vector
+        const int n = r - j - sub;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t keep = kF32<F> ? k < n ? ~0u : 0u : (2 * k < n ? 0xffffu : 0u) | (2 * k + 1 < n ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int i = 0; i < L; ++i) w[i][k] &= keep;
+        }
+      }
       float uv[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) uv[e] = u[j + sub + e];
@@ -587,7 +622,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Rows rows, const float* p
   const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
   const int row = (int)(i / rows.R), j = (int)(i % rows.R);
   const int a = adapter_of(rows, row);
-  if (a < 0 || j >= rank_of(rows, a)) return;
+  if (a < 0 || j >= whole(rank_of(rows, a))) return;
   v4f v = *reinterpret_cast<const v4f*>(part + i);
 #pragma unroll 4
   for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const v4f*>(part + (int64_t)s * rows.T * rows.R + i);
@@ -738,7 +773,7 @@ __global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, 
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, m = lane % 16, g = lane / 16;
   const int c0 = ((int)blockIdx.x - (second ? jobs.j[0].blocks : 0)) * COLS, j0 = blockIdx.z * RR;
   const int r = rank_of(rows, it.a), C = job.C;
-  const bool some = j0 + Q * m < r, in = c0 + 8 * m < C;
+  const bool some = j0 + Q * m < whole(r), in = c0 + 8 * m < C;
   const int32_t* order = plan.order + plan.start[it.a];
   const uint16_t* x = job.x + c0 + (in ? 8 * m : 0);
   const float* p = job.p + j0 + (some ? Q * m : 0);
@@ -819,6 +854,8 @@ __global__ __launch_bounds__(THREADS, 2) void sums_kernel(Rows rows, Plan plan, 
       v4f v = *reinterpret_cast<const v4f*>(sums + o * ld + e);
 #pragma unroll
       for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const v4f*>(sums + w * PART + o * ld + e);
+      // zeros behind the adapter's ranks: products with what is not finite in x are none
+      v = job.swapped ? counted(v, j, r) : j < r ? v : v4f{0.f, 0.f, 0.f, 0.f};
       const int64_t at = job.swapped ? (int64_t)c * rows.R + j : (int64_t)j * C + c;
       if (it.slot >= 0) {
         *reinterpret_cast<v4f*>(job.part + it.slot * job.one + at) = v;

@@ -77,8 +77,8 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B:
     ``x`` (.., in) and ``y`` (.., out) bf16 with the same leading dimensions; ``lora_A`` (count, rank, in) and ``lora_B``
     (count, out, rank), float32 or bfloat16, the rank a multiple of 16; ``adapters`` int32 or int64, one number for each of
     ``x``'s first dimension, or first dimensions (a request's rows, or every row), on the device, where nothing waits for it.
-    ``s_a = scale * scales[a]`` (``scales`` float32, default 1).  ``ranks`` (int32): the ranks of each adapter that count; the
-    rest, zeros in a bank whose adapters differ, is not read and gets zero gradients.
+    ``s_a = scale * scales[a]`` (``scales`` float32, default 1).  ``ranks`` (int32): the ranks of each adapter that count; what
+    the storage holds behind them enters nothing, and gets zero gradients.
 
     Sums are float32 and ``out`` is rounded once.  Float32 factors (and the sums between the products) enter the matrix
     units as two bf16 parts, 2^-17 of a value off at most, or on the way to a float32 gradient as three, which hold it.  Rows

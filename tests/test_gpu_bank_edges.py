@@ -1,0 +1,53 @@
+"""GPU tests of a bank of adapters at its edges."""
+import pytest
+import torch
+
+from test_gpu_lora_bank import DTYPES, _check, _formula, _ids, _make
+
+pytestmark = pytest.mark.gpu
+
+
+# -- ranks ------------------------------------------------------------------------------------------------------------
+RANKS = [5, 0, 64, 33, 17, 16, 1, 50]
+
+
+@pytest.mark.parametrize("behind", [3.0, float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("lead, of, R, K, N", [
+    ((40,), (40,), 64, 128, 192),           # single rows in one launch
+    ((40,), (40,), 128, 1600, 192),         # and in two
+    ((500,), (500,), 64, 128, 320),         # tiles that meet several adapters
+    ((4, 300), (4,), 144, 1088, 2112),      # tiles of one, ranks past a workgroup's, slices
+    ((2, 20000), (2,), 64, 64, 128)])       # a "down" in one slice, pieces
+def test_ranks_are_counted_one_by_one(k2, dev, lead, of, R, K, N, dtype, behind):
+    """An adapter's rank counts as it is, whatever the storage holds behind it: the formula's values with zeros there, and
+    gradients of exactly zero."""
+    ids = _ids(of, len(RANKS), "mixed")
+    x, y, A, B, ids, scales, rk, dy = _make(dev, lead, ids, len(RANKS), R, K, N, DTYPES[dtype], RANKS)
+    want, size = _formula(x, y, A, B, ids, scales, dy)
+    for a, r in enumerate(RANKS):
+        A[a, r:], B[a, :, r:] = behind, behind
+    with torch.no_grad():
+        served = k2.add_adapters(y, x, A, B, ids, scales, rk)
+    leaves = [t.clone().requires_grad_() for t in (x, A, B)]
+    out = k2.add_adapters(y, *leaves, ids, scales, rk)
+    grads = torch.autograd.grad(out, leaves, dy)
+    rows = out.shape[:-1].numel()
+    assert torch.equal(out, served)
+    for got, w, s, terms in zip((out.detach(), *grads), want, size, (K + R, N + R, N + rows, K + rows)):
+        _check(got, w, s, terms, dtype)
+    for a, r in enumerate(RANKS):
+        assert not int(grads[1][a, r:].count_nonzero()) and not int(grads[2][a, :, r:].count_nonzero()), a
+
+
+@pytest.mark.parametrize("rows", [30, 300])
+def test_ranks_behind_an_adapters_own_keep_zero_gradients(k2, dev, rows):
+    """Also where a row of its own is not finite."""
+    ids = torch.arange(rows) % 2
+    x, y, A, B, ids, scales, rk, dy = _make(dev, (rows,), ids, 2, 64, 128, 64, torch.float32, [5, 20])
+    x[0, 3], dy[0, 5] = float("nan"), float("inf")
+    leaves = [t.clone().requires_grad_() for t in (A, B)]
+    dA, dB = torch.autograd.grad(k2.add_adapters(y, x, *leaves, ids, scales, rk), leaves, dy)
+    for a, r in enumerate((5, 20)):
+        assert not int(dA[a, r:].count_nonzero()) and not int(dB[a, :, r:].count_nonzero())
+    assert torch.isfinite(dA[1]).all() and torch.isfinite(dB[1]).all() and not torch.isfinite(dA[0]).all()
