@@ -8,7 +8,11 @@ train at once: each gets the gradients of its own rows.  :func:`add_adapters` is
 from __future__ import annotations
 
 import contextlib
+import contextvars
 import math
+import sys
+import threading
+import weakref
 
 import torch
 import torch.nn as nn
@@ -103,13 +107,76 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B:
     return _lib.bank_fwd(y, x, A, B, ids, scales, ranks, float(scale), False)[0]
 
 
+class _Body:
+    """A ``with`` body of :func:`lora_requests`: the requests of some banks, ahead of those of the bodies around it."""
+
+    def __init__(self, banks, ids, outer):
+        self.banks, self.ids, self.outer, self.open = weakref.WeakSet(banks), ids, outer, True
+
+    def of(self, bank) -> "_Body | None":
+        """The innermost body of ``bank``, from this one outwards."""
+        body = self
+        while body is not None and bank not in body.banks:
+            body = body.outer
+        return body
+
+
+# The body that the caller is in: a thread's, or an asyncio task's (what it starts with a copy of its context included)
+_body: contextvars.ContextVar = contextvars.ContextVar("lora_requests", default=None)
+# The body of a thread's last entry or forward pass, for passes that autograd recomputes: those run on threads of its own,
+# which have none here
+_last: dict = {}
+
+
+def _entered() -> _Body | None:
+    body = _body.get()
+    while body is not None and not body.open:       # a task that outlived the body it was started in
+        body = body.outer
+    return body
+
+
+def _backward_callers() -> list:
+    """The threads that are inside a backward pass: this one if it called one, and those that wait for theirs."""
+    me, name, out = threading.get_ident(), "_engine_run_backward", []
+    for ident, frame in sys._current_frames().items():
+        if ident == me:
+            while frame is not None and frame.f_code.co_name != name:
+                frame = frame.f_back
+        if frame is not None and frame.f_code.co_name == name:
+            out.append(ident)
+    return out
+
+
+def _requests(bank) -> torch.Tensor | None:
+    """The requests that ``bank`` runs with now where its call names none."""
+    body, me = _entered(), threading.get_ident()
+    if torch._C._current_graph_task_id() < 0:
+        last = _last.get(me)
+        if body is not None or last is None or last.of(bank) is not None:
+            _last[me] = body
+        found = None if body is None else body.of(bank)
+        return bank._own if found is None else found.ids
+    found = None if body is None else body.of(bank)
+    if found is None:
+        callers = [_last[t] for t in _backward_callers() if t in _last]
+        bodies = [None if b is None else b.of(bank) for b in callers or list(_last.values())]
+        found = bodies[0] if bodies else None
+        ids = [bank._own if b is None else b.ids for b in bodies]
+        if any(i is not ids[0] for i in ids):
+            raise RuntimeError("backward passes of several threads recompute a bank's forward at once: nothing tells whose "
+                               "requests it wants; open lora_requests in the recomputed function")
+    return bank._own if found is None else found.ids
+
+
 class LoRABank(nn.Module):
     """``base(x) + s_a (x A_a^T) B_a^T`` over a bank of ``count`` adapters of up to ``rank`` ranks: ``lora_A`` (count, rank, in),
     ``lora_B`` (count, out, rank), with the rank rounded up to a multiple of 16 (zero ranks, which training leaves zero).
     Initialised as ``LoRALinear`` (``lora.py:30-41``): ``A`` kaiming-uniform, ``B`` zeros, ``scale = alpha / rank``.
 
-    Which rows use which adapter comes with the call, or from :func:`lora_requests` around the model's; without either the
-    output is ``base(x)``.  ``scale_mul`` and ``lora_scaled`` act on all adapters."""
+    Which rows use which adapter comes with the call, or from :func:`lora_requests` around the model's, or from ``adapters``
+    (one setting for all threads); without any the output is ``base(x)``.  ``scale_mul`` and ``lora_scaled`` act on all adapters."""
+
+    _own = None     # the requests of all calls that are in no body
 
     def __init__(self, base: nn.Module, count: int, rank: int, alpha: float | None = None, dtype: torch.dtype = torch.float32):
         super().__init__()
@@ -125,7 +192,6 @@ class LoRABank(nn.Module):
         self.base = base
         base.requires_grad_(False)
         self.count, self.rank, self.scale_mul = count, rank, 1.0
-        self.adapters = None
         home = base.weight.device
         held = rank + -rank % _lib.RANK_ALIGN
         self.lora_A = nn.Parameter(torch.zeros(count, held, K, device=home, dtype=dtype))
@@ -137,6 +203,17 @@ class LoRABank(nn.Module):
         scale = torch.full((count,), (rank if alpha is None else alpha) / rank, dtype=torch.float32, device=home)
         self.register_buffer("scale_bits", scale.view(torch.int32))
         self.register_buffer("ranks", torch.full((count,), rank, dtype=torch.int32, device=home))
+
+    @property
+    def adapters(self) -> torch.Tensor | None:
+        """The requests of the caller's body of :func:`lora_requests`, else those set here."""
+        body = _entered()
+        found = None if body is None else body.of(self)
+        return self._own if found is None else found.ids
+
+    @adapters.setter
+    def adapters(self, ids: torch.Tensor | None) -> None:
+        self._own = ids
 
     @property
     def scales(self) -> torch.Tensor:
@@ -169,7 +246,7 @@ class LoRABank(nn.Module):
         return f"count={self.count}, rank={self.rank}"
 
     def forward(self, x: torch.Tensor, adapters: torch.Tensor | None = None) -> torch.Tensor:
-        ids, base = self.adapters if adapters is None else adapters, self.base
+        ids, base = _requests(self) if adapters is None else adapters, self.base
         if ids is None or self.scale_mul == 0.0:
             return base(x)
         A, B = self.lora_A, self.lora_B
@@ -188,16 +265,22 @@ _lora._SCALED += (LoRABank,)
 def lora_requests(model: nn.Module, adapters: torch.Tensor | None):
     """Within the ``with`` body the rows of every bank's input in ``model`` use the adapters of ``adapters``: one number for
     each entry of the input's first dimension (the requests of a batch), or of its first dimensions; None: the base alone.
-    A checkpointed forward runs again in its backward pass: keep that inside the body too."""
-    banks = [m for m in model.modules() if isinstance(m, LoRABank)]
-    saved = [m.adapters for m in banks]
-    for m in banks:
-        m.adapters = adapters
+
+    A body is its thread's, or its asyncio task's, alone (``asyncio.to_thread`` and tasks take it with them while it is open;
+    a plain thread opens its own), so threads may run requests of their own through one model.  A checkpointed forward runs
+    again in its backward pass, with the requests of the thread that called that: keep it inside the body too."""
+    body = _Body([m for m in model.modules() if isinstance(m, LoRABank)], adapters, _entered())
+    token, me, outside = _body.set(body), threading.get_ident(), torch._C._current_graph_task_id() < 0
+    if outside:
+        _last[me] = body
     try:
         yield
     finally:
-        for m, v in zip(banks, saved):
-            m.adapters = v
+        body.open = False
+        with contextlib.suppress(ValueError):       # left in another context than entered: its holders see that it is closed
+            _body.reset(token)
+        if outside:
+            _last[me] = _entered()
 
 
 def inject_lora_bank(dit, count: int, rank: int, alpha: float | None = None, *, targets=DEFAULT_TARGETS,

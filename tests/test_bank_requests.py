@@ -1,0 +1,180 @@
+"""CPU tests of what a bank of adapters is asked for, and of its files."""
+import asyncio
+import threading
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from test_adapter_checks import _Dit
+
+
+@pytest.fixture
+def seen(k2, monkeypatch):
+    """A model of banks, and the requests that each of their calls used, in place of the kernel (there is none on the CPU)."""
+    import krea2_amd.lora_bank as lb
+    calls = []
+
+    def add(y, x, A, B, ids, scales, ranks, scale):
+        calls.append(ids)
+        return y + (x @ A[0].t()) @ B[0].t()
+
+    monkeypatch.setattr(lb, "add_adapters", add)
+    dit = _Dit()
+    banks = k2.inject_lora_bank(dit, 2, 16)
+    return dit, banks, calls
+
+
+def _ids(*v):
+    return torch.tensor(v)
+
+
+def test_threads_keep_their_requests(k2, seen):
+    """Two threads whose bodies overlap, the first one out first: each sees its own, and nothing stays behind."""
+    dit, banks, calls = seen
+    bank = banks["blocks.0.mlp.up"]
+    mine, its = _ids(0), _ids(1)
+    turns = [threading.Event() for _ in range(4)]
+    out, x = {}, torch.zeros(1, 64)
+
+    def other():
+        assert turns[0].wait(20)
+        out["before"] = bank.adapters
+        with k2.lora_requests(dit, its):
+            turns[1].set()
+            assert turns[2].wait(20)            # the first body has ended
+            out["inside"] = bank.adapters
+            bank(x)
+            out["used"] = calls[-1]
+        out["behind"] = bank.adapters
+        turns[3].set()
+
+    t = threading.Thread(target=other)
+    t.start()
+    with k2.lora_requests(dit, mine):
+        turns[0].set()
+        assert turns[1].wait(20)
+        assert bank.adapters is mine
+        bank(x)
+        assert calls[-1] is mine
+    turns[2].set()
+    assert turns[3].wait(20)
+    t.join()
+    assert out["before"] is None and out["inside"] is its and out["used"] is its and out["behind"] is None
+    assert all(b.adapters is None for b in banks.values())
+    n = len(calls)
+    bank(x)
+    assert len(calls) == n                      # the base alone
+
+
+def test_tasks_keep_their_requests(k2, seen):
+    """Two tasks of one thread that wait inside their bodies, and a function that one sends to another thread."""
+    dit, banks, calls = seen
+    bank = banks["blocks.0.mlp.up"]
+    found = []
+
+    async def one(ids, n):
+        with k2.lora_requests(dit, ids):
+            for _ in range(n):
+                await asyncio.sleep(0.01)
+                found.append(bank.adapters is ids)
+            found.append(await asyncio.to_thread(lambda: bank.adapters is ids))
+        found.append(bank.adapters is None)
+
+    async def both():
+        await asyncio.gather(one(_ids(0), 2), one(_ids(1), 4))
+
+    asyncio.run(both())
+    assert found and all(found) and bank.adapters is None
+
+
+def test_bodies_nest(k2, seen):
+    dit, banks, calls = seen
+    bank, a, b = banks["blocks.1.attn.wo"], _ids(0), _ids(1)
+    with k2.lora_requests(dit, a):
+        with k2.lora_requests(dit.blocks[0], b):        # other banks
+            assert bank.adapters is a and banks["blocks.0.attn.wo"].adapters is b
+        with pytest.raises(KeyError):
+            with k2.lora_requests(dit, None):
+                assert bank.adapters is None
+                raise KeyError
+        assert bank.adapters is a
+    assert bank.adapters is None
+    bank.adapters = b                                   # requests of the bank's own, where no body is open
+    assert bank.adapters is b
+    with k2.lora_requests(dit, a):
+        assert bank.adapters is a
+    assert bank.adapters is b
+    bank.adapters = None
+
+
+def _train(dit, x, reentrant):
+    def run(t):
+        for b in dit.blocks:
+            t = b.mlp.up(t)
+        return t
+
+    return checkpoint(run, x, use_reentrant=reentrant)
+
+
+def test_passes_of_two_threads_are_recomputed_with_their_own(k2, seen):
+    """Also where one has no requests and the other's body is open meanwhile."""
+    dit, banks, calls = seen
+    ids, used, errors = _ids(0), {}, []
+    gate = threading.Barrier(2, timeout=20)
+
+    def work(name, wanted):
+        try:
+            x = torch.randn(1, 64, requires_grad=True)
+            if wanted is None:
+                gate.wait()
+                y = _train(dit, x, False)
+                n = len(calls)
+                y.sum().backward()
+                used[name] = len(calls) - n
+                gate.wait()
+            else:
+                with k2.lora_requests(dit, wanted):
+                    y = _train(dit, x, False)
+                    gate.wait()
+                    gate.wait()
+                    n = len(calls)
+                    y.sum().backward()
+                    used[name] = calls[n:]
+        except Exception as e:          # noqa: BLE001 - shown below
+            errors.append(e)
+            gate.abort()
+
+    threads = [threading.Thread(target=work, args=a) for a in (("with", ids), ("without", None))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and used["without"] == 0 and [u is ids for u in used["with"]] == [True, True]
+
+
+@pytest.mark.parametrize("other", ["same", "another", "none", "own"])
+def test_a_recomputed_pass_that_two_threads_may_want_is_refused(k2, seen, monkeypatch, other):
+    """A thread of autograd's own, while two threads wait for their backward passes: it runs where both have the same requests
+    or it opened a body, and with one of them alone as that one."""
+    import krea2_amd.lora_bank as lb
+    dit, banks, calls = seen
+    bank, x, ids = banks["blocks.0.mlp.up"], torch.zeros(1, 64), _ids(0)
+    bodies = [lb._Body(banks.values(), i, None) for i in (ids, _ids(0) if other == "another" else ids)]
+    monkeypatch.setattr(lb, "_last", {-5: bodies[0], -6: None if other == "none" else bodies[1]})
+    monkeypatch.setattr(lb, "_backward_callers", lambda: [-7, -5, -6])
+    monkeypatch.setattr(torch._C, "_current_graph_task_id", lambda: 1)
+    if other == "same":
+        bank(x)
+        assert calls[-1] is ids
+    elif other == "own":
+        mine = _ids(1)
+        with k2.lora_requests(dit, mine):
+            bank(x)
+        assert calls[-1] is mine and set(lb._last) == {-5, -6}
+    else:
+        with pytest.raises(RuntimeError, match="several threads"):
+            bank(x)
+    monkeypatch.setattr(lb, "_backward_callers", lambda: [-5])
+    bank(x)
+    assert calls[-1] is ids

@@ -1,8 +1,12 @@
 """GPU tests of a bank of adapters at its edges."""
+import contextlib
+import threading
+
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
-from test_gpu_lora_bank import DTYPES, _check, _formula, _ids, _make
+from test_gpu_lora_bank import DTYPES, _check, _formula, _ids, _linear, _make
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +55,56 @@ def test_ranks_behind_an_adapters_own_keep_zero_gradients(k2, dev, rows):
     for a, r in enumerate((5, 20)):
         assert not int(dA[a, r:].count_nonzero()) and not int(dB[a, :, r:].count_nonzero())
     assert torch.isfinite(dA[1]).all() and torch.isfinite(dB[1]).all() and not torch.isfinite(dA[0]).all()
+
+
+# -- requests of threads ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_recomputed_passes_use_the_requests_of_the_thread_that_called_them(k2, dev, reentrant):
+    """Two threads with requests of their own and one without, their bodies open all at once, one backward pass after another:
+    each gets the gradients that it gets alone."""
+    bank = k2.LoRABank(_linear(k2, dev, 256, 256, "w8a8"), 2, 16)
+    with torch.no_grad():
+        bank.lora_B.normal_(0.0, 0.1)
+    x = torch.randn(2, 8, 256, device=dev).bfloat16()
+    wanted = [torch.tensor([0, 1], device=dev), None, torch.tensor([1, -1], device=dev)]
+
+    def forward(leaf):
+        return checkpoint(lambda t: bank(bank(t)), leaf, use_reentrant=reentrant)
+
+    def grads(y, leaf):
+        bank.zero_grad()
+        y.float().square().sum().backward()
+        out = [t.grad for t in (leaf, bank.lora_A, bank.lora_B)]
+        return [None if t is None else t.clone() for t in out]
+
+    alone = []
+    for ids in wanted:
+        leaf = x.clone().requires_grad_()
+        with k2.lora_requests(bank, ids) if ids is not None else contextlib.nullcontext():
+            alone.append(grads(forward(leaf), leaf))
+    got, errors, gate = [None] * 3, [], threading.Barrier(3, timeout=60)
+
+    def work(i):
+        try:
+            leaf = x.clone().requires_grad_()
+            with k2.lora_requests(bank, wanted[i]) if wanted[i] is not None else contextlib.nullcontext():
+                y = forward(leaf)
+                for turn in (2, 0, 1):
+                    gate.wait()
+                    if turn == i:
+                        got[i] = grads(y, leaf)
+                    gate.wait()
+        except Exception as e:          # noqa: BLE001 - shown below
+            errors.append(e)
+            gate.abort()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for a, b in zip(got, alone):
+        assert all((p is None) == (q is None) and (p is None or torch.equal(p, q)) for p, q in zip(a, b))
+    assert alone[1][1] is None and not torch.equal(alone[0][0], alone[2][0])
