@@ -112,6 +112,10 @@ class _Body:
 
     def __init__(self, banks, ids, outer):
         self.banks, self.ids, self.outer, self.open = weakref.WeakSet(banks), ids, outer, True
+        self.named = ids is not None
+
+    def close(self) -> None:
+        self.open, self.ids = False, None
 
     def of(self, bank) -> "_Body | None":
         """The innermost body of ``bank``, from this one outwards."""
@@ -157,15 +161,19 @@ def _requests(bank) -> torch.Tensor | None:
         found = None if body is None else body.of(bank)
         return bank._own if found is None else found.ids
     found = None if body is None else body.of(bank)
-    if found is None:
+    if found is None:       # on a thread of autograd's own, or with no body left
         callers = [_last[t] for t in _backward_callers() if t in _last]
-        bodies = [None if b is None else b.of(bank) for b in callers or list(_last.values())]
+        callers = callers or [b for b in list(_last.values()) if b is None or b.open]
+        bodies = [None if b is None else b.of(bank) for b in callers]
         found = bodies[0] if bodies else None
+        if any(b is not None and not b.open and b.named for b in bodies):
+            raise RuntimeError("a bank's forward is recomputed outside the lora_requests body that it ran in, where it would run "
+                               "without its adapters: keep the backward pass inside the body")
         ids = [bank._own if b is None else b.ids for b in bodies]
         if any(i is not ids[0] for i in ids):
             raise RuntimeError("backward passes of several threads recompute a bank's forward at once: nothing tells whose "
                                "requests it wants; open lora_requests in the recomputed function")
-    return bank._own if found is None else found.ids
+    return bank._own if found is None or not found.open else found.ids
 
 
 class LoRABank(nn.Module):
@@ -268,7 +276,8 @@ def lora_requests(model: nn.Module, adapters: torch.Tensor | None):
 
     A body is its thread's, or its asyncio task's, alone (``asyncio.to_thread`` and tasks take it with them while it is open;
     a plain thread opens its own), so threads may run requests of their own through one model.  A checkpointed forward runs
-    again in its backward pass, with the requests of the thread that called that: keep it inside the body too."""
+    again in its backward pass, with the requests of the thread that called that: keep it inside the body too (a bank whose last
+    body the thread has left is refused there)."""
     body = _Body([m for m in model.modules() if isinstance(m, LoRABank)], adapters, _entered())
     token, me, outside = _body.set(body), threading.get_ident(), torch._C._current_graph_task_id() < 0
     if outside:
@@ -276,11 +285,11 @@ def lora_requests(model: nn.Module, adapters: torch.Tensor | None):
     try:
         yield
     finally:
-        body.open = False
+        body.close()
         with contextlib.suppress(ValueError):       # left in another context than entered: its holders see that it is closed
             _body.reset(token)
         if outside:
-            _last[me] = _entered()
+            _last[me] = _entered() or body      # closed: a backward pass that comes yet finds that it came too late
 
 
 def inject_lora_bank(dit, count: int, rank: int, alpha: float | None = None, *, targets=DEFAULT_TARGETS,

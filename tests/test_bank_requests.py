@@ -178,3 +178,33 @@ def test_a_recomputed_pass_that_two_threads_may_want_is_refused(k2, seen, monkey
     monkeypatch.setattr(lb, "_backward_callers", lambda: [-5])
     bank(x)
     assert calls[-1] is ids
+
+
+# -- recomputed passes ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_a_pass_recomputed_outside_its_body_is_refused(k2, seen, reentrant):
+    """It would run without the adapters.  Inside the body, in one of its own, and without requests it runs."""
+    dit, banks, calls = seen
+    ids = _ids(0)
+    x = torch.randn(1, 64, requires_grad=True)
+    with k2.lora_requests(dit, ids):
+        y = _train(dit, x, reentrant)
+        y.sum().backward()
+    assert len(calls) == 4 and all(c is ids for c in calls)
+    with k2.lora_requests(dit, ids):
+        y = _train(dit, x, reentrant)
+    with pytest.raises(RuntimeError, match="lora_requests"):
+        y.sum().backward()
+    with k2.lora_requests(dit, ids):
+        y = _train(dit, x, reentrant)
+    with k2.lora_requests(dit, ids):
+        y.sum().backward()
+    for body in (False, True):                          # a forward pass without requests, and with those of no adapter
+        del calls[:]
+        if body:
+            with k2.lora_requests(dit, None):
+                y = _train(dit, x, reentrant)
+        else:
+            y = _train(dit, x, reentrant)
+        y.sum().backward()
+        assert not calls

@@ -108,3 +108,22 @@ def test_recomputed_passes_use_the_requests_of_the_thread_that_called_them(k2, d
     for a, b in zip(got, alone):
         assert all((p is None) == (q is None) and (p is None or torch.equal(p, q)) for p, q in zip(a, b))
     assert alone[1][1] is None and not torch.equal(alone[0][0], alone[2][0])
+
+
+# -- recomputed passes ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_a_pass_recomputed_outside_its_body_is_refused(k2, dev, reentrant):
+    """On autograd's own thread: it would run without the adapters, whose factors would get no gradients."""
+    bank = k2.LoRABank(_linear(k2, dev, 256, 256, "w8a8"), 2, 16)
+    x = torch.randn(2, 8, 256, device=dev).bfloat16().requires_grad_()
+    ids = torch.tensor([0, 1], device=dev)
+    with k2.lora_requests(bank, ids):
+        y = checkpoint(lambda t: bank(bank(t)), x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="outside the lora_requests body"):
+        y.float().sum().backward()
+    with k2.lora_requests(bank, ids):
+        checkpoint(lambda t: bank(bank(t)), x, use_reentrant=reentrant).float().sum().backward()
+    assert bank.lora_B.grad is not None
+    bank.zero_grad()
+    checkpoint(lambda t: bank(bank(t)), x, use_reentrant=reentrant).float().sum().backward()      # the base alone
+    assert bank.lora_B.grad is None
