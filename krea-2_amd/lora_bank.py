@@ -44,6 +44,21 @@ class _AddAdaptersFn(torch.autograd.Function):
         return (dy if need[0] else None, *grads, None, None, None, None)
 
 
+class _NoRowsFn(torch.autograd.Function):
+    """A batch without rows: products of no rows, whose gradients are zeros."""
+
+    @staticmethod
+    def forward(ctx, y, x, A, B):
+        ctx.save_for_backward(x, A, B)
+        return y.clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        return (dy if need[0] else None, *(torch.zeros_like(t) if n else None for t, n in zip(ctx.saved_tensors, need[1:])))
+
+
 class _BankLinearFn(torch.autograd.Function):
     """``add_adapters`` over the output of a frozen quantized base, as one node: the base's input gradient is what the adapters'
     is added to, in place (autograd would make both tensors, and a third)."""
@@ -98,7 +113,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B:
     if scales is not None and scales.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("scales get no gradient: detach them")
     if x.numel() == 0 and x.shape[-1] == lora_A.shape[-1] and y.shape[-1] == lora_B.shape[1]:
-        return y.clone()
+        return _NoRowsFn.apply(y, x, lora_A, lora_B) if grad else y.clone()
     if x.dtype == y.dtype == torch.bfloat16:
         x, y = _rows(x), _rows(y)
     A, B, ids = lora_A.contiguous(), lora_B.contiguous(), adapters.contiguous()

@@ -208,3 +208,19 @@ def test_a_pass_recomputed_outside_its_body_is_refused(k2, seen, reentrant):
             y = _train(dit, x, reentrant)
         y.sum().backward()
         assert not calls
+
+
+# -- batches without rows ---------------------------------------------------------------------------------------------
+def test_a_batch_without_rows_has_a_pass_back(k2):
+    """Zeros for both factors, as products of no rows give."""
+    x = torch.zeros(0, 3, 64, dtype=torch.bfloat16, requires_grad=True)
+    y = torch.zeros(0, 3, 128, dtype=torch.bfloat16, requires_grad=True)
+    A, B, ids = torch.ones(4, 16, 64, requires_grad=True), torch.ones(4, 128, 16, requires_grad=True), torch.zeros(0, dtype=torch.int64)
+    for leaves in ((y, x, A, B), (A,), (B,), (x,)):
+        args = [t if any(t is v for v in leaves) else t.detach() for t in (y, x, A, B)]
+        out = k2.add_adapters(*args, ids)
+        assert out.shape == y.shape and out.requires_grad
+        for g, t in zip(torch.autograd.grad(out, leaves, torch.zeros_like(out)), leaves):
+            assert g.shape == t.shape and g.dtype == t.dtype and not int(g.count_nonzero())
+    with torch.no_grad():
+        assert not k2.add_adapters(y, x, A, B, ids).requires_grad

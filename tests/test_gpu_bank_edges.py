@@ -57,6 +57,20 @@ def test_ranks_behind_an_adapters_own_keep_zero_gradients(k2, dev, rows):
     assert torch.isfinite(dA[1]).all() and torch.isfinite(dB[1]).all() and not torch.isfinite(dA[0]).all()
 
 
+# -- batches without rows ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["w8a8", "linear"])
+def test_a_batch_without_rows_trains_nothing(k2, dev, kind):
+    """Its pass back gives zeros, as products of no rows do."""
+    bank = k2.LoRABank(_linear(k2, dev, 256, 256, kind), 2, 16)
+    x = torch.zeros(0, 5, 256, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    out = bank(x, torch.zeros(0, dtype=torch.int64, device=dev))
+    assert out.shape == (0, 5, 256)
+    out.float().sum().backward()
+    assert x.grad.shape == x.shape
+    for p in (bank.lora_A, bank.lora_B):
+        assert p.grad.shape == p.shape and p.grad.dtype == p.dtype and not int(p.grad.count_nonzero())
+
+
 # -- requests of threads ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("reentrant", [True, False])
 def test_recomputed_passes_use_the_requests_of_the_thread_that_called_them(k2, dev, reentrant):
