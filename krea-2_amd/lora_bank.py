@@ -66,14 +66,16 @@ class _BankLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, A, B, ids, scales, ranks, scale, base):
         out, u = _lib.bank_fwd(_rows(base(x)), x, A, B, ids, scales, ranks, scale, ctx.needs_input_grad[2])
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, u, A, B, ids, scales, ranks)
+        # the base's too: autograd refuses one that changed in place
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, u, A, B, ids, scales, ranks,
+                              *base.input_grad_reads())
         ctx.scale, ctx.base = scale, base
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, u, A, B, ids, scales, ranks = ctx.saved_tensors
+        x, u, A, B, ids, scales, ranks = ctx.saved_tensors[:7]
         need = ctx.needs_input_grad[:3]
         d, dx = _rows(dy), None
         if need[0]:

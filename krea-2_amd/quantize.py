@@ -309,6 +309,10 @@ class ConvRotLinear(nn.Module):
         """The gradient of the layer's input, (rows, in) bf16, from that of its output (contiguous (rows, out) bf16)."""
         return _lib.gemm_dx(dy, self.qweight, self.weight_scale, w4=self.mode == "w4a8", wt=self.dx_weight())
 
+    def input_grad_reads(self) -> tuple:
+        """The parameters that :meth:`input_grad` reads."""
+        return self.qweight, self.wscale
+
 
 def quantize_dit_convrot(dit, mode: str = "w8a8") -> int:
     """Replace the transformer blocks' ``nn.Linear`` with :class:`ConvRotLinear` in place.
@@ -486,6 +490,10 @@ class Fp8Linear(nn.Module):
     def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
         """The gradient of the layer's input, (rows, in) bf16, from that of its output (contiguous (rows, out) bf16)."""
         return _lib.gemm_dx_fp8(dy, self.weight_fp8, self.scale.to(torch.bfloat16).contiguous())
+
+    def input_grad_reads(self) -> tuple:
+        """The parameters that :meth:`input_grad` reads."""
+        return self.weight_fp8, self.scale
 
 
 def quantize_dit_fp8(dit) -> int:

@@ -71,6 +71,23 @@ def test_a_batch_without_rows_trains_nothing(k2, dev, kind):
         assert p.grad.shape == p.shape and p.grad.dtype == p.dtype and not int(p.grad.count_nonzero())
 
 
+# -- a base that changes ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["w8a8", "w4a8", "fp8"])
+def test_a_base_changed_in_place_between_the_passes_is_refused(k2, dev, kind):
+    """As autograd refuses it where LoRALinear's node saves the weights."""
+    base = _linear(k2, dev, 256, 256, kind)
+    bank = k2.LoRABank(base, 1, 16)
+    x = torch.randn(4, 256, device=dev).bfloat16().requires_grad_()
+    ids = torch.zeros(4, dtype=torch.int64, device=dev)
+    out = bank(x, ids)
+    with torch.no_grad():
+        weight = base.weight_fp8 if kind == "fp8" else base.qweight
+        weight.view(torch.uint8).add_(1) if kind == "fp8" else weight.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
+    bank(x, ids).float().sum().backward()
+
+
 # -- requests of threads ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("reentrant", [True, False])
 def test_recomputed_passes_use_the_requests_of_the_thread_that_called_them(k2, dev, reentrant):
