@@ -8,6 +8,7 @@ multiple of 256 elements; ``state[p]`` holds views of them.
 from __future__ import annotations
 
 import importlib
+import inspect
 import math
 from types import SimpleNamespace
 
@@ -154,28 +155,37 @@ class AdamW(torch.optim.Optimizer):
                 self._moments_of(g)
 
     # -- the step ------------------------------------------------------------------------------------------------
-    def step(self, closure=None):
-        """One step of every parameter that has a gradient; ``closure``, if given, is called first and its value returned."""
-        hooks = _hooks(self)
-        args, kwargs = (closure,) if closure is not None else (), {}
-        for hook in hooks[0]:
+    def step(self, *args, **kwargs):
+        """``step(closure=None)``: one step of every parameter that has a gradient; ``closure``, if given, is called first and
+        its value returned."""
+        if torch.autograd._profiler_enabled():
+            with torch.autograd.profiler.record_function("Optimizer.step#AdamW.step"):
+                return self._hooked((self, *args), kwargs)
+        return self._hooked((self, *args), kwargs)
+
+    def _hooked(self, args: tuple, kwargs: dict):
+        """A step between its hooks, which get what torch gives them: the arguments with the optimizer ahead; those in front may
+        return others."""
+        for hook in [*_EVERY[0].values(), *self._optimizer_step_pre_hooks.values()]:
             given = hook(self, args, kwargs)
             if given is not None:
+                if not (isinstance(given, tuple) and len(given) == 2):
+                    raise RuntimeError(f"a hook ahead of a step must return None or a tuple (args, kwargs), got {given!r}")
                 args, kwargs = given
-        closure = args[0] if args else kwargs.get("closure")
+        loss = AdamW._closure_and_step(*args, **kwargs)
+        for hook in [*self._optimizer_step_post_hooks.values(), *_EVERY[1].values()]:
+            hook(self, args, kwargs)
+        return loss
+
+    def _closure_and_step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if torch.autograd._profiler_enabled():
-            with torch.autograd.profiler.record_function("Optimizer.step#AdamW.step"):
-                self._step()
-        else:
-            self._step()
-        for hook in hooks[1]:
-            hook(self, args, kwargs)
+        self._step()
         return loss
 
+    step.__signature__ = inspect.signature(_closure_and_step)
     step.hooked = True      # hooks and the profiler's label are above: torch's own wrapper takes 12 of a small step's 28 us
 
     def _step(self) -> None:
@@ -197,12 +207,6 @@ class AdamW(torch.optim.Optimizer):
                              g["seed"])
             norm = out if len(groups) == 1 else norm
         self.grad_norm = None if norm is None else norm[0]
-
-
-def _hooks(opt: torch.optim.Optimizer):
-    """What is registered to run ahead of a step and behind it: for every optimizer, and for this one."""
-    return ([*_EVERY[0].values(), *opt._optimizer_step_pre_hooks.values()],
-            [*opt._optimizer_step_post_hooks.values(), *_EVERY[1].values()])
 
 
 def _kinds(bits: int) -> dict:
