@@ -1460,6 +1460,17 @@ def grad_norm(params: list, max_norm: float, scale: bool):
     return r[0] if r else None
 
 
+def same_items(a: list, b: list) -> bool:
+    """Whether two lists hold the same objects."""
+    return _fast().same_items(a, b)
+
+
+def unchanged(state: dict, keys: list, dicts: list, values: list) -> bool:
+    """Whether a dict of dicts has these keys and values, and those these values, as objects (448 parameters of 3 values: 10
+    us)."""
+    return _fast().unchanged(state, keys, dicts, values)
+
+
 def _check_adamw(params, starts, exp_avg, steps, stochastic) -> None:
     if len(params) != len(starts) or steps.numel() != len(starts):
         raise ValueError(f"the group has {len(params)} parameters now, and had {len(starts)} when its moments were laid out")

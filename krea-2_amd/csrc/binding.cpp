@@ -763,6 +763,32 @@ bool each_of(PyObject* list, F&& f) {
 
 void changed(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
+// same_items(list, list) -> whether they hold the same objects
+PyObject* py_same_items(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(2)
+  if (!PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1])) Py_RETURN_FALSE;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i)
+    if (PyList_GET_ITEM(a[0], i) != PyList_GET_ITEM(a[1], i)) Py_RETURN_FALSE;
+  Py_RETURN_TRUE;
+}
+
+// unchanged(dict of dicts, its keys, its values, their values) -> whether these are the objects that it holds, in this order
+PyObject* py_unchanged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  K2Q_ARGS(4)
+  if (!PyDict_Check(a[0]) || !PyList_Check(a[1]) || !PyList_Check(a[2]) || !PyList_Check(a[3])) Py_RETURN_FALSE;
+  const Py_ssize_t count = PyList_GET_SIZE(a[1]), values = PyList_GET_SIZE(a[3]);
+  if (PyDict_Size(a[0]) != count || PyList_GET_SIZE(a[2]) != count) Py_RETURN_FALSE;
+  PyObject *key, *d, *v;
+  Py_ssize_t i = 0, k = 0;
+  for (Py_ssize_t at = 0; PyDict_Next(a[0], &at, &key, &d); ++i) {
+    if (i >= count || key != PyList_GET_ITEM(a[1], i) || d != PyList_GET_ITEM(a[2], i) || !PyDict_Check(d)) Py_RETURN_FALSE;
+    for (Py_ssize_t in = 0; PyDict_Next(d, &in, nullptr, &v); ++k)
+      if (k >= values || v != PyList_GET_ITEM(a[3], k)) Py_RETURN_FALSE;
+  }
+  if (k != values) Py_RETURN_FALSE;
+  Py_RETURN_TRUE;
+}
+
 // grad_norm(params, max_norm, scale) -> (out,): {norm, factor} of the parameters' gradients, which are multiplied by the
 // factor; with scale false the partial sums of squares that adamw takes; () where none has a gradient
 PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -1055,6 +1081,7 @@ PyMethodDef methods[] = {K2Q_METHOD(bind),        K2Q_METHOD(device_checked), K2
                          K2Q_METHOD(resnorm_bwd), K2Q_METHOD(rotary),         K2Q_METHOD(linear_infer),
                          K2Q_METHOD(capture_id),  K2Q_METHOD(resnorm_stream_bwd),
                          K2Q_METHOD(grad_norm),   K2Q_METHOD(adamw),          K2Q_METHOD(moments),
+                         K2Q_METHOD(same_items),  K2Q_METHOD(unchanged),
                          K2Q_METHOD(bank_fwd),    K2Q_METHOD(bank_bwd),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_k2q_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

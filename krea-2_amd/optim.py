@@ -3,7 +3,8 @@ the two lines that the reference's trainer takes from torch (``train_t2i_lora_ca
 
 :class:`AdamW` keeps its moments in 32 bits, or in 8 bits with a scale for every 256 elements: 2 bytes for an element in
 place of 8, and 16 bytes moved by a step in place of 28.  A group's moments lie in flat buffers, each parameter's at a
-multiple of 256 elements; ``state[p]`` holds views of them.
+multiple of 256 elements; ``state[p]`` holds views of them.  What is put in their place, or taken out, counts: the next step
+lays the group's moments out anew from what ``state`` says, zeros where it says nothing.
 """
 from __future__ import annotations
 
@@ -63,6 +64,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm = None if max_norm is None else float(max_norm)
         self.grad_norm = None
         self._held = {}         # id of a group's list of parameters -> its moments' buffers (which hold the list)
+        self._seen = None       # the state's keys, its values and theirs, as they were last found to be those buffers'
         super().__init__(params, defaults)
 
     def add_param_group(self, param_group: dict) -> None:
@@ -76,7 +78,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state) -> None:
         self.__dict__.setdefault("max_norm", None)
-        self.grad_norm, self._held = None, {}       # laid out again from the states at the next step
+        self.grad_norm, self._held, self._seen = None, {}, None       # laid out again from the states at the next step
         super().__setstate__(state)
         for group in self.param_groups:
             for name, value in self.defaults.items():
@@ -88,7 +90,9 @@ class AdamW(torch.optim.Optimizer):
         """A group's buffers, made when they are not there: zeros, or the states that its parameters have."""
         params = group["params"]
         held = self._held.get(id(params))
-        if held is not None:
+        # a list that grew or shrank is refused by the step; one with others in it, or in other bits, is laid out anew
+        if held is not None and (len(params) != len(held.of) or
+                                 held.bits == group["state_bits"] and _lib.same_items(params, held.of)):
             return held
         devices = {p.device for p in params}
         if len(devices) != 1 or next(iter(devices)).type != "cuda":
@@ -100,11 +104,12 @@ class AdamW(torch.optim.Optimizer):
         for k, p in enumerate(params):
             if p.dtype not in _lib.STEP_DTYPES:
                 raise ValueError(f"parameter {k} is {p.dtype}, not one of {_lib.STEP_DTYPES}")
+            _check_state(self.state.get(p) or None, p, group["state_bits"])
         starts, total = [], 0
         for p in params:
             starts.append(total)
             total += -(-p.numel() // _BLOCK) * _BLOCK
-        held = SimpleNamespace(params=params, bits=group["state_bits"], starts=starts,
+        held = SimpleNamespace(params=params, of=list(params), bits=group["state_bits"], starts=starts, states=[],
                                steps=torch.zeros(len(params), device=dev))
         kinds = _kinds(held.bits)
         for name, (dtype, per) in kinds.items():
@@ -121,8 +126,24 @@ class AdamW(torch.optim.Optimizer):
                     for name, view in new.items():
                         _copy(view, old[name])
                 self.state[p] = new
+                held.states.append((new, list(new.values())))
         self._held[id(params)] = held
+        self._note_state()
         return held
+
+    def _note_state(self) -> None:
+        dicts = list(self.state.values())
+        self._seen = (list(self.state), dicts, [v for d in dicts for v in d.values()])
+
+    def _follow_state(self) -> None:
+        """Drop the buffers of groups whose states are not theirs any more: the next use makes them from the states."""
+        if self._seen is not None and _lib.unchanged(self.state, *self._seen):
+            return
+        for key, held in list(self._held.items()):
+            if not all(self.state.get(p) is d and _lib.same_items(list(d.values()), views)
+                       for p, (d, views) in zip(held.of, held.states)):
+                del self._held[key]
+        self._note_state()
 
     def moments(self, group: int = 0, dtype: torch.dtype = torch.float32):
         """``(exp_avg, exp_avg_sq)`` of a group's parameters as numbers, flat, each parameter's from a multiple of 256
@@ -130,6 +151,7 @@ class AdamW(torch.optim.Optimizer):
         bfloat16)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
+        self._follow_state()
         held = self._moments_of(self.param_groups[group])
         if held.bits == 32 or not held.exp_avg.numel():
             return held.exp_avg.to(dtype), held.exp_avg_sq.to(dtype)
@@ -190,6 +212,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _step(self) -> None:
         groups, squares, norm = self.param_groups, None, None
+        self._follow_state()
         if self.max_norm is not None and len(groups) > 1:       # of one group, the step's own call takes it
             squares = _lib.grad_norm([p for g in groups for p in g["params"]], self.max_norm, False)
             if squares is not None:
@@ -197,7 +220,7 @@ class AdamW(torch.optim.Optimizer):
         for g in groups:
             if not g["params"]:
                 continue
-            held = self._held.get(id(g["params"])) or self._moments_of(g)
+            held = self._moments_of(g)
             lr, lr_of = g["lr"], None
             if isinstance(lr, torch.Tensor):
                 lr, lr_of = (0.0, lr) if lr.is_cuda else (float(lr), None)
@@ -254,5 +277,7 @@ def _check_state(state: dict | None, p: torch.Tensor, bits: int) -> None:
         raise ValueError(f"a state in {bits} bits holds {sorted(('step', *kinds))}, got {sorted(state)}")
     for name, (dtype, per) in kinds.items():
         shape = tuple(p.shape) if per == 1 else (-(-p.numel() // per),)
-        if state[name].dtype != dtype or tuple(state[name].shape) != shape:
-            raise ValueError(f"{name} must be {dtype} {shape}, got {state[name].dtype} {tuple(state[name].shape)}")
+        t = state[name]
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != shape:
+            got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
+            raise ValueError(f"{name} must be {dtype} {shape}, got {got}")
