@@ -248,22 +248,37 @@ class LoRABank(nn.Module):
     @torch.no_grad()
     def set_adapter(self, index: int, A: torch.Tensor, B: torch.Tensor, alpha: float | None = None) -> None:
         """Put an adapter's factors (rank, in) and (out, rank) in place ``index``; ``alpha`` defaults to their rank."""
-        r = A.shape[0]
-        if not 0 <= index < self.count:
-            raise ValueError(f"adapter {index} of {self.count}")
-        if A.shape != (r, self.lora_A.shape[2]) or B.shape != (self.lora_B.shape[1], r) or not 1 <= r <= self.lora_A.shape[1]:
-            raise ValueError(f"factors {tuple(A.shape)} and {tuple(B.shape)} do not fit a bank of rank {self.lora_A.shape[1]}, "
-                             f"{self.lora_A.shape[2]} -> {self.lora_B.shape[1]}")
+        r = self._fits(index, A, B)
         for held, t in ((self.lora_A[index], A), (self.lora_B[index].t(), B.t())):
             held[:r].copy_(t)
             held[r:].zero_()
         self.scales[index] = (r if alpha is None else alpha) / r
         self.ranks[index] = r
 
-    def adapter(self, index: int):
-        """``(A, B, alpha)`` of an adapter, without the zero ranks (views; waits for the device)."""
+    @torch.no_grad()
+    def _remove(self, index: int) -> None:
+        """No adapter in place ``index``: rank 0, whose rows keep the base's output and which training leaves as it is."""
+        self._place(index)
+        self.lora_A[index].zero_()
+        self.lora_B[index].zero_()
+        self.scales[index] = 1.0
+        self.ranks[index] = 0
+
+    def _place(self, index: int) -> None:
         if not 0 <= index < self.count:
             raise ValueError(f"adapter {index} of {self.count}")
+
+    def _fits(self, index: int, A: torch.Tensor, B: torch.Tensor) -> int:
+        """The rank of factors that have a place here."""
+        self._place(index)
+        (held, K), N, r = self.lora_A.shape[1:], self.lora_B.shape[1], A.shape[0] if A.dim() else 0
+        if A.shape != (r, K) or B.shape != (N, r) or not 1 <= r <= held:
+            raise ValueError(f"factors {tuple(A.shape)} and {tuple(B.shape)} do not fit a bank of rank {held}, {K} -> {N}")
+        return r
+
+    def adapter(self, index: int):
+        """``(A, B, alpha)`` of an adapter, without the zero ranks (views; waits for the device)."""
+        self._place(index)
         r = int(self.ranks[index])
         return self.lora_A[index, :r], self.lora_B[index, :, :r], float(self.scales[index]) * r
 
@@ -320,8 +335,8 @@ def inject_lora_bank(dit, count: int, rank: int, alpha: float | None = None, *, 
 
 def load_lora_into(banks: dict, index: int, path: str, *, key_prefix: str = "diffusion_model") -> int:
     """Load a saved adapter (:func:`save_lora`) into place ``index`` of ``banks``, its scale ``alpha / rank`` from the file's
-    metadata (1 without).  A bank that the file does not name gets no adapter there (zero factors).  Returns how many of the
-    file's adapters have no bank (0: everything loaded)."""
+    metadata (1 without).  A bank that the file does not name gets no adapter there (rank 0).  Returns how many of the file's
+    adapters have no bank (0: everything loaded).  A file that does not fit one of the banks changes none."""
     from safetensors import safe_open
 
     with safe_open(path, framework="pt") as f:
@@ -331,19 +346,29 @@ def load_lora_into(banks: dict, index: int, path: str, *, key_prefix: str = "dif
     if not names:
         raise ValueError(f"{path} holds no adapters under {key_prefix!r}")
     ratio = float(meta["alpha"]) / float(meta["rank"]) if "alpha" in meta and "rank" in meta else 1.0
+    pairs = {name: [saved.get(_lora._key(key_prefix, name, w)) for w in ("A", "B")] for name in banks}
     for name, bank in banks.items():
-        A, B = (saved.get(_lora._key(key_prefix, name, w)) for w in ("A", "B"))
+        if any(t is None for t in pairs[name]):
+            bank._place(index)
+        else:
+            bank._fits(index, *pairs[name])
+    for name, bank in banks.items():
+        A, B = pairs[name]
         if A is None or B is None:
-            A, B = torch.zeros(1, bank.lora_A.shape[2]), torch.zeros(bank.lora_B.shape[1], 1)
-        bank.set_adapter(index, A, B, ratio * A.shape[0])
+            bank._remove(index)
+        else:
+            bank.set_adapter(index, A, B, ratio * A.shape[0])
     return len(names - set(banks))
 
 
 def save_lora_from(banks: dict, index: int, path: str, *, metadata: dict | None = None,
                    key_prefix: str = "diffusion_model") -> None:
-    """Write adapter ``index`` of ``banks`` as a file of its own, as :func:`save_lora` writes one.  All banks must hold one rank
-    and one alpha there."""
+    """Write adapter ``index`` of ``banks`` as a file of its own, as :func:`save_lora` writes one.  All banks that hold one there
+    must hold one rank and one alpha; those of rank 0 are left out."""
     parts = {name: bank.adapter(index) for name, bank in banks.items()}
+    parts = {name: part for name, part in parts.items() if part[0].shape[0]}
+    if not parts:
+        raise ValueError(f"no adapter is held in place {index}")
     kinds = {(A.shape[0], alpha) for A, _, alpha in parts.values()}
     if len(kinds) != 1:
         raise ValueError(f"the banks' ranks and alphas differ at {index}: {sorted(kinds)}")

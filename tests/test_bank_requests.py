@@ -224,3 +224,54 @@ def test_a_batch_without_rows_has_a_pass_back(k2):
             assert g.shape == t.shape and g.dtype == t.dtype and not int(g.count_nonzero())
     with torch.no_grad():
         assert not k2.add_adapters(y, x, A, B, ids).requires_grad
+
+
+# -- files ------------------------------------------------------------------------------------------------------------
+def _file(k2, path, rank, only="", seed=0):
+    adapters = k2.inject_lora(_Dit(), rank, float(rank))
+    g = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for m in adapters.values():
+            m.lora_A.copy_(m.lora_A.bfloat16())
+            m.lora_B.copy_(torch.randn(m.lora_B.shape, generator=g).bfloat16())
+    kept = {n: m for n, m in adapters.items() if only in n}
+    k2.save_lora(kept, str(path), rank=rank, alpha=float(rank))
+    return str(path), kept
+
+
+def test_a_file_that_does_not_fit_every_bank_changes_none(k2, tmp_path):
+    banks = k2.inject_lora_bank(_Dit(), 2, 32)
+    small = k2.inject_lora_bank(_Dit(), 2, 16)
+    last = list(banks)[-1]
+    banks[last] = small[last]
+    path, _ = _file(k2, tmp_path / "a", 20)
+    before = [t.clone() for b in banks.values() for t in (b.lora_A, b.lora_B, b.scales, b.ranks)]
+    with pytest.raises(ValueError, match="fit a bank"):
+        k2.load_lora_into(banks, 1, path)
+    with pytest.raises(ValueError, match="adapter 2 of 2"):
+        k2.load_lora_into(banks, 2, path)
+    after = [t for b in banks.values() for t in (b.lora_A, b.lora_B, b.scales, b.ranks)]
+    assert all(torch.equal(a, b) for a, b in zip(before, after))
+
+
+def test_banks_that_a_file_does_not_name_hold_no_adapter_there(k2, tmp_path):
+    """Rank 0, which the file written back leaves out again."""
+    banks = k2.inject_lora_bank(_Dit(), 2, 16)
+    path, kept = _file(k2, tmp_path / "a", 16, only="attn")
+    assert k2.load_lora_into(banks, 1, path) == 0
+    for name, b in banks.items():
+        assert b.ranks.tolist() == [16, 16 if "attn" in name else 0]
+        A, B, alpha = b.adapter(1)
+        assert A.shape[0] == B.shape[1] == int(b.ranks[1]) and alpha == float(b.ranks[1])
+        if "attn" not in name:
+            assert not int(b.lora_A[1].count_nonzero()) and not int(b.lora_B[1].count_nonzero())
+    out = str(tmp_path / "b")
+    k2.save_lora_from(banks, 1, out)
+    from safetensors.torch import load_file
+    a, b = load_file(path), load_file(out)
+    assert set(a) == set(b) and all(torch.equal(a[k], b[k]) for k in a)
+    assert k2.load_lora_into(banks, 0, out) == 0
+    for b in banks.values():                # an adapter that none of the banks holds
+        b.ranks[0] = 0
+    with pytest.raises(ValueError, match="no adapter"):
+        k2.save_lora_from(banks, 0, out)
