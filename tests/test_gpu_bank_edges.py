@@ -57,6 +57,43 @@ def test_ranks_behind_an_adapters_own_keep_zero_gradients(k2, dev, rows):
     assert torch.isfinite(dA[1]).all() and torch.isfinite(dB[1]).all() and not torch.isfinite(dA[0]).all()
 
 
+# -- precision --------------------------------------------------------------------------------------------------------
+def _two_parts(t):
+    """float32 as two bf16 parts, in float64."""
+    hi = t.bfloat16()
+    return hi.double() + (t - hi.float()).bfloat16().double()
+
+
+@pytest.mark.parametrize("how", ["sorted", "mixed"])
+@pytest.mark.parametrize("lead, of, count, R, K, N", [
+    ((65,), (65,), 3, 32, 320, 64), ((3, 50), (3,), 5, 48, 128, 256), ((2, 120), (2,), 1, 16, 256, 320),
+    ((70,), (70,), 2, 144, 64, 128), ((2, 33, 3), (2, 33), 4, 64, 64, 192)])
+def test_gradients_of_f32_factors_hold_its_bits(k2, dev, lead, of, count, R, K, N, how):
+    """dA and dB in f32 are off by the sums' roundings alone.  Their operands enter in three bf16 parts, which hold them
+    whole.  A sum of n products (n at most 320 here) takes 3 n / 32 matrix instructions, of which each rounds a running sum a
+    few times (4, say): 120 roundings of up to 2^-24 of a sum that grows as the root of its terms come to 2^-24 sqrt(120 / 2)
+    of the result, as a norm over many, 4.6e-7 for the first product and as much for the second: 6.5e-7 together.  With two
+    parts an operand is off by 2^-17 of itself at most, and that is above the bar for these inputs (shown in float64)."""
+    bar = 1e-6
+    ids = _ids(of, count, how)
+    x, y, A, B, ids, scales, _, dy = _make(dev, lead, ids, count, R, K, N, torch.float32)
+    want, _ = _formula(x, y, A, B, ids, scales, dy)
+    leaves = [t.clone().requires_grad_() for t in (A, B)]
+    got = torch.autograd.grad(k2.add_adapters(y, x, *leaves, ids, scales), leaves, dy)
+    for g, w in zip(got, want[2:]):
+        assert float((g.double() - w).norm()) <= bar * float(w.norm())
+    rows = x.shape[:-1].numel()
+    each = ids.reshape(-1).repeat_interleave(rows // ids.numel())
+    off = torch.zeros(2, dtype=torch.float64)
+    for a in range(count):
+        at = (each == a).nonzero()[:, 0]
+        xa, da, s = x.reshape(rows, K)[at].double(), dy.reshape(rows, N)[at].double(), float(scales[a])
+        g, u = s * da @ _two_parts(B[a]), s * xa @ _two_parts(A[a]).t()
+        off[0] += float((_two_parts(g.float()).t() @ xa - want[2][a]).square().sum())
+        off[1] += float((da.t() @ _two_parts(u.float()) - want[3][a]).square().sum())
+    assert all(float(o) ** 0.5 > bar * float(w.norm()) for o, w in zip(off, want[2:]))
+
+
 # -- batches without rows ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", ["w8a8", "linear"])
 def test_a_batch_without_rows_trains_nothing(k2, dev, kind):
