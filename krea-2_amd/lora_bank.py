@@ -199,7 +199,12 @@ class LoRABank(nn.Module):
     Initialised as ``LoRALinear`` (``lora.py:30-41``): ``A`` kaiming-uniform, ``B`` zeros, ``scale = alpha / rank``.
 
     Which rows use which adapter comes with the call, or from :func:`lora_requests` around the model's, or from ``adapters``
-    (one setting for all threads); without any the output is ``base(x)``.  ``scale_mul`` and ``lora_scaled`` act on all adapters."""
+    (one setting for all threads); without any the output is ``base(x)``.  ``scale_mul`` and ``lora_scaled`` act on all adapters.
+
+    The adapters are one parameter to an optimizer.  One that no row of a step had gets gradients of zeros, and a step moves
+    it all the same: by its weight decay, and by the momentum that earlier steps left (its count of steps goes on too).
+    Without decay, one that never had a row stays bit for bit.  Adapters that are to stay as they are while others train
+    belong in a bank that is not stepped, or are put back (:meth:`set_adapter`) from their files."""
 
     _own = None     # the requests of all calls that are in no body
 

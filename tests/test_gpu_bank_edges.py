@@ -1,5 +1,8 @@
-"""GPU tests of a bank of adapters at its edges."""
+"""GPU tests of a bank of adapters at its edges: ranks that are no multiple of 16 in storage that holds something behind them,
+gradients in the precision of their type, batches and adapters without rows, bases that change between the passes, and
+requests of several threads."""
 import contextlib
+import copy
 import threading
 
 import pytest
@@ -106,6 +109,45 @@ def test_a_batch_without_rows_trains_nothing(k2, dev, kind):
     assert x.grad.shape == x.shape
     for p in (bank.lora_A, bank.lora_B):
         assert p.grad.shape == p.shape and p.grad.dtype == p.dtype and not int(p.grad.count_nonzero())
+
+
+# -- adapters without rows --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adapters_without_rows_are_stepped_as_zero_gradients(k2, dev, bits):
+    """A bank's adapters are one parameter: the step decays one that no row had, and moves one that had rows before on, as
+    torch's step does with a gradient of zeros.  Without decay, one that never had rows stays bit for bit."""
+    banks = []
+    for decay in (0.0, 0.1):
+        torch.manual_seed(0)
+        bank = k2.LoRABank(_linear(k2, dev, 128, 192, "linear"), 3, 16)
+        with torch.no_grad():
+            bank.lora_B.normal_()
+        banks.append((bank, k2.AdamW([bank.lora_A, bank.lora_B], lr=1e-2, weight_decay=decay, state_bits=bits)))
+    alike = copy.deepcopy(banks[1][0])
+    other = torch.optim.AdamW([alike.lora_A, alike.lora_B], lr=1e-2, weight_decay=0.1)
+    x = torch.randn(2, 9, 128, generator=torch.Generator().manual_seed(1)).to(dev).bfloat16()
+    start = [p.detach().clone() for p in (banks[0][0].lora_A, banks[0][0].lora_B)]
+    before = None
+    for ids in ([0, 1], [1, 1]):        # adapter 0 in the first step alone, adapter 2 in none
+        ids = torch.tensor(ids, device=dev)
+        for bank, opt in banks:
+            opt.zero_grad()
+            bank(x, ids).float().square().sum().backward()
+        for p, q in zip((alike.lora_A, alike.lora_B), (banks[1][0].lora_A, banks[1][0].lora_B)):
+            p.grad = q.grad.clone()
+        before = [p.detach().clone() for p in (banks[1][0].lora_A, banks[1][0].lora_B)]
+        for _, opt in banks:
+            opt.step()
+        other.step()
+    for p, s in zip((banks[0][0].lora_A, banks[0][0].lora_B), start):
+        assert torch.equal(p[2], s[2])                      # no decay and never a row
+    for p, q, b, s in zip((banks[1][0].lora_A, banks[1][0].lora_B), (alike.lora_A, alike.lora_B), before, start):
+        if bits == 32:
+            # two updates of 1e-2, each off by 8 roundings of its terms
+            assert bool(((p - q).abs() <= 2.0 ** -22 * q.abs() + 2 * 1e-2 * 2.0 ** -20).all())
+        # two steps of 1 - 1e-2 * 0.1, each rounded once, and the factor itself
+        assert bool(((p[2].double() - s[2].double() * (1 - 1e-3) ** 2).abs() <= 4 * 2.0 ** -24 * s[2].abs()).all())
+        assert not torch.equal(p[0], b[0])                  # on its momentum
 
 
 # -- a base that changes ----------------------------------------------------------------------------------------------
