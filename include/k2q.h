@@ -408,7 +408,7 @@ int k2q_gemm_dx_grouped_ws(const k2q_dx_segment* seg, int64_t nseg, int64_t M, i
  *   without rows and for ranks past its own.  dx, dA (with x), dB (with u) are nullable; one at least is given.
  * x T x K, y, out and dy T x N, dx T x K: bf16, contiguous.  Sums are f32 in a fixed order; f32 factors, u and g enter the
  * products in 16 bits of precision where the result is bf16, in 24 where it is f32.  K and N multiples of 64 up to 2^24, R of
- * 16 up to K2Q_MAX_RANK, count <= K2Q_MAX_ADAPTERS, T <= 2^30 - 64, T max(K, N) <= 2^37, T R <= 2^33, R max(K, N) <= 2^31.
+ * 16 up to K2Q_MAX_RANK, count <= K2Q_MAX_ADAPTERS, T <= 2^30, T max(K, N) <= 2^37, T R <= 2^33, R max(K, N) <= 2^31.
  * ws: *_ws_bytes bytes, 16-byte aligned (need_factors: dA or dB is given). */
 #define K2Q_MAX_ADAPTERS 1024
 typedef struct {

@@ -1549,8 +1549,8 @@ def check_bank(t, width: int, A, B, ids, scales, ranks) -> None:
             raise ValueError(f"{name} must be {count} contiguous {dtype} values on {dev}, got {tuple(v.shape)} {v.dtype} on "
                              f"{v.device}")
     T, most = t.numel() // width, max(K, N)
-    if T > (1 << 30) - 64 or T * most > 1 << 37 or T * R > 1 << 33 or R * most > 1 << 31:
-        raise ValueError(f"{T} rows of {K} -> {N} features and rank {R}: the most are 2^30 - 64 rows, 2^37 elements of a tensor of "
+    if T > 1 << 30 or T * most > 1 << 37 or T * R > 1 << 33 or R * most > 1 << 31:
+        raise ValueError(f"{T} rows of {K} -> {N} features and rank {R}: the most are 2^30 rows, 2^37 elements of a tensor of "
                          "the batch, 2^33 of rows x rank and 2^31 of a factor")
     _device_check(dev)
 

@@ -939,7 +939,7 @@ bool bank_of(const Tensor* A, const Tensor* B, const Tensor* ids, const Tensor* 
   o.T = t.numel() / t.size(t.dim() - 1);
   o.per = o.T / ids->numel();
   const int64_t most = K > N ? K : N;
-  if (o.T > (1 << 30) - 64 || o.T * most > (int64_t)1 << 37 || o.T * R > (int64_t)1 << 33 || R * most > (int64_t)1 << 31)
+  if (o.T > 1 << 30 || o.T * most > (int64_t)1 << 37 || o.T * R > (int64_t)1 << 33 || R * most > (int64_t)1 << 31)
     return false;
   o.b = {A->data_ptr(), B->data_ptr(), ids->data_ptr(), as<int32_t>(ptr(ranks)), as<float>(ptr(scales)), (float)scale,
          it == at::kLong, ty == at::kFloat ? K2Q_DTYPE_F32 : K2Q_DTYPE_BF16, (int32_t)count, (int32_t)R, (int32_t)K,

@@ -899,10 +899,10 @@ int check(const k2q_bank* b, int64_t T, int64_t per) {
       !b->ids || !k2q_aligned(b->ids, b->ids64 ? 8 : 4) || !k2q_aligned(b->ranks, 4) || !k2q_aligned(b->scales, 4) || T < 1 ||
       per < 1 || T % per)
     return K2Q_EINVAL;
-  // The row numbers of a piece, up to T + its length, fit 32 bits; and so do the threads of a launch: 256 for each 64 rows
-  // and 256 columns of "up", 64 rows of "down", T R / 4 of the join, R (K + N) / 4 of the gradients' join.
+  // The row numbers of a piece, up to T + its length, fit 32 bits; and so do the threads of a launch: T C / 64 of "up",
+  // T R / 4 of the join, R (K + N) / 4 of the gradients' join.
   const int64_t most = b->K > b->N ? b->K : b->N;
-  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > (1 << 30) - ROWS || most > 1 << 24 || T * most > (int64_t)1 << 37 ||
+  if (b->count > K2Q_MAX_ADAPTERS || b->R > K2Q_MAX_RANK || T > 1 << 30 || most > 1 << 24 || T * most > (int64_t)1 << 37 ||
       T * b->R > (int64_t)1 << 33 || b->R * most > (int64_t)1 << 31)
     return K2Q_EUNSUPPORTED;
   return K2Q_OK;

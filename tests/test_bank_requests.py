@@ -1,6 +1,5 @@
 """CPU tests of what a bank of adapters is asked for, and of its files."""
 import asyncio
-import ctypes
 import threading
 
 import pytest
@@ -276,18 +275,3 @@ def test_banks_that_a_file_does_not_name_hold_no_adapter_there(k2, tmp_path):
         b.ranks[0] = 0
     with pytest.raises(ValueError, match="no adapter"):
         k2.save_lora_from(banks, 0, out)
-
-
-# -- sizes ------------------------------------------------------------------------------------------------------------
-def test_rows_beyond_a_launchs_threads_are_refused(k2):
-    """A tile of 64 rows is a workgroup of 256 threads at least, and a launch has fewer than 2^32 (addresses that are never
-    read)."""
-    lib, a = k2._lib.load(), 4096
-    b = k2._lib.Bank(A=a, B=a, ids=a, scale=1.0, ids64=1, dtype=1, count=3, R=16, K=64, N=64)
-    p = ctypes.addressof(b)
-    for T in (1 << 30, (1 << 30) - 63):
-        assert lib.k2q_bank_fwd(p, T, 1, a, a, a, None, a, 1 << 62, None) == -4
-        assert lib.k2q_bank_bwd(p, T, 1, a, a, a, None, a, a, a, a, 1 << 62, None) == -4
-        assert lib.k2q_bank_fwd_ws_bytes(p, T, 1) == 0 and lib.k2q_bank_bwd_ws_bytes(p, T, 1, 1) == 0
-    T = (1 << 30) - 64
-    assert lib.k2q_bank_fwd_ws_bytes(p, T, 1) >= T * 16 * 4 and lib.k2q_bank_bwd_ws_bytes(p, T, 1, 1) >= T * 16 * 8
