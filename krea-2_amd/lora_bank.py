@@ -130,9 +130,17 @@ class _Body:
     def __init__(self, banks, ids, outer):
         self.banks, self.ids, self.outer, self.open = weakref.WeakSet(banks), ids, outer, True
         self.named = ids is not None
+        self._count(1)
 
     def close(self) -> None:
         self.open, self.ids = False, None
+        self._count(-1)
+
+    def _count(self, by: int) -> None:
+        if self.named:
+            with _counting:
+                for bank in self.banks:
+                    bank.__dict__["_named"] = bank._named + by
 
     def of(self, bank) -> "_Body | None":
         """The innermost body of ``bank``, from this one outwards."""
@@ -141,6 +149,8 @@ class _Body:
             body = body.outer
         return body
 
+
+_counting = threading.Lock()
 
 # The body that the caller is in: a thread's, or an asyncio task's (what it starts with a copy of its context included)
 _body: contextvars.ContextVar = contextvars.ContextVar("lora_requests", default=None)
@@ -170,6 +180,8 @@ def _backward_callers() -> list:
 
 def _requests(bank) -> torch.Tensor | None:
     """The requests that ``bank`` runs with now where its call names none."""
+    if torch.compiler.is_compiling() and not bank._named and bank._own is None:
+        return None         # no body names any: what follows cannot be traced into a graph
     body, me = _entered(), threading.get_ident()
     if torch._C._current_graph_task_id() < 0:
         last = _last.get(me)
@@ -207,6 +219,7 @@ class LoRABank(nn.Module):
     belong in a bank that is not stepped, or are put back (:meth:`set_adapter`) from their files."""
 
     _own = None     # the requests of all calls that are in no body
+    _named = 0      # bodies that are open now, in any thread, and name requests
 
     def __init__(self, base: nn.Module, count: int, rank: int, alpha: float | None = None, dtype: torch.dtype = torch.float32):
         super().__init__()

@@ -180,6 +180,18 @@ def test_a_recomputed_pass_that_two_threads_may_want_is_refused(k2, seen, monkey
     assert calls[-1] is ids
 
 
+def test_a_compiled_bank_without_requests_is_one_graph(k2):
+    bank = k2.LoRABank(torch.nn.Linear(64, 128), 2, 16)
+    x = torch.randn(2, 64)
+    run = torch.compile(bank, backend="eager", fullgraph=True)
+    assert torch.equal(run(x), bank.base(x))
+    with k2.lora_requests(bank, None):
+        assert torch.equal(run(x), bank.base(x))
+    with k2.lora_requests(bank, _ids(0)):
+        assert bank._named == 1
+    assert bank._named == 0 and torch.equal(run(x), bank.base(x))
+
+
 # -- recomputed passes ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("reentrant", [True, False])
 def test_a_pass_recomputed_outside_its_body_is_refused(k2, seen, reentrant):
