@@ -334,16 +334,36 @@ __device__ __forceinline__ T rounded(float p, int stochastic, uint32_t random) {
 
 // One element's moments and parameter, in 32 bits:
 //   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  p = decay p - size m / (root sqrt(v) + eps)
-// Moments in 32 bits are bound by memory, and their root and quotient are rounded correctly.  With codes the vector unit is as
-// busy as memory (about 60 operations an element, 80 with random rounding of the parameter): the hardware's root and
-// reciprocals, 1 ulp off each, take a third of what the exact ones take.
-template <bool kFast>
-__device__ __forceinline__ void element(const Step& a, const Scalars& s, float g, float& m, float& v, float& r, float& p) {
-  m = __builtin_fmaf(m, a.beta1, g * a.alpha1);
-  v = __builtin_fmaf(v, a.beta2, g * g * a.alpha2);
-  r = kFast ? __builtin_amdgcn_sqrtf(v) : sqrtf(v);
-  const float d = __builtin_fmaf(r, s.root, a.eps), u = kFast ? m * __builtin_amdgcn_rcpf(d) : m / d;
-  p = __builtin_fmaf(p, s.decay, -s.size * u);
+// Moments in 32 bits are bound by memory, and their root and quotient are rounded correctly.  With codes (kCodes) every
+// operation that leads to a code rounds on its own and correctly, so that a code is what the formula's 32-bit operations
+// give: fused or off by an ulp, one in 2^18 fell to the other side of its border, and the element's next update moved by up to an
+// eighth.  The parameter's quotient alone is the hardware's there, 1 ulp off: the vector unit is as busy as memory (about 65
+// operations an element, 85 with random rounding of the parameter).
+template <bool kCodes>
+__device__ __forceinline__ void moments_of(const Step& a, float g, float& m, float& v) {
+  if constexpr (kCodes) {
+    m = m * a.beta1 + g * a.alpha1;
+    v = v * a.beta2 + g * g * a.alpha2;
+  } else {
+    m = __builtin_fmaf(m, a.beta1, g * a.alpha1);
+    v = __builtin_fmaf(v, a.beta2, g * g * a.alpha2);
+  }
+}
+
+template <bool kCodes>
+__device__ __forceinline__ float updated(const Step& a, const Scalars& s, float m, float r, float p) {
+  const float d = __builtin_fmaf(r, s.root, a.eps), u = kCodes ? m * __builtin_amdgcn_rcpf(d) : m / d;
+  return __builtin_fmaf(p, s.decay, -s.size * u);
+}
+
+// The root of a value from LEAST to below infinity: a Newton step from the hardware's reciprocal root, whose residual is exact
+// there.  Rounded correctly but where the root lies within 2^-21 of a step from the middle of two.  396M bf16 parameters with
+// random rounding: 785 us with the hardware's roots and reciprocals, 808 with this and divisions, 895 with sqrtf.
+constexpr uint32_t LEAST = 0x0D800000u;      // 2^-100
+
+__device__ __forceinline__ float root_of(float v) {
+  const float y = __builtin_amdgcn_rsqf(v), r = v * y;
+  return __builtin_fmaf(__builtin_fmaf(-r, r, v), 0.5f * y, r);
 }
 
 template <typename T, bool kCodes, int N>
@@ -397,19 +417,30 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
         }
       }
       const float sm = st.m_scale[place / BLOCK], sv = st.v_scale[place / BLOCK];
-      uint32_t bm = 0, bv = 0;
+      uint32_t bm = 0, bv = 0, far = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int q = j / 4, i = j % 4;
-        m[q][i] = decode_m(wm[q], i) * sm;
         const float root = value_v(wv[q] >> (8 * i) & 0xFFu) * sv;
-        float mj = m[q][i], vj = root * root, rj, pj = p[q][i];
-        element<true>(st, s, g[q][i] * by, mj, vj, rj, pj);
+        float mj = decode_m(wm[q], i) * sm, vj = root * root;
+        moments_of<true>(st, g[q][i] * by, mj, vj);
         m[q][i] = mj;
-        r[q][i] = rj;
-        p[q][i] = pj;
+        r[q][i] = vj;
         bm = max(bm, __float_as_uint(mj) & 0x7FFFFFFFu);
-        bv = max(bv, __float_as_uint(rj) & 0x7FFFFFFFu);
+        far = max(far, __float_as_uint(vj) - LEAST);
+      }
+      if (__ballot(far >= INFINITE - LEAST)) {      // zeros too
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j / 4][j % 4] = sqrtf(r[j / 4][j % 4]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j / 4][j % 4] = root_of(r[j / 4][j % 4]);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int q = j / 4, i = j % 4;
+        p[q][i] = updated<true>(st, s, m[q][i], r[q][i], p[q][i]);
+        bv = max(bv, __float_as_uint(r[q][i]) & 0x7FFFFFFFu);
       }
       bm = half_max(bm);
       bv = half_max(bv);
@@ -428,8 +459,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
       float am = __uint_as_float(bm), av = __uint_as_float(bv);
       am = am < SMALLEST ? 0.f : am;
       av = av < SMALLEST ? 0.f : av;
-      const float fm = am > 0.f ? M_TOP * __builtin_amdgcn_rcpf(am) : 0.f;
-      const float fv = av > 0.f ? V_TOP * __builtin_amdgcn_rcpf(av) : 0.f;
+      const float fm = am > 0.f ? M_TOP * (1.f / am) : 0.f;
+      const float fv = av > 0.f ? V_TOP * (1.f / av) : 0.f;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         wm[q] = wv[q] = 0;
@@ -467,11 +498,11 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(Table<N> a, int64_t chun
       v4f wm = __builtin_nontemporal_load(fm), wv = __builtin_nontemporal_load(fv);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float mj = wm[i], vj = wv[i], rj, pj = p[0][i];
-        element<false>(st, s, g[0][i] * by, mj, vj, rj, pj);
+        float mj = wm[i], vj = wv[i];
+        moments_of<false>(st, g[0][i] * by, mj, vj);
         wm[i] = mj;
         wv[i] = vj;
-        p[0][i] = pj;
+        p[0][i] = updated<false>(st, s, mj, sqrtf(vj), p[0][i]);
       }
       __builtin_nontemporal_store(wm, fm);
       __builtin_nontemporal_store(wv, fv);
