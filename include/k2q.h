@@ -448,7 +448,8 @@ int k2q_bank_bwd(const k2q_bank* b, int64_t T, int64_t per, const uint16_t* dy, 
  * e4m3(code) scale; v = (u(code) scale)^2 with u(c) = c / 16 below 16 and (16 + c % 16) 2^(c / 16 - 5) from there on; a scale is
  * the block's largest |m| / 448 or sqrt(v) / 31744, a block whose largest is under 2^-100 holds zeros, and a code is rounded at
  * random between its neighbours, roots above zero to 1 at least.  Random bits are a function of seed, T and the element's
- * place at + i.  Each operation that leads to a code rounds to 32 bits on its own.  Values of m that are not finite stay so (code 0x7F); a root that is not finite has code 255.
+ * place at + i.  Each operation that leads to a code rounds to 32 bits on its own.  Values of m that are not finite stay so
+ * (code 0x7F); a root that is not finite has code 255.
  * t[i].index strictly increasing; ws of k2q_adamw_ws_bytes(count) bytes, 16-byte aligned.
  * k2q_moments: m and v (f32 or bf16) of n codes, n a multiple of K2Q_MOMENT_BLOCK. */
 #define K2Q_MOMENT_BLOCK 256

@@ -26,6 +26,6 @@ from .optim import AdamW, clip_grad_norm_
 __all__ = ["ConvRotLinear", "quantize_dit_convrot", "set_dx_weight_cache", "MODES", "Fp8Linear", "quantize_dit_fp8",
            "save_quantized_base", "load_quantized_base", "fuse_producers", "group_siblings", "modulated_rmsnorm",
            "residual_rmsnorm", "input_codes", "swiglu", "RotaryEmbedding", "RotaryScaling", "AdamW", "clip_grad_norm_",
-           "LoRABank", "add_adapters", "inject_lora_bank", "lora_requests", "load_lora_into", "save_lora_from", "LoRALinear", "inject_lora",
-           "inject_lora_te", "QWEN_TE_TARGETS", "lora_scaled", "lora_disabled", "lora_parameters", "save_lora",
+           "LoRABank", "add_adapters", "inject_lora_bank", "lora_requests", "load_lora_into", "save_lora_from", "LoRALinear",
+           "inject_lora", "inject_lora_te", "QWEN_TE_TARGETS", "lora_scaled", "lora_disabled", "lora_parameters", "save_lora",
            "load_lora_weights", "load_lora", "DEFAULT_TARGETS", "_lib"]

@@ -1466,8 +1466,7 @@ def same_items(a: list, b: list) -> bool:
 
 
 def unchanged(state: dict, keys: list, dicts: list, values: list) -> bool:
-    """Whether a dict of dicts has these keys and values, and those these values, as objects (448 parameters of 3 values: 10
-    us)."""
+    """Whether a dict of dicts has these keys and values, and those these values, as objects."""
     return _fast().unchanged(state, keys, dicts, values)
 
 

@@ -357,8 +357,9 @@ __device__ __forceinline__ float updated(const Step& a, const Scalars& s, float 
 }
 
 // The root of a value from LEAST to below infinity: a Newton step from the hardware's reciprocal root, whose residual is exact
-// there.  Rounded correctly but where the root lies within 2^-21 of a step from the middle of two.  396M bf16 parameters with
-// random rounding: 785 us with the hardware's roots and reciprocals, 808 with this and divisions, 895 with sqrtf.
+// there.  Rounded correctly but where the root lies within 2^-21 of a step from the middle of two.  bf16 parameters with random
+// rounding, with the hardware's roots and reciprocals / this and divisions / sqrtf: 396M with codes at random 785 / 808 / 895 us,
+// 434M of a training's 858 / 900.
 constexpr uint32_t LEAST = 0x0D800000u;      // 2^-100
 
 __device__ __forceinline__ float root_of(float v) {
@@ -584,8 +585,8 @@ int64_t norm_parts(const k2q_step_tensor* t, int64_t count) {
   return parts;
 }
 
-// f(table) over the tensors of one type, N and fewer than 2^24 workgroups at a time.  Behind a pass over the gradients they go backwards:
-// what that pass read last is still in the last-level cache.
+// f(table) over the tensors of one type, N and fewer than 2^24 workgroups at a time.  Behind a pass over the gradients they go
+// backwards: what that pass read last is still in the last-level cache.
 template <int N, class F>
 void tables(const k2q_step_tensor* t, int64_t count, int dtype, int64_t chunk, bool backwards, F&& f) {
   Table<N> a{};

@@ -103,8 +103,8 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B:
 
     Sums are float32 and ``out`` is rounded once.  Float32 factors (and the sums between the products) enter the matrix
     units as two bf16 parts, 2^-17 of a value off at most, or on the way to a float32 gradient as three, which hold it.  Rows
-    may have any order; rows of one adapter that lie together are faster.  Differentiable in ``y``, ``x`` and both factors.  A value that is infinite or NaN spoils its own row, and the
-    gradients of its row's adapter."""
+    may have any order; rows of one adapter that lie together are faster.  Differentiable in ``y``, ``x`` and both factors.  A
+    value that is infinite or NaN spoils its own row, and the gradients of its row's adapter."""
     grad = torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or lora_A.requires_grad or lora_B.requires_grad)
     if not grad and not _lib.observed() and not (scales is not None and scales.requires_grad):
         out = _lib.bank_native(y, x, lora_A, lora_B, adapters, scales, ranks, scale, False)

@@ -39,7 +39,7 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 
 class AdamW(torch.optim.Optimizer):
     """AdamW (Loshchilov and Hutter, "Decoupled weight decay regularization", 2019) with the update of ``torch.optim.AdamW``,
-    in float32, over parameters in float32, bfloat16 or float16 whose gradients have their type.
+    in float32, over contiguous parameters in float32, bfloat16 or float16 whose gradients have their type.
 
     ``max_norm``: the gradients, over all groups together, are first brought to this 2-norm at most, as ``clip_grad_norm_``
     does it, but they are not written: the step multiplies them as it reads them.  :attr:`grad_norm` holds the norm of the
@@ -49,7 +49,8 @@ class AdamW(torch.optim.Optimizer):
     by the largest of 256 neighbours.  ``stochastic=True`` rounds bfloat16 parameters to one of their two neighbours at
     random instead of to the nearest, so that updates below half a step are not lost (the reference's full fine-tune does
     that, ``fused_adamw.py:44-56``).  Codes and such parameters are rounded by chance, with bits that are a function of
-    ``seed``, the step and the element's place in its group: equal runs give equal results.
+    ``seed``, the step and the element's place in its group: equal runs give equal results.  Groups with one seed share
+    those bits place by place; each may have its own.
 
     ``lr`` may be a float32 tensor of one element on the device (read there, for captured graphs).  Without ``max_norm``, a
     gradient that is infinite or NaN spoils its own element, as in torch.  Make a step, or load a state, before a graph
