@@ -781,7 +781,8 @@ PyObject* py_unchanged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PyObject *key, *d, *v;
   Py_ssize_t i = 0, k = 0;
   for (Py_ssize_t at = 0; PyDict_Next(a[0], &at, &key, &d); ++i) {
-    if (i >= count || key != PyList_GET_ITEM(a[1], i) || d != PyList_GET_ITEM(a[2], i) || !PyDict_Check(d)) Py_RETURN_FALSE;
+    if (i >= count || key != PyList_GET_ITEM(a[1], i) || d != PyList_GET_ITEM(a[2], i)) Py_RETURN_FALSE;
+    if (!PyDict_Check(d)) continue;
     for (Py_ssize_t in = 0; PyDict_Next(d, &in, nullptr, &v); ++k)
       if (k >= values || v != PyList_GET_ITEM(a[3], k)) Py_RETURN_FALSE;
   }

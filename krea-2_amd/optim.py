@@ -134,7 +134,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _note_state(self) -> None:
         dicts = list(self.state.values())
-        self._seen = (list(self.state), dicts, [v for d in dicts for v in d.values()])
+        self._seen = (list(self.state), dicts, [v for d in dicts if isinstance(d, dict) for v in d.values()])
 
     def _follow_state(self) -> None:
         """Drop the buffers of groups whose states are not theirs any more: the next use makes them from the states."""

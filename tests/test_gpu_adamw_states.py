@@ -161,3 +161,16 @@ def test_other_bits_than_the_moments_have_are_refused(k2, dev):
     opt.state.clear()
     opt.step()
     assert opt.state[p]["exp_avg"].dtype == torch.float8_e4m3fn and float(opt.state[p]["step"]) == 1
+
+
+def test_entries_of_the_users_own_stay(k2, dev):
+    """What a program keeps in the state beside the parameters', and a parameter's that no group has any more."""
+    a, b, oa, ob = _pair(k2, dev, lr=1e-2)
+    oa.state["note"] = 3
+    oa.state["more"]["x"] = a[0]
+    _steps(oa, ob, a, b, 0)
+    held = oa.state[a[1]]["exp_avg"].data_ptr()
+    oa.state["note"] = 4
+    _steps(oa, ob, a, b, 2)
+    _equal(a, b, oa, ob, 4)
+    assert oa.state["note"] == 4 and oa.state["more"]["x"] is a[0] and oa.state[a[1]]["exp_avg"].data_ptr() == held
