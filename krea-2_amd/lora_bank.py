@@ -166,6 +166,11 @@ def _entered() -> _Body | None:
     return body
 
 
+def _ids_in(body: _Body | None, bank) -> torch.Tensor | None:
+    found = None if body is None else body.of(bank)
+    return bank._own if found is None or not found.open else found.ids
+
+
 def _backward_callers() -> list:
     """The threads that are inside a backward pass: this one if it called one, and those that wait for theirs."""
     me, name, out = threading.get_ident(), "_engine_run_backward", []
@@ -187,22 +192,20 @@ def _requests(bank) -> torch.Tensor | None:
         last = _last.get(me)
         if body is not None or last is None or last.of(bank) is not None:
             _last[me] = body
-        found = None if body is None else body.of(bank)
-        return bank._own if found is None else found.ids
-    found = None if body is None else body.of(bank)
-    if found is None:       # on a thread of autograd's own, or with no body left
+        return _ids_in(body, bank)
+    if body is None or body.of(bank) is None:       # on a thread of autograd's own, or with no body left
         callers = [_last[t] for t in _backward_callers() if t in _last]
         callers = callers or [b for b in list(_last.values()) if b is None or b.open]
         bodies = [None if b is None else b.of(bank) for b in callers]
-        found = bodies[0] if bodies else None
         if any(b is not None and not b.open and b.named for b in bodies):
             raise RuntimeError("a bank's forward is recomputed outside the lora_requests body that it ran in, where it would run "
                                "without its adapters: keep the backward pass inside the body")
-        ids = [bank._own if b is None else b.ids for b in bodies]
+        ids = [_ids_in(b, bank) for b in callers]
         if any(i is not ids[0] for i in ids):
             raise RuntimeError("backward passes of several threads recompute a bank's forward at once: nothing tells whose "
                                "requests it wants; open lora_requests in the recomputed function")
-    return bank._own if found is None or not found.open else found.ids
+        return ids[0] if ids else bank._own
+    return _ids_in(body, bank)
 
 
 class LoRABank(nn.Module):
@@ -250,9 +253,7 @@ class LoRABank(nn.Module):
     @property
     def adapters(self) -> torch.Tensor | None:
         """The requests of the caller's body of :func:`lora_requests`, else those set here."""
-        body = _entered()
-        found = None if body is None else body.of(self)
-        return self._own if found is None else found.ids
+        return _ids_in(_entered(), self)
 
     @adapters.setter
     def adapters(self, ids: torch.Tensor | None) -> None:
@@ -275,7 +276,7 @@ class LoRABank(nn.Module):
 
     @torch.no_grad()
     def _remove(self, index: int) -> None:
-        """No adapter in place ``index``: rank 0, whose rows keep the base's output and which training leaves as it is."""
+        """No adapter in place ``index``: rank 0, whose rows keep the base's output."""
         self._place(index)
         self.lora_A[index].zero_()
         self.lora_B[index].zero_()
